@@ -411,6 +411,43 @@ int s2cnn_s2_analysis_real_basis_grad(const float *g, const float *table, float 
 int s2cnn_so3_integrate(const float *x, const float *w, float *out, int b, long n, void *stream);
 int s2cnn_so3_integrate_grad(const float *g, const float *w, float *gx, int b, long n, void *stream);
 
+/* ---- attention --------------------------------------------------------------------------
+ * out[b,h,i] = sum_j P_ij v[b,h',j],  P = softmax over j of  x_ij = scale q[b,h,i].k[b,h',j] + table[h,n] + key_bias[b,j],
+ * h' = h / (heads / kv_heads), n = buckets[b,i,j].  A key takes no part where j >= lengths[b] or key_bias[b,j] = -inf (its k and
+ * v are not used at all then), a pair where n is outside 0 .. n_buckets - 1.  A row without any key: out = 0, no gradients.
+ * Types of q, k, v, table, out and all gradients: dtype; sums, the softmax and its gradient are float32, float32 products
+ * have float32 errors.  A tensor's vectors are contiguous, strides are those of (batch, head, vector) in entries.
+ * Optional pointers may be NULL: table and buckets (together; n_buckets 0), key_bias, lengths, stats and out_f32 (if no
+ * backward pass follows).  fwd reads q .. lengths and writes out, stats and out_f32; bwd reads those and gout and writes gq, and where not NULL gtable,
+ * gk and gv (both or none).  Results do not depend on the order of execution.
+ */
+#define S2CNN_F32 0
+#define S2CNN_BF16 1
+#define S2CNN_F16 2
+
+typedef struct s2cnn_attention_t {
+  const void *q, *k, *v;       /* [batch, heads, n_q, d], [batch, kv_heads, n_k, d] twice   */
+  const void *table;           /* [heads, n_buckets], n_buckets <= 64                      */
+  const signed char *buckets;  /* [batch, n_q, n_k], rows contiguous                       */
+  const float *key_bias;       /* [batch, n_k], rows contiguous                            */
+  const int *lengths;          /* [batch]                                                  */
+  void *out;                   /* [batch, heads, n_q, d]                                   */
+  float *stats;                /* [batch, heads, n_q, 2], for bwd; 8-byte aligned          */
+  float *out_f32;              /* [batch, heads, n_q, d] dense, for bwd: out before its rounding (16-bit types; else unused) */
+  const void *gout;
+  void *gq, *gk, *gv, *gtable;
+  long q_stride[3], k_stride[3], v_stride[3], out_stride[3], gout_stride[3], gq_stride[3], gk_stride[3], gv_stride[3];
+  long bucket_stride[2];       /* of batch (0: shared) and query, in bytes                 */
+  long key_bias_stride;        /* of batch (0: shared), in entries                         */
+  int batch, heads, kv_heads, n_q, n_k, d;      /* n_q >= 1; n_k >= 0 (bwd: >= 1); 1 <= d <= 128 */
+  int n_buckets, dtype;
+  float scale;
+} s2cnn_attention_t;
+
+size_t s2cnn_attention_workspace(const s2cnn_attention_t *a, int backward);     /* 0 also for sizes that are refused */
+int s2cnn_attention_fwd(const s2cnn_attention_t *a, void *workspace, size_t workspace_bytes, void *stream);
+int s2cnn_attention_bwd(const s2cnn_attention_t *a, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,6 +8,7 @@ from .so3_ft import so3_rft
 from .s2_ft import s2_rft
 from .so3_real import so3_mm_real, so3_rft_real, so3_spectrum_to_complex, so3_spectrum_to_real
 from .s2_real import s2_mm_real, s2_rft_real, s2_spectrum_to_real
+from .attention import attention, s2_angle_buckets, s2_log_weights
 
 s2_near_identity_grid, s2_equatorial_grid, s2_soft_grid = (
     _s2_grid.s2_near_identity_grid, _s2_grid.s2_equatorial_grid, _s2_grid.s2_soft_grid)

@@ -22,6 +22,18 @@ _FT3_SIG = [_c_float_p, _c_float_p, _c_float_p, _c_float_p, _vp, _size_t, _int, 
 _FT3R_SIG = [_c_float_p, _c_float_p, _c_float_p, _c_float_p, _vp, _size_t, _int, _int, _long, _vp]
 _WS_SIG = [_int, _int, _long, _int]
 
+
+
+class Attention(ctypes.Structure):
+    """s2cnn_attention_t"""
+    _fields_ = ([(n, _vp) for n in ("q", "k", "v", "table", "buckets", "key_bias", "lengths", "out", "stats", "out_f32", "gout", "gq", "gk", "gv", "gtable")]
+                + [(n + "_stride", _long * 3) for n in ("q", "k", "v", "out", "gout", "gq", "gk", "gv")]
+                + [("bucket_stride", _long * 2), ("key_bias_stride", _long)]
+                + [(n, _int) for n in ("batch", "heads", "kv_heads", "n_q", "n_k", "d", "n_buckets", "dtype")] + [("scale", _float)])
+
+
+_ATTENTION_P = ctypes.POINTER(Attention)
+
 SIGNATURES = {
     "s2cnn_abi_version": (_int, []),
     "s2cnn_strerror": (ctypes.c_char_p, [_int]),
@@ -84,6 +96,9 @@ SIGNATURES = {
     "s2cnn_s2_synthesis_workspace": (_size_t, _WS_SIG),
     "s2cnn_s2_synthesis": (_int, _FT_SIG),
     "s2cnn_so3_integrate": (_int, [_c_float_p, _c_float_p, _c_float_p, _int, _long, _vp]),
+    "s2cnn_attention_workspace": (_size_t, [_ATTENTION_P, _int]),
+    "s2cnn_attention_fwd": (_int, [_ATTENTION_P, _vp, _size_t, _vp]),
+    "s2cnn_attention_bwd": (_int, [_ATTENTION_P, _vp, _size_t, _vp]),
     "s2cnn_so3_integrate_grad": (_int, [_c_float_p, _c_float_p, _c_float_p, _int, _long, _vp]),
 }
 
@@ -168,9 +183,41 @@ def require_gpu_f32(*tensors):
             raise RuntimeError(
                 "s2cnn_amd runs float32 tensors on the GPU only (got %s on %s); there is no CPU path"
                 % (t.dtype, t.device))
-        if t.device.index != torch._C._cuda_getDevice():
-            raise RuntimeError("operand on %s but the current device is cuda:%d: call inside torch.cuda.device(%d)"
-                               % (t.device, torch.cuda.current_device(), t.device.index))
+        _require_current_device(t)
+
+
+def _require_current_device(t):
+    if t.device.index != torch._C._cuda_getDevice():
+        raise RuntimeError("operand on %s but the current device is cuda:%d: call inside torch.cuda.device(%d)"
+                           % (t.device, torch.cuda.current_device(), t.device.index))
+
+
+FLOATS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}     # S2CNN_F32, S2CNN_BF16, S2CNN_F16
+
+
+def require_gpu_float(*tensors):
+    """Operands of the operators that take three types: float32, bfloat16 or float16, all the same, on the current GPU.
+    None is passed over.  Returns the type's number in the library."""
+    dtype = tensors[0].dtype
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda or dtype not in FLOATS:
+            raise RuntimeError("float32, bfloat16 or float16 tensors on the GPU only (got %s on %s); there is no CPU path" % (t.dtype, t.device))
+        if t.dtype != dtype:
+            raise RuntimeError("operands of one type only (got %s and %s)" % (dtype, t.dtype))
+        _require_current_device(t)
+    return FLOATS[dtype]
+
+
+def require_gpu_of(dtype, *tensors):
+    """Operands of a fixed type on the current GPU; None is passed over."""
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda or t.dtype != dtype:
+            raise RuntimeError("expected a %s tensor on the GPU (got %s on %s); there is no CPU path" % (dtype, t.dtype, t.device))
+        _require_current_device(t)
 
 
 def stream_ptr():

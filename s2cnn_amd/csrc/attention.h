@@ -1,0 +1,381 @@
+// What the attention kernels share: operand fragments of the matrix cores, the tiles of rows in LDS, the loads.
+//
+// All three kernels have one form.  A wave keeps 32 COLUMNS for good (queries, or keys in the kernel of the key and value
+// gradients), their vectors as B operands in registers, and runs over tiles of 32 ROWS of the other side, which the workgroup
+// stages in LDS.  A product of rows and columns (v_mfma_f32_32x32x16: 32 rows x 32 columns) leaves lane (h, c), h = lane / 32,
+// c = lane % 32, with column c and the rows 8 g + 4 h + i in register 4 g + i: the softmax of a column and all that is known
+// per column stays in one lane and the one 32 further on.  The second product contracts over the rows: register 8 t + j of
+// a lane is taken as slot j of its B operand of step t, which makes slot j the row 16 t + 8 (j / 4) + 4 h + j % 4, and the A
+// operand (the staged rows, transposed) is laid out in that order.  So the probabilities never leave their registers.
+//
+// float32 is computed on the bf16 matrix cores, each value the sum of three bf16 parts, six of the nine products of parts
+// (split_bf16.h: the error is that of a float32 product; here without its power of two: parts of values below 2^-107 are
+// lost).  bfloat16 and float16 take one product.  Everything between the products is float32.
+#pragma once
+#include "split_bf16.h"
+
+namespace s2cnn {
+namespace attn {
+
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+
+constexpr float LOG2E = 1.44269504088896340736f;
+constexpr int ROWS = 32;             // rows of a staged tile, columns of a wave
+constexpr int MAX_BUCKETS = 64;
+
+struct F32 { typedef float type; static constexpr int PARTS = 3; static constexpr bool HALF = false; };
+struct BF16 { typedef __bf16 type; static constexpr int PARTS = 1; static constexpr bool HALF = false; };
+// HALF: probabilities and their gradients are held times powers of two, as float16 has few exponents (see ScoreScale)
+struct F16 { typedef _Float16 type; static constexpr int PARTS = 1; static constexpr bool HALF = true; };
+
+__device__ __forceinline__ float ninf() { return -__builtin_inff(); }
+__device__ __forceinline__ float pinf() { return __builtin_inff(); }
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// the maximum / sum of a lane and the one 32 away, in both
+__device__ __forceinline__ float half_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// ---- operands -------------------------------------------------------------------------------------------------------
+template <class T> struct Frag { uint4 part[T::PARTS]; };
+
+template <class T> __device__ __forceinline__ v16f mfma(uint4 a, uint4 b, v16f c) {
+  if constexpr (T::HALF) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+}
+
+// c += a b, small products first
+template <class T> __device__ __forceinline__ void mma(const Frag<T>& a, const Frag<T>& b, v16f& c) {
+  if constexpr (T::PARTS == 3) {
+    c = mfma<T>(a.part[2], b.part[0], c);
+    c = mfma<T>(a.part[0], b.part[2], c);
+    c = mfma<T>(a.part[1], b.part[1], c);
+    c = mfma<T>(a.part[1], b.part[0], c);
+    c = mfma<T>(a.part[0], b.part[1], c);
+  }
+  c = mfma<T>(a.part[0], b.part[0], c);
+}
+
+// two values as packed parts
+template <class T> __device__ __forceinline__ void cut(float x, float y, unsigned (&w)[T::PARTS]) {
+  if constexpr (T::PARTS == 3) split_pair<true>(x, y, w[0], w[1], w[2]);
+  else if constexpr (T::HALF) w[0] = __builtin_bit_cast(unsigned, __builtin_convertvector(v2f{x, y}, v2h));
+  else w[0] = pack_bf16(x, y);
+}
+// what a packed pair of 16-bit values holds
+template <class T> __device__ __forceinline__ v2f uncut(unsigned w) {
+  if constexpr (T::HALF) return __builtin_convertvector(__builtin_bit_cast(v2h, w), v2f);
+  else return v2f{__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)};
+}
+// two values as the matrix cores will see them
+template <class T> __device__ __forceinline__ void round_pair(float& x, float& y) {
+  if constexpr (T::PARTS == 1) {
+    unsigned w[1];
+    cut<T>(x, y, w);
+    const v2f r = uncut<T>(w[0]);
+    x = r[0], y = r[1];
+  }
+}
+template <class T> __device__ __forceinline__ Frag<T> cut8(const float* x) {
+  unsigned w[4][T::PARTS];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) cut<T>(x[2 * i], x[2 * i + 1], w[i]);
+  Frag<T> f;
+#pragma unroll
+  for (int p = 0; p < T::PARTS; ++p) f.part[p] = make_uint4(w[0][p], w[1][p], w[2][p], w[3][p]);
+  return f;
+}
+// registers 8 t .. 8 t + 7 of a product of rows and columns as the operand of step t of the product over the rows
+template <class T> __device__ __forceinline__ Frag<T> cut_rows(const v16f& s, int t) {
+  float x[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] = s[8 * t + j];
+  return cut8<T>(x);
+}
+
+// ---- vectors in memory ----------------------------------------------------------------------------------------------
+// The vectors of one (batch, head): vector i starts at base + i stride and has d entries.  wide: aligned for loads of four
+// entries, d a multiple of four.
+template <class T> struct Vectors {
+  const typename T::type* base;
+  long stride;
+  int n, d;
+  bool wide;
+};
+
+struct Quad { uint4 w; };            // four entries as they are in memory: floats, or 16-bit values in x and y
+
+// entries 4 q .. 4 q + 3 of the vector at `p`, zero from d on
+template <class T> __device__ __forceinline__ Quad load_quad(const typename T::type* p, int q, int d, bool wide) {
+  Quad v;
+  if (wide) {
+    const int at = 4 * q < d ? 4 * q : 0;
+    if constexpr (T::PARTS == 3) v.w = *reinterpret_cast<const uint4*>(p + at);
+    else {
+      const uint2 u = *reinterpret_cast<const uint2*>(p + at);
+      v.w = make_uint4(u.x, u.y, 0, 0);
+    }
+    if (4 * q >= d) v.w = make_uint4(0, 0, 0, 0);
+  } else {
+    unsigned e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = 4 * q + i;
+      if constexpr (T::PARTS == 3) e[i] = reinterpret_cast<const unsigned*>(p)[at < d ? at : 0];
+      else e[i] = reinterpret_cast<const unsigned short*>(p)[at < d ? at : 0];
+      if (at >= d) e[i] = 0;
+    }
+    if constexpr (T::PARTS == 3) v.w = make_uint4(e[0], e[1], e[2], e[3]);
+    else v.w = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, 0, 0);
+  }
+  return v;
+}
+template <class T> __device__ __forceinline__ void quad_parts(const Quad& v, unsigned (&lo)[T::PARTS], unsigned (&hi)[T::PARTS]) {
+  if constexpr (T::PARTS == 3) {
+    cut<T>(__uint_as_float(v.w.x), __uint_as_float(v.w.y), lo);
+    cut<T>(__uint_as_float(v.w.z), __uint_as_float(v.w.w), hi);
+  } else {
+    lo[0] = v.w.x;
+    hi[0] = v.w.y;
+  }
+}
+template <class T> __device__ __forceinline__ void quad_values(const Quad& v, float (&x)[4]) {
+  if constexpr (T::PARTS == 3) {
+    x[0] = __uint_as_float(v.w.x), x[1] = __uint_as_float(v.w.y), x[2] = __uint_as_float(v.w.z), x[3] = __uint_as_float(v.w.w);
+  } else {
+    const v2f a = uncut<T>(v.w.x), b = uncut<T>(v.w.y);
+    x[0] = a[0], x[1] = a[1], x[2] = b[0], x[3] = b[1];
+  }
+}
+template <class T> __device__ __forceinline__ void store_quad(typename T::type* p, int at, int d, bool wide, float a, float b, float c, float e) {
+  if (at >= d) return;
+  if (wide) {
+    if constexpr (T::PARTS == 3) *reinterpret_cast<float4*>(p + at) = make_float4(a, b, c, e);
+    else {
+      unsigned u[1], v[1];
+      cut<T>(a, b, u), cut<T>(c, e, v);
+      *reinterpret_cast<uint2*>(p + at) = make_uint2(u[0], v[0]);
+    }
+    return;
+  }
+  const float x[4] = {a, b, c, e};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (at + i < d) p[at + i] = (typename T::type)x[i];
+}
+
+// The B operands of one column: the vector at `p`, in steps of 16 entries, 8 of them in either half of the wave.
+template <class T, int D> __device__ __forceinline__ void load_column(const typename T::type* p, int d, bool wide, bool ok, int half, Frag<T> (&f)[D / 16]) {
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s) {
+    Quad a = load_quad<T>(p, 4 * s + 2 * half, d, wide), b = load_quad<T>(p, 4 * s + 2 * half + 1, d, wide);
+    if (!ok) a.w = b.w = make_uint4(0, 0, 0, 0);
+    unsigned w[4][T::PARTS];
+    quad_parts<T>(a, w[0], w[1]);
+    quad_parts<T>(b, w[2], w[3]);
+#pragma unroll
+    for (int q = 0; q < T::PARTS; ++q) f[s].part[q] = make_uint4(w[0][q], w[1][q], w[2][q], w[3][q]);
+  }
+}
+
+// acc[b][4 g + i] is entry 32 b + 8 g + 4 half + i of the lane's column
+template <class T, int D> __device__ __forceinline__ void store_column(typename T::type* p, int d, bool wide, int half, const v16f (&acc)[D / 32], float factor) {
+#pragma unroll
+  for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      store_quad<T>(p, 32 * b + 8 * g + 4 * half, d, wide, acc[b][4 * g] * factor, acc[b][4 * g + 1] * factor, acc[b][4 * g + 2] * factor,
+                    acc[b][4 * g + 3] * factor);
+}
+// the same into an array of partial sums, D floats a column
+template <int D> __device__ __forceinline__ void store_partial(float* p, int half, const v16f (&acc)[D / 32]) {
+#pragma unroll
+  for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<float4*>(p + 32 * b + 8 * g + 4 * half) = make_float4(acc[b][4 * g], acc[b][4 * g + 1], acc[b][4 * g + 2], acc[b][4 * g + 3]);
+}
+
+// ---- a tile of 32 rows in LDS ---------------------------------------------------------------------------------------
+// Two layouts, both as the A operands are read: 1 KB per part and step, 16 bytes a lane.
+//   by rows: step s of the product over the entries; lane (h, r) reads entries 16 s + 8 h .. + 7 of row r
+//   by entries: block b of 32 entries, step t of the product over the rows; lane (h, m) reads entry 32 b + m of the rows above
+// A thread of the staging holds a block of 4 rows x 4 entries, and writes 8 bytes per row or entry.  The 16-byte slots are
+// permuted (by s and h, or by m / 8) so that these writes go to all banks; readers permute within 128 bytes and lose nothing.
+template <class T, int D> struct Tile {
+  static constexpr int STEPS = D / 16;                             // as many KB per part in either layout
+  static constexpr int BYTES = T::PARTS * STEPS * 1024;
+  static constexpr int BLOCKS = (ROWS / 4) * (D / 4);
+
+  static __device__ __forceinline__ int row_slot(int s, int h, int r) { return (h * 32 + r) ^ ((2 * s + h) & 7); }
+  static __device__ __forceinline__ int entry_slot(int h, int m) { return h * 32 + (m ^ ((m >> 3) & 3)); }
+
+  static __device__ __forceinline__ Frag<T> by_rows(const unsigned char* lds, int s, int lane) {
+    Frag<T> f;
+    const int at = row_slot(s, lane >> 5, lane & 31);
+#pragma unroll
+    for (int p = 0; p < T::PARTS; ++p) f.part[p] = *reinterpret_cast<const uint4*>(lds + ((p * STEPS + s) * 64 + at) * 16);
+    return f;
+  }
+  static __device__ __forceinline__ Frag<T> by_entries(const unsigned char* lds, int b, int t, int lane) {
+    Frag<T> f;
+    const int at = entry_slot(lane >> 5, lane & 31);
+#pragma unroll
+    for (int p = 0; p < T::PARTS; ++p) f.part[p] = *reinterpret_cast<const uint4*>(lds + ((p * STEPS + 2 * b + t) * 64 + at) * 16);
+    return f;
+  }
+
+  // block k of the tile: rows 4 (k / (D / 4)), entries 4 (k % (D / 4))
+  static __device__ __forceinline__ void write(unsigned char* rows, unsigned char* entries, int k, const Quad (&v)[4]) {
+    const int q = k % (D / 4), kg = k / (D / 4);
+    unsigned w[4][2][T::PARTS];                                    // [row][pair of entries][part]
+#pragma unroll
+    for (int i = 0; i < 4; ++i) quad_parts<T>(v[i], w[i][0], w[i][1]);
+    if (rows) {
+      const int s = q >> 2, h = (q >> 1) & 1;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = row_slot(s, h, 4 * kg + i);
+#pragma unroll
+        for (int p = 0; p < T::PARTS; ++p)
+          *reinterpret_cast<uint2*>(rows + ((p * STEPS + s) * 64 + at) * 16 + (q & 1) * 8) = make_uint2(w[i][0][p], w[i][1][p]);
+      }
+    }
+    if (entries) {
+      const int b = q >> 3, t = kg >> 2, half = (kg >> 1) & 1, h = kg & 1;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int at = entry_slot(h, (4 * q + j) & 31);
+        const unsigned sel = (j & 1) ? 0x07060302u : 0x05040100u;  // the entry's 16 bits of two rows
+#pragma unroll
+        for (int p = 0; p < T::PARTS; ++p)
+          *reinterpret_cast<uint2*>(entries + ((p * STEPS + 2 * b + t) * 64 + at) * 16 + half * 8) =
+              make_uint2(__builtin_amdgcn_perm(w[1][j >> 1][p], w[0][j >> 1][p], sel), __builtin_amdgcn_perm(w[3][j >> 1][p], w[2][j >> 1][p], sel));
+      }
+    }
+  }
+};
+
+// Two tensors staged by the same tiles of rows: THREADS threads fetch the blocks of a tile into registers, and write them later.
+template <class T, int D, int THREADS> struct Stage {
+  typedef Tile<T, D> Tl;
+  static constexpr int PER = (2 * Tl::BLOCKS + THREADS - 1) / THREADS;
+  Quad v[PER][4];
+
+  __device__ __forceinline__ void fetch(const Vectors<T>& a, const Vectors<T>& b, int row0, int tid) {
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      const int k = u * THREADS + tid, kk = k % Tl::BLOCKS;
+      if (2 * Tl::BLOCKS % THREADS != 0 && k >= 2 * Tl::BLOCKS) break;
+      const Vectors<T>& x = k < Tl::BLOCKS ? a : b;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = row0 + 4 * (kk / (D / 4)) + i;
+        v[u][i] = load_quad<T>(x.base + (long)min(row, x.n - 1) * x.stride, kk % (D / 4), x.d, x.wide);
+      }
+    }
+  }
+  // keep(row of the tile): false for rows that count as zero, whatever their memory holds
+  template <class Keep>
+  __device__ __forceinline__ void write(unsigned char* a_rows, unsigned char* a_entries, unsigned char* b_rows, unsigned char* b_entries, int tid, Keep keep) {
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      const int k = u * THREADS + tid, kk = k % Tl::BLOCKS;
+      if (2 * Tl::BLOCKS % THREADS != 0 && k >= 2 * Tl::BLOCKS) break;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (!keep(4 * (kk / (D / 4)) + i)) v[u][i].w = make_uint4(0, 0, 0, 0);
+      if (k < Tl::BLOCKS) Tl::write(a_rows, a_entries, kk, v[u]);
+      else Tl::write(b_rows, b_entries, kk, v[u]);
+    }
+  }
+};
+
+// ---- scores -----------------------------------------------------------------------------------------------------------
+// Scores are kept in base 2: x = log2(e) (scale q.k + table + key bias), the factor in the scale, the table and the key biases.
+// The reference that a query's probabilities are taken to, 2^(x - reference), is an integer, its largest score rounded up: a
+// probability rounded to 16 bits is then the same whatever the reference was when it was formed, up to the power of two, and
+// the sums, the output and the backward pass all use the same, rounded ones.  They are so the exact softmax of weights that
+// are off by a rounding each, rows of its gradient sum to zero as they should, and a factor between references is exact.
+// A key bias of the type's lowest value stays finite so: keys that all have it share a row evenly, as they do without the factor.
+__device__ __forceinline__ float key_bias_base2(const float* key_bias, int key) { return fmaxf(key_bias[key], -2.3e38f) * LOG2E; }
+// value of a key in LDS: -inf for keys that take no part
+__device__ __forceinline__ float key_value(const float* key_bias, int key, int end) {
+  if (key >= end) return ninf();
+  if (!key_bias) return 0.f;
+  return key_bias[key] == ninf() ? ninf() : key_bias_base2(key_bias, key);
+}
+
+// the table's rows of heads head0 .. head0 + heads - 1 in LDS, n_buckets + 1 entries a head, the last one for excluded pairs
+template <class T> __device__ __forceinline__ void stage_table(float* lds, const void* table, int n_buckets, int head0, int heads, int tid, int threads) {
+  const typename T::type* t = static_cast<const typename T::type*>(table);
+  for (int k = tid; k < heads * (n_buckets + 1); k += threads) {
+    const int h = k / (n_buckets + 1), n = k % (n_buckets + 1);
+    lds[k] = n == n_buckets ? ninf() : (float)t[(long)(head0 + h) * n_buckets + n] * LOG2E;
+  }
+}
+
+// buckets of the lane's column and keys key0 + 8 g + 4 half + i, a byte each; 255 past the end
+__device__ __forceinline__ void load_buckets(const signed char* row, int key0, int end, int half, unsigned (&w)[4]) {
+  if (key0 + ROWS <= end) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) __builtin_memcpy(&w[g], row + key0 + 8 * g + 4 * half, 4);
+  } else {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      w[g] = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = key0 + 8 * g + 4 * half + i;
+        w[g] |= (key < end ? (unsigned)(unsigned char)row[key] : 255u) << (8 * i);
+      }
+    }
+  }
+}
+__device__ __forceinline__ int bucket_of(unsigned w, int i, int n_buckets) { return min((int)((w >> (8 * i)) & 255u), n_buckets); }
+
+// ---- arguments ------------------------------------------------------------------------------------------------------
+// The header's struct and what the entry has made of it.
+enum Wide { WIDE_Q = 1, WIDE_K = 2, WIDE_V = 4, WIDE_OUT = 8, WIDE_GOUT = 16, WIDE_GQ = 32, WIDE_GK = 64, WIDE_GV = 128 };
+struct Args {
+  s2cnn_attention_t a;
+  int wide;                // tensors whose vectors can be read and written four entries at a time
+  int splits;              // parts of the long axis (keys; queries in the kernel of dk and dv)
+  int tiles;               // workgroups along the columns
+  int workgroups;
+  float* partial;          // results of the parts
+  float* gtable_partial;   // of every workgroup
+  float* delta;            // [batch, heads, n_q] dout . out; float16: then the same of max |dout|
+};
+
+// Consecutive workgroups go to the eight XCDs in turn: the ones that read the same rows are given numbers of one XCD.
+__device__ __forceinline__ int work_of_block(int workgroups) {
+  const int per = (workgroups + 7) / 8;
+  return (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
+}
+inline unsigned blocks_for(int workgroups) { return (unsigned)((workgroups + 7) / 8 * 8); }
+
+
+// ---- launches -------------------------------------------------------------------------------------------------------
+// How a kernel's work is laid out: waves per workgroup, workgroups along the columns, parts of the long axis.
+struct Plan { int waves, tiles, splits; long workgroups; };
+struct Plans { int D; Plan fwd, grad_q, grad_kv; };
+
+template <class K> void launch(K kernel, const Args& p, int waves, size_t lds, hipStream_t stream) {
+  (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  hipLaunchKernelGGL(kernel, dim3(blocks_for(p.workgroups)), dim3(64 * waves), lds, stream, p);
+}
+
+// one translation unit per type
+template <class T> void forward(const Args& p, const Plans& plans, hipStream_t stream);
+template <class T> void backward(Args p, const Plans& plans, float* partial_q, float* partial_kv, hipStream_t stream);
+
+}  // namespace attn
+}  // namespace s2cnn

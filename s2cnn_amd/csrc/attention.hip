@@ -1,0 +1,142 @@
+// Entry points of the attention kernels: checks, the layout of the work, workspaces.
+#include "attention.h"
+
+namespace s2cnn {
+namespace attn {
+extern template void forward<F32>(const Args&, const Plans&, hipStream_t);
+extern template void forward<BF16>(const Args&, const Plans&, hipStream_t);
+extern template void forward<F16>(const Args&, const Plans&, hipStream_t);
+extern template void backward<F32>(Args, const Plans&, float*, float*, hipStream_t);
+extern template void backward<BF16>(Args, const Plans&, float*, float*, hipStream_t);
+extern template void backward<F16>(Args, const Plans&, float*, float*, hipStream_t);
+
+namespace {
+
+constexpr int CUS = 256;
+
+// Columns of one group of heads, groups, and tiles of the long axis.  A workgroup of one wave where one wave holds all columns.
+// The long axis is cut while compute units would have no workgroup, into parts of at least four tiles.
+Plan plan(long columns, long groups, long long_tiles) {
+  Plan p;
+  p.waves = columns <= 32 ? 1 : 4;
+  p.tiles = columns < 1 ? 1 : (int)((columns + 32 * p.waves - 1) / (32 * p.waves));
+  const long base = p.tiles * groups, want = p.waves == 1 ? 4 * CUS : 2 * CUS;
+  long splits = base >= want / 2 ? 1 : (want + base - 1) / base;
+  if (splits > long_tiles / 4) splits = long_tiles / 4;
+  p.splits = splits < 1 ? 1 : (int)splits;
+  p.workgroups = base * p.splits;
+  return p;
+}
+
+long tiles_of(long n) { return (n + ROWS - 1) / ROWS; }
+
+Plans plans_of(const s2cnn_attention_t& a) {
+  Plans p;
+  p.D = a.d <= 32 ? 32 : a.d <= 64 ? 64 : 128;
+  const long group = a.heads / a.kv_heads;
+  p.fwd = plan(group * a.n_q, (long)a.batch * a.kv_heads, tiles_of(a.n_k));
+  p.grad_q = plan(a.n_q, (long)a.batch * a.heads, tiles_of(a.n_k));
+  p.grad_kv = plan(a.n_k, (long)a.batch * a.kv_heads, group * tiles_of(a.n_q));
+  return p;
+}
+
+bool sizes_ok(const s2cnn_attention_t* a) {
+  if (!a) return false;
+  if (a->dtype != S2CNN_F32 && a->dtype != S2CNN_BF16 && a->dtype != S2CNN_F16) return false;
+  if (a->batch < 1 || a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads || a->n_q < 1 || a->n_k < 0 || a->d < 1 || a->d > 128) return false;
+  const bool bias = a->buckets || a->table || a->n_buckets;
+  if (bias && (!a->buckets || !a->table || a->n_buckets < 1 || a->n_buckets > MAX_BUCKETS || a->heads / a->kv_heads > 128)) return false;
+  const long limit = 1L << 30;
+  if ((long)a->heads / a->kv_heads * a->n_q > limit || a->n_k > limit || (long)a->batch * a->heads > limit) return false;
+  const Plans p = plans_of(*a);
+  return p.fwd.workgroups < limit && p.grad_q.workgroups < limit && p.grad_kv.workgroups < limit && (long)a->batch * a->heads * a->n_q < 4 * limit &&
+         (long)a->batch * a->kv_heads * a->n_k < 4 * limit;
+}
+
+size_t up(size_t n) { return (n + 255) / 256 * 256; }
+
+size_t forward_bytes(const s2cnn_attention_t& a, const Plans& p) {
+  return p.fwd.splits > 1 ? up((size_t)p.fwd.splits * a.batch * a.heads * a.n_q * (p.D + 2) * sizeof(float)) : 0;
+}
+struct Backward { size_t delta, table, q, kv, bytes; };   // where the parts of the workspace begin
+Backward backward_layout(const s2cnn_attention_t& a, const Plans& p) {
+  const size_t queries = (size_t)a.batch * a.heads * a.n_q, keys = (size_t)a.batch * a.kv_heads * a.n_k;
+  Backward w;
+  w.delta = 0;
+  w.table = up(queries * (a.dtype == S2CNN_F16 ? 2 : 1) * sizeof(float));
+  w.q = w.table + up((size_t)p.grad_q.workgroups * a.n_buckets * sizeof(float));
+  w.kv = w.q + (p.grad_q.splits > 1 ? up((size_t)p.grad_q.splits * queries * p.D * sizeof(float)) : 0);
+  w.bytes = w.kv + (p.grad_kv.splits > 1 ? up((size_t)p.grad_kv.splits * 2 * keys * p.D * sizeof(float)) : 0);
+  return w;
+}
+
+int wide(const s2cnn_attention_t& a) {
+  const int size = a.dtype == S2CNN_F32 ? 4 : 2;
+  const auto one = [&](const void* p, const long* s, int bit) {
+    return a.d % 4 == 0 && s[0] % 4 == 0 && s[1] % 4 == 0 && s[2] % 4 == 0 && reinterpret_cast<uintptr_t>(p) % (4 * size) == 0 ? bit : 0;
+  };
+  return one(a.q, a.q_stride, WIDE_Q) | one(a.k, a.k_stride, WIDE_K) | one(a.v, a.v_stride, WIDE_V) | one(a.out, a.out_stride, WIDE_OUT) |
+         one(a.gout, a.gout_stride, WIDE_GOUT) | one(a.gq, a.gq_stride, WIDE_GQ) | one(a.gk, a.gk_stride, WIDE_GK) | one(a.gv, a.gv_stride, WIDE_GV);
+}
+
+bool aligned_to_type(const s2cnn_attention_t& a) {
+  const uintptr_t mask = a.dtype == S2CNN_F32 ? 3 : 1;
+  for (const void* p : {a.q, a.k, a.v, a.table, (const void*)a.out, a.gout, (const void*)a.gq, (const void*)a.gk, (const void*)a.gv, (const void*)a.gtable})
+    if (reinterpret_cast<uintptr_t>(p) & mask) return false;
+  return !((reinterpret_cast<uintptr_t>(a.key_bias) | reinterpret_cast<uintptr_t>(a.out_f32) | reinterpret_cast<uintptr_t>(a.lengths)) & 3) && aligned8(a.stats);
+}
+
+}  // namespace
+}  // namespace attn
+}  // namespace s2cnn
+
+using namespace s2cnn;
+using namespace s2cnn::attn;
+
+extern "C" size_t s2cnn_attention_workspace(const s2cnn_attention_t* a, int backward) {
+  if (!sizes_ok(a)) return 0;
+  const Plans p = plans_of(*a);
+  return backward ? backward_layout(*a, p).bytes : forward_bytes(*a, p);
+}
+
+extern "C" int s2cnn_attention_fwd(const s2cnn_attention_t* a, void* workspace, size_t workspace_bytes, void* stream) {
+  clear_stale_error();
+  if (!sizes_ok(a) || !a->q || !a->out || (a->n_k > 0 && (!a->k || !a->v))) return S2CNN_EINVAL;
+  if (!aligned_to_type(*a)) return S2CNN_EALIGN;
+  const Plans plans = plans_of(*a);
+  const size_t need = forward_bytes(*a, plans);
+  if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return S2CNN_EWORKSPACE;
+  Args p{};
+  p.a = *a;
+  p.wide = wide(*a);
+  p.splits = plans.fwd.splits, p.tiles = plans.fwd.tiles, p.workgroups = (int)plans.fwd.workgroups;
+  p.partial = static_cast<float*>(workspace);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (a->dtype == S2CNN_F32) forward<F32>(p, plans, st);
+  else if (a->dtype == S2CNN_BF16) forward<BF16>(p, plans, st);
+  else forward<F16>(p, plans, st);
+  return launch_status();
+}
+
+extern "C" int s2cnn_attention_bwd(const s2cnn_attention_t* a, void* workspace, size_t workspace_bytes, void* stream) {
+  clear_stale_error();
+  if (!sizes_ok(a) || a->n_k < 1 || !a->q || !a->k || !a->v || !a->out || !a->stats || !a->gout || !a->gq || !a->gk != !a->gv) return S2CNN_EINVAL;
+  if ((a->gtable && !a->table) || (a->dtype != S2CNN_F32 && !a->out_f32)) return S2CNN_EINVAL;
+  if (!aligned_to_type(*a)) return S2CNN_EALIGN;
+  const Plans plans = plans_of(*a);
+  const Backward w = backward_layout(*a, plans);
+  if (!workspace || workspace_bytes < w.bytes || !aligned16(workspace)) return S2CNN_EWORKSPACE;
+  char* const at = static_cast<char*>(workspace);
+  Args p{};
+  p.a = *a;
+  p.wide = wide(*a);
+  p.delta = reinterpret_cast<float*>(at + w.delta);
+  p.gtable_partial = reinterpret_cast<float*>(at + w.table);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  float* const q = reinterpret_cast<float*>(at + w.q);
+  float* const kv = reinterpret_cast<float*>(at + w.kv);
+  if (a->dtype == S2CNN_F32) backward<F32>(p, plans, q, kv, st);
+  else if (a->dtype == S2CNN_BF16) backward<BF16>(p, plans, q, kv, st);
+  else backward<F16>(p, plans, q, kv, st);
+  return launch_status();
+}

@@ -1,0 +1,203 @@
+// Attention, forward: out = softmax(scale q k^T + table[bucket] + key bias) v in one pass over the keys.
+//
+// A wave keeps 32 queries, a workgroup of W waves stages tiles of 32 keys and values for all of them.  Per tile: scores (rows:
+// keys), running maximum and sum per query, probabilities as they are in registers into the product with the transposed
+// values.  The columns run over all queries of the heads that share a key head, so that a single query of 8 heads reads its
+// keys once; few columns and many keys: the keys are split over workgroups, and a second kernel joins their results.
+#pragma once
+#include "attention.h"
+
+namespace s2cnn {
+namespace attn {
+
+template <class T, int D, int W> __global__ __launch_bounds__(64 * W, 2) void forward_kernel(Args p) {
+  typedef Tile<T, D> Tl;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  unsigned char* const lds_k = smem;
+  unsigned char* const lds_v = smem + Tl::BYTES;
+  float* const lds_kb = reinterpret_cast<float*>(smem + 2 * Tl::BYTES);       // [2][ROWS]
+  float* const lds_table = lds_kb + 2 * ROWS;
+  const s2cnn_attention_t& a = p.a;
+
+  const int work = work_of_block(p.workgroups);
+  if (work >= p.workgroups) return;
+  const int tile = work % p.tiles, split = work / p.tiles % p.splits, bh = work / p.tiles / p.splits;
+  const int b = bh / a.kv_heads, hk = bh % a.kv_heads, group = a.heads / a.kv_heads;
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
+  const int columns = group * a.n_q, column0 = tile * 32 * W;
+  const int column = column0 + (tid >> 6) * 32 + (lane & 31);
+  const bool ok = column < columns;
+  const int c = ok ? column : columns - 1;
+  const int head = hk * group + c / a.n_q, query = c % a.n_q;
+  const int head0 = hk * group + column0 / a.n_q, heads = hk * group + min(columns - 1, column0 + 32 * W - 1) / a.n_q - head0 + 1;
+
+  int end = a.n_k;
+  if (a.lengths) end = max(0, min(end, a.lengths[b]));
+  const int chunk = ((a.n_k + ROWS - 1) / ROWS + p.splits - 1) / p.splits * ROWS;
+  const int key0 = split * chunk;
+  end = min(end, key0 + chunk);
+
+  typedef typename T::type E;
+  const Vectors<T> k{static_cast<const E*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[1], a.k_stride[2], a.n_k, a.d, (p.wide & WIDE_K) != 0};
+  const Vectors<T> v{static_cast<const E*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[1], a.v_stride[2], a.n_k, a.d, (p.wide & WIDE_V) != 0};
+  const float* const key_bias = a.key_bias ? a.key_bias + b * a.key_bias_stride : nullptr;
+  const signed char* const buckets = a.buckets ? a.buckets + b * a.bucket_stride[0] + query * a.bucket_stride[1] : nullptr;
+  const float* const table = lds_table + (head - head0) * (a.n_buckets + 1);
+
+  Stage<T, D, 64 * W> stage;
+  unsigned words[4] = {0, 0, 0, 0};
+  if (key0 < end) {
+    stage.fetch(k, v, key0, tid);
+    if (buckets) load_buckets(buckets, key0, end, half, words);
+  }
+  if (tid < ROWS) lds_kb[tid] = key_value(key_bias, key0 + tid, end);
+  if (buckets) stage_table<T>(lds_table, a.table, a.n_buckets, head0, heads, tid, 64 * W);
+  Frag<T> qf[D / 16];
+  load_column<T, D>(static_cast<const E*>(a.q) + b * a.q_stride[0] + head * a.q_stride[1] + query * a.q_stride[2], a.d, (p.wide & WIDE_Q) != 0, ok, half, qf);
+
+  constexpr float SHIFT = T::HALF ? 10.f : 0.f;       // probabilities times 2^10 in float16: its smallest normal number is 2^-14
+  const float scale = a.scale * LOG2E;
+  float m = ninf(), l = 0.f;
+  v16f o[D / 32] = {};
+  int slot = 0;
+  for (int key = key0; key < end; key += ROWS, slot ^= 1) {
+    const float* const kb = lds_kb + slot * ROWS;
+    __syncthreads();
+    stage.write(lds_k, nullptr, nullptr, lds_v, tid, [&](int r) { return kb[r] != ninf(); });
+    __syncthreads();
+    unsigned now[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) now[g] = words[g];
+    float kb_next = 0.f;
+    const bool more = key + ROWS < end;
+    if (more) {
+      stage.fetch(k, v, key + ROWS, tid);
+      if (buckets) load_buckets(buckets, key + ROWS, end, half, words);
+      if (tid < ROWS) kb_next = key_value(key_bias, key + ROWS + tid, end);
+    }
+
+    v16f s = {};
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) mma<T>(Tl::by_rows(lds_k, i, lane), qf[i], s);
+    float top = ninf();
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float4 kb4 = *reinterpret_cast<const float4*>(kb + 8 * g + 4 * half);
+      const float kbs[4] = {kb4.x, kb4.y, kb4.z, kb4.w};
+      if (buckets) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int n = bucket_of(now[g], i, a.n_buckets);
+          const float x = fmaf(s[4 * g + i], scale, table[n]) + kbs[i];
+          s[4 * g + i] = n == a.n_buckets ? ninf() : x;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[4 * g + i] = fmaf(s[4 * g + i], scale, kbs[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, s[4 * g + i]);
+    }
+    top = ceilf(fmaxf(half_max(top), m));
+    const float ref = (top == ninf() ? 0.f : top) - SHIFT;
+    if (__any(top > m)) {
+      const float fade = exp2_(m - SHIFT - ref);      // a power of two
+      l *= fade;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) o[i] *= fade;
+    }
+    m = top;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[i] = exp2_(s[i] - ref);
+      if constexpr (T::PARTS == 3) l += s[i];
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const Frag<T> pf = cut_rows<T>(s, t);
+      if constexpr (T::PARTS == 1) {
+        const unsigned w[4] = {pf.part[0].x, pf.part[0].y, pf.part[0].z, pf.part[0].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const v2f r = uncut<T>(w[j]);
+          l += r[0], l += r[1];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) mma<T>(Tl::by_entries(lds_v, i, t, lane), pf, o[i]);
+    }
+    if (more && tid < ROWS) lds_kb[(slot ^ 1) * ROWS + tid] = kb_next;
+  }
+
+  l = half_sum(l);
+  if (!ok) return;
+  const long row = ((long)b * a.heads + head) * a.n_q + query;
+  if (p.splits > 1) {
+    const long rows = (long)a.batch * a.heads * a.n_q;
+    float* const part = p.partial;
+    store_partial<D>(part + (split * rows + row) * D, half, o);
+    if (half == 0) reinterpret_cast<float2*>(part + p.splits * rows * D)[split * rows + row] = make_float2(m, l);
+    return;
+  }
+  // a row without keys: zeros, and statistics by which every probability is zero
+  const bool any = l != 0.f;
+  const float inv = any ? 1.f / l : 0.f;
+  const long at = b * a.out_stride[0] + head * a.out_stride[1] + query * a.out_stride[2];
+  store_column<T, D>(static_cast<E*>(a.out) + at, a.d, (p.wide & WIDE_OUT) != 0, half, o, inv);
+  if (T::PARTS == 1 && a.out_f32) store_column<F32, D>(a.out_f32 + row * a.d, a.d, a.d % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out_f32) & 15) == 0, half, o, inv);
+  if (half == 0 && a.stats) reinterpret_cast<float2*>(a.stats)[row] = any ? make_float2(m - SHIFT, inv) : make_float2(pinf(), 0.f);
+}
+
+// One wave joins the parts of one query: the sums of all parts, each times 2^(its maximum - the maximum of all).
+template <class T, int D> __global__ __launch_bounds__(256) void join_kernel(Args p) {
+  const s2cnn_attention_t& a = p.a;
+  const long rows = (long)a.batch * a.heads * a.n_q, row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const int lane = threadIdx.x & 63;
+  const float* const part = p.partial;
+  const float2* const ml = reinterpret_cast<const float2*>(part + p.splits * rows * D);
+  constexpr float SHIFT = T::HALF ? 10.f : 0.f;
+  float m = ninf();
+  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, ml[s * rows + row].x);
+  const float ref = m == ninf() ? 0.f : m;
+  float l = 0.f, o[(D + 63) / 64] = {};
+  for (int s = 0; s < p.splits; ++s) {
+    const float2 x = ml[s * rows + row];
+    const float w = exp2_(x.x - ref);
+    l = fmaf(x.y, w, l);
+#pragma unroll
+    for (int i = 0; i < (D + 63) / 64; ++i)
+      if (lane + 64 * i < D) o[i] = fmaf(part[(s * rows + row) * D + lane + 64 * i], w, o[i]);
+  }
+  const bool any = l != 0.f;
+  const float inv = any ? 1.f / l : 0.f;
+  const int query = (int)(row % a.n_q), head = (int)(row / a.n_q % a.heads), b = (int)(row / a.n_q / a.heads);
+  const long at = b * a.out_stride[0] + head * a.out_stride[1] + query * a.out_stride[2];
+  typedef typename T::type E;
+#pragma unroll
+  for (int i = 0; i < (D + 63) / 64; ++i) {
+    if (lane + 64 * i >= a.d) continue;
+    static_cast<E*>(a.out)[at + lane + 64 * i] = (E)(o[i] * inv);
+    if (T::PARTS == 1 && a.out_f32) a.out_f32[row * a.d + lane + 64 * i] = o[i] * inv;
+  }
+  if (lane == 0 && a.stats) reinterpret_cast<float2*>(a.stats)[row] = any ? make_float2(m - SHIFT, inv) : make_float2(pinf(), 0.f);
+}
+
+template <class T, int D> void forward_d(const Args& p, const Plans& plans, hipStream_t stream) {
+  const s2cnn_attention_t& a = p.a;
+  const Plan& f = plans.fwd;
+  const int heads = min(a.heads / a.kv_heads, (32 * f.waves - 1) / a.n_q + 2);
+  const size_t lds = 2 * Tile<T, D>::BYTES + (2 * ROWS + (a.buckets ? heads * (a.n_buckets + 1) : 0)) * sizeof(float);
+  if (f.waves == 1) launch(forward_kernel<T, D, 1>, p, 1, lds, stream);
+  else launch(forward_kernel<T, D, 4>, p, 4, lds, stream);
+  if (f.splits > 1)
+    hipLaunchKernelGGL((join_kernel<T, D>), dim3((unsigned)(((long)a.batch * a.heads * a.n_q + 3) / 4)), dim3(256), 0, stream, p);
+}
+template <class T> void forward(const Args& p, const Plans& plans, hipStream_t stream) {
+  if (plans.D == 32) forward_d<T, 32>(p, plans, stream);
+  else if (plans.D == 64) forward_d<T, 64>(p, plans, stream);
+  else forward_d<T, 128>(p, plans, stream);
+}
+
+}  // namespace attn
+}  // namespace s2cnn
