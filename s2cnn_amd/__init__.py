@@ -9,6 +9,7 @@ from .s2_ft import s2_rft
 from .so3_real import so3_mm_real, so3_rft_real, so3_spectrum_to_complex, so3_spectrum_to_real
 from .s2_real import s2_mm_real, s2_rft_real, s2_spectrum_to_real
 from .attention import attention, s2_angle_buckets, s2_log_weights
+from .layer_norm import dropout, dropout_add_layer_norm, layer_norm
 
 s2_near_identity_grid, s2_equatorial_grid, s2_soft_grid = (
     _s2_grid.s2_near_identity_grid, _s2_grid.s2_equatorial_grid, _s2_grid.s2_soft_grid)

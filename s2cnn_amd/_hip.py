@@ -99,6 +99,10 @@ SIGNATURES = {
     "s2cnn_attention_workspace": (_size_t, [_ATTENTION_P, _int]),
     "s2cnn_attention_fwd": (_int, [_ATTENTION_P, _vp, _size_t, _vp]),
     "s2cnn_attention_bwd": (_int, [_ATTENTION_P, _vp, _size_t, _vp]),
+    "s2cnn_layer_norm_fwd": (_int, [_vp] * 7 + [_long, _long, _float, ctypes.c_double, ctypes.c_ulonglong, _vp, _int, _vp]),
+    "s2cnn_layer_norm_bwd_workspace": (_size_t, [_long, _long, _int]),
+    "s2cnn_layer_norm_bwd": (_int, [_vp] * 10 + [_size_t, _long, _long, ctypes.c_double, ctypes.c_ulonglong, _vp, _int, _int, _vp]),
+    "s2cnn_dropout": (_int, [_vp, _vp, _long, ctypes.c_double, ctypes.c_ulonglong, _vp, _int, _vp]),
     "s2cnn_so3_integrate_grad": (_int, [_c_float_p, _c_float_p, _c_float_p, _int, _long, _vp]),
 }
 
@@ -218,6 +222,10 @@ def require_gpu_of(dtype, *tensors):
         if not t.is_cuda or t.dtype != dtype:
             raise RuntimeError("expected a %s tensor on the GPU (got %s on %s); there is no CPU path" % (dtype, t.dtype, t.device))
         _require_current_device(t)
+
+
+def ptr_or_none(t):
+    return t.data_ptr() if t is not None else None
 
 
 def stream_ptr():

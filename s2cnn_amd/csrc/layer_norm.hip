@@ -1,0 +1,514 @@
+// Layer normalisation over the last axis, dropout, and the step between two sublayers that joins residual, dropout and
+// normalisation; forward and backward.  All are bound by memory: every tensor is read once and written once, in 16 bytes a
+// lane, and what is formed on the way stays in registers.
+//
+// A row belongs to a group of L lanes, each with up to K chunks of 16 bytes of it: L = 8 up to 32 chunks, so that short rows
+// leave few lanes idle and are summed in three lane exchanges, then 16, 32, 64, and a workgroup of 256; rows of more than
+// 1024 chunks are read again per pass.  Mean and variance are formed one after the other from the registers (the variance from the centred
+// values, not as a difference of large sums).
+//
+//   forward    y = (h - mean) rstd w + b, h = x, or residual + dropout(x)
+//   backward   u = g w, dh = rstd (u - mean(u) - xh mean(u xh)) (+ the gradient of h), dx = dropout(dh); dw = sum g xh, db = sum g
+//
+// The two sums over the rows are kept in registers by the groups, which run over many rows each, joined per workgroup in LDS,
+// and a second kernel adds the workgroups' sums in a fixed order.
+#include "counter_random.h"
+
+namespace s2cnn {
+namespace norm {
+
+typedef _Float16 half_t;
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+
+// 16 bytes of a type
+template <class T> struct Chunk;
+template <> struct Chunk<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void get(const uint4& u, float (&v)[4]) {
+    v[0] = __uint_as_float(u.x), v[1] = __uint_as_float(u.y), v[2] = __uint_as_float(u.z), v[3] = __uint_as_float(u.w);
+  }
+  static __device__ __forceinline__ uint4 put(const float (&v)[4]) {
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+  }
+};
+template <class T, class T2> struct Chunk16 {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void get(const uint4& u, float (&v)[8]) {
+    const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f2 x = __builtin_convertvector(__builtin_bit_cast(T2, w[i]), f2);
+      v[2 * i] = x[0], v[2 * i + 1] = x[1];
+    }
+  }
+  static __device__ __forceinline__ uint4 put(const float (&v)[8]) {
+    unsigned w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __builtin_bit_cast(unsigned, __builtin_convertvector(f2{v[2 * i], v[2 * i + 1]}, T2));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+template <> struct Chunk<__bf16> : Chunk16<__bf16, bf2> {};
+template <> struct Chunk<half_t> : Chunk16<half_t, h2> {};
+
+// The n first entries of a chunk at p (any alignment of the type's: rows of odd length), the others zero.
+template <class T> __device__ __forceinline__ uint4 load_chunk(const T* p, int n) {
+  constexpr int N = Chunk<T>::N;
+  uint4 u = make_uint4(0, 0, 0, 0);
+  if (n >= N) {
+    __builtin_memcpy(&u, p, 16);
+    return u;
+  }
+  unsigned w[4] = {0, 0, 0, 0};
+  for (int i = 0; i < n; ++i) {
+    if constexpr (N == 4) {
+      unsigned e;
+      __builtin_memcpy(&e, p + i, 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = i == j ? e : w[j];
+    } else {
+      unsigned short e;
+      __builtin_memcpy(&e, p + i, 2);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] |= i / 2 == j ? (unsigned)e << (16 * (i & 1)) : 0u;
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <class T> __device__ __forceinline__ void store_chunk(T* p, int n, const float (&v)[Chunk<T>::N]) {
+  if (n >= Chunk<T>::N) {
+    const uint4 u = Chunk<T>::put(v);
+    __builtin_memcpy(p, &u, 16);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < Chunk<T>::N; ++i)
+    if (i < n) p[i] = (T)v[i];
+}
+
+// ---- sums over a group of L lanes, in all of them -------------------------------------------------------------------
+template <int CTRL> __device__ __forceinline__ float add_dpp(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+template <int L> __device__ __forceinline__ float sum_lanes(float v) {
+  v = add_dpp<0xB1>(v);                       // the neighbour
+  v = add_dpp<0x4E>(v);                       // two further
+  if (L >= 8) v = add_dpp<0x141>(v);          // 8 lanes mirrored: the other four
+  if (L >= 16) v = add_dpp<0x140>(v);         // 16 lanes mirrored: the other eight
+  if (L >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  if (L >= 64) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  return v;
+}
+// `slot`: LDS of four floats that no other sum before the next barrier uses
+template <int L> __device__ __forceinline__ float sum_group(float v, float* slot) {
+  if constexpr (L <= 64) return sum_lanes<L>(v);
+  v = sum_lanes<64>(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return (slot[0] + slot[1]) + (slot[2] + slot[3]);
+}
+
+struct Forward {
+  const void *x, *residual, *weight, *bias;
+  void *h, *y;
+  float* stats;                  // [rows, 2] mean, rstd; may be NULL
+  long rows;
+  int features;
+  float eps;
+  Dropout drop;
+};
+struct Backward {
+  const void *h, *g, *g_h, *weight;
+  const float* stats;
+  void *gx, *gresidual;
+  float* partial;                // [workgroups, 2, features], or NULL
+  long rows;
+  int features;
+  Dropout drop;
+};
+
+constexpr int THREADS = 256;
+
+// LONG: more than K L chunks a row; h is formed again in every pass
+template <class T, int L, int K, bool STEP, bool LONG> __global__ __launch_bounds__(THREADS) void forward_kernel(Forward p) {
+  typedef Chunk<T> C;
+  __shared__ float slots[2][4];
+  const int lane = threadIdx.x % L, chunks = (p.features + C::N - 1) / C::N;
+  const int passes = LONG ? (chunks + K * L - 1) / (K * L) : 1;
+  const unsigned long long key = STEP && p.drop.on ? dropout_seed(p.drop) : 0;
+  const T* const w = static_cast<const T*>(p.weight);
+  const T* const b = static_cast<const T*>(p.bias);
+  const float inv_n = 1.f / (float)p.features;
+
+  const auto load_h = [&](long row, int c, float (&v)[C::N]) {       // chunk c of a row: x, or residual + dropout(x)
+    const int n = p.features - c * C::N;
+    const long at = row * p.features + (long)c * C::N;
+    C::get(load_chunk<T>(static_cast<const T*>(p.x) + at, n), v);
+    if constexpr (STEP) {
+      float r[C::N];
+      C::get(load_chunk<T>(static_cast<const T*>(p.residual) + at, n), r);
+      if (p.drop.on) drop<C::N>(p.drop, key, at, v);
+#pragma unroll
+      for (int i = 0; i < C::N; ++i) v[i] += r[i];
+    }
+  };
+
+  for (long row0 = (long)blockIdx.x * (THREADS / L); row0 < p.rows; row0 += (long)gridDim.x * (THREADS / L)) {
+    const long row = row0 + threadIdx.x / L;
+    const bool ok = row < p.rows;
+    const long r = ok ? row : p.rows - 1;
+    float v[K][C::N], sum = 0.f;
+    for (int pass = 0; pass < passes; ++pass) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int c = (pass * K + k) * L + lane;
+        if (c < chunks) load_h(r, c, v[k]);
+        else
+#pragma unroll
+          for (int i = 0; i < C::N; ++i) v[k][i] = 0.f;
+#pragma unroll
+        for (int i = 0; i < C::N; ++i) sum += v[k][i];                // entries past the row's end are zero
+      }
+    }
+    const float mean = sum_group<L>(sum, slots[0]) * inv_n;
+    float square = 0.f;
+    for (int pass = 0; pass < passes; ++pass) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int c = (pass * K + k) * L + lane, n = p.features - c * C::N;
+        if (LONG && c < chunks) load_h(r, c, v[k]);
+#pragma unroll
+        for (int i = 0; i < C::N; ++i)
+          if (i < n) square = fmaf(v[k][i] - mean, v[k][i] - mean, square);
+      }
+    }
+    const float rstd = 1.f / sqrtf(fmaf(sum_group<L>(square, slots[1]), inv_n, p.eps));
+    for (int pass = 0; pass < passes; ++pass) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int c = (pass * K + k) * L + lane, n = p.features - c * C::N;
+        if (c >= chunks || !ok) continue;
+        if (LONG) load_h(r, c, v[k]);
+        const long at = r * p.features + (long)c * C::N;
+        if constexpr (STEP) store_chunk<T>(static_cast<T*>(p.h) + at, n, v[k]);
+        float ws[C::N], bs[C::N], y[C::N];
+        if (w) C::get(load_chunk<T>(w + c * C::N, n), ws);
+        if (b) C::get(load_chunk<T>(b + c * C::N, n), bs);
+#pragma unroll
+        for (int i = 0; i < C::N; ++i) {
+          y[i] = (v[k][i] - mean) * rstd;
+          y[i] = w ? (b ? fmaf(y[i], ws[i], bs[i]) : y[i] * ws[i]) : (b ? y[i] + bs[i] : y[i]);
+        }
+        store_chunk<T>(static_cast<T*>(p.y) + at, n, y);
+      }
+    }
+    if (p.stats && lane == 0 && ok) reinterpret_cast<float2*>(p.stats)[r] = make_float2(mean, rstd);
+  }
+}
+
+template <class T, int L, int K, bool STEP, bool LONG> __global__ __launch_bounds__(THREADS) void backward_kernel(Backward p) {
+  typedef Chunk<T> C;
+  __shared__ float slots[2][4];
+  extern __shared__ float joined[];                                 // the sums of THREADS / L groups, where L < THREADS
+  const int lane = threadIdx.x % L, chunks = (p.features + C::N - 1) / C::N;
+  const int passes = LONG ? (chunks + K * L - 1) / (K * L) : 1;
+  const unsigned long long key = STEP && p.drop.on ? dropout_seed(p.drop) : 0;
+  const T* const w = static_cast<const T*>(p.weight);
+  const T* const hs = static_cast<const T*>(p.h);
+  const T* const gs = static_cast<const T*>(p.g);
+  const float inv_n = 1.f / (float)p.features;
+  float gw[K][C::N] = {}, gb[K][C::N] = {};
+
+  for (long row0 = (long)blockIdx.x * (THREADS / L); row0 < p.rows; row0 += (long)gridDim.x * (THREADS / L)) {
+    const long row = row0 + threadIdx.x / L;
+    const bool ok = row < p.rows;
+    const long r = ok ? row : p.rows - 1;
+    const float2 st = reinterpret_cast<const float2*>(p.stats)[r];
+    uint4 hraw[K], graw[K];
+    float a = 0.f, c2 = 0.f;
+    const auto form = [&](int c, const uint4& hr, const uint4& gr, float (&xh)[C::N], float (&g)[C::N], float (&u)[C::N]) {
+      C::get(hr, xh);
+      C::get(gr, g);
+      float ws[C::N];
+      if (w) C::get(load_chunk<T>(w + c * C::N, p.features - c * C::N), ws);
+#pragma unroll
+      for (int i = 0; i < C::N; ++i) {
+        xh[i] = (xh[i] - st.x) * st.y;
+        u[i] = w ? g[i] * ws[i] : g[i];
+      }
+    };
+    for (int pass = 0; pass < passes; ++pass) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int c = (pass * K + k) * L + lane, n = p.features - c * C::N;
+        hraw[k] = graw[k] = make_uint4(0, 0, 0, 0);
+        if (c >= chunks) continue;
+        hraw[k] = load_chunk<T>(hs + r * p.features + (long)c * C::N, n);
+        graw[k] = load_chunk<T>(gs + r * p.features + (long)c * C::N, n);
+      }
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int c = (pass * K + k) * L + lane;
+        if (c >= chunks) continue;
+        float xh[C::N], g[C::N], u[C::N];
+        form(c, hraw[k], graw[k], xh, g, u);                        // entries past the row's end: g = u = 0
+#pragma unroll
+        for (int i = 0; i < C::N; ++i) {
+          a += u[i];
+          c2 = fmaf(u[i], xh[i], c2);
+          if (!LONG && ok) gw[k][i] = fmaf(g[i], xh[i], gw[k][i]), gb[k][i] += g[i];
+        }
+      }
+    }
+    a = sum_group<L>(a, slots[0]) * inv_n;
+    c2 = sum_group<L>(c2, slots[1]) * inv_n;
+    for (int pass = 0; pass < passes; ++pass) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int c = (pass * K + k) * L + lane, n = p.features - c * C::N;
+        if (c >= chunks || !ok) continue;
+        const long at = r * p.features + (long)c * C::N;
+        if (LONG) hraw[k] = load_chunk<T>(hs + at, n), graw[k] = load_chunk<T>(gs + at, n);
+        float xh[C::N], g[C::N], u[C::N];
+        form(c, hraw[k], graw[k], xh, g, u);
+#pragma unroll
+        for (int i = 0; i < C::N; ++i) u[i] = st.y * (u[i] - a - xh[i] * c2);
+        if constexpr (STEP) {
+          if (p.g_h) {
+            float e[C::N];
+            C::get(load_chunk<T>(static_cast<const T*>(p.g_h) + at, n), e);
+#pragma unroll
+            for (int i = 0; i < C::N; ++i) u[i] += e[i];
+          }
+          if (p.gresidual) store_chunk<T>(static_cast<T*>(p.gresidual) + at, n, u);
+          if (p.gx) {
+            if (p.drop.on) drop<C::N>(p.drop, key, at, u);
+            store_chunk<T>(static_cast<T*>(p.gx) + at, n, u);
+          }
+        } else {
+          store_chunk<T>(static_cast<T*>(p.gx) + at, n, u);
+        }
+      }
+    }
+  }
+  if (LONG || !p.partial) return;
+  float* const out = p.partial + (long)blockIdx.x * 2 * p.features;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = k * L + lane, n = p.features - c * C::N;
+      const float (&v)[C::N] = which ? gb[k] : gw[k];
+      if constexpr (L < THREADS) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < C::N; ++i) joined[(i * (THREADS / L) + threadIdx.x / L) * L + lane] = v[i];
+        __syncthreads();
+        if (threadIdx.x < L)
+#pragma unroll
+          for (int i = 0; i < C::N; ++i) {
+            float t = 0.f;
+            for (int s = 0; s < THREADS / L; ++s) t += joined[(i * (THREADS / L) + s) * L + lane];
+            if (i < n) out[which * p.features + c * C::N + i] = t;
+          }
+      } else {
+#pragma unroll
+        for (int i = 0; i < C::N; ++i)
+          if (i < n) out[which * p.features + c * C::N + i] = v[i];
+      }
+    }
+  }
+}
+
+// dw, db of rows longer than the registers hold: a workgroup takes 64 features and a part of the rows
+template <class T> __global__ __launch_bounds__(THREADS) void long_weights_kernel(Backward p, int parts) {
+  __shared__ float sums[2][4][64];
+  const int f = blockIdx.x * 64 + (threadIdx.x & 63), wave = threadIdx.x >> 6;
+  float gw = 0.f, gb = 0.f;
+  if (f < p.features)
+    for (long r = (long)blockIdx.y * 4 + wave; r < p.rows; r += 4L * parts) {
+      const float2 st = reinterpret_cast<const float2*>(p.stats)[r];
+      const float g = (float)static_cast<const T*>(p.g)[r * p.features + f], h = (float)static_cast<const T*>(p.h)[r * p.features + f];
+      gw = fmaf(g, (h - st.x) * st.y, gw);
+      gb += g;
+    }
+  sums[0][wave][threadIdx.x & 63] = gw;
+  sums[1][wave][threadIdx.x & 63] = gb;
+  __syncthreads();
+  if (wave < 2 && f < p.features) {
+    const float (&s)[4][64] = sums[wave];
+    const int i = threadIdx.x & 63;
+    p.partial[((long)blockIdx.y * 2 + wave) * p.features + f] = (s[0][i] + s[1][i]) + (s[2][i] + s[3][i]);
+  }
+}
+
+// the sums of the workgroups: 32 features a workgroup, 32 groups of lanes over the parts
+template <class T> __global__ __launch_bounds__(1024) void sum_kernel(const float* partial, int parts, int features, T* gw, T* gb) {
+  __shared__ float sums[32][33];
+  const int i = threadIdx.x & 31, s = threadIdx.x >> 5;
+  const long col = (long)blockIdx.x * 32 + i, width = 2L * features;
+  float t = 0.f;
+  if (col < width)
+    for (int k = s; k < parts; k += 32) t += partial[k * width + col];
+  sums[s][i] = t;
+  __syncthreads();
+  t = sum_lanes<32>(sums[i][s]);                    // lanes over the groups: feature s
+  const long out = (long)blockIdx.x * 32 + s;
+  if (i == 0 && out < width) {
+    if (out < features) {
+      if (gw) gw[out] = (T)t;
+    } else if (gb) {
+      gb[out - features] = (T)t;
+    }
+  }
+}
+
+// y = x times the factor of each element; 8 elements a thread, one counter
+template <class T> __global__ __launch_bounds__(THREADS) void dropout_kernel(const T* x, T* y, long n, Dropout d) {
+  typedef Chunk<T> C;
+  const unsigned long long key = dropout_seed(d);
+  const long stride = (long)gridDim.x * THREADS * 8;
+  for (long at = ((long)blockIdx.x * THREADS + threadIdx.x) * 8; at < n; at += stride) {
+    uint4 raw[8 / C::N];
+#pragma unroll
+    for (int k = 0; k < 8 / C::N; ++k) {
+      const long left = n - at - k * C::N;
+      raw[k] = left > 0 ? load_chunk<T>(x + at + k * C::N, (int)min(left, 8L)) : make_uint4(0, 0, 0, 0);
+    }
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8 / C::N; ++k) C::get(raw[k], reinterpret_cast<float (&)[C::N]>(v[k * C::N]));
+    if (d.on) drop<8>(d, key, at, v);
+#pragma unroll
+    for (int k = 0; k < 8 / C::N; ++k) {
+      const long left = n - at - k * C::N;
+      if (left > 0) store_chunk<T>(y + at + k * C::N, (int)min(left, 8L), reinterpret_cast<float (&)[C::N]>(v[k * C::N]));
+    }
+  }
+}
+
+// ---- launches -------------------------------------------------------------------------------------------------------
+constexpr int CUS = 256;
+
+int group_of(int dtype, int features) {              // lanes of a row
+  const int chunks = (features + (dtype == S2CNN_F32 ? 3 : 7)) / (dtype == S2CNN_F32 ? 4 : 8);
+  return chunks <= 32 ? 8 : chunks <= 64 ? 16 : chunks <= 128 ? 32 : chunks <= 256 ? 64 : 256;
+}
+bool is_long(int dtype, int features) { return features > (dtype == S2CNN_F32 ? 4096 : 8192); }
+// Workgroups that run over all rows.  Backward: their number is that of the partial sums, two a CU; forward: eight a CU.
+int workgroups(int dtype, long rows, int features, bool backward) {
+  const long per = THREADS / group_of(dtype, features), need = (rows + per - 1) / per, most = CUS * (backward ? 2 : 8);
+  return (int)(need < most ? need : most);
+}
+int parts_of(int dtype, long rows, int features) {
+  if (!is_long(dtype, features)) return workgroups(dtype, rows, features, true);
+  return (int)((rows + 63) / 64 < 64 ? (rows + 63) / 64 : 64);
+}
+
+template <class T, int L, int K, bool STEP, bool LONG = false> void launch(const Forward& p, int wgs, hipStream_t s) {
+  hipLaunchKernelGGL((forward_kernel<T, L, K, STEP, LONG>), dim3((unsigned)wgs), dim3(THREADS), 0, s, p);
+}
+template <class T, int L, int K, bool STEP, bool LONG = false> void launch(const Backward& p, int wgs, hipStream_t s) {
+  const size_t lds = !LONG && L < THREADS ? THREADS * Chunk<T>::N * sizeof(float) : 0;
+  hipLaunchKernelGGL((backward_kernel<T, L, K, STEP, LONG>), dim3((unsigned)wgs), dim3(THREADS), lds, s, p);
+}
+template <class T, bool STEP, class P> void dispatch(const P& p, int wgs, hipStream_t s) {
+  const int chunks = (p.features + Chunk<T>::N - 1) / Chunk<T>::N;
+  if (chunks <= 8) launch<T, 8, 1, STEP>(p, wgs, s);
+  else if (chunks <= 16) launch<T, 8, 2, STEP>(p, wgs, s);
+  else if (chunks <= 32) launch<T, 8, 4, STEP>(p, wgs, s);
+  else if (chunks <= 64) launch<T, 16, 4, STEP>(p, wgs, s);
+  else if (chunks <= 128) launch<T, 32, 4, STEP>(p, wgs, s);
+  else if (chunks <= 256) launch<T, 64, 4, STEP>(p, wgs, s);
+  else if (chunks <= 1024) launch<T, 256, 4, STEP>(p, wgs, s);
+  else launch<T, 256, 4, STEP, true>(p, wgs, s);
+}
+template <class T> void forward(const Forward& p, bool step, int wgs, hipStream_t s) {
+  if (step) dispatch<T, true>(p, wgs, s);
+  else dispatch<T, false>(p, wgs, s);
+}
+template <class T> void backward(const Backward& p, bool step, int dtype, void* gw, void* gb, hipStream_t s) {
+  const int wgs = workgroups(dtype, p.rows, p.features, true), parts = parts_of(dtype, p.rows, p.features);
+  if (step) dispatch<T, true>(p, wgs, s);
+  else dispatch<T, false>(p, wgs, s);
+  if (!p.partial) return;
+  if (is_long(dtype, p.features))
+    hipLaunchKernelGGL(long_weights_kernel<T>, dim3((unsigned)((p.features + 63) / 64), (unsigned)parts), dim3(THREADS), 0, s, p, parts);
+  hipLaunchKernelGGL(sum_kernel<T>, dim3((unsigned)((2L * p.features + 31) / 32)), dim3(1024), 0, s, p.partial, parts, p.features, static_cast<T*>(gw),
+                     static_cast<T*>(gb));
+}
+template <class T> void dropout(const void* x, void* y, long n, const Dropout& d, hipStream_t s) {
+  const long need = (n + 8 * THREADS - 1) / (8 * THREADS), most = CUS * 16;
+  hipLaunchKernelGGL(dropout_kernel<T>, dim3((unsigned)(need < most ? need : most)), dim3(THREADS), 0, s, static_cast<const T*>(x), static_cast<T*>(y), n, d);
+}
+
+bool sizes_ok(long rows, long features, int dtype) {
+  return rows >= 1 && rows < (1L << 31) && features >= 1 && features < (1L << 24) && (dtype == S2CNN_F32 || dtype == S2CNN_BF16 || dtype == S2CNN_F16);
+}
+template <class... P> bool aligned(int dtype, P... p) {
+  const uintptr_t mask = dtype == S2CNN_F32 ? 3 : 1;
+  return !((reinterpret_cast<uintptr_t>(p) | ...) & mask);
+}
+
+}  // namespace norm
+}  // namespace s2cnn
+
+using namespace s2cnn;
+using namespace s2cnn::norm;
+
+extern "C" int s2cnn_layer_norm_fwd(const void* x, const void* residual, const void* weight, const void* bias, void* h, void* y, float* stats, long rows,
+                              long features, float eps, double p, unsigned long long seed, const long long* seed_at, int dtype, void* stream) {
+  clear_stale_error();
+  if (!sizes_ok(rows, features, dtype) || !x || !y || !residual != !h || !(p >= 0.0 && p < 1.0) || (!residual && p != 0.0)) return S2CNN_EINVAL;
+  if (!aligned(dtype, x, residual, weight, bias, h, y) || !aligned8(stats) || !aligned8(seed_at)) return S2CNN_EALIGN;
+  const Forward f{x, residual, weight, bias, h, y, stats, rows, (int)features, eps, make_dropout(p, seed, seed_at)};
+  const int wgs = workgroups(dtype, rows, (int)features, false);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dtype == S2CNN_F32) norm::forward<float>(f, residual != nullptr, wgs, s);
+  else if (dtype == S2CNN_BF16) norm::forward<__bf16>(f, residual != nullptr, wgs, s);
+  else norm::forward<half_t>(f, residual != nullptr, wgs, s);
+  return launch_status();
+}
+
+extern "C" size_t s2cnn_layer_norm_bwd_workspace(long rows, long features, int dtype) {
+  if (!sizes_ok(rows, features, dtype)) return 0;
+  return (size_t)parts_of(dtype, rows, (int)features) * 2 * features * sizeof(float);
+}
+
+extern "C" int s2cnn_layer_norm_bwd(const void* h, const void* g, const void* g_h, const void* weight, const float* stats, void* gx, void* gresidual, void* gweight,
+                              void* gbias, void* workspace, size_t workspace_bytes, long rows, long features, double p, unsigned long long seed,
+                              const long long* seed_at, int step, int dtype, void* stream) {
+  clear_stale_error();
+  if (!sizes_ok(rows, features, dtype) || !h || !g || !stats || !(p >= 0.0 && p < 1.0)) return S2CNN_EINVAL;
+  if (step ? (!gx && !gresidual) : (!gx || gresidual || g_h || p != 0.0)) return S2CNN_EINVAL;
+  if (!aligned(dtype, h, g, g_h, weight, gx, gresidual, gweight, gbias) || !aligned8(stats) || !aligned8(seed_at)) return S2CNN_EALIGN;
+  const bool sums = gweight || gbias;
+  if (sums && (!workspace || workspace_bytes < s2cnn_layer_norm_bwd_workspace(rows, features, dtype) || !aligned16(workspace))) return S2CNN_EWORKSPACE;
+  const norm::Backward b{h, g, g_h, weight, stats, gx, gresidual, sums ? static_cast<float*>(workspace) : nullptr, rows, (int)features, make_dropout(p, seed, seed_at)};
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dtype == S2CNN_F32) norm::backward<float>(b, step != 0, dtype, gweight, gbias, s);
+  else if (dtype == S2CNN_BF16) norm::backward<__bf16>(b, step != 0, dtype, gweight, gbias, s);
+  else norm::backward<half_t>(b, step != 0, dtype, gweight, gbias, s);
+  return launch_status();
+}
+
+extern "C" int s2cnn_dropout(const void* x, void* y, long n, double p, unsigned long long seed, const long long* seed_at, int dtype, void* stream) {
+  clear_stale_error();
+  if (!x || !y || n < 1 || n >= (1L << 40) || !(p >= 0.0 && p < 1.0) || (dtype != S2CNN_F32 && dtype != S2CNN_BF16 && dtype != S2CNN_F16)) return S2CNN_EINVAL;
+  if (!aligned(dtype, x, y) || !aligned8(seed_at)) return S2CNN_EALIGN;
+  const Dropout d = make_dropout(p, seed, seed_at);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dtype == S2CNN_F32) norm::dropout<float>(x, y, n, d, s);
+  else if (dtype == S2CNN_BF16) norm::dropout<__bf16>(x, y, n, d, s);
+  else norm::dropout<half_t>(x, y, n, d, s);
+  return launch_status();
+}
