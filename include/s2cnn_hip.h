@@ -432,7 +432,7 @@ typedef struct s2cnn_attention_t {
   const float *key_bias;       /* [batch, n_k], rows contiguous                            */
   const int *lengths;          /* [batch]                                                  */
   void *out;                   /* [batch, heads, n_q, d]                                   */
-  float *stats;                /* [batch, heads, n_q, 2], for bwd; 8-byte aligned          */
+  float *stats;                /* [stats_floats], from fwd for bwd; 8-byte aligned         */
   float *out_f32;              /* [batch, heads, n_q, d] dense, for bwd: out before its rounding (16-bit types; else unused) */
   const void *gout;
   void *gq, *gk, *gv, *gtable;
@@ -444,6 +444,8 @@ typedef struct s2cnn_attention_t {
   float scale;
 } s2cnn_attention_t;
 
+#define S2CNN_ATTENTION_STRIDE_LIMIT (1L << 26)   /* strides of vectors of q, k, v, gout are below this */
+size_t s2cnn_attention_stats_floats(const s2cnn_attention_t *a);
 size_t s2cnn_attention_workspace(const s2cnn_attention_t *a, int backward);     /* 0 also for sizes that are refused */
 int s2cnn_attention_fwd(const s2cnn_attention_t *a, void *workspace, size_t workspace_bytes, void *stream);
 int s2cnn_attention_bwd(const s2cnn_attention_t *a, void *workspace, size_t workspace_bytes, void *stream);

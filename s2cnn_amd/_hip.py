@@ -96,6 +96,7 @@ SIGNATURES = {
     "s2cnn_s2_synthesis_workspace": (_size_t, _WS_SIG),
     "s2cnn_s2_synthesis": (_int, _FT_SIG),
     "s2cnn_so3_integrate": (_int, [_c_float_p, _c_float_p, _c_float_p, _int, _long, _vp]),
+    "s2cnn_attention_stats_floats": (_size_t, [_ATTENTION_P]),
     "s2cnn_attention_workspace": (_size_t, [_ATTENTION_P, _int]),
     "s2cnn_attention_fwd": (_int, [_ATTENTION_P, _vp, _size_t, _vp]),
     "s2cnn_attention_bwd": (_int, [_ATTENTION_P, _vp, _size_t, _vp]),

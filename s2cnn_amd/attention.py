@@ -23,6 +23,11 @@ def _unit_last(t):
     return t if t.stride(-1) == 1 or t.size(-1) == 1 else t.contiguous()
 
 
+def _vectors(t):
+    """`t` as the kernels read it: vectors contiguous, less than 2^26 entries apart."""
+    return t if (t.stride(-1) == 1 or t.size(-1) == 1) and t.stride(-2) < 1 << 26 else t.contiguous()
+
+
 def _like(t):
     """Uninitialised, of the shape and order of axes of `t`, vectors contiguous."""
     out = torch.empty_like(t)
@@ -60,14 +65,15 @@ def _run(name, a, backward, device):
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, buckets, key_bias, lengths, scale, dtype, needs_grad):  # pylint: disable=W
-        q, k, v = _unit_last(q), _unit_last(k), _unit_last(v)
+        q, k, v = _vectors(q), _vectors(k), _vectors(v)
         out = _like(q)
-        stats = q.new_empty(q.shape[:3] + (2,), dtype=torch.float32) if needs_grad else None
+        stats = None
         exact = q.new_empty(q.shape, dtype=torch.float32) if needs_grad and q.dtype != torch.float32 else None     # out before its rounding
         if out.numel():
             a = _describe(q, k, v, table, buckets, key_bias, lengths, scale, dtype)
             a.out, a.out_stride[:] = out.data_ptr(), _strides(out)
             if needs_grad:
+                stats = q.new_empty(_hip.lib().s2cnn_attention_stats_floats(ctypes.byref(a)), dtype=torch.float32)
                 a.stats, a.out_f32 = stats.data_ptr(), exact.data_ptr() if exact is not None else None
             _run("s2cnn_attention_fwd", a, 0, q.device)
         if needs_grad:
@@ -82,7 +88,7 @@ class _Attention(torch.autograd.Function):
         if not out.numel() or not k.size(2):
             return (torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v),
                     torch.zeros_like(table) if table is not None else None) + (None,) * 6
-        g = _unit_last(g)
+        g = _vectors(g)
         gq = _like(q)
         wants_kv = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         gk, gv = (_like(k), _like(v)) if wants_kv else (None, None)

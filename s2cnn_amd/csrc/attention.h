@@ -171,17 +171,24 @@ template <class T> __device__ __forceinline__ void store_quad(typename T::type* 
     if (at + i < d) p[at + i] = (typename T::type)x[i];
 }
 
-// The B operands of one column: the vector at `p`, in steps of 16 entries, 8 of them in either half of the wave.
-template <class T, int D> __device__ __forceinline__ void load_column(const typename T::type* p, int d, bool wide, bool ok, int half, Frag<T> (&f)[D / 16]) {
+// The B operands of one column: the vector at `p` (float32: times `factor`), in steps of 16 entries, 8 of them in either half of
+// the wave.
+template <class T, int D>
+__device__ __forceinline__ void load_column(const typename T::type* p, int d, bool wide, bool ok, int half, float factor, Frag<T> (&f)[D / 16]) {
 #pragma unroll
   for (int s = 0; s < D / 16; ++s) {
     Quad a = load_quad<T>(p, 4 * s + 2 * half, d, wide), b = load_quad<T>(p, 4 * s + 2 * half + 1, d, wide);
     if (!ok) a.w = b.w = make_uint4(0, 0, 0, 0);
-    unsigned w[4][T::PARTS];
-    quad_parts<T>(a, w[0], w[1]);
-    quad_parts<T>(b, w[2], w[3]);
+    if constexpr (T::PARTS == 3) {
+      float x[8];
+      quad_values<T>(a, reinterpret_cast<float (&)[4]>(x[0]));
+      quad_values<T>(b, reinterpret_cast<float (&)[4]>(x[4]));
 #pragma unroll
-    for (int q = 0; q < T::PARTS; ++q) f[s].part[q] = make_uint4(w[0][q], w[1][q], w[2][q], w[3][q]);
+      for (int i = 0; i < 8; ++i) x[i] *= factor;
+      f[s] = cut8<T>(x);
+    } else {
+      f[s].part[0] = make_uint4(a.w.x, a.w.y, b.w.x, b.w.y);
+    }
   }
 }
 
@@ -263,38 +270,89 @@ template <class T, int D> struct Tile {
   }
 };
 
+// LDS of a kernel that stages `layouts` layouts of a tile: two tiles where they fit beside a second workgroup (of half the wave
+// slots), so that a tile is written while the one before is used, with one barrier per tile; else one.
+template <class T, int D> constexpr int buffers(int layouts) { return 2 * layouts * Tile<T, D>::BYTES <= 80 * 1024 ? 2 : 1; }
+
 // Two tensors staged by the same tiles of rows: THREADS threads fetch the blocks of a tile into registers, and write them later.
+// The address of a block's rows is a uniform pointer, moved on by the tile, and an offset of the thread that stays (below
+// 2^31 bytes: the entry checks 32 strides).
 template <class T, int D, int THREADS> struct Stage {
   typedef Tile<T, D> Tl;
+  typedef typename T::type E;
   static constexpr int PER = (2 * Tl::BLOCKS + THREADS - 1) / THREADS;
+  static constexpr bool IDLE = 2 * Tl::BLOCKS % THREADS != 0;      // some threads have no block
   Quad v[PER][4];
+
+  // of the thread's block u: which tensor (uniform in a wave), and which block of it
+  static __device__ __forceinline__ bool second(int u, int tid) {
+    if constexpr (Tl::BLOCKS % THREADS == 0) return u >= PER / 2;
+    else return __builtin_amdgcn_readfirstlane(u * THREADS + tid) >= Tl::BLOCKS;
+  }
+  static __device__ __forceinline__ bool idle(int u, int tid) { return IDLE && __builtin_amdgcn_readfirstlane(u * THREADS + tid) >= 2 * Tl::BLOCKS; }
+  static __device__ __forceinline__ int block(int u, int tid) { return (u * THREADS + tid) % Tl::BLOCKS; }
 
   __device__ __forceinline__ void fetch(const Vectors<T>& a, const Vectors<T>& b, int row0, int tid) {
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
-      const int k = u * THREADS + tid, kk = k % Tl::BLOCKS;
-      if (2 * Tl::BLOCKS % THREADS != 0 && k >= 2 * Tl::BLOCKS) break;
-      const Vectors<T>& x = k < Tl::BLOCKS ? a : b;
+      if (idle(u, tid)) break;
+      const Vectors<T>& x = second(u, tid) ? b : a;
+      const int kk = block(u, tid), q = kk % (D / 4), row = 4 * (kk / (D / 4));
+      const E* const base = x.base + (long)row0 * x.stride;
+      const int stride = (int)x.stride, left = x.n - 1 - row0;     // last row of the tile that exists
+      if (x.wide && left >= ROWS - 1) {
+        const int at = row * stride + (4 * q < x.d ? 4 * q : 0);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = row0 + 4 * (kk / (D / 4)) + i;
-        v[u][i] = load_quad<T>(x.base + (long)min(row, x.n - 1) * x.stride, kk % (D / 4), x.d, x.wide);
+        for (int i = 0; i < 4; ++i) {
+          const E* const p = base + i * x.stride + (unsigned)at;
+          if constexpr (T::PARTS == 3) v[u][i].w = *reinterpret_cast<const uint4*>(p);
+          else {
+            const uint2 w = *reinterpret_cast<const uint2*>(p);
+            v[u][i].w = make_uint4(w.x, w.y, 0, 0);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[u][i] = load_quad<T>(base + (long)min(row + i, left) * x.stride, q, x.d, x.wide);
       }
     }
   }
   // keep(row of the tile): false for rows that count as zero, whatever their memory holds
   template <class Keep>
-  __device__ __forceinline__ void write(unsigned char* a_rows, unsigned char* a_entries, unsigned char* b_rows, unsigned char* b_entries, int tid, Keep keep) {
+  __device__ __forceinline__ void write(unsigned char* a_rows, unsigned char* a_entries, unsigned char* b_rows, unsigned char* b_entries, int tid, int d, Keep keep) {
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
-      const int k = u * THREADS + tid, kk = k % Tl::BLOCKS;
-      if (2 * Tl::BLOCKS % THREADS != 0 && k >= 2 * Tl::BLOCKS) break;
+      if (idle(u, tid)) break;
+      const int kk = block(u, tid), row = 4 * (kk / (D / 4));
+      const bool column = 4 * (kk % (D / 4)) < d;
+      bool k[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (!keep(4 * (kk / (D / 4)) + i)) v[u][i].w = make_uint4(0, 0, 0, 0);
-      if (k < Tl::BLOCKS) Tl::write(a_rows, a_entries, kk, v[u]);
-      else Tl::write(b_rows, b_entries, kk, v[u]);
+      for (int i = 0; i < 4; ++i) k[i] = keep(row + i) && column;
+      if (!__all(k[0] && k[1] && k[2] && k[3])) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!k[i]) v[u][i].w = make_uint4(0, 0, 0, 0);
+      }
+      if (second(u, tid)) Tl::write(b_rows, b_entries, kk, v[u]);
+      else Tl::write(a_rows, a_entries, kk, v[u]);
     }
+  }
+  // the largest |entry| of the second tensor's blocks, as they were written
+  __device__ __forceinline__ float largest_second(int tid) const {
+    float t = 0.f;
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      if (idle(u, tid)) break;
+      if (!second(u, tid)) continue;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x[4];
+        quad_values<T>(v[u][i], x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t = fmaxf(t, fabsf(x[e]));
+      }
+    }
+    return t;
   }
 };
 
@@ -304,14 +362,20 @@ template <class T, int D, int THREADS> struct Stage {
 // probability rounded to 16 bits is then the same whatever the reference was when it was formed, up to the power of two, and
 // the sums, the output and the backward pass all use the same, rounded ones.  They are so the exact softmax of weights that
 // are off by a rounding each, rows of its gradient sum to zero as they should, and a factor between references is exact.
-// A key bias of the type's lowest value stays finite so: keys that all have it share a row evenly, as they do without the factor.
-__device__ __forceinline__ float key_bias_base2(const float* key_bias, int key) { return fmaxf(key_bias[key], -2.3e38f) * LOG2E; }
-// value of a key in LDS: -inf for keys that take no part
-__device__ __forceinline__ float key_value(const float* key_bias, int key, int end) {
-  if (key >= end) return ninf();
+//
+// The product starts from the key's bias instead of zero: x = c (q.k + bias / c) + table, c = log2(e) scale; float32 takes c into
+// the columns as they are loaded, and needs no factor.  Biases are held within +-3e38, so that one of the type's lowest value
+// stays finite: keys that all have it share a row evenly.
+__device__ __forceinline__ float key_value(const float* key_bias, int key, int end, float inv_c) {
+  if (key >= end) return ninf() * inv_c;                   // takes no part
   if (!key_bias) return 0.f;
-  return key_bias[key] == ninf() ? ninf() : key_bias_base2(key_bias, key);
+  const float b = key_bias[key], x = b * LOG2E * inv_c;
+  return fabsf(b) < pinf() ? __builtin_amdgcn_fmed3f(x, -3e38f, 3e38f) : x;
 }
+
+// A tile's values of its rows (keys' biases; the queries' statistics) in LDS, in a ring: tile t's are read in step t, and in step
+// t - 1, in which its rows are written; they are put there in step t - 2.
+constexpr int RING = 4;
 
 // the table's rows of heads head0 .. head0 + heads - 1 in LDS, n_buckets + 1 entries a head, the last one for excluded pairs
 template <class T> __device__ __forceinline__ void stage_table(float* lds, const void* table, int n_buckets, int head0, int heads, int tid, int threads) {
@@ -346,6 +410,8 @@ __device__ __forceinline__ int bucket_of(unsigned w, int i, int n_buckets) { ret
 enum Wide { WIDE_Q = 1, WIDE_K = 2, WIDE_V = 4, WIDE_OUT = 8, WIDE_GOUT = 16, WIDE_GQ = 32, WIDE_GK = 64, WIDE_GV = 128 };
 struct Args {
   s2cnn_attention_t a;
+  float c, inv_c;          // log2(e) scale and its inverse
+  int forward_splits;
   int wide;                // tensors whose vectors can be read and written four entries at a time
   int splits;              // parts of the long axis (keys; queries in the kernel of dk and dv)
   int tiles;               // workgroups along the columns

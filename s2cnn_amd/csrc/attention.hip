@@ -40,6 +40,8 @@ Plans plans_of(const s2cnn_attention_t& a) {
   return p;
 }
 
+long stats_floats(const s2cnn_attention_t& a, const Plans& p) { return 2L * a.batch * a.heads * a.n_q + (long)a.batch * a.kv_heads * p.fwd.splits; }
+
 bool sizes_ok(const s2cnn_attention_t* a) {
   if (!a) return false;
   if (a->dtype != S2CNN_F32 && a->dtype != S2CNN_BF16 && a->dtype != S2CNN_F16) return false;
@@ -48,6 +50,8 @@ bool sizes_ok(const s2cnn_attention_t* a) {
   if (bias && (!a->buckets || !a->table || a->n_buckets < 1 || a->n_buckets > MAX_BUCKETS || a->heads / a->kv_heads > 128)) return false;
   const long limit = 1L << 30;
   if ((long)a->heads / a->kv_heads * a->n_q > limit || a->n_k > limit || (long)a->batch * a->heads > limit) return false;
+  for (const long* s : {a->q_stride, a->k_stride, a->v_stride, a->gout_stride})
+    if (s[2] < 0 || s[2] >= S2CNN_ATTENTION_STRIDE_LIMIT) return false;
   const Plans p = plans_of(*a);
   return p.fwd.workgroups < limit && p.grad_q.workgroups < limit && p.grad_kv.workgroups < limit && (long)a->batch * a->heads * a->n_q < 4 * limit &&
          (long)a->batch * a->kv_heads * a->n_k < 4 * limit;
@@ -79,6 +83,18 @@ int wide(const s2cnn_attention_t& a) {
          one(a.gout, a.gout_stride, WIDE_GOUT) | one(a.gq, a.gq_stride, WIDE_GQ) | one(a.gk, a.gk_stride, WIDE_GK) | one(a.gv, a.gv_stride, WIDE_GV);
 }
 
+Args args_of(const s2cnn_attention_t& a, const Plans& plans) {
+  Args p{};
+  p.a = a;
+  p.wide = wide(a);
+  p.forward_splits = plans.fwd.splits;
+  // float32 takes the factor into its columns; the others into the scores, and its inverse into the biases: never zero
+  const float c = a.dtype == S2CNN_F32 ? 1.f : a.scale * LOG2E;
+  p.c = fabsf(c) < 1e-30f ? 1e-30f : c;
+  p.inv_c = 1.f / p.c;
+  return p;
+}
+
 bool aligned_to_type(const s2cnn_attention_t& a) {
   const uintptr_t mask = a.dtype == S2CNN_F32 ? 3 : 1;
   for (const void* p : {a.q, a.k, a.v, a.table, (const void*)a.out, a.gout, (const void*)a.gq, (const void*)a.gk, (const void*)a.gv, (const void*)a.gtable})
@@ -99,6 +115,8 @@ extern "C" size_t s2cnn_attention_workspace(const s2cnn_attention_t* a, int back
   return backward ? backward_layout(*a, p).bytes : forward_bytes(*a, p);
 }
 
+extern "C" size_t s2cnn_attention_stats_floats(const s2cnn_attention_t* a) { return sizes_ok(a) ? (size_t)stats_floats(*a, plans_of(*a)) : 0; }
+
 extern "C" int s2cnn_attention_fwd(const s2cnn_attention_t* a, void* workspace, size_t workspace_bytes, void* stream) {
   clear_stale_error();
   if (!sizes_ok(a) || !a->q || !a->out || (a->n_k > 0 && (!a->k || !a->v))) return S2CNN_EINVAL;
@@ -106,9 +124,7 @@ extern "C" int s2cnn_attention_fwd(const s2cnn_attention_t* a, void* workspace, 
   const Plans plans = plans_of(*a);
   const size_t need = forward_bytes(*a, plans);
   if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return S2CNN_EWORKSPACE;
-  Args p{};
-  p.a = *a;
-  p.wide = wide(*a);
+  Args p = args_of(*a, plans);
   p.splits = plans.fwd.splits, p.tiles = plans.fwd.tiles, p.workgroups = (int)plans.fwd.workgroups;
   p.partial = static_cast<float*>(workspace);
   const hipStream_t st = static_cast<hipStream_t>(stream);
@@ -127,9 +143,7 @@ extern "C" int s2cnn_attention_bwd(const s2cnn_attention_t* a, void* workspace, 
   const Backward w = backward_layout(*a, plans);
   if (!workspace || workspace_bytes < w.bytes || !aligned16(workspace)) return S2CNN_EWORKSPACE;
   char* const at = static_cast<char*>(workspace);
-  Args p{};
-  p.a = *a;
-  p.wide = wide(*a);
+  Args p = args_of(*a, plans);
   p.delta = reinterpret_cast<float*>(at + w.delta);
   p.gtable_partial = reinterpret_cast<float*>(at + w.table);
   const hipStream_t st = static_cast<hipStream_t>(stream);

@@ -31,17 +31,25 @@ template <class T> __device__ __forceinline__ ScoreScale score_scale(int n_k, fl
 }
 
 // ---- dq, dtable, delta ----------------------------------------------------------------------------------------------
-// Columns: queries of one head.  dtable: every lane adds to sums of its own in LDS, [wave][bucket][lane], one more bucket for
-// pairs that have none; a wave's instructions run in order, so no sum depends on timing.
-template <class T, int D, int W> __global__ __launch_bounds__(64 * W, 1) void grad_q_kernel(Args p) {
+// Sums of the table's gradient.  LDS adds floats at one lane per three clocks (190 clocks a wave instruction, measured) and
+// integers at full rate (7 clocks, 64 bits), and integers give the same sum in any order: a value goes in as a 64-bit integer
+// in units of a power of two that the workgroup knows beforehand.  |ds| <= 2 max(sum_d |dout_d|) max |v|, both maxima over what the
+// workgroup sees, and a query's |ds| add up to no more than that: 2^50 units for twice the bound leaves room for the queries of a
+// workgroup, and a unit is 2^-49 of the bound, 2^-28 of a typical ds in a row of 10^6 keys.
+// 32 copies, one per query of a wave and shared by waves, keep lanes from the same address.
+struct TableSums {
+  static constexpr int COPIES = 32;
+  static constexpr double MAGIC = 6755399441055744.0;        // 1.5 * 2^52: adding it rounds to an integer, which its low bits hold
+  static __host__ __device__ int words(int n_buckets) { return (n_buckets + 1) * COPIES; }       // one more for excluded pairs
+};
+
+template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS * D > 128 ? 1 : 2) void grad_q_kernel(Args p) {
   typedef Tile<T, D> Tl;
+  constexpr int BUFS = buffers<T, D>(3), BUF = 3 * Tl::BYTES;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  unsigned char* const lds_k = smem;
-  unsigned char* const lds_kt = smem + Tl::BYTES;
-  unsigned char* const lds_v = smem + 2 * Tl::BYTES;
-  float* const lds_kb = reinterpret_cast<float*>(smem + 3 * Tl::BYTES);       // [2][ROWS]
-  float* const lds_table = lds_kb + 2 * ROWS;                                 // [MAX_BUCKETS + 4]
-  float* const lds_sums = lds_table + MAX_BUCKETS + 4;
+  float* const lds_kb = reinterpret_cast<float*>(smem + BUFS * BUF);          // [RING][ROWS]
+  float* const lds_table = lds_kb + RING * ROWS;                              // [MAX_BUCKETS + 4]
+  unsigned long long* const lds_sums = reinterpret_cast<unsigned long long*>(lds_table + MAX_BUCKETS + 4);
   const s2cnn_attention_t& a = p.a;
 
   const int work = work_of_block(p.workgroups);
@@ -52,7 +60,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, 1) void gr
   const int query_ = tile * 32 * W + wave * 32 + (lane & 31);
   const bool ok = query_ < a.n_q;
   const int query = ok ? query_ : a.n_q - 1;
-  const long row = ((long)b * a.heads + head) * a.n_q + query;
+  const long row = ((long)b * a.heads + head) * a.n_q + query, rows = (long)a.batch * a.heads * a.n_q;
 
   int end = a.n_k;
   if (a.lengths) end = max(0, min(end, a.lengths[b]));
@@ -65,8 +73,9 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, 1) void gr
   const Vectors<T> v{static_cast<const E*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[1], a.v_stride[2], a.n_k, a.d, (p.wide & WIDE_V) != 0};
   const float* const key_bias = a.key_bias ? a.key_bias + b * a.key_bias_stride : nullptr;
   const signed char* const buckets = a.buckets ? a.buckets + b * a.bucket_stride[0] + query * a.bucket_stride[1] : nullptr;
-  float* const sums = lds_sums + (wave * (a.n_buckets + 1)) * 64 + lane;
+  unsigned long long* const sums = lds_sums + (lane & 31);
   const bool table_grad = a.gtable != nullptr;
+  const float dead = ninf() * p.inv_c;
 
   Stage<T, D, 64 * W> stage;
   unsigned words[4] = {0, 0, 0, 0};
@@ -74,10 +83,10 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, 1) void gr
     stage.fetch(k, v, key0, tid);
     if (buckets) load_buckets(buckets, key0, end, half, words);
   }
-  if (tid < ROWS) lds_kb[tid] = key_value(key_bias, key0 + tid, end);
+  if (tid < 2 * ROWS) lds_kb[tid] = key_value(key_bias, key0 + tid, end, p.inv_c);
   if (buckets) stage_table<T>(lds_table, a.table, a.n_buckets, head, 1, tid, 64 * W);
   if (table_grad)
-    for (int n = 0; n <= a.n_buckets; ++n) sums[n * 64] = 0.f;
+    for (int n = tid; n < TableSums::words(a.n_buckets); n += 64 * W) lds_sums[n] = 0;
 
   Frag<T> qf[D / 16], gf[D / 16];
   const E* const g_row = static_cast<const E*>(a.gout) + b * a.gout_stride[0] + head * a.gout_stride[1] + query * a.gout_stride[2];
@@ -87,9 +96,10 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, 1) void gr
   const float2 stats = reinterpret_cast<const float2*>(a.stats)[row];
   const float m = ok ? stats.x : pinf(), inv_l = ok ? stats.y : 0.f;
   const bool live = inv_l != 0.f;                          // a row without keys takes no part, whatever its gradient holds
-  load_column<T, D>(static_cast<const E*>(a.q) + b * a.q_stride[0] + head * a.q_stride[1] + query * a.q_stride[2], a.d, (p.wide & WIDE_Q) != 0, live, half, qf);
-  load_column<T, D>(g_row, a.d, wide_g, live, half, gf);
-  float delta = 0.f, largest = 0.f;
+  load_column<T, D>(static_cast<const E*>(a.q) + b * a.q_stride[0] + head * a.q_stride[1] + query * a.q_stride[2], a.d, (p.wide & WIDE_Q) != 0, live, half,
+                    a.scale * LOG2E, qf);
+  load_column<T, D>(g_row, a.d, wide_g, live, half, 1.f, gf);
+  float delta = 0.f, largest = 0.f, total = 0.f;
 #pragma unroll
   for (int i = 0; i < D / 8; ++i) {
     const int quad = 4 * (i / 2) + 2 * half + i % 2;
@@ -99,72 +109,106 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, 1) void gr
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       delta = fmaf(g4[j], o4[j], delta);
+      total += fabsf(g4[j]);
       if constexpr (T::HALF) largest = fmaxf(largest, fabsf(g4[j]));
     }
   }
   delta = live ? half_sum(delta) : 0.f;
+  total = live ? half_sum(total) : 0.f;
   if constexpr (T::HALF) largest = live ? half_max(largest) : 0.f;
   if (split == 0 && half == 0 && ok) {
     p.delta[row] = delta;
-    if constexpr (T::HALF) p.delta[(long)a.batch * a.heads * a.n_q + row] = largest;
+    if constexpr (T::HALF) p.delta[rows + row] = largest;
   }
   const ScoreScale sc = score_scale<T>(a.n_k, largest);
   const float rl = inv_l * sc.p, delta_s = delta * sc.ds;
+  const float undo = T::HALF ? 1.f / (sc.p * sc.ds) : 1.f;
 
-  const float scale = a.scale * LOG2E;
+  // the unit of the table's sums; NaN where the gradient or a value seen by some query is none or infinite: delta is too, then
+  double unit = 0.0;
+  if (table_grad) {
+    float vmax = 0.f;
+    for (int i = 0; i < p.forward_splits; ++i) vmax = fmaxf(vmax, a.stats[2 * rows + (b * a.kv_heads + hk) * p.forward_splits + i]);
+    double bound = fabsf(delta) < pinf() ? (double)total * vmax : (double)pinf();
+#pragma unroll
+    for (int i = 32; i; i >>= 1) bound = fmax(bound, __shfl_xor(bound, i));
+    double* const at = reinterpret_cast<double*>(smem);
+    if (lane == 0) at[wave] = bound;
+    __syncthreads();
+    for (int i = 0; i < W; ++i) bound = fmax(bound, at[i]);
+    __syncthreads();
+    unit = bound == 0.0 ? 1.0 : bound < (double)pinf() ? ldexp(1.0, 48 - ilogb(bound)) : (double)__builtin_nanf("");
+  }
+  const double to_units = unit * undo;
+  const auto write = [&](int step) {
+    unsigned char* const to = smem + step % BUFS * BUF;
+    const float* const kb = lds_kb + step % RING * ROWS;
+    stage.write(to, to + Tl::BYTES, to + 2 * Tl::BYTES, nullptr, tid, a.d, [&](int r) { return kb[r] != dead; });
+  };
+  if (BUFS == 2) {
+    __syncthreads();
+    if (key0 < end) write(0);
+    if (key0 + ROWS < end) stage.fetch(k, v, key0 + ROWS, tid);
+  }
+
   v16f dq[D / 32] = {};
-  int slot = 0;
-  for (int key = key0; key < end; key += ROWS, slot ^= 1) {
-    const float* const kb = lds_kb + slot * ROWS;
+  int step = 0;
+  for (int key = key0; key < end; key += ROWS, ++step) {
+    const bool more = key + ROWS < end;
     __syncthreads();
-    stage.write(lds_k, lds_kt, lds_v, nullptr, tid, [&](int r) { return kb[r] != ninf(); });
-    __syncthreads();
+    if (BUFS == 1) {
+      write(step);
+      __syncthreads();
+    }
+    const unsigned char* const lds_k = smem + step % BUFS * BUF;
+    const unsigned char* const lds_kt = lds_k + Tl::BYTES;
+    const unsigned char* const lds_v = lds_k + 2 * Tl::BYTES;
+    const float* const kb = lds_kb + step % RING * ROWS;
+
+    v16f s, dp = {};
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float4 kb4 = *reinterpret_cast<const float4*>(kb + 8 * g + 4 * half);
+      s[4 * g] = kb4.x, s[4 * g + 1] = kb4.y, s[4 * g + 2] = kb4.z, s[4 * g + 3] = kb4.w;
+    }
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) mma<T>(Tl::by_rows(lds_k, i, lane), qf[i], s);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) mma<T>(Tl::by_rows(lds_v, i, lane), gf[i], dp);
+    if (BUFS == 2 && more) write(step + 1);
     unsigned now[4];
 #pragma unroll
     for (int g = 0; g < 4; ++g) now[g] = words[g];
     float kb_next = 0.f;
-    const bool more = key + ROWS < end;
-    if (more) {
-      stage.fetch(k, v, key + ROWS, tid);
-      if (buckets) load_buckets(buckets, key + ROWS, end, half, words);
-      if (tid < ROWS) kb_next = key_value(key_bias, key + ROWS + tid, end);
-    }
+    if (key + BUFS * ROWS < end) stage.fetch(k, v, key + BUFS * ROWS, tid);
+    if (more && buckets) load_buckets(buckets, key + ROWS, end, half, words);
+    if (tid < ROWS) kb_next = key_value(key_bias, key + 2 * ROWS + tid, end, p.inv_c);
 
-    v16f s = {}, dp = {};
     int n_of[16];
+    if (buckets) {
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      mma<T>(Tl::by_rows(lds_k, i, lane), qf[i], s);
-      mma<T>(Tl::by_rows(lds_v, i, lane), gf[i], dp);
-    }
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const float4 kb4 = *reinterpret_cast<const float4*>(kb + 8 * g + 4 * half);
-      const float kbs[4] = {kb4.x, kb4.y, kb4.z, kb4.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 4 * g + i;
-        float x;
-        int n = 0;
-        if (buckets) {
-          n = bucket_of(now[g], i, a.n_buckets);
-          x = fmaf(s[r], scale, lds_table[n]) + kbs[i];
-          if (n == a.n_buckets) x = ninf();
-        } else {
-          x = fmaf(s[r], scale, kbs[i]);
-        }
-        s[r] = exp2_(x - m);
-        n_of[r] = n;
+      for (int r = 0; r < 16; ++r) {
+        n_of[r] = bucket_of(now[r / 4], r % 4, a.n_buckets);
+        const float t = lds_table[n_of[r]];
+        s[r] = T::PARTS == 3 ? s[r] + t : fmaf(s[r], p.c, t);
       }
+    } else if (T::PARTS == 1) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] *= p.c;
     }
 #pragma unroll
     for (int r = 0; r < 16; r += 2) {
-      float pr[2] = {s[r], s[r + 1]};
+      float pr[2] = {exp2_(s[r] - m), exp2_(s[r + 1] - m)};
       round_pair<T>(pr[0], pr[1]);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        s[r + i] = pr[i] * rl * (T::HALF ? fmaf(dp[r + i], sc.ds, -delta_s) : dp[r + i] - delta);
-        if (table_grad) __hip_atomic_fetch_add(sums + n_of[r + i] * 64, s[r + i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+      for (int i = 0; i < 2; ++i) s[r + i] = pr[i] * rl * (T::HALF ? fmaf(dp[r + i], sc.ds, -delta_s) : dp[r + i] - delta);
+    }
+    if (table_grad) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const double x = __builtin_fma((double)s[r], to_units, TableSums::MAGIC);
+        const unsigned long long bits = __builtin_bit_cast(unsigned long long, x) - __builtin_bit_cast(unsigned long long, TableSums::MAGIC);
+        __hip_atomic_fetch_add(sums + n_of[r] * TableSums::COPIES, bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
       }
     }
 #pragma unroll
@@ -173,25 +217,20 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, 1) void gr
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) mma<T>(Tl::by_entries(lds_kt, i, t, lane), f, dq[i]);
     }
-    if (more && tid < ROWS) lds_kb[(slot ^ 1) * ROWS + tid] = kb_next;
+    if (tid < ROWS) lds_kb[(step + 2) % RING * ROWS + tid] = kb_next;
   }
 
-  const float undo = T::HALF ? 1.f / (sc.p * sc.ds) : 1.f;
   if (table_grad) {
-    if constexpr (T::HALF)
-      for (int n = 0; n < a.n_buckets; ++n) sums[n * 64] *= undo;
     __syncthreads();
     float* const part = p.gtable_partial + ((long)bh * p.splits * p.tiles + split * p.tiles + tile) * a.n_buckets;
     for (int n = tid; n < a.n_buckets; n += 64 * W) {
-      float t = 0.f;
-      for (int w = 0; w < W; ++w)
-        for (int i = 0; i < 64; ++i) t += lds_sums[(w * (a.n_buckets + 1) + n) * 64 + ((i + n) & 63)];   // lanes start at banks of their own
-      part[n] = t;
+      unsigned long long t = 0;
+      for (int i = 0; i < TableSums::COPIES; ++i) t += lds_sums[n * TableSums::COPIES + ((i + n) & 31)];   // lanes start at banks of their own
+      part[n] = (float)((double)(long long)t / unit);
     }
   }
   if (!ok) return;
   if (p.splits > 1) {
-    const long rows = (long)a.batch * a.heads * a.n_q;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) dq[i] *= a.scale * undo;
     store_partial<D>(p.partial + (split * rows + row) * D, half, dq);
@@ -202,15 +241,12 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, 1) void gr
 
 // ---- dk, dv ---------------------------------------------------------------------------------------------------------
 // Columns: keys of one key head.  Rows: the queries of its heads, tile by tile, head by head.
-template <class T, int D, int W> __global__ __launch_bounds__(64 * W, 1) void grad_kv_kernel(Args p) {
+template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS * D > 64 ? 1 : 2) void grad_kv_kernel(Args p) {
   typedef Tile<T, D> Tl;
+  constexpr int BUFS = 2 * 4 * Tl::BYTES <= 100 * 1024 ? 2 : 1, BUF = 4 * Tl::BYTES;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  unsigned char* const lds_q = smem;
-  unsigned char* const lds_qt = smem + Tl::BYTES;
-  unsigned char* const lds_g = smem + 2 * Tl::BYTES;
-  unsigned char* const lds_gt = smem + 3 * Tl::BYTES;
-  float* const lds_rows = reinterpret_cast<float*>(smem + 4 * Tl::BYTES);     // [2][3][ROWS]: m, 1 / l, delta
-  float* const lds_table = lds_rows + 6 * ROWS;
+  float* const lds_rows = reinterpret_cast<float*>(smem + BUFS * BUF);        // [RING][3][ROWS]: m, 1 / l, delta; first two negated
+  float* const lds_table = lds_rows + 3 * RING * ROWS;
   const s2cnn_attention_t& a = p.a;
 
   const int work = work_of_block(p.workgroups);
@@ -234,12 +270,13 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, 1) void gr
   typedef typename T::type E;
   const float* const key_bias = a.key_bias ? a.key_bias + b * a.key_bias_stride : nullptr;
   const signed char* const buckets = a.buckets ? a.buckets + b * a.bucket_stride[0] + key : nullptr;
-  const float kb = ok ? key_value(key_bias, key, end) : ninf();
-  const bool live = kb != ninf();
+  const float dead = ninf() * p.inv_c, kb_c = ok ? key_value(key_bias, key, end, p.inv_c) : dead, kb = kb_c * p.c;
+  const bool live = kb_c != dead;
 
   Frag<T> kf[D / 16], vf[D / 16];
-  load_column<T, D>(static_cast<const E*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[1] + key * a.k_stride[2], a.d, (p.wide & WIDE_K) != 0, live, half, kf);
-  load_column<T, D>(static_cast<const E*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[1] + key * a.v_stride[2], a.d, (p.wide & WIDE_V) != 0, live, half, vf);
+  load_column<T, D>(static_cast<const E*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[1] + key * a.k_stride[2], a.d, (p.wide & WIDE_K) != 0, live, half,
+                    a.scale * LOG2E, kf);
+  load_column<T, D>(static_cast<const E*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[1] + key * a.v_stride[2], a.d, (p.wide & WIDE_V) != 0, live, half, 1.f, vf);
 
   ScoreScale sc;
   if constexpr (T::HALF) {                                 // one for all heads and queries: they are summed
@@ -266,29 +303,41 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, 1) void gr
   struct Row { float m, rl, delta; };
   const auto row_of = [&](int r) -> Row {                  // what thread tid < ROWS brings for row tid of tile r
     const int query = r % per_head * ROWS + tid;
-    if (query >= a.n_q) return {pinf(), 0.f, 0.f};
+    if (r >= last || query >= a.n_q) return {ninf(), 0.f, 0.f};
     const long row = ((long)b * a.heads + hk * group + r / per_head) * a.n_q + query;
     const float2 st = reinterpret_cast<const float2*>(a.stats)[row];
-    return {st.x, st.y * sc.p, p.delta[row] * sc.ds};
+    return {-st.x, st.y * sc.p, -p.delta[row]};
   };
-  const auto put_row = [&](int slot, const Row& x) {
-    float* const to = lds_rows + slot * 3 * ROWS + tid;
+  const auto put_row = [&](int r, const Row& x) {
+    float* const to = lds_rows + (r - first) % RING * 3 * ROWS + tid;
     to[0] = x.m, to[ROWS] = x.rl, to[2 * ROWS] = x.delta;
   };
-  if (first < last) {
-    fetch(first);
-    if (tid < ROWS) put_row(0, row_of(first));
-  }
+  const auto write = [&](int r) {
+    unsigned char* const to = smem + (r - first) % BUFS * BUF;
+    const float* const rows = lds_rows + (r - first) % RING * 3 * ROWS;
+    stage.write(to, to + Tl::BYTES, to + 2 * Tl::BYTES, to + 3 * Tl::BYTES, tid, a.d, [&](int i) { return rows[ROWS + i] != 0.f; });
+  };
+  if (first < last) fetch(first);
+  if (tid < ROWS) put_row(first, row_of(first)), put_row(first + 1, row_of(first + 1));
   if (buckets) stage_table<T>(lds_table, a.table, a.n_buckets, hk * group, group, tid, 64 * W);
+  if (BUFS == 2) {
+    __syncthreads();
+    if (first < last) write(first);
+    if (first + 1 < last) fetch(first + 1);
+  }
 
-  const float scale = a.scale * LOG2E;
   v16f dk[D / 32] = {}, dv[D / 32] = {};
-  int slot = 0;
-  for (int r = first; r < last; ++r, slot ^= 1) {
-    const float* const rows = lds_rows + slot * 3 * ROWS;
+  for (int r = first; r < last; ++r) {
+    const float* const rows = lds_rows + (r - first) % RING * 3 * ROWS;
+    const unsigned char* const lds_q = smem + (r - first) % BUFS * BUF;
+    const unsigned char* const lds_qt = lds_q + Tl::BYTES;
+    const unsigned char* const lds_g = lds_q + 2 * Tl::BYTES;
+    const unsigned char* const lds_gt = lds_q + 3 * Tl::BYTES;
     __syncthreads();
-    stage.write(lds_q, lds_qt, lds_g, lds_gt, tid, [&](int i) { return rows[ROWS + i] != 0.f; });
-    __syncthreads();
+    if (BUFS == 1) {
+      write(r);
+      __syncthreads();
+    }
     const int query0 = r % per_head * ROWS;
     unsigned n_of[16];
     if (buckets) {
@@ -296,47 +345,53 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, 1) void gr
       for (int i = 0; i < 16; ++i)
         n_of[i] = (unsigned char)buckets[min(query0 + 8 * (i / 4) + 4 * half + i % 4, a.n_q - 1) * a.bucket_stride[1]];
     }
-    Row next = {};
-    const bool more = r + 1 < last;
-    if (more) {
-      fetch(r + 1);
-      if (tid < ROWS) next = row_of(r + 1);
-    }
     const float* const table = lds_table + r / per_head * (a.n_buckets + 1);
 
-    v16f s = {}, dp = {};
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      mma<T>(Tl::by_rows(lds_q, i, lane), kf[i], s);
-      mma<T>(Tl::by_rows(lds_g, i, lane), vf[i], dp);
-    }
+    // float32: the scores start from -m; dp starts from -delta
+    v16f s = {}, dp;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const float4 m4 = *reinterpret_cast<const float4*>(rows + 8 * g + 4 * half), l4 = *reinterpret_cast<const float4*>(rows + ROWS + 8 * g + 4 * half),
-                   d4 = *reinterpret_cast<const float4*>(rows + 2 * ROWS + 8 * g + 4 * half);
-      const float ms[4] = {m4.x, m4.y, m4.z, m4.w}, ls[4] = {l4.x, l4.y, l4.z, l4.w}, ds[4] = {d4.x, d4.y, d4.z, d4.w};
+      const float4 d4 = *reinterpret_cast<const float4*>(rows + 2 * ROWS + 8 * g + 4 * half);
+      dp[4 * g] = d4.x, dp[4 * g + 1] = d4.y, dp[4 * g + 2] = d4.z, dp[4 * g + 3] = d4.w;
+      if constexpr (T::PARTS == 3) {
+        const float4 m4 = *reinterpret_cast<const float4*>(rows + 8 * g + 4 * half);
+        s[4 * g] = m4.x, s[4 * g + 1] = m4.y, s[4 * g + 2] = m4.z, s[4 * g + 3] = m4.w;
+      }
+    }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = 4 * g + i;
-        float x;
-        if (buckets) {
-          const int n = min((int)n_of[j], a.n_buckets);
-          x = fmaf(s[j], scale, table[n]) + kb;
-          if (n == a.n_buckets) x = ninf();
-        } else {
-          x = fmaf(s[j], scale, kb);
-        }
-        s[j] = exp2_(x - ms[i]);
+    for (int i = 0; i < D / 16; ++i) mma<T>(Tl::by_rows(lds_q, i, lane), kf[i], s);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) mma<T>(Tl::by_rows(lds_g, i, lane), vf[i], dp);
+    if (BUFS == 2 && r + 1 < last) write(r + 1);
+    Row next = {};
+    if (r + BUFS < last) fetch(r + BUFS);
+    if (tid < ROWS) next = row_of(r + 2);
+
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float4 l4 = *reinterpret_cast<const float4*>(rows + ROWS + 8 * g + 4 * half);
+      const float ls[4] = {l4.x, l4.y, l4.z, l4.w};
+      float ms[4] = {0.f, 0.f, 0.f, 0.f};
+      if constexpr (T::PARTS == 1) {
+        const float4 m4 = *reinterpret_cast<const float4*>(rows + 8 * g + 4 * half);
+        ms[0] = m4.x, ms[1] = m4.y, ms[2] = m4.z, ms[3] = m4.w;
       }
 #pragma unroll
       for (int i = 0; i < 4; i += 2) {
-        float pr[2] = {s[4 * g + i], s[4 * g + i + 1]};
+        float pr[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int j = 4 * g + i + e;
+          const float t = buckets ? table[min((int)n_of[j], a.n_buckets)] : 0.f;
+          const float x = T::PARTS == 3 ? (buckets ? s[j] + t : s[j]) + kb : ((buckets ? fmaf(s[j], p.c, t) : s[j] * p.c) + kb) + ms[i + e];
+          pr[e] = exp2_(x);
+        }
         round_pair<T>(pr[0], pr[1]);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int j = 4 * g + i + e;
           s[j] = pr[e] * ls[i + e];
-          dp[j] = s[j] * (T::HALF ? fmaf(dp[j], sc.ds, -ds[i + e]) : dp[j] - ds[i + e]);
+          dp[j] = s[j] * (T::HALF ? dp[j] * sc.ds : dp[j]);
         }
       }
     }
@@ -349,7 +404,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, 1) void gr
         mma<T>(Tl::by_entries(lds_qt, i, t, lane), df, dk[i]);
       }
     }
-    if (more && tid < ROWS) put_row(slot ^ 1, next);
+    if (tid < ROWS) put_row(r + 2, next);
   }
 
   if (!ok) return;
@@ -404,7 +459,8 @@ template <class T, int D> void backward_d(Args& p, const Plans& plans, float* pa
   };
   use(plans.grad_q, partial_q);
   const int waves_q = plans.grad_q.waves;
-  const size_t lds_q = 3 * Tile<T, D>::BYTES + (2 * ROWS + MAX_BUCKETS + 4 + (a.gtable ? waves_q * (a.n_buckets + 1) * 64 : 0)) * sizeof(float);
+  const size_t lds_q = buffers<T, D>(3) * 3 * Tile<T, D>::BYTES + (RING * ROWS + MAX_BUCKETS + 4) * sizeof(float) +
+                       (a.gtable ? TableSums::words(a.n_buckets) * sizeof(unsigned long long) : 0);
   if (waves_q == 1) launch(grad_q_kernel<T, D, 1>, p, 1, lds_q, stream);
   else launch(grad_q_kernel<T, D, 4>, p, 4, lds_q, stream);
   if (plans.grad_q.splits > 1) sum_vectors<T>(partial_q, plans.grad_q.splits, D, a.gq, a.gq_stride, a.batch, a.heads, a.n_q, a.d, stream);
@@ -413,7 +469,7 @@ template <class T, int D> void backward_d(Args& p, const Plans& plans, float* pa
                        plans.grad_q.splits * plans.grad_q.tiles, a.n_buckets, static_cast<typename T::type*>(a.gtable));
   if (!a.gk) return;
   use(plans.grad_kv, partial_kv);
-  const size_t lds_kv = 4 * Tile<T, D>::BYTES + (6 * ROWS + (a.buckets ? a.heads / a.kv_heads * (a.n_buckets + 1) : 0)) * sizeof(float);
+  const size_t lds_kv = (2 * 4 * Tile<T, D>::BYTES <= 100 * 1024 ? 2 : 1) * 4 * Tile<T, D>::BYTES + (3 * RING * ROWS + (a.buckets ? a.heads / a.kv_heads * (a.n_buckets + 1) : 0)) * sizeof(float);
   if (plans.grad_kv.waves == 1) launch(grad_kv_kernel<T, D, 1>, p, 1, lds_kv, stream);
   else launch(grad_kv_kernel<T, D, 4>, p, 4, lds_kv, stream);
   if (plans.grad_kv.splits > 1) {

@@ -10,13 +10,12 @@
 namespace s2cnn {
 namespace attn {
 
-template <class T, int D, int W> __global__ __launch_bounds__(64 * W, 2) void forward_kernel(Args p) {
+template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS * D > 192 ? 1 : 2) void forward_kernel(Args p) {
   typedef Tile<T, D> Tl;
+  constexpr int BUFS = buffers<T, D>(2), BUF = 2 * Tl::BYTES;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  unsigned char* const lds_k = smem;
-  unsigned char* const lds_v = smem + Tl::BYTES;
-  float* const lds_kb = reinterpret_cast<float*>(smem + 2 * Tl::BYTES);       // [2][ROWS]
-  float* const lds_table = lds_kb + 2 * ROWS;
+  float* const lds_kb = reinterpret_cast<float*>(smem + BUFS * BUF);          // [RING][ROWS]
+  float* const lds_table = lds_kb + RING * ROWS;
   const s2cnn_attention_t& a = p.a;
 
   const int work = work_of_block(p.workgroups);
@@ -43,6 +42,8 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, 2) void fo
   const float* const key_bias = a.key_bias ? a.key_bias + b * a.key_bias_stride : nullptr;
   const signed char* const buckets = a.buckets ? a.buckets + b * a.bucket_stride[0] + query * a.bucket_stride[1] : nullptr;
   const float* const table = lds_table + (head - head0) * (a.n_buckets + 1);
+  const bool measure = a.stats && tile == 0;                // this workgroup finds the largest |v| of its keys for the backward pass
+  const float dead = ninf() * p.inv_c;
 
   Stage<T, D, 64 * W> stage;
   unsigned words[4] = {0, 0, 0, 0};
@@ -50,54 +51,69 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, 2) void fo
     stage.fetch(k, v, key0, tid);
     if (buckets) load_buckets(buckets, key0, end, half, words);
   }
-  if (tid < ROWS) lds_kb[tid] = key_value(key_bias, key0 + tid, end);
+  if (tid < 2 * ROWS) lds_kb[tid] = key_value(key_bias, key0 + tid, end, p.inv_c);
   if (buckets) stage_table<T>(lds_table, a.table, a.n_buckets, head0, heads, tid, 64 * W);
   Frag<T> qf[D / 16];
-  load_column<T, D>(static_cast<const E*>(a.q) + b * a.q_stride[0] + head * a.q_stride[1] + query * a.q_stride[2], a.d, (p.wide & WIDE_Q) != 0, ok, half, qf);
+  load_column<T, D>(static_cast<const E*>(a.q) + b * a.q_stride[0] + head * a.q_stride[1] + query * a.q_stride[2], a.d, (p.wide & WIDE_Q) != 0, ok, half,
+                    a.scale * LOG2E, qf);
+  float largest = 0.f;
+  const auto write = [&](int step) {
+    unsigned char* const to = smem + step % BUFS * BUF;
+    const float* const kb = lds_kb + step % RING * ROWS;
+    stage.write(to, nullptr, nullptr, to + Tl::BYTES, tid, a.d, [&](int r) { return kb[r] != dead; });
+    if (measure) largest = fmaxf(largest, stage.largest_second(tid));
+  };
+  if (BUFS == 2) {
+    __syncthreads();
+    if (key0 < end) write(0);
+    if (key0 + ROWS < end) stage.fetch(k, v, key0 + ROWS, tid);
+  }
 
   constexpr float SHIFT = T::HALF ? 10.f : 0.f;       // probabilities times 2^10 in float16: its smallest normal number is 2^-14
-  const float scale = a.scale * LOG2E;
   float m = ninf(), l = 0.f;
   v16f o[D / 32] = {};
-  int slot = 0;
-  for (int key = key0; key < end; key += ROWS, slot ^= 1) {
-    const float* const kb = lds_kb + slot * ROWS;
+  int step = 0;
+  for (int key = key0; key < end; key += ROWS, ++step) {
+    const bool more = key + ROWS < end;
     __syncthreads();
-    stage.write(lds_k, nullptr, nullptr, lds_v, tid, [&](int r) { return kb[r] != ninf(); });
-    __syncthreads();
+    if (BUFS == 1) {
+      write(step);
+      __syncthreads();
+    }
+    const unsigned char* const lds_k = smem + step % BUFS * BUF;
+    const unsigned char* const lds_v = lds_k + Tl::BYTES;
+    const float* const kb = lds_kb + step % RING * ROWS;
+
+    v16f s;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float4 kb4 = *reinterpret_cast<const float4*>(kb + 8 * g + 4 * half);
+      s[4 * g] = kb4.x, s[4 * g + 1] = kb4.y, s[4 * g + 2] = kb4.z, s[4 * g + 3] = kb4.w;
+    }
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) mma<T>(Tl::by_rows(lds_k, i, lane), qf[i], s);
+    if (BUFS == 2 && more) write(step + 1);
     unsigned now[4];
 #pragma unroll
     for (int g = 0; g < 4; ++g) now[g] = words[g];
     float kb_next = 0.f;
-    const bool more = key + ROWS < end;
-    if (more) {
-      stage.fetch(k, v, key + ROWS, tid);
-      if (buckets) load_buckets(buckets, key + ROWS, end, half, words);
-      if (tid < ROWS) kb_next = key_value(key_bias, key + ROWS + tid, end);
-    }
+    if (key + BUFS * ROWS < end) stage.fetch(k, v, key + BUFS * ROWS, tid);
+    if (more && buckets) load_buckets(buckets, key + ROWS, end, half, words);
+    if (tid < ROWS) kb_next = key_value(key_bias, key + 2 * ROWS + tid, end, p.inv_c);
 
-    v16f s = {};
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) mma<T>(Tl::by_rows(lds_k, i, lane), qf[i], s);
     float top = ninf();
+    if (buckets) {
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const float4 kb4 = *reinterpret_cast<const float4*>(kb + 8 * g + 4 * half);
-      const float kbs[4] = {kb4.x, kb4.y, kb4.z, kb4.w};
-      if (buckets) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int n = bucket_of(now[g], i, a.n_buckets);
-          const float x = fmaf(s[4 * g + i], scale, table[n]) + kbs[i];
-          s[4 * g + i] = n == a.n_buckets ? ninf() : x;
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[4 * g + i] = fmaf(s[4 * g + i], scale, kbs[i]);
+      for (int r = 0; r < 16; ++r) {
+        const float t = table[bucket_of(now[r / 4], r % 4, a.n_buckets)];
+        s[r] = T::PARTS == 3 ? s[r] + t : fmaf(s[r], p.c, t);
       }
+    } else if (T::PARTS == 1) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) top = fmaxf(top, s[4 * g + i]);
+      for (int r = 0; r < 16; ++r) s[r] *= p.c;
     }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
     top = ceilf(fmaxf(half_max(top), m));
     const float ref = (top == ninf() ? 0.f : top) - SHIFT;
     if (__any(top > m)) {
@@ -126,14 +142,22 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, 2) void fo
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) mma<T>(Tl::by_entries(lds_v, i, t, lane), pf, o[i]);
     }
-    if (more && tid < ROWS) lds_kb[(slot ^ 1) * ROWS + tid] = kb_next;
+    if (tid < ROWS) lds_kb[(step + 2) % RING * ROWS + tid] = kb_next;
   }
 
+  const long row = ((long)b * a.heads + head) * a.n_q + query, rows = (long)a.batch * a.heads * a.n_q;
+  if (measure) {
+#pragma unroll
+    for (int i = 32; i; i >>= 1) largest = fmaxf(largest, __shfl_xor(largest, i));
+    __syncthreads();
+    if (lane == 0) lds_kb[tid >> 6] = largest;
+    __syncthreads();
+    for (int i = 0; i < W; ++i) largest = fmaxf(largest, lds_kb[i]);
+    if (tid == 0) a.stats[2 * rows + bh * p.splits + split] = largest;
+  }
   l = half_sum(l);
   if (!ok) return;
-  const long row = ((long)b * a.heads + head) * a.n_q + query;
   if (p.splits > 1) {
-    const long rows = (long)a.batch * a.heads * a.n_q;
     float* const part = p.partial;
     store_partial<D>(part + (split * rows + row) * D, half, o);
     if (half == 0) reinterpret_cast<float2*>(part + p.splits * rows * D)[split * rows + row] = make_float2(m, l);
@@ -142,8 +166,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, 2) void fo
   // a row without keys: zeros, and statistics by which every probability is zero
   const bool any = l != 0.f;
   const float inv = any ? 1.f / l : 0.f;
-  const long at = b * a.out_stride[0] + head * a.out_stride[1] + query * a.out_stride[2];
-  store_column<T, D>(static_cast<E*>(a.out) + at, a.d, (p.wide & WIDE_OUT) != 0, half, o, inv);
+  store_column<T, D>(static_cast<E*>(a.out) + b * a.out_stride[0] + head * a.out_stride[1] + query * a.out_stride[2], a.d, (p.wide & WIDE_OUT) != 0, half, o, inv);
   if (T::PARTS == 1 && a.out_f32) store_column<F32, D>(a.out_f32 + row * a.d, a.d, a.d % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out_f32) & 15) == 0, half, o, inv);
   if (half == 0 && a.stats) reinterpret_cast<float2*>(a.stats)[row] = any ? make_float2(m - SHIFT, inv) : make_float2(pinf(), 0.f);
 }
@@ -187,7 +210,7 @@ template <class T, int D> void forward_d(const Args& p, const Plans& plans, hipS
   const s2cnn_attention_t& a = p.a;
   const Plan& f = plans.fwd;
   const int heads = min(a.heads / a.kv_heads, (32 * f.waves - 1) / a.n_q + 2);
-  const size_t lds = 2 * Tile<T, D>::BYTES + (2 * ROWS + (a.buckets ? heads * (a.n_buckets + 1) : 0)) * sizeof(float);
+  const size_t lds = buffers<T, D>(2) * 2 * Tile<T, D>::BYTES + (RING * ROWS + (a.buckets ? heads * (a.n_buckets + 1) : 0)) * sizeof(float);
   if (f.waves == 1) launch(forward_kernel<T, D, 1>, p, 1, lds, stream);
   else launch(forward_kernel<T, D, 4>, p, 4, lds, stream);
   if (f.splits > 1)
