@@ -439,12 +439,12 @@ typedef struct s2cnn_attention_t {
   long q_stride[3], k_stride[3], v_stride[3], out_stride[3], gout_stride[3], gq_stride[3], gk_stride[3], gv_stride[3];
   long bucket_stride[2];       /* of batch (0: shared) and query, in bytes                 */
   long key_bias_stride;        /* of batch (0: shared), in entries                         */
-  int batch, heads, kv_heads, n_q, n_k, d;      /* n_q >= 1; n_k >= 0 (bwd: >= 1); 1 <= d <= 128 */
+  int batch, heads, kv_heads, n_q, n_k, d;      /* n_q >= 1; n_k >= 0 (bwd: >= 1); 4 <= d <= 128 */
   int n_buckets, dtype;
   float scale;
 } s2cnn_attention_t;
 
-#define S2CNN_ATTENTION_STRIDE_LIMIT (1L << 26)   /* strides of vectors of q, k, v, gout are below this */
+#define S2CNN_ATTENTION_STRIDE_LIMIT (1L << 26)   /* strides of vectors of q, k, v, gout and of rows of buckets are below this */
 size_t s2cnn_attention_stats_floats(const s2cnn_attention_t *a);
 size_t s2cnn_attention_workspace(const s2cnn_attention_t *a, int backward);     /* 0 also for sizes that are refused */
 int s2cnn_attention_fwd(const s2cnn_attention_t *a, void *workspace, size_t workspace_bytes, void *stream);

@@ -142,16 +142,20 @@ def attention(q, k, v, table=None, buckets=None, key_bias=None, lengths=None, sc
     _hip.require_gpu_of(torch.float32, key_bias)
     _hip.require_gpu_of(torch.int32, lengths)
     assert key_bias is None or not key_bias.requires_grad, "key_bias is not differentiated"
+    d = q.size(3)
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    if d < 4:                                            # the kernels read four entries at a time
+        q, k, v = (torch.nn.functional.pad(t, (0, 4 - d)) for t in (q, k, v))
     if table is not None:
         table = table.contiguous()
-        buckets = _unit_last(buckets)
+        buckets = buckets if buckets.stride(-1) == 1 and buckets.stride(-2) < 1 << 26 else buckets.contiguous()
     if key_bias is not None:
         key_bias = _unit_last(key_bias)
     if lengths is not None:
         lengths = lengths.contiguous()
-    scale = 1.0 / math.sqrt(q.size(3)) if scale is None else float(scale)
     needs_grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, table))
-    return _Attention.apply(q, k, v, table, buckets, key_bias, lengths, scale, dtype, needs_grad)
+    out = _Attention.apply(q, k, v, table, buckets, key_bias, lengths, scale, dtype, needs_grad)
+    return out[..., :d] if d < 4 else out
 
 
 def s2_angle_buckets(points_q, points_k=None, n_buckets=32, max_angle=math.pi, device=None):

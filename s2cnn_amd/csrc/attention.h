@@ -43,6 +43,19 @@ __device__ __forceinline__ float half_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// LDS accesses of 16 and 8 bytes, free of the types that the bytes are written and read as: where a workgroup is one wave, its
+// barriers order nothing for the compiler, and accesses of different types may then be exchanged.
+__device__ __forceinline__ uint4 read16(const unsigned char* p) {
+  uint4 v;
+  __builtin_memcpy(&v, __builtin_assume_aligned(p, 16), 16);
+  return v;
+}
+__device__ __forceinline__ void read16(const float* p, float (&x)[4]) { __builtin_memcpy(x, __builtin_assume_aligned(p, 16), 16); }
+__device__ __forceinline__ void write8(unsigned char* p, unsigned a, unsigned b) {
+  const uint2 v = make_uint2(a, b);
+  __builtin_memcpy(__builtin_assume_aligned(p, 8), &v, 8);
+}
+
 // ---- operands -------------------------------------------------------------------------------------------------------
 template <class T> struct Frag { uint4 part[T::PARTS]; };
 
@@ -101,39 +114,43 @@ template <class T> __device__ __forceinline__ Frag<T> cut_rows(const v16f& s, in
 }
 
 // ---- vectors in memory ----------------------------------------------------------------------------------------------
-// The vectors of one (batch, head): vector i starts at base + i stride and has d entries.  wide: aligned for loads of four
-// entries, d a multiple of four.
+// The vectors of one (batch, head): vector i starts at base + i stride, at any entry, and has d entries.
 template <class T> struct Vectors {
   const typename T::type* base;
   long stride;
   int n, d;
-  bool wide;
 };
 
 struct Quad { uint4 w; };            // four entries as they are in memory: floats, or 16-bit values in x and y
 
-// entries 4 q .. 4 q + 3 of the vector at `p`, zero from d on
-template <class T> __device__ __forceinline__ Quad load_quad(const typename T::type* p, int q, int d, bool wide) {
+// A vector of d >= 4 entries is read, multiplied and written in quads: quad q holds entries 4 q .. 4 q + 3, the last one of a d
+// that is no multiple of four the entries d - 4 .. d - 1, so that every access is one of four entries inside the vector.  Quads
+// from d on hold any entries of it.  Columns have zeros for what is there twice or not at all (load_quad), so that it adds nothing to
+// the products over the entries; in the products over the rows it makes entries that are written twice, or not.
+// Vectors need no alignment: the memory pipeline takes any.
+__device__ __forceinline__ int quad_at(int q, int d) { return 4 * q < d ? min(4 * q, d - 4) : 0; }
+__device__ __forceinline__ int slot_of(int entry, int d) { return entry < (d & ~3) ? entry : entry + 4 - (d & 3); }    // where the quads hold it
+template <class T> __device__ __forceinline__ Quad load_four(const typename T::type* p) {
   Quad v;
-  if (wide) {
-    const int at = 4 * q < d ? 4 * q : 0;
-    if constexpr (T::PARTS == 3) v.w = *reinterpret_cast<const uint4*>(p + at);
-    else {
-      const uint2 u = *reinterpret_cast<const uint2*>(p + at);
-      v.w = make_uint4(u.x, u.y, 0, 0);
-    }
-    if (4 * q >= d) v.w = make_uint4(0, 0, 0, 0);
+  if constexpr (T::PARTS == 3) __builtin_memcpy(&v.w, p, 16);
+  else {
+    uint2 u;
+    __builtin_memcpy(&u, p, 8);
+    v.w = make_uint4(u.x, u.y, 0, 0);
+  }
+  return v;
+}
+template <class T> __device__ __forceinline__ Quad load_quad(const typename T::type* p, int q, int d) {
+  Quad v = load_four<T>(p + quad_at(q, d));
+  const int twice = 4 * q < d ? 4 * q - quad_at(q, d) : 4;        // so many of its first entries
+  if constexpr (T::PARTS == 3) {
+    if (twice > 0) v.w.x = 0;
+    if (twice > 1) v.w.y = 0;
+    if (twice > 2) v.w.z = 0;
+    if (twice > 3) v.w.w = 0;
   } else {
-    unsigned e[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int at = 4 * q + i;
-      if constexpr (T::PARTS == 3) e[i] = reinterpret_cast<const unsigned*>(p)[at < d ? at : 0];
-      else e[i] = reinterpret_cast<const unsigned short*>(p)[at < d ? at : 0];
-      if (at >= d) e[i] = 0;
-    }
-    if constexpr (T::PARTS == 3) v.w = make_uint4(e[0], e[1], e[2], e[3]);
-    else v.w = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, 0, 0);
+    v.w.x &= twice > 1 ? 0 : twice > 0 ? 0xffff0000u : ~0u;
+    v.w.y &= twice > 3 ? 0 : twice > 2 ? 0xffff0000u : ~0u;
   }
   return v;
 }
@@ -154,30 +171,26 @@ template <class T> __device__ __forceinline__ void quad_values(const Quad& v, fl
     x[0] = a[0], x[1] = a[1], x[2] = b[0], x[3] = b[1];
   }
 }
-template <class T> __device__ __forceinline__ void store_quad(typename T::type* p, int at, int d, bool wide, float a, float b, float c, float e) {
-  if (at >= d) return;
-  if (wide) {
-    if constexpr (T::PARTS == 3) *reinterpret_cast<float4*>(p + at) = make_float4(a, b, c, e);
-    else {
-      unsigned u[1], v[1];
-      cut<T>(a, b, u), cut<T>(c, e, v);
-      *reinterpret_cast<uint2*>(p + at) = make_uint2(u[0], v[0]);
-    }
-    return;
+template <class T> __device__ __forceinline__ void store_quad(typename T::type* p, int q, int d, float a, float b, float c, float e) {
+  if (4 * q >= d) return;
+  if constexpr (T::PARTS == 3) {
+    const float4 x = make_float4(a, b, c, e);
+    __builtin_memcpy(p + quad_at(q, d), &x, 16);
+  } else {
+    unsigned u[1], v[1];
+    cut<T>(a, b, u), cut<T>(c, e, v);
+    const uint2 x = make_uint2(u[0], v[0]);
+    __builtin_memcpy(p + quad_at(q, d), &x, 8);
   }
-  const float x[4] = {a, b, c, e};
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (at + i < d) p[at + i] = (typename T::type)x[i];
 }
 
 // The B operands of one column: the vector at `p` (float32: times `factor`), in steps of 16 entries, 8 of them in either half of
 // the wave.
 template <class T, int D>
-__device__ __forceinline__ void load_column(const typename T::type* p, int d, bool wide, bool ok, int half, float factor, Frag<T> (&f)[D / 16]) {
+__device__ __forceinline__ void load_column(const typename T::type* p, int d, bool ok, int half, float factor, Frag<T> (&f)[D / 16]) {
 #pragma unroll
   for (int s = 0; s < D / 16; ++s) {
-    Quad a = load_quad<T>(p, 4 * s + 2 * half, d, wide), b = load_quad<T>(p, 4 * s + 2 * half + 1, d, wide);
+    Quad a = load_quad<T>(p, 4 * s + 2 * half, d), b = load_quad<T>(p, 4 * s + 2 * half + 1, d);
     if (!ok) a.w = b.w = make_uint4(0, 0, 0, 0);
     if constexpr (T::PARTS == 3) {
       float x[8];
@@ -193,12 +206,12 @@ __device__ __forceinline__ void load_column(const typename T::type* p, int d, bo
 }
 
 // acc[b][4 g + i] is entry 32 b + 8 g + 4 half + i of the lane's column
-template <class T, int D> __device__ __forceinline__ void store_column(typename T::type* p, int d, bool wide, int half, const v16f (&acc)[D / 32], float factor) {
+template <class T, int D> __device__ __forceinline__ void store_column(typename T::type* p, int d, int half, const v16f (&acc)[D / 32], float factor) {
 #pragma unroll
   for (int b = 0; b < D / 32; ++b)
 #pragma unroll
     for (int g = 0; g < 4; ++g)
-      store_quad<T>(p, 32 * b + 8 * g + 4 * half, d, wide, acc[b][4 * g] * factor, acc[b][4 * g + 1] * factor, acc[b][4 * g + 2] * factor,
+      store_quad<T>(p, 8 * b + 2 * g + half, d, acc[b][4 * g] * factor, acc[b][4 * g + 1] * factor, acc[b][4 * g + 2] * factor,
                     acc[b][4 * g + 3] * factor);
 }
 // the same into an array of partial sums, D floats a column
@@ -216,6 +229,7 @@ template <int D> __device__ __forceinline__ void store_partial(float* p, int hal
 //   by entries: block b of 32 entries, step t of the product over the rows; lane (h, m) reads entry 32 b + m of the rows above
 // A thread of the staging holds a block of 4 rows x 4 entries, and writes 8 bytes per row or entry.  The 16-byte slots are
 // permuted (by s and h, or by m / 8) so that these writes go to all banks; readers permute within 128 bytes and lose nothing.
+enum Layouts { BY_ROWS = 1, BY_ENTRIES = 2, BOTH = 3 };
 template <class T, int D> struct Tile {
   static constexpr int STEPS = D / 16;                             // as many KB per part in either layout
   static constexpr int BYTES = T::PARTS * STEPS * 1024;
@@ -228,34 +242,34 @@ template <class T, int D> struct Tile {
     Frag<T> f;
     const int at = row_slot(s, lane >> 5, lane & 31);
 #pragma unroll
-    for (int p = 0; p < T::PARTS; ++p) f.part[p] = *reinterpret_cast<const uint4*>(lds + ((p * STEPS + s) * 64 + at) * 16);
+    for (int p = 0; p < T::PARTS; ++p) f.part[p] = read16(lds + ((p * STEPS + s) * 64 + at) * 16);
     return f;
   }
   static __device__ __forceinline__ Frag<T> by_entries(const unsigned char* lds, int b, int t, int lane) {
     Frag<T> f;
     const int at = entry_slot(lane >> 5, lane & 31);
 #pragma unroll
-    for (int p = 0; p < T::PARTS; ++p) f.part[p] = *reinterpret_cast<const uint4*>(lds + ((p * STEPS + 2 * b + t) * 64 + at) * 16);
+    for (int p = 0; p < T::PARTS; ++p) f.part[p] = read16(lds + ((p * STEPS + 2 * b + t) * 64 + at) * 16);
     return f;
   }
 
-  // block k of the tile: rows 4 (k / (D / 4)), entries 4 (k % (D / 4))
-  static __device__ __forceinline__ void write(unsigned char* rows, unsigned char* entries, int k, const Quad (&v)[4]) {
+  // block k of the tile: rows 4 (k / (D / 4)), entries 4 (k % (D / 4)); LAYOUTS: which of the two
+  template <int LAYOUTS> static __device__ __forceinline__ void write(unsigned char* rows, unsigned char* entries, int k, const Quad (&v)[4]) {
     const int q = k % (D / 4), kg = k / (D / 4);
     unsigned w[4][2][T::PARTS];                                    // [row][pair of entries][part]
 #pragma unroll
     for (int i = 0; i < 4; ++i) quad_parts<T>(v[i], w[i][0], w[i][1]);
-    if (rows) {
+    if constexpr ((LAYOUTS & BY_ROWS) != 0) {
       const int s = q >> 2, h = (q >> 1) & 1;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int at = row_slot(s, h, 4 * kg + i);
 #pragma unroll
         for (int p = 0; p < T::PARTS; ++p)
-          *reinterpret_cast<uint2*>(rows + ((p * STEPS + s) * 64 + at) * 16 + (q & 1) * 8) = make_uint2(w[i][0][p], w[i][1][p]);
+          write8(rows + ((p * STEPS + s) * 64 + at) * 16 + (q & 1) * 8, w[i][0][p], w[i][1][p]);
       }
     }
-    if (entries) {
+    if constexpr ((LAYOUTS & BY_ENTRIES) != 0) {
       const int b = q >> 3, t = kg >> 2, half = (kg >> 1) & 1, h = kg & 1;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -263,23 +277,27 @@ template <class T, int D> struct Tile {
         const unsigned sel = (j & 1) ? 0x07060302u : 0x05040100u;  // the entry's 16 bits of two rows
 #pragma unroll
         for (int p = 0; p < T::PARTS; ++p)
-          *reinterpret_cast<uint2*>(entries + ((p * STEPS + 2 * b + t) * 64 + at) * 16 + half * 8) =
-              make_uint2(__builtin_amdgcn_perm(w[1][j >> 1][p], w[0][j >> 1][p], sel), __builtin_amdgcn_perm(w[3][j >> 1][p], w[2][j >> 1][p], sel));
+          write8(entries + ((p * STEPS + 2 * b + t) * 64 + at) * 16 + half * 8, __builtin_amdgcn_perm(w[1][j >> 1][p], w[0][j >> 1][p], sel),
+                 __builtin_amdgcn_perm(w[3][j >> 1][p], w[2][j >> 1][p], sel));
       }
     }
   }
 };
 
-// LDS of a kernel that stages `layouts` layouts of a tile: two tiles where they fit beside a second workgroup (of half the wave
-// slots), so that a tile is written while the one before is used, with one barrier per tile; else one.
-template <class T, int D> constexpr int buffers(int layouts) { return 2 * layouts * Tile<T, D>::BYTES <= 80 * 1024 ? 2 : 1; }
+// LDS of a kernel that stages `layouts` layouts of a tile: two tiles where they fit beside a second workgroup, so that a tile is
+// written while the one before is used, with one barrier per tile; else one.  One, too, where the workgroup is a wave: it fetches
+// a tile and writes it at once (a thread has up to eight blocks then, too many registers to hold beside the operands), and the
+// other waves of the CU are what hides the wait.
+template <class T, int D, int W> constexpr int buffers(int layouts) { return W > 1 && 2 * layouts * Tile<T, D>::BYTES <= 80 * 1024 ? 2 : 1; }
 
-// Two tensors staged by the same tiles of rows: THREADS threads fetch the blocks of a tile into registers, and write them later.
+// Two tensors staged by the same tiles of rows, in the layouts LA and LB (those of the first, then those of the second): THREADS threads
+// fetch the blocks of a tile into registers, and write them later.
 // The address of a block's rows is a uniform pointer, moved on by the tile, and an offset of the thread that stays (below
 // 2^31 bytes: the entry checks 32 strides).
-template <class T, int D, int THREADS> struct Stage {
+template <class T, int D, int THREADS, int LA, int LB> struct Stage {
   typedef Tile<T, D> Tl;
   typedef typename T::type E;
+  static constexpr int A = LA == BOTH ? 2 * Tl::BYTES : Tl::BYTES;      // where the second tensor's layouts begin
   static constexpr int PER = (2 * Tl::BLOCKS + THREADS - 1) / THREADS;
   static constexpr bool IDLE = 2 * Tl::BLOCKS % THREADS != 0;      // some threads have no block
   Quad v[PER][4];
@@ -292,50 +310,52 @@ template <class T, int D, int THREADS> struct Stage {
   static __device__ __forceinline__ bool idle(int u, int tid) { return IDLE && __builtin_amdgcn_readfirstlane(u * THREADS + tid) >= 2 * Tl::BLOCKS; }
   static __device__ __forceinline__ int block(int u, int tid) { return (u * THREADS + tid) % Tl::BLOCKS; }
 
-  __device__ __forceinline__ void fetch(const Vectors<T>& a, const Vectors<T>& b, int row0, int tid) {
+  // blocks [U0, U1) of the thread
+  template <int U0 = 0, int U1 = PER> __device__ __forceinline__ void fetch(const Vectors<T>& a, const Vectors<T>& b, int row0, int tid) {
 #pragma unroll
-    for (int u = 0; u < PER; ++u) {
+    for (int u = U0; u < U1; ++u) {
       if (idle(u, tid)) break;
       const Vectors<T>& x = second(u, tid) ? b : a;
       const int kk = block(u, tid), q = kk % (D / 4), row = 4 * (kk / (D / 4));
       const E* const base = x.base + (long)row0 * x.stride;
-      const int stride = (int)x.stride, left = x.n - 1 - row0;     // last row of the tile that exists
-      if (x.wide && left >= ROWS - 1) {
-        const int at = row * stride + (4 * q < x.d ? 4 * q : 0);
+      const int stride = (int)x.stride, left = x.n - 1 - row0, at = quad_at(q, x.d);     // left: last row of the tile that exists
+      if (left >= ROWS - 1) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const E* const p = base + i * x.stride + (unsigned)at;
-          if constexpr (T::PARTS == 3) v[u][i].w = *reinterpret_cast<const uint4*>(p);
-          else {
-            const uint2 w = *reinterpret_cast<const uint2*>(p);
-            v[u][i].w = make_uint4(w.x, w.y, 0, 0);
-          }
-        }
+        for (int i = 0; i < 4; ++i) v[u][i] = load_four<T>(base + i * x.stride + (unsigned)(row * stride + at));
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[u][i] = load_quad<T>(base + (long)min(row + i, left) * x.stride, q, x.d, x.wide);
+        for (int i = 0; i < 4; ++i) v[u][i] = load_four<T>(base + (unsigned)(min(row + i, left) * stride + at));
       }
     }
   }
   // keep(row of the tile): false for rows that count as zero, whatever their memory holds
-  template <class Keep>
-  __device__ __forceinline__ void write(unsigned char* a_rows, unsigned char* a_entries, unsigned char* b_rows, unsigned char* b_entries, int tid, int d, Keep keep) {
+  template <int U0 = 0, int U1 = PER, class Keep>
+  __device__ __forceinline__ void write(unsigned char* to, int tid, Keep keep) {
 #pragma unroll
-    for (int u = 0; u < PER; ++u) {
+    for (int u = U0; u < U1; ++u) {
       if (idle(u, tid)) break;
       const int kk = block(u, tid), row = 4 * (kk / (D / 4));
-      const bool column = 4 * (kk % (D / 4)) < d;
       bool k[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) k[i] = keep(row + i) && column;
+      for (int i = 0; i < 4; ++i) k[i] = keep(row + i);
       if (!__all(k[0] && k[1] && k[2] && k[3])) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (!k[i]) v[u][i].w = make_uint4(0, 0, 0, 0);
       }
-      if (second(u, tid)) Tl::write(b_rows, b_entries, kk, v[u]);
-      else Tl::write(a_rows, a_entries, kk, v[u]);
+      if (second(u, tid)) Tl::template write<LB>(to + A, to + A + (LB == BOTH ? Tl::BYTES : 0), kk, v[u]);
+      else Tl::template write<LA>(to, to + (LA == BOTH ? Tl::BYTES : 0), kk, v[u]);
     }
+  }
+  // a wave's own way: fetch and write, one tensor after the other, so that half the registers do
+  template <class Keep>
+  __device__ __forceinline__ void fetch_and_write(const Vectors<T>& a, const Vectors<T>& b, int row0, unsigned char* to, int tid, Keep keep) {
+    static_assert(THREADS == 64, "one wave");
+    fetch<0, PER / 2>(a, b, row0, tid);
+    write<0, PER / 2>(to, tid, keep);
+    __builtin_amdgcn_sched_barrier(0);
+    fetch<PER / 2, PER>(a, b, row0, tid);
+    write<PER / 2, PER>(to, tid, keep);
   }
   // the largest |entry| of the second tensor's blocks, as they were written
   __device__ __forceinline__ float largest_second(int tid) const {
@@ -407,12 +427,10 @@ __device__ __forceinline__ int bucket_of(unsigned w, int i, int n_buckets) { ret
 
 // ---- arguments ------------------------------------------------------------------------------------------------------
 // The header's struct and what the entry has made of it.
-enum Wide { WIDE_Q = 1, WIDE_K = 2, WIDE_V = 4, WIDE_OUT = 8, WIDE_GOUT = 16, WIDE_GQ = 32, WIDE_GK = 64, WIDE_GV = 128 };
 struct Args {
   s2cnn_attention_t a;
   float c, inv_c;          // log2(e) scale and its inverse
   int forward_splits;
-  int wide;                // tensors whose vectors can be read and written four entries at a time
   int splits;              // parts of the long axis (keys; queries in the kernel of dk and dv)
   int tiles;               // workgroups along the columns
   int workgroups;
@@ -430,6 +448,10 @@ inline unsigned blocks_for(int workgroups) { return (unsigned)((workgroups + 7) 
 
 
 // ---- launches -------------------------------------------------------------------------------------------------------
+// Whether there are workgroups of one wave.  Not for float32 heads of more than 64 entries: a wave's operands and a thread's share of a tile
+// are more than its registers then.
+template <class T, int D> constexpr bool few_waves = T::PARTS * D <= 256;
+
 // How a kernel's work is laid out: waves per workgroup, workgroups along the columns, parts of the long axis.
 struct Plan { int waves, tiles, splits; long workgroups; };
 struct Plans { int D; Plan fwd, grad_q, grad_kv; };

@@ -16,9 +16,9 @@ constexpr int CUS = 256;
 
 // Columns of one group of heads, groups, and tiles of the long axis.  A workgroup of one wave where one wave holds all columns.
 // The long axis is cut while compute units would have no workgroup, into parts of at least four tiles.
-Plan plan(long columns, long groups, long long_tiles) {
+Plan plan(long columns, long groups, long long_tiles, bool few) {
   Plan p;
-  p.waves = columns <= 32 ? 1 : 4;
+  p.waves = few && columns <= 32 ? 1 : 4;
   p.tiles = columns < 1 ? 1 : (int)((columns + 32 * p.waves - 1) / (32 * p.waves));
   const long base = p.tiles * groups, want = p.waves == 1 ? 4 * CUS : 2 * CUS;
   long splits = base >= want / 2 ? 1 : (want + base - 1) / base;
@@ -34,9 +34,10 @@ Plans plans_of(const s2cnn_attention_t& a) {
   Plans p;
   p.D = a.d <= 32 ? 32 : a.d <= 64 ? 64 : 128;
   const long group = a.heads / a.kv_heads;
-  p.fwd = plan(group * a.n_q, (long)a.batch * a.kv_heads, tiles_of(a.n_k));
-  p.grad_q = plan(a.n_q, (long)a.batch * a.heads, tiles_of(a.n_k));
-  p.grad_kv = plan(a.n_k, (long)a.batch * a.kv_heads, group * tiles_of(a.n_q));
+  const bool few = a.dtype != S2CNN_F32 || p.D <= 64;       // few_waves
+  p.fwd = plan(group * a.n_q, (long)a.batch * a.kv_heads, tiles_of(a.n_k), few);
+  p.grad_q = plan(a.n_q, (long)a.batch * a.heads, tiles_of(a.n_k), few);
+  p.grad_kv = plan(a.n_k, (long)a.batch * a.kv_heads, group * tiles_of(a.n_q), few);
   return p;
 }
 
@@ -45,9 +46,10 @@ long stats_floats(const s2cnn_attention_t& a, const Plans& p) { return 2L * a.ba
 bool sizes_ok(const s2cnn_attention_t* a) {
   if (!a) return false;
   if (a->dtype != S2CNN_F32 && a->dtype != S2CNN_BF16 && a->dtype != S2CNN_F16) return false;
-  if (a->batch < 1 || a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads || a->n_q < 1 || a->n_k < 0 || a->d < 1 || a->d > 128) return false;
+  if (a->batch < 1 || a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads || a->n_q < 1 || a->n_k < 0 || a->d < 4 || a->d > 128) return false;
   const bool bias = a->buckets || a->table || a->n_buckets;
   if (bias && (!a->buckets || !a->table || a->n_buckets < 1 || a->n_buckets > MAX_BUCKETS || a->heads / a->kv_heads > 128)) return false;
+  if (a->buckets && (a->bucket_stride[1] < 0 || a->bucket_stride[1] >= S2CNN_ATTENTION_STRIDE_LIMIT)) return false;
   const long limit = 1L << 30;
   if ((long)a->heads / a->kv_heads * a->n_q > limit || a->n_k > limit || (long)a->batch * a->heads > limit) return false;
   for (const long* s : {a->q_stride, a->k_stride, a->v_stride, a->gout_stride})
@@ -74,19 +76,9 @@ Backward backward_layout(const s2cnn_attention_t& a, const Plans& p) {
   return w;
 }
 
-int wide(const s2cnn_attention_t& a) {
-  const int size = a.dtype == S2CNN_F32 ? 4 : 2;
-  const auto one = [&](const void* p, const long* s, int bit) {
-    return a.d % 4 == 0 && s[0] % 4 == 0 && s[1] % 4 == 0 && s[2] % 4 == 0 && reinterpret_cast<uintptr_t>(p) % (4 * size) == 0 ? bit : 0;
-  };
-  return one(a.q, a.q_stride, WIDE_Q) | one(a.k, a.k_stride, WIDE_K) | one(a.v, a.v_stride, WIDE_V) | one(a.out, a.out_stride, WIDE_OUT) |
-         one(a.gout, a.gout_stride, WIDE_GOUT) | one(a.gq, a.gq_stride, WIDE_GQ) | one(a.gk, a.gk_stride, WIDE_GK) | one(a.gv, a.gv_stride, WIDE_GV);
-}
-
 Args args_of(const s2cnn_attention_t& a, const Plans& plans) {
   Args p{};
   p.a = a;
-  p.wide = wide(a);
   p.forward_splits = plans.fwd.splits;
   // float32 takes the factor into its columns; the others into the scores, and its inverse into the biases: never zero
   const float c = a.dtype == S2CNN_F32 ? 1.f : a.scale * LOG2E;

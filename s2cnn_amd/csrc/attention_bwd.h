@@ -45,7 +45,7 @@ struct TableSums {
 
 template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS * D > 128 ? 1 : 2) void grad_q_kernel(Args p) {
   typedef Tile<T, D> Tl;
-  constexpr int BUFS = buffers<T, D>(3), BUF = 3 * Tl::BYTES;
+  constexpr int BUFS = buffers<T, D, W>(3), BUF = 3 * Tl::BYTES;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   float* const lds_kb = reinterpret_cast<float*>(smem + BUFS * BUF);          // [RING][ROWS]
   float* const lds_table = lds_kb + RING * ROWS;                              // [MAX_BUCKETS + 4]
@@ -69,18 +69,18 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
   end = min(end, key0 + chunk);
 
   typedef typename T::type E;
-  const Vectors<T> k{static_cast<const E*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[1], a.k_stride[2], a.n_k, a.d, (p.wide & WIDE_K) != 0};
-  const Vectors<T> v{static_cast<const E*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[1], a.v_stride[2], a.n_k, a.d, (p.wide & WIDE_V) != 0};
+  const Vectors<T> k{static_cast<const E*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[1], a.k_stride[2], a.n_k, a.d};
+  const Vectors<T> v{static_cast<const E*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[1], a.v_stride[2], a.n_k, a.d};
   const float* const key_bias = a.key_bias ? a.key_bias + b * a.key_bias_stride : nullptr;
   const signed char* const buckets = a.buckets ? a.buckets + b * a.bucket_stride[0] + query * a.bucket_stride[1] : nullptr;
   unsigned long long* const sums = lds_sums + (lane & 31);
   const bool table_grad = a.gtable != nullptr;
   const float dead = ninf() * p.inv_c;
 
-  Stage<T, D, 64 * W> stage;
+  Stage<T, D, 64 * W, BOTH, BY_ROWS> stage;
   unsigned words[4] = {0, 0, 0, 0};
   if (key0 < end) {
-    stage.fetch(k, v, key0, tid);
+    if (W > 1) stage.fetch(k, v, key0, tid);
     if (buckets) load_buckets(buckets, key0, end, half, words);
   }
   if (tid < 2 * ROWS) lds_kb[tid] = key_value(key_bias, key0 + tid, end, p.inv_c);
@@ -91,21 +91,19 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
   Frag<T> qf[D / 16], gf[D / 16];
   const E* const g_row = static_cast<const E*>(a.gout) + b * a.gout_stride[0] + head * a.gout_stride[1] + query * a.gout_stride[2];
   const float* const o_row = T::PARTS == 3 ? static_cast<const float*>(a.out) + b * a.out_stride[0] + head * a.out_stride[1] + query * a.out_stride[2] : a.out_f32 + row * a.d;
-  const bool wide_g = (p.wide & WIDE_GOUT) != 0;
-  const bool wide_o = T::PARTS == 3 ? (p.wide & WIDE_OUT) != 0 : a.d % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out_f32) & 15) == 0;
   const float2 stats = reinterpret_cast<const float2*>(a.stats)[row];
   const float m = ok ? stats.x : pinf(), inv_l = ok ? stats.y : 0.f;
   const bool live = inv_l != 0.f;                          // a row without keys takes no part, whatever its gradient holds
-  load_column<T, D>(static_cast<const E*>(a.q) + b * a.q_stride[0] + head * a.q_stride[1] + query * a.q_stride[2], a.d, (p.wide & WIDE_Q) != 0, live, half,
+  load_column<T, D>(static_cast<const E*>(a.q) + b * a.q_stride[0] + head * a.q_stride[1] + query * a.q_stride[2], a.d, live, half,
                     a.scale * LOG2E, qf);
-  load_column<T, D>(g_row, a.d, wide_g, live, half, 1.f, gf);
+  load_column<T, D>(g_row, a.d, live, half, 1.f, gf);
   float delta = 0.f, largest = 0.f, total = 0.f;
 #pragma unroll
   for (int i = 0; i < D / 8; ++i) {
     const int quad = 4 * (i / 2) + 2 * half + i % 2;
     float g4[4], o4[4];
-    quad_values<T>(load_quad<T>(g_row, quad, a.d, wide_g), g4);
-    quad_values<F32>(load_quad<F32>(o_row, quad, a.d, wide_o), o4);
+    quad_values<T>(load_quad<T>(g_row, quad, a.d), g4);
+    quad_values<F32>(load_quad<F32>(o_row, quad, a.d), o4);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       delta = fmaf(g4[j], o4[j], delta);
@@ -143,7 +141,9 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
   const auto write = [&](int step) {
     unsigned char* const to = smem + step % BUFS * BUF;
     const float* const kb = lds_kb + step % RING * ROWS;
-    stage.write(to, to + Tl::BYTES, to + 2 * Tl::BYTES, nullptr, tid, a.d, [&](int r) { return kb[r] != dead; });
+    const auto keep = [&](int r) { return kb[r] != dead; };
+    if constexpr (W == 1) stage.fetch_and_write(k, v, key0 + step * ROWS, to, tid, keep);
+    else stage.write(to, tid, keep);
   };
   if (BUFS == 2) {
     __syncthreads();
@@ -168,8 +168,10 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     v16f s, dp = {};
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const float4 kb4 = *reinterpret_cast<const float4*>(kb + 8 * g + 4 * half);
-      s[4 * g] = kb4.x, s[4 * g + 1] = kb4.y, s[4 * g + 2] = kb4.z, s[4 * g + 3] = kb4.w;
+      float start[4];
+      read16(kb + 8 * g + 4 * half, start);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[4 * g + i] = start[i];
     }
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) mma<T>(Tl::by_rows(lds_k, i, lane), qf[i], s);
@@ -180,7 +182,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
 #pragma unroll
     for (int g = 0; g < 4; ++g) now[g] = words[g];
     float kb_next = 0.f;
-    if (key + BUFS * ROWS < end) stage.fetch(k, v, key + BUFS * ROWS, tid);
+    if (W > 1 && key + BUFS * ROWS < end) stage.fetch(k, v, key + BUFS * ROWS, tid);
     if (more && buckets) load_buckets(buckets, key + ROWS, end, half, words);
     if (tid < ROWS) kb_next = key_value(key_bias, key + 2 * ROWS + tid, end, p.inv_c);
 
@@ -207,7 +209,9 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const double x = __builtin_fma((double)s[r], to_units, TableSums::MAGIC);
-        const unsigned long long bits = __builtin_bit_cast(unsigned long long, x) - __builtin_bit_cast(unsigned long long, TableSums::MAGIC);
+        const unsigned long long raw = __builtin_bit_cast(unsigned long long, x);
+        const unsigned high = (unsigned)(raw >> 32) - (unsigned)(__builtin_bit_cast(unsigned long long, TableSums::MAGIC) >> 32);   // its low half is zero
+        const unsigned long long bits = (unsigned long long)high << 32 | (unsigned)raw;
         __hip_atomic_fetch_add(sums + n_of[r] * TableSums::COPIES, bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
       }
     }
@@ -236,14 +240,16 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     store_partial<D>(p.partial + (split * rows + row) * D, half, dq);
     return;
   }
-  store_column<T, D>(static_cast<E*>(a.gq) + b * a.gq_stride[0] + head * a.gq_stride[1] + query * a.gq_stride[2], a.d, (p.wide & WIDE_GQ) != 0, half, dq, a.scale * undo);
+  store_column<T, D>(static_cast<E*>(a.gq) + b * a.gq_stride[0] + head * a.gq_stride[1] + query * a.gq_stride[2], a.d, half, dq, a.scale * undo);
 }
 
 // ---- dk, dv ---------------------------------------------------------------------------------------------------------
 // Columns: keys of one key head.  Rows: the queries of its heads, tile by tile, head by head.
+template <class T, int D, int W> constexpr int kv_buffers() { return W > 1 && 2 * 4 * Tile<T, D>::BYTES <= 100 * 1024 ? 2 : 1; }
+
 template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS * D > 64 ? 1 : 2) void grad_kv_kernel(Args p) {
   typedef Tile<T, D> Tl;
-  constexpr int BUFS = 2 * 4 * Tl::BYTES <= 100 * 1024 ? 2 : 1, BUF = 4 * Tl::BYTES;
+  constexpr int BUFS = kv_buffers<T, D, W>(), BUF = 4 * Tl::BYTES;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   float* const lds_rows = reinterpret_cast<float*>(smem + BUFS * BUF);        // [RING][3][ROWS]: m, 1 / l, delta; first two negated
   float* const lds_table = lds_rows + 3 * RING * ROWS;
@@ -269,14 +275,15 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
 
   typedef typename T::type E;
   const float* const key_bias = a.key_bias ? a.key_bias + b * a.key_bias_stride : nullptr;
-  const signed char* const buckets = a.buckets ? a.buckets + b * a.bucket_stride[0] + key : nullptr;
+  const signed char* const buckets = a.buckets ? a.buckets + b * a.bucket_stride[0] : nullptr;
+  const unsigned bucket_offset = (unsigned)(4 * half * (int)a.bucket_stride[1] + key);
   const float dead = ninf() * p.inv_c, kb_c = ok ? key_value(key_bias, key, end, p.inv_c) : dead, kb = kb_c * p.c;
   const bool live = kb_c != dead;
 
   Frag<T> kf[D / 16], vf[D / 16];
-  load_column<T, D>(static_cast<const E*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[1] + key * a.k_stride[2], a.d, (p.wide & WIDE_K) != 0, live, half,
+  load_column<T, D>(static_cast<const E*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[1] + key * a.k_stride[2], a.d, live, half,
                     a.scale * LOG2E, kf);
-  load_column<T, D>(static_cast<const E*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[1] + key * a.v_stride[2], a.d, (p.wide & WIDE_V) != 0, live, half, 1.f, vf);
+  load_column<T, D>(static_cast<const E*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[1] + key * a.v_stride[2], a.d, live, half, 1.f, vf);
 
   ScoreScale sc;
   if constexpr (T::HALF) {                                 // one for all heads and queries: they are summed
@@ -293,13 +300,11 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     sc = score_scale<T>(a.n_k, t);
   }
 
-  Stage<T, D, 64 * W> stage;
-  const auto fetch = [&](int r) {
-    const int head = hk * group + r / per_head;
-    const Vectors<T> q{static_cast<const E*>(a.q) + b * a.q_stride[0] + head * a.q_stride[1], a.q_stride[2], a.n_q, a.d, (p.wide & WIDE_Q) != 0};
-    const Vectors<T> g{static_cast<const E*>(a.gout) + b * a.gout_stride[0] + head * a.gout_stride[1], a.gout_stride[2], a.n_q, a.d, (p.wide & WIDE_GOUT) != 0};
-    stage.fetch(q, g, r % per_head * ROWS, tid);
+  Stage<T, D, 64 * W, BOTH, BOTH> stage;
+  const auto queries = [&](int r, const void* base, const long (&stride)[3]) -> Vectors<T> {     // of the head of tile r
+    return {static_cast<const E*>(base) + b * stride[0] + (hk * group + r / per_head) * stride[1], stride[2], a.n_q, a.d};
   };
+  const auto fetch = [&](int r) { stage.fetch(queries(r, a.q, a.q_stride), queries(r, a.gout, a.gout_stride), r % per_head * ROWS, tid); };
   struct Row { float m, rl, delta; };
   const auto row_of = [&](int r) -> Row {                  // what thread tid < ROWS brings for row tid of tile r
     const int query = r % per_head * ROWS + tid;
@@ -315,9 +320,12 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
   const auto write = [&](int r) {
     unsigned char* const to = smem + (r - first) % BUFS * BUF;
     const float* const rows = lds_rows + (r - first) % RING * 3 * ROWS;
-    stage.write(to, to + Tl::BYTES, to + 2 * Tl::BYTES, to + 3 * Tl::BYTES, tid, a.d, [&](int i) { return rows[ROWS + i] != 0.f; });
+    const auto keep = [&](int i) { return rows[ROWS + i] != 0.f; };
+    if constexpr (W == 1)
+      stage.fetch_and_write(queries(r, a.q, a.q_stride), queries(r, a.gout, a.gout_stride), r % per_head * ROWS, to, tid, keep);
+    else stage.write(to, tid, keep);
   };
-  if (first < last) fetch(first);
+  if (W > 1 && first < last) fetch(first);
   if (tid < ROWS) put_row(first, row_of(first)), put_row(first + 1, row_of(first + 1));
   if (buckets) stage_table<T>(lds_table, a.table, a.n_buckets, hk * group, group, tid, 64 * W);
   if (BUFS == 2) {
@@ -341,9 +349,15 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     const int query0 = r % per_head * ROWS;
     unsigned n_of[16];
     if (buckets) {
+      const signed char* const at = buckets + query0 * a.bucket_stride[1];       // uniform; the lane's key and half are an offset
+      if (query0 + ROWS <= a.n_q) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        n_of[i] = (unsigned char)buckets[min(query0 + 8 * (i / 4) + 4 * half + i % 4, a.n_q - 1) * a.bucket_stride[1]];
+        for (int i = 0; i < 16; ++i) n_of[i] = (unsigned char)(at + (8 * (i / 4) + i % 4) * a.bucket_stride[1])[bucket_offset];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          n_of[i] = (unsigned char)at[(unsigned)(min(8 * (i / 4) + 4 * half + i % 4, a.n_q - 1 - query0) * (int)a.bucket_stride[1] + key)];
+      }
     }
     const float* const table = lds_table + r / per_head * (a.n_buckets + 1);
 
@@ -351,31 +365,32 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     v16f s = {}, dp;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const float4 d4 = *reinterpret_cast<const float4*>(rows + 2 * ROWS + 8 * g + 4 * half);
-      dp[4 * g] = d4.x, dp[4 * g + 1] = d4.y, dp[4 * g + 2] = d4.z, dp[4 * g + 3] = d4.w;
+      float start[4];
+      read16(rows + 2 * ROWS + 8 * g + 4 * half, start);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) dp[4 * g + i] = start[i];
       if constexpr (T::PARTS == 3) {
-        const float4 m4 = *reinterpret_cast<const float4*>(rows + 8 * g + 4 * half);
-        s[4 * g] = m4.x, s[4 * g + 1] = m4.y, s[4 * g + 2] = m4.z, s[4 * g + 3] = m4.w;
+        read16(rows + 8 * g + 4 * half, start);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[4 * g + i] = start[i];
       }
     }
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) mma<T>(Tl::by_rows(lds_q, i, lane), kf[i], s);
+    if constexpr (T::PARTS * D > 256) __builtin_amdgcn_sched_barrier(0);     // no operand of a later product is read before: registers
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) mma<T>(Tl::by_rows(lds_g, i, lane), vf[i], dp);
+    if constexpr (T::PARTS * D > 256) __builtin_amdgcn_sched_barrier(0);     // no operand of a later product is read before: registers
     if (BUFS == 2 && r + 1 < last) write(r + 1);
     Row next = {};
-    if (r + BUFS < last) fetch(r + BUFS);
+    if (W > 1 && r + BUFS < last) fetch(r + BUFS);
     if (tid < ROWS) next = row_of(r + 2);
 
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const float4 l4 = *reinterpret_cast<const float4*>(rows + ROWS + 8 * g + 4 * half);
-      const float ls[4] = {l4.x, l4.y, l4.z, l4.w};
-      float ms[4] = {0.f, 0.f, 0.f, 0.f};
-      if constexpr (T::PARTS == 1) {
-        const float4 m4 = *reinterpret_cast<const float4*>(rows + 8 * g + 4 * half);
-        ms[0] = m4.x, ms[1] = m4.y, ms[2] = m4.z, ms[3] = m4.w;
-      }
+      float ls[4], ms[4] = {0.f, 0.f, 0.f, 0.f};
+      read16(rows + ROWS + 8 * g + 4 * half, ls);
+      if constexpr (T::PARTS == 1) read16(rows + 8 * g + 4 * half, ms);
 #pragma unroll
       for (int i = 0; i < 4; i += 2) {
         float pr[2];
@@ -395,6 +410,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
         }
       }
     }
+    if constexpr (T::PARTS * D > 256) __builtin_amdgcn_sched_barrier(0);     // no operand of a later product is read before: registers
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const Frag<T> pf = cut_rows<T>(s, t), df = cut_rows<T>(dp, t);
@@ -418,8 +434,8 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     store_partial<D>(part + ((p.splits + split) * columns + column) * D, half, dv);
     return;
   }
-  store_column<T, D>(static_cast<E*>(a.gk) + b * a.gk_stride[0] + hk * a.gk_stride[1] + key * a.gk_stride[2], a.d, (p.wide & WIDE_GK) != 0, half, dk, fk);
-  store_column<T, D>(static_cast<E*>(a.gv) + b * a.gv_stride[0] + hk * a.gv_stride[1] + key * a.gv_stride[2], a.d, (p.wide & WIDE_GV) != 0, half, dv, fv);
+  store_column<T, D>(static_cast<E*>(a.gk) + b * a.gk_stride[0] + hk * a.gk_stride[1] + key * a.gk_stride[2], a.d, half, dk, fk);
+  store_column<T, D>(static_cast<E*>(a.gv) + b * a.gv_stride[0] + hk * a.gv_stride[1] + key * a.gv_stride[2], a.d, half, dv, fv);
 }
 
 // ---- sums of partial results, in a fixed order ----------------------------------------------------------------------
@@ -431,7 +447,7 @@ template <class T, int D> __global__ __launch_bounds__(256) void sum_vectors_ker
   typename T::type* const out = to + i / n / heads * s0 + i / n % heads * s1 + i % n * s2;
   for (int e = threadIdx.x & 63; e < d; e += 64) {
     float t = 0.f;
-    for (int s = 0; s < splits; ++s) t += part[(s * vectors + i) * D + e];
+    for (int s = 0; s < splits; ++s) t += part[(s * vectors + i) * D + slot_of(e, d)];
     out[e] = (typename T::type)t;
   }
 }
@@ -459,19 +475,23 @@ template <class T, int D> void backward_d(Args& p, const Plans& plans, float* pa
   };
   use(plans.grad_q, partial_q);
   const int waves_q = plans.grad_q.waves;
-  const size_t lds_q = buffers<T, D>(3) * 3 * Tile<T, D>::BYTES + (RING * ROWS + MAX_BUCKETS + 4) * sizeof(float) +
+  const size_t lds_q = (waves_q == 1 ? buffers<T, D, 1>(3) : buffers<T, D, 4>(3)) * 3 * Tile<T, D>::BYTES + (RING * ROWS + MAX_BUCKETS + 4) * sizeof(float) +
                        (a.gtable ? TableSums::words(a.n_buckets) * sizeof(unsigned long long) : 0);
-  if (waves_q == 1) launch(grad_q_kernel<T, D, 1>, p, 1, lds_q, stream);
-  else launch(grad_q_kernel<T, D, 4>, p, 4, lds_q, stream);
+  if constexpr (few_waves<T, D>) {
+    if (waves_q == 1) launch(grad_q_kernel<T, D, 1>, p, 1, lds_q, stream);
+  }
+  if (waves_q != 1) launch(grad_q_kernel<T, D, 4>, p, 4, lds_q, stream);
   if (plans.grad_q.splits > 1) sum_vectors<T>(partial_q, plans.grad_q.splits, D, a.gq, a.gq_stride, a.batch, a.heads, a.n_q, a.d, stream);
   if (a.gtable)
     hipLaunchKernelGGL(sum_table_kernel<T>, dim3((unsigned)(a.heads * a.n_buckets)), dim3(64), 0, stream, p.gtable_partial, a.batch, a.heads,
                        plans.grad_q.splits * plans.grad_q.tiles, a.n_buckets, static_cast<typename T::type*>(a.gtable));
   if (!a.gk) return;
   use(plans.grad_kv, partial_kv);
-  const size_t lds_kv = (2 * 4 * Tile<T, D>::BYTES <= 100 * 1024 ? 2 : 1) * 4 * Tile<T, D>::BYTES + (3 * RING * ROWS + (a.buckets ? a.heads / a.kv_heads * (a.n_buckets + 1) : 0)) * sizeof(float);
-  if (plans.grad_kv.waves == 1) launch(grad_kv_kernel<T, D, 1>, p, 1, lds_kv, stream);
-  else launch(grad_kv_kernel<T, D, 4>, p, 4, lds_kv, stream);
+  const size_t lds_kv = (plans.grad_kv.waves == 1 ? kv_buffers<T, D, 1>() : kv_buffers<T, D, 4>()) * 4 * Tile<T, D>::BYTES + (3 * RING * ROWS + (a.buckets ? a.heads / a.kv_heads * (a.n_buckets + 1) : 0)) * sizeof(float);
+  if constexpr (few_waves<T, D>) {
+    if (plans.grad_kv.waves == 1) launch(grad_kv_kernel<T, D, 1>, p, 1, lds_kv, stream);
+  }
+  if (plans.grad_kv.waves != 1) launch(grad_kv_kernel<T, D, 4>, p, 4, lds_kv, stream);
   if (plans.grad_kv.splits > 1) {
     const long columns = (long)a.batch * a.kv_heads * a.n_k;
     sum_vectors<T>(partial_kv, plans.grad_kv.splits, D, a.gk, a.gk_stride, a.batch, a.kv_heads, a.n_k, a.d, stream);

@@ -12,7 +12,7 @@ namespace attn {
 
 template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS * D > 192 ? 1 : 2) void forward_kernel(Args p) {
   typedef Tile<T, D> Tl;
-  constexpr int BUFS = buffers<T, D>(2), BUF = 2 * Tl::BYTES;
+  constexpr int BUFS = buffers<T, D, W>(2), BUF = 2 * Tl::BYTES;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   float* const lds_kb = reinterpret_cast<float*>(smem + BUFS * BUF);          // [RING][ROWS]
   float* const lds_table = lds_kb + RING * ROWS;
@@ -37,30 +37,32 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
   end = min(end, key0 + chunk);
 
   typedef typename T::type E;
-  const Vectors<T> k{static_cast<const E*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[1], a.k_stride[2], a.n_k, a.d, (p.wide & WIDE_K) != 0};
-  const Vectors<T> v{static_cast<const E*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[1], a.v_stride[2], a.n_k, a.d, (p.wide & WIDE_V) != 0};
+  const Vectors<T> k{static_cast<const E*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[1], a.k_stride[2], a.n_k, a.d};
+  const Vectors<T> v{static_cast<const E*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[1], a.v_stride[2], a.n_k, a.d};
   const float* const key_bias = a.key_bias ? a.key_bias + b * a.key_bias_stride : nullptr;
   const signed char* const buckets = a.buckets ? a.buckets + b * a.bucket_stride[0] + query * a.bucket_stride[1] : nullptr;
   const float* const table = lds_table + (head - head0) * (a.n_buckets + 1);
   const bool measure = a.stats && tile == 0;                // this workgroup finds the largest |v| of its keys for the backward pass
   const float dead = ninf() * p.inv_c;
 
-  Stage<T, D, 64 * W> stage;
+  Stage<T, D, 64 * W, BY_ROWS, BY_ENTRIES> stage;
   unsigned words[4] = {0, 0, 0, 0};
   if (key0 < end) {
-    stage.fetch(k, v, key0, tid);
+    if (W > 1) stage.fetch(k, v, key0, tid);
     if (buckets) load_buckets(buckets, key0, end, half, words);
   }
   if (tid < 2 * ROWS) lds_kb[tid] = key_value(key_bias, key0 + tid, end, p.inv_c);
   if (buckets) stage_table<T>(lds_table, a.table, a.n_buckets, head0, heads, tid, 64 * W);
   Frag<T> qf[D / 16];
-  load_column<T, D>(static_cast<const E*>(a.q) + b * a.q_stride[0] + head * a.q_stride[1] + query * a.q_stride[2], a.d, (p.wide & WIDE_Q) != 0, ok, half,
+  load_column<T, D>(static_cast<const E*>(a.q) + b * a.q_stride[0] + head * a.q_stride[1] + query * a.q_stride[2], a.d, ok, half,
                     a.scale * LOG2E, qf);
   float largest = 0.f;
   const auto write = [&](int step) {
     unsigned char* const to = smem + step % BUFS * BUF;
     const float* const kb = lds_kb + step % RING * ROWS;
-    stage.write(to, nullptr, nullptr, to + Tl::BYTES, tid, a.d, [&](int r) { return kb[r] != dead; });
+    const auto keep = [&](int r) { return kb[r] != dead; };
+    if constexpr (W == 1) stage.fetch_and_write(k, v, key0 + step * ROWS, to, tid, keep);
+    else stage.write(to, tid, keep);
     if (measure) largest = fmaxf(largest, stage.largest_second(tid));
   };
   if (BUFS == 2) {
@@ -87,8 +89,10 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     v16f s;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const float4 kb4 = *reinterpret_cast<const float4*>(kb + 8 * g + 4 * half);
-      s[4 * g] = kb4.x, s[4 * g + 1] = kb4.y, s[4 * g + 2] = kb4.z, s[4 * g + 3] = kb4.w;
+      float start[4];
+      read16(kb + 8 * g + 4 * half, start);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[4 * g + i] = start[i];
     }
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) mma<T>(Tl::by_rows(lds_k, i, lane), qf[i], s);
@@ -97,7 +101,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
 #pragma unroll
     for (int g = 0; g < 4; ++g) now[g] = words[g];
     float kb_next = 0.f;
-    if (key + BUFS * ROWS < end) stage.fetch(k, v, key + BUFS * ROWS, tid);
+    if (W > 1 && key + BUFS * ROWS < end) stage.fetch(k, v, key + BUFS * ROWS, tid);
     if (more && buckets) load_buckets(buckets, key + ROWS, end, half, words);
     if (tid < ROWS) kb_next = key_value(key_bias, key + 2 * ROWS + tid, end, p.inv_c);
 
@@ -166,12 +170,12 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
   // a row without keys: zeros, and statistics by which every probability is zero
   const bool any = l != 0.f;
   const float inv = any ? 1.f / l : 0.f;
-  store_column<T, D>(static_cast<E*>(a.out) + b * a.out_stride[0] + head * a.out_stride[1] + query * a.out_stride[2], a.d, (p.wide & WIDE_OUT) != 0, half, o, inv);
-  if (T::PARTS == 1 && a.out_f32) store_column<F32, D>(a.out_f32 + row * a.d, a.d, a.d % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out_f32) & 15) == 0, half, o, inv);
+  store_column<T, D>(static_cast<E*>(a.out) + b * a.out_stride[0] + head * a.out_stride[1] + query * a.out_stride[2], a.d, half, o, inv);
+  if (T::PARTS == 1 && a.out_f32) store_column<F32, D>(a.out_f32 + row * a.d, a.d, half, o, inv);
   if (half == 0 && a.stats) reinterpret_cast<float2*>(a.stats)[row] = any ? make_float2(m - SHIFT, inv) : make_float2(pinf(), 0.f);
 }
 
-// One wave joins the parts of one query: the sums of all parts, each times 2^(its maximum - the maximum of all).
+// One wave joins the parts of one query.
 template <class T, int D> __global__ __launch_bounds__(256) void join_kernel(Args p) {
   const s2cnn_attention_t& a = p.a;
   const long rows = (long)a.batch * a.heads * a.n_q, row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -180,18 +184,31 @@ template <class T, int D> __global__ __launch_bounds__(256) void join_kernel(Arg
   const float* const part = p.partial;
   const float2* const ml = reinterpret_cast<const float2*>(part + p.splits * rows * D);
   constexpr float SHIFT = T::HALF ? 10.f : 0.f;
+  // lane s has the maximum and the sum of part s (of 64 parts at a time): its weight, 2^(its maximum - the maximum of all)
   float m = ninf();
-  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, ml[s * rows + row].x);
+  for (int s = lane; s < p.splits; s += 64) m = fmaxf(m, ml[s * rows + row].x);
+#pragma unroll
+  for (int i = 32; i; i >>= 1) m = fmaxf(m, __shfl_xor(m, i));
   const float ref = m == ninf() ? 0.f : m;
   float l = 0.f, o[(D + 63) / 64] = {};
-  for (int s = 0; s < p.splits; ++s) {
-    const float2 x = ml[s * rows + row];
-    const float w = exp2_(x.x - ref);
-    l = fmaf(x.y, w, l);
+  for (int s0 = 0; s0 < p.splits; s0 += 64) {
+    float w = 0.f;
+    if (s0 + lane < p.splits) {
+      const float2 x = ml[(s0 + lane) * rows + row];
+      w = exp2_(x.x - ref);
+      l = fmaf(x.y, w, l);
+    }
+    const int n = min(64, p.splits - s0);
+#pragma unroll 8
+    for (int s = 0; s < n; ++s) {
+      const float ws = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), s));
 #pragma unroll
-    for (int i = 0; i < (D + 63) / 64; ++i)
-      if (lane + 64 * i < D) o[i] = fmaf(part[(s * rows + row) * D + lane + 64 * i], w, o[i]);
+      for (int i = 0; i < (D + 63) / 64; ++i)
+        if (lane + 64 * i < a.d) o[i] = fmaf(part[((s0 + s) * rows + row) * D + slot_of(lane + 64 * i, a.d)], ws, o[i]);
+    }
   }
+#pragma unroll
+  for (int i = 32; i; i >>= 1) l += __shfl_xor(l, i);
   const bool any = l != 0.f;
   const float inv = any ? 1.f / l : 0.f;
   const int query = (int)(row % a.n_q), head = (int)(row / a.n_q % a.heads), b = (int)(row / a.n_q / a.heads);
@@ -210,9 +227,11 @@ template <class T, int D> void forward_d(const Args& p, const Plans& plans, hipS
   const s2cnn_attention_t& a = p.a;
   const Plan& f = plans.fwd;
   const int heads = min(a.heads / a.kv_heads, (32 * f.waves - 1) / a.n_q + 2);
-  const size_t lds = buffers<T, D>(2) * 2 * Tile<T, D>::BYTES + (RING * ROWS + (a.buckets ? heads * (a.n_buckets + 1) : 0)) * sizeof(float);
-  if (f.waves == 1) launch(forward_kernel<T, D, 1>, p, 1, lds, stream);
-  else launch(forward_kernel<T, D, 4>, p, 4, lds, stream);
+  const size_t lds = (f.waves == 1 ? buffers<T, D, 1>(2) : buffers<T, D, 4>(2)) * 2 * Tile<T, D>::BYTES + (RING * ROWS + (a.buckets ? heads * (a.n_buckets + 1) : 0)) * sizeof(float);
+  if constexpr (few_waves<T, D>) {
+    if (f.waves == 1) launch(forward_kernel<T, D, 1>, p, 1, lds, stream);
+  }
+  if (f.waves != 1) launch(forward_kernel<T, D, 4>, p, 4, lds, stream);
   if (f.splits > 1)
     hipLaunchKernelGGL((join_kernel<T, D>), dim3((unsigned)(((long)a.batch * a.heads * a.n_q + 3) / 4)), dim3(256), 0, stream, p);
 }

@@ -131,6 +131,17 @@ def test_forward_and_gradients(hip, size, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("d", [64, 65, 100, 127, 128])
+def test_wide_heads_with_few_columns(hip, d, dtype):
+    """Few queries, few keys, one and several tiles of the other side: the workgroups of one wave, which have the most per lane."""
+    for i, (nq, nk) in enumerate([(1, 32), (2, 31), (3, 33), (31, 64), (32, 100), (1, 300), (5, 129), (64, 1), (100, 32), (257, 31), (40, 20)]):
+        for kind in (dict(), dict(nb=11, excluded=0.2, key_bias="batch", ragged=True)):
+            s, g = _inputs(2, 2, 1, nq, nk, d, dtype, seed=i, **kind)
+            _check(s, g, dtype, "%d %d %s" % (nq, nk, kind))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("nb", [1, 2, 63, 64])
 def test_tables_of_every_size(hip, nb):
     s, g = _inputs(2, 3, 3, 70, 90, 24, F32, nb=nb, excluded=0.1)
