@@ -43,7 +43,7 @@ struct TableSums {
   static __host__ __device__ int words(int n_buckets) { return (n_buckets + 1) * COPIES; }       // one more for excluded pairs
 };
 
-template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS * D > 128 ? 1 : 2) void grad_q_kernel(Args p) {
+template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS * D > 96 ? 1 : 2) void grad_q_kernel(Args p) {
   typedef Tile<T, D> Tl;
   constexpr int BUFS = buffers<T, D, W>(3), BUF = 3 * Tl::BYTES;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -247,7 +247,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
 // Columns: keys of one key head.  Rows: the queries of its heads, tile by tile, head by head.
 template <class T, int D, int W> constexpr int kv_buffers() { return W > 1 && 2 * 4 * Tile<T, D>::BYTES <= 100 * 1024 ? 2 : 1; }
 
-template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS * D > 64 ? 1 : 2) void grad_kv_kernel(Args p) {
+template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS * D > 96 ? 1 : 2) void grad_kv_kernel(Args p) {
   typedef Tile<T, D> Tl;
   constexpr int BUFS = kv_buffers<T, D, W>(), BUF = 4 * Tl::BYTES;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -325,7 +325,21 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
       stage.fetch_and_write(queries(r, a.q, a.q_stride), queries(r, a.gout, a.gout_stride), r % per_head * ROWS, to, tid, keep);
     else stage.write(to, tid, keep);
   };
+  unsigned n_of[16];                                       // the tile's buckets, fetched a tile ahead
+  const auto fetch_buckets = [&](int r) {
+    const int query0 = r % per_head * ROWS;
+    const signed char* const at = buckets + query0 * a.bucket_stride[1];         // uniform; the lane's key and half are an offset
+    if (query0 + ROWS <= a.n_q) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) n_of[i] = (unsigned char)(at + (8 * (i / 4) + i % 4) * a.bucket_stride[1])[bucket_offset];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        n_of[i] = (unsigned char)at[(unsigned)(min(8 * (i / 4) + 4 * half + i % 4, a.n_q - 1 - query0) * (int)a.bucket_stride[1] + key)];
+    }
+  };
   if (W > 1 && first < last) fetch(first);
+  if (buckets && first < last) fetch_buckets(first);
   if (tid < ROWS) put_row(first, row_of(first)), put_row(first + 1, row_of(first + 1));
   if (buckets) stage_table<T>(lds_table, a.table, a.n_buckets, hk * group, group, tid, 64 * W);
   if (BUFS == 2) {
@@ -345,19 +359,6 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     if (BUFS == 1) {
       write(r);
       __syncthreads();
-    }
-    const int query0 = r % per_head * ROWS;
-    unsigned n_of[16];
-    if (buckets) {
-      const signed char* const at = buckets + query0 * a.bucket_stride[1];       // uniform; the lane's key and half are an offset
-      if (query0 + ROWS <= a.n_q) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) n_of[i] = (unsigned char)(at + (8 * (i / 4) + i % 4) * a.bucket_stride[1])[bucket_offset];
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          n_of[i] = (unsigned char)at[(unsigned)(min(8 * (i / 4) + 4 * half + i % 4, a.n_q - 1 - query0) * (int)a.bucket_stride[1] + key)];
-      }
     }
     const float* const table = lds_table + r / per_head * (a.n_buckets + 1);
 
@@ -385,6 +386,12 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     Row next = {};
     if (W > 1 && r + BUFS < last) fetch(r + BUFS);
     if (tid < ROWS) next = row_of(r + 2);
+    float bias[16];
+    if (buckets) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) bias[i] = table[min((int)n_of[i], a.n_buckets)];
+      if (r + 1 < last) fetch_buckets(r + 1);
+    }
 
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
@@ -397,8 +404,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int j = 4 * g + i + e;
-          const float t = buckets ? table[min((int)n_of[j], a.n_buckets)] : 0.f;
-          const float x = T::PARTS == 3 ? (buckets ? s[j] + t : s[j]) + kb : ((buckets ? fmaf(s[j], p.c, t) : s[j] * p.c) + kb) + ms[i + e];
+          const float x = T::PARTS == 3 ? (buckets ? s[j] + bias[j] : s[j]) + kb : ((buckets ? fmaf(s[j], p.c, bias[j]) : s[j] * p.c) + kb) + ms[i + e];
           pr[e] = exp2_(x);
         }
         round_pair<T>(pr[0], pr[1]);
