@@ -288,7 +288,7 @@ template <class T, int D> struct Tile {
 // written while the one before is used, with one barrier per tile; else one.  One, too, where the workgroup is a wave: it fetches
 // a tile and writes it at once (a thread has up to eight blocks then, too many registers to hold beside the operands), and the
 // other waves of the CU are what hides the wait.
-template <class T, int D, int W> constexpr int buffers(int layouts) { return W > 1 && 2 * layouts * Tile<T, D>::BYTES <= 80 * 1024 ? 2 : 1; }
+template <class T, int D, int W> constexpr int buffers(int layouts) { return W > 1 && 2 * layouts * Tile<T, D>::BYTES <= 64 * 1024 ? 2 : 1; }
 
 // Two tensors staged by the same tiles of rows, in the layouts LA and LB (those of the first, then those of the second): THREADS threads
 // fetch the blocks of a tile into registers, and write them later.
@@ -383,8 +383,8 @@ template <class T, int D, int THREADS, int LA, int LB> struct Stage {
 // the sums, the output and the backward pass all use the same, rounded ones.  They are so the exact softmax of weights that
 // are off by a rounding each, rows of its gradient sum to zero as they should, and a factor between references is exact.
 //
-// The product starts from the key's bias instead of zero: x = c (q.k + bias / c) + table, c = log2(e) scale; float32 takes c into
-// the columns as they are loaded, and needs no factor.  Biases are held within +-3e38, so that one of the type's lowest value
+// The product starts from the biases instead of zero: x = c (q.k + bias / c), c = log2(e) scale; float32 takes c into the columns as
+// they are loaded, and needs no factor.  Biases are held within +-3e38, so that one of the type's lowest value
 // stays finite: keys that all have it share a row evenly.
 __device__ __forceinline__ float key_value(const float* key_bias, int key, int end, float inv_c) {
   if (key >= end) return ninf() * inv_c;                   // takes no part
@@ -424,6 +424,26 @@ __device__ __forceinline__ void load_buckets(const signed char* row, int key0, i
   }
 }
 __device__ __forceinline__ int bucket_of(unsigned w, int i, int n_buckets) { return min((int)((w >> (8 * i)) & 255u), n_buckets); }
+
+// What the scores of a tile start from: the keys' biases, and the table's entries of the pairs where there are buckets.  In the
+// accumulators before the product begins, they need no registers beside them.
+template <class T> __device__ __forceinline__ void start_scores(v16f& s, const float* kb, int half, bool buckets, const unsigned (&words)[4], const float* table,
+                                                                int n_buckets, float inv_c) {
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    float start[4];
+    read16(kb + 8 * g + 4 * half, start);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[4 * g + i] = start[i];
+  }
+  if (buckets) {
+    float t[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) t[r] = table[bucket_of(words[r / 4], r % 4, n_buckets)];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = T::PARTS == 3 ? s[r] + t[r] : fmaf(t[r], inv_c, s[r]);
+  }
+}
 
 // ---- arguments ------------------------------------------------------------------------------------------------------
 // The header's struct and what the entry has made of it.

@@ -43,7 +43,7 @@ struct TableSums {
   static __host__ __device__ int words(int n_buckets) { return (n_buckets + 1) * COPIES; }       // one more for excluded pairs
 };
 
-template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS * D > 96 ? 1 : 2) void grad_q_kernel(Args p) {
+template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || T::PARTS * D > 192 ? 1 : 2) void grad_q_kernel(Args p) {
   typedef Tile<T, D> Tl;
   constexpr int BUFS = buffers<T, D, W>(3), BUF = 3 * Tl::BYTES;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -166,13 +166,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     const float* const kb = lds_kb + step % RING * ROWS;
 
     v16f s, dp = {};
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      float start[4];
-      read16(kb + 8 * g + 4 * half, start);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[4 * g + i] = start[i];
-    }
+    start_scores<T>(s, kb, half, buckets != nullptr, words, lds_table, a.n_buckets, p.inv_c);
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) mma<T>(Tl::by_rows(lds_k, i, lane), qf[i], s);
 #pragma unroll
@@ -186,33 +180,21 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     if (more && buckets) load_buckets(buckets, key + ROWS, end, half, words);
     if (tid < ROWS) kb_next = key_value(key_bias, key + 2 * ROWS + tid, end, p.inv_c);
 
-    int n_of[16];
-    if (buckets) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        n_of[r] = bucket_of(now[r / 4], r % 4, a.n_buckets);
-        const float t = lds_table[n_of[r]];
-        s[r] = T::PARTS == 3 ? s[r] + t : fmaf(s[r], p.c, t);
-      }
-    } else if (T::PARTS == 1) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] *= p.c;
-    }
 #pragma unroll
     for (int r = 0; r < 16; r += 2) {
-      float pr[2] = {exp2_(s[r] - m), exp2_(s[r + 1] - m)};
+      float pr[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) pr[i] = exp2_(T::PARTS == 3 ? s[r + i] - m : s[r + i] * p.c - m);
       round_pair<T>(pr[0], pr[1]);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) s[r + i] = pr[i] * rl * (T::HALF ? fmaf(dp[r + i], sc.ds, -delta_s) : dp[r + i] - delta);
-    }
-    if (table_grad) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const double x = __builtin_fma((double)s[r], to_units, TableSums::MAGIC);
-        const unsigned long long raw = __builtin_bit_cast(unsigned long long, x);
-        const unsigned high = (unsigned)(raw >> 32) - (unsigned)(__builtin_bit_cast(unsigned long long, TableSums::MAGIC) >> 32);   // its low half is zero
-        const unsigned long long bits = (unsigned long long)high << 32 | (unsigned)raw;
-        __hip_atomic_fetch_add(sums + n_of[r] * TableSums::COPIES, bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+      for (int i = 0; i < 2; ++i) {
+        s[r + i] = pr[i] * rl * (T::HALF ? fmaf(dp[r + i], sc.ds, -delta_s) : dp[r + i] - delta);
+        if (table_grad) {
+          const double x = __builtin_fma((double)s[r + i], to_units, TableSums::MAGIC);
+          const unsigned long long raw = __builtin_bit_cast(unsigned long long, x);
+          const unsigned high = (unsigned)(raw >> 32) - (unsigned)(__builtin_bit_cast(unsigned long long, TableSums::MAGIC) >> 32);   // its low half is zero
+          __hip_atomic_fetch_add(sums + bucket_of(now[r / 4], r % 4 + i, a.n_buckets) * TableSums::COPIES, (unsigned long long)high << 32 | (unsigned)raw, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        }
       }
     }
 #pragma unroll
@@ -245,14 +227,16 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
 
 // ---- dk, dv ---------------------------------------------------------------------------------------------------------
 // Columns: keys of one key head.  Rows: the queries of its heads, tile by tile, head by head.
-template <class T, int D, int W> constexpr int kv_buffers() { return W > 1 && 2 * 4 * Tile<T, D>::BYTES <= 100 * 1024 ? 2 : 1; }
+constexpr int BUCKET_LD = 9;
+template <class T, int D, int W> constexpr int kv_buffers() { return buffers<T, D, W>(4); }
 
-template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS * D > 96 ? 1 : 2) void grad_kv_kernel(Args p) {
+template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || D > 64 ? 1 : 2) void grad_kv_kernel(Args p) {
   typedef Tile<T, D> Tl;
   constexpr int BUFS = kv_buffers<T, D, W>(), BUF = 4 * Tl::BYTES;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   float* const lds_rows = reinterpret_cast<float*>(smem + BUFS * BUF);        // [RING][3][ROWS]: m, 1 / l, delta; first two negated
-  float* const lds_table = lds_rows + 3 * RING * ROWS;
+  unsigned* const lds_buckets = reinterpret_cast<unsigned*>(lds_rows + 3 * RING * ROWS);      // [2][32 W keys][8 words of four queries, one unused]
+  float* const lds_table = lds_rows + 3 * RING * ROWS + 2 * 32 * W * BUCKET_LD;
   const s2cnn_attention_t& a = p.a;
 
   const int work = work_of_block(p.workgroups);
@@ -276,7 +260,6 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
   typedef typename T::type E;
   const float* const key_bias = a.key_bias ? a.key_bias + b * a.key_bias_stride : nullptr;
   const signed char* const buckets = a.buckets ? a.buckets + b * a.bucket_stride[0] : nullptr;
-  const unsigned bucket_offset = (unsigned)(4 * half * (int)a.bucket_stride[1] + key);
   const float dead = ninf() * p.inv_c, kb_c = ok ? key_value(key_bias, key, end, p.inv_c) : dead, kb = kb_c * p.c;
   const bool live = kb_c != dead;
 
@@ -325,18 +308,31 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
       stage.fetch_and_write(queries(r, a.q, a.q_stride), queries(r, a.gout, a.gout_stride), r % per_head * ROWS, to, tid, keep);
     else stage.write(to, tid, keep);
   };
-  unsigned n_of[16];                                       // the tile's buckets, fetched a tile ahead
+  // The tile's buckets pass through LDS too: a thread fetches those of 4 queries and 4 keys, and writes them the other way round, a word
+  // of four queries per key.
+  unsigned bucket_words[4];
+  const int block_query = 4 * (tid / (8 * W)), block_key = 4 * (tid % (8 * W));
   const auto fetch_buckets = [&](int r) {
-    const int query0 = r % per_head * ROWS;
-    const signed char* const at = buckets + query0 * a.bucket_stride[1];         // uniform; the lane's key and half are an offset
-    if (query0 + ROWS <= a.n_q) {
+    const int left = a.n_q - 1 - r % per_head * ROWS, key0 = tile * 32 * W + block_key;
+    const signed char* const at = buckets + (long)(r % per_head * ROWS) * a.bucket_stride[1] + tile * 32 * W;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) n_of[i] = (unsigned char)(at + (8 * (i / 4) + i % 4) * a.bucket_stride[1])[bucket_offset];
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        n_of[i] = (unsigned char)at[(unsigned)(min(8 * (i / 4) + 4 * half + i % 4, a.n_q - 1 - query0) * (int)a.bucket_stride[1] + key)];
+    for (int i = 0; i < 4; ++i) {
+      const signed char* const from = at + (unsigned)(min(block_query + i, left) * (int)a.bucket_stride[1] + block_key);
+      if (key0 + 4 <= a.n_k) __builtin_memcpy(&bucket_words[i], from, 4);
+      else {
+        bucket_words[i] = 0;
+        for (int e = 0; e < 4; ++e) bucket_words[i] |= (key0 + e < a.n_k ? (unsigned)(unsigned char)from[e] : 255u) << (8 * e);
+      }
     }
+  };
+  const auto write_buckets = [&](int r) {
+    unsigned* const to = lds_buckets + (r - first) % 2 * 32 * W * BUCKET_LD + block_key * BUCKET_LD + block_query / 4;
+    const unsigned a0 = __builtin_amdgcn_perm(bucket_words[1], bucket_words[0], 0x05010400u), a1 = __builtin_amdgcn_perm(bucket_words[1], bucket_words[0], 0x07030602u);
+    const unsigned b0 = __builtin_amdgcn_perm(bucket_words[3], bucket_words[2], 0x05010400u), b1 = __builtin_amdgcn_perm(bucket_words[3], bucket_words[2], 0x07030602u);
+    to[0] = __builtin_amdgcn_perm(b0, a0, 0x05040100u);
+    to[BUCKET_LD] = __builtin_amdgcn_perm(b0, a0, 0x07060302u);
+    to[2 * BUCKET_LD] = __builtin_amdgcn_perm(b1, a1, 0x05040100u);
+    to[3 * BUCKET_LD] = __builtin_amdgcn_perm(b1, a1, 0x07060302u);
   };
   if (W > 1 && first < last) fetch(first);
   if (buckets && first < last) fetch_buckets(first);
@@ -346,6 +342,8 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     __syncthreads();
     if (first < last) write(first);
     if (first + 1 < last) fetch(first + 1);
+    if (buckets && first < last) write_buckets(first);
+    if (buckets && first + 1 < last) fetch_buckets(first + 1);
   }
 
   v16f dk[D / 32] = {}, dv[D / 32] = {};
@@ -358,12 +356,25 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     __syncthreads();
     if (BUFS == 1) {
       write(r);
+      if (buckets) write_buckets(r);
       __syncthreads();
     }
     const float* const table = lds_table + r / per_head * (a.n_buckets + 1);
 
-    // float32: the scores start from -m; dp starts from -delta
+    // the scores start from the table's entries (float32: less m), dp from -delta
     v16f s = {}, dp;
+    if (buckets) {
+      const unsigned* const words = lds_buckets + ((r - first) % 2 * 32 * W + wave * 32 + (lane & 31)) * BUCKET_LD + half;
+      float t[16];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const unsigned word = words[2 * g];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[4 * g + i] = table[bucket_of(word, i, a.n_buckets)];
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) s[j] = T::PARTS == 3 ? t[j] : t[j] * p.inv_c;
+    }
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       float start[4];
@@ -373,25 +384,23 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
       if constexpr (T::PARTS == 3) {
         read16(rows + 8 * g + 4 * half, start);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[4 * g + i] = start[i];
+        for (int i = 0; i < 4; ++i) s[4 * g + i] += start[i];
       }
     }
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) mma<T>(Tl::by_rows(lds_q, i, lane), kf[i], s);
-    if constexpr (T::PARTS * D > 256) __builtin_amdgcn_sched_barrier(0);     // no operand of a later product is read before: registers
+    if constexpr (T::PARTS * D > 128) __builtin_amdgcn_sched_barrier(0);     // no operand of a later product is read before: registers
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) mma<T>(Tl::by_rows(lds_g, i, lane), vf[i], dp);
-    if constexpr (T::PARTS * D > 256) __builtin_amdgcn_sched_barrier(0);     // no operand of a later product is read before: registers
-    if (BUFS == 2 && r + 1 < last) write(r + 1);
+    if constexpr (T::PARTS * D > 128) __builtin_amdgcn_sched_barrier(0);     // no operand of a later product is read before: registers
+    if (BUFS == 2 && r + 1 < last) {
+      write(r + 1);
+      if (buckets) write_buckets(r + 1);
+    }
     Row next = {};
     if (W > 1 && r + BUFS < last) fetch(r + BUFS);
     if (tid < ROWS) next = row_of(r + 2);
-    float bias[16];
-    if (buckets) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) bias[i] = table[min((int)n_of[i], a.n_buckets)];
-      if (r + 1 < last) fetch_buckets(r + 1);
-    }
+    if (buckets && r + BUFS < last) fetch_buckets(r + BUFS);
 
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
@@ -404,8 +413,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int j = 4 * g + i + e;
-          const float x = T::PARTS == 3 ? (buckets ? s[j] + bias[j] : s[j]) + kb : ((buckets ? fmaf(s[j], p.c, bias[j]) : s[j] * p.c) + kb) + ms[i + e];
-          pr[e] = exp2_(x);
+          pr[e] = exp2_(T::PARTS == 3 ? s[j] + kb : fmaf(s[j], p.c, kb) + ms[i + e]);
         }
         round_pair<T>(pr[0], pr[1]);
 #pragma unroll
@@ -416,7 +424,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
         }
       }
     }
-    if constexpr (T::PARTS * D > 256) __builtin_amdgcn_sched_barrier(0);     // no operand of a later product is read before: registers
+    if constexpr (T::PARTS * D > 128) __builtin_amdgcn_sched_barrier(0);     // no operand of a later product is read before: registers
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const Frag<T> pf = cut_rows<T>(s, t), df = cut_rows<T>(dp, t);
@@ -493,7 +501,7 @@ template <class T, int D> void backward_d(Args& p, const Plans& plans, float* pa
                        plans.grad_q.splits * plans.grad_q.tiles, a.n_buckets, static_cast<typename T::type*>(a.gtable));
   if (!a.gk) return;
   use(plans.grad_kv, partial_kv);
-  const size_t lds_kv = (plans.grad_kv.waves == 1 ? kv_buffers<T, D, 1>() : kv_buffers<T, D, 4>()) * 4 * Tile<T, D>::BYTES + (3 * RING * ROWS + (a.buckets ? a.heads / a.kv_heads * (a.n_buckets + 1) : 0)) * sizeof(float);
+  const size_t lds_kv = (plans.grad_kv.waves == 1 ? kv_buffers<T, D, 1>() : kv_buffers<T, D, 4>()) * 4 * Tile<T, D>::BYTES + (3 * RING * ROWS + 2 * 32 * plans.grad_kv.waves * BUCKET_LD + (a.buckets ? a.heads / a.kv_heads * (a.n_buckets + 1) : 0)) * sizeof(float);
   if constexpr (few_waves<T, D>) {
     if (plans.grad_kv.waves == 1) launch(grad_kv_kernel<T, D, 1>, p, 1, lds_kv, stream);
   }

@@ -87,32 +87,17 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     const float* const kb = lds_kb + step % RING * ROWS;
 
     v16f s;
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      float start[4];
-      read16(kb + 8 * g + 4 * half, start);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[4 * g + i] = start[i];
-    }
+    start_scores<T>(s, kb, half, buckets != nullptr, words, table, a.n_buckets, p.inv_c);
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) mma<T>(Tl::by_rows(lds_k, i, lane), qf[i], s);
     if (BUFS == 2 && more) write(step + 1);
-    unsigned now[4];
-#pragma unroll
-    for (int g = 0; g < 4; ++g) now[g] = words[g];
     float kb_next = 0.f;
     if (W > 1 && key + BUFS * ROWS < end) stage.fetch(k, v, key + BUFS * ROWS, tid);
     if (more && buckets) load_buckets(buckets, key + ROWS, end, half, words);
     if (tid < ROWS) kb_next = key_value(key_bias, key + 2 * ROWS + tid, end, p.inv_c);
 
     float top = ninf();
-    if (buckets) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float t = table[bucket_of(now[r / 4], r % 4, a.n_buckets)];
-        s[r] = T::PARTS == 3 ? s[r] + t : fmaf(s[r], p.c, t);
-      }
-    } else if (T::PARTS == 1) {
+    if constexpr (T::PARTS == 1) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] *= p.c;
     }
@@ -120,12 +105,10 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
     top = ceilf(fmaxf(half_max(top), m));
     const float ref = (top == ninf() ? 0.f : top) - SHIFT;
-    if (__any(top > m)) {
-      const float fade = exp2_(m - SHIFT - ref);      // a power of two
-      l *= fade;
+    const float fade = exp2_(m - SHIFT - ref);      // a power of two
+    l *= fade;
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) o[i] *= fade;
-    }
+    for (int i = 0; i < D / 32; ++i) o[i] *= fade;
     m = top;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
