@@ -20,7 +20,7 @@ Plan plan(long columns, long groups, long long_tiles, bool few) {
   Plan p;
   p.waves = few && columns <= 32 ? 1 : 4;
   p.tiles = columns < 1 ? 1 : (int)((columns + 32 * p.waves - 1) / (32 * p.waves));
-  const long base = p.tiles * groups, want = p.waves == 1 ? 4 * CUS : 2 * CUS;
+  const long base = p.tiles * groups, want = p.waves == 1 ? 6 * CUS : 2 * CUS;
   long splits = base > CUS ? 1 : (want + base - 1) / base;
   if (splits > long_tiles / 4) splits = long_tiles / 4;
   p.splits = splits < 1 ? 1 : (int)splits;

@@ -10,7 +10,7 @@
 namespace s2cnn {
 namespace attn {
 
-template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS * D > 192 ? 1 : 2) void forward_kernel(Args p) {
+template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS * D > 192 ? 1 : T::PARTS * D > 64 || W == 1 ? 2 : 4) void forward_kernel(Args p) {
   typedef Tile<T, D> Tl;
   constexpr int BUFS = buffers<T, D, W>(2), BUF = 2 * Tl::BYTES;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -158,50 +158,62 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
   if (half == 0 && a.stats) reinterpret_cast<float2*>(a.stats)[row] = any ? make_float2(m - SHIFT, inv) : make_float2(pinf(), 0.f);
 }
 
-// One wave joins the parts of one query.
+// A workgroup joins the parts of one query, a quarter of them per wave: lane s of a wave has the maximum and the sum of its part s (of 64
+// at a time), and so its weight, 2^(its maximum - the maximum of all).
 template <class T, int D> __global__ __launch_bounds__(256) void join_kernel(Args p) {
+  __shared__ float lds_o[4][D], lds_l[4];
   const s2cnn_attention_t& a = p.a;
-  const long rows = (long)a.batch * a.heads * a.n_q, row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= rows) return;
-  const int lane = threadIdx.x & 63;
+  const long rows = (long)a.batch * a.heads * a.n_q, row = blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const float* const part = p.partial;
   const float2* const ml = reinterpret_cast<const float2*>(part + p.splits * rows * D);
   constexpr float SHIFT = T::HALF ? 10.f : 0.f;
-  // lane s has the maximum and the sum of part s (of 64 parts at a time): its weight, 2^(its maximum - the maximum of all)
+  constexpr int PER = (D + 63) / 64;
   float m = ninf();
   for (int s = lane; s < p.splits; s += 64) m = fmaxf(m, ml[s * rows + row].x);
 #pragma unroll
   for (int i = 32; i; i >>= 1) m = fmaxf(m, __shfl_xor(m, i));
   const float ref = m == ninf() ? 0.f : m;
-  float l = 0.f, o[(D + 63) / 64] = {};
-  for (int s0 = 0; s0 < p.splits; s0 += 64) {
+  const int per_wave = (p.splits + 3) / 4, first = wave * per_wave, last = min(p.splits, first + per_wave);
+  float l = 0.f, o[PER] = {};
+  for (int s0 = first; s0 < last; s0 += 64) {
     float w = 0.f;
-    if (s0 + lane < p.splits) {
+    if (s0 + lane < last) {
       const float2 x = ml[(s0 + lane) * rows + row];
       w = exp2_(x.x - ref);
       l = fmaf(x.y, w, l);
     }
-    const int n = min(64, p.splits - s0);
+    const int n = min(64, last - s0);
 #pragma unroll 8
     for (int s = 0; s < n; ++s) {
       const float ws = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), s));
 #pragma unroll
-      for (int i = 0; i < (D + 63) / 64; ++i)
-        if (lane + 64 * i < a.d) o[i] = fmaf(part[((s0 + s) * rows + row) * D + slot_of(lane + 64 * i, a.d)], ws, o[i]);
+      for (int i = 0; i < PER; ++i)
+        if (lane + 64 * i < D) o[i] = fmaf(part[((s0 + s) * rows + row) * D + lane + 64 * i], ws, o[i]);
     }
   }
 #pragma unroll
   for (int i = 32; i; i >>= 1) l += __shfl_xor(l, i);
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    if (lane + 64 * i < D) lds_o[wave][lane + 64 * i] = o[i];
+  if (lane == 0) lds_l[wave] = l;
+  __syncthreads();
+  if (wave) return;
+  l = (lds_l[0] + lds_l[1]) + (lds_l[2] + lds_l[3]);
   const bool any = l != 0.f;
   const float inv = any ? 1.f / l : 0.f;
   const int query = (int)(row % a.n_q), head = (int)(row / a.n_q % a.heads), b = (int)(row / a.n_q / a.heads);
   const long at = b * a.out_stride[0] + head * a.out_stride[1] + query * a.out_stride[2];
   typedef typename T::type E;
 #pragma unroll
-  for (int i = 0; i < (D + 63) / 64; ++i) {
-    if (lane + 64 * i >= a.d) continue;
-    static_cast<E*>(a.out)[at + lane + 64 * i] = (E)(o[i] * inv);
-    if (T::PARTS == 1 && a.out_f32) a.out_f32[row * a.d + lane + 64 * i] = o[i] * inv;
+  for (int i = 0; i < PER; ++i) {
+    const int e = lane + 64 * i;
+    if (e >= a.d) continue;
+    const int slot = slot_of(e, a.d);
+    const float x = ((lds_o[0][slot] + lds_o[1][slot]) + (lds_o[2][slot] + lds_o[3][slot])) * inv;
+    static_cast<E*>(a.out)[at + e] = (E)x;
+    if (T::PARTS == 1 && a.out_f32) a.out_f32[row * a.d + e] = x;
   }
   if (lane == 0 && a.stats) reinterpret_cast<float2*>(a.stats)[row] = any ? make_float2(m - SHIFT, inv) : make_float2(pinf(), 0.f);
 }
@@ -216,7 +228,7 @@ template <class T, int D> void forward_d(const Args& p, const Plans& plans, hipS
   }
   if (f.waves != 1) launch(forward_kernel<T, D, 4>, p, 4, lds, stream);
   if (f.splits > 1)
-    hipLaunchKernelGGL((join_kernel<T, D>), dim3((unsigned)(((long)a.batch * a.heads * a.n_q + 3) / 4)), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((join_kernel<T, D>), dim3((unsigned)((long)a.batch * a.heads * a.n_q)), dim3(256), 0, stream, p);
 }
 template <class T> void forward(const Args& p, const Plans& plans, hipStream_t stream) {
   if (plans.D == 32) forward_d<T, 32>(p, plans, stream);

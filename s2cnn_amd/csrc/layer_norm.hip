@@ -401,7 +401,7 @@ constexpr int CUS = 256;
 
 int group_of(int dtype, int features) {              // lanes of a row
   const int chunks = (features + (dtype == S2CNN_F32 ? 3 : 7)) / (dtype == S2CNN_F32 ? 4 : 8);
-  return chunks <= 32 ? 8 : chunks <= 64 ? 16 : chunks <= 128 ? 32 : chunks <= 256 ? 64 : 256;
+  return chunks <= 16 ? 8 : chunks <= 32 ? 16 : chunks <= 64 ? 32 : chunks <= 256 ? 64 : 256;
 }
 bool is_long(int dtype, int features) { return features > (dtype == S2CNN_F32 ? 4096 : 8192); }
 // Workgroups that run over all rows.  Backward: their number is that of the partial sums, two a CU; forward: eight a CU.
@@ -425,9 +425,9 @@ template <class T, bool STEP, class P> void dispatch(const P& p, int wgs, hipStr
   const int chunks = (p.features + Chunk<T>::N - 1) / Chunk<T>::N;
   if (chunks <= 8) launch<T, 8, 1, STEP>(p, wgs, s);
   else if (chunks <= 16) launch<T, 8, 2, STEP>(p, wgs, s);
-  else if (chunks <= 32) launch<T, 8, 4, STEP>(p, wgs, s);
-  else if (chunks <= 64) launch<T, 16, 4, STEP>(p, wgs, s);
-  else if (chunks <= 128) launch<T, 32, 4, STEP>(p, wgs, s);
+  else if (chunks <= 32) launch<T, 16, 2, STEP>(p, wgs, s);
+  else if (chunks <= 64) launch<T, 32, 2, STEP>(p, wgs, s);
+  else if (chunks <= 128) launch<T, 64, 2, STEP>(p, wgs, s);
   else if (chunks <= 256) launch<T, 64, 4, STEP>(p, wgs, s);
   else if (chunks <= 1024) launch<T, 256, 4, STEP>(p, wgs, s);
   else launch<T, 256, 4, STEP, true>(p, wgs, s);
