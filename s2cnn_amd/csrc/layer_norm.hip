@@ -53,11 +53,16 @@ template <class T, class T2> struct Chunk16 {
 template <> struct Chunk<__bf16> : Chunk16<__bf16, bf2> {};
 template <> struct Chunk<half_t> : Chunk16<half_t, h2> {};
 
+typedef unsigned loose4 __attribute__((ext_vector_type(4), aligned(2)));    // 16 bytes at any entry
 // The n first entries of a chunk at p (any alignment of the type's: rows of odd length), the others zero.
-template <class T> __device__ __forceinline__ uint4 load_chunk(const T* p, int n) {
+template <class T> __device__ __forceinline__ uint4 load_chunk(const T* p, int n, bool stream = false) {
   constexpr int N = Chunk<T>::N;
   uint4 u = make_uint4(0, 0, 0, 0);
   if (n >= N) {
+    if (stream) {
+      const loose4 x = __builtin_nontemporal_load(reinterpret_cast<const loose4*>(p));
+      return make_uint4(x[0], x[1], x[2], x[3]);
+    }
     __builtin_memcpy(&u, p, 16);
     return u;
   }
@@ -77,10 +82,11 @@ template <class T> __device__ __forceinline__ uint4 load_chunk(const T* p, int n
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
-template <class T> __device__ __forceinline__ void store_chunk(T* p, int n, const float (&v)[Chunk<T>::N]) {
+template <class T> __device__ __forceinline__ void store_chunk(T* p, int n, const float (&v)[Chunk<T>::N], bool stream = false) {
   if (n >= Chunk<T>::N) {
     const uint4 u = Chunk<T>::put(v);
-    __builtin_memcpy(p, &u, 16);
+    if (stream) __builtin_nontemporal_store(loose4{u.x, u.y, u.z, u.w}, reinterpret_cast<loose4*>(p));
+    else __builtin_memcpy(p, &u, 16);
     return;
   }
 #pragma unroll
@@ -162,6 +168,18 @@ template <class T, int L, int K, bool STEP, bool LONG> __global__ __launch_bound
     }
   };
 
+  uint4 wraw[K], braw[K];                                           // loads in the loop would wait for those of the rows
+  const auto fetch_weights = [&](int pass) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (pass * K + k) * L + lane, n = p.features - c * C::N;
+      wraw[k] = braw[k] = make_uint4(0, 0, 0, 0);
+      if (w && c < chunks) wraw[k] = load_chunk<T>(w + c * C::N, n);
+      if (b && c < chunks) braw[k] = load_chunk<T>(b + c * C::N, n);
+    }
+  };
+  if (!LONG) fetch_weights(0);
+
   for (long row0 = (long)blockIdx.x * (THREADS / L); row0 < p.rows; row0 += (long)gridDim.x * (THREADS / L)) {
     const long row = row0 + threadIdx.x / L;
     const bool ok = row < p.rows;
@@ -193,6 +211,7 @@ template <class T, int L, int K, bool STEP, bool LONG> __global__ __launch_bound
     }
     const float rstd = 1.f / sqrtf(fmaf(sum_group<L>(square, slots[1]), inv_n, p.eps));
     for (int pass = 0; pass < passes; ++pass) {
+      if (LONG) fetch_weights(pass);
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         const int c = (pass * K + k) * L + lane, n = p.features - c * C::N;
@@ -201,8 +220,8 @@ template <class T, int L, int K, bool STEP, bool LONG> __global__ __launch_bound
         const long at = r * p.features + (long)c * C::N;
         if constexpr (STEP) store_chunk<T>(static_cast<T*>(p.h) + at, n, v[k]);
         float ws[C::N], bs[C::N], y[C::N];
-        if (w) C::get(load_chunk<T>(w + c * C::N, n), ws);
-        if (b) C::get(load_chunk<T>(b + c * C::N, n), bs);
+        C::get(wraw[k], ws);
+        C::get(braw[k], bs);
 #pragma unroll
         for (int i = 0; i < C::N; ++i) {
           y[i] = (v[k][i] - mean) * rstd;
@@ -227,19 +246,44 @@ template <class T, int L, int K, bool STEP, bool LONG> __global__ __launch_bound
   const T* const gs = static_cast<const T*>(p.g);
   const float inv_n = 1.f / (float)p.features;
   float gw[K][C::N] = {}, gb[K][C::N] = {};
+  uint4 hnext[K], gnext[K], wraw[K];                                // the group's next row; the weights, whose loads in the loop would wait for it
+  float2 stnext = make_float2(0.f, 0.f);
+  const auto fetch_weights = [&](int pass) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (pass * K + k) * L + lane;
+      wraw[k] = w && c < chunks ? load_chunk<T>(w + c * C::N, p.features - c * C::N) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  const auto fetch = [&](long row, int pass, uint4 (&h)[K], uint4 (&g)[K]) {
+    const long r = row < p.rows ? row : p.rows - 1;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (pass * K + k) * L + lane, n = p.features - c * C::N;
+      h[k] = g[k] = make_uint4(0, 0, 0, 0);
+      if (c >= chunks) continue;
+      h[k] = load_chunk<T>(hs + r * p.features + (long)c * C::N, n);
+      g[k] = load_chunk<T>(gs + r * p.features + (long)c * C::N, n);
+    }
+  };
+  if (!LONG) {
+    fetch_weights(0);
+    fetch((long)blockIdx.x * (THREADS / L) + threadIdx.x / L, 0, hnext, gnext);
+    stnext = reinterpret_cast<const float2*>(p.stats)[min((long)blockIdx.x * (THREADS / L) + threadIdx.x / L, p.rows - 1)];
+  }
 
   for (long row0 = (long)blockIdx.x * (THREADS / L); row0 < p.rows; row0 += (long)gridDim.x * (THREADS / L)) {
     const long row = row0 + threadIdx.x / L;
     const bool ok = row < p.rows;
     const long r = ok ? row : p.rows - 1;
-    const float2 st = reinterpret_cast<const float2*>(p.stats)[r];
+    const float2 st = LONG ? reinterpret_cast<const float2*>(p.stats)[r] : stnext;
     uint4 hraw[K], graw[K];
     float a = 0.f, c2 = 0.f;
-    const auto form = [&](int c, const uint4& hr, const uint4& gr, float (&xh)[C::N], float (&g)[C::N], float (&u)[C::N]) {
-      C::get(hr, xh);
-      C::get(gr, g);
+    const auto form = [&](int k, float (&xh)[C::N], float (&g)[C::N], float (&u)[C::N]) {
+      C::get(hraw[k], xh);
+      C::get(graw[k], g);
       float ws[C::N];
-      if (w) C::get(load_chunk<T>(w + c * C::N, p.features - c * C::N), ws);
+      C::get(wraw[k], ws);
 #pragma unroll
       for (int i = 0; i < C::N; ++i) {
         xh[i] = (xh[i] - st.x) * st.y;
@@ -247,20 +291,21 @@ template <class T, int L, int K, bool STEP, bool LONG> __global__ __launch_bound
       }
     };
     for (int pass = 0; pass < passes; ++pass) {
+      if (LONG) fetch(r, pass, hraw, graw);
+      else {
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const int c = (pass * K + k) * L + lane, n = p.features - c * C::N;
-        hraw[k] = graw[k] = make_uint4(0, 0, 0, 0);
-        if (c >= chunks) continue;
-        hraw[k] = load_chunk<T>(hs + r * p.features + (long)c * C::N, n);
-        graw[k] = load_chunk<T>(gs + r * p.features + (long)c * C::N, n);
+        for (int k = 0; k < K; ++k) hraw[k] = hnext[k], graw[k] = gnext[k];
+        const long next = row + (long)gridDim.x * (THREADS / L);
+        fetch(next, 0, hnext, gnext);
+        stnext = reinterpret_cast<const float2*>(p.stats)[next < p.rows ? next : p.rows - 1];
       }
+      if (LONG) fetch_weights(pass);
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         const int c = (pass * K + k) * L + lane;
         if (c >= chunks) continue;
         float xh[C::N], g[C::N], u[C::N];
-        form(c, hraw[k], graw[k], xh, g, u);                        // entries past the row's end: g = u = 0
+        form(k, xh, g, u);                        // entries past the row's end: g = u = 0
 #pragma unroll
         for (int i = 0; i < C::N; ++i) {
           a += u[i];
@@ -277,9 +322,9 @@ template <class T, int L, int K, bool STEP, bool LONG> __global__ __launch_bound
         const int c = (pass * K + k) * L + lane, n = p.features - c * C::N;
         if (c >= chunks || !ok) continue;
         const long at = r * p.features + (long)c * C::N;
-        if (LONG) hraw[k] = load_chunk<T>(hs + at, n), graw[k] = load_chunk<T>(gs + at, n);
+        if (LONG) hraw[k] = load_chunk<T>(hs + at, n), graw[k] = load_chunk<T>(gs + at, n), wraw[k] = w ? load_chunk<T>(w + c * C::N, n) : make_uint4(0, 0, 0, 0);
         float xh[C::N], g[C::N], u[C::N];
-        form(c, hraw[k], graw[k], xh, g, u);
+        form(k, xh, g, u);
 #pragma unroll
         for (int i = 0; i < C::N; ++i) u[i] = st.y * (u[i] - a - xh[i] * c2);
         if constexpr (STEP) {
@@ -372,26 +417,45 @@ template <class T> __global__ __launch_bounds__(1024) void sum_kernel(const floa
   }
 }
 
-// y = x times the factor of each element; 8 elements a thread, one counter
-template <class T> __global__ __launch_bounds__(THREADS) void dropout_kernel(const T* x, T* y, long n, Dropout d) {
+// Dropout of a tensor.  16-bit types: a lane's 16 bytes are the eight elements of a counter.  float32: they are four, and two
+// neighbouring lanes have the halves of one; a lane takes two chunks, 64 lanes apart, the even one forms the counter of the first and the
+// odd one that of the second, and they exchange halves, so that accesses stay contiguous and no counter is formed twice.
+template <class T> __global__ __launch_bounds__(THREADS) void dropout_kernel(const T* x, T* y, long n, Dropout d, bool stream) {
   typedef Chunk<T> C;
+  constexpr int PER = 8 / C::N;                                     // chunks a lane, 64 lanes apart
   const unsigned long long key = dropout_seed(d);
-  const long stride = (long)gridDim.x * THREADS * 8;
-  for (long at = ((long)blockIdx.x * THREADS + threadIdx.x) * 8; at < n; at += stride) {
-    uint4 raw[8 / C::N];
+  const int lane = threadIdx.x & 63;
+  for (long first = ((long)blockIdx.x * THREADS + (threadIdx.x & ~63)) * 8; first < n; first += (long)gridDim.x * THREADS * 8) {     // the wave's
+    uint4 raw[PER];
+    long left[PER];
 #pragma unroll
-    for (int k = 0; k < 8 / C::N; ++k) {
-      const long left = n - at - k * C::N;
-      raw[k] = left > 0 ? load_chunk<T>(x + at + k * C::N, (int)min(left, 8L)) : make_uint4(0, 0, 0, 0);
+    for (int k = 0; k < PER; ++k) {
+      const long at = first + (k * 64 + lane) * C::N;
+      left[k] = n - at;
+      raw[k] = left[k] > 0 ? load_chunk<T>(x + at, (int)min(left[k], 8L), stream) : make_uint4(0, 0, 0, 0);
     }
-    float v[8];
+    unsigned w[PER][C::N / 2];                                      // 16 bits an element
+    if (d.on) {
+      if constexpr (PER == 1) {
+        const uint4 r = philox((unsigned long long)(first + lane * 8) >> 3, key);
+        w[0][0] = r.x, w[0][1] = r.y, w[0][2] = r.z, w[0][3] = r.w;
+      } else {
+        const bool odd = lane & 1;
+        const uint4 r = philox((unsigned long long)(first + ((odd ? 64 : 0) + (lane & ~1)) * 4) >> 3, key);
+        const unsigned s0 = __builtin_amdgcn_update_dpp(0, odd ? r.x : r.z, 0xB1, 0xf, 0xf, true), s1 = __builtin_amdgcn_update_dpp(0, odd ? r.y : r.w, 0xB1, 0xf, 0xf, true);
+        w[0][0] = odd ? s0 : r.x, w[0][1] = odd ? s1 : r.y;
+        w[1][0] = odd ? r.z : s0, w[1][1] = odd ? r.w : s1;
+      }
+    }
 #pragma unroll
-    for (int k = 0; k < 8 / C::N; ++k) C::get(raw[k], reinterpret_cast<float (&)[C::N]>(v[k * C::N]));
-    if (d.on) drop<8>(d, key, at, v);
+    for (int k = 0; k < PER; ++k) {
+      float v[C::N];
+      C::get(raw[k], v);
+      if (d.on) {
 #pragma unroll
-    for (int k = 0; k < 8 / C::N; ++k) {
-      const long left = n - at - k * C::N;
-      if (left > 0) store_chunk<T>(y + at + k * C::N, (int)min(left, 8L), reinterpret_cast<float (&)[C::N]>(v[k * C::N]));
+        for (int i = 0; i < C::N; ++i) v[i] = ((w[k][i / 2] >> (16 * (i % 2))) & 0xffffu) >= d.threshold ? v[i] * d.factor : 0.f;
+      }
+      if (left[k] > 0) store_chunk<T>(y + first + (k * 64 + lane) * C::N, (int)min(left[k], 8L), v, stream);
     }
   }
 }
@@ -448,7 +512,8 @@ template <class T> void backward(const Backward& p, bool step, int dtype, void* 
 }
 template <class T> void dropout(const void* x, void* y, long n, const Dropout& d, hipStream_t s) {
   const long need = (n + 8 * THREADS - 1) / (8 * THREADS), most = CUS * 16;
-  hipLaunchKernelGGL(dropout_kernel<T>, dim3((unsigned)(need < most ? need : most)), dim3(THREADS), 0, s, static_cast<const T*>(x), static_cast<T*>(y), n, d);
+  hipLaunchKernelGGL(dropout_kernel<T>, dim3((unsigned)(need < most ? need : most)), dim3(THREADS), 0, s, static_cast<const T*>(x), static_cast<T*>(y), n, d,
+                     (size_t)n * sizeof(T) >= STREAM_BYTES);
 }
 
 bool sizes_ok(long rows, long features, int dtype) {
