@@ -203,26 +203,30 @@ FLOATS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}     # S2CNN_F32
 def require_gpu_float(*tensors):
     """Operands of the operators that take three types: float32, bfloat16 or float16, all the same, on the current GPU.
     None is passed over.  Returns the type's number in the library."""
-    dtype = tensors[0].dtype
+    dtype, device = tensors[0].dtype, torch._C._cuda_getDevice() if tensors[0].is_cuda else -1
+    if dtype not in FLOATS or device < 0:
+        raise RuntimeError("float32, bfloat16 or float16 tensors on the GPU only (got %s on %s); there is no CPU path" % (dtype, tensors[0].device))
     for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda or dtype not in FLOATS:
-            raise RuntimeError("float32, bfloat16 or float16 tensors on the GPU only (got %s on %s); there is no CPU path" % (t.dtype, t.device))
-        if t.dtype != dtype:
-            raise RuntimeError("operands of one type only (got %s and %s)" % (dtype, t.dtype))
-        _require_current_device(t)
+        if t is not None and (t.dtype != dtype or t.get_device() != device):
+            if t.dtype != dtype:
+                raise RuntimeError("operands of one type only (got %s and %s)" % (dtype, t.dtype))
+            _refuse_device(t)
     return FLOATS[dtype]
 
 
-def require_gpu_of(dtype, *tensors):
-    """Operands of a fixed type on the current GPU; None is passed over."""
-    for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda or t.dtype != dtype:
-            raise RuntimeError("expected a %s tensor on the GPU (got %s on %s); there is no CPU path" % (dtype, t.dtype, t.device))
-        _require_current_device(t)
+def require_gpu_of(dtype, t):
+    """An operand of a fixed type on the current GPU, or None."""
+    if t is not None:
+        if t.dtype != dtype:
+            raise RuntimeError("expected a %s tensor (got %s)" % (dtype, t.dtype))
+        if not t.is_cuda or t.get_device() != torch._C._cuda_getDevice():
+            _refuse_device(t)
+
+
+def _refuse_device(t):
+    if not t.is_cuda:
+        raise RuntimeError("expected a tensor on the GPU (got one on %s); there is no CPU path" % t.device)
+    _require_current_device(t)
 
 
 def ptr_or_none(t):

@@ -8,6 +8,7 @@ logarithm of the quadrature weights as `key_bias` the sum over keys is the integ
 """
 import ctypes
 import math
+from functools import lru_cache
 
 import numpy as np
 import torch
@@ -17,10 +18,6 @@ from . import _hip
 
 MAX_HEAD = 128
 MAX_BUCKETS = 64
-
-
-def _unit_last(t):
-    return t if t.stride(-1) == 1 or t.size(-1) == 1 else t.contiguous()
 
 
 def _vectors(t):
@@ -34,32 +31,34 @@ def _like(t):
     return out if out.stride(-1) == 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
-def _strides(t):
-    """Strides of (batch, head, vector); 0 for an axis of one entry, whatever the tensor says."""
-    return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape[:3]))
-
-
-def _describe(q, k, v, table, buckets, key_bias, lengths, scale, dtype):
+@lru_cache(maxsize=1024)
+def _plan(shape_q, shape_k, strides, bucket_stride, key_bias_stride, n_buckets, dtype, scale, backward):
+    """(the library's struct without its pointers, floats of the statistics, bytes of the workspace) of a call of these sizes.
+    strides: of q, k, v, out and, backward, the gradients of out, q, k, v, as torch gives them."""
     a = _hip.Attention()
-    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    a.q_stride[:], a.k_stride[:], a.v_stride[:] = _strides(q), _strides(k), _strides(v)
-    a.batch, a.heads, a.n_q, a.d = q.shape
-    a.kv_heads, a.n_k = k.size(1), k.size(2)
-    a.dtype, a.scale = dtype, scale
-    if table is not None:
-        a.table, a.buckets, a.n_buckets = table.data_ptr(), buckets.data_ptr(), table.size(1)
-        a.bucket_stride[:] = (buckets.stride(0) if buckets.dim() == 3 else 0, buckets.stride(-2))
-    if key_bias is not None:
-        a.key_bias, a.key_bias_stride = key_bias.data_ptr(), key_bias.stride(0) if key_bias.dim() == 2 else 0
-    if lengths is not None:
-        a.lengths = lengths.data_ptr()
-    return a
+    a.batch, a.heads, a.n_q, a.d = shape_q
+    a.kv_heads, a.n_k = shape_k[1], shape_k[2]
+    a.dtype, a.scale, a.n_buckets = dtype, scale, n_buckets
+    a.bucket_stride[:], a.key_bias_stride = bucket_stride, key_bias_stride
+    queries, keys = shape_q[:3], shape_k[:3]
+    for name, shape, stride in zip(("q", "k", "v", "out", "gout", "gq", "gk", "gv"), (queries, keys, keys, queries, queries, queries, keys, keys), strides):
+        # 0 for an axis of one entry, whatever the tensor says
+        getattr(a, name + "_stride")[:] = tuple(s if n > 1 else 0 for s, n in zip(stride, shape))
+    if n_buckets:
+        a.table = a.buckets = 16                          # some address: the sizes depend on there being one
+    lib, ref = _hip.lib(), ctypes.byref(a)
+    sizes = lib.s2cnn_attention_stats_floats(ref), lib.s2cnn_attention_workspace(ref, backward)
+    a.table = a.buckets = None
+    return (bytes(a), *sizes)
 
 
-def _run(name, a, backward, device):
-    nbytes = _hip.lib().s2cnn_attention_workspace(ctypes.byref(a), backward)
-    ws = _hip.workspace(nbytes, device) if nbytes else None
-    _hip.call(name, ctypes.byref(a), _hip.ptr(ws) if nbytes else None, nbytes, _hip.stream_ptr())
+def _run(name, plan, device, **pointers):
+    a = _hip.Attention.from_buffer_copy(plan[0])
+    for field, tensor in pointers.items():
+        if tensor is not None:
+            setattr(a, field, tensor.data_ptr())
+    ws = _hip.workspace(plan[2], device) if plan[2] else None
+    _hip.call(name, ctypes.byref(a), _hip.ptr_or_none(ws), plan[2], _hip.stream_ptr())
 
 
 class _Attention(torch.autograd.Function):
@@ -67,44 +66,39 @@ class _Attention(torch.autograd.Function):
     def forward(ctx, q, k, v, table, buckets, key_bias, lengths, scale, dtype, needs_grad):  # pylint: disable=W
         q, k, v = _vectors(q), _vectors(k), _vectors(v)
         out = _like(q)
-        stats = None
-        exact = q.new_empty(q.shape, dtype=torch.float32) if needs_grad and q.dtype != torch.float32 else None     # out before its rounding
+        sizes = ((buckets.stride(0) if buckets.dim() == 3 else 0, buckets.stride(-2)) if buckets is not None else (0, 0),
+                 key_bias.stride(0) if key_bias is not None and key_bias.dim() == 2 else 0,
+                 table.size(1) if table is not None else 0, dtype, scale)
+        stats = exact = None
         if out.numel():
-            a = _describe(q, k, v, table, buckets, key_bias, lengths, scale, dtype)
-            a.out, a.out_stride[:] = out.data_ptr(), _strides(out)
+            plan = _plan(q.shape, k.shape, (q.stride(), k.stride(), v.stride(), out.stride()), *sizes, 0)
             if needs_grad:
-                stats = q.new_empty(_hip.lib().s2cnn_attention_stats_floats(ctypes.byref(a)), dtype=torch.float32)
-                a.stats, a.out_f32 = stats.data_ptr(), exact.data_ptr() if exact is not None else None
-            _run("s2cnn_attention_fwd", a, 0, q.device)
+                stats = q.new_empty(plan[1], dtype=torch.float32)
+                exact = q.new_empty(q.shape, dtype=torch.float32) if dtype else None         # out before its rounding
+            _run("s2cnn_attention_fwd", plan, q.device, q=q, k=k, v=v, table=table, buckets=buckets, key_bias=key_bias, lengths=lengths, out=out,
+                 stats=stats, out_f32=exact)
         if needs_grad:
             ctx.save_for_backward(q, k, v, table, buckets, key_bias, lengths, out, stats, exact)
-            ctx.scale, ctx.dtype = scale, dtype
+            ctx.sizes = sizes
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):  # pylint: disable=W
         q, k, v, table, buckets, key_bias, lengths, out, stats, exact = ctx.saved_tensors
+        wants_q, wants_k, wants_v, wants_table = ctx.needs_input_grad[:4]
         if not out.numel() or not k.size(2):
             return (torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v),
                     torch.zeros_like(table) if table is not None else None) + (None,) * 6
         g = _vectors(g)
         gq = _like(q)
-        wants_kv = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        gk, gv = (_like(k), _like(v)) if wants_kv else (None, None)
-        gtable = torch.empty_like(table) if table is not None and ctx.needs_input_grad[3] else None
-        a = _describe(q, k, v, table, buckets, key_bias, lengths, ctx.scale, ctx.dtype)
-        a.out, a.out_stride[:], a.stats = out.data_ptr(), _strides(out), stats.data_ptr()
-        a.out_f32 = exact.data_ptr() if exact is not None else None
-        a.gout, a.gout_stride[:] = g.data_ptr(), _strides(g)
-        a.gq, a.gq_stride[:] = gq.data_ptr(), _strides(gq)
-        if wants_kv:
-            a.gk, a.gk_stride[:], a.gv, a.gv_stride[:] = gk.data_ptr(), _strides(gk), gv.data_ptr(), _strides(gv)
-        if gtable is not None:
-            a.gtable = gtable.data_ptr()
-        _run("s2cnn_attention_bwd", a, 1, q.device)
-        return (gq if ctx.needs_input_grad[0] else None, gk if ctx.needs_input_grad[1] else None, gv if ctx.needs_input_grad[2] else None,
-                gtable, None, None, None, None, None, None)
+        gk, gv = (_like(k), _like(v)) if wants_k or wants_v else (None, None)
+        gtable = torch.empty_like(table) if wants_table else None
+        strides = (q.stride(), k.stride(), v.stride(), out.stride(), g.stride(), gq.stride()) + ((gk.stride(), gv.stride()) if gk is not None else ())
+        plan = _plan(q.shape, k.shape, strides, *ctx.sizes, 1)
+        _run("s2cnn_attention_bwd", plan, q.device, q=q, k=k, v=v, table=table, buckets=buckets, key_bias=key_bias, lengths=lengths, out=out, stats=stats,
+             out_f32=exact, gout=g, gq=gq, gk=gk, gv=gv, gtable=gtable)
+        return (gq if wants_q else None, gk if wants_k else None, gv if wants_v else None, gtable, None, None, None, None, None, None)
 
 
 def attention(q, k, v, table=None, buckets=None, key_bias=None, lengths=None, scale=None):
@@ -148,9 +142,9 @@ def attention(q, k, v, table=None, buckets=None, key_bias=None, lengths=None, sc
         q, k, v = (torch.nn.functional.pad(t, (0, 4 - d)) for t in (q, k, v))
     if table is not None:
         table = table.contiguous()
-        buckets = buckets if buckets.stride(-1) == 1 and buckets.stride(-2) < 1 << 26 else buckets.contiguous()
+        buckets = _vectors(buckets)
     if key_bias is not None:
-        key_bias = _unit_last(key_bias)
+        key_bias = key_bias if key_bias.stride(-1) == 1 or n_k == 1 else key_bias.contiguous()
     if lengths is not None:
         lengths = lengths.contiguous()
     needs_grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, table))

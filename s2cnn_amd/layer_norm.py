@@ -5,6 +5,8 @@ The reference normalises with nn.BatchNorm3d between its layers (examples/shrec1
 of `attention` and pointwise layers over the points of a sphere is trained with these.  Random numbers come from a
 counter: the mask is a function of the seed and of an element's index, formed again in the backward pass.
 """
+from functools import lru_cache
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -29,6 +31,11 @@ def _check_dropout(p, seed):
 def _require_seed(seed):
     if torch.is_tensor(seed):
         _hip.require_gpu_of(torch.int64, seed)
+
+
+@lru_cache(maxsize=1024)
+def _workspace_floats(rows, features, dtype):
+    return _hip.lib().s2cnn_layer_norm_bwd_workspace(rows, features, dtype) // 4
 
 
 class _Dropout(torch.autograd.Function):
@@ -110,15 +117,15 @@ class _LayerNorm(torch.autograd.Function):
         wants_x = wants_x or (not step) or not wants_residual                # one of the two is always written
         gx = torch.empty_like(h) if wants_x else None
         gresidual = torch.empty_like(h) if step and wants_residual else None
-        new = torch.empty if rows else torch.zeros
-        gw = new(features, dtype=h.dtype, device=h.device) if wants_weight else None
-        gb = new(features, dtype=h.dtype, device=h.device) if wants_bias else None
+        new = h.new_empty if rows else h.new_zeros
+        gw = new(features) if wants_weight else None
+        gb = new(features) if wants_bias else None
         if rows:
-            nbytes = _hip.lib().s2cnn_layer_norm_bwd_workspace(rows, features, ctx.dtype) if wants_weight or wants_bias else 0
-            ws = _hip.workspace(nbytes, h.device) if nbytes else None
+            floats = _workspace_floats(rows, features, ctx.dtype) if wants_weight or wants_bias else 0
+            ws = h.new_empty(floats, dtype=torch.float32) if floats else None
             number, at = _seed_args(seed)
             _hip.call("s2cnn_layer_norm_bwd", h.data_ptr(), g.data_ptr(), _hip.ptr_or_none(g_h), _hip.ptr_or_none(weight), stats.data_ptr(),
-                      _hip.ptr_or_none(gx), _hip.ptr_or_none(gresidual), _hip.ptr_or_none(gw), _hip.ptr_or_none(gb), _hip.ptr_or_none(ws), nbytes,
+                      _hip.ptr_or_none(gx), _hip.ptr_or_none(gresidual), _hip.ptr_or_none(gw), _hip.ptr_or_none(gb), _hip.ptr_or_none(ws), 4 * floats,
                       rows, features, ctx.p, number, at, int(step), ctx.dtype, _hip.stream_ptr())
         return gx, gresidual, gw, gb, None, None, None, None, None
 
