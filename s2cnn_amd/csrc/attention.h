@@ -65,14 +65,15 @@ template <class T> __device__ __forceinline__ v16f mfma(uint4 a, uint4 b, v16f c
 }
 
 // c += a b, small products first
+template <class T> __device__ __forceinline__ void mma_small(const Frag<T>& a, const Frag<T>& b, v16f& c) {
+  c = mfma<T>(a.part[2], b.part[0], c);
+  c = mfma<T>(a.part[0], b.part[2], c);
+  c = mfma<T>(a.part[1], b.part[1], c);
+  c = mfma<T>(a.part[1], b.part[0], c);
+  c = mfma<T>(a.part[0], b.part[1], c);
+}
 template <class T> __device__ __forceinline__ void mma(const Frag<T>& a, const Frag<T>& b, v16f& c) {
-  if constexpr (T::PARTS == 3) {
-    c = mfma<T>(a.part[2], b.part[0], c);
-    c = mfma<T>(a.part[0], b.part[2], c);
-    c = mfma<T>(a.part[1], b.part[1], c);
-    c = mfma<T>(a.part[1], b.part[0], c);
-    c = mfma<T>(a.part[0], b.part[1], c);
-  }
+  if constexpr (T::PARTS == 3) mma_small<T>(a, b, c);
   c = mfma<T>(a.part[0], b.part[0], c);
 }
 
@@ -244,6 +245,9 @@ template <class T, int D> struct Tile {
 #pragma unroll
     for (int p = 0; p < T::PARTS; ++p) f.part[p] = read16(lds + ((p * STEPS + s) * 64 + at) * 16);
     return f;
+  }
+  static __device__ __forceinline__ uint4 first_by_rows(const unsigned char* lds, int s, int lane) {      // the first part alone
+    return read16(lds + (s * 64 + row_slot(s, lane >> 5, lane & 31)) * 16);
   }
   static __device__ __forceinline__ Frag<T> by_entries(const unsigned char* lds, int b, int t, int lane) {
     Frag<T> f;

@@ -96,7 +96,10 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
   const bool live = inv_l != 0.f;                          // a row without keys takes no part, whatever its gradient holds
   load_column<T, D>(static_cast<const E*>(a.q) + b * a.q_stride[0] + head * a.q_stride[1] + query * a.q_stride[2], a.d, live, half,
                     a.scale * LOG2E, qf);
-  load_column<T, D>(g_row, a.d, live, half, 1.f, gf);
+  // The matrix cores round sums down, not to nearest: a bias of a fraction of a unit in dp's last place, lost in the noise everywhere but
+  // in the table's gradient, where the bias of every pair adds up.  Queries of odd lanes form -dp, whose bias has the other sign.
+  const float sign = T::PARTS == 3 && (lane & 1) ? -1.f : 1.f;
+  load_column<T, D>(g_row, a.d, live, half, sign, gf);
   float delta = 0.f, largest = 0.f, total = 0.f;
 #pragma unroll
   for (int i = 0; i < D / 8; ++i) {
@@ -119,7 +122,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
     if constexpr (T::HALF) p.delta[rows + row] = largest;
   }
   const ScoreScale sc = score_scale<T>(a.n_k, largest);
-  const float rl = inv_l * sc.p, delta_s = delta * sc.ds;
+  const float rl = inv_l * sc.p * sign, delta_s = delta * sc.ds * sign;
   const float undo = T::HALF ? 1.f / (sc.p * sc.ds) : 1.f;
 
   // the unit of the table's sums; NaN where the gradient or a value seen by some query is none or infinite: delta is too, then
@@ -170,7 +173,14 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) mma<T>(Tl::by_rows(lds_k, i, lane), qf[i], s);
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) mma<T>(Tl::by_rows(lds_v, i, lane), gf[i], dp);
+    for (int i = 0; i < D / 16; ++i) {
+      if constexpr (T::PARTS == 3) mma_small<T>(Tl::by_rows(lds_v, i, lane), gf[i], dp);
+      else mma<T>(Tl::by_rows(lds_v, i, lane), gf[i], dp);
+    }
+    if constexpr (T::PARTS == 3) {
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) dp = mfma<T>(Tl::first_by_rows(lds_v, i, lane), gf[i].part[0], dp);
+    }
     if (BUFS == 2 && more) write(step + 1);
     unsigned now[4];
 #pragma unroll
@@ -188,7 +198,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
       round_pair<T>(pr[0], pr[1]);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        s[r + i] = pr[i] * rl * (T::HALF ? fmaf(dp[r + i], sc.ds, -delta_s) : dp[r + i] - delta);
+        s[r + i] = pr[i] * rl * (T::HALF ? fmaf(dp[r + i], sc.ds, -delta_s) : dp[r + i] - delta_s);
         if (table_grad) {
           const double x = __builtin_fma((double)s[r + i], to_units, TableSums::MAGIC);
           const unsigned long long raw = __builtin_bit_cast(unsigned long long, x);
