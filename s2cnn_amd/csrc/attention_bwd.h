@@ -209,7 +209,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
     }
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const Frag<T> f = cut_rows<T>(s, t);
+      const TwoParts<T> f = cut_rows_in_two<T>(s, t);
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) mma<T>(Tl::by_entries(lds_kt, i, t, lane), f, dq[i]);
     }
@@ -437,7 +437,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
     if constexpr (T::PARTS * D > 128) __builtin_amdgcn_sched_barrier(0);     // no operand of a later product is read before: registers
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const Frag<T> pf = cut_rows<T>(s, t), df = cut_rows<T>(dp, t);
+      const TwoParts<T> pf = cut_rows_in_two<T>(s, t), df = cut_rows_in_two<T>(dp, t);
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
         mma<T>(Tl::by_entries(lds_gt, i, t, lane), pf, dv[i]);
