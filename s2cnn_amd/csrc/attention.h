@@ -88,6 +88,11 @@ template <class T> __device__ __forceinline__ v2f uncut(unsigned w) {
   if constexpr (T::HALF) return __builtin_convertvector(__builtin_bit_cast(v2h, w), v2f);
   else return v2f{__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)};
 }
+// sum + the two values of a packed pair
+template <class T> __device__ __forceinline__ float add_pair(unsigned w, float sum) {
+  if constexpr (T::HALF) return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, w), __builtin_bit_cast(v2h, 0x3c003c00u), sum, false);
+  else return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, w), __builtin_bit_cast(v2bf, 0x3f803f80u), sum, false);
+}
 // two values as the matrix cores will see them
 template <class T> __device__ __forceinline__ void round_pair(float& x, float& y) {
   if constexpr (T::PARTS == 1) {
@@ -212,10 +217,11 @@ template <class T> __device__ __forceinline__ void store_quad(typename T::type* 
   }
 }
 
-// The B operands of one column: the vector at `p` (float32: times `factor`), in steps of 16 entries, 8 of them in either half of
+// The B operands of one column: the vector at `p` (float32: times `factor`, 16-bit types: with its sign), in steps of 16 entries, 8 of them in either half of
 // the wave.
 template <class T, int D>
 __device__ __forceinline__ void load_column(const typename T::type* p, int d, bool ok, int half, float factor, Frag<T> (&f)[D / 16]) {
+  const unsigned flip = factor < 0.f ? 0x80008000u : 0u;
 #pragma unroll
   for (int s = 0; s < D / 16; ++s) {
     Quad a = load_quad<T>(p, 4 * s + 2 * half, d), b = load_quad<T>(p, 4 * s + 2 * half + 1, d);
@@ -228,7 +234,7 @@ __device__ __forceinline__ void load_column(const typename T::type* p, int d, bo
       for (int i = 0; i < 8; ++i) x[i] *= factor;
       f[s] = cut8<T>(x);
     } else {
-      f[s].part[0] = make_uint4(a.w.x, a.w.y, b.w.x, b.w.y);
+      f[s].part[0] = make_uint4(a.w.x ^ flip, a.w.y ^ flip, b.w.x ^ flip, b.w.y ^ flip);
     }
   }
 }
@@ -414,8 +420,8 @@ template <class T, int D, int THREADS, int LA, int LB> struct Stage {
 // the sums, the output and the backward pass all use the same, rounded ones.  They are so the exact softmax of weights that
 // are off by a rounding each, rows of its gradient sum to zero as they should, and a factor between references is exact.
 //
-// The product starts from the biases instead of zero: x = c (q.k + bias / c), c = log2(e) scale; float32 takes c into the columns as
-// they are loaded, and needs no factor.  Biases are held within +-3e38, so that one of the type's lowest value
+// The product starts from the biases instead of zero: x = c (q.k + bias / c), c = log2(e) |scale|; float32 takes c into the columns as
+// they are loaded, and needs no factor; the other types take the sign.  Biases are held within +-3e38, so that one of the type's lowest value
 // stays finite: keys that all have it share a row evenly.
 __device__ __forceinline__ float key_value(const float* key_bias, int key, int end, float inv_c) {
   if (key >= end) return ninf() * inv_c;                   // takes no part
@@ -480,7 +486,7 @@ template <class T> __device__ __forceinline__ void start_scores(v16f& s, const f
 // The header's struct and what the entry has made of it.
 struct Args {
   s2cnn_attention_t a;
-  float c, inv_c;          // log2(e) scale and its inverse
+  float c, inv_c;          // log2(e) |scale| and its inverse; 1 for float32
   int forward_splits;
   int splits;              // parts of the long axis (keys; queries in the kernel of dk and dv)
   int tiles;               // workgroups along the columns

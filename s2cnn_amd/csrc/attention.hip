@@ -81,8 +81,8 @@ Args args_of(const s2cnn_attention_t& a, const Plans& plans) {
   p.a = a;
   p.forward_splits = plans.fwd.splits;
   // float32 takes the factor into its columns; the others into the scores, and its inverse into the biases: never zero
-  const float c = a.dtype == S2CNN_F32 ? 1.f : a.scale * LOG2E;
-  p.c = fabsf(c) < 1e-30f ? 1e-30f : c;
+  const float c = a.dtype == S2CNN_F32 ? 1.f : fabsf(a.scale) * LOG2E;
+  p.c = c < 1e-30f ? 1e-30f : c;
   p.inv_c = 1.f / p.c;
   return p;
 }

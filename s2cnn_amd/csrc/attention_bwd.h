@@ -122,7 +122,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
     if constexpr (T::HALF) p.delta[rows + row] = largest;
   }
   const ScoreScale sc = score_scale<T>(a.n_k, largest);
-  const float rl = inv_l * sc.p * sign, delta_s = delta * sc.ds * sign;
+  const float rl = inv_l * sc.p * sc.ds * sign, delta_rl = delta * sign * rl;         // ds = p (dp - delta) / l, as p (dp rl - delta rl)
   const float undo = T::HALF ? 1.f / (sc.p * sc.ds) : 1.f;
 
   // the unit of the table's sums; NaN where the gradient or a value seen by some query is none or infinite: delta is too, then
@@ -194,11 +194,11 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
     for (int r = 0; r < 16; r += 2) {
       float pr[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) pr[i] = exp2_(T::PARTS == 3 ? s[r + i] - m : s[r + i] * p.c - m);
+      for (int i = 0; i < 2; ++i) pr[i] = exp2_(T::PARTS == 3 ? s[r + i] - m : fmaf(s[r + i], p.c, -m));
       round_pair<T>(pr[0], pr[1]);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        s[r + i] = pr[i] * rl * (T::HALF ? fmaf(dp[r + i], sc.ds, -delta_s) : dp[r + i] - delta_s);
+        s[r + i] = pr[i] * fmaf(dp[r + i], rl, -delta_rl);
         if (table_grad) {
           const double x = __builtin_fma((double)s[r + i], to_units, TableSums::MAGIC);
           const unsigned long long raw = __builtin_bit_cast(unsigned long long, x);

@@ -97,13 +97,9 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     if (tid < ROWS) kb_next = key_value(key_bias, key + 2 * ROWS + tid, end, p.inv_c);
 
     float top = ninf();
-    if constexpr (T::PARTS == 1) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] *= p.c;
-    }
 #pragma unroll
     for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
-    top = ceilf(fmaxf(half_max(top), m));
+    top = ceilf(fmaxf(T::PARTS == 3 ? half_max(top) : half_max(top) * p.c, m));
     const float ref = (top == ninf() ? 0.f : top) - SHIFT;
     const float fade = exp2_(m - SHIFT - ref);      // a power of two
     l *= fade;
@@ -112,7 +108,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     m = top;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      s[i] = exp2_(s[i] - ref);
+      s[i] = exp2_(T::PARTS == 3 ? s[i] - ref : fmaf(s[i], p.c, -ref));
       if constexpr (T::PARTS == 3) l += s[i];
     }
 #pragma unroll
@@ -121,10 +117,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
       if constexpr (T::PARTS == 1) {
         const unsigned w[4] = {pf.part[0].x, pf.part[0].y, pf.part[0].z, pf.part[0].w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const v2f r = uncut<T>(w[j]);
-          l += r[0], l += r[1];
-        }
+        for (int j = 0; j < 4; ++j) l = add_pair<T>(w[j], l);
       }
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) mma<T>(Tl::by_entries(lds_v, i, t, lane), pf, o[i]);
