@@ -175,7 +175,11 @@ template <class T> __device__ __forceinline__ Quad load_four(const typename T::t
 }
 template <class T> __device__ __forceinline__ Quad load_quad(const typename T::type* p, int q, int d) {
   Quad v = load_four<T>(p + quad_at(q, d));
-  const int twice = 4 * q < d ? 4 * q - quad_at(q, d) : 4;        // so many of its first entries
+  // So many of its first entries count as zero.  A column's quads each have their own number and four conditions on it, which the
+  // compiler must not share between the vectors of a column (hundreds of scalar registers, and spills of them that gave wrong results):
+  // the empty statement hides that the numbers are equal.
+  int twice = 4 * q < d ? 4 * q - quad_at(q, d) : 4;
+  asm volatile("" : "+v"(twice));
   if constexpr (T::PARTS == 3) {
     if (twice > 0) v.w.x = 0;
     if (twice > 1) v.w.y = 0;

@@ -36,9 +36,9 @@ template <class T> __device__ __forceinline__ ScoreScale score_scale(int n_k, fl
 // in units of a power of two that the workgroup knows beforehand.  |ds| <= 2 max(sum_d |dout_d|) max |v|, both maxima over what the
 // workgroup sees, and a query's |ds| add up to no more than that: 2^50 units for twice the bound leaves room for the queries of a
 // workgroup, and a unit is 2^-49 of the bound, 2^-28 of a typical ds in a row of 10^6 keys.
-// 32 copies, one per query of a wave and shared by waves, keep lanes from the same address.
+// 64 copies, one per lane and shared by waves, keep lanes from the same address.
 struct TableSums {
-  static constexpr int COPIES = 32;
+  static constexpr int COPIES = 64;
   static constexpr double MAGIC = 6755399441055744.0;        // 1.5 * 2^52: adding it rounds to an integer, which its low bits hold
   static __host__ __device__ int words(int n_buckets) { return (n_buckets + 1) * COPIES; }       // one more for excluded pairs
 };
@@ -73,7 +73,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
   const Vectors<T> v{static_cast<const E*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[1], a.v_stride[2], a.n_k, a.d};
   const float* const key_bias = a.key_bias ? a.key_bias + b * a.key_bias_stride : nullptr;
   const signed char* const buckets = a.buckets ? a.buckets + b * a.bucket_stride[0] + query * a.bucket_stride[1] : nullptr;
-  unsigned long long* const sums = lds_sums + (lane & 31);
+  unsigned long long* const sums = lds_sums + lane;
   const bool table_grad = a.gtable != nullptr;
   const float dead = ninf() * p.inv_c;
 
@@ -221,7 +221,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
     float* const part = p.gtable_partial + ((long)bh * p.splits * p.tiles + split * p.tiles + tile) * a.n_buckets;
     for (int n = tid; n < a.n_buckets; n += 64 * W) {
       unsigned long long t = 0;
-      for (int i = 0; i < TableSums::COPIES; ++i) t += lds_sums[n * TableSums::COPIES + ((i + n) & 31)];   // lanes start at banks of their own
+      for (int i = 0; i < TableSums::COPIES; ++i) t += lds_sums[n * TableSums::COPIES + ((i + n) & 63)];   // lanes start at banks of their own
       part[n] = (float)((double)(long long)t / unit);
     }
   }
