@@ -427,11 +427,13 @@ template <class T, int D, int THREADS, int LA, int LB> struct Stage {
 // The product starts from the biases instead of zero: x = c (q.k + bias / c), c = log2(e) |scale|; float32 takes c into the columns as
 // they are loaded, and needs no factor; the other types take the sign.  Biases are held within +-3e38, so that one of the type's lowest value
 // stays finite: keys that all have it share a row evenly.
-__device__ __forceinline__ float key_value(const float* key_bias, int key, int end, float inv_c) {
-  if (key >= end) return ninf() * inv_c;                   // takes no part
-  if (!key_bias) return 0.f;
-  const float b = key_bias[key], x = b * LOG2E * inv_c;
-  return fabsf(b) < pinf() ? __builtin_amdgcn_fmed3f(x, -3e38f, 3e38f) : x;
+// In two steps, the load and what is made of it: the tiles' loads are under way in between, and a wait for this one, issued before them,
+// is no wait for them.
+__device__ __forceinline__ float load_key_bias(const float* key_bias, int key, int end) { return key_bias ? key_bias[max(min(key, end - 1), 0)] : 0.f; }
+__device__ __forceinline__ float key_value(float bias, int key, int end, float inv_c) {
+  const float x = bias * LOG2E * inv_c;
+  const float y = fabsf(bias) < pinf() ? __builtin_amdgcn_fmed3f(x, -3e38f, 3e38f) : x;
+  return key < end ? y : ninf() * inv_c;                   // -inf: takes no part
 }
 
 // A tile's values of its rows (keys' biases; the queries' statistics) in LDS, in a ring: tile t's are read in step t, and in step
@@ -465,6 +467,10 @@ __device__ __forceinline__ void load_buckets(const signed char* row, int key0, i
   }
 }
 __device__ __forceinline__ int bucket_of(unsigned w, int i, int n_buckets) { return min((int)((w >> (8 * i)) & 255u), n_buckets); }
+
+// Whether a wave's words of a tile exclude every pair of it: with a bias over near points only, most tiles of far ones.  The wave leaves
+// them out: they would add zeros.  (Excluded by negative numbers; by positive ones beyond the table they are formed as any other.)
+__device__ __forceinline__ bool none_takes_part(const unsigned (&w)[4]) { return __all((w[0] & w[1] & w[2] & w[3] & 0x80808080u) == 0x80808080u); }
 
 // What the scores of a tile start from: the keys' biases, and the table's entries of the pairs where there are buckets.  In the
 // accumulators before the product begins, they need no registers beside them.

@@ -83,7 +83,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
     if (W > 1) stage.fetch(k, v, key0, tid);
     if (buckets) load_buckets(buckets, key0, end, half, words);
   }
-  if (tid < 2 * ROWS) lds_kb[tid] = key_value(key_bias, key0 + tid, end, p.inv_c);
+  if (tid < 2 * ROWS) lds_kb[tid] = key_value(key0 < end ? load_key_bias(key_bias, key0 + tid, end) : 0.f, key0 + tid, end, p.inv_c);
   if (buckets) stage_table<T>(lds_table, a.table, a.n_buckets, head, 1, tid, 64 * W);
   if (table_grad)
     for (int n = tid; n < TableSums::words(a.n_buckets); n += 64 * W) lds_sums[n] = 0;
@@ -168,52 +168,51 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
     const unsigned char* const lds_v = lds_k + 2 * Tl::BYTES;
     const float* const kb = lds_kb + step % RING * ROWS;
 
-    v16f s, dp = {};
-    start_scores<T>(s, kb, half, buckets != nullptr, words, lds_table, a.n_buckets, p.inv_c);
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) mma<T>(Tl::by_rows(lds_k, i, lane), qf[i], s);
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      if constexpr (T::PARTS == 3) mma_small<T>(Tl::by_rows(lds_v, i, lane), gf[i], dp);
-      else mma<T>(Tl::by_rows(lds_v, i, lane), gf[i], dp);
-    }
-    if constexpr (T::PARTS == 3) {
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) dp = mfma<T>(Tl::first_by_rows(lds_v, i, lane), gf[i].part[0], dp);
-    }
     if (BUFS == 2 && more) write(step + 1);
-    unsigned now[4];
-#pragma unroll
-    for (int g = 0; g < 4; ++g) now[g] = words[g];
-    float kb_next = 0.f;
+    const unsigned now[4] = {words[0], words[1], words[2], words[3]};
+    const float bias_next = tid < ROWS ? load_key_bias(key_bias, key + 2 * ROWS + tid, end) : 0.f;
     if (W > 1 && key + BUFS * ROWS < end) stage.fetch(k, v, key + BUFS * ROWS, tid);
     if (more && buckets) load_buckets(buckets, key + ROWS, end, half, words);
-    if (tid < ROWS) kb_next = key_value(key_bias, key + 2 * ROWS + tid, end, p.inv_c);
 
+    if (!buckets || !none_takes_part(now)) {
+      v16f s, dp = {};
+      start_scores<T>(s, kb, half, buckets != nullptr, now, lds_table, a.n_buckets, p.inv_c);
 #pragma unroll
-    for (int r = 0; r < 16; r += 2) {
-      float pr[2];
+      for (int i = 0; i < D / 16; ++i) mma<T>(Tl::by_rows(lds_k, i, lane), qf[i], s);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) pr[i] = exp2_(T::PARTS == 3 ? s[r + i] - m : fmaf(s[r + i], p.c, -m));
-      round_pair<T>(pr[0], pr[1]);
+      for (int i = 0; i < D / 16; ++i) {
+        if constexpr (T::PARTS == 3) mma_small<T>(Tl::by_rows(lds_v, i, lane), gf[i], dp);
+        else mma<T>(Tl::by_rows(lds_v, i, lane), gf[i], dp);
+      }
+      if constexpr (T::PARTS == 3) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        s[r + i] = pr[i] * fmaf(dp[r + i], rl, -delta_rl);
-        if (table_grad) {
-          const double x = __builtin_fma((double)s[r + i], to_units, TableSums::MAGIC);
-          const unsigned long long raw = __builtin_bit_cast(unsigned long long, x);
-          const unsigned high = (unsigned)(raw >> 32) - (unsigned)(__builtin_bit_cast(unsigned long long, TableSums::MAGIC) >> 32);   // its low half is zero
-          __hip_atomic_fetch_add(sums + bucket_of(now[r / 4], r % 4 + i, a.n_buckets) * TableSums::COPIES, (unsigned long long)high << 32 | (unsigned)raw, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        for (int i = 0; i < D / 16; ++i) dp = mfma<T>(Tl::first_by_rows(lds_v, i, lane), gf[i].part[0], dp);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        float pr[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) pr[i] = exp2_(T::PARTS == 3 ? s[r + i] - m : fmaf(s[r + i], p.c, -m));
+        round_pair<T>(pr[0], pr[1]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          s[r + i] = pr[i] * fmaf(dp[r + i], rl, -delta_rl);
+          if (table_grad) {
+            const double x = __builtin_fma((double)s[r + i], to_units, TableSums::MAGIC);
+            const unsigned long long raw = __builtin_bit_cast(unsigned long long, x);
+            const unsigned high = (unsigned)(raw >> 32) - (unsigned)(__builtin_bit_cast(unsigned long long, TableSums::MAGIC) >> 32);   // its low half is zero
+            __hip_atomic_fetch_add(sums + bucket_of(now[r / 4], r % 4 + i, a.n_buckets) * TableSums::COPIES, (unsigned long long)high << 32 | (unsigned)raw, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+          }
         }
       }
-    }
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const TwoParts<T> f = cut_rows_in_two<T>(s, t);
+      for (int t = 0; t < 2; ++t) {
+        const TwoParts<T> f = cut_rows_in_two<T>(s, t);
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) mma<T>(Tl::by_entries(lds_kt, i, t, lane), f, dq[i]);
+        for (int i = 0; i < D / 32; ++i) mma<T>(Tl::by_entries(lds_kt, i, t, lane), f, dq[i]);
+      }
     }
-    if (tid < ROWS) lds_kb[(step + 2) % RING * ROWS + tid] = kb_next;
+    if (tid < ROWS) lds_kb[(step + 2) % RING * ROWS + tid] = key_value(bias_next, key + 2 * ROWS + tid, end, p.inv_c);
   }
 
   if (table_grad) {
@@ -270,7 +269,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
   typedef typename T::type E;
   const float* const key_bias = a.key_bias ? a.key_bias + b * a.key_bias_stride : nullptr;
   const signed char* const buckets = a.buckets ? a.buckets + b * a.bucket_stride[0] : nullptr;
-  const float dead = ninf() * p.inv_c, kb_c = ok ? key_value(key_bias, key, end, p.inv_c) : dead, kb = kb_c * p.c;
+  const float dead = ninf() * p.inv_c, kb_c = ok ? key_value(load_key_bias(key_bias, key, a.n_k), key, end, p.inv_c) : dead, kb = kb_c * p.c;
   const bool live = kb_c != dead;
 
   Frag<T> kf[D / 16], vf[D / 16];
@@ -298,17 +297,17 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
     return {static_cast<const E*>(base) + b * stride[0] + (hk * group + r / per_head) * stride[1], stride[2], a.n_q, a.d};
   };
   const auto fetch = [&](int r) { stage.fetch(queries(r, a.q, a.q_stride), queries(r, a.gout, a.gout_stride), r % per_head * ROWS, tid); };
-  struct Row { float m, rl, delta; };
-  const auto row_of = [&](int r) -> Row {                  // what thread tid < ROWS brings for row tid of tile r
-    const int query = r % per_head * ROWS + tid;
-    if (r >= last || query >= a.n_q) return {ninf(), 0.f, 0.f};
-    const long row = ((long)b * a.heads + hk * group + r / per_head) * a.n_q + query;
-    const float2 st = reinterpret_cast<const float2*>(a.stats)[row];
-    return {-st.x, st.y * sc.p, -p.delta[row]};
+  // what thread tid < ROWS brings for row tid of tile r: the load, and what is made of it (as load_key_bias, key_value)
+  struct Row { float2 stats; float delta; };
+  const auto load_row = [&](int r) -> Row {
+    const int rr = min(r, last - 1);
+    const long row = ((long)b * a.heads + hk * group + rr / per_head) * a.n_q + min(rr % per_head * ROWS + tid, a.n_q - 1);
+    return {reinterpret_cast<const float2*>(a.stats)[row], p.delta[row]};
   };
   const auto put_row = [&](int r, const Row& x) {
     float* const to = lds_rows + (r - first) % RING * 3 * ROWS + tid;
-    to[0] = x.m, to[ROWS] = x.rl, to[2 * ROWS] = x.delta;
+    const bool none = r >= last || r % per_head * ROWS + tid >= a.n_q;
+    to[0] = none ? ninf() : -x.stats.x, to[ROWS] = none ? 0.f : x.stats.y * sc.p, to[2 * ROWS] = none ? 0.f : -x.delta;
   };
   const auto write = [&](int r) {
     unsigned char* const to = smem + (r - first) % BUFS * BUF;
@@ -346,7 +345,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
   };
   if (W > 1 && first < last) fetch(first);
   if (buckets && first < last) fetch_buckets(first);
-  if (tid < ROWS) put_row(first, row_of(first)), put_row(first + 1, row_of(first + 1));
+  if (first < last && tid < ROWS) put_row(first, load_row(first)), put_row(first + 1, load_row(first + 1));
   if (buckets) stage_table<T>(lds_table, a.table, a.n_buckets, hk * group, group, tid, 64 * W);
   if (BUFS == 2) {
     __syncthreads();
@@ -371,77 +370,80 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
     }
     const float* const table = lds_table + r / per_head * (a.n_buckets + 1);
 
-    // the scores start from the table's entries (float32: less m), dp from -delta
-    v16f s = {}, dp;
-    if (buckets) {
-      const unsigned* const words = lds_buckets + ((r - first) % 2 * 32 * W + wave * 32 + (lane & 31)) * BUCKET_LD + half;
-      float t[16];
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const unsigned word = words[2 * g];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) t[4 * g + i] = table[bucket_of(word, i, a.n_buckets)];
-      }
-#pragma unroll
-      for (int j = 0; j < 16; ++j) s[j] = T::PARTS == 3 ? t[j] : t[j] * p.inv_c;
-    }
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      float start[4];
-      read16(rows + 2 * ROWS + 8 * g + 4 * half, start);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) dp[4 * g + i] = start[i];
-      if constexpr (T::PARTS == 3) {
-        read16(rows + 8 * g + 4 * half, start);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[4 * g + i] += start[i];
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) mma<T>(Tl::by_rows(lds_q, i, lane), kf[i], s);
-    if constexpr (T::PARTS * D > 128) __builtin_amdgcn_sched_barrier(0);     // no operand of a later product is read before: registers
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) mma<T>(Tl::by_rows(lds_g, i, lane), vf[i], dp);
-    if constexpr (T::PARTS * D > 128) __builtin_amdgcn_sched_barrier(0);     // no operand of a later product is read before: registers
     if (BUFS == 2 && r + 1 < last) {
       write(r + 1);
       if (buckets) write_buckets(r + 1);
     }
     Row next = {};
+    if (tid < ROWS) next = load_row(r + 2);
     if (W > 1 && r + BUFS < last) fetch(r + BUFS);
-    if (tid < ROWS) next = row_of(r + 2);
     if (buckets && r + BUFS < last) fetch_buckets(r + BUFS);
 
+    unsigned words[4] = {0, 0, 0, 0};
+    if (buckets) {
+      const unsigned* const from = lds_buckets + ((r - first) % 2 * 32 * W + wave * 32 + (lane & 31)) * BUCKET_LD + half;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      float ls[4], ms[4] = {0.f, 0.f, 0.f, 0.f};
-      read16(rows + ROWS + 8 * g + 4 * half, ls);
-      if constexpr (T::PARTS == 1) read16(rows + 8 * g + 4 * half, ms);
+      for (int g = 0; g < 4; ++g) words[g] = from[2 * g];
+    }
+    if (!buckets || !none_takes_part(words)) {
+      // the scores start from the table's entries (float32: less m), dp from -delta
+      v16f s = {}, dp;
+      if (buckets) {
+        float t[16];
 #pragma unroll
-      for (int i = 0; i < 4; i += 2) {
-        float pr[2];
+        for (int j = 0; j < 16; ++j) t[j] = table[bucket_of(words[j / 4], j % 4, a.n_buckets)];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int j = 4 * g + i + e;
-          pr[e] = exp2_(T::PARTS == 3 ? s[j] + kb : fmaf(s[j], p.c, kb) + ms[i + e]);
-        }
-        round_pair<T>(pr[0], pr[1]);
+        for (int j = 0; j < 16; ++j) s[j] = T::PARTS == 3 ? t[j] : t[j] * p.inv_c;
+      }
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int j = 4 * g + i + e;
-          s[j] = pr[e] * ls[i + e];
-          dp[j] = s[j] * (T::HALF ? dp[j] * sc.ds : dp[j]);
+      for (int g = 0; g < 4; ++g) {
+        float start[4];
+        read16(rows + 2 * ROWS + 8 * g + 4 * half, start);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dp[4 * g + i] = start[i];
+        if constexpr (T::PARTS == 3) {
+          read16(rows + 8 * g + 4 * half, start);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[4 * g + i] += start[i];
         }
       }
-    }
-    if constexpr (T::PARTS * D > 128) __builtin_amdgcn_sched_barrier(0);     // no operand of a later product is read before: registers
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const TwoParts<T> pf = cut_rows_in_two<T>(s, t), df = cut_rows_in_two<T>(dp, t);
+      for (int i = 0; i < D / 16; ++i) mma<T>(Tl::by_rows(lds_q, i, lane), kf[i], s);
+      if constexpr (T::PARTS * D > 128) __builtin_amdgcn_sched_barrier(0);     // no operand of a later product is read before: registers
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        mma<T>(Tl::by_entries(lds_gt, i, t, lane), pf, dv[i]);
-        mma<T>(Tl::by_entries(lds_qt, i, t, lane), df, dk[i]);
+      for (int i = 0; i < D / 16; ++i) mma<T>(Tl::by_rows(lds_g, i, lane), vf[i], dp);
+      if constexpr (T::PARTS * D > 128) __builtin_amdgcn_sched_barrier(0);     // no operand of a later product is read before: registers
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        float ls[4], ms[4] = {0.f, 0.f, 0.f, 0.f};
+        read16(rows + ROWS + 8 * g + 4 * half, ls);
+        if constexpr (T::PARTS == 1) read16(rows + 8 * g + 4 * half, ms);
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          float pr[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int j = 4 * g + i + e;
+            pr[e] = exp2_(T::PARTS == 3 ? s[j] + kb : fmaf(s[j], p.c, kb) + ms[i + e]);
+          }
+          round_pair<T>(pr[0], pr[1]);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int j = 4 * g + i + e;
+            s[j] = pr[e] * ls[i + e];
+            dp[j] = s[j] * (T::HALF ? dp[j] * sc.ds : dp[j]);
+          }
+        }
+      }
+      if constexpr (T::PARTS * D > 128) __builtin_amdgcn_sched_barrier(0);     // no operand of a later product is read before: registers
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const TwoParts<T> pf = cut_rows_in_two<T>(s, t), df = cut_rows_in_two<T>(dp, t);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          mma<T>(Tl::by_entries(lds_gt, i, t, lane), pf, dv[i]);
+          mma<T>(Tl::by_entries(lds_qt, i, t, lane), df, dk[i]);
+        }
       }
     }
     if (tid < ROWS) put_row(r + 2, next);

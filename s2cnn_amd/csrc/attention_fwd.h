@@ -51,7 +51,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     if (W > 1) stage.fetch(k, v, key0, tid);
     if (buckets) load_buckets(buckets, key0, end, half, words);
   }
-  if (tid < 2 * ROWS) lds_kb[tid] = key_value(key_bias, key0 + tid, end, p.inv_c);
+  if (tid < 2 * ROWS) lds_kb[tid] = key_value(key0 < end ? load_key_bias(key_bias, key0 + tid, end) : 0.f, key0 + tid, end, p.inv_c);
   if (buckets) stage_table<T>(lds_table, a.table, a.n_buckets, head0, heads, tid, 64 * W);
   Frag<T> qf[D / 16];
   load_column<T, D>(static_cast<const E*>(a.q) + b * a.q_stride[0] + head * a.q_stride[1] + query * a.q_stride[2], a.d, ok, half,
@@ -86,43 +86,45 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     const unsigned char* const lds_v = lds_k + Tl::BYTES;
     const float* const kb = lds_kb + step % RING * ROWS;
 
-    v16f s;
-    start_scores<T>(s, kb, half, buckets != nullptr, words, table, a.n_buckets, p.inv_c);
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) mma<T>(Tl::by_rows(lds_k, i, lane), qf[i], s);
     if (BUFS == 2 && more) write(step + 1);
-    float kb_next = 0.f;
+    const float bias_next = tid < ROWS ? load_key_bias(key_bias, key + 2 * ROWS + tid, end) : 0.f;
     if (W > 1 && key + BUFS * ROWS < end) stage.fetch(k, v, key + BUFS * ROWS, tid);
+    const unsigned now[4] = {words[0], words[1], words[2], words[3]};
     if (more && buckets) load_buckets(buckets, key + ROWS, end, half, words);
-    if (tid < ROWS) kb_next = key_value(key_bias, key + 2 * ROWS + tid, end, p.inv_c);
 
-    float top = ninf();
+    if (!buckets || !none_takes_part(now)) {
+      v16f s;
+      start_scores<T>(s, kb, half, buckets != nullptr, now, table, a.n_buckets, p.inv_c);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
-    top = ceilf(fmaxf(T::PARTS == 3 ? half_max(top) : half_max(top) * p.c, m));
-    const float ref = (top == ninf() ? 0.f : top) - SHIFT;
-    const float fade = exp2_(m - SHIFT - ref);      // a power of two
-    l *= fade;
+      for (int i = 0; i < D / 16; ++i) mma<T>(Tl::by_rows(lds_k, i, lane), qf[i], s);
+      float top = ninf();
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) o[i] *= fade;
-    m = top;
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
+      top = ceilf(fmaxf(T::PARTS == 3 ? half_max(top) : half_max(top) * p.c, m));
+      const float ref = (top == ninf() ? 0.f : top) - SHIFT;
+      const float fade = exp2_(m - SHIFT - ref);      // a power of two
+      l *= fade;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      s[i] = exp2_(T::PARTS == 3 ? s[i] - ref : fmaf(s[i], p.c, -ref));
-      if constexpr (T::PARTS == 3) l += s[i];
-    }
+      for (int i = 0; i < D / 32; ++i) o[i] *= fade;
+      m = top;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const Frag<T> pf = cut_rows<T>(s, t);
-      if constexpr (T::PARTS == 1) {
-        const unsigned w[4] = {pf.part[0].x, pf.part[0].y, pf.part[0].z, pf.part[0].w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) l = add_pair<T>(w[j], l);
+      for (int i = 0; i < 16; ++i) {
+        s[i] = exp2_(T::PARTS == 3 ? s[i] - ref : fmaf(s[i], p.c, -ref));
+        if constexpr (T::PARTS == 3) l += s[i];
       }
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) mma<T>(Tl::by_entries(lds_v, i, t, lane), pf, o[i]);
+      for (int t = 0; t < 2; ++t) {
+        const Frag<T> pf = cut_rows<T>(s, t);
+        if constexpr (T::PARTS == 1) {
+          const unsigned w[4] = {pf.part[0].x, pf.part[0].y, pf.part[0].z, pf.part[0].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) l = add_pair<T>(w[j], l);
+        }
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) mma<T>(Tl::by_entries(lds_v, i, t, lane), pf, o[i]);
+      }
     }
-    if (tid < ROWS) lds_kb[(step + 2) % RING * ROWS + tid] = kb_next;
+    if (tid < ROWS) lds_kb[(step + 2) % RING * ROWS + tid] = key_value(bias_next, key + 2 * ROWS + tid, end, p.inv_c);
   }
 
   const long row = ((long)b * a.heads + head) * a.n_q + query, rows = (long)a.batch * a.heads * a.n_q;
