@@ -449,22 +449,29 @@ template <class T> __device__ __forceinline__ void stage_table(float* lds, const
   }
 }
 
-// buckets of the lane's column and keys key0 + 8 g + 4 half + i, a byte each; 255 past the end
+// Buckets of the lane's column and keys key0 + 8 g + 4 half + i, a byte each; 255 past the end.  A lane loads 16 bytes, the first or the second
+// half of its row's 32, in place of four words of four: a quarter of the requests, each of which is to 32 rows.  The two lanes of a row
+// then exchange words: those of groups 0 and 2 are the first two of either, those of 1 and 3 the others.  The exchange is left to
+// place_buckets, so that the load can be under way.
 __device__ __forceinline__ void load_buckets(const signed char* row, int key0, int end, int half, unsigned (&w)[4]) {
   if (key0 + ROWS <= end) {
 #pragma unroll
-    for (int g = 0; g < 4; ++g) __builtin_memcpy(&w[g], row + key0 + 8 * g + 4 * half, 4);
+    for (int g = 0; g < 4; ++g) __builtin_memcpy(&w[g], row + key0 + 16 * half + 4 * g, 4);
   } else {
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       w[g] = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int key = key0 + 8 * g + 4 * half + i;
+        const int key = key0 + 16 * half + 4 * g + i;
         w[g] |= (key < end ? (unsigned)(unsigned char)row[key] : 255u) << (8 * i);
       }
     }
   }
+}
+__device__ __forceinline__ void place_buckets(const unsigned (&w)[4], unsigned (&now)[4]) {
+  const auto a = __builtin_amdgcn_permlane32_swap(w[0], w[1], false, false), b = __builtin_amdgcn_permlane32_swap(w[2], w[3], false, false);
+  now[0] = a[0], now[1] = b[0], now[2] = a[1], now[3] = b[1];
 }
 __device__ __forceinline__ int bucket_of(unsigned w, int i, int n_buckets) { return min((int)((w >> (8 * i)) & 255u), n_buckets); }
 

@@ -169,7 +169,8 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
     const float* const kb = lds_kb + step % RING * ROWS;
 
     if (BUFS == 2 && more) write(step + 1);
-    const unsigned now[4] = {words[0], words[1], words[2], words[3]};
+    unsigned now[4] = {0, 0, 0, 0};
+    if (buckets) place_buckets(words, now);
     const float bias_next = tid < ROWS ? load_key_bias(key_bias, key + 2 * ROWS + tid, end) : 0.f;
     if (W > 1 && key + BUFS * ROWS < end) stage.fetch(k, v, key + BUFS * ROWS, tid);
     if (more && buckets) load_buckets(buckets, key + ROWS, end, half, words);

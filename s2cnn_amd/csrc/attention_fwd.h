@@ -89,7 +89,8 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     if (BUFS == 2 && more) write(step + 1);
     const float bias_next = tid < ROWS ? load_key_bias(key_bias, key + 2 * ROWS + tid, end) : 0.f;
     if (W > 1 && key + BUFS * ROWS < end) stage.fetch(k, v, key + BUFS * ROWS, tid);
-    const unsigned now[4] = {words[0], words[1], words[2], words[3]};
+    unsigned now[4] = {0, 0, 0, 0};
+    if (buckets) place_buckets(words, now);
     if (more && buckets) load_buckets(buckets, key + ROWS, end, half, words);
 
     if (!buckets || !none_takes_part(now)) {
