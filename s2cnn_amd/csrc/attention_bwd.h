@@ -294,37 +294,39 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
   }
 
   Stage<T, D, 64 * W, BOTH, BOTH> stage;
-  const auto queries = [&](int r, const void* base, const long (&stride)[3]) -> Vectors<T> {     // of the head of tile r
-    return {static_cast<const E*>(base) + b * stride[0] + (hk * group + r / per_head) * stride[1], stride[2], a.n_q, a.d};
+  struct Place {                                           // of a tile: its head of the group, its first query
+    int head, query;
+    __device__ __forceinline__ Place next(int n_q) const { return query + ROWS < n_q ? Place{head, query + ROWS} : Place{head + 1, 0}; }
   };
-  const auto fetch = [&](int r) { stage.fetch(queries(r, a.q, a.q_stride), queries(r, a.gout, a.gout_stride), r % per_head * ROWS, tid); };
+  const auto queries = [&](const Place& at, const void* base, const long (&stride)[3]) -> Vectors<T> {
+    return {static_cast<const E*>(base) + b * stride[0] + (hk * group + at.head) * stride[1], stride[2], a.n_q, a.d};
+  };
+  const auto fetch = [&](const Place& at) { stage.fetch(queries(at, a.q, a.q_stride), queries(at, a.gout, a.gout_stride), at.query, tid); };
   // what thread tid < ROWS brings for row tid of tile r: the load, and what is made of it (as load_key_bias, key_value)
   struct Row { float2 stats; float delta; };
-  const auto load_row = [&](int r) -> Row {
-    const int rr = min(r, last - 1);
-    const long row = ((long)b * a.heads + hk * group + rr / per_head) * a.n_q + min(rr % per_head * ROWS + tid, a.n_q - 1);
+  const auto load_row = [&](const Place& at) -> Row {
+    const long row = ((long)b * a.heads + hk * group + min(at.head, group - 1)) * a.n_q + min(at.query + tid, a.n_q - 1);
     return {reinterpret_cast<const float2*>(a.stats)[row], p.delta[row]};
   };
-  const auto put_row = [&](int r, const Row& x) {
-    float* const to = lds_rows + (r - first) % RING * 3 * ROWS + tid;
-    const bool none = r >= last || r % per_head * ROWS + tid >= a.n_q;
+  const auto put_row = [&](int step, const Place& at, const Row& x) {
+    float* const to = lds_rows + step % RING * 3 * ROWS + tid;
+    const bool none = at.head >= group || at.query + tid >= a.n_q;
     to[0] = none ? ninf() : -x.stats.x, to[ROWS] = none ? 0.f : x.stats.y * sc.p, to[2 * ROWS] = none ? 0.f : -x.delta;
   };
-  const auto write = [&](int r) {
-    unsigned char* const to = smem + (r - first) % BUFS * BUF;
-    const float* const rows = lds_rows + (r - first) % RING * 3 * ROWS;
+  const auto write = [&](int step, const Place& at) {
+    unsigned char* const to = smem + step % BUFS * BUF;
+    const float* const rows = lds_rows + step % RING * 3 * ROWS;
     const auto keep = [&](int i) { return rows[ROWS + i] != 0.f; };
-    if constexpr (W == 1)
-      stage.fetch_and_write(queries(r, a.q, a.q_stride), queries(r, a.gout, a.gout_stride), r % per_head * ROWS, to, tid, keep);
+    if constexpr (W == 1) stage.fetch_and_write(queries(at, a.q, a.q_stride), queries(at, a.gout, a.gout_stride), at.query, to, tid, keep);
     else stage.write(to, tid, keep);
   };
   // The tile's buckets pass through LDS too: a thread fetches those of 4 queries and 4 keys, and writes them the other way round, a word
   // of four queries per key.
   unsigned bucket_words[4];
   const int block_query = 4 * (tid / (8 * W)), block_key = 4 * (tid % (8 * W));
-  const auto fetch_buckets = [&](int r) {
-    const int left = a.n_q - 1 - r % per_head * ROWS, key0 = tile * 32 * W + block_key;
-    const signed char* const at = buckets + (long)(r % per_head * ROWS) * a.bucket_stride[1] + tile * 32 * W;
+  const auto fetch_buckets = [&](const Place& place) {
+    const int left = a.n_q - 1 - place.query, key0 = tile * 32 * W + block_key;
+    const signed char* const at = buckets + (long)place.query * a.bucket_stride[1] + tile * 32 * W;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const signed char* const from = at + (unsigned)(min(block_query + i, left) * (int)a.bucket_stride[1] + block_key);
@@ -335,8 +337,8 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
       }
     }
   };
-  const auto write_buckets = [&](int r) {
-    unsigned* const to = lds_buckets + (r - first) % 2 * 32 * W * BUCKET_LD + block_key * BUCKET_LD + block_query / 4;
+  const auto write_buckets = [&](int step) {
+    unsigned* const to = lds_buckets + step % 2 * 32 * W * BUCKET_LD + block_key * BUCKET_LD + block_query / 4;
     const unsigned a0 = __builtin_amdgcn_perm(bucket_words[1], bucket_words[0], 0x05010400u), a1 = __builtin_amdgcn_perm(bucket_words[1], bucket_words[0], 0x07030602u);
     const unsigned b0 = __builtin_amdgcn_perm(bucket_words[3], bucket_words[2], 0x05010400u), b1 = __builtin_amdgcn_perm(bucket_words[3], bucket_words[2], 0x07030602u);
     to[0] = __builtin_amdgcn_perm(b0, a0, 0x05040100u);
@@ -344,45 +346,47 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
     to[2 * BUCKET_LD] = __builtin_amdgcn_perm(b1, a1, 0x05040100u);
     to[3 * BUCKET_LD] = __builtin_amdgcn_perm(b1, a1, 0x07060302u);
   };
-  if (W > 1 && first < last) fetch(first);
-  if (buckets && first < last) fetch_buckets(first);
-  if (first < last && tid < ROWS) put_row(first, load_row(first)), put_row(first + 1, load_row(first + 1));
+  Place here{first / per_head, first % per_head * ROWS}, next = here.next(a.n_q), after = next.next(a.n_q);     // of this step, the next, the one after
+  if (first < last) {
+    if (W > 1) fetch(here);
+    if (buckets) fetch_buckets(here);
+    if (tid < ROWS) put_row(0, here, load_row(here)), put_row(1, next, load_row(next));
+  }
   if (buckets) stage_table<T>(lds_table, a.table, a.n_buckets, hk * group, group, tid, 64 * W);
   if (BUFS == 2) {
     __syncthreads();
-    if (first < last) write(first);
-    if (first + 1 < last) fetch(first + 1);
-    if (buckets && first < last) write_buckets(first);
-    if (buckets && first + 1 < last) fetch_buckets(first + 1);
+    if (first < last) write(0, here);
+    if (first + 1 < last) fetch(next);
+    if (buckets && first < last) write_buckets(0);
+    if (buckets && first + 1 < last) fetch_buckets(next);
   }
 
   v16f dk[D / 32] = {}, dv[D / 32] = {};
-  for (int r = first; r < last; ++r) {
-    const float* const rows = lds_rows + (r - first) % RING * 3 * ROWS;
-    const unsigned char* const lds_q = smem + (r - first) % BUFS * BUF;
+  for (int r = first, step = 0; r < last; ++r, ++step) {
+    const float* const rows = lds_rows + step % RING * 3 * ROWS;
+    const unsigned char* const lds_q = smem + step % BUFS * BUF;
     const unsigned char* const lds_qt = lds_q + Tl::BYTES;
     const unsigned char* const lds_g = lds_q + 2 * Tl::BYTES;
     const unsigned char* const lds_gt = lds_q + 3 * Tl::BYTES;
     __syncthreads();
     if (BUFS == 1) {
-      write(r);
-      if (buckets) write_buckets(r);
+      write(step, here);
+      if (buckets) write_buckets(step);
       __syncthreads();
+    } else if (r + 1 < last) {
+      write(step + 1, next);
+      if (buckets) write_buckets(step + 1);
     }
-    const float* const table = lds_table + r / per_head * (a.n_buckets + 1);
-
-    if (BUFS == 2 && r + 1 < last) {
-      write(r + 1);
-      if (buckets) write_buckets(r + 1);
+    const float* const table = lds_table + here.head * (a.n_buckets + 1);
+    Row ahead = {};
+    if (tid < ROWS) ahead = load_row(after);
+    if (r + BUFS < last) {
+      if (W > 1) fetch(BUFS == 1 ? next : after);
+      if (buckets) fetch_buckets(BUFS == 1 ? next : after);
     }
-    Row next = {};
-    if (tid < ROWS) next = load_row(r + 2);
-    if (W > 1 && r + BUFS < last) fetch(r + BUFS);
-    if (buckets && r + BUFS < last) fetch_buckets(r + BUFS);
-
     unsigned words[4] = {0, 0, 0, 0};
     if (buckets) {
-      const unsigned* const from = lds_buckets + ((r - first) % 2 * 32 * W + wave * 32 + (lane & 31)) * BUCKET_LD + half;
+      const unsigned* const from = lds_buckets + (step % 2 * 32 * W + wave * 32 + (lane & 31)) * BUCKET_LD + half;
 #pragma unroll
       for (int g = 0; g < 4; ++g) words[g] = from[2 * g];
     }
@@ -447,7 +451,8 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
         }
       }
     }
-    if (tid < ROWS) put_row(r + 2, next);
+    if (tid < ROWS) put_row(step + 2, after, ahead);
+    here = next, next = after, after = after.next(a.n_q);
   }
 
   if (!ok) return;
