@@ -471,17 +471,28 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
 }
 
 // ---- sums of partial results, in a fixed order ----------------------------------------------------------------------
-// Vectors: one wave each; [splits][vectors][D] -> the tensor.
-template <class T, int D> __global__ __launch_bounds__(256) void sum_vectors_kernel(const float* part, int splits, typename T::type* to, long s0, long s1, long s2,
-                                                                                   int heads, int n, int d, long vectors) {
-  const long i = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (i >= vectors) return;
-  typename T::type* const out = to + i / n / heads * s0 + i / n % heads * s1 + i % n * s2;
-  for (int e = threadIdx.x & 63; e < d; e += 64) {
-    float t = 0.f;
-    for (int s = 0; s < splits; ++s) t += part[(s * vectors + i) * D + slot_of(e, d)];
-    out[e] = (typename T::type)t;
+// Vectors: D / 4 lanes each, a quad a lane; [tensor][splits][vectors][D] -> the tensors (dk and dv, or dq alone).
+struct Sums {
+  const float* part;
+  void* to[2];
+  long stride[2][3];
+  int splits, heads, n, d;
+  long vectors;
+};
+template <class T, int D> __global__ __launch_bounds__(256) void sum_vectors_kernel(Sums p) {
+  constexpr int LANES = D / 4;
+  const long i = ((long)blockIdx.x * 256 + threadIdx.x) / LANES;
+  const int q = threadIdx.x % LANES, which = blockIdx.y;
+  if (i >= p.vectors || 4 * q >= p.d) return;
+  float t[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < p.splits; ++s) {
+    float x[4];
+    read16(p.part + ((which * p.splits + s) * p.vectors + i) * D + 4 * q, x);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) t[e] += x[e];
   }
+  const long (&st)[3] = p.stride[which];
+  store_quad<T>(static_cast<typename T::type*>(p.to[which]) + i / p.n / p.heads * st[0] + i / p.n % p.heads * st[1] + i % p.n * st[2], q, p.d, t[0], t[1], t[2], t[3]);
 }
 // dtable: one wave per (head, bucket); partials [batch][heads][per][n_buckets]
 template <class T> __global__ __launch_bounds__(64) void sum_table_kernel(const float* part, int batch, int heads, int per, int n_buckets, typename T::type* out) {
@@ -493,11 +504,10 @@ template <class T> __global__ __launch_bounds__(64) void sum_table_kernel(const 
   if (threadIdx.x == 0) out[blockIdx.x] = (typename T::type)t;
 }
 
-template <class T> void sum_vectors(const float* part, int splits, int D, void* to, const long* stride, int batch, int heads, int n, int d, hipStream_t stream) {
-  const long vectors = (long)batch * heads * n;
-  const auto kernel = D == 32 ? sum_vectors_kernel<T, 32> : D == 64 ? sum_vectors_kernel<T, 64> : sum_vectors_kernel<T, 128>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)((vectors + 3) / 4)), dim3(256), 0, stream, part, splits, static_cast<typename T::type*>(to), stride[0], stride[1],
-                     stride[2], heads, n, d, vectors);
+template <class T, int D> void sum_vectors(const float* part, int splits, int tensors, void* const (&to)[2], const long* s0, const long* s1, int batch, int heads, int n, int d,
+                                           hipStream_t stream) {
+  const Sums p{part, {to[0], to[1]}, {{s0[0], s0[1], s0[2]}, {s1[0], s1[1], s1[2]}}, splits, heads, n, d, (long)batch * heads * n};
+  hipLaunchKernelGGL((sum_vectors_kernel<T, D>), dim3((unsigned)((p.vectors * (D / 4) + 255) / 256), (unsigned)tensors), dim3(256), 0, stream, p);
 }
 
 template <class T, int D> void backward_d(Args& p, const Plans& plans, float* partial_q, float* partial_kv, hipStream_t stream) {
@@ -513,7 +523,7 @@ template <class T, int D> void backward_d(Args& p, const Plans& plans, float* pa
     if (waves_q == 1) launch(grad_q_kernel<T, D, 1>, p, 1, lds_q, stream);
   }
   if (waves_q != 1) launch(grad_q_kernel<T, D, 4>, p, 4, lds_q, stream);
-  if (plans.grad_q.splits > 1) sum_vectors<T>(partial_q, plans.grad_q.splits, D, a.gq, a.gq_stride, a.batch, a.heads, a.n_q, a.d, stream);
+  if (plans.grad_q.splits > 1) sum_vectors<T, D>(partial_q, plans.grad_q.splits, 1, {a.gq, nullptr}, a.gq_stride, a.gq_stride, a.batch, a.heads, a.n_q, a.d, stream);
   if (a.gtable)
     hipLaunchKernelGGL(sum_table_kernel<T>, dim3((unsigned)(a.heads * a.n_buckets)), dim3(64), 0, stream, p.gtable_partial, a.batch, a.heads,
                        plans.grad_q.splits * plans.grad_q.tiles, a.n_buckets, static_cast<typename T::type*>(a.gtable));
@@ -524,11 +534,8 @@ template <class T, int D> void backward_d(Args& p, const Plans& plans, float* pa
     if (plans.grad_kv.waves == 1) launch(grad_kv_kernel<T, D, 1>, p, 1, lds_kv, stream);
   }
   if (plans.grad_kv.waves != 1) launch(grad_kv_kernel<T, D, 4>, p, 4, lds_kv, stream);
-  if (plans.grad_kv.splits > 1) {
-    const long columns = (long)a.batch * a.kv_heads * a.n_k;
-    sum_vectors<T>(partial_kv, plans.grad_kv.splits, D, a.gk, a.gk_stride, a.batch, a.kv_heads, a.n_k, a.d, stream);
-    sum_vectors<T>(partial_kv + plans.grad_kv.splits * columns * D, plans.grad_kv.splits, D, a.gv, a.gv_stride, a.batch, a.kv_heads, a.n_k, a.d, stream);
-  }
+  if (plans.grad_kv.splits > 1)
+    sum_vectors<T, D>(partial_kv, plans.grad_kv.splits, 2, {a.gk, a.gv}, a.gk_stride, a.gv_stride, a.batch, a.kv_heads, a.n_k, a.d, stream);
 }
 template <class T> void backward(Args p, const Plans& plans, float* partial_q, float* partial_kv, hipStream_t stream) {
   if (plans.D == 32) backward_d<T, 32>(p, plans, partial_q, partial_kv, stream);
