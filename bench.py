@@ -487,7 +487,7 @@ def measure_example_network(torch, name, steps, warmup, batch=32):
     out = {"workload": "%s training step (s2cnn_amd/harness.py), batch %d, synthetic data" % (name, batch),
            "ms_per_step": round(ms, 3), "samples_per_s": round(batch / (ms * 1e-3), 1), "first_loss": round(losses[0], 4),
            "last_loss": round(losses[-1], 4), "library_ms": round(sum(calls.values()), 3), "library_calls_ms": calls}
-    if name == "mnist":
+    if name in ("mnist", "sphere_transformer"):
         # the same step captured into one HIP graph and replayed (the eager step is bound by its launches)
         _, rlosses, rms = harness.train_steps_replayed(name, batch=batch, steps=max(steps, 20), warmup=3, lr=0.01)
         out["graph_replay"] = {"ms_per_step": round(rms, 3), "samples_per_s": round(batch / (rms * 1e-3), 1),
@@ -535,7 +535,7 @@ def main():
                     help="also time the per-volume 64^3 kernels with their Wigner contraction compiled out (adds a `fft_floor` object)")
     ap.add_argument("--overlap", action="store_true",
                     help="also time a transform and a product of half the layer's batch on one stream and on two (adds an `overlap` object)")
-    ap.add_argument("--network", nargs="?", const="config5", default=None, choices=["config5", "mnist", "shrec17", "shrec17_original"],
+    ap.add_argument("--network", nargs="?", const="config5", default=None, choices=["config5", "mnist", "shrec17", "shrec17_original", "sphere_transformer"],
                     help="also time a whole network, forward + backward (adds a `network` object): config5 = the SHREC17-shaped "
                          "network of benchmark config 5 (default); mnist, shrec17, shrec17_original = the reference's example "
                          "networks (s2cnn_amd/harness.py) in a training step with SGD on a synthetic batch of 32")

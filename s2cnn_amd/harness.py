@@ -11,6 +11,9 @@ other (examples/shrec17/train.py:123 saves `model.state_dict()`, examples/shrec1
   Shrec17ModelOriginal examples/shrec17/model_original.py   features 6, 50, 70, 350, bandwidths 128, 32, 22, 7, maximum over the
                                                             grid instead of the integral, BatchNorm1d in the output layer
 
+  SphereTransformer    (not of the reference)               S2Conv 6->96 (b 64->10), ReLU, mean over gamma, two transformer blocks
+                                                            over the 400 points, attention pooling, Linear, log_softmax
+
 Data sets, loaders and logging of the reference's scripts are not reproduced: `train_steps` feeds a fixed synthetic batch.
 """
 import time
@@ -20,7 +23,7 @@ import torch.nn.functional as F
 from torch import nn
 
 from .soft.bn_relu import evaluate_sequence, run_sequence
-from . import (S2Convolution, SO3Convolution, s2_equatorial_grid, s2_near_identity_grid, so3_equatorial_grid, so3_integrate,
+from . import (S2Convolution, S2Transformer, SO3Convolution, s2_equatorial_grid, s2_near_identity_grid, so3_equatorial_grid, so3_integrate,
                so3_near_identity_grid)
 
 
@@ -106,11 +109,30 @@ class Shrec17ModelOriginal(nn.Module):
         return F.log_softmax(self.out_layer(x), dim=1)
 
 
+class SphereTransformer(nn.Module):
+    """Not of the reference: its first spectral layer, local features by correlation, then a transformer over the points of the
+    sphere in place of further layers and of the integral.  S2Conv 6->96 (b 64->10, kernel about the identity), ReLU, the
+    mean over gamma (a signal on the sphere), two blocks of 6 heads with a bias by 32 buckets of the angle, pooling, Linear."""
+
+    def __init__(self, nclasses, dropout=0.1):
+        super().__init__()
+        features, b_in, b = 96, 64, 10
+        grid = s2_near_identity_grid(n_alpha=8, max_beta=0.2, n_beta=2)
+        self.conv = S2Convolution(nfeature_in=6, nfeature_out=features, b_in=b_in, b_out=b, grid=grid, activation="relu")
+        self.transformer = S2Transformer(features, heads=6, b=b, layers=2, dropout=dropout)
+        self.out_layer = nn.Linear(features, nclasses)
+
+    def forward(self, x):  # pylint: disable=W0221
+        x = self.conv(x).mean(-1)                                           # [batch, feature, beta, alpha]
+        return F.log_softmax(self.out_layer(self.transformer(x)), dim=1)
+
+
 NETWORKS = {
     # name: (constructor, input shape without the batch, number of classes, loss on the network's output)
     "mnist": (S2ConvNet_original, (1, 60, 60), 10, F.cross_entropy),                       # examples/mnist/run.py:211-223
     "shrec17": (lambda: Shrec17Model(55), (6, 128, 128), 55, F.nll_loss),                  # examples/shrec17/train.py:70-82
     "shrec17_original": (lambda: Shrec17ModelOriginal(55), (6, 256, 256), 55, F.nll_loss),
+    "sphere_transformer": (lambda: SphereTransformer(55), (6, 128, 128), 55, F.nll_loss),
 }
 
 

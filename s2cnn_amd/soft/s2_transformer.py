@@ -1,0 +1,122 @@
+"""Layers of a transformer over the points of the sphere: every point attends to every other (or to those within an angle), with a
+learned bias by the angle of the two and with the quadrature weights of the points, and a learned query attends to all of them
+in place of the integral.  The reference has neither (its layers mix places by correlation with a local kernel,
+s2cnn/soft/so3_conv.py:36-58, and by the integral at the end, so3_integrate.py:7-31); they go between its layers and its head.
+
+Rotations about the polar axis by a grid step permute the points of a ring and leave angles and weights as they are: the
+block commutes with them exactly, with other rotations as far as the grid resolves the signal.
+"""
+import math
+
+import torch
+import torch.nn.functional as F
+from torch import nn
+
+from ..attention import attention, s2_angle_buckets, s2_log_weights
+from ..layer_norm import dropout_add_layer_norm, layer_norm
+from ..s2_grid import s2_soft_grid
+
+
+class _Norm(nn.Module):
+    """Weight and bias of a layer normalisation; the names of nn.LayerNorm."""
+
+    def __init__(self, features):
+        super().__init__()
+        self.weight = nn.Parameter(torch.ones(features))
+        self.bias = nn.Parameter(torch.zeros(features))
+
+
+class _PointWeights(nn.Module):
+    """Logarithms of the quadrature weights, float32 whatever type the module is converted to (`Module.to` leaves integers alone):
+    rounded to 16 bits they would be off by a hundredth."""
+
+    def __init__(self, b):
+        super().__init__()
+        self.register_buffer("bits", s2_log_weights(b).view(torch.int32), persistent=False)
+
+    def forward(self):  # pylint: disable=W
+        return self.bits.view(torch.float32)
+
+
+class S2TransformerBlock(nn.Module):
+    """Attention over the 4 b^2 points of the 2b x 2b grid and a pointwise network, each with a residual and a normalisation
+    before it.  Between the sublayers the residual, the dropout and the next normalisation are one pass over the features.
+
+    The block takes and gives the pair (h, y): the residual stream, and its normalisation by the block's first norm.  `norm`
+    makes the first pair of a stack; the last normalisation of a block is that of the block after it (`next_norm`).
+    """
+
+    def __init__(self, features, heads, b, n_buckets=32, max_angle=math.pi, hidden=None, dropout=0.0):
+        super().__init__()
+        assert features % heads == 0
+        self.features, self.heads, self.b, self.dropout = features, heads, b, dropout
+        hidden = 2 * features if hidden is None else hidden
+        self.norm1, self.norm2 = _Norm(features), _Norm(features)
+        self.qkv, self.out = nn.Linear(features, 3 * features), nn.Linear(features, features)
+        self.expand, self.contract = nn.Linear(features, hidden), nn.Linear(hidden, features)
+        self.bias_table = nn.Parameter(torch.zeros(heads, n_buckets))
+        self.register_buffer("buckets", s2_angle_buckets(s2_soft_grid(b), n_buckets=n_buckets, max_angle=max_angle), persistent=False)
+        self.log_weights = _PointWeights(b)
+
+    def norm(self, h):
+        """(h, y) of the residual stream h [batch, points, features]"""
+        return h, layer_norm(h, self.norm1.weight, self.norm1.bias)
+
+    def _step(self, x, h, seed, norm):
+        p = self.dropout if self.training else 0.0
+        return dropout_add_layer_norm(x.to(h.dtype), h, p, seed, norm.weight, norm.bias)
+
+    def forward(self, h, y, next_norm, seeds):  # pylint: disable=W
+        """(h, y) [batch, points, features] -> (h, y), y normalised by next_norm; seeds: two seeds for the dropout of this call"""
+        batch, points, features = h.shape
+        assert points == 4 * self.b ** 2
+        q, k, v = self.qkv(y).view(batch, points, 3, self.heads, features // self.heads).permute(2, 0, 3, 1, 4)
+        x = attention(q, k, v, table=self.bias_table.to(q.dtype), buckets=self.buckets, key_bias=self.log_weights())
+        x = self.out(x.transpose(1, 2).reshape(batch, points, features))
+        h, y = self._step(x, h, seeds[0], self.norm2)
+        x = self.contract(F.relu(self.expand(y)))
+        return self._step(x, h, seeds[1], next_norm)
+
+
+class S2AttentionPool(nn.Module):
+    """One learned query per head attends to all points, with their quadrature weights: [batch, points, features] ->
+    [batch, features].  With queries of zeros (as at the start) it is the integral of the values over the sphere."""
+
+    def __init__(self, features, heads, b):
+        super().__init__()
+        assert features % heads == 0
+        self.heads = heads
+        self.query = nn.Parameter(torch.zeros(heads, 1, features // heads))
+        self.kv = nn.Linear(features, 2 * features)
+        self.log_weights = _PointWeights(b)
+
+    def forward(self, y):  # pylint: disable=W
+        batch, points, features = y.shape
+        k, v = self.kv(y).view(batch, points, 2, self.heads, features // self.heads).permute(2, 0, 3, 1, 4)
+        q = self.query.to(k.dtype).expand(batch, -1, -1, -1)
+        return attention(q, k, v, key_bias=self.log_weights()).reshape(batch, features)
+
+
+class S2Transformer(nn.Module):
+    """A stack of blocks and the pooling after it: [batch, features, 2b, 2b] -> [batch, features].  `drops` counts the forward passes on
+    the device, so that each training step drops others, replayed from a graph too."""
+
+    def __init__(self, features, heads, b, layers, n_buckets=32, max_angle=math.pi, dropout=0.0):
+        super().__init__()
+        self.blocks = nn.ModuleList(S2TransformerBlock(features, heads, b, n_buckets, max_angle, dropout=dropout) for _ in range(layers))
+        self.last_norm = _Norm(features)
+        self.pool = S2AttentionPool(features, heads, b)
+        self.register_buffer("drops", torch.zeros(1, dtype=torch.int64))
+        self.register_buffer("calls", torch.arange(2 * layers), persistent=False)
+
+    def forward(self, x):  # pylint: disable=W
+        h = x.flatten(2).transpose(1, 2).contiguous()                       # [batch, points, features]
+        seeds = self.calls.split(1)
+        if self.training:
+            self.drops.add_(1)
+            seeds = (self.drops * (2 * len(self.blocks)) + self.calls).split(1)
+        h, y = self.blocks[0].norm(h)
+        for i, block in enumerate(self.blocks):
+            following = self.blocks[i + 1].norm1 if i + 1 < len(self.blocks) else self.last_norm
+            h, y = block(h, y, following, seeds[2 * i:2 * i + 2])
+        return self.pool(y)

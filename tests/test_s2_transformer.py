@@ -1,0 +1,146 @@
+"""The transformer over the points of the sphere (s2cnn_amd/soft/s2_transformer.py) against its formulas in 64 bits on the CPU, its
+symmetry, its training step eager and replayed from a graph.
+
+Tolerance of outputs and gradients: ten products, normalisations and attentions one after the other, each of which may add what a
+float32 attention may (128 * 2^-24 in the 2-norm), twice that for gradients: 1e-4 and 2e-4."""
+import io
+import math
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+import s2cnn_amd
+from s2cnn_amd import harness
+
+
+def _stack(**kw):
+    torch.manual_seed(5)
+    model = s2cnn_amd.S2Transformer(**{**dict(features=24, heads=3, b=3, layers=2, n_buckets=6), **kw})
+    for name, p in model.named_parameters():             # nothing left at zero or one
+        if name.endswith("bias_table") or name.endswith("query") or "norm" in name:
+            p.data += 0.5 * torch.randn(p.shape)
+    return model
+
+
+def _plain(model, x, masks, heads):
+    """The same function in torch's own operators; masks: what each dropout multiplies by."""
+    def norm(h, m):
+        return F.layer_norm(h, h.shape[-1:], m.weight, m.bias)
+
+    def split(t, n):
+        return t.unflatten(-1, (n, heads, t.shape[-1] // (n * heads))).permute(2, 0, 3, 1, 4)
+
+    h = x.flatten(2).transpose(1, 2)
+    for i, block in enumerate(model.blocks):
+        q, k, v = split(block.qkv(norm(h, block.norm1)), 3)
+        n = block.buckets.long()
+        s = q @ k.transpose(-1, -2) / math.sqrt(q.shape[-1]) + block.bias_table[:, n.clamp(min=0)] + block.log_weights().to(q.dtype)
+        a = torch.softmax(s.masked_fill(n < 0, -math.inf), -1) @ v
+        h = h + masks[2 * i] * block.out(a.transpose(1, 2).flatten(2))
+        h = h + masks[2 * i + 1] * block.contract(F.relu(block.expand(norm(h, block.norm2))))
+    k, v = split(model.pool.kv(norm(h, model.last_norm)), 2)
+    s = (model.pool.query * k).sum(-1) / math.sqrt(k.shape[-1]) + model.pool.log_weights().to(k.dtype)
+    return (torch.softmax(s, -1).unsqueeze(-1) * v).sum(-2).flatten(1)
+
+
+def _relative(a, b):
+    a, b = a.detach().double().cpu(), b.detach()
+    return float((a - b).norm() / b.norm())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("p,angle", [(0.0, math.pi), (0.25, 1.2)])
+def test_equals_the_formulas(hip, p, angle):
+    model = _stack(max_angle=angle, dropout=p)
+    plain = _stack(max_angle=angle, dropout=p).double()
+    x, g = torch.randn(2, 24, 6, 6), torch.randn(2, 24)
+    model.cuda()
+    xg = x.cuda().requires_grad_()
+    xp = x.double().requires_grad_()
+    y = model(xg)
+    y.backward(g.cuda())
+    seeds = [4 + i for i in range(4)]                    # first call: drops = 1, four dropouts a call
+    masks = [s2cnn_amd.dropout(torch.ones(2, 36, 24, device="cuda"), p, s).double().cpu() for s in seeds]
+    want = _plain(plain, xp, masks, 3)
+    want.backward(g.double())
+    assert _relative(y, want) < 1e-4
+    assert _relative(xg.grad, xp.grad) < 2e-4
+    for (name, a), b in zip(model.named_parameters(), plain.parameters()):
+        assert _relative(a.grad, b.grad) < 2e-4 or float(b.grad.norm()) < 1e-9, name
+
+
+@pytest.mark.gpu
+def test_invariant_under_rotations_about_the_axis(hip):
+    """A rotation by a grid step about the polar axis permutes the points of each ring: the blocks permute with them, the pooling
+    does not see it.  Sums in another order: 1e-4 as above."""
+    model = _stack(b=4, n_buckets=16).cuda().eval()
+    x = torch.randn(2, 24, 8, 8, device="cuda")
+    with torch.no_grad():
+        a, b = model(x), model(x.roll(3, -1))
+    assert _relative(b, a.double().cpu()) < 1e-4
+
+
+@pytest.mark.gpu
+def test_pooling_starts_as_the_integral(hip):
+    """Queries of zeros: the mean of the values with the quadrature weights."""
+    torch.manual_seed(1)
+    pool = s2cnn_amd.S2AttentionPool(16, 2, 5).cuda()
+    y = torch.randn(3, 100, 16, device="cuda")
+    w = pool.log_weights().double().exp()
+    want = torch.einsum("p,bpf->bf", w / w.sum(), pool.kv(y)[..., 16:].double())
+    assert _relative(pool(y), want.detach().cpu()) < 1e-5
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_sixteen_bit_and_autocast(hip, dtype):
+    """Twenty roundings one after the other, each of half a unit: 10 units of the type in the 2-norm."""
+    model, plain = _stack(), _stack().double()
+    x = torch.randn(2, 24, 6, 6)
+    want = _plain(plain, x.double(), [1.0] * 4, 3).detach()
+    unit = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -11
+    with torch.no_grad():
+        model.cuda().eval()
+        with torch.autocast("cuda", dtype=dtype):
+            cast = model(x.cuda())
+        assert _relative(cast, want) < 10 * unit
+        assert _relative(model.to(dtype)(x.cuda().to(dtype)), want) < 10 * unit
+
+
+@pytest.mark.gpu
+def test_network_trains_and_reloads(hip):
+    model, losses, _ = harness.train_steps("sphere_transformer", batch=8, steps=8, warmup=0, lr=0.02)
+    print("sphere transformer losses:", ["%.4f" % l for l in losses], flush=True)
+    assert all(l == l for l in losses) and losses[-1] < losses[0]
+    x, _ = harness.synthetic_batch("sphere_transformer", 8, "cuda:0")
+    model.eval()
+    with torch.no_grad():
+        want = model(x)
+    buf = io.BytesIO()
+    torch.save(model.state_dict(), buf)
+    buf.seek(0)
+    twin = harness.NETWORKS["sphere_transformer"][0]().cuda()
+    twin.load_state_dict(torch.load(buf, weights_only=True))
+    twin.eval()
+    with torch.no_grad():
+        assert torch.equal(twin(x), want)
+
+
+@pytest.mark.gpu
+def test_step_replayed_from_a_graph(hip):
+    """Each replay drops other elements than the one before: the losses are those of as many eager steps."""
+    _, eager, _ = harness.train_steps("sphere_transformer", batch=4, steps=5, warmup=3, lr=0.02)
+    _, replayed, _ = harness.train_steps_replayed("sphere_transformer", batch=4, steps=5, warmup=3, lr=0.02)
+    print("eager", ["%.5f" % l for l in eager[3:]], "replayed", ["%.5f" % l for l in replayed], flush=True)
+    assert max(abs(a - b) for a, b in zip(eager[3:], replayed)) < 1e-4 * abs(eager[0])
+
+
+def test_refusals():
+    with pytest.raises(AssertionError):
+        s2cnn_amd.S2TransformerBlock(25, 3, 3)
+    with pytest.raises(AssertionError):
+        s2cnn_amd.S2AttentionPool(25, 3, 3)
+    block = s2cnn_amd.S2TransformerBlock(24, 3, 3)
+    with pytest.raises(AssertionError):
+        block(torch.zeros(1, 35, 24), torch.zeros(1, 35, 24), block.norm1, (1, 2))
