@@ -444,7 +444,7 @@ typedef struct s2cnn_attention_t {
   float scale;
 } s2cnn_attention_t;
 
-#define S2CNN_ATTENTION_STRIDE_LIMIT (1L << 26)   /* strides of vectors of q, k, v, gout and of rows of buckets are below this */
+#define S2CNN_ATTENTION_STRIDE_LIMIT (1L << 25)   /* strides of vectors of q, k, v, gout and of rows of buckets are below this */
 size_t s2cnn_attention_stats_floats(const s2cnn_attention_t *a);
 size_t s2cnn_attention_workspace(const s2cnn_attention_t *a, int backward);     /* 0 also for sizes that are refused */
 int s2cnn_attention_fwd(const s2cnn_attention_t *a, void *workspace, size_t workspace_bytes, void *stream);

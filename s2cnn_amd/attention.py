@@ -21,8 +21,8 @@ MAX_BUCKETS = 64
 
 
 def _vectors(t):
-    """`t` as the kernels read it: vectors contiguous, less than 2^26 entries apart."""
-    return t if (t.stride(-1) == 1 or t.size(-1) == 1) and t.stride(-2) < 1 << 26 else t.contiguous()
+    """`t` as the kernels read it: vectors contiguous, less than 2^25 entries apart."""
+    return t if (t.stride(-1) == 1 or t.size(-1) == 1) and t.stride(-2) < 1 << 25 else t.contiguous()
 
 
 def _like(t):

@@ -173,6 +173,25 @@ template <class T> __device__ __forceinline__ Quad load_four(const typename T::t
   }
   return v;
 }
+// the same from a uniform pointer and an offset in bytes: a scalar address and one register a lane, which the compiler would otherwise
+// make 64-bit sums in every lane
+template <class T> __device__ __forceinline__ Quad load_four_at(const typename T::type* uniform, unsigned bytes) {
+  typedef unsigned words4 __attribute__((ext_vector_type(4), aligned(4), may_alias));
+  typedef unsigned words2 __attribute__((ext_vector_type(2), aligned(2), may_alias));
+  typedef const __attribute__((address_space(1))) char global_bytes;
+  unsigned long long address = reinterpret_cast<unsigned long long>(uniform);
+  asm("" : "+s"(address), "+v"(bytes));
+  global_bytes* const p = reinterpret_cast<global_bytes*>(address) + bytes;
+  Quad v;
+  if constexpr (T::PARTS == 3) {
+    const words4 u = *reinterpret_cast<const __attribute__((address_space(1))) words4*>(p);
+    v.w = make_uint4(u.x, u.y, u.z, u.w);
+  } else {
+    const words2 u = *reinterpret_cast<const __attribute__((address_space(1))) words2*>(p);
+    v.w = make_uint4(u.x, u.y, 0, 0);
+  }
+  return v;
+}
 template <class T> __device__ __forceinline__ Quad load_quad(const typename T::type* p, int q, int d) {
   Quad v = load_four<T>(p + quad_at(q, d));
   // So many of its first entries count as zero.  A column's quads each have their own number and four conditions on it, which the
@@ -334,7 +353,7 @@ template <class T, int D, int W> constexpr int buffers(int layouts) { return W >
 // Two tensors staged by the same tiles of rows, in the layouts LA and LB (those of the first, then those of the second): THREADS threads
 // fetch the blocks of a tile into registers, and write them later.
 // The address of a block's rows is a uniform pointer, moved on by the tile, and an offset of the thread that stays (below
-// 2^31 bytes: the entry checks 32 strides).
+// 2^32 bytes: the entry checks 32 strides).
 template <class T, int D, int THREADS, int LA, int LB> struct Stage {
   typedef Tile<T, D> Tl;
   typedef typename T::type E;
@@ -342,6 +361,7 @@ template <class T, int D, int THREADS, int LA, int LB> struct Stage {
   static constexpr int PER = (2 * Tl::BLOCKS + THREADS - 1) / THREADS;
   static constexpr bool IDLE = 2 * Tl::BLOCKS % THREADS != 0;      // some threads have no block
   Quad v[PER][4];
+  unsigned offset[PER];
 
   // of the thread's block u: which tensor (uniform in a wave), and which block of it
   static __device__ __forceinline__ bool second(int u, int tid) {
@@ -351,21 +371,34 @@ template <class T, int D, int THREADS, int LA, int LB> struct Stage {
   static __device__ __forceinline__ bool idle(int u, int tid) { return IDLE && __builtin_amdgcn_readfirstlane(u * THREADS + tid) >= 2 * Tl::BLOCKS; }
   static __device__ __forceinline__ int block(int u, int tid) { return (u * THREADS + tid) % Tl::BLOCKS; }
 
+  // bytes from the tile's first row to row i of block u, or to row `last` if that comes before it
+  static __device__ __forceinline__ unsigned place(const Vectors<T>& x, int u, int tid, int i, int last) {
+    const int kk = block(u, tid);
+    return (unsigned)sizeof(E) * (unsigned)(min(4 * (kk / (D / 4)) + i, last) * (int)x.stride + quad_at(kk % (D / 4), x.d));
+  }
+  // before the first fetch; the strides and sizes are those of all
+  __device__ __forceinline__ void prepare(const Vectors<T>& a, const Vectors<T>& b, int tid) {
+    if constexpr (THREADS == 64) return;                   // a wave has too many blocks to keep their offsets
+#pragma unroll
+    for (int u = 0; u < PER; ++u) offset[u] = place(second(u, tid) ? b : a, u, tid, 0, ROWS);
+  }
+
   // blocks [U0, U1) of the thread
   template <int U0 = 0, int U1 = PER> __device__ __forceinline__ void fetch(const Vectors<T>& a, const Vectors<T>& b, int row0, int tid) {
 #pragma unroll
     for (int u = U0; u < U1; ++u) {
       if (idle(u, tid)) break;
       const Vectors<T>& x = second(u, tid) ? b : a;
-      const int kk = block(u, tid), q = kk % (D / 4), row = 4 * (kk / (D / 4));
       const E* const base = x.base + (long)row0 * x.stride;
-      const int stride = (int)x.stride, left = x.n - 1 - row0, at = quad_at(q, x.d);     // left: last row of the tile that exists
+      const int left = x.n - 1 - row0;                     // last row of the tile that exists
       if (left >= ROWS - 1) {
+        const unsigned at = THREADS == 64 ? place(x, u, tid, 0, ROWS) : offset[u];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[u][i] = load_four<T>(base + i * x.stride + (unsigned)(row * stride + at));
+        for (int i = 0; i < 4; ++i) v[u][i] = load_four_at<T>(base + i * x.stride, at);
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[u][i] = load_four<T>(base + (unsigned)(min(row + i, left) * stride + at));
+        for (int i = 0; i < 4; ++i) v[u][i] = load_four_at<T>(base, place(x, u, tid, i, left));
+        asm volatile("");                                  // keeps the last load of both branches from becoming one, of a 64-bit address
       }
     }
   }
@@ -518,6 +551,13 @@ __device__ __forceinline__ int work_of_block(int workgroups) {
   const int per = (workgroups + 7) / 8;
   return (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
 }
+// Signal and head of group i of per heads a signal.  The heads of a signal are neighbours, on one XCD; where signals have lengths of their
+// own, the signals of a head are, so that no XCD has the longest ones alone.
+struct Group { int b, head; };
+__device__ __forceinline__ Group group_of(const s2cnn_attention_t& a, int i, int per) { return a.lengths ? Group{i % a.batch, i / a.batch} : Group{i / per, i % per}; }
+// Tiles of one number see as many pairs in every group (near the poles of a grid with a bias over near points: few), and a CU's workgroups
+// are 32 apart: each group's tiles are turned by three eighths.
+__device__ __forceinline__ int tile_of(const Args& p, int work, int group) { return (work + group % 8 * (p.tiles * 3 / 8)) % p.tiles; }
 inline unsigned blocks_for(int workgroups) { return (unsigned)((workgroups + 7) / 8 * 8); }
 
 

@@ -54,8 +54,9 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
 
   const int work = work_of_block(p.workgroups);
   if (work >= p.workgroups) return;
-  const int tile = work % p.tiles, split = work / p.tiles % p.splits, bh = work / p.tiles / p.splits;
-  const int b = bh / a.heads, head = bh % a.heads, hk = head / (a.heads / a.kv_heads);
+  const int split = work / p.tiles % p.splits, bh = work / p.tiles / p.splits, tile = tile_of(p, work, bh);
+  const Group of = group_of(a, bh, a.heads);
+  const int b = of.b, head = of.head, hk = head / (a.heads / a.kv_heads);
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6;
   const int query_ = tile * 32 * W + wave * 32 + (lane & 31);
   const bool ok = query_ < a.n_q;
@@ -80,6 +81,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
   Stage<T, D, 64 * W, BOTH, BY_ROWS> stage;
   unsigned words[4] = {0, 0, 0, 0};
   if (key0 < end) {
+    stage.prepare(k, v, tid);
     if (W > 1) stage.fetch(k, v, key0, tid);
     if (buckets) load_buckets(buckets, key0, end, half, words);
   }
@@ -93,7 +95,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
   const float* const o_row = T::PARTS == 3 ? static_cast<const float*>(a.out) + b * a.out_stride[0] + head * a.out_stride[1] + query * a.out_stride[2] : a.out_f32 + row * a.d;
   const float2 stats = reinterpret_cast<const float2*>(a.stats)[row];
   const float m = ok ? stats.x : pinf(), inv_l = ok ? stats.y : 0.f;
-  const bool live = inv_l != 0.f;                          // a row without keys takes no part, whatever its gradient holds
+  const bool live = inv_l != 0.f, active = __any(live);    // a row without keys takes no part, whatever its gradient holds
   load_column<T, D>(static_cast<const E*>(a.q) + b * a.q_stride[0] + head * a.q_stride[1] + query * a.q_stride[2], a.d, live, half,
                     a.scale * LOG2E, qf);
   // The matrix cores round sums down, not to nearest: a bias of a fraction of a unit in dp's last place, lost in the noise everywhere but
@@ -175,7 +177,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
     if (W > 1 && key + BUFS * ROWS < end) stage.fetch(k, v, key + BUFS * ROWS, tid);
     if (more && buckets) load_buckets(buckets, key + ROWS, end, half, words);
 
-    if (!buckets || !none_takes_part(now)) {
+    if (active && (!buckets || !none_takes_part(now))) {
       v16f s, dp = {};
       start_scores<T>(s, kb, half, buckets != nullptr, now, lds_table, a.n_buckets, p.inv_c);
 #pragma unroll
@@ -218,7 +220,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
 
   if (table_grad) {
     __syncthreads();
-    float* const part = p.gtable_partial + ((long)bh * p.splits * p.tiles + split * p.tiles + tile) * a.n_buckets;
+    float* const part = p.gtable_partial + (((long)b * a.heads + head) * p.splits * p.tiles + split * p.tiles + tile) * a.n_buckets;
     for (int n = tid; n < a.n_buckets; n += 64 * W) {
       unsigned long long t = 0;
       for (int i = 0; i < TableSums::COPIES; ++i) t += lds_sums[n * TableSums::COPIES + ((i + n) & 63)];   // lanes start at banks of their own
@@ -251,8 +253,9 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
 
   const int work = work_of_block(p.workgroups);
   if (work >= p.workgroups) return;
-  const int tile = work % p.tiles, split = work / p.tiles % p.splits, bh = work / p.tiles / p.splits;
-  const int b = bh / a.kv_heads, hk = bh % a.kv_heads, group = a.heads / a.kv_heads;
+  const int split = work / p.tiles % p.splits, bh = work / p.tiles / p.splits, tile = tile_of(p, work, bh);
+  const Group of = group_of(a, bh, a.kv_heads);
+  const int b = of.b, hk = of.head, group = a.heads / a.kv_heads;
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6;
   const int key_ = tile * 32 * W + wave * 32 + (lane & 31);
   const bool ok = key_ < a.n_k;
@@ -271,7 +274,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
   const float* const key_bias = a.key_bias ? a.key_bias + b * a.key_bias_stride : nullptr;
   const signed char* const buckets = a.buckets ? a.buckets + b * a.bucket_stride[0] : nullptr;
   const float dead = ninf() * p.inv_c, kb_c = ok ? key_value(load_key_bias(key_bias, key, a.n_k), key, end, p.inv_c) : dead, kb = kb_c * p.c;
-  const bool live = kb_c != dead;
+  const bool live = kb_c != dead, active = __any(live);
 
   Frag<T> kf[D / 16], vf[D / 16];
   load_column<T, D>(static_cast<const E*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[1] + key * a.k_stride[2], a.d, live, half,
@@ -348,6 +351,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
   };
   Place here{first / per_head, first % per_head * ROWS}, next = here.next(a.n_q), after = next.next(a.n_q);     // of this step, the next, the one after
   if (first < last) {
+    stage.prepare(queries(here, a.q, a.q_stride), queries(here, a.gout, a.gout_stride), tid);
     if (W > 1) fetch(here);
     if (buckets) fetch_buckets(here);
     if (tid < ROWS) put_row(0, here, load_row(here)), put_row(1, next, load_row(next));
@@ -390,7 +394,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
 #pragma unroll
       for (int g = 0; g < 4; ++g) words[g] = from[2 * g];
     }
-    if (!buckets || !none_takes_part(words)) {
+    if (active && (!buckets || !none_takes_part(words))) {
       // the scores start from the table's entries (float32: less m), dp from -delta
       v16f s = {}, dp;
       if (buckets) {

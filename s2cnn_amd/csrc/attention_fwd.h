@@ -20,12 +20,13 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
 
   const int work = work_of_block(p.workgroups);
   if (work >= p.workgroups) return;
-  const int tile = work % p.tiles, split = work / p.tiles % p.splits, bh = work / p.tiles / p.splits;
-  const int b = bh / a.kv_heads, hk = bh % a.kv_heads, group = a.heads / a.kv_heads;
+  const int split = work / p.tiles % p.splits, bh = work / p.tiles / p.splits, tile = tile_of(p, work, bh);
+  const Group of = group_of(a, bh, a.kv_heads);
+  const int b = of.b, hk = of.head, group = a.heads / a.kv_heads;
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int columns = group * a.n_q, column0 = tile * 32 * W;
   const int column = column0 + (tid >> 6) * 32 + (lane & 31);
-  const bool ok = column < columns;
+  const bool ok = column < columns, active = __any(ok);     // a wave without columns only stages
   const int c = ok ? column : columns - 1;
   const int head = hk * group + c / a.n_q, query = c % a.n_q;
   const int head0 = hk * group + column0 / a.n_q, heads = hk * group + min(columns - 1, column0 + 32 * W - 1) / a.n_q - head0 + 1;
@@ -48,6 +49,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
   Stage<T, D, 64 * W, BY_ROWS, BY_ENTRIES> stage;
   unsigned words[4] = {0, 0, 0, 0};
   if (key0 < end) {
+    stage.prepare(k, v, tid);
     if (W > 1) stage.fetch(k, v, key0, tid);
     if (buckets) load_buckets(buckets, key0, end, half, words);
   }
@@ -93,7 +95,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     if (buckets) place_buckets(words, now);
     if (more && buckets) load_buckets(buckets, key + ROWS, end, half, words);
 
-    if (!buckets || !none_takes_part(now)) {
+    if (active && (!buckets || !none_takes_part(now))) {
       v16f s;
       start_scores<T>(s, kb, half, buckets != nullptr, now, table, a.n_buckets, p.inv_c);
 #pragma unroll
@@ -136,7 +138,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     if (lane == 0) lds_kb[tid >> 6] = largest;
     __syncthreads();
     for (int i = 0; i < W; ++i) largest = fmaxf(largest, lds_kb[i]);
-    if (tid == 0) a.stats[2 * rows + bh * p.splits + split] = largest;
+    if (tid == 0) a.stats[2 * rows + (b * a.kv_heads + hk) * p.splits + split] = largest;
   }
   l = half_sum(l);
   if (!ok) return;
