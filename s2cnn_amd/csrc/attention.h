@@ -470,7 +470,8 @@ __device__ __forceinline__ float key_value(float bias, int key, int end, float i
 }
 
 // A tile's values of its rows (keys' biases; the queries' statistics) in LDS, in a ring: tile t's are read in step t, and in step
-// t - 1, in which its rows are written; they are put there in step t - 2.
+// t - 1, in which its rows are written; they are put there at the start of step t - 2, and loaded in step t - 3: put at that step's end
+// they would wait for its tile's loads too, which are issued after them.
 constexpr int RING = 4;
 
 // the table's rows of heads head0 .. head0 + heads - 1 in LDS, n_buckets + 1 entries a head, the last one for excluded pairs

@@ -86,6 +86,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
     if (buckets) load_buckets(buckets, key0, end, half, words);
   }
   if (tid < 2 * ROWS) lds_kb[tid] = key_value(key0 < end ? load_key_bias(key_bias, key0 + tid, end) : 0.f, key0 + tid, end, p.inv_c);
+  float bias_ahead = tid < ROWS && key0 < end ? load_key_bias(key_bias, key0 + 2 * ROWS + tid, end) : 0.f;
   if (buckets) stage_table<T>(lds_table, a.table, a.n_buckets, head, 1, tid, 64 * W);
   if (table_grad)
     for (int n = tid; n < TableSums::words(a.n_buckets); n += 64 * W) lds_sums[n] = 0;
@@ -170,10 +171,11 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
     const unsigned char* const lds_v = lds_k + 2 * Tl::BYTES;
     const float* const kb = lds_kb + step % RING * ROWS;
 
+    if (tid < ROWS) lds_kb[(step + 2) % RING * ROWS + tid] = key_value(bias_ahead, key + 2 * ROWS + tid, end, p.inv_c);
     if (BUFS == 2 && more) write(step + 1);
     unsigned now[4] = {0, 0, 0, 0};
     if (buckets) place_buckets(words, now);
-    const float bias_next = tid < ROWS ? load_key_bias(key_bias, key + 2 * ROWS + tid, end) : 0.f;
+    if (tid < ROWS) bias_ahead = load_key_bias(key_bias, key + 3 * ROWS + tid, end);
     if (W > 1 && key + BUFS * ROWS < end) stage.fetch(k, v, key + BUFS * ROWS, tid);
     if (more && buckets) load_buckets(buckets, key + ROWS, end, half, words);
 
@@ -215,7 +217,6 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
         for (int i = 0; i < D / 32; ++i) mma<T>(Tl::by_entries(lds_kt, i, t, lane), f, dq[i]);
       }
     }
-    if (tid < ROWS) lds_kb[(step + 2) % RING * ROWS + tid] = key_value(bias_next, key + 2 * ROWS + tid, end, p.inv_c);
   }
 
   if (table_grad) {
@@ -350,11 +351,12 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
     to[3 * BUCKET_LD] = __builtin_amdgcn_perm(b1, a1, 0x07060302u);
   };
   Place here{first / per_head, first % per_head * ROWS}, next = here.next(a.n_q), after = next.next(a.n_q);     // of this step, the next, the one after
+  Row ahead = {};
   if (first < last) {
     stage.prepare(queries(here, a.q, a.q_stride), queries(here, a.gout, a.gout_stride), tid);
     if (W > 1) fetch(here);
     if (buckets) fetch_buckets(here);
-    if (tid < ROWS) put_row(0, here, load_row(here)), put_row(1, next, load_row(next));
+    if (tid < ROWS) put_row(0, here, load_row(here)), put_row(1, next, load_row(next)), ahead = load_row(after);
   }
   if (buckets) stage_table<T>(lds_table, a.table, a.n_buckets, hk * group, group, tid, 64 * W);
   if (BUFS == 2) {
@@ -373,6 +375,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
     const unsigned char* const lds_g = lds_q + 2 * Tl::BYTES;
     const unsigned char* const lds_gt = lds_q + 3 * Tl::BYTES;
     __syncthreads();
+    if (tid < ROWS) put_row(step + 2, after, ahead);
     if (BUFS == 1) {
       write(step, here);
       if (buckets) write_buckets(step);
@@ -382,8 +385,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
       if (buckets) write_buckets(step + 1);
     }
     const float* const table = lds_table + here.head * (a.n_buckets + 1);
-    Row ahead = {};
-    if (tid < ROWS) ahead = load_row(after);
+    if (tid < ROWS) ahead = load_row(after.next(a.n_q));
     if (r + BUFS < last) {
       if (W > 1) fetch(BUFS == 1 ? next : after);
       if (buckets) fetch_buckets(BUFS == 1 ? next : after);
@@ -455,7 +457,6 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
         }
       }
     }
-    if (tid < ROWS) put_row(step + 2, after, ahead);
     here = next, next = after, after = after.next(a.n_q);
   }
 

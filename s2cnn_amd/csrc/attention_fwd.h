@@ -54,6 +54,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     if (buckets) load_buckets(buckets, key0, end, half, words);
   }
   if (tid < 2 * ROWS) lds_kb[tid] = key_value(key0 < end ? load_key_bias(key_bias, key0 + tid, end) : 0.f, key0 + tid, end, p.inv_c);
+  float bias_ahead = tid < ROWS && key0 < end ? load_key_bias(key_bias, key0 + 2 * ROWS + tid, end) : 0.f;
   if (buckets) stage_table<T>(lds_table, a.table, a.n_buckets, head0, heads, tid, 64 * W);
   Frag<T> qf[D / 16];
   load_column<T, D>(static_cast<const E*>(a.q) + b * a.q_stride[0] + head * a.q_stride[1] + query * a.q_stride[2], a.d, ok, half,
@@ -88,8 +89,9 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     const unsigned char* const lds_v = lds_k + Tl::BYTES;
     const float* const kb = lds_kb + step % RING * ROWS;
 
+    if (tid < ROWS) lds_kb[(step + 2) % RING * ROWS + tid] = key_value(bias_ahead, key + 2 * ROWS + tid, end, p.inv_c);
     if (BUFS == 2 && more) write(step + 1);
-    const float bias_next = tid < ROWS ? load_key_bias(key_bias, key + 2 * ROWS + tid, end) : 0.f;
+    if (tid < ROWS) bias_ahead = load_key_bias(key_bias, key + 3 * ROWS + tid, end);
     if (W > 1 && key + BUFS * ROWS < end) stage.fetch(k, v, key + BUFS * ROWS, tid);
     unsigned now[4] = {0, 0, 0, 0};
     if (buckets) place_buckets(words, now);
@@ -127,7 +129,6 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
         for (int i = 0; i < D / 32; ++i) mma<T>(Tl::by_entries(lds_v, i, t, lane), pf, o[i]);
       }
     }
-    if (tid < ROWS) lds_kb[(step + 2) % RING * ROWS + tid] = key_value(bias_next, key + 2 * ROWS + tid, end, p.inv_c);
   }
 
   const long row = ((long)b * a.heads + head) * a.n_q + query, rows = (long)a.batch * a.heads * a.n_q;
