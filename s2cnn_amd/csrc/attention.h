@@ -313,31 +313,34 @@ template <class T, int D> struct Tile {
     return f;
   }
 
-  // block k of the tile: rows 4 (k / (D / 4)), entries 4 (k % (D / 4)); LAYOUTS: which of the two
-  template <int LAYOUTS> static __device__ __forceinline__ void write(unsigned char* rows, unsigned char* entries, int k, const Quad (&v)[4]) {
-    const int q = k % (D / 4), kg = k / (D / 4);
+  // where block k of the tile (rows 4 (k / (D / 4)), entries 4 (k % (D / 4))) is written: its first row, its first entry.  The others
+  // are as many slots on, exclusive or: they differ in the two lowest bits of the slot alone
+  static __device__ __forceinline__ unsigned rows_at(int k) {
+    const int q = k % (D / 4), kg = k / (D / 4), s = q >> 2, h = (q >> 1) & 1;
+    return (unsigned)((s * 64 + row_slot(s, h, 4 * kg)) * 16 + (q & 1) * 8);
+  }
+  static __device__ __forceinline__ unsigned entries_at(int k) {
+    const int q = k % (D / 4), kg = k / (D / 4), b = q >> 3, t = kg >> 2, half = (kg >> 1) & 1, h = kg & 1;
+    return (unsigned)(((2 * b + t) * 64 + entry_slot(h, (4 * q) & 31)) * 16 + half * 8);
+  }
+  // a block into the layouts, at the places `at_rows` and `at_entries`; LAYOUTS: which of the two
+  template <int LAYOUTS> static __device__ __forceinline__ void write(unsigned char* rows, unsigned char* entries, unsigned at_rows, unsigned at_entries, const Quad (&v)[4]) {
     unsigned w[4][2][T::PARTS];                                    // [row][pair of entries][part]
 #pragma unroll
     for (int i = 0; i < 4; ++i) quad_parts<T>(v[i], w[i][0], w[i][1]);
     if constexpr ((LAYOUTS & BY_ROWS) != 0) {
-      const int s = q >> 2, h = (q >> 1) & 1;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int at = row_slot(s, h, 4 * kg + i);
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int p = 0; p < T::PARTS; ++p)
-          write8(rows + ((p * STEPS + s) * 64 + at) * 16 + (q & 1) * 8, w[i][0][p], w[i][1][p]);
-      }
+        for (int p = 0; p < T::PARTS; ++p) write8(rows + (at_rows ^ (16 * i)) + p * STEPS * 1024, w[i][0][p], w[i][1][p]);
     }
     if constexpr ((LAYOUTS & BY_ENTRIES) != 0) {
-      const int b = q >> 3, t = kg >> 2, half = (kg >> 1) & 1, h = kg & 1;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int at = entry_slot(h, (4 * q + j) & 31);
         const unsigned sel = (j & 1) ? 0x07060302u : 0x05040100u;  // the entry's 16 bits of two rows
 #pragma unroll
         for (int p = 0; p < T::PARTS; ++p)
-          write8(entries + ((p * STEPS + 2 * b + t) * 64 + at) * 16 + half * 8, __builtin_amdgcn_perm(w[1][j >> 1][p], w[0][j >> 1][p], sel),
+          write8(entries + (at_entries ^ (16 * j)) + p * STEPS * 1024, __builtin_amdgcn_perm(w[1][j >> 1][p], w[0][j >> 1][p], sel),
                  __builtin_amdgcn_perm(w[3][j >> 1][p], w[2][j >> 1][p], sel));
       }
     }
@@ -361,7 +364,7 @@ template <class T, int D, int THREADS, int LA, int LB> struct Stage {
   static constexpr int PER = (2 * Tl::BLOCKS + THREADS - 1) / THREADS;
   static constexpr bool IDLE = 2 * Tl::BLOCKS % THREADS != 0;      // some threads have no block
   Quad v[PER][4];
-  unsigned offset[PER];
+  unsigned offset[PER], at_rows[PER], at_entries[PER];
 
   // of the thread's block u: which tensor (uniform in a wave), and which block of it
   static __device__ __forceinline__ bool second(int u, int tid) {
@@ -380,7 +383,10 @@ template <class T, int D, int THREADS, int LA, int LB> struct Stage {
   __device__ __forceinline__ void prepare(const Vectors<T>& a, const Vectors<T>& b, int tid) {
     if constexpr (THREADS == 64) return;                   // a wave has too many blocks to keep their offsets
 #pragma unroll
-    for (int u = 0; u < PER; ++u) offset[u] = place(second(u, tid) ? b : a, u, tid, 0, ROWS);
+    for (int u = 0; u < PER; ++u) {
+      offset[u] = place(second(u, tid) ? b : a, u, tid, 0, ROWS);
+      at_rows[u] = Tl::rows_at(block(u, tid)), at_entries[u] = Tl::entries_at(block(u, tid));
+    }
   }
 
   // blocks [U0, U1) of the thread
@@ -417,8 +423,10 @@ template <class T, int D, int THREADS, int LA, int LB> struct Stage {
         for (int i = 0; i < 4; ++i)
           if (!k[i]) v[u][i].w = make_uint4(0, 0, 0, 0);
       }
-      if (second(u, tid)) Tl::template write<LB>(to + A, to + A + (LB == BOTH ? Tl::BYTES : 0), kk, v[u]);
-      else Tl::template write<LA>(to, to + (LA == BOTH ? Tl::BYTES : 0), kk, v[u]);
+      unsigned r = THREADS == 64 ? Tl::rows_at(kk) : at_rows[u], e = THREADS == 64 ? Tl::entries_at(kk) : at_entries[u];
+      asm volatile("" : "+v"(r), "+v"(e));                 // four places each, formed here: kept from tile to tile they were registers spilled
+      if (second(u, tid)) Tl::template write<LB>(to + A, to + A + (LB == BOTH ? Tl::BYTES : 0), r, e, v[u]);
+      else Tl::template write<LA>(to, to + (LA == BOTH ? Tl::BYTES : 0), r, e, v[u]);
     }
   }
   // a wave's own way: fetch and write, one tensor after the other, so that half the registers do
