@@ -108,9 +108,11 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
       top = ceilf(fmaxf(T::PARTS == 3 ? half_max(top) : half_max(top) * p.c, m));
       const float ref = (top == ninf() ? 0.f : top) - SHIFT;
       const float fade = exp2_(m - SHIFT - ref);      // a power of two
-      l *= fade;
+      if (__any(fade != 1.f)) {
+        l *= fade;
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) o[i] *= fade;
+        for (int i = 0; i < D / 32; ++i) o[i] *= fade;
+      }
       m = top;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
