@@ -555,13 +555,14 @@ struct Args {
   float* delta;            // [batch, heads, n_q] dout . out; float16: then the same of max |dout|
 };
 
-// Consecutive workgroups go to the eight XCDs in turn: the ones that read the same rows are given numbers of one XCD.
-__device__ __forceinline__ int work_of_block(int workgroups) {
-  const int per = (workgroups + 7) / 8;
+// Consecutive workgroups go to the eight XCDs in turn: the ones that read the same rows are given numbers of one XCD.  Not where signals
+// have lengths of their own: an XCD would have the longest ones alone, so each gets tiles of all.
+__device__ __forceinline__ int work_of_block(const Args& p) {
+  if (p.a.lengths) return (int)blockIdx.x;
+  const int per = (p.workgroups + 7) / 8;
   return (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
 }
-// Signal and head of group i of per heads a signal.  The heads of a signal are neighbours, on one XCD; where signals have lengths of their
-// own, the signals of a head are, so that no XCD has the longest ones alone.
+// Signal and head of group i of `per` heads a signal; of signals with lengths of their own, the heads follow those of the other signals.
 struct Group { int b, head; };
 __device__ __forceinline__ Group group_of(const s2cnn_attention_t& a, int i, int per) { return a.lengths ? Group{i % a.batch, i / a.batch} : Group{i / per, i % per}; }
 // Tiles of one number see as many pairs in every group (near the poles of a grid with a bias over near points: few), and a CU's workgroups

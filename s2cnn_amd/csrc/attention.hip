@@ -15,14 +15,14 @@ namespace {
 constexpr int CUS = 256;
 
 // Columns of one group of heads, groups, and tiles of the long axis.  A workgroup of one wave where one wave holds all columns.
-// The long axis is cut while compute units would have no workgroup, into parts of at least four tiles.
+// The long axis is cut where there are less than six workgroups of one wave, or two of four, for each compute unit, into parts of at
+// least four tiles, or sixteen where every unit has a workgroup without: the parts are written and read again.
 Plan plan(long columns, long groups, long long_tiles, bool few) {
   Plan p;
   p.waves = few && columns <= 32 ? 1 : 4;
   p.tiles = columns < 1 ? 1 : (int)((columns + 32 * p.waves - 1) / (32 * p.waves));
   const long base = p.tiles * groups, want = p.waves == 1 ? 6 * CUS : 2 * CUS;
-  long splits = base > CUS ? 1 : (want + base - 1) / base;
-  if (splits > long_tiles / 4) splits = long_tiles / 4;
+  const long splits = min((want + base - 1) / base, long_tiles / (base > CUS ? 16 : 4));
   p.splits = splits < 1 ? 1 : (int)splits;
   p.workgroups = base * p.splits;
   return p;

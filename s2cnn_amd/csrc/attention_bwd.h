@@ -52,7 +52,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
   unsigned long long* const lds_sums = reinterpret_cast<unsigned long long*>(lds_table + MAX_BUCKETS + 4);
   const s2cnn_attention_t& a = p.a;
 
-  const int work = work_of_block(p.workgroups);
+  const int work = work_of_block(p);
   if (work >= p.workgroups) return;
   const int split = work / p.tiles % p.splits, bh = work / p.tiles / p.splits, tile = tile_of(p, work, bh);
   const Group of = group_of(a, bh, a.heads);
@@ -252,7 +252,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
   float* const lds_table = lds_rows + 3 * RING * ROWS + 2 * 32 * W * BUCKET_LD;
   const s2cnn_attention_t& a = p.a;
 
-  const int work = work_of_block(p.workgroups);
+  const int work = work_of_block(p);
   if (work >= p.workgroups) return;
   const int split = work / p.tiles % p.splits, bh = work / p.tiles / p.splits, tile = tile_of(p, work, bh);
   const Group of = group_of(a, bh, a.kv_heads);

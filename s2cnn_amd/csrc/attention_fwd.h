@@ -18,7 +18,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
   float* const lds_table = lds_kb + RING * ROWS;
   const s2cnn_attention_t& a = p.a;
 
-  const int work = work_of_block(p.workgroups);
+  const int work = work_of_block(p);
   if (work >= p.workgroups) return;
   const int split = work / p.tiles % p.splits, bh = work / p.tiles / p.splits, tile = tile_of(p, work, bh);
   const Group of = group_of(a, bh, a.kv_heads);
@@ -219,6 +219,39 @@ template <class T, int D> __global__ __launch_bounds__(256) void join_kernel(Arg
   if (lane == 0 && a.stats) reinterpret_cast<float2*>(a.stats)[row] = any ? make_float2(m - SHIFT, inv) : make_float2(pinf(), 0.f);
 }
 
+// The same for few parts, where what is read is many queries: D / 4 lanes a query, four entries a lane.
+constexpr int FEW_PARTS = 8;
+template <class T, int D> __global__ __launch_bounds__(256) void join_few_kernel(Args p) {
+  const s2cnn_attention_t& a = p.a;
+  constexpr int LANES = D / 4;
+  constexpr float SHIFT = T::HALF ? 10.f : 0.f;
+  const long rows = (long)a.batch * a.heads * a.n_q, row = ((long)blockIdx.x * 256 + threadIdx.x) / LANES;
+  const int q = threadIdx.x % LANES;
+  if (row >= rows) return;
+  const float* const part = p.partial;
+  const float2* const ml = reinterpret_cast<const float2*>(part + p.splits * rows * D);
+  float m = ninf();
+  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, ml[s * rows + row].x);
+  const float ref = m == ninf() ? 0.f : m;
+  float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < p.splits; ++s) {
+    const float2 x = ml[s * rows + row];
+    const float w = exp2_(x.x - ref);
+    float y[4];
+    read16(part + (s * rows + row) * D + 4 * q, y);
+    l = fmaf(x.y, w, l);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = fmaf(y[e], w, o[e]);
+  }
+  const bool any = l != 0.f;
+  const float inv = any ? 1.f / l : 0.f;
+  const int query = (int)(row % a.n_q), head = (int)(row / a.n_q % a.heads), b = (int)(row / a.n_q / a.heads);
+  typedef typename T::type E;
+  store_quad<T>(static_cast<E*>(a.out) + b * a.out_stride[0] + head * a.out_stride[1] + query * a.out_stride[2], q, a.d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+  if (T::PARTS == 1 && a.out_f32) store_quad<F32>(a.out_f32 + row * a.d, q, a.d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+  if (q == 0 && a.stats) reinterpret_cast<float2*>(a.stats)[row] = any ? make_float2(m - SHIFT, inv) : make_float2(pinf(), 0.f);
+}
+
 template <class T, int D> void forward_d(const Args& p, const Plans& plans, hipStream_t stream) {
   const s2cnn_attention_t& a = p.a;
   const Plan& f = plans.fwd;
@@ -228,8 +261,9 @@ template <class T, int D> void forward_d(const Args& p, const Plans& plans, hipS
     if (f.waves == 1) launch(forward_kernel<T, D, 1>, p, 1, lds, stream);
   }
   if (f.waves != 1) launch(forward_kernel<T, D, 4>, p, 4, lds, stream);
-  if (f.splits > 1)
-    hipLaunchKernelGGL((join_kernel<T, D>), dim3((unsigned)((long)a.batch * a.heads * a.n_q)), dim3(256), 0, stream, p);
+  const long rows = (long)a.batch * a.heads * a.n_q;
+  if (f.splits > FEW_PARTS) hipLaunchKernelGGL((join_kernel<T, D>), dim3((unsigned)rows), dim3(256), 0, stream, p);
+  else if (f.splits > 1) hipLaunchKernelGGL((join_few_kernel<T, D>), dim3((unsigned)((rows * (D / 4) + 255) / 256)), dim3(256), 0, stream, p);
 }
 template <class T> void forward(const Args& p, const Plans& plans, hipStream_t stream) {
   if (plans.D == 32) forward_d<T, 32>(p, plans, stream);
