@@ -38,12 +38,12 @@ template <class T> __device__ __forceinline__ ScoreScale score_scale(int n_k, fl
 // workgroup, and a unit is 2^-49 of the bound, 2^-28 of a typical ds in a row of 10^6 keys.
 // 64 copies, one per lane and shared by waves, keep lanes from the same address.
 struct TableSums {
-  static constexpr int COPIES = 64;
+  static constexpr int COPIES = 32;
   static constexpr double MAGIC = 6755399441055744.0;        // 1.5 * 2^52: adding it rounds to an integer, which its low bits hold
   static __host__ __device__ int words(int n_buckets) { return (n_buckets + 1) * COPIES; }       // one more for excluded pairs
 };
 
-template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || T::PARTS * D > 192 ? 1 : 2) void grad_q_kernel(Args p) {
+template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || T::PARTS * D > 192 ? 1 : D == 32 ? 3 : 2) void grad_q_kernel(Args p) {
   typedef Tile<T, D> Tl;
   constexpr int BUFS = buffers<T, D, W>(3), BUF = 3 * Tl::BYTES;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -74,7 +74,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
   const Vectors<T> v{static_cast<const E*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[1], a.v_stride[2], a.n_k, a.d};
   const float* const key_bias = a.key_bias ? a.key_bias + b * a.key_bias_stride : nullptr;
   const signed char* const buckets = a.buckets ? a.buckets + b * a.bucket_stride[0] + query * a.bucket_stride[1] : nullptr;
-  unsigned long long* const sums = lds_sums + lane;
+  unsigned long long* const sums = lds_sums + lane % TableSums::COPIES;
   const bool table_grad = a.gtable != nullptr;
   const float dead = ninf() * p.inv_c;
 
@@ -184,6 +184,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
       start_scores<T>(s, kb, half, buckets != nullptr, now, lds_table, a.n_buckets, p.inv_c);
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) mma<T>(Tl::by_rows(lds_k, i, lane), qf[i], s);
+
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) {
         if constexpr (T::PARTS == 3) mma_small<T>(Tl::by_rows(lds_v, i, lane), gf[i], dp);
@@ -210,6 +211,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
           }
         }
       }
+
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const TwoParts<T> f = cut_rows_in_two<T>(s, t);
@@ -224,7 +226,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
     float* const part = p.gtable_partial + (((long)b * a.heads + head) * p.splits * p.tiles + split * p.tiles + tile) * a.n_buckets;
     for (int n = tid; n < a.n_buckets; n += 64 * W) {
       unsigned long long t = 0;
-      for (int i = 0; i < TableSums::COPIES; ++i) t += lds_sums[n * TableSums::COPIES + ((i + n) & 63)];   // lanes start at banks of their own
+      for (int i = 0; i < TableSums::COPIES; ++i) t += lds_sums[n * TableSums::COPIES + ((i + n) % TableSums::COPIES)];   // lanes start at banks of their own
       part[n] = (float)((double)(long long)t / unit);
     }
   }
@@ -241,9 +243,9 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
 // ---- dk, dv ---------------------------------------------------------------------------------------------------------
 // Columns: keys of one key head.  Rows: the queries of its heads, tile by tile, head by head.
 constexpr int BUCKET_LD = 9;
-template <class T, int D, int W> constexpr int kv_buffers() { return buffers<T, D, W>(4); }
+template <class T, int D, int W> constexpr int kv_buffers() { return T::PARTS * D == 96 ? 1 : buffers<T, D, W>(4); }
 
-template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || D > 64 ? 1 : 2) void grad_kv_kernel(Args p) {
+template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || D > 64 ? 1 : D == 32 ? 3 : 2) void grad_kv_kernel(Args p) {
   typedef Tile<T, D> Tl;
   constexpr int BUFS = kv_buffers<T, D, W>(), BUF = 4 * Tl::BYTES;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
