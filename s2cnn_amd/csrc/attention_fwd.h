@@ -159,10 +159,11 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
   if (half == 0 && a.stats) reinterpret_cast<float2*>(a.stats)[row] = any ? make_float2(m - SHIFT, inv) : make_float2(pinf(), 0.f);
 }
 
-// A workgroup joins the parts of one query, a quarter of them per wave: lane s of a wave has the maximum and the sum of its part s (of 64
+// A workgroup joins the parts of one query, shared out to sixteen waves: lane s of a wave has the maximum and the sum of its part s (of 64
 // at a time), and so its weight, 2^(its maximum - the maximum of all).
-template <class T, int D> __global__ __launch_bounds__(256) void join_kernel(Args p) {
-  __shared__ float lds_o[4][D], lds_l[4];
+constexpr int JOIN_WAVES = 16;
+template <class T, int D> __global__ __launch_bounds__(64 * JOIN_WAVES) void join_kernel(Args p) {
+  __shared__ float lds_o[JOIN_WAVES][D], lds_l[JOIN_WAVES];
   const s2cnn_attention_t& a = p.a;
   const long rows = (long)a.batch * a.heads * a.n_q, row = blockIdx.x;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -175,7 +176,7 @@ template <class T, int D> __global__ __launch_bounds__(256) void join_kernel(Arg
 #pragma unroll
   for (int i = 32; i; i >>= 1) m = fmaxf(m, __shfl_xor(m, i));
   const float ref = m == ninf() ? 0.f : m;
-  const int per_wave = (p.splits + 3) / 4, first = wave * per_wave, last = min(p.splits, first + per_wave);
+  const int per_wave = (p.splits + JOIN_WAVES - 1) / JOIN_WAVES, first = wave * per_wave, last = min(p.splits, first + per_wave);
   float l = 0.f, o[PER] = {};
   for (int s0 = first; s0 < last; s0 += 64) {
     float w = 0.f;
@@ -201,7 +202,9 @@ template <class T, int D> __global__ __launch_bounds__(256) void join_kernel(Arg
   if (lane == 0) lds_l[wave] = l;
   __syncthreads();
   if (wave) return;
-  l = (lds_l[0] + lds_l[1]) + (lds_l[2] + lds_l[3]);
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < JOIN_WAVES; ++w) l += lds_l[w];
   const bool any = l != 0.f;
   const float inv = any ? 1.f / l : 0.f;
   const int query = (int)(row % a.n_q), head = (int)(row / a.n_q % a.heads), b = (int)(row / a.n_q / a.heads);
@@ -212,7 +215,10 @@ template <class T, int D> __global__ __launch_bounds__(256) void join_kernel(Arg
     const int e = lane + 64 * i;
     if (e >= a.d) continue;
     const int slot = slot_of(e, a.d);
-    const float x = ((lds_o[0][slot] + lds_o[1][slot]) + (lds_o[2][slot] + lds_o[3][slot])) * inv;
+    float x = 0.f;
+#pragma unroll
+    for (int w = 0; w < JOIN_WAVES; ++w) x += lds_o[w][slot];
+    x *= inv;
     static_cast<E*>(a.out)[at + e] = (E)x;
     if (T::PARTS == 1 && a.out_f32) a.out_f32[row * a.d + e] = x;
   }
@@ -262,7 +268,7 @@ template <class T, int D> void forward_d(const Args& p, const Plans& plans, hipS
   }
   if (f.waves != 1) launch(forward_kernel<T, D, 4>, p, 4, lds, stream);
   const long rows = (long)a.batch * a.heads * a.n_q;
-  if (f.splits > FEW_PARTS) hipLaunchKernelGGL((join_kernel<T, D>), dim3((unsigned)rows), dim3(256), 0, stream, p);
+  if (f.splits > FEW_PARTS) hipLaunchKernelGGL((join_kernel<T, D>), dim3((unsigned)rows), dim3(64 * JOIN_WAVES), 0, stream, p);
   else if (f.splits > 1) hipLaunchKernelGGL((join_few_kernel<T, D>), dim3((unsigned)((rows * (D / 4) + 255) / 256)), dim3(256), 0, stream, p);
 }
 template <class T> void forward(const Args& p, const Plans& plans, hipStream_t stream) {
