@@ -116,8 +116,8 @@ def attention(q, k, v, table=None, buckets=None, key_bias=None, lengths=None, sc
     :param scale: 1 / sqrt(d) if None
     :return out: [batch, heads, n_q, d]; zero for a query all of whose keys are excluded (its gradients are zero too)
 
-    Sums, the softmax and its gradient are float32; float32 operands are multiplied to the accuracy of float32, the others'
-    probabilities are rounded to the type of v.  The backward pass recomputes the probabilities.  Results do not depend on the order of execution.
+    Sums, the softmax and its gradient are float32; float32 operands are multiplied to the accuracy of float32, and of the other types
+    only the results are rounded.  The backward pass recomputes the probabilities.  Results do not depend on the order of execution.
     """
     assert q.dim() == 4 and k.dim() == 4 and v.dim() == 4
     assert k.shape == v.shape

@@ -93,15 +93,6 @@ template <class T> __device__ __forceinline__ float add_pair(unsigned w, float s
   if constexpr (T::HALF) return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, w), __builtin_bit_cast(v2h, 0x3c003c00u), sum, false);
   else return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, w), __builtin_bit_cast(v2bf, 0x3f803f80u), sum, false);
 }
-// two values as the matrix cores will see them
-template <class T> __device__ __forceinline__ void round_pair(float& x, float& y) {
-  if constexpr (T::PARTS == 1) {
-    unsigned w[1];
-    cut<T>(x, y, w);
-    const v2f r = uncut<T>(w[0]);
-    x = r[0], y = r[1];
-  }
-}
 template <class T> __device__ __forceinline__ Frag<T> cut8(const float* x) {
   unsigned w[4][T::PARTS];
 #pragma unroll
@@ -119,9 +110,11 @@ template <class T> __device__ __forceinline__ Frag<T> cut_rows(const v16f& s, in
   return cut8<T>(x);
 }
 
-// The 16-bit types' gradients of scores, and the probabilities of the backward pass, go into their products as two parts: rounded to one
-// they would add a second error as large as that of the probabilities' own rounding (gradients 1.65 times as far off as
-// with exact products, 1.35 times with two parts), and the matrix cores have the time.
+// The 16-bit types' probabilities and their gradients go into their products as two parts, 16 bits in bfloat16 and 22 in float16.  Rounded to
+// one they are off by as much as the result's own rounding: out and its gradients were 1.35 times as far from exact ones as rounded exact
+// ones are, the table's gradient up to 1.5 times; with two parts the ratio is 1.00.  The price is a half more matrix instructions in the
+// forward pass (73 -> 82 us at 16 signals, 8 heads, 1024 points of 64 entries); the backward pass, which had to round its
+// probabilities as the forward pass did, gains as much.
 template <class T> struct TwoParts {
   static constexpr int N = T::PARTS == 1 ? 2 : 1;
   Frag<T> part[N];
@@ -460,10 +453,9 @@ template <class T, int D, int THREADS, int LA, int LB> struct Stage {
 
 // ---- scores -----------------------------------------------------------------------------------------------------------
 // Scores are kept in base 2: x = log2(e) (scale q.k + table + key bias), the factor in the scale, the table and the key biases.
-// The reference that a query's probabilities are taken to, 2^(x - reference), is an integer, its largest score rounded up: a
-// probability rounded to 16 bits is then the same whatever the reference was when it was formed, up to the power of two, and
-// the sums, the output and the backward pass all use the same, rounded ones.  They are so the exact softmax of weights that
-// are off by a rounding each, rows of its gradient sum to zero as they should, and a factor between references is exact.
+// The reference that a query's probabilities are taken to, 2^(x - reference), is an integer, its largest score rounded up: a change of
+// it is an exact factor, and a query seldom has one after its first tiles, so that the output is multiplied only in those.  The
+// sum of a query is that of the parts that enter its product, so that a query with one key has its value exactly.
 //
 // The product starts from the biases instead of zero: x = c (q.k + bias / c), c = log2(e) |scale|; float32 takes c into the columns as
 // they are loaded, and needs no factor; the other types take the sign.  Biases are held within +-3e38, so that one of the type's lowest value
@@ -551,7 +543,7 @@ struct Args {
   int tiles;               // workgroups along the columns
   int workgroups;
   float* partial;          // results of the parts
-  float* gtable_partial;   // of every workgroup
+  double* gtable_partial;  // of every workgroup
   float* delta;            // [batch, heads, n_q] dout . out; float16: then the same of max |dout|
 };
 

@@ -70,7 +70,7 @@ Backward backward_layout(const s2cnn_attention_t& a, const Plans& p) {
   Backward w;
   w.delta = 0;
   w.table = up(queries * (a.dtype == S2CNN_F16 ? 2 : 1) * sizeof(float));
-  w.q = w.table + up((size_t)p.grad_q.workgroups * a.n_buckets * sizeof(float));
+  w.q = w.table + up((size_t)p.grad_q.workgroups * a.n_buckets * sizeof(double));
   w.kv = w.q + (p.grad_q.splits > 1 ? up((size_t)p.grad_q.splits * queries * p.D * sizeof(float)) : 0);
   w.bytes = w.kv + (p.grad_kv.splits > 1 ? up((size_t)p.grad_kv.splits * 2 * keys * p.D * sizeof(float)) : 0);
   return w;
@@ -137,7 +137,7 @@ extern "C" int s2cnn_attention_bwd(const s2cnn_attention_t* a, void* workspace, 
   char* const at = static_cast<char*>(workspace);
   Args p = args_of(*a, plans);
   p.delta = reinterpret_cast<float*>(at + w.delta);
-  p.gtable_partial = reinterpret_cast<float*>(at + w.table);
+  p.gtable_partial = reinterpret_cast<double*>(at + w.table);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   float* const q = reinterpret_cast<float*>(at + w.q);
   float* const kv = reinterpret_cast<float*>(at + w.kv);

@@ -2,7 +2,7 @@
 //   p = 2^(x - m) / l,  ds = p (dp - delta),  dp = dout v^T,  delta = dout . out (per query),
 //   dq = scale ds k,  dk = scale ds^T q,  dv = p^T dout,  dtable[head, n] = sum of ds over the pairs of bucket n.
 // Where one key holds most of a query's softmax, dp - delta is a small difference: for the 16-bit types delta is formed from
-// the output before its rounding (out_f32), and the probabilities are the rounded ones that made it.
+// the output before its rounding (out_f32).
 // Two kernels, each with its results in registers to the end and no atomics between workgroups, so that results do not depend
 // on the order of execution: one keeps queries and runs over keys (dq, dtable, and delta for the other), one keeps keys and
 // runs over the queries of all heads that share them (dk, dv).  The price is that both form x and dp: seven products instead
@@ -36,7 +36,8 @@ template <class T> __device__ __forceinline__ ScoreScale score_scale(int n_k, fl
 // in units of a power of two that the workgroup knows beforehand.  |ds| <= 2 max(sum_d |dout_d|) max |v|, both maxima over what the
 // workgroup sees, and a query's |ds| add up to no more than that: 2^50 units for twice the bound leaves room for the queries of a
 // workgroup, and a unit is 2^-49 of the bound, 2^-28 of a typical ds in a row of 10^6 keys.
-// 64 copies, one per lane and shared by waves, keep lanes from the same address.
+// 32 copies, one per lane of a half and shared by waves, keep lanes from the same address.  Sums of a workgroup are added in 64 bits to the
+// end: entries of the table's gradient are small differences of large sums.
 struct TableSums {
   static constexpr int COPIES = 32;
   static constexpr double MAGIC = 6755399441055744.0;        // 1.5 * 2^52: adding it rounds to an integer, which its low bits hold
@@ -199,7 +200,6 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
         float pr[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) pr[i] = exp2_(T::PARTS == 3 ? s[r + i] - m : fmaf(s[r + i], p.c, -m));
-        round_pair<T>(pr[0], pr[1]);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           s[r + i] = pr[i] * fmaf(dp[r + i], rl, -delta_rl);
@@ -223,11 +223,11 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
 
   if (table_grad) {
     __syncthreads();
-    float* const part = p.gtable_partial + (((long)b * a.heads + head) * p.splits * p.tiles + split * p.tiles + tile) * a.n_buckets;
+    double* const part = p.gtable_partial + (((long)b * a.heads + head) * p.splits * p.tiles + split * p.tiles + tile) * a.n_buckets;
     for (int n = tid; n < a.n_buckets; n += 64 * W) {
       unsigned long long t = 0;
       for (int i = 0; i < TableSums::COPIES; ++i) t += lds_sums[n * TableSums::COPIES + ((i + n) % TableSums::COPIES)];   // lanes start at banks of their own
-      part[n] = (float)((double)(long long)t / unit);
+      part[n] = (double)(long long)t / unit;
     }
   }
   if (!ok) return;
@@ -439,7 +439,6 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
             const int j = 4 * g + i + e;
             pr[e] = exp2_(T::PARTS == 3 ? s[j] + kb : fmaf(s[j], p.c, kb) + ms[i + e]);
           }
-          round_pair<T>(pr[0], pr[1]);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int j = 4 * g + i + e;
@@ -502,13 +501,13 @@ template <class T, int D> __global__ __launch_bounds__(256) void sum_vectors_ker
   store_quad<T>(static_cast<typename T::type*>(p.to[which]) + i / p.n / p.heads * st[0] + i / p.n % p.heads * st[1] + i % p.n * st[2], q, p.d, t[0], t[1], t[2], t[3]);
 }
 // dtable: one wave per (head, bucket); partials [batch][heads][per][n_buckets]
-template <class T> __global__ __launch_bounds__(64) void sum_table_kernel(const float* part, int batch, int heads, int per, int n_buckets, typename T::type* out) {
+template <class T> __global__ __launch_bounds__(64) void sum_table_kernel(const double* part, int batch, int heads, int per, int n_buckets, typename T::type* out) {
   const int head = blockIdx.x / n_buckets, n = blockIdx.x % n_buckets;
-  float t = 0.f;
+  double t = 0.0;
   for (long k = threadIdx.x; k < (long)batch * per; k += 64) t += part[((k / per * heads + head) * per + k % per) * n_buckets + n];
 #pragma unroll
   for (int s = 32; s; s >>= 1) t += __shfl_xor(t, s);
-  if (threadIdx.x == 0) out[blockIdx.x] = (typename T::type)t;
+  if (threadIdx.x == 0) out[blockIdx.x] = (typename T::type)(float)t;
 }
 
 template <class T, int D> void sum_vectors(const float* part, int splits, int tensors, void* const (&to)[2], const long* s0, const long* s1, int batch, int heads, int n, int d,

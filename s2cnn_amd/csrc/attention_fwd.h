@@ -121,11 +121,14 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
       }
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const Frag<T> pf = cut_rows<T>(s, t);
+        const TwoParts<T> pf = cut_rows_in_two<T>(s, t);
         if constexpr (T::PARTS == 1) {
-          const unsigned w[4] = {pf.part[0].x, pf.part[0].y, pf.part[0].z, pf.part[0].w};
 #pragma unroll
-          for (int j = 0; j < 4; ++j) l = add_pair<T>(w[j], l);
+          for (int i = 0; i < 2; ++i) {
+            const unsigned w[4] = {pf.part[i].part[0].x, pf.part[i].part[0].y, pf.part[i].part[0].z, pf.part[i].part[0].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) l = add_pair<T>(w[j], l);
+          }
         }
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) mma<T>(Tl::by_entries(lds_v, i, t, lane), pf, o[i]);
