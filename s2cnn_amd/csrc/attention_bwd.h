@@ -7,6 +7,11 @@
 // on the order of execution: one keeps queries and runs over keys (dq, dtable, and delta for the other), one keeps keys and
 // runs over the queries of all heads that share them (dk, dv).  The price is that both form x and dp: seven products instead
 // of five; storing ds would cost 2 n_q n_k floats of traffic per head, more time than two products.
+//
+// What bounds them, and what they measured.  float32, 4 signals, 8 heads, 4096 points, D = 64: dq 1.23 ms (168 TFLOP/s of float32 products),
+// dk and dv 1.57 ms (175): matrix instructions take 0.46 of a SIMD's time, vector ones 0.44 and 0.36.  bfloat16, 16 signals, 8 heads on 2,
+// 1024 points, those within a radian: 134 and 150 us, vector instructions 0.40 and 0.35 of the time, matrix ones 0.12 and 0.15, the rest the
+// latency of a tile's steps with two or three waves a SIMD.  float32, 32 signals, 5 heads, 400 points of 20 entries: 69 and 79 us.
 #pragma once
 #include "attention.h"
 
@@ -44,6 +49,8 @@ struct TableSums {
   static __host__ __device__ int words(int n_buckets) { return (n_buckets + 1) * COPIES; }       // one more for excluded pairs
 };
 
+// Workgroups of four waves a CU: three at D = 32 and for the 16-bit types at 64, two for the others up to float32 at 64, all without spills but
+// float32 at 32 (14 registers; 69 us against 90 with two, 32 signals, 5 heads, 400 points: 640 workgroups at once instead of in two rounds).
 template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || T::PARTS * D > 192 ? 1 : D == 32 || T::PARTS * D == 64 ? 3 : 2) void grad_q_kernel(Args p) {
   typedef Tile<T, D> Tl;
   constexpr int BUFS = buffers<T, D, W>(3), BUF = 3 * Tl::BYTES;
@@ -243,6 +250,8 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
 // ---- dk, dv ---------------------------------------------------------------------------------------------------------
 // Columns: keys of one key head.  Rows: the queries of its heads, tile by tile, head by head.
 constexpr int BUCKET_LD = 9;
+// One tile in LDS, not two, for float32 at D = 32: so three workgroups fit a CU (79 us against 92 with two, at the size above), although 24
+// registers are spilled for it.  For the 16-bit types at 64 the third costs 38, and 189 us against 156.
 template <class T, int D, int W> constexpr int kv_buffers() { return T::PARTS * D == 96 ? 1 : buffers<T, D, W>(4); }
 
 template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || D > 64 ? 1 : D == 32 ? 3 : 2) void grad_kv_kernel(Args p) {
@@ -500,7 +509,7 @@ template <class T, int D> __global__ __launch_bounds__(256) void sum_vectors_ker
   const long (&st)[3] = p.stride[which];
   store_quad<T>(static_cast<typename T::type*>(p.to[which]) + i / p.n / p.heads * st[0] + i / p.n % p.heads * st[1] + i % p.n * st[2], q, p.d, t[0], t[1], t[2], t[3]);
 }
-// dtable: one wave per (head, bucket); partials [batch][heads][per][n_buckets]
+// dtable: one wave per (head, bucket), 5 us, a launch and a trip to memory; partials [batch][heads][per][n_buckets]
 template <class T> __global__ __launch_bounds__(64) void sum_table_kernel(const double* part, int batch, int heads, int per, int n_buckets, typename T::type* out) {
   const int head = blockIdx.x / n_buckets, n = blockIdx.x % n_buckets;
   double t = 0.0;

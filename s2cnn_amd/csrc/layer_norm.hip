@@ -2,7 +2,7 @@
 // normalisation; forward and backward.  All are bound by memory: every tensor is read once and written once, in 16 bytes a
 // lane, and what is formed on the way stays in registers.
 //
-// A row belongs to a group of L lanes, each with up to K chunks of 16 bytes of it: L = 8 up to 32 chunks, so that short rows
+// A row belongs to a group of L lanes, each with up to K chunks of 16 bytes of it: L = 8 up to 16 chunks, so that short rows
 // leave few lanes idle and are summed in three lane exchanges, then 16, 32, 64, and a workgroup of 256; rows of more than
 // 1024 chunks are read again per pass.  Mean and variance are formed one after the other from the registers (the variance from the centred
 // values, not as a difference of large sums).
@@ -11,7 +11,13 @@
 //   backward   u = g w, dh = rstd (u - mean(u) - xh mean(u xh)) (+ the gradient of h), dx = dropout(dh); dw = sum g xh, db = sum g
 //
 // The two sums over the rows are kept in registers by the groups, which run over many rows each, joined per workgroup in LDS,
-// and a second kernel adds the workgroups' sums in a fixed order.
+// and a second kernel adds the workgroups' sums in a fixed order.  The backward pass reads h as it was rounded to the tensors' type: the
+// weights' gradient of 16-bit types has that rounding beside its own, for a third less traffic than x and the residual again.
+//
+// Measured, with a copy of 1 GiB at 5.1 TB/s: 65536 rows of 1024 in bfloat16: forward 58 us, 4.6 TB/s, backward 82 us, 4.9 TB/s; the step
+// with a residual and dropout, 16384 rows of 512: 18 us, 3.7 TB/s, and 24 us, 3.5 TB/s (tensors of 17 MB: a third of the time is launch and
+// first loads); 12800 rows of 100 in float32: 5 and 9 us; the sums of the workgroups 3 to 6 us on top.  Dropout of 67 million float32:
+// 88 us, 6.1 TB/s, its accesses not kept in the caches (at 5.1 TB/s as ordinary ones).
 #include "counter_random.h"
 
 namespace s2cnn {
