@@ -2,8 +2,8 @@
 
 Tolerances.  u = 2^-24, 2^-8, 2^-11 is the unit roundoff of float32, bfloat16, float16.  float32: a score of magnitude up to
 about 8 carries some 8 roundings of that size, so a probability is off by at most 64 u, a gradient by twice that: 128 u in the
-2-norm.  The 16-bit types: the result, the probabilities, their gradients and the output in the sum `delta` are rounded once each,
-independent errors of 0.45 u on average: 0.9 u together, and 2 u allowed.  Differences that cancel (a softmax over one key has no gradient)
+2-norm.  The 16-bit types: the result is rounded, an error of 0.45 u on average, and 2 u allowed; what comes before is exact to well
+within that.  Differences that cancel (a softmax over one key has no gradient)
 are float32 sums: 4 * 2^-24 of the sum of magnitudes on top."""
 import math
 
@@ -139,6 +139,37 @@ def test_wide_heads_with_few_columns(hip, d, dtype):
         for kind in (dict(), dict(nb=11, excluded=0.2, key_bias="batch", ragged=True)):
             s, g = _inputs(2, 2, 1, nq, nk, d, dtype, seed=i, **kind)
             _check(s, g, dtype, "%d %d %s" % (nq, nk, kind))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("size", [(300, 1, 1, 20, 1030, 20), (9, 33, 33, 40, 1030, 20), (11, 26, 13, 33, 1090, 100), (1, 290, 145, 30, 1100, 64), (2, 2, 2, 33, 4000, 50)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_long_rows_in_parts(hip, size, dtype):
+    """Sizes whose long rows are cut although every compute unit has a workgroup (parts joined four entries a lane), and into many parts
+    where few have one; lengths of zero and such that leave a part empty, rows without keys in one part or in all."""
+    s, g = _inputs(*size, dtype, nb=5, excluded=0.1, key_bias="all", ragged=size[0] > 1)
+    nk = size[4]
+    s["buckets"][1, : nk // 2] = -1
+    s["buckets"][2, nk // 2:] = -1
+    s["buckets"][3] = -1
+    out, _ = _check(s, g, dtype)
+    assert (out[:, :, 3] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+def test_sixteen_bit_results_are_rounded_once(hip, dtype):
+    """A rounding is off by a uniform part of half a spacing, 2^-8 to 2^-9 of a bfloat16: 0.43 u in the 2-norm.  Everything before it is
+    float32 or two parts (2^-16 of a probability): 0.5 u allowed."""
+    s, g = _inputs(2, 4, 2, 300, 500, 64, dtype, nb=32, excluded=0.1, key_bias="all")
+    for n in ("q", "k", "v"):
+        s[n].requires_grad_()
+    out = s2cnn_amd.attention(**s)
+    grads = torch.autograd.grad(out, [s[n] for n in ("q", "k", "v")], g)
+    want, want_grads, _ = _reference(**s, g=g)
+    for got, exact in ((out, want), *((t, want_grads[n]) for n, t in zip(("q", "k", "v"), grads))):
+        assert (got.detach().cpu().double() - exact).norm() <= TOL[dtype] / 4 * exact.norm()
 
 
 @pytest.mark.gpu
