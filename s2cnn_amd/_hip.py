@@ -229,6 +229,15 @@ def _refuse_device(t):
     _require_current_device(t)
 
 
+def once_differentiable(backward):
+    """torch's decorator of that name, whose cost (4 us a call) is left out where no graph of the gradients is asked for."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
+
+
 def ptr_or_none(t):
     return t.data_ptr() if t is not None else None
 

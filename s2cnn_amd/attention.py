@@ -8,11 +8,11 @@ logarithm of the quadrature weights as `key_bias` the sum over keys is the integ
 """
 import ctypes
 import math
+import struct
 from functools import lru_cache
 
 import numpy as np
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _hip
 
@@ -52,11 +52,13 @@ def _plan(shape_q, shape_k, strides, bucket_stride, key_bias_stride, n_buckets, 
     return (bytes(a), *sizes)
 
 
-def _run(name, plan, device, **pointers):
+_POINTERS = struct.Struct("15P")                         # the struct's first fields, in the order of _run's arguments
+
+
+def _run(name, plan, device, q, k, v, table, buckets, key_bias, lengths, out, stats, out_f32, gout=None, gq=None, gk=None, gv=None, gtable=None):
     a = _hip.Attention.from_buffer_copy(plan[0])
-    for field, tensor in pointers.items():
-        if tensor is not None:
-            setattr(a, field, tensor.data_ptr())
+    _POINTERS.pack_into(a, 0, *[0 if t is None else t.data_ptr() for t in
+                                (q, k, v, table, buckets, key_bias, lengths, out, stats, out_f32, gout, gq, gk, gv, gtable)])
     ws = _hip.workspace(plan[2], device) if plan[2] else None
     _hip.call(name, ctypes.byref(a), _hip.ptr_or_none(ws), plan[2], _hip.stream_ptr())
 
@@ -75,15 +77,14 @@ class _Attention(torch.autograd.Function):
             if needs_grad:
                 stats = q.new_empty(plan[1], dtype=torch.float32)
                 exact = q.new_empty(q.shape, dtype=torch.float32) if dtype else None         # out before its rounding
-            _run("s2cnn_attention_fwd", plan, q.device, q=q, k=k, v=v, table=table, buckets=buckets, key_bias=key_bias, lengths=lengths, out=out,
-                 stats=stats, out_f32=exact)
+            _run("s2cnn_attention_fwd", plan, q.device, q, k, v, table, buckets, key_bias, lengths, out, stats, exact)
         if needs_grad:
             ctx.save_for_backward(q, k, v, table, buckets, key_bias, lengths, out, stats, exact)
             ctx.sizes = sizes
         return out
 
     @staticmethod
-    @once_differentiable
+    @_hip.once_differentiable
     def backward(ctx, g):  # pylint: disable=W
         q, k, v, table, buckets, key_bias, lengths, out, stats, exact = ctx.saved_tensors
         wants_q, wants_k, wants_v, wants_table = ctx.needs_input_grad[:4]
@@ -96,8 +97,7 @@ class _Attention(torch.autograd.Function):
         gtable = torch.empty_like(table) if wants_table else None
         strides = (q.stride(), k.stride(), v.stride(), out.stride(), g.stride(), gq.stride()) + ((gk.stride(), gv.stride()) if gk is not None else ())
         plan = _plan(q.shape, k.shape, strides, *ctx.sizes, 1)
-        _run("s2cnn_attention_bwd", plan, q.device, q=q, k=k, v=v, table=table, buckets=buckets, key_bias=key_bias, lengths=lengths, out=out, stats=stats,
-             out_f32=exact, gout=g, gq=gq, gk=gk, gv=gv, gtable=gtable)
+        _run("s2cnn_attention_bwd", plan, q.device, q, k, v, table, buckets, key_bias, lengths, out, stats, exact, g, gq, gk, gv, gtable)
         return (gq if wants_q else None, gk if wants_k else None, gv if wants_v else None, gtable, None, None, None, None, None, None)
 
 

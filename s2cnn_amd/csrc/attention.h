@@ -544,6 +544,7 @@ struct Args {
   int workgroups;
   float* partial;          // results of the parts
   double* gtable_partial;  // of every workgroup
+  int gtable_parts;        // workgroups of a signal and head
   float* delta;            // [batch, heads, n_q] dout . out; float16: then the same of max |dout|
 };
 
@@ -560,7 +561,7 @@ __device__ __forceinline__ Group group_of(const s2cnn_attention_t& a, int i, int
 // Tiles of one number see as many pairs in every group (near the poles of a grid with a bias over near points: few), and a CU's workgroups
 // are 32 apart: each group's tiles are turned by three eighths.
 __device__ __forceinline__ int tile_of(const Args& p, int work, int group) { return (work + group % 8 * (p.tiles * 3 / 8)) % p.tiles; }
-inline unsigned blocks_for(int workgroups) { return (unsigned)((workgroups + 7) / 8 * 8); }
+__host__ __device__ inline int blocks_for(int workgroups) { return (workgroups + 7) / 8 * 8; }
 
 
 // ---- launches -------------------------------------------------------------------------------------------------------
@@ -572,9 +573,9 @@ template <class T, int D> constexpr bool few_waves = T::PARTS * D <= 256;
 struct Plan { int waves, tiles, splits; long workgroups; };
 struct Plans { int D; Plan fwd, grad_q, grad_kv; };
 
-template <class K> void launch(K kernel, const Args& p, int waves, size_t lds, hipStream_t stream) {
+template <class K> void launch(K kernel, const Args& p, int waves, size_t lds, hipStream_t stream, int beyond = 0) {
   (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-  hipLaunchKernelGGL(kernel, dim3(blocks_for(p.workgroups)), dim3(64 * waves), lds, stream, p);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks_for(p.workgroups) + beyond)), dim3(64 * waves), lds, stream, p);
 }
 
 // one translation unit per type

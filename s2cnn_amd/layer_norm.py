@@ -8,7 +8,6 @@ counter: the mask is a function of the seed and of an element's index, formed ag
 from functools import lru_cache
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _hip
 
@@ -47,7 +46,7 @@ class _Dropout(torch.autograd.Function):
         return _Dropout.run(x, p, seed, dtype)
 
     @staticmethod
-    @once_differentiable
+    @_hip.once_differentiable
     def backward(ctx, g):  # pylint: disable=W
         return _Dropout.run(g, ctx.p, ctx.saved_tensors[0] if ctx.seed is None else ctx.seed, ctx.dtype), None, None, None
 
@@ -101,7 +100,7 @@ class _LayerNorm(torch.autograd.Function):
         return y if h is None else (h, y)
 
     @staticmethod
-    @once_differentiable
+    @_hip.once_differentiable
     def backward(ctx, *grads):  # pylint: disable=W
         h, weight, stats, seed = ctx.saved_tensors
         step = len(grads) == 2
