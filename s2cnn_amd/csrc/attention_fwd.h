@@ -42,7 +42,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
 
   int end = a.n_k;
   if (a.lengths) end = max(0, min(end, a.lengths[b]));
-  const int chunk = ((a.n_k + ROWS - 1) / ROWS + p.splits - 1) / p.splits * ROWS;
+  const int chunk = ((end + ROWS - 1) / ROWS + p.splits - 1) / p.splits * ROWS;      // parts of the keys that the signal has
   const int key0 = split * chunk;
   end = min(end, key0 + chunk);
 
