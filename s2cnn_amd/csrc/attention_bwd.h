@@ -268,7 +268,7 @@ constexpr int BUCKET_LD = 9;
 // registers are spilled for it.  For the 16-bit types at 64 the third costs 38, and 189 us against 156.
 template <class T, int D, int W> constexpr int kv_buffers() { return T::PARTS * D == 96 ? 1 : buffers<T, D, W>(4); }
 
-template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || D > 64 ? 1 : D == 32 ? 3 : 2) void grad_kv_kernel(Args p) {
+template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || T::PARTS * D > 192 ? 1 : D == 32 ? 3 : 2) void grad_kv_kernel(Args p) {
   typedef Tile<T, D> Tl;
   constexpr int BUFS = kv_buffers<T, D, W>(), BUF = 4 * Tl::BYTES;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -447,10 +447,8 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
       }
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) mma<T>(Tl::by_rows(lds_q, i, lane), kf[i], s);
-      if constexpr (T::PARTS * D > 128) __builtin_amdgcn_sched_barrier(0);     // no operand of a later product is read before: registers
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) mma<T>(Tl::by_rows(lds_g, i, lane), vf[i], dp);
-      if constexpr (T::PARTS * D > 128) __builtin_amdgcn_sched_barrier(0);     // no operand of a later product is read before: registers
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         float ls[4], ms[4] = {0.f, 0.f, 0.f, 0.f};
@@ -472,7 +470,6 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
           }
         }
       }
-      if constexpr (T::PARTS * D > 128) __builtin_amdgcn_sched_barrier(0);     // no operand of a later product is read before: registers
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const TwoParts<T> pf = cut_rows_in_two<T>(s, t), df = cut_rows_in_two<T>(dp, t);
