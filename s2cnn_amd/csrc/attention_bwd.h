@@ -265,7 +265,8 @@ template <class T> __global__ __launch_bounds__(256) void sum_table_kernel(Args 
 // Columns: keys of one key head.  Rows: the queries of its heads, tile by tile, head by head.
 constexpr int BUCKET_LD = 9;
 // One tile in LDS, not two, for float32 at D = 32: so three workgroups fit a CU (79 us against 92 with two, at the size above), although 24
-// registers are spilled for it.  For the 16-bit types at 64 the third costs 38, and 189 us against 156.
+// registers are spilled for it.  For the 16-bit types at 64 the third costs 38, and 189 us against 156; at 128 the second costs 29, and is
+// worth it (322 us against 409, 4 signals, 8 heads, 2048 points of 100).
 template <class T, int D, int W> constexpr int kv_buffers() { return T::PARTS * D == 96 ? 1 : buffers<T, D, W>(4); }
 
 template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || T::PARTS * D > 192 ? 1 : D == 32 ? 3 : 2) void grad_kv_kernel(Args p) {
