@@ -17,10 +17,11 @@
 namespace s2cnn {
 namespace attn {
 
-// Workgroups of four waves a CU: four for the 16-bit types up to D = 64 (127 registers, none spilled), two for the others; float32 at D = 32
-// takes 136 and gets three.  Three for the 16-bit types at 128 cost 14 registers, and 135 us against 101 (7 sets of 1009 queries and up to 2501
-// keys, 6 heads of 100); one for float32 at 128 leaves more registers, and takes 537 us against 397 (4 signals, 8 heads, 2048 points of 100).
-template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || T::PARTS * D > 64 ? 2 : 4) void forward_kernel(Args p) {
+// Workgroups of four waves a CU: four for the 16-bit types up to D = 64 (127 registers, none spilled), three for float32 at 64 (4 spilled; 868 us
+// against 906 with two, 4 signals, 8 heads, 4096 points, on one card), two for the others; float32 at 32 takes 136 and gets three.  Three for the
+// 16-bit types at 128 cost 14 registers, and 135 us against 101 (7 sets of 1009 queries and up to 2501 keys, 6 heads of 100); one for
+// float32 at 128 leaves more registers, and takes 537 us against 397 (4 signals, 8 heads, 2048 points of 100).
+template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS * D == 192 && W > 1 ? 3 : W == 1 || T::PARTS * D > 64 ? 2 : 4) void forward_kernel(Args p) {
   typedef Tile<T, D> Tl;
   constexpr int BUFS = buffers<T, D, W>(2), BUF = 2 * Tl::BYTES;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
