@@ -456,13 +456,14 @@ int s2cnn_attention_bwd(const s2cnn_attention_t *a, void *workspace, size_t work
  *           Philox4x32-10 of counter i / 8 and key seed: half i % 2 of word (i % 8) / 2, i the index in the dense tensor.  The gradient is
  *           the same map.  seed_at: device memory that holds the seed instead, or NULL.
  * fwd     : y = (h - mean) rstd weight + bias per row, rstd = 1 / sqrt(variance + eps), variance = mean of (h - mean)^2;
- *           residual NULL: h = x (p = 0, argument h unused); else h = residual + dropout(x) is written too.  stats [rows, 2]: mean, rstd
- *           for bwd, or NULL.
+ *           residual NULL: h = x (p = 0, argument h unused); else h = residual + dropout(x) is written too.  stats [stats_floats; step:
+ *           whether there is a residual]: mean and rstd per row and what bwd needs of h beyond its rounding, or NULL.
  * bwd     : from h (fwd's x or h), g = gradient of y: gx, and where not NULL gweight and gbias.  step != 0: d = that gradient + g_h (gradient
  *           of h, or NULL); gresidual = d, gx = dropout(d), either may be NULL.
  */
 int s2cnn_layer_norm_fwd(const void *x, const void *residual, const void *weight, const void *bias, void *h, void *y, float *stats,
                          long rows, long features, float eps, double p, unsigned long long seed, const long long *seed_at, int dtype, void *stream);
+size_t s2cnn_layer_norm_stats_floats(long rows, long features, int dtype, int step);
 size_t s2cnn_layer_norm_bwd_workspace(long rows, long features, int dtype);
 int s2cnn_layer_norm_bwd(const void *h, const void *g, const void *g_h, const void *weight, const float *stats, void *gx, void *gresidual,
                          void *gweight, void *gbias, void *workspace, size_t workspace_bytes, long rows, long features, double p,

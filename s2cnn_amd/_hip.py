@@ -101,6 +101,7 @@ SIGNATURES = {
     "s2cnn_attention_fwd": (_int, [_ATTENTION_P, _vp, _size_t, _vp]),
     "s2cnn_attention_bwd": (_int, [_ATTENTION_P, _vp, _size_t, _vp]),
     "s2cnn_layer_norm_fwd": (_int, [_vp] * 7 + [_long, _long, _float, ctypes.c_double, ctypes.c_ulonglong, _vp, _int, _vp]),
+    "s2cnn_layer_norm_stats_floats": (_size_t, [_long, _long, _int, _int]),
     "s2cnn_layer_norm_bwd_workspace": (_size_t, [_long, _long, _int]),
     "s2cnn_layer_norm_bwd": (_int, [_vp] * 10 + [_size_t, _long, _long, ctypes.c_double, ctypes.c_ulonglong, _vp, _int, _int, _vp]),
     "s2cnn_dropout": (_int, [_vp, _vp, _long, ctypes.c_double, ctypes.c_ulonglong, _vp, _int, _vp]),

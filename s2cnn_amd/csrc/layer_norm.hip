@@ -11,8 +11,9 @@
 //   backward   u = g w, dh = rstd (u - mean(u) - xh mean(u xh)) (+ the gradient of h), dx = dropout(dh); dw = sum g xh, db = sum g
 //
 // The two sums over the rows are kept in registers by the groups, which run over many rows each, joined per workgroup in LDS,
-// and a second kernel adds the workgroups' sums in a fixed order.  The backward pass reads h as it was rounded to the tensors' type: the
-// weights' gradient of 16-bit types has that rounding beside its own, for a third less traffic than x and the residual again.
+// and a second kernel adds the workgroups' sums in a fixed order.  The backward pass reads h, which is rounded to the tensors' type; in the
+// step with a residual what the rounding left goes along in 8 bits an entry (16-bit types).  Without it the weights' gradient had that rounding
+// beside its own, 1.41 times the error; x and the residual once more instead of h would be twice the traffic.
 //
 // Measured, with a copy of 1 GiB at 5.1 TB/s: 65536 rows of 1024 in bfloat16: forward 58 us, 4.6 TB/s, backward 82 us, 4.9 TB/s; the step
 // with a residual and dropout, 16384 rows of 512: 18 us, 3.7 TB/s, and 24 us, 3.5 TB/s (tensors of 17 MB: a third of the time is launch and
@@ -58,6 +59,38 @@ template <class T, class T2> struct Chunk16 {
 };
 template <> struct Chunk<__bf16> : Chunk16<__bf16, bf2> {};
 template <> struct Chunk<half_t> : Chunk16<half_t, h2> {};
+
+// What the rounding of v to a 16-bit type leaves, in units of 2^-7 of half a spacing (of numbers of that exponent): 8 bits with a sign.
+template <class T> __device__ __forceinline__ float low_unit(float rounded) {      // 2^exponent, times 2^-15 or 2^-18
+  return __uint_as_float(__float_as_uint(rounded) & 0x7f800000u) * (__is_same(T, __bf16) ? 0x1p-15f : 0x1p-18f);
+}
+template <class T> __device__ __forceinline__ uint2 low_parts(const float (&v)[Chunk<T>::N]) {
+  unsigned w[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < Chunk<T>::N; ++i) {
+    const float r = (float)(T)v[i], inverse = __uint_as_float(0x7f000000u - (__float_as_uint(r) & 0x7f800000u)) * (__is_same(T, __bf16) ? 0x1p15f : 0x1p18f);
+    const float q = __builtin_amdgcn_fmed3f(rintf((v[i] - r) * inverse), -127.f, 127.f);
+    w[i / 4] |= ((unsigned)(int)q & 255u) << (8 * (i % 4));
+  }
+  return make_uint2(w[0], w[1]);
+}
+template <class T> __device__ __forceinline__ void add_low(const uint2& low, float (&v)[Chunk<T>::N]) {
+  const unsigned w[2] = {low.x, low.y};
+#pragma unroll
+  for (int i = 0; i < Chunk<T>::N; ++i) v[i] = fmaf((float)((int)(w[i / 4] << (24 - 8 * (i % 4))) >> 24), low_unit<T>(v[i]), v[i]);
+}
+__device__ __forceinline__ uint2 load_low(const signed char* p, int n) {
+  uint2 u = make_uint2(0, 0);
+  if (n >= 8) __builtin_memcpy(&u, p, 8);
+  else
+    for (int i = 0; i < n; ++i) (i < 4 ? u.x : u.y) |= (unsigned)(unsigned char)p[i] << (8 * (i % 4));
+  return u;
+}
+__device__ __forceinline__ void store_low(signed char* p, int n, const uint2& u) {
+  if (n >= 8) __builtin_memcpy(p, &u, 8);
+  else
+    for (int i = 0; i < n; ++i) p[i] = (signed char)((i < 4 ? u.x : u.y) >> (8 * (i % 4)));
+}
 
 typedef unsigned loose4 __attribute__((ext_vector_type(4), aligned(2)));    // 16 bytes at any entry
 // The n first entries of a chunk at p (any alignment of the type's: rows of odd length), the others zero.
@@ -132,7 +165,7 @@ template <int L> __device__ __forceinline__ float sum_group(float v, float* slot
 struct Forward {
   const void *x, *residual, *weight, *bias;
   void *h, *y;
-  float* stats;                  // [rows, 2] mean, rstd; may be NULL
+  float* stats;                  // [rows, 2] mean, rstd, then the low parts of h; may be NULL
   long rows;
   int features;
   float eps;
@@ -224,7 +257,11 @@ template <class T, int L, int K, bool STEP, bool LONG> __global__ __launch_bound
         if (c >= chunks || !ok) continue;
         if (LONG) load_h(r, c, v[k]);
         const long at = r * p.features + (long)c * C::N;
-        if constexpr (STEP) store_chunk<T>(static_cast<T*>(p.h) + at, n, v[k]);
+        if constexpr (STEP) {
+          store_chunk<T>(static_cast<T*>(p.h) + at, n, v[k]);
+          if constexpr (C::N == 8)
+            if (p.stats) store_low(reinterpret_cast<signed char*>(p.stats + 2 * p.rows) + at, n, low_parts<T>(v[k]));
+        }
         float ws[C::N], bs[C::N], y[C::N];
         C::get(wraw[k], ws);
         C::get(braw[k], bs);
@@ -252,6 +289,9 @@ template <class T, int L, int K, bool STEP, bool LONG> __global__ __launch_bound
   const T* const gs = static_cast<const T*>(p.g);
   const float inv_n = 1.f / (float)p.features;
   float gw[K][C::N] = {}, gb[K][C::N] = {};
+  constexpr bool LOW = STEP && C::N == 8;
+  const signed char* const lows = reinterpret_cast<const signed char*>(p.stats + 2 * p.rows);
+  uint2 lnext[K], lraw[K];
   uint4 hnext[K], gnext[K], wraw[K];                                // the group's next row; the weights, whose loads in the loop would wait for it
   float2 stnext = make_float2(0.f, 0.f);
   const auto fetch_weights = [&](int pass) {
@@ -261,20 +301,22 @@ template <class T, int L, int K, bool STEP, bool LONG> __global__ __launch_bound
       wraw[k] = w && c < chunks ? load_chunk<T>(w + c * C::N, p.features - c * C::N) : make_uint4(0, 0, 0, 0);
     }
   };
-  const auto fetch = [&](long row, int pass, uint4 (&h)[K], uint4 (&g)[K]) {
+  const auto fetch = [&](long row, int pass, uint4 (&h)[K], uint4 (&g)[K], uint2 (&low)[K]) {
     const long r = row < p.rows ? row : p.rows - 1;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = (pass * K + k) * L + lane, n = p.features - c * C::N;
       h[k] = g[k] = make_uint4(0, 0, 0, 0);
+      low[k] = make_uint2(0, 0);
       if (c >= chunks) continue;
+      if constexpr (LOW) low[k] = load_low(lows + r * p.features + (long)c * C::N, n);
       h[k] = load_chunk<T>(hs + r * p.features + (long)c * C::N, n);
       g[k] = load_chunk<T>(gs + r * p.features + (long)c * C::N, n);
     }
   };
   if (!LONG) {
     fetch_weights(0);
-    fetch((long)blockIdx.x * (THREADS / L) + threadIdx.x / L, 0, hnext, gnext);
+    fetch((long)blockIdx.x * (THREADS / L) + threadIdx.x / L, 0, hnext, gnext, lnext);
     stnext = reinterpret_cast<const float2*>(p.stats)[min((long)blockIdx.x * (THREADS / L) + threadIdx.x / L, p.rows - 1)];
   }
 
@@ -287,6 +329,7 @@ template <class T, int L, int K, bool STEP, bool LONG> __global__ __launch_bound
     float a = 0.f, c2 = 0.f;
     const auto form = [&](int k, float (&xh)[C::N], float (&g)[C::N], float (&u)[C::N]) {
       C::get(hraw[k], xh);
+      if constexpr (LOW) add_low<T>(lraw[k], xh);
       C::get(graw[k], g);
       float ws[C::N];
       C::get(wraw[k], ws);
@@ -297,12 +340,12 @@ template <class T, int L, int K, bool STEP, bool LONG> __global__ __launch_bound
       }
     };
     for (int pass = 0; pass < passes; ++pass) {
-      if (LONG) fetch(r, pass, hraw, graw);
+      if (LONG) fetch(r, pass, hraw, graw, lraw);
       else {
 #pragma unroll
-        for (int k = 0; k < K; ++k) hraw[k] = hnext[k], graw[k] = gnext[k];
+        for (int k = 0; k < K; ++k) hraw[k] = hnext[k], graw[k] = gnext[k], lraw[k] = lnext[k];
         const long next = row + (long)gridDim.x * (THREADS / L);
-        fetch(next, 0, hnext, gnext);
+        fetch(next, 0, hnext, gnext, lnext);
         stnext = reinterpret_cast<const float2*>(p.stats)[next < p.rows ? next : p.rows - 1];
       }
       if (LONG) fetch_weights(pass);
@@ -329,6 +372,7 @@ template <class T, int L, int K, bool STEP, bool LONG> __global__ __launch_bound
         if (c >= chunks || !ok) continue;
         const long at = r * p.features + (long)c * C::N;
         if (LONG) hraw[k] = load_chunk<T>(hs + at, n), graw[k] = load_chunk<T>(gs + at, n), wraw[k] = w ? load_chunk<T>(w + c * C::N, n) : make_uint4(0, 0, 0, 0);
+        if constexpr (LONG && LOW) lraw[k] = load_low(lows + at, n);
         float xh[C::N], g[C::N], u[C::N];
         form(k, xh, g, u);
 #pragma unroll
@@ -381,14 +425,17 @@ template <class T, int L, int K, bool STEP, bool LONG> __global__ __launch_bound
 }
 
 // dw, db of rows longer than the registers hold: a workgroup takes 64 features and a part of the rows
-template <class T> __global__ __launch_bounds__(THREADS) void long_weights_kernel(Backward p, int parts) {
+template <class T> __global__ __launch_bounds__(THREADS) void long_weights_kernel(Backward p, int parts, bool low) {
   __shared__ float sums[2][4][64];
   const int f = blockIdx.x * 64 + (threadIdx.x & 63), wave = threadIdx.x >> 6;
   float gw = 0.f, gb = 0.f;
   if (f < p.features)
     for (long r = (long)blockIdx.y * 4 + wave; r < p.rows; r += 4L * parts) {
       const float2 st = reinterpret_cast<const float2*>(p.stats)[r];
-      const float g = (float)static_cast<const T*>(p.g)[r * p.features + f], h = (float)static_cast<const T*>(p.h)[r * p.features + f];
+      const float g = (float)static_cast<const T*>(p.g)[r * p.features + f];
+      float h = (float)static_cast<const T*>(p.h)[r * p.features + f];
+      if constexpr (Chunk<T>::N == 8)
+        if (low) h = fmaf((float)reinterpret_cast<const signed char*>(p.stats + 2 * p.rows)[r * p.features + f], low_unit<T>(h), h);
       gw = fmaf(g, (h - st.x) * st.y, gw);
       gb += g;
     }
@@ -512,7 +559,7 @@ template <class T> void backward(const Backward& p, bool step, int dtype, void* 
   else dispatch<T, false>(p, wgs, s);
   if (!p.partial) return;
   if (is_long(dtype, p.features))
-    hipLaunchKernelGGL(long_weights_kernel<T>, dim3((unsigned)((p.features + 63) / 64), (unsigned)parts), dim3(THREADS), 0, s, p, parts);
+    hipLaunchKernelGGL(long_weights_kernel<T>, dim3((unsigned)((p.features + 63) / 64), (unsigned)parts), dim3(THREADS), 0, s, p, parts, step);
   hipLaunchKernelGGL(sum_kernel<T>, dim3((unsigned)((2L * p.features + 31) / 32)), dim3(1024), 0, s, p.partial, parts, p.features, static_cast<T*>(gw),
                      static_cast<T*>(gb));
 }
@@ -548,6 +595,11 @@ extern "C" int s2cnn_layer_norm_fwd(const void* x, const void* residual, const v
   else if (dtype == S2CNN_BF16) norm::forward<__bf16>(f, residual != nullptr, wgs, s);
   else norm::forward<half_t>(f, residual != nullptr, wgs, s);
   return launch_status();
+}
+
+extern "C" size_t s2cnn_layer_norm_stats_floats(long rows, long features, int dtype, int step) {
+  if (!sizes_ok(rows, features, dtype)) return 0;
+  return 2 * (size_t)rows + (step && dtype != S2CNN_F32 ? ((size_t)rows * features + 3) / 4 : 0);
 }
 
 extern "C" size_t s2cnn_layer_norm_bwd_workspace(long rows, long features, int dtype) {

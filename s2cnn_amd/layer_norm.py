@@ -37,6 +37,11 @@ def _workspace_floats(rows, features, dtype):
     return _hip.lib().s2cnn_layer_norm_bwd_workspace(rows, features, dtype) // 4
 
 
+@lru_cache(maxsize=1024)
+def _stats_floats(rows, features, dtype, step):
+    return _hip.lib().s2cnn_layer_norm_stats_floats(rows, features, dtype, step)
+
+
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, p, seed, dtype):  # pylint: disable=W
@@ -89,7 +94,7 @@ class _LayerNorm(torch.autograd.Function):
         residual = residual.contiguous() if residual is not None else None
         y = torch.empty_like(x)
         h = torch.empty_like(x) if residual is not None else None
-        stats = x.new_empty((rows, 2), dtype=torch.float32) if needs_grad else None
+        stats = x.new_empty(_stats_floats(rows, features, dtype, residual is not None), dtype=torch.float32) if needs_grad else None
         number, at = _seed_args(seed)
         if rows:
             _hip.call("s2cnn_layer_norm_fwd", x.data_ptr(), _hip.ptr_or_none(residual), _hip.ptr_or_none(weight), _hip.ptr_or_none(bias),
@@ -160,7 +165,7 @@ def dropout_add_layer_norm(x, residual, p, seed, weight=None, bias=None, eps=1e-
     h = residual + dropout(x, p, seed), y = layer_norm(h, weight, bias, eps) in one pass: what stands between two sublayers.
 
     :param x, residual: [..., features] of one shape and type
-    :return (h, y): contiguous; y is formed from h before h is rounded to the type of x
+    :return (h, y): contiguous; y and the gradients are formed from h before h is rounded to the type of x
     """
     assert residual.shape == x.shape
     _check_affine(x, weight, bias)

@@ -126,6 +126,34 @@ def test_step(hip, shape, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,unit", [(torch.bfloat16, 2.0 ** -8), (torch.float16, 2.0 ** -11)], ids=["bf16", "f16"])
+@pytest.mark.parametrize("shape", [(600, 200), (301, 77), (12, 9001)], ids=lambda s: "%dx%d" % s)
+@pytest.mark.parametrize("size", [2.0 ** -6, 1.0, 2.0 ** 6])
+def test_sixteen_bit_step_is_rounded_once(hip, shape, size, dtype, unit):
+    """A rounding is off by a uniform part of half a spacing: 0.43 u in the 2-norm over many numbers, with a spread of 1 / sqrt(2 n) over n of
+    them, four of which are allowed.  The gradients are those of h before its rounding, of which the backward pass has 7 more bits.
+    Rows of any magnitude, with zeros among them."""
+    (x, w, b, g), r = _make(*shape, dtype, seed=4)
+    res, g_h = (r(*shape).to(dtype).cuda() for _ in range(2))
+    with torch.no_grad():
+        x *= size
+        res *= size
+        x[:, ::3] = 0
+        res[:, ::6] = 0
+        w.fill_(1.0)
+    for t in (x, res, w, b):
+        t.requires_grad_()
+    p, seed = 0.25, 3
+    _, y = s2cnn_amd.dropout_add_layer_norm(x, res, p, seed, w, b, eps=EPS)
+    gx, gr, gw, gb = torch.autograd.grad(y, [x, res, w, b], g)
+    xd, rd, wd, gd = (t.detach().cpu().double() for t in (x, res, w, g))
+    f = _factors(x.numel(), p, seed).view(shape)
+    dh, dw, db, _, _ = _gradients(rd + xd * f, wd, gd)
+    for got, want in ((gr, dh), (gx, dh * f), (gw, dw), (gb, db)):
+        assert (got.detach().cpu().double() - want).norm() <= 0.45 * unit * (1 + 4 / (2 * want.numel()) ** 0.5) * want.norm()
+
+
+@pytest.mark.gpu
 @TYPES
 @pytest.mark.parametrize("n", [1, 7, 8, 9, 1000, 4097, 100003])
 def test_dropout(hip, n, dtype):
