@@ -185,6 +185,14 @@ template <class T> __device__ __forceinline__ Quad load_four_at(const typename T
   }
   return v;
 }
+// likewise a word of any alignment
+__device__ __forceinline__ unsigned load_word_at(const signed char* uniform, unsigned bytes) {
+  typedef unsigned word __attribute__((aligned(1), may_alias));
+  typedef const __attribute__((address_space(1))) char global_bytes;
+  unsigned long long address = reinterpret_cast<unsigned long long>(uniform);
+  asm("" : "+s"(address), "+v"(bytes));
+  return *reinterpret_cast<const __attribute__((address_space(1))) word*>(reinterpret_cast<global_bytes*>(address) + bytes);
+}
 template <class T> __device__ __forceinline__ Quad load_quad(const typename T::type* p, int q, int d) {
   Quad v = load_four<T>(p + quad_at(q, d));
   // So many of its first entries count as zero.  A column's quads each have their own number and four conditions on it, which the
@@ -388,12 +396,13 @@ template <class T, int D, int THREADS, int LA, int LB> struct Stage {
     for (int u = U0; u < U1; ++u) {
       if (idle(u, tid)) break;
       const Vectors<T>& x = second(u, tid) ? b : a;
-      const E* const base = x.base + (long)row0 * x.stride;
+      const unsigned stride = (unsigned)x.stride;          // below 2^25, so that products with it are of 32 bits
+      const E* const base = x.base + (unsigned long long)(unsigned)row0 * stride;
       const int left = x.n - 1 - row0;                     // last row of the tile that exists
       if (left >= ROWS - 1) {
         const unsigned at = THREADS == 64 ? place(x, u, tid, 0, ROWS) : offset[u];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[u][i] = load_four_at<T>(base + i * x.stride, at);
+        for (int i = 0; i < 4; ++i) v[u][i] = load_four_at<T>(base + i * stride, at);
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[u][i] = load_four_at<T>(base, place(x, u, tid, i, left));

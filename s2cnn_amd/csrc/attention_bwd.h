@@ -356,9 +356,15 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || 
   // of four queries per key.
   unsigned bucket_words[4];
   const int block_query = 4 * (tid / (8 * W)), block_key = 4 * (tid % (8 * W));
+  const unsigned bucket_stride = (unsigned)a.bucket_stride[1], bucket_offset = block_query * bucket_stride + block_key;
   const auto fetch_buckets = [&](const Place& place) {
     const int left = a.n_q - 1 - place.query, key0 = tile * 32 * W + block_key;
-    const signed char* const at = buckets + (long)place.query * a.bucket_stride[1] + tile * 32 * W;
+    const signed char* const at = buckets + (unsigned long long)(unsigned)place.query * bucket_stride + tile * 32 * W;
+    if (left >= ROWS - 1 && (tile + 1) * 32 * W <= a.n_k) {                // for all threads alike
+#pragma unroll
+      for (int i = 0; i < 4; ++i) bucket_words[i] = load_word_at(at + i * bucket_stride, bucket_offset);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const signed char* const from = at + (unsigned)(min(block_query + i, left) * (int)a.bucket_stride[1] + block_key);
