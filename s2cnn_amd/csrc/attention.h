@@ -56,6 +56,8 @@ __device__ __forceinline__ void write8(unsigned char* p, unsigned a, unsigned b)
   __builtin_memcpy(__builtin_assume_aligned(p, 8), &v, 8);
 }
 
+__device__ __forceinline__ void write4(unsigned char* p, unsigned a) { __builtin_memcpy(__builtin_assume_aligned(p, 4), &a, 4); }
+
 // ---- operands -------------------------------------------------------------------------------------------------------
 template <class T> struct Frag { uint4 part[T::PARTS]; };
 
@@ -314,24 +316,24 @@ template <class T, int D> struct Tile {
     return f;
   }
 
-  // where block k of the tile (rows 4 (k / (D / 4)), entries 4 (k % (D / 4))) is written: its first row, its first entry.  The others
-  // are as many slots on, exclusive or: they differ in the two lowest bits of the slot alone
-  static __device__ __forceinline__ unsigned rows_at(int k) {
-    const int q = k % (D / 4), kg = k / (D / 4), s = q >> 2, h = (q >> 1) & 1;
-    return (unsigned)((s * 64 + row_slot(s, h, 4 * kg)) * 16 + (q & 1) * 8);
+  // where a block of the tile is written that begins with row `row` (a multiple of two) and entry 4 q: its first row, its first entry.  The
+  // others are as many slots on, exclusive or: they differ in the two lowest bits of the slot alone
+  static __device__ __forceinline__ unsigned rows_at(int row, int q) {
+    const int s = q >> 2, h = (q >> 1) & 1;
+    return (unsigned)((s * 64 + row_slot(s, h, row)) * 16 + (q & 1) * 8);
   }
-  static __device__ __forceinline__ unsigned entries_at(int k) {
-    const int q = k % (D / 4), kg = k / (D / 4), b = q >> 3, t = kg >> 2, half = (kg >> 1) & 1, h = kg & 1;
-    return (unsigned)(((2 * b + t) * 64 + entry_slot(h, (4 * q) & 31)) * 16 + half * 8);
+  static __device__ __forceinline__ unsigned entries_at(int row, int q) {
+    const int b = q >> 3, t = row >> 4, half = (row >> 3) & 1, h = (row >> 2) & 1;
+    return (unsigned)(((2 * b + t) * 64 + entry_slot(h, (4 * q) & 31)) * 16 + half * 8 + (row & 3) * 2);
   }
-  // a block into the layouts, at the places `at_rows` and `at_entries`; LAYOUTS: which of the two
-  template <int LAYOUTS> static __device__ __forceinline__ void write(unsigned char* rows, unsigned char* entries, unsigned at_rows, unsigned at_entries, const Quad (&v)[4]) {
-    unsigned w[4][2][T::PARTS];                                    // [row][pair of entries][part]
+  // a block of N rows (2 or 4) into the layouts, at the places `at_rows` and `at_entries`; LAYOUTS: which of the two
+  template <int LAYOUTS, int N> static __device__ __forceinline__ void write(unsigned char* rows, unsigned char* entries, unsigned at_rows, unsigned at_entries, const Quad (&v)[N]) {
+    unsigned w[N][2][T::PARTS];                                    // [row][pair of entries][part]
 #pragma unroll
-    for (int i = 0; i < 4; ++i) quad_parts<T>(v[i], w[i][0], w[i][1]);
+    for (int i = 0; i < N; ++i) quad_parts<T>(v[i], w[i][0], w[i][1]);
     if constexpr ((LAYOUTS & BY_ROWS) != 0) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < N; ++i)
 #pragma unroll
         for (int p = 0; p < T::PARTS; ++p) write8(rows + (at_rows ^ (16 * i)) + p * STEPS * 1024, w[i][0][p], w[i][1][p]);
     }
@@ -340,9 +342,12 @@ template <class T, int D> struct Tile {
       for (int j = 0; j < 4; ++j) {
         const unsigned sel = (j & 1) ? 0x07060302u : 0x05040100u;  // the entry's 16 bits of two rows
 #pragma unroll
-        for (int p = 0; p < T::PARTS; ++p)
-          write8(entries + (at_entries ^ (16 * j)) + p * STEPS * 1024, __builtin_amdgcn_perm(w[1][j >> 1][p], w[0][j >> 1][p], sel),
-                 __builtin_amdgcn_perm(w[3][j >> 1][p], w[2][j >> 1][p], sel));
+        for (int p = 0; p < T::PARTS; ++p) {
+          unsigned char* const to = entries + (at_entries ^ (16 * j)) + p * STEPS * 1024;
+          const unsigned two = __builtin_amdgcn_perm(w[1][j >> 1][p], w[0][j >> 1][p], sel);
+          if constexpr (N == 4) write8(to, two, __builtin_amdgcn_perm(w[3][j >> 1][p], w[2][j >> 1][p], sel));
+          else write4(to, two);
+        }
       }
     }
   }
@@ -362,31 +367,35 @@ template <class T, int D, int THREADS, int LA, int LB> struct Stage {
   typedef Tile<T, D> Tl;
   typedef typename T::type E;
   static constexpr int A = LA == BOTH ? 2 * Tl::BYTES : Tl::BYTES;      // where the second tensor's layouts begin
-  static constexpr int PER = (2 * Tl::BLOCKS + THREADS - 1) / THREADS;
-  static constexpr bool IDLE = 2 * Tl::BLOCKS % THREADS != 0;      // some threads have no block
-  Quad v[PER][4];
+  static constexpr int N = 2 * Tl::BLOCKS < THREADS ? 2 : 4;           // rows of a block: two where four leave threads without one
+  static constexpr int BLOCKS = Tl::BLOCKS * 4 / N;
+  static constexpr int PER = (2 * BLOCKS + THREADS - 1) / THREADS;
+  static constexpr bool IDLE = 2 * BLOCKS % THREADS != 0;      // some threads have no block
+  Quad v[PER][N];
   unsigned offset[PER], at_rows[PER], at_entries[PER];
 
   // of the thread's block u: which tensor (uniform in a wave), and which block of it
   static __device__ __forceinline__ bool second(int u, int tid) {
-    if constexpr (Tl::BLOCKS % THREADS == 0) return u >= PER / 2;
-    else return __builtin_amdgcn_readfirstlane(u * THREADS + tid) >= Tl::BLOCKS;
+    if constexpr (BLOCKS % THREADS == 0) return u >= PER / 2;
+    else return __builtin_amdgcn_readfirstlane(u * THREADS + tid) >= BLOCKS;
   }
-  static __device__ __forceinline__ bool idle(int u, int tid) { return IDLE && __builtin_amdgcn_readfirstlane(u * THREADS + tid) >= 2 * Tl::BLOCKS; }
-  static __device__ __forceinline__ int block(int u, int tid) { return (u * THREADS + tid) % Tl::BLOCKS; }
+  static __device__ __forceinline__ bool idle(int u, int tid) { return IDLE && __builtin_amdgcn_readfirstlane(u * THREADS + tid) >= 2 * BLOCKS; }
+  static __device__ __forceinline__ int block(int u, int tid) { return (u * THREADS + tid) % BLOCKS; }
 
   // bytes from the tile's first row to row i of block u, or to row `last` if that comes before it
   static __device__ __forceinline__ unsigned place(const Vectors<T>& x, int u, int tid, int i, int last) {
     const int kk = block(u, tid);
-    return (unsigned)sizeof(E) * (unsigned)(min(4 * (kk / (D / 4)) + i, last) * (int)x.stride + quad_at(kk % (D / 4), x.d));
+    return (unsigned)sizeof(E) * (unsigned)(min(N * (kk / (D / 4)) + i, last) * (int)x.stride + quad_at(kk % (D / 4), x.d));
   }
+  static __device__ __forceinline__ unsigned in_rows(int u, int tid) { return Tl::rows_at(N * (block(u, tid) / (D / 4)), block(u, tid) % (D / 4)); }
+  static __device__ __forceinline__ unsigned in_entries(int u, int tid) { return Tl::entries_at(N * (block(u, tid) / (D / 4)), block(u, tid) % (D / 4)); }
   // before the first fetch; the strides and sizes are those of all
   __device__ __forceinline__ void prepare(const Vectors<T>& a, const Vectors<T>& b, int tid) {
     if constexpr (THREADS == 64) return;                   // a wave has too many blocks to keep their offsets
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
       offset[u] = place(second(u, tid) ? b : a, u, tid, 0, ROWS);
-      at_rows[u] = Tl::rows_at(block(u, tid)), at_entries[u] = Tl::entries_at(block(u, tid));
+      at_rows[u] = in_rows(u, tid), at_entries[u] = in_entries(u, tid);
     }
   }
 
@@ -402,10 +411,10 @@ template <class T, int D, int THREADS, int LA, int LB> struct Stage {
       if (left >= ROWS - 1) {
         const unsigned at = THREADS == 64 ? place(x, u, tid, 0, ROWS) : offset[u];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[u][i] = load_four_at<T>(base + i * stride, at);
+        for (int i = 0; i < N; ++i) v[u][i] = load_four_at<T>(base + i * stride, at);
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[u][i] = load_four_at<T>(base, place(x, u, tid, i, left));
+        for (int i = 0; i < N; ++i) v[u][i] = load_four_at<T>(base, place(x, u, tid, i, left));
         asm volatile("");                                  // keeps the last load of both branches from becoming one, of a 64-bit address
       }
     }
@@ -416,19 +425,19 @@ template <class T, int D, int THREADS, int LA, int LB> struct Stage {
 #pragma unroll
     for (int u = U0; u < U1; ++u) {
       if (idle(u, tid)) break;
-      const int kk = block(u, tid), row = 4 * (kk / (D / 4));
-      bool k[4];
+      const int row = N * (block(u, tid) / (D / 4));
+      bool k[N], all = true;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) k[i] = keep(row + i);
-      if (!__all(k[0] && k[1] && k[2] && k[3])) {
+      for (int i = 0; i < N; ++i) k[i] = keep(row + i), all = all && k[i];
+      if (!__all(all)) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < N; ++i)
           if (!k[i]) v[u][i].w = make_uint4(0, 0, 0, 0);
       }
-      unsigned r = THREADS == 64 ? Tl::rows_at(kk) : at_rows[u], e = THREADS == 64 ? Tl::entries_at(kk) : at_entries[u];
+      unsigned r = THREADS == 64 ? in_rows(u, tid) : at_rows[u], e = THREADS == 64 ? in_entries(u, tid) : at_entries[u];
       asm volatile("" : "+v"(r), "+v"(e));                 // four places each, formed here: kept from tile to tile they were registers spilled
-      if (second(u, tid)) Tl::template write<LB>(to + A, to + A + (LB == BOTH ? Tl::BYTES : 0), r, e, v[u]);
-      else Tl::template write<LA>(to, to + (LA == BOTH ? Tl::BYTES : 0), r, e, v[u]);
+      if (second(u, tid)) Tl::template write<LB, N>(to + A, to + A + (LB == BOTH ? Tl::BYTES : 0), r, e, v[u]);
+      else Tl::template write<LA, N>(to, to + (LA == BOTH ? Tl::BYTES : 0), r, e, v[u]);
     }
   }
   // a wave's own way: fetch and write, one tensor after the other, so that half the registers do
@@ -449,7 +458,7 @@ template <class T, int D, int THREADS, int LA, int LB> struct Stage {
       if (idle(u, tid)) break;
       if (!second(u, tid)) continue;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < N; ++i) {
         float x[4];
         quad_values<T>(v[u][i], x);
 #pragma unroll
