@@ -8,10 +8,11 @@
 // runs over the queries of all heads that share them (dk, dv).  The price is that both form x and dp: seven products instead
 // of five; storing ds would cost 2 n_q n_k floats of traffic per head, more time than two products.
 //
-// What bounds them, and what they measured.  float32, 4 signals, 8 heads, 4096 points, D = 64: dq 1.23 ms (168 TFLOP/s of float32 products),
-// dk and dv 1.57 ms (175): matrix instructions take 0.46 of a SIMD's time, vector ones 0.44 and 0.36.  bfloat16, 16 signals, 8 heads on 2,
-// 1024 points, those within a radian: 134 and 150 us, vector instructions 0.40 and 0.35 of the time, matrix ones 0.12 and 0.15, the rest the
-// latency of a tile's steps with two or three waves a SIMD.  float32, 32 signals, 5 heads, 400 points of 20 entries: 69 and 79 us.
+// What bounds them, and what they measured.  float32, 4 signals, 8 heads, 4096 points, D = 64: dq 1.24 ms (166 TFLOP/s of float32 products),
+// dk and dv 1.47 ms (187): matrix and vector instructions together take nine tenths of a SIMD's time, and a third of a tile's step goes into
+// staging its rows.  bfloat16, 16 signals, 8 heads on 2, 1024 points, those within a radian: 134 and 142 us, vector instructions 0.40 and 0.35 of
+// the time, matrix ones 0.12 and 0.15, the rest the latency of a tile's steps with two or three waves a SIMD.  float32, 32 signals, 5 heads,
+// 400 points of 20 entries: 65 and 73 us.
 #pragma once
 #include "attention.h"
 

@@ -16,7 +16,7 @@
 // beside its own, 1.41 times the error; x and the residual once more instead of h would be twice the traffic.
 //
 // Measured, with a copy of 1 GiB at 5.1 TB/s: 65536 rows of 1024 in bfloat16: forward 58 us, 4.6 TB/s, backward 82 us, 4.9 TB/s; the step
-// with a residual and dropout, 16384 rows of 512: 18 us, 3.7 TB/s, and 24 us, 3.5 TB/s (tensors of 17 MB: a third of the time is launch and
+// with a residual and dropout, 16384 rows of 512: 20 us, 3.8 TB/s, and 25 us, 3.7 TB/s (tensors of 17 MB: a third of the time is launch and
 // first loads); 12800 rows of 100 in float32: 5 and 9 us; the sums of the workgroups 3 to 6 us on top.  Dropout of 67 million float32:
 // 88 us, 6.1 TB/s, its accesses past the caches.
 #include "counter_random.h"
