@@ -25,6 +25,11 @@ def _vectors(t):
     return t if (t.stride(-1) == 1 or t.size(-1) == 1) and t.stride(-2) < 1 << 25 else t.contiguous()
 
 
+def _even(t, few):
+    """`t` with the vectors of neighbouring heads one after the other where they are few (see `few` in _Attention): the kernels take them together."""
+    return t if not few or t.size(2) == 1 or t.stride(1) == t.size(2) * t.stride(2) else t.contiguous()
+
+
 def _like(t):
     """Uninitialised, of the shape and order of axes of `t`, vectors contiguous."""
     out = torch.empty_like(t)
@@ -66,7 +71,8 @@ def _run(name, plan, device, q, k, v, table, buckets, key_bias, lengths, out, st
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, buckets, key_bias, lengths, scale, dtype, needs_grad):  # pylint: disable=W
-        q, k, v = _vectors(q), _vectors(k), _vectors(v)
+        few = buckets is None and q.size(2) < 32 and q.size(1) > k.size(1)       # queries of heads that share keys
+        q, k, v = _even(_vectors(q), few), _vectors(k), _vectors(v)
         out = _like(q)
         sizes = ((buckets.stride(0) if buckets.dim() == 3 else 0, buckets.stride(-2)) if buckets is not None else (0, 0),
                  key_bias.stride(0) if key_bias is not None and key_bias.dim() == 2 else 0,
@@ -80,7 +86,7 @@ class _Attention(torch.autograd.Function):
             _run("s2cnn_attention_fwd", plan, q.device, q, k, v, table, buckets, key_bias, lengths, out, stats, exact)
         if needs_grad:
             ctx.save_for_backward(q, k, v, table, buckets, key_bias, lengths, out, stats, exact)
-            ctx.sizes = sizes
+            ctx.sizes, ctx.few = sizes, few
         return out
 
     @staticmethod
@@ -91,7 +97,7 @@ class _Attention(torch.autograd.Function):
         if not out.numel() or not k.size(2):
             return (torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v),
                     torch.zeros_like(table) if table is not None else None) + (None,) * 6
-        g = _vectors(g)
+        g = _even(_vectors(g), ctx.few)
         gq = _like(q)
         gk, gv = (_like(k), _like(v)) if wants_k or wants_v else (None, None)
         gtable = torch.empty_like(table) if wants_table else None
