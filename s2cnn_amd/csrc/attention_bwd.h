@@ -51,8 +51,9 @@ struct TableSums {
 };
 
 // Workgroups of four waves a CU: three at D = 32 and for the 16-bit types at 64, two for the others up to float32 at 64, all without spills but
-// float32 at 32 (14 registers; 69 us against 90 with two, 32 signals, 5 heads, 400 points: 640 workgroups at once instead of in two rounds).
-template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || T::PARTS * D > 192 ? 1 : D == 32 || T::PARTS * D == 64 ? 3 : 2) void grad_q_kernel(Args p) {
+// float32 at 32 (2 registers; 69 us against 90 with two, 32 signals, 5 heads, 400 points: 640 workgroups at once instead of in two rounds).
+// Of one wave: so that two fit a SIMD (135 us against 252 with one, one query a head over 13824 keys of 106, 8 signals, 8 heads, float16).
+template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS * D > 192 ? 1 : W > 1 && (D == 32 || T::PARTS * D == 64) ? 3 : 2) void grad_q_kernel(Args p) {
   typedef Tile<T, D> Tl;
   constexpr int BUFS = buffers<T, D, W>(3), BUF = 3 * Tl::BYTES;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -270,7 +271,7 @@ constexpr int BUCKET_LD = 9;
 // worth it (322 us against 409, 4 signals, 8 heads, 2048 points of 100).
 template <class T, int D, int W> constexpr int kv_buffers() { return T::PARTS * D == 96 ? 1 : buffers<T, D, W>(4); }
 
-template <class T, int D, int W> __global__ __launch_bounds__(64 * W, W == 1 || T::PARTS * D > 192 ? 1 : D == 32 ? 3 : 2) void grad_kv_kernel(Args p) {
+template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS * D > 192 || W == 1 ? 1 : D == 32 ? 3 : 2) void grad_kv_kernel(Args p) {
   typedef Tile<T, D> Tl;
   constexpr int BUFS = kv_buffers<T, D, W>(), BUF = 4 * Tl::BYTES;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];

@@ -158,6 +158,20 @@ def test_long_rows_in_parts(hip, size, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("nq", [1, 5, 40])
+def test_heads_that_share_keys_taken_together(hip, nq, dtype):
+    """No buckets: the queries of a key head's heads as those of one, where they lie one after the other (or are copied so, being few), with key
+    biases, lengths, gradients in another layout than the outputs, and a query expanded over the signals."""
+    s, g = _inputs(3, 6, 2, nq, 200, 20, dtype, key_bias="batch", ragged=True)
+    for layout in (s["q"], s["q"].contiguous()):
+        for gradient in (g, g.transpose(1, 2).contiguous().transpose(1, 2)):
+            _check({**{n: t.detach() for n, t in s.items()}, "q": layout.detach()}, gradient, dtype)
+    one = s["q"][:1].detach().contiguous()
+    _check({**{n: t.detach() for n, t in s.items()}, "q": one.expand(3, -1, -1, -1)}, g, dtype)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
 def test_sixteen_bit_results_are_rounded_once(hip, dtype):
     """A rounding is off by a uniform part of half a spacing, 2^-8 to 2^-9 of a bfloat16: 0.43 u in the 2-norm.  Everything before it is
