@@ -563,7 +563,7 @@ struct Args {
   float* partial;          // results of the parts
   double* gtable_partial;  // of every workgroup
   int gtable_parts;        // workgroups of a signal and head
-  float* delta;            // [batch, heads, n_q] dout . out; float16: then the same of max |dout|
+  float* delta;            // [batch, heads, n_q] dout . out; float16: then the exponents of their ds
 };
 
 // Consecutive workgroups go to the eight XCDs in turn: the ones that read the same rows are given numbers of one XCD.  Not where signals

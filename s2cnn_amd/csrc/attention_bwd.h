@@ -21,19 +21,36 @@ namespace attn {
 
 // float16 has 30 binades: probabilities of a long row and gradients of a scaled loss do not fit it as they are.  Probabilities
 // are held times 2^p, 2^p the power of two at n_k (at most 2^15), gradients of scores times 2^(p / 2) and the power of two that brings
-// the largest |dout| to one.  Both are taken off the results.  All are one for the other types.
+// the largest |dout| to one.  Where values are large that is too much: |ds| = P |dp - delta| is at most a half of M = sum_d |dout_d| max |v|,
+// and the power is lowered to where M stays below 2^16, ds below 2^15 (float16 ends at 65504; its second part then still reaches 2^-39 of
+// that).  Both powers are taken off the results.  All are one for the other types.
 struct ScoreScale {
   float p = 1.f, ds = 1.f;                    // of probabilities; of ds on top of that
 };
-template <class T> __device__ __forceinline__ ScoreScale score_scale(int n_k, float largest) {
+constexpr int ANY_DS = 1000;                  // the exponent of a query without a gradient
+__device__ __forceinline__ int p_exponent(int n_k) { return min(15, 31 - __clz(max(n_k, 1))); }
+// the exponent of a query's ScoreScale::ds; bound: its M.  Of several queries: the least one
+__device__ __forceinline__ int ds_exponent(int n_k, float largest, float bound) {
+  if (!(largest > 0.f)) return ANY_DS;
+  const int e = p_exponent(n_k), ordinary = -max(-40, min(40, ilogbf(largest) + 1)) - (e + 1) / 2;
+  return bound > 0.f && bound < pinf() ? min(ordinary, 15 - e - ilogbf(bound)) : ordinary;
+}
+template <class T> __device__ __forceinline__ ScoreScale score_scale(int n_k, int exponent) {
   ScoreScale s;
   if constexpr (T::HALF) {
-    const int e = min(15, 31 - __clz(max(n_k, 1)));
-    const int g = largest > 0.f ? max(-40, min(40, ilogbf(largest) + 1)) : 0;
-    s.p = ldexpf(1.f, e);
-    s.ds = ldexpf(1.f, -g - (e + 1) / 2);
+    s.p = ldexpf(1.f, p_exponent(n_k));
+    s.ds = ldexpf(1.f, exponent == ANY_DS ? 0 : exponent);
   }
   return s;
+}
+
+// The largest |v| that the forward pass saw of a signal's key head: that of its parts.
+__device__ __forceinline__ float largest_value(const float* of_parts, int parts) {
+  float t = 0.f;
+  for (int i = threadIdx.x & 63; i < parts; i += 64) t = fmaxf(t, of_parts[i]);
+#pragma unroll
+  for (int s = 32; s; s >>= 1) t = fmaxf(t, __shfl_xor(t, s));
+  return t;
 }
 
 // ---- dq, dtable, delta ----------------------------------------------------------------------------------------------
@@ -130,19 +147,19 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
   delta = live ? half_sum(delta) : 0.f;
   total = live ? half_sum(total) : 0.f;
   if constexpr (T::HALF) largest = live ? half_max(largest) : 0.f;
+  const float vmax = T::HALF || table_grad ? largest_value(a.stats + 2 * rows + (b * a.kv_heads + hk) * p.forward_splits, p.forward_splits) : 0.f;
+  const int exponent = T::HALF ? ds_exponent(a.n_k, largest, total * vmax) : 0;
   if (split == 0 && half == 0 && ok) {
     p.delta[row] = delta;
-    if constexpr (T::HALF) p.delta[rows + row] = largest;
+    if constexpr (T::HALF) p.delta[rows + row] = (float)exponent;
   }
-  const ScoreScale sc = score_scale<T>(a.n_k, largest);
+  const ScoreScale sc = score_scale<T>(a.n_k, exponent);
   const float rl = inv_l * sc.p * sc.ds * sign, delta_rl = delta * sign * rl;         // ds = p (dp - delta) / l, as p (dp rl - delta rl)
   const float undo = T::HALF ? 1.f / (sc.p * sc.ds) : 1.f;
 
   // the unit of the table's sums; NaN where the gradient or a value seen by some query is none or infinite: delta is too, then
   double unit = 0.0;
   if (table_grad) {
-    float vmax = 0.f;
-    for (int i = 0; i < p.forward_splits; ++i) vmax = fmaxf(vmax, a.stats[2 * rows + (b * a.kv_heads + hk) * p.forward_splits + i]);
     double bound = fabsf(delta) < pinf() ? (double)total * vmax : (double)pinf();
 #pragma unroll
     for (int i = 32; i; i >>= 1) bound = fmax(bound, __shfl_xor(bound, i));
@@ -314,17 +331,17 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
 
   ScoreScale sc;
   if constexpr (T::HALF) {                                 // one for all heads and queries: they are summed
-    float* const lds_max = lds_rows;
-    const float* const largest = p.delta + (long)a.batch * a.heads * a.n_q + ((long)b * a.heads + hk * group) * a.n_q;
-    float t = 0.f;
-    for (long i = tid; i < (long)group * a.n_q; i += 64 * W) t = fmaxf(t, largest[i]);
+    float* const lds_min = lds_rows;
+    const float* const exponents = p.delta + (long)a.batch * a.heads * a.n_q + ((long)b * a.heads + hk * group) * a.n_q;
+    float t = ANY_DS;
+    for (long i = tid; i < (long)group * a.n_q; i += 64 * W) t = fminf(t, exponents[i]);
 #pragma unroll
-    for (int s = 32; s; s >>= 1) t = fmaxf(t, __shfl_xor(t, s));
-    if (lane == 0) lds_max[wave] = t;
+    for (int s = 32; s; s >>= 1) t = fminf(t, __shfl_xor(t, s));
+    if (lane == 0) lds_min[wave] = t;
     __syncthreads();
-    for (int w = 0; w < W; ++w) t = fmaxf(t, lds_max[w]);
+    for (int w = 0; w < W; ++w) t = fminf(t, lds_min[w]);
     __syncthreads();
-    sc = score_scale<T>(a.n_k, t);
+    sc = score_scale<T>(a.n_k, (int)t);
   }
 
   Stage<T, D, 64 * W, BOTH, BOTH> stage;

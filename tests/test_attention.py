@@ -337,6 +337,32 @@ def test_small_and_large_gradients(hip, dtype, factor):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("nq,nk,length,d,value", [(3, 32768, 2, 128, 16.0), (3, 32768, 2, 128, 500.0), (70, 4096, 2, 64, 64.0), (70, 4096, 4096, 64, 64.0),
+                                                  (40, 1024, 2, 64, 128.0), (3, 64, 64, 64, 500.0), (150, 2, 2, 20, 500.0)])
+def test_float16_gradients_of_large_values(hip, nq, nk, length, d, value):
+    """Two keys that share a row, their values +-`value` in every entry, and a gradient of ones: gradients of scores up to d value / 2, which
+    float16 holds, times the power of two that rows of n_k keys have, which it would not.  And values of that size for all keys.  The
+    output of the two keys is a difference that cancels: sums of magnitudes on top, as for gradients."""
+    s, g = _inputs(1, 2, 1, nq, nk, d, F16, key_bias="all")
+    s["lengths"] = torch.tensor([length], dtype=torch.int32, device="cuda")
+    wide = {**s, "v": (s["v"].float() * (value / 8)).half()}
+    s["k"][:, :, 1] = s["k"][:, :, 0]
+    s["key_bias"][:2] = 10.0
+    s["v"][:, :, 0], s["v"][:, :, 1] = value, -value
+    for what, t, gradient in (("two keys", s, torch.ones_like(g)), ("all keys", wide, g), ("a small gradient", wide, g * 2.0 ** -6)):
+        t = {n: x.detach() for n, x in t.items()}
+        names = ["q", "k", "v"]
+        for n in names:
+            t[n].requires_grad_()
+        out = s2cnn_amd.attention(**t)
+        grads = torch.autograd.grad(out, [t[n] for n in names], gradient)
+        want, want_grads, mags = _reference(**t, g=gradient)
+        _close(out, want, F16, what + " out", _reference(**{**t, "v": t["v"].abs()}))
+        for n, x in zip(names, grads):
+            _close(x, want_grads[n], F16, what + " gradient of " + n, mags[n])
+
+
+@pytest.mark.gpu
 def test_scale_and_large_scores(hip):
     """Scores up to about 90 (a softmax that one key holds): 2^-24 of such a score, some 8 times, is 4e-5 of a probability."""
     s, g = _inputs(1, 2, 2, 40, 200, 32, F32)
