@@ -66,16 +66,17 @@ template <class T> __device__ __forceinline__ v16f mfma(uint4 a, uint4 b, v16f c
   else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
 }
 
-// c += a b, small products first
-template <class T> __device__ __forceinline__ void mma_small(const Frag<T>& a, const Frag<T>& b, v16f& c) {
-  c = mfma<T>(a.part[2], b.part[0], c);
-  c = mfma<T>(a.part[0], b.part[2], c);
+// c += a b, small products first.  TURNED: in the order of the product of b and a, so that the sums are the same
+template <class T, bool TURNED = false> __device__ __forceinline__ void mma_small(const Frag<T>& a, const Frag<T>& b, v16f& c) {
+  constexpr int I = TURNED ? 0 : 2, J = TURNED ? 0 : 1;
+  c = mfma<T>(a.part[I], b.part[2 - I], c);
+  c = mfma<T>(a.part[2 - I], b.part[I], c);
   c = mfma<T>(a.part[1], b.part[1], c);
-  c = mfma<T>(a.part[1], b.part[0], c);
-  c = mfma<T>(a.part[0], b.part[1], c);
+  c = mfma<T>(a.part[J], b.part[1 - J], c);
+  c = mfma<T>(a.part[1 - J], b.part[J], c);
 }
-template <class T> __device__ __forceinline__ void mma(const Frag<T>& a, const Frag<T>& b, v16f& c) {
-  if constexpr (T::PARTS == 3) mma_small<T>(a, b, c);
+template <class T, bool TURNED = false> __device__ __forceinline__ void mma(const Frag<T>& a, const Frag<T>& b, v16f& c) {
+  if constexpr (T::PARTS == 3) mma_small<T, TURNED>(a, b, c);
   c = mfma<T>(a.part[0], b.part[0], c);
 }
 
@@ -84,6 +85,15 @@ template <class T> __device__ __forceinline__ void cut(float x, float y, unsigne
   if constexpr (T::PARTS == 3) split_pair<true>(x, y, w[0], w[1], w[2]);
   else if constexpr (T::HALF) w[0] = __builtin_bit_cast(unsigned, __builtin_convertvector(v2f{x, y}, v2h));
   else w[0] = pack_bf16(x, y);
+}
+// two values times a factor as packed parts, float32; what is left of a first part is that of the product before its rounding.  Written
+// out, so that it is so in every kernel: left to the compiler's contraction, one had other scores than another.
+template <class T> __device__ __forceinline__ void cut_scaled(float x, float y, float factor, unsigned (&w)[3]) {
+  w[0] = pack_bf16(x * factor, y * factor);
+  const v2f h = {__uint_as_float(w[0] << 16), __uint_as_float(w[0] & 0xffff0000u)};
+  const float xr = fmaf(x, factor, -h[0]), yr = fmaf(y, factor, -h[1]);
+  w[1] = pack_bf16(xr, yr);
+  w[2] = pack_bf16(xr - __uint_as_float(w[1] << 16), yr - __uint_as_float(w[1] & 0xffff0000u));
 }
 // what a packed pair of 16-bit values holds
 template <class T> __device__ __forceinline__ v2f uncut(unsigned w) {
@@ -95,10 +105,12 @@ template <class T> __device__ __forceinline__ float add_pair(unsigned w, float s
   if constexpr (T::HALF) return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, w), __builtin_bit_cast(v2h, 0x3c003c00u), sum, false);
   else return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, w), __builtin_bit_cast(v2bf, 0x3f803f80u), sum, false);
 }
-template <class T> __device__ __forceinline__ Frag<T> cut8(const float* x) {
+template <class T, bool SCALE = false> __device__ __forceinline__ Frag<T> cut8(const float* x, float factor = 1.f) {
   unsigned w[4][T::PARTS];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) cut<T>(x[2 * i], x[2 * i + 1], w[i]);
+  for (int i = 0; i < 4; ++i)
+    if constexpr (SCALE) cut_scaled<T>(x[2 * i], x[2 * i + 1], factor, w[i]);
+    else cut<T>(x[2 * i], x[2 * i + 1], w[i]);
   Frag<T> f;
 #pragma unroll
   for (int p = 0; p < T::PARTS; ++p) f.part[p] = make_uint4(w[0][p], w[1][p], w[2][p], w[3][p]);
@@ -213,8 +225,11 @@ template <class T> __device__ __forceinline__ Quad load_quad(const typename T::t
   }
   return v;
 }
-template <class T> __device__ __forceinline__ void quad_parts(const Quad& v, unsigned (&lo)[T::PARTS], unsigned (&hi)[T::PARTS]) {
-  if constexpr (T::PARTS == 3) {
+template <class T, bool SCALE = false> __device__ __forceinline__ void quad_parts(const Quad& v, unsigned (&lo)[T::PARTS], unsigned (&hi)[T::PARTS], float factor = 1.f) {
+  if constexpr (SCALE) {
+    cut_scaled<T>(__uint_as_float(v.w.x), __uint_as_float(v.w.y), factor, lo);
+    cut_scaled<T>(__uint_as_float(v.w.z), __uint_as_float(v.w.w), factor, hi);
+  } else if constexpr (T::PARTS == 3) {
     cut<T>(__uint_as_float(v.w.x), __uint_as_float(v.w.y), lo);
     cut<T>(__uint_as_float(v.w.z), __uint_as_float(v.w.w), hi);
   } else {
@@ -256,9 +271,7 @@ __device__ __forceinline__ void load_column(const typename T::type* p, int d, bo
       float x[8];
       quad_values<T>(a, reinterpret_cast<float (&)[4]>(x[0]));
       quad_values<T>(b, reinterpret_cast<float (&)[4]>(x[4]));
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] *= factor;
-      f[s] = cut8<T>(x);
+      f[s] = cut8<T, true>(x, factor);
     } else {
       f[s].part[0] = make_uint4(a.w.x ^ flip, a.w.y ^ flip, b.w.x ^ flip, b.w.y ^ flip);
     }
@@ -327,10 +340,11 @@ template <class T, int D> struct Tile {
     return (unsigned)(((2 * b + t) * 64 + entry_slot(h, (4 * q) & 31)) * 16 + half * 8 + (row & 3) * 2);
   }
   // a block of N rows (2 or 4) into the layouts, at the places `at_rows` and `at_entries`; LAYOUTS: which of the two
-  template <int LAYOUTS, int N> static __device__ __forceinline__ void write(unsigned char* rows, unsigned char* entries, unsigned at_rows, unsigned at_entries, const Quad (&v)[N]) {
+  template <int LAYOUTS, int N, bool SCALE = false>
+  static __device__ __forceinline__ void write(unsigned char* rows, unsigned char* entries, unsigned at_rows, unsigned at_entries, const Quad (&v)[N], float factor = 1.f) {
     unsigned w[N][2][T::PARTS];                                    // [row][pair of entries][part]
 #pragma unroll
-    for (int i = 0; i < N; ++i) quad_parts<T>(v[i], w[i][0], w[i][1]);
+    for (int i = 0; i < N; ++i) quad_parts<T, SCALE>(v[i], w[i][0], w[i][1], factor);
     if constexpr ((LAYOUTS & BY_ROWS) != 0) {
 #pragma unroll
       for (int i = 0; i < N; ++i)
@@ -363,7 +377,8 @@ template <class T, int D, int W> constexpr int buffers(int layouts) { return W >
 // fetch the blocks of a tile into registers, and write them later.
 // The address of a block's rows is a uniform pointer, moved on by the tile, and an offset of the thread that stays (below
 // 2^32 bytes: the entry checks 32 strides).
-template <class T, int D, int THREADS, int LA, int LB> struct Stage {
+// SCALE: the first tensor is staged times `factor` (float32).
+template <class T, int D, int THREADS, int LA, int LB, bool SCALE = false> struct Stage {
   typedef Tile<T, D> Tl;
   typedef typename T::type E;
   static constexpr int A = LA == BOTH ? 2 * Tl::BYTES : Tl::BYTES;      // where the second tensor's layouts begin
@@ -373,6 +388,7 @@ template <class T, int D, int THREADS, int LA, int LB> struct Stage {
   static constexpr bool IDLE = 2 * BLOCKS % THREADS != 0;      // some threads have no block
   Quad v[PER][N];
   unsigned offset[PER], at_rows[PER], at_entries[PER];
+  float factor = 1.f;
 
   // of the thread's block u: which tensor (uniform in a wave), and which block of it
   static __device__ __forceinline__ bool second(int u, int tid) {
@@ -437,7 +453,7 @@ template <class T, int D, int THREADS, int LA, int LB> struct Stage {
       unsigned r = THREADS == 64 ? in_rows(u, tid) : at_rows[u], e = THREADS == 64 ? in_entries(u, tid) : at_entries[u];
       asm volatile("" : "+v"(r), "+v"(e));                 // four places each, formed here: kept from tile to tile they were registers spilled
       if (second(u, tid)) Tl::template write<LB, N>(to + A, to + A + (LB == BOTH ? Tl::BYTES : 0), r, e, v[u]);
-      else Tl::template write<LA, N>(to, to + (LA == BOTH ? Tl::BYTES : 0), r, e, v[u]);
+      else Tl::template write<LA, N, SCALE>(to, to + (LA == BOTH ? Tl::BYTES : 0), r, e, v[u], factor);
     }
   }
   // a wave's own way: fetch and write, one tensor after the other, so that half the registers do
@@ -475,8 +491,9 @@ template <class T, int D, int THREADS, int LA, int LB> struct Stage {
 // it is an exact factor, and a query seldom has one after its first tiles, so that the output is multiplied only in those.  The
 // sum of a query is that of the parts that enter its product, so that a query with one key has its value exactly.
 //
-// The product starts from the biases instead of zero: x = c (q.k + bias / c), c = log2(e) |scale|; float32 takes c into the columns as
-// they are loaded, and needs no factor; the other types take the sign.  Biases are held within +-3e38, so that one of the type's lowest value
+// The product starts from the biases instead of zero: x = c (q.k + bias / c), c = log2(e) |scale|; float32 takes c into the queries as
+// they are loaded, and needs no factor; the other types take the sign.  All kernels form a score from the same numbers in the same order: the
+// references are of scores as the forward pass had them, and a score of a thousand that is rounded otherwise makes another probability.  Biases are held within +-3e38, so that one of the type's lowest value
 // stays finite: keys that all have it share a row evenly.
 // In two steps, the load and what is made of it: the tiles' loads are under way in between, and a wait for this one, issued before them,
 // is no wait for them.

@@ -292,7 +292,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
   typedef Tile<T, D> Tl;
   constexpr int BUFS = kv_buffers<T, D, W>(), BUF = 4 * Tl::BYTES;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  float* const lds_rows = reinterpret_cast<float*>(smem + BUFS * BUF);        // [RING][3][ROWS]: m, 1 / l, delta; first two negated
+  float* const lds_rows = reinterpret_cast<float*>(smem + BUFS * BUF);        // [RING][3][ROWS]: -m, 1 / l, -delta
   unsigned* const lds_buckets = reinterpret_cast<unsigned*>(lds_rows + 3 * RING * ROWS);      // [2][32 W keys][8 words of four queries, one unused]
   float* const lds_table = lds_rows + 3 * RING * ROWS + 2 * 32 * W * BUCKET_LD;
   const s2cnn_attention_t& a = p.a;
@@ -321,12 +321,12 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
   typedef typename T::type E;
   const float* const key_bias = a.key_bias ? a.key_bias + b * a.key_bias_stride : nullptr;
   const signed char* const buckets = a.buckets ? a.buckets + b * a.bucket_stride[0] : nullptr;
-  const float dead = ninf() * p.inv_c, kb_c = ok ? key_value(load_key_bias(key_bias, key, a.n_k), key, end, p.inv_c) : dead, kb = kb_c * p.c;
+  const float dead = ninf() * p.inv_c, kb_c = ok ? key_value(load_key_bias(key_bias, key, a.n_k), key, end, p.inv_c) : dead;
   const bool live = kb_c != dead, active = __any(live);
 
   Frag<T> kf[D / 16], vf[D / 16];
   load_column<T, D>(static_cast<const E*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[1] + key * a.k_stride[2], a.d, live, half,
-                    a.scale * LOG2E, kf);
+                    T::PARTS == 3 ? 1.f : a.scale, kf);
   load_column<T, D>(static_cast<const E*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[1] + key * a.v_stride[2], a.d, live, half, 1.f, vf);
 
   ScoreScale sc;
@@ -344,7 +344,8 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     sc = score_scale<T>(a.n_k, (int)t);
   }
 
-  Stage<T, D, 64 * W, BOTH, BOTH> stage;
+  Stage<T, D, 64 * W, BOTH, BOTH, T::PARTS == 3> stage;
+  stage.factor = a.scale * LOG2E;
   struct Place {                                           // of a tile: its head of the group, its first query
     int head, query;
     __device__ __forceinline__ Place next(int n_q) const { return query + ROWS < n_q ? Place{head, query + ROWS} : Place{head + 1, 0}; }
@@ -450,14 +451,17 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
       for (int g = 0; g < 4; ++g) words[g] = from[2 * g];
     }
     if (active && (!buckets || !none_takes_part(words))) {
-      // the scores start from the table's entries (float32: less m), dp from -delta
-      v16f s = {}, dp;
+      // the scores start from the biases, dp from -delta
+      v16f s, dp;
       if (buckets) {
         float t[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) t[j] = table[bucket_of(words[j / 4], j % 4, a.n_buckets)];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) s[j] = T::PARTS == 3 ? t[j] : t[j] * p.inv_c;
+        for (int j = 0; j < 16; ++j) s[j] = T::PARTS == 3 ? kb_c + t[j] : fmaf(t[j], p.inv_c, kb_c);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[j] = kb_c;
       }
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
@@ -465,35 +469,27 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
         read16(rows + 2 * ROWS + 8 * g + 4 * half, start);
 #pragma unroll
         for (int i = 0; i < 4; ++i) dp[4 * g + i] = start[i];
-        if constexpr (T::PARTS == 3) {
-          read16(rows + 8 * g + 4 * half, start);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[4 * g + i] += start[i];
-        }
       }
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) mma<T>(Tl::by_rows(lds_q, i, lane), kf[i], s);
+      for (int i = 0; i < D / 16; ++i) mma<T, true>(Tl::by_rows(lds_q, i, lane), kf[i], s);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        float ms[4];
+        read16(rows + 8 * g + 4 * half, ms);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[4 * g + i] = exp2_(T::PARTS == 3 ? s[4 * g + i] + ms[i] : fmaf(s[4 * g + i], p.c, ms[i]));
+      }
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) mma<T>(Tl::by_rows(lds_g, i, lane), vf[i], dp);
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        float ls[4], ms[4] = {0.f, 0.f, 0.f, 0.f};
+        float ls[4];
         read16(rows + ROWS + 8 * g + 4 * half, ls);
-        if constexpr (T::PARTS == 1) read16(rows + 8 * g + 4 * half, ms);
 #pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-          float pr[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int j = 4 * g + i + e;
-            pr[e] = exp2_(T::PARTS == 3 ? s[j] + kb : fmaf(s[j], p.c, kb) + ms[i + e]);
-          }
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int j = 4 * g + i + e;
-            s[j] = pr[e] * ls[i + e];
-            dp[j] = s[j] * (T::HALF ? dp[j] * sc.ds : dp[j]);
-          }
+        for (int i = 0; i < 4; ++i) {
+          const int j = 4 * g + i;
+          s[j] *= ls[i];
+          dp[j] = s[j] * (T::HALF ? dp[j] * sc.ds : dp[j]);
         }
       }
 #pragma unroll
@@ -510,7 +506,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
   }
 
   if (!ok) return;
-  const float fk = T::HALF ? a.scale / (sc.p * sc.ds) : a.scale, fv = T::HALF ? 1.f / sc.p : 1.f;
+  const float fk = T::PARTS == 3 ? 1.f / LOG2E : T::HALF ? a.scale / (sc.p * sc.ds) : a.scale, fv = T::HALF ? 1.f / sc.p : 1.f;
   if (p.splits > 1) {
     const long columns = (long)a.batch * a.kv_heads * a.n_k;
     float* const part = p.partial;

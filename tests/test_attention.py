@@ -373,6 +373,41 @@ def test_scale_and_large_scores(hip):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("nq,nk,d", [(9, 150, 16), (150, 150, 16), (70, 40, 100)])
+@pytest.mark.parametrize("bias", [-1e4, -1e6, 1e6])
+def test_probabilities_of_both_passes_are_the_same(hip, bias, nq, nk, d, dtype):
+    """A large bias on every key, by the keys or by the table, leaves a score few bits, and the two passes have to round it alike: with values of
+    one the outputs are one, and the gradients of the values add up to that of the outputs.  The probabilities of a row add up to one but for
+    some 8 roundings of float32, and what is returned is rounded: TOL of the sum of magnitudes."""
+    for by_table in (False, True):
+        s, g = _inputs(1, 4, 2, nq, nk, d, dtype, nb=3, key_bias="all")
+        if by_table:
+            limit = torch.finfo(dtype).max / 4
+            s["table"] = torch.full_like(s["table"], max(-limit, min(limit, bias)))
+        else:
+            s["key_bias"] = torch.full_like(s["key_bias"], bias)
+        s["v"] = torch.ones_like(s["v"]).requires_grad_()
+        out = s2cnn_amd.attention(**s)
+        gv, = torch.autograd.grad(out, s["v"], g)
+        assert (out.double() - 1).abs().max().item() <= TOL[dtype]
+        sums = g.double().sum(2).view(1, 2, 2, d).sum(2)
+        mags = g.double().abs().sum(2).view(1, 2, 2, d).sum(2)
+        assert ((gv.double().sum(2) - sums).abs() <= TOL[dtype] * mags).all(), ((gv.double().sum(2) - sums).abs() / mags).max().item() / TOL[dtype]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,size", [(F32, 3e4), (F32, 1e3), (BF16, 1e3), (F16, 1e3)], ids=["f32-3e4", "f32-1e3", "bf16", "f16"])
+@pytest.mark.parametrize("nq", [9, 150])
+def test_gradients_of_large_scores(hip, nq, dtype, size):
+    """Queries and keys of a thousand and more: scores of 10^7 to 10^10, which round to hundreds and lie further apart than that: one key has the row."""
+    s, g = _inputs(1, 2, 2, nq, 150, 64, dtype)
+    s["q"] *= size
+    s["k"] *= size
+    _check(s, g, dtype)
+
+
+@pytest.mark.gpu
 def test_same_bits_every_time_and_on_other_streams(hip):
     s, g = _inputs(2, 4, 2, 200, 300, 32, F32, nb=32, excluded=0.1, key_bias="all", ragged=True)
     out, grads = _check(s, g, F32)
