@@ -493,16 +493,38 @@ template <class T, int D, int THREADS, int LA, int LB, bool SCALE = false> struc
 //
 // The product starts from the biases instead of zero: x = c (q.k + bias / c), c = log2(e) |scale|; float32 takes c into the queries as
 // they are loaded, and needs no factor; the other types take the sign.  All kernels form a score from the same numbers in the same order: the
-// references are of scores as the forward pass had them, and a score of a thousand that is rounded otherwise makes another probability.  Biases are held within +-3e38, so that one of the type's lowest value
+// references are of scores as the forward pass had them, and a score of a thousand that is rounded otherwise makes another probability.  Biases are held within +-3e38 of a score, so that one of the type's lowest value
 // stays finite: keys that all have it share a row evenly.
 // In two steps, the load and what is made of it: the tiles' loads are under way in between, and a wait for this one, issued before them,
 // is no wait for them.
 __device__ __forceinline__ float load_key_bias(const float* key_bias, int key, int end) { return key_bias ? key_bias[max(min(key, end - 1), 0)] : 0.f; }
-__device__ __forceinline__ float key_value(float bias, int key, int end, float inv_c) {
+// most: the largest magnitude of a bias, in units of c
+__device__ __forceinline__ float key_value(float bias, int key, int end, float inv_c, float most) {
   const float x = bias * LOG2E * inv_c;
-  const float y = fabsf(bias) < pinf() ? __builtin_amdgcn_fmed3f(x, -3e38f, 3e38f) : x;
-  return key < end ? y : ninf() * inv_c;                   // -inf: takes no part
+  const float y = fabsf(bias) < pinf() ? __builtin_amdgcn_fmed3f(x, -most, most) : x;
+  return key < end ? y : ninf();                           // takes no part
 }
+
+// Scores of the 16-bit types are multiplied by c and taken off their reference in one operation, whose product is not rounded; the reference is
+// a rounded product, off by up to 2^-25 of it.  That is nothing for any score of use, but at 2^27 (float16) a probability of 2^9, at 2^32 none or
+// infinity: rows whose keys all have biases of -10^9, or the type's lowest value.  Where a query's largest score has passed 2^24, its scores and
+// the reference are taken times the power of two that brings it below: a factor of the query in place of c, exact, the same in all kernels, and no
+// operation more.  Such scores keep a resolution of 2^-24 of the largest in place of one unit, which is what their sums are rounded to.
+__device__ __forceinline__ float shrink(float top) {
+  const int e = (int)((__float_as_uint(top) >> 23) & 255u) - 127;
+  return __uint_as_float((unsigned)(127 - max(0, e - 23)) << 23);
+}
+// What a query's probabilities are taken to, from its largest score rounded up, and the factor of its scores.  float16: 2^10 of the probabilities,
+// as its smallest normal number is 2^-14.
+struct Reference { float at, c; };
+template <class T> __device__ __forceinline__ Reference reference(float top, float c) {
+  if constexpr (T::PARTS == 3) return {top, c};
+  const float by = shrink(top);
+  return {fmaf(top, by, T::HALF ? -10.f : 0.f), c * by};
+}
+template <class T> __device__ __forceinline__ float off_reference(float s, const Reference& r) { return T::PARTS == 3 ? s - r.at : fmaf(s, r.c, -r.at); }
+// 2^(a - b) of two largest scores, a <= b, as the probabilities that are taken to them have it
+template <class T> __device__ __forceinline__ float fade_to(float b, float a) { return exp2_(T::PARTS == 3 ? a - b : (a - b) * shrink(b)); }
 
 // A tile's values of its rows (keys' biases; the queries' statistics) in LDS, in a ring: tile t's are read in step t, and in step
 // t - 1, in which its rows are written; they are put there at the start of step t - 2, and loaded in step t - 3: put at that step's end
@@ -573,6 +595,7 @@ template <class T> __device__ __forceinline__ void start_scores(v16f& s, const f
 struct Args {
   s2cnn_attention_t a;
   float c, inv_c;          // log2(e) |scale| and its inverse; 1 for float32
+  float most;              // see key_value
   int forward_splits;
   int splits;              // parts of the long axis (keys; queries in the kernel of dk and dv)
   int tiles;               // workgroups along the columns

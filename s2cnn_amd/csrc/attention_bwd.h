@@ -1,5 +1,5 @@
 // Attention, backward.  The probabilities are recomputed from the scores and the two statistics of each query:
-//   p = 2^(x - m) / l,  ds = p (dp - delta),  dp = dout v^T,  delta = dout . out (per query),
+//   p = 2^(x - m) / l (m, l: largest score, sum),  ds = p (dp - delta),  dp = dout v^T,  delta = dout . out (per query),
 //   dq = scale ds k,  dk = scale ds^T q,  dv = p^T dout,  dtable[head, n] = sum of ds over the pairs of bucket n.
 // Where one key holds most of a query's softmax, dp - delta is a small difference: for the 16-bit types delta is formed from
 // the output before its rounding (out_f32).
@@ -103,7 +103,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
   const signed char* const buckets = a.buckets ? a.buckets + b * a.bucket_stride[0] + query * a.bucket_stride[1] : nullptr;
   unsigned long long* const sums = lds_sums + lane % TableSums::COPIES;
   const bool table_grad = a.gtable != nullptr;
-  const float dead = ninf() * p.inv_c;
+  const float dead = ninf();
 
   Stage<T, D, 64 * W, BOTH, BY_ROWS> stage;
   unsigned words[4] = {0, 0, 0, 0};
@@ -112,7 +112,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     if (W > 1) stage.fetch(k, v, key0, tid);
     if (buckets) load_buckets(buckets, key0, end, half, words);
   }
-  if (tid < 2 * ROWS) lds_kb[tid] = key_value(key0 < end ? load_key_bias(key_bias, key0 + tid, end) : 0.f, key0 + tid, end, p.inv_c);
+  if (tid < 2 * ROWS) lds_kb[tid] = key_value(key0 < end ? load_key_bias(key_bias, key0 + tid, end) : 0.f, key0 + tid, end, p.inv_c, p.most);
   float bias_ahead = tid < ROWS && key0 < end ? load_key_bias(key_bias, key0 + 2 * ROWS + tid, end) : 0.f;
   if (buckets) stage_table<T>(lds_table, a.table, a.n_buckets, head, 1, tid, 64 * W);
   if (table_grad)
@@ -122,7 +122,8 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
   const E* const g_row = static_cast<const E*>(a.gout) + b * a.gout_stride[0] + head * a.gout_stride[1] + query * a.gout_stride[2];
   const float* const o_row = T::PARTS == 3 ? static_cast<const float*>(a.out) + b * a.out_stride[0] + head * a.out_stride[1] + query * a.out_stride[2] : a.out_f32 + row * a.d;
   const float2 stats = reinterpret_cast<const float2*>(a.stats)[row];
-  const float m = ok ? stats.x : pinf(), inv_l = ok ? stats.y : 0.f;
+  const Reference ref = reference<T>(ok ? stats.x : pinf(), p.c);
+  const float inv_l = ok ? stats.y : 0.f;
   const bool live = inv_l != 0.f, active = __any(live);    // a row without keys takes no part, whatever its gradient holds
   load_column<T, D>(static_cast<const E*>(a.q) + b * a.q_stride[0] + head * a.q_stride[1] + query * a.q_stride[2], a.d, live, half,
                     a.scale * LOG2E, qf);
@@ -198,7 +199,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     const unsigned char* const lds_v = lds_k + 2 * Tl::BYTES;
     const float* const kb = lds_kb + step % RING * ROWS;
 
-    if (tid < ROWS) lds_kb[(step + 2) % RING * ROWS + tid] = key_value(bias_ahead, key + 2 * ROWS + tid, end, p.inv_c);
+    if (tid < ROWS) lds_kb[(step + 2) % RING * ROWS + tid] = key_value(bias_ahead, key + 2 * ROWS + tid, end, p.inv_c, p.most);
     if (BUFS == 2 && more) write(step + 1);
     unsigned now[4] = {0, 0, 0, 0};
     if (buckets) place_buckets(words, now);
@@ -225,7 +226,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
       for (int r = 0; r < 16; r += 2) {
         float pr[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) pr[i] = exp2_(T::PARTS == 3 ? s[r + i] - m : fmaf(s[r + i], p.c, -m));
+        for (int i = 0; i < 2; ++i) pr[i] = exp2_(off_reference<T>(s[r + i], ref));
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           s[r + i] = pr[i] * fmaf(dp[r + i], rl, -delta_rl);
@@ -286,15 +287,16 @@ constexpr int BUCKET_LD = 9;
 // One tile in LDS, not two, for float32 at D = 32: so three workgroups fit a CU (79 us against 92 with two, at the size above), although 24
 // registers are spilled for it.  For the 16-bit types at 64 the third costs 38, and 189 us against 156; at 128 the second costs 29, and is
 // worth it (322 us against 409, 4 signals, 8 heads, 2048 points of 100).
+template <class T> constexpr int row_arrays = T::PARTS == 3 ? 3 : 4;      // numbers of a row in LDS
 template <class T, int D, int W> constexpr int kv_buffers() { return T::PARTS * D == 96 ? 1 : buffers<T, D, W>(4); }
 
 template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS * D > 192 || W == 1 ? 1 : D == 32 ? 3 : 2) void grad_kv_kernel(Args p) {
   typedef Tile<T, D> Tl;
-  constexpr int BUFS = kv_buffers<T, D, W>(), BUF = 4 * Tl::BYTES;
+  constexpr int BUFS = kv_buffers<T, D, W>(), BUF = 4 * Tl::BYTES, ARRAYS = row_arrays<T>;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  float* const lds_rows = reinterpret_cast<float*>(smem + BUFS * BUF);        // [RING][3][ROWS]: -m, 1 / l, -delta
-  unsigned* const lds_buckets = reinterpret_cast<unsigned*>(lds_rows + 3 * RING * ROWS);      // [2][32 W keys][8 words of four queries, one unused]
-  float* const lds_table = lds_rows + 3 * RING * ROWS + 2 * 32 * W * BUCKET_LD;
+  float* const lds_rows = reinterpret_cast<float*>(smem + BUFS * BUF);        // [RING][ARRAYS][ROWS]: -reference, 1 / l, -delta, factor (16-bit types)
+  unsigned* const lds_buckets = reinterpret_cast<unsigned*>(lds_rows + ARRAYS * RING * ROWS);      // [2][32 W keys][8 words of four queries, one unused]
+  float* const lds_table = lds_rows + ARRAYS * RING * ROWS + 2 * 32 * W * BUCKET_LD;
   const s2cnn_attention_t& a = p.a;
 
   const int own = blocks_for(p.workgroups);
@@ -321,7 +323,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
   typedef typename T::type E;
   const float* const key_bias = a.key_bias ? a.key_bias + b * a.key_bias_stride : nullptr;
   const signed char* const buckets = a.buckets ? a.buckets + b * a.bucket_stride[0] : nullptr;
-  const float dead = ninf() * p.inv_c, kb_c = ok ? key_value(load_key_bias(key_bias, key, a.n_k), key, end, p.inv_c) : dead;
+  const float dead = ninf(), kb_c = ok ? key_value(load_key_bias(key_bias, key, a.n_k), key, end, p.inv_c, p.most) : dead;
   const bool live = kb_c != dead, active = __any(live);
 
   Frag<T> kf[D / 16], vf[D / 16];
@@ -361,13 +363,15 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     return {reinterpret_cast<const float2*>(a.stats)[row], p.delta[row]};
   };
   const auto put_row = [&](int step, const Place& at, const Row& x) {
-    float* const to = lds_rows + step % RING * 3 * ROWS + tid;
+    float* const to = lds_rows + step % RING * ARRAYS * ROWS + tid;
     const bool none = at.head >= group || at.query + tid >= a.n_q;
-    to[0] = none ? ninf() : -x.stats.x, to[ROWS] = none ? 0.f : x.stats.y * sc.p, to[2 * ROWS] = none ? 0.f : -x.delta;
+    const Reference ref = reference<T>(x.stats.x, p.c);
+    if constexpr (T::PARTS == 1) to[3 * ROWS] = ref.c;
+    to[0] = none ? ninf() : -ref.at, to[ROWS] = none ? 0.f : x.stats.y * sc.p, to[2 * ROWS] = none ? 0.f : -x.delta;
   };
   const auto write = [&](int step, const Place& at) {
     unsigned char* const to = smem + step % BUFS * BUF;
-    const float* const rows = lds_rows + step % RING * 3 * ROWS;
+    const float* const rows = lds_rows + step % RING * ARRAYS * ROWS;
     const auto keep = [&](int i) { return rows[ROWS + i] != 0.f; };
     if constexpr (W == 1) stage.fetch_and_write(queries(at, a.q, a.q_stride), queries(at, a.gout, a.gout_stride), at.query, to, tid, keep);
     else stage.write(to, tid, keep);
@@ -423,7 +427,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
 
   v16f dk[D / 32] = {}, dv[D / 32] = {};
   for (int r = first, step = 0; r < last; ++r, ++step) {
-    const float* const rows = lds_rows + step % RING * 3 * ROWS;
+    const float* const rows = lds_rows + step % RING * ARRAYS * ROWS;
     const unsigned char* const lds_q = smem + step % BUFS * BUF;
     const unsigned char* const lds_qt = lds_q + Tl::BYTES;
     const unsigned char* const lds_g = lds_q + 2 * Tl::BYTES;
@@ -474,10 +478,11 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
       for (int i = 0; i < D / 16; ++i) mma<T, true>(Tl::by_rows(lds_q, i, lane), kf[i], s);
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        float ms[4];
+        float ms[4], cs[4] = {1.f, 1.f, 1.f, 1.f};
         read16(rows + 8 * g + 4 * half, ms);
+        if constexpr (T::PARTS == 1) read16(rows + 3 * ROWS + 8 * g + 4 * half, cs);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[4 * g + i] = exp2_(T::PARTS == 3 ? s[4 * g + i] + ms[i] : fmaf(s[4 * g + i], p.c, ms[i]));
+        for (int i = 0; i < 4; ++i) s[4 * g + i] = exp2_(off_reference<T>(s[4 * g + i], Reference{-ms[i], cs[i]}));
       }
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) mma<T>(Tl::by_rows(lds_g, i, lane), vf[i], dp);
@@ -571,7 +576,7 @@ template <class T, int D> void backward_d(Args& p, const Plans& plans, float* pa
     return;
   }
   use(plans.grad_kv, partial_kv);
-  const size_t lds_kv = (plans.grad_kv.waves == 1 ? kv_buffers<T, D, 1>() : kv_buffers<T, D, 4>()) * 4 * Tile<T, D>::BYTES + (3 * RING * ROWS + 2 * 32 * plans.grad_kv.waves * BUCKET_LD + (a.buckets ? a.heads / a.kv_heads * (a.n_buckets + 1) : 0)) * sizeof(float);
+  const size_t lds_kv = (plans.grad_kv.waves == 1 ? kv_buffers<T, D, 1>() : kv_buffers<T, D, 4>()) * 4 * Tile<T, D>::BYTES + (row_arrays<T> * RING * ROWS + 2 * 32 * plans.grad_kv.waves * BUCKET_LD + (a.buckets ? a.heads / a.kv_heads * (a.n_buckets + 1) : 0)) * sizeof(float);
   if constexpr (few_waves<T, D>) {
     if (plans.grad_kv.waves == 1) launch(grad_kv_kernel<T, D, 1>, p, 1, lds_kv, stream, pairs);
   }

@@ -55,7 +55,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
   const signed char* const buckets = a.buckets ? a.buckets + b * a.bucket_stride[0] + query * a.bucket_stride[1] : nullptr;
   const float* const table = lds_table + (head - head0) * (a.n_buckets + 1);
   const bool measure = a.stats && tile == 0;                // this workgroup finds the largest |v| of its keys for the backward pass
-  const float dead = ninf() * p.inv_c;
+  const float dead = ninf();
 
   Stage<T, D, 64 * W, BY_ROWS, BY_ENTRIES> stage;
   unsigned words[4] = {0, 0, 0, 0};
@@ -64,7 +64,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     if (W > 1) stage.fetch(k, v, key0, tid);
     if (buckets) load_buckets(buckets, key0, end, half, words);
   }
-  if (tid < 2 * ROWS) lds_kb[tid] = key_value(key0 < end ? load_key_bias(key_bias, key0 + tid, end) : 0.f, key0 + tid, end, p.inv_c);
+  if (tid < 2 * ROWS) lds_kb[tid] = key_value(key0 < end ? load_key_bias(key_bias, key0 + tid, end) : 0.f, key0 + tid, end, p.inv_c, p.most);
   float bias_ahead = tid < ROWS && key0 < end ? load_key_bias(key_bias, key0 + 2 * ROWS + tid, end) : 0.f;
   if (buckets) stage_table<T>(lds_table, a.table, a.n_buckets, head0, heads, tid, 64 * W);
   Frag<T> qf[D / 16];
@@ -85,8 +85,8 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     if (key0 + ROWS < end) stage.fetch(k, v, key0 + ROWS, tid);
   }
 
-  constexpr float SHIFT = T::HALF ? 10.f : 0.f;       // probabilities times 2^10 in float16: its smallest normal number is 2^-14
   float m = ninf(), l = 0.f;
+  Reference ref = reference<T>(0.f, p.c);
   v16f o[D / 32] = {};
   int step = 0;
   for (int key = key0; key < end; key += ROWS, ++step) {
@@ -100,7 +100,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     const unsigned char* const lds_v = lds_k + Tl::BYTES;
     const float* const kb = lds_kb + step % RING * ROWS;
 
-    if (tid < ROWS) lds_kb[(step + 2) % RING * ROWS + tid] = key_value(bias_ahead, key + 2 * ROWS + tid, end, p.inv_c);
+    if (tid < ROWS) lds_kb[(step + 2) % RING * ROWS + tid] = key_value(bias_ahead, key + 2 * ROWS + tid, end, p.inv_c, p.most);
     if (BUFS == 2 && more) write(step + 1);
     if (tid < ROWS) bias_ahead = load_key_bias(key_bias, key + 3 * ROWS + tid, end);
     if (W > 1 && key + BUFS * ROWS < end) stage.fetch(k, v, key + BUFS * ROWS, tid);
@@ -117,17 +117,17 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
       top = ceilf(fmaxf(T::PARTS == 3 ? half_max(top) : half_max(top) * p.c, m));
-      const float ref = (top == ninf() ? 0.f : top) - SHIFT;
-      const float fade = exp2_(m - SHIFT - ref);      // a power of two
-      if (__any(fade != 1.f)) {
+      if (__any(top != m)) {
+        const float fade = top == m ? 1.f : fade_to<T>(top, m);       // a power of two
         l *= fade;
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) o[i] *= fade;
+        m = top;
+        ref = reference<T>(top == ninf() ? 0.f : top, p.c);
       }
-      m = top;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        s[i] = exp2_(T::PARTS == 3 ? s[i] - ref : fmaf(s[i], p.c, -ref));
+        s[i] = exp2_(off_reference<T>(s[i], ref));
         if constexpr (T::PARTS == 3) l += s[i];
       }
 #pragma unroll
@@ -170,7 +170,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
   const float inv = any ? 1.f / l : 0.f;
   store_column<T, D>(static_cast<E*>(a.out) + b * a.out_stride[0] + head * a.out_stride[1] + query * a.out_stride[2], a.d, half, o, inv);
   if (T::PARTS == 1 && a.out_f32) store_column<F32, D>(a.out_f32 + row * a.d, a.d, half, o, inv);
-  if (half == 0 && a.stats) reinterpret_cast<float2*>(a.stats)[row] = any ? make_float2(m - SHIFT, inv) : make_float2(pinf(), 0.f);
+  if (half == 0 && a.stats) reinterpret_cast<float2*>(a.stats)[row] = any ? make_float2(m, inv) : make_float2(pinf(), 0.f);
 }
 
 // A workgroup joins the parts of one query, shared out to sixteen waves: lane s of a wave has the maximum and the sum of its part s (of 64
@@ -183,20 +183,19 @@ template <class T, int D> __global__ __launch_bounds__(64 * JOIN_WAVES) void joi
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const float* const part = p.partial;
   const float2* const ml = reinterpret_cast<const float2*>(part + p.splits * rows * D);
-  constexpr float SHIFT = T::HALF ? 10.f : 0.f;
   constexpr int PER = (D + 63) / 64;
   float m = ninf();
   for (int s = lane; s < p.splits; s += 64) m = fmaxf(m, ml[s * rows + row].x);
 #pragma unroll
   for (int i = 32; i; i >>= 1) m = fmaxf(m, __shfl_xor(m, i));
-  const float ref = m == ninf() ? 0.f : m;
+  const float top = m == ninf() ? 0.f : m;
   const int per_wave = (p.splits + JOIN_WAVES - 1) / JOIN_WAVES, first = wave * per_wave, last = min(p.splits, first + per_wave);
   float l = 0.f, o[PER] = {};
   for (int s0 = first; s0 < last; s0 += 64) {
     float w = 0.f;
     if (s0 + lane < last) {
       const float2 x = ml[(s0 + lane) * rows + row];
-      w = exp2_(x.x - ref);
+      w = fade_to<T>(top, x.x);
       l = fmaf(x.y, w, l);
     }
     const int n = min(64, last - s0);
@@ -236,7 +235,7 @@ template <class T, int D> __global__ __launch_bounds__(64 * JOIN_WAVES) void joi
     static_cast<E*>(a.out)[at + e] = (E)x;
     if (T::PARTS == 1 && a.out_f32) a.out_f32[row * a.d + e] = x;
   }
-  if (lane == 0 && a.stats) reinterpret_cast<float2*>(a.stats)[row] = any ? make_float2(m - SHIFT, inv) : make_float2(pinf(), 0.f);
+  if (lane == 0 && a.stats) reinterpret_cast<float2*>(a.stats)[row] = any ? make_float2(m, inv) : make_float2(pinf(), 0.f);
 }
 
 // The same for few parts, where what is read is many queries: D / 4 lanes a query, four entries a lane.  42378 queries of 128 entries in two
@@ -245,7 +244,6 @@ constexpr int FEW_PARTS = 8;
 template <class T, int D> __global__ __launch_bounds__(256) void join_few_kernel(Args p) {
   const s2cnn_attention_t& a = p.a;
   constexpr int LANES = D / 4;
-  constexpr float SHIFT = T::HALF ? 10.f : 0.f;
   const long rows = (long)a.batch * a.heads * a.n_q, row = ((long)blockIdx.x * 256 + threadIdx.x) / LANES;
   const int q = threadIdx.x % LANES;
   if (row >= rows) return;
@@ -253,11 +251,11 @@ template <class T, int D> __global__ __launch_bounds__(256) void join_few_kernel
   const float2* const ml = reinterpret_cast<const float2*>(part + p.splits * rows * D);
   float m = ninf();
   for (int s = 0; s < p.splits; ++s) m = fmaxf(m, ml[s * rows + row].x);
-  const float ref = m == ninf() ? 0.f : m;
+  const float top = m == ninf() ? 0.f : m;
   float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
   for (int s = 0; s < p.splits; ++s) {
     const float2 x = ml[s * rows + row];
-    const float w = exp2_(x.x - ref);
+    const float w = fade_to<T>(top, x.x);
     float y[4];
     read16(part + (s * rows + row) * D + 4 * q, y);
     l = fmaf(x.y, w, l);
@@ -270,7 +268,7 @@ template <class T, int D> __global__ __launch_bounds__(256) void join_few_kernel
   typedef typename T::type E;
   store_quad<T>(static_cast<E*>(a.out) + b * a.out_stride[0] + head * a.out_stride[1] + query * a.out_stride[2], q, a.d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
   if (T::PARTS == 1 && a.out_f32) store_quad<F32>(a.out_f32 + row * a.d, q, a.d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-  if (q == 0 && a.stats) reinterpret_cast<float2*>(a.stats)[row] = any ? make_float2(m - SHIFT, inv) : make_float2(pinf(), 0.f);
+  if (q == 0 && a.stats) reinterpret_cast<float2*>(a.stats)[row] = any ? make_float2(m, inv) : make_float2(pinf(), 0.f);
 }
 
 template <class T, int D> void forward_d(const Args& p, const Plans& plans, hipStream_t stream) {

@@ -397,14 +397,52 @@ def test_probabilities_of_both_passes_are_the_same(hip, bias, nq, nk, d, dtype):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dtype,size", [(F32, 3e4), (F32, 1e3), (BF16, 1e3), (F16, 1e3)], ids=["f32-3e4", "f32-1e3", "bf16", "f16"])
+@pytest.mark.parametrize("dtype,size", [(F32, 3e4), (F32, 1e3), (BF16, 1e3), (F16, 1e3), (BF16, 3e4), (BF16, 1e6), (F16, 4e3)],
+                         ids=["f32-3e4", "f32-1e3", "bf16", "f16", "bf16-3e4", "bf16-1e6", "f16-4e3"])
 @pytest.mark.parametrize("nq", [9, 150])
 def test_gradients_of_large_scores(hip, nq, dtype, size):
-    """Queries and keys of a thousand and more: scores of 10^7 to 10^10, which round to hundreds and lie further apart than that: one key has the row."""
+    """Queries and keys of a thousand and more: scores of 10^7 to 10^13, which round to hundreds and lie further apart than that: one key has the row."""
     s, g = _inputs(1, 2, 2, nq, 150, 64, dtype)
     s["q"] *= size
     s["k"] *= size
     _check(s, g, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("low", [torch.finfo(torch.float32).min, -1e30, -1e9, -1e8, -1e5])
+def test_masked_keys_beside_others(hip, low, dtype):
+    """Keys that a large negative bias leaves without weight, whole tiles of them before and after the others, in one pass and in parts."""
+    for nq, nk, kind in ((9, 150, {}), (150, 150, dict(nb=5)), (1, 1500, {}), (40, 1500, dict(nb=5, excluded=0.1))):
+        s, g = _inputs(1, 2, 2, nq, nk, 16, dtype, key_bias="all", **kind)
+        s["key_bias"][:70] = low
+        s["key_bias"][-40:] = low
+        _check(s, g, dtype, "%d %d" % (nq, nk))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("scale", [None, 3.0, 1e-3])
+@pytest.mark.parametrize("low", [torch.finfo(torch.float32).min, -1e30, -1e9, -1e7, 1e9, 1e30])
+def test_every_key_has_the_same_large_bias(hip, low, scale, dtype):
+    """Weights that add up to one in both passes (see test_probabilities_of_both_passes_are_the_same), and even ones where the bias leaves nothing
+    of the scores, 2^-24 of 10^30 being far more than any.  Each of the values' gradients is rounded: below float16's smallest normal number by
+    2^-25."""
+    for nq, nk in ((9, 150), (150, 150), (1, 1500)):
+        s, g = _inputs(1, 2, 2, nq, nk, 16, dtype)
+        s["key_bias"] = torch.full((nk,), low, device="cuda")
+        values = s["v"]
+        if abs(low) >= 1e30:
+            _close(s2cnn_amd.attention(**s, scale=scale), values.cpu().double().mean(2, keepdim=True).expand(-1, -1, nq, -1), dtype, "even")
+        s["v"] = torch.ones_like(values)
+        for n in ("q", "k", "v"):
+            s[n].requires_grad_()
+        out = s2cnn_amd.attention(**s, scale=scale)
+        assert (out.double() - 1).abs().max().item() <= TOL[dtype]
+        gq, gk, gv = torch.autograd.grad(out, [s["q"], s["k"], s["v"]], g)
+        spacing = nk * 2.0 ** -25 if dtype == F16 else 0.0
+        assert ((gv.double().sum(2) - g.double().sum(2)).abs() <= TOL[dtype] * g.double().abs().sum(2) + spacing).all()
+        assert torch.isfinite(gq).all() and torch.isfinite(gk).all()
 
 
 @pytest.mark.gpu
