@@ -493,8 +493,8 @@ template <class T, int D, int THREADS, int LA, int LB, bool SCALE = false> struc
 //
 // The product starts from the biases instead of zero: x = c (q.k + bias / c), c = log2(e) |scale|; float32 takes c into the queries as
 // they are loaded, and needs no factor; the other types take the sign.  All kernels form a score from the same numbers in the same order: the
-// references are of scores as the forward pass had them, and a score of a thousand that is rounded otherwise makes another probability.  Biases are held within +-3e38 of a score, so that one of the type's lowest value
-// stays finite: keys that all have it share a row evenly.
+// references are of scores as the forward pass had them, and a score of a thousand that is rounded otherwise makes another probability.  Biases of keys and entries of the table are held within +-1.5e38 of a score, so that
+// the type's lowest value stays finite, and the sum of two: keys that all have it share a row evenly.
 // In two steps, the load and what is made of it: the tiles' loads are under way in between, and a wait for this one, issued before them,
 // is no wait for them.
 __device__ __forceinline__ float load_key_bias(const float* key_bias, int key, int end) { return key_bias ? key_bias[max(min(key, end - 1), 0)] : 0.f; }
@@ -531,12 +531,14 @@ template <class T> __device__ __forceinline__ float fade_to(float b, float a) { 
 // they would wait for its tile's loads too, which are issued after them.
 constexpr int RING = 4;
 
-// the table's rows of heads head0 .. head0 + heads - 1 in LDS, n_buckets + 1 entries a head, the last one for excluded pairs
-template <class T> __device__ __forceinline__ void stage_table(float* lds, const void* table, int n_buckets, int head0, int heads, int tid, int threads) {
+// the table's rows of heads head0 .. head0 + heads - 1 in LDS, n_buckets + 1 entries a head, the last one for excluded pairs; most: the largest
+// magnitude of a finite one
+template <class T> __device__ __forceinline__ void stage_table(float* lds, const void* table, int n_buckets, int head0, int heads, float most, int tid, int threads) {
   const typename T::type* t = static_cast<const typename T::type*>(table);
   for (int k = tid; k < heads * (n_buckets + 1); k += threads) {
     const int h = k / (n_buckets + 1), n = k % (n_buckets + 1);
-    lds[k] = n == n_buckets ? ninf() : (float)t[(long)(head0 + h) * n_buckets + n] * LOG2E;
+    const float x = n == n_buckets ? ninf() : (float)t[(long)(head0 + h) * n_buckets + n];
+    lds[k] = fabsf(x) < pinf() ? __builtin_amdgcn_fmed3f(x * LOG2E, -most, most) : x;
   }
 }
 

@@ -103,7 +103,7 @@ Args args_of(const s2cnn_attention_t& a, const Plans& plans) {
   const float c = a.dtype == S2CNN_F32 ? 1.f : fabsf(a.scale) * LOG2E;
   p.c = c < 1e-30f ? 1e-30f : c;
   p.inv_c = 1.f / p.c;
-  p.most = 3e38f / (p.c > 1.f ? p.c : 1.f);                // times c, too, it is finite
+  p.most = 1.5e38f / (p.c > 1.f ? p.c : 1.f);              // twice it is finite, times c too
   return p;
 }
 

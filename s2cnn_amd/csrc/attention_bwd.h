@@ -114,7 +114,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
   }
   if (tid < 2 * ROWS) lds_kb[tid] = key_value(key0 < end ? load_key_bias(key_bias, key0 + tid, end) : 0.f, key0 + tid, end, p.inv_c, p.most);
   float bias_ahead = tid < ROWS && key0 < end ? load_key_bias(key_bias, key0 + 2 * ROWS + tid, end) : 0.f;
-  if (buckets) stage_table<T>(lds_table, a.table, a.n_buckets, head, 1, tid, 64 * W);
+  if (buckets) stage_table<T>(lds_table, a.table, a.n_buckets, head, 1, p.most * p.c, tid, 64 * W);
   if (table_grad)
     for (int n = tid; n < TableSums::words(a.n_buckets); n += 64 * W) lds_sums[n] = 0;
 
@@ -416,7 +416,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
     if (buckets) fetch_buckets(here);
     if (tid < ROWS) put_row(0, here, load_row(here)), put_row(1, next, load_row(next)), ahead = load_row(after);
   }
-  if (buckets) stage_table<T>(lds_table, a.table, a.n_buckets, hk * group, group, tid, 64 * W);
+  if (buckets) stage_table<T>(lds_table, a.table, a.n_buckets, hk * group, group, p.most * p.c, tid, 64 * W);
   if (BUFS == 2) {
     __syncthreads();
     if (first < last) write(0, here);

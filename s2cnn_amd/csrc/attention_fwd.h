@@ -66,7 +66,7 @@ template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS *
   }
   if (tid < 2 * ROWS) lds_kb[tid] = key_value(key0 < end ? load_key_bias(key_bias, key0 + tid, end) : 0.f, key0 + tid, end, p.inv_c, p.most);
   float bias_ahead = tid < ROWS && key0 < end ? load_key_bias(key_bias, key0 + 2 * ROWS + tid, end) : 0.f;
-  if (buckets) stage_table<T>(lds_table, a.table, a.n_buckets, head0, heads, tid, 64 * W);
+  if (buckets) stage_table<T>(lds_table, a.table, a.n_buckets, head0, heads, p.most * p.c, tid, 64 * W);
   Frag<T> qf[D / 16];
   load_column<T, D>(static_cast<const E*>(a.q) + b * a.q_stride[0] + head * a.q_stride[1] + query * a.q_stride[2], a.d, ok, half,
                     a.scale * LOG2E, qf);

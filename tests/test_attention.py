@@ -268,6 +268,24 @@ def test_infinite_entries_of_the_table_exclude(hip):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("nq,nk", [(9, 70), (150, 70), (2, 1500)])
+def test_lowest_value_in_the_table(hip, nq, nk, dtype):
+    """Entries of the type's lowest value: no weight beside other pairs, even weights in a row that has no others (of float16 it is a bias as any
+    other; 64 bits lose the scores beside that of the others, too), on keys of the lowest bias as well."""
+    for low_keys in (False, True):
+        s, g = _inputs(2, 2, 1, nq, nk, 16, dtype, nb=4, excluded=0.1, key_bias="all")
+        s["table"][:, 2] = torch.finfo(dtype).min
+        if dtype != F16:
+            s["buckets"][1] = 2
+        if low_keys:
+            s["key_bias"][3:40] = torch.finfo(F32).min
+        out, grads = _check(s, g, dtype)
+        if dtype != F16 and not low_keys:
+            _close(out[:, :, 1], s["v"].cpu().double().mean(2).expand(-1, 2, -1), dtype, "even")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
 def test_layouts(hip, dtype):
     """Contiguous, heads split off a joint projection, unaligned, reversed axes, a strided last axis, shared (expanded) inputs."""
