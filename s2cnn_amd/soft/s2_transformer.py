@@ -99,7 +99,10 @@ class S2AttentionPool(nn.Module):
 
 class S2Transformer(nn.Module):
     """A stack of blocks and the pooling after it: [batch, features, 2b, 2b] -> [batch, features].  `drops` counts the forward passes on
-    the device, so that each training step drops others, replayed from a graph too."""
+    the device, so that each training step drops others, replayed from a graph too.
+
+    A pass that is run again in the backward pass, to save memory, has to drop what the first one did: its seeds are taken before it and
+    given to both, `checkpoint(model, x, model.next_seeds())`.  Without them it is refused there."""
 
     def __init__(self, features, heads, b, layers, n_buckets=32, max_angle=math.pi, dropout=0.0):
         super().__init__()
@@ -109,12 +112,19 @@ class S2Transformer(nn.Module):
         self.register_buffer("drops", torch.zeros(1, dtype=torch.int64))
         self.register_buffer("calls", torch.arange(2 * layers), persistent=False)
 
-    def forward(self, x):  # pylint: disable=W
+    def next_seeds(self):
+        """The seeds of the dropouts of one pass in training, [2 layers]: others at each call."""
+        self.drops.add_(1)
+        return self.drops * (2 * len(self.blocks)) + self.calls
+
+    def forward(self, x, seeds=None):  # pylint: disable=W
+        """seeds: from next_seeds, or None to count one pass on"""
+        if self.training and seeds is None:
+            if torch._C._current_graph_task_id() != -1 and any(block.dropout for block in self.blocks):
+                raise RuntimeError("S2Transformer run again in the backward pass: it would drop other elements than before; give it the seeds of next_seeds()")
+            seeds = self.next_seeds()
+        seeds = (seeds if self.training else self.calls).split(1)
         h = x.flatten(2).transpose(1, 2).contiguous()                       # [batch, points, features]
-        seeds = self.calls.split(1)
-        if self.training:
-            self.drops.add_(1)
-            seeds = (self.drops * (2 * len(self.blocks)) + self.calls).split(1)
         h, y = self.blocks[0].norm(h)
         for i, block in enumerate(self.blocks):
             following = self.blocks[i + 1].norm1 if i + 1 < len(self.blocks) else self.last_norm

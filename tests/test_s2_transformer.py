@@ -109,6 +109,37 @@ def test_sixteen_bit_and_autocast(hip, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_run_again_in_the_backward_pass(hip, reentrant):
+    """With its seeds given, a pass that is formed again in the backward pass gives the gradients of the one that is kept; without them it is
+    refused (two passes may have been counted since), unless nothing is dropped."""
+    from torch.utils.checkpoint import checkpoint
+    model = _stack(dropout=0.25).cuda()
+    gen = torch.Generator().manual_seed(3)
+    x, g = torch.randn(2, 24, 6, 6, generator=gen).cuda(), torch.randn(2, 24, generator=gen).cuda()
+
+    def gradients(f):
+        model.zero_grad()
+        xs = x.clone().requires_grad_()
+        y = f(xs)
+        y.backward(g)
+        return [y.detach(), xs.grad] + [p.grad for p in model.parameters()]
+
+    seeds = model.next_seeds()
+    want = gradients(lambda t: model(t, seeds))
+    for a, b in zip(gradients(lambda t: checkpoint(model, t, seeds, use_reentrant=reentrant)), want):
+        assert torch.equal(a, b)
+    blocks = torch.cat([model(x, s) for s in (seeds, model.next_seeds())])
+    assert torch.equal(blocks[:2], want[0]) and not torch.equal(blocks[2:], want[0])
+    with pytest.raises(RuntimeError, match="next_seeds"):
+        gradients(lambda t: checkpoint(model, t, use_reentrant=reentrant))
+    for block in model.blocks:
+        block.dropout = 0.0
+    for a, b in zip(gradients(lambda t: checkpoint(model, t, use_reentrant=reentrant)), gradients(model)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
 def test_network_trains_and_reloads(hip):
     model, losses, _ = harness.train_steps("sphere_transformer", batch=8, steps=8, warmup=0, lr=0.02)
     print("sphere transformer losses:", ["%.4f" % l for l in losses], flush=True)
