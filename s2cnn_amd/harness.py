@@ -114,12 +114,12 @@ class SphereTransformer(nn.Module):
     sphere in place of further layers and of the integral.  S2Conv 6->96 (b 64->10, kernel about the identity), ReLU, the
     mean over gamma (a signal on the sphere), two blocks of 6 heads with a bias by 32 buckets of the angle, pooling, Linear."""
 
-    def __init__(self, nclasses, dropout=0.1):
+    def __init__(self, nclasses, dropout=0.1, seed=0):
         super().__init__()
         features, b_in, b = 96, 64, 10
         grid = s2_near_identity_grid(n_alpha=8, max_beta=0.2, n_beta=2)
         self.conv = S2Convolution(nfeature_in=6, nfeature_out=features, b_in=b_in, b_out=b, grid=grid, activation="relu")
-        self.transformer = S2Transformer(features, heads=6, b=b, layers=2, dropout=dropout)
+        self.transformer = S2Transformer(features, heads=6, b=b, layers=2, dropout=dropout, seed=seed)
         self.out_layer = nn.Linear(features, nclasses)
 
     def forward(self, x):  # pylint: disable=W0221

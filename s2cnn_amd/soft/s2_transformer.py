@@ -102,15 +102,20 @@ class S2Transformer(nn.Module):
     the device, so that each training step drops others, replayed from a graph too.
 
     A pass that is run again in the backward pass, to save memory, has to drop what the first one did: its seeds are taken before it and
-    given to both, `checkpoint(model, x, model.next_seeds())`.  Without them it is refused there."""
+    given to both, `checkpoint(model, x, model.next_seeds())`.  Without them it is refused there.
 
-    def __init__(self, features, heads, b, layers, n_buckets=32, max_angle=math.pi, dropout=0.0):
+    What is dropped is a function of `seed` and of the count alone, not of torch's generator: stacks of one network, the ranks of a
+    data-parallel job and runs that are to differ need a `seed` each (`torch.initial_seed() + rank`, say).  Its low 32 bits count, and stacks
+    in which they differ never use the same number.  It is the program's to keep, as the learning rate is: no part of the state dict."""
+
+    def __init__(self, features, heads, b, layers, n_buckets=32, max_angle=math.pi, dropout=0.0, seed=0):
         super().__init__()
         self.blocks = nn.ModuleList(S2TransformerBlock(features, heads, b, n_buckets, max_angle, dropout=dropout) for _ in range(layers))
         self.last_norm = _Norm(features)
         self.pool = S2AttentionPool(features, heads, b)
         self.register_buffer("drops", torch.zeros(1, dtype=torch.int64))
-        self.register_buffer("calls", torch.arange(2 * layers), persistent=False)
+        high = (seed & 0xFFFFFFFF) << 32                                    # the count takes the low 32 bits
+        self.register_buffer("calls", torch.arange(2 * layers) + (high - (1 << 64) if high >> 63 else high), persistent=False)
 
     def next_seeds(self):
         """The seeds of the dropouts of one pass in training, [2 layers]: others at each call."""

@@ -139,6 +139,28 @@ def test_run_again_in_the_backward_pass(hip, reentrant):
         assert torch.equal(a, b)
 
 
+def test_seeds_of_stacks():
+    """Stacks of other seeds, of whatever depth, share no number in any of their passes; one of the same seed repeats them; without one they count
+    from the number of calls, as ever.  `seed` may be any integer."""
+    def first(seed, layers=2, passes=50):
+        model = s2cnn_amd.S2Transformer(8, 2, 2, layers, dropout=0.1, **({} if seed is None else {"seed": seed}))
+        return [n for _ in range(passes) for n in model.next_seeds().tolist()]
+
+    assert first(None)[:4] == [4, 5, 6, 7] and first(0) == first(None)
+    seeds = (0, 1, 2, 12345, -1, 2 ** 31, 2 ** 32 - 2)
+    numbers = [n for seed in seeds for n in first(seed, 1 + seed % 3)]
+    assert len(set(numbers)) == len(numbers)
+    assert first(7) == first(7) and first(7) == first(7 + 2 ** 40)
+
+
+@pytest.mark.gpu
+def test_stacks_of_one_network_drop_other_elements(hip):
+    x = torch.randn(2, 24, 6, 6, generator=torch.Generator().manual_seed(2)).cuda()
+    with torch.no_grad():
+        a, b, again = (_stack(dropout=0.25, **kw).cuda()(x) for kw in (dict(), dict(seed=1), dict(seed=1)))
+    assert not torch.equal(a, b) and torch.equal(b, again)
+
+
 @pytest.mark.gpu
 def test_network_trains_and_reloads(hip):
     model, losses, _ = harness.train_steps("sphere_transformer", batch=8, steps=8, warmup=0, lr=0.02)
