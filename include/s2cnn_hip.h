@@ -418,7 +418,7 @@ int s2cnn_so3_integrate_grad(const float *g, const float *w, float *gx, int b, l
  * Types of q, k, v, table, out and all gradients: dtype; sums, the softmax and its gradient are float32, float32 products
  * have float32 errors.  A tensor's vectors are contiguous, strides are those of (batch, head, vector) in entries.
  * Optional pointers may be NULL: table and buckets (together; n_buckets 0), key_bias, lengths, stats and out_f32 (if no
- * backward pass follows).  fwd reads q .. lengths and writes out, stats and out_f32; bwd reads those and gout and writes gq, and where not NULL gtable,
+ * backward pass follows); where n_k is 0 also k, v and buckets.  fwd reads q .. lengths and writes out, stats and out_f32; bwd reads those and gout and writes gq, and where not NULL gtable,
  * gk and gv (both or none).  Results do not depend on the order of execution.
  */
 #define S2CNN_F32 0

@@ -534,6 +534,24 @@ def test_some_gradients_only_and_empty_sizes(hip):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+def test_no_keys_with_a_table(hip, dtype):
+    """n_k = 0 with buckets (an empty tensor, which has no address), key biases and lengths: zeros, as without them."""
+    for per_batch in (False, True):
+        s, g = _inputs(2, 4, 2, 5, 0, 8, dtype, nb=3, per_batch=per_batch, key_bias="all")
+        s["lengths"] = torch.zeros(2, dtype=torch.int32, device="cuda")
+        with torch.no_grad():
+            assert (s2cnn_amd.attention(**s) == 0).all()
+        names = ["q", "k", "v", "table"]
+        for n in names:
+            s[n].requires_grad_()
+        out = s2cnn_amd.attention(**s)
+        assert out.shape == (2, 4, 5, 8) and (out == 0).all()
+        for n, grad in zip(names, torch.autograd.grad(out, [s[n] for n in names], g)):
+            assert grad.shape == s[n].shape and (grad == 0).all()
+
+
+@pytest.mark.gpu
 def test_double_backward_is_refused(hip):
     s, g = _inputs(1, 1, 1, 4, 5, 8, F32)
     q = s["q"].requires_grad_()
@@ -613,6 +631,19 @@ def test_entry_points_refuse_without_a_gpu():
     assert lib.s2cnn_attention_workspace(long_axis, 0) > 0                      # the keys are split
     assert lib.s2cnn_attention_fwd(long_axis, None, 0, None) == -2
     assert lib.s2cnn_attention_workspace(a(d=0), 1) == 0
+
+
+def _sizes(**kw):
+    """floats of the statistics of a call of these sizes, 0 if it is refused (host only)"""
+    import ctypes
+    from s2cnn_amd import _hip
+    a = _hip.Attention(**{**dict(batch=1, heads=2, kv_heads=1, n_q=4, n_k=5, d=8, scale=1.0), **kw})
+    return _hip.lib().s2cnn_attention_stats_floats(ctypes.byref(a))
+
+
+def test_no_keys_need_no_buckets():
+    assert _sizes(n_k=0, table=0x1000, n_buckets=3) > 0
+    assert _sizes(table=0x1000, n_buckets=3) == 0 and _sizes(n_k=0, buckets=0x1000, n_buckets=3) == 0
 
 
 def test_angle_buckets():
