@@ -427,7 +427,7 @@ int s2cnn_so3_integrate_grad(const float *g, const float *w, float *gx, int b, l
 
 typedef struct s2cnn_attention_t {
   const void *q, *k, *v;       /* [batch, heads, n_q, d], [batch, kv_heads, n_k, d] twice   */
-  const void *table;           /* [heads, n_buckets], n_buckets <= 64                      */
+  const void *table;           /* [heads, n_buckets], n_buckets <= 64, heads <= 128 kv_heads */
   const signed char *buckets;  /* [batch, n_q, n_k], rows contiguous                       */
   const float *key_bias;       /* [batch, n_k], rows contiguous                            */
   const int *lengths;          /* [batch]                                                  */

@@ -18,6 +18,7 @@ from . import _hip
 
 MAX_HEAD = 128
 MAX_BUCKETS = 64
+MAX_GROUP = 128                  # heads that share a key head where there are buckets: a workgroup holds the table's rows of all of them
 
 
 def _vectors(t):
@@ -113,7 +114,7 @@ def attention(q, k, v, table=None, buckets=None, key_bias=None, lengths=None, sc
 
     :param q: [batch, heads, n_q, d], d <= 128; float32, bfloat16 or float16, any strides (copied if the last axis is strided)
     :param k, v: [batch, kv_heads, n_k, d], kv_heads dividing heads: head h reads the keys of h // (heads // kv_heads)
-    :param table: [heads, n_buckets], n_buckets <= 64, the type of q: the learned bias; with buckets
+    :param table: [heads, n_buckets], n_buckets <= 64, the type of q: the learned bias; with buckets, and at most 128 heads a key head
     :param buckets: [n_q, n_k] or [batch, n_q, n_k] int8: the bucket of every pair.  A number outside 0 .. n_buckets - 1
         excludes the pair; what k and v hold there has still to be finite, as 0 * inf is not 0
     :param key_bias: [n_k] or [batch, n_k] float32, not differentiated: logarithms of quadrature weights, or -inf for a key
@@ -134,6 +135,7 @@ def attention(q, k, v, table=None, buckets=None, key_bias=None, lengths=None, sc
     n_q, n_k = q.size(2), k.size(2)
     if table is not None:
         assert table.dim() == 2 and table.size(0) == q.size(1) and 1 <= table.size(1) <= MAX_BUCKETS
+        assert q.size(1) <= MAX_GROUP * k.size(1), "at most %d heads a key head with buckets" % MAX_GROUP
         assert buckets.shape in ((n_q, n_k), (q.size(0), n_q, n_k))
     assert key_bias is None or key_bias.shape in ((n_k,), (q.size(0), n_k))
     assert lengths is None or lengths.shape == (q.size(0),)

@@ -23,6 +23,7 @@ typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr int ROWS = 32;             // rows of a staged tile, columns of a wave
 constexpr int MAX_BUCKETS = 64;
+constexpr int MAX_GROUP = 128;       // heads that share a key head where there are buckets: the table's rows of all of them are 33 KB of LDS
 
 struct F32 { typedef float type; static constexpr int PARTS = 3; static constexpr bool HALF = false; };
 struct BF16 { typedef __bf16 type; static constexpr int PARTS = 1; static constexpr bool HALF = false; };

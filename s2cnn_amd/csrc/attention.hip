@@ -49,7 +49,7 @@ bool sizes_ok(const s2cnn_attention_t* a) {
   if (a->dtype != S2CNN_F32 && a->dtype != S2CNN_BF16 && a->dtype != S2CNN_F16) return false;
   if (a->batch < 1 || a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads || a->n_q < 1 || a->n_k < 0 || a->d < 4 || a->d > 128) return false;
   const bool bias = a->buckets || a->table || a->n_buckets;
-  if (bias && ((!a->buckets && a->n_k > 0) || !a->table || a->n_buckets < 1 || a->n_buckets > MAX_BUCKETS || a->heads / a->kv_heads > 128)) return false;
+  if (bias && ((!a->buckets && a->n_k > 0) || !a->table || a->n_buckets < 1 || a->n_buckets > MAX_BUCKETS || a->heads / a->kv_heads > MAX_GROUP)) return false;
   if (a->buckets && (a->bucket_stride[1] < 0 || a->bucket_stride[1] >= S2CNN_ATTENTION_STRIDE_LIMIT)) return false;
   const long limit = 1L << 30;
   if ((long)a->heads / a->kv_heads * a->n_q > limit || a->n_k > limit || (long)a->batch * a->heads > limit) return false;

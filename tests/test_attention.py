@@ -641,6 +641,26 @@ def _sizes(**kw):
     return _hip.lib().s2cnn_attention_stats_floats(ctypes.byref(a))
 
 
+def test_heads_that_share_a_key_head_with_buckets():
+    """128 of them at most: refused by name, and by the entry; any number without buckets."""
+    z = torch.zeros
+    n = z(1, 1, dtype=torch.int8)
+    with pytest.raises(AssertionError, match="128"):
+        s2cnn_amd.attention(z(1, 129, 1, 8), z(1, 1, 1, 8), z(1, 1, 1, 8), table=z(129, 3), buckets=n)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        s2cnn_amd.attention(z(1, 256, 1, 8), z(1, 2, 1, 8), z(1, 2, 1, 8), table=z(256, 3), buckets=n)
+    with_buckets = dict(table=0x1000, buckets=0x1000, n_buckets=3)
+    assert _sizes(heads=129, **with_buckets) == 0 and _sizes(heads=128, **with_buckets) > 0 and _sizes(heads=129) > 0
+
+
+@pytest.mark.gpu
+def test_most_heads_a_key_head(hip):
+    s, g = _inputs(1, 128, 1, 3, 40, 128, F32, nb=64)
+    _check(s, g, F32, "128 heads, 64 buckets")
+    s, g = _inputs(1, 129, 1, 3, 40, 16, F32)
+    _check(s, g, F32, "129 heads")
+
+
 def test_no_keys_need_no_buckets():
     assert _sizes(n_k=0, table=0x1000, n_buckets=3) > 0
     assert _sizes(table=0x1000, n_buckets=3) == 0 and _sizes(n_k=0, buckets=0x1000, n_buckets=3) == 0
