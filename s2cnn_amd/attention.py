@@ -75,7 +75,7 @@ class _Attention(torch.autograd.Function):
         few = buckets is None and q.size(2) < 32 and q.size(1) > k.size(1)       # queries of heads that share keys
         q, k, v = _even(_vectors(q), few), _vectors(k), _vectors(v)
         out = _like(q)
-        sizes = ((buckets.stride(0) if buckets.dim() == 3 else 0, buckets.stride(-2)) if buckets is not None else (0, 0),
+        sizes = ((buckets.stride(0) if buckets.dim() == 3 else 0, buckets.stride(-2) if q.size(2) > 1 else 0) if buckets is not None else (0, 0),
                  key_bias.stride(0) if key_bias is not None and key_bias.dim() == 2 else 0,
                  table.size(1) if table is not None else 0, dtype, scale)
         stats = exact = None

@@ -633,6 +633,22 @@ def test_entry_points_refuse_without_a_gpu():
     assert lib.s2cnn_attention_workspace(a(d=0), 1) == 0
 
 
+@pytest.mark.gpu
+def test_vectors_and_buckets_of_one_row_far_apart(hip):
+    """One query, or key, of a storage whose rows are 2^25 entries apart: the stride of an axis of one entry is nobody's limit."""
+    s, g = _inputs(2, 2, 1, 1, 50, 16, F32, nb=4, excluded=0.2)
+    wide = torch.full((2, 1 << 25), 3, dtype=torch.int8, device="cuda")
+    wide[1, 7:57] = s["buckets"][0]
+    want, grads = _check(dict(s), g, F32)
+    out, again = _check({**{n: t.detach() for n, t in s.items()}, "buckets": wide[1:, 7:57]}, g, F32)
+    assert torch.equal(out, want) and all(torch.equal(again[n], grads[n]) for n in grads)
+    far = torch.empty(2 * (1 << 25), dtype=BF16, device="cuda").as_strided((1, 2, 1, 16), (0, 16, 1 << 25, 1))
+    s, g = _inputs(1, 2, 2, 1, 1, 16, BF16)
+    far.copy_(s["q"])
+    for n in ("q", "k", "v"):
+        _check({**{m: t.detach() for m, t in s.items()}, n: far}, g, BF16)
+
+
 def _sizes(**kw):
     """floats of the statistics of a call of these sizes, 0 if it is refused (host only)"""
     import ctypes
