@@ -211,7 +211,7 @@ __device__ __forceinline__ unsigned load_word_at(const signed char* uniform, uns
 template <class T> __device__ __forceinline__ Quad load_quad(const typename T::type* p, int q, int d) {
   Quad v = load_four<T>(p + quad_at(q, d));
   // So many of its first entries count as zero.  A column's quads each have their own number and four conditions on it, which the
-  // compiler must not share between the vectors of a column (hundreds of scalar registers, and spills of them that gave wrong results):
+  // compiler must not share between the vectors of a column (hundreds of scalar registers, and spills of them that went with wrong results; the build refuses those):
   // the empty statement hides that the numbers are equal.
   int twice = 4 * q < d ? 4 * q - quad_at(q, d) : 4;
   asm volatile("" : "+v"(twice));
