@@ -416,7 +416,7 @@ int s2cnn_so3_integrate_grad(const float *g, const float *w, float *gx, int b, l
  * h' = h / (heads / kv_heads), n = buckets[b,i,j].  A key takes no part where j >= lengths[b] or key_bias[b,j] = -inf (its k and
  * v are not used at all then), a pair where n is outside 0 .. n_buckets - 1.  A row without any key: out = 0, no gradients.
  * Types of q, k, v, table, out and all gradients: dtype; sums, the softmax and its gradient are float32, float32 products
- * have float32 errors.  A tensor's vectors are contiguous, strides are those of (batch, head, vector) in entries.
+ * have float32 errors.  Entries of q, k, v and gout that take part are finite (of an infinite one come NaN or infinities).  A tensor's vectors are contiguous, strides are those of (batch, head, vector) in entries.
  * Optional pointers may be NULL: table and buckets (together; n_buckets 0), key_bias, lengths, stats and out_f32 (if no
  * backward pass follows); where n_k is 0 also k, v and buckets.  fwd reads q .. lengths and writes out, stats and out_f32; bwd reads those and gout and writes gq, and where not NULL gtable,
  * gk and gv (both or none).  Results do not depend on the order of execution.

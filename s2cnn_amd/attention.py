@@ -123,8 +123,13 @@ def attention(q, k, v, table=None, buckets=None, key_bias=None, lengths=None, sc
     :param scale: 1 / sqrt(d) if None
     :return out: [batch, heads, n_q, d]; zero for a query all of whose keys are excluded (its gradients are zero too)
 
-    Sums, the softmax and its gradient are float32; float32 operands are multiplied to the accuracy of float32, and of the other types
-    only the results are rounded.  The backward pass recomputes the probabilities.  Results do not depend on the order of execution.
+    Sums, the softmax and its gradient are float32; float32 operands are multiplied to the accuracy of float32.  Of the other types the results
+    are rounded, and before them nothing to less than 16 bits (float16: 22): probabilities and their gradients, as two parts.  The backward pass
+    recomputes the probabilities.  Results do not depend on the order of execution.
+
+    What takes part has to be finite.  Of an infinite entry of v or q, and of k in float32, come NaN (or an infinity) in all that depends on it,
+    where the formula may have an infinity, or no weight for that key: products are of parts of the operands, and an infinity has none.  A table's
+    entry or a key bias may be -inf; those of the type's lowest value leave no weight beside others, and even weights among themselves.
     """
     assert q.dim() == 4 and k.dim() == 4 and v.dim() == 4
     assert k.shape == v.shape

@@ -241,6 +241,35 @@ def test_keys_that_take_no_part_may_hold_anything(hip, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("nq", [5, 150])
+def test_what_is_not_finite_stays_where_it_is_and_is_not_lost(hip, nq, value, dtype):
+    """An infinite value, or one that is no number, of a key that takes part: no finite number in that entry of the output, the other entries as
+    ever.  In a query: nowhere but in its row.  In the gradient of a query: nowhere but in the gradients of its row and of the keys."""
+    s, g = _inputs(1, 2, 2, nq, 77, 24, dtype)
+    out, grads = _check(dict(s), g, dtype)
+    with torch.no_grad():
+        v = s["v"].clone()
+        v[0, 1, 70, 3] = value
+        got = s2cnn_amd.attention(s["q"], s["k"], v)
+        assert not torch.isfinite(got[0, 1, :, 3]).any()
+        got[0, 1, :, 3] = out[0, 1, :, 3]
+        assert torch.equal(got, out)
+        q = s["q"].clone()
+        q[0, 1, 2, 5] = value
+        got = s2cnn_amd.attention(q, s["k"], s["v"])
+        assert not torch.isfinite(got[0, 1, 2]).any()
+        got[0, 1, 2] = out[0, 1, 2]
+        assert torch.equal(got, out)
+    g = g.clone()
+    g[0, 1, 2, 5] = value
+    again = torch.autograd.grad(s2cnn_amd.attention(s["q"], s["k"], s["v"]), [s["q"], s["k"], s["v"]], g)
+    assert not torch.isfinite(again[0][0, 1, 2]).any() and not torch.isfinite(again[2][0, 1, :, 5]).any()
+    assert torch.equal(again[0][:, 0], grads["q"][:, 0]) and torch.equal(again[1][:, 0], grads["k"][:, 0]) and torch.equal(again[2][:, 0], grads["v"][:, 0])
+
+
+@pytest.mark.gpu
 def test_lowest_value_as_a_mask(hip):
     """Key biases of float32's lowest value: no weight beside other keys, even weights where all keys have it."""
     s, g = _inputs(2, 2, 2, 9, 70, 16, F32, key_bias="batch")
