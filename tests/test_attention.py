@@ -421,6 +421,31 @@ def test_scale_and_large_scores(hip):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("scale", [-0.5, 1e-3, 2.0, 0.0])
+@pytest.mark.parametrize("size", [(2, 4, 2, 3, 70, 24), (2, 4, 2, 150, 140, 24), (2, 2, 1, 1, 900, 100), (1, 2, 2, 40, 60, 2)], ids=lambda s: "x".join(map(str, s)))
+def test_gradients_at_other_scales(hip, size, scale, dtype):
+    """Negative, small, large and no scale, with a table, key biases and lengths: the 16-bit types take its sign into the queries, its magnitude
+    into the scores and its inverse into the biases.  float32's allowance is for scores of 8 and grows with them.  float16 gradients of a
+    small scale lie below its smallest normal number: spacings of 2^-24 on top."""
+    for kind in (dict(), dict(nb=5, excluded=0.1, key_bias="batch", ragged=True)):
+        s, g = _inputs(*size, dtype, **kind)
+        names = [n for n in ("q", "k", "v", "table") if n in s]
+        for n in names:
+            s[n].requires_grad_()
+        out = s2cnn_amd.attention(**s, scale=scale)
+        grads = torch.autograd.grad(out, [s[n] for n in names], g)
+        want, want_grads, mags = _reference(**s, scale=scale, g=g)
+        top = abs(scale) * s["q"].detach().norm(dim=-1).max().item() * s["k"].detach().norm(dim=-1).max().item()
+        tol = TOL[dtype] * (max(1.0, top / 8) if dtype == F32 else 1.0)
+        for what, t, exact, mag in [("out", out, want, None)] + [(n, t, want_grads[n], mags[n]) for n, t in zip(names, grads)]:
+            spacing = 2.0 ** -25 * math.sqrt(t.numel()) if dtype == F16 else 0.0
+            extra = 4 * 2.0 ** -24 * mag.norm().item() if mag is not None else 0.0
+            err = (t.detach().cpu().double() - exact).norm().item()
+            assert err <= tol * exact.norm().item() + extra + spacing, (what, kind, err, exact.norm().item())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
 @pytest.mark.parametrize("nq,nk,d", [(9, 150, 16), (150, 150, 16), (70, 40, 100)])
 @pytest.mark.parametrize("bias", [-1e4, -1e6, 1e6])
 def test_probabilities_of_both_passes_are_the_same(hip, bias, nq, nk, d, dtype):
@@ -507,6 +532,21 @@ def test_same_bits_every_time_and_on_other_streams(hip):
         assert torch.equal(again, out)
         for n, t in zip(names, got):
             assert torch.equal(t, grads[n]), n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("size", [(2, 4, 2, 200, 300, 64), (1, 8, 2, 2, 3000, 50), (3, 6, 3, 130, 700, 100)], ids=lambda s: "x".join(map(str, s)))
+def test_same_bits_every_time_in_sixteen_bits(hip, size, dtype):
+    """Other calls in between, so that workspaces and outputs lie in memory that held something else."""
+    s, g = _inputs(*size, dtype, nb=32, excluded=0.1, key_bias="all", ragged=size[0] > 1)
+    other, other_g = _inputs(*size, dtype, nb=32, excluded=0.1, key_bias="all", seed=1)
+    want, grads = _check(s, g, dtype)
+    for _ in range(3):
+        _check({n: t.detach() for n, t in other.items()}, other_g, dtype)
+        out = s2cnn_amd.attention(**s)
+        again = torch.autograd.grad(out, [s[n] for n in grads], g)
+        assert torch.equal(out, want) and all(torch.equal(a, b) for a, b in zip(again, grads.values()))
 
 
 @pytest.mark.gpu

@@ -170,6 +170,29 @@ def test_dropout(hip, n, dtype):
     assert torch.equal(s2cnn_amd.dropout(x, 1e-7, 1), x)                     # no multiple of 2^-16 but zero
 
 
+@pytest.mark.gpu
+@TYPES
+def test_dropout_of_large_tensors(hip, dtype):
+    """Sizes that go past the caches (float32) and beyond one round of the workgroups: the head and the tail against the generator in integers,
+    all of it against pieces, whose elements are those of the same index."""
+    n, p, seed = (1 << 26) + 1003, 0.3, 21
+    x = torch.ones(n, dtype=dtype, device="cuda")
+    y = s2cnn_amd.dropout(x, p, seed)
+    head = _factors(40000, p, seed).to(dtype)
+    assert torch.equal(y[:40000].cpu(), head)
+    first = (n - 4000) // 8 * 8
+    drop, bits = round(p * 65536), []
+    for c in range(first // 8, (n + 7) // 8):
+        for w in _philox(c, seed):
+            bits += [w & 0xFFFF, w >> 16]
+    tail = (torch.tensor(np.array(bits[:n - first]) >= drop).double() * (65536 / (65536 - drop))).to(dtype)
+    assert torch.equal(y[first:].cpu(), tail)
+    kept = (y != 0).double().mean().item()
+    assert abs(kept - (1 - drop / 65536)) < 6 * (0.3 * 0.7 / n) ** 0.5
+    for m in (1 << 20, (1 << 22) + 5):                                            # pieces from the start
+        assert torch.equal(s2cnn_amd.dropout(x[:m], p, seed), y[:m])
+
+
 def test_generator_known_answer():
     """The published answer of Philox4x32-10 for a zero counter and key, and for all bits set in the words used here."""
     assert _philox(0, 0) == [0x6627e8d5, 0xe169c58d, 0xbc57ac4c, 0x9b00dbd8]

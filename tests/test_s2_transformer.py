@@ -109,6 +109,33 @@ def test_sixteen_bit_and_autocast(hip, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("cast", [False, True], ids=["module", "autocast"])
+def test_sixteen_bit_gradients(hip, cast, dtype):
+    """As test_sixteen_bit_and_autocast, twice as many roundings on the way to a gradient: 20 units of the type in the 2-norm of all gradients of
+    the parameters together, and of the input's."""
+    model, plain = _stack(), _stack().double()
+    gen = torch.Generator().manual_seed(6)
+    x, g = torch.randn(2, 24, 6, 6, generator=gen), torch.randn(2, 24, generator=gen)
+    xp = x.double().requires_grad_()
+    _plain(plain, xp, [1.0] * 4, 3).backward(g.double())
+    unit = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -11
+    model.cuda()
+    if cast:
+        xg = x.cuda().requires_grad_()
+        with torch.autocast("cuda", dtype=dtype):
+            y = model(xg)
+    else:
+        model.to(dtype)
+        xg = x.cuda().to(dtype).requires_grad_()
+        y = model(xg)
+    y.backward(g.cuda().to(y.dtype))
+    assert _relative(xg.grad, xp.grad) < 20 * unit
+    a, b = (torch.cat([p.grad.detach().double().cpu().flatten() for p in m.parameters()]) for m in (model, plain))
+    assert _relative(a, b) < 20 * unit
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("reentrant", [False, True])
 def test_run_again_in_the_backward_pass(hip, reentrant):
     """With its seeds given, a pass that is formed again in the backward pass gives the gradients of the one that is kept; without them it is
