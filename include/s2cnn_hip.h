@@ -468,6 +468,10 @@ size_t s2cnn_layer_norm_bwd_workspace(long rows, long features, int dtype);
 int s2cnn_layer_norm_bwd(const void *h, const void *g, const void *g_h, const void *weight, const float *stats, void *gx, void *gresidual,
                          void *gweight, void *gbias, void *workspace, size_t workspace_bytes, long rows, long features, double p,
                          unsigned long long seed, const long long *seed_at, int step, int dtype, void *stream);
+/* out[f] = sum over the rows of x [rows, features], dense, of dtype; out and the sums float32: the gradient of a bias.  No memory is cleared on the
+ * way: the call can be captured into a graph (a sum that clears its counters with a memset gives other results there, from the second replay on). */
+size_t s2cnn_column_sums_workspace(long rows, long features, int dtype);
+int s2cnn_column_sums(const void *x, float *out, void *workspace, size_t workspace_bytes, long rows, long features, int dtype, void *stream);
 int s2cnn_dropout(const void *x, void *y, long n, double p, unsigned long long seed, const long long *seed_at, int dtype, void *stream);
 
 #ifdef __cplusplus

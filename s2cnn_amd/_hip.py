@@ -104,6 +104,8 @@ SIGNATURES = {
     "s2cnn_layer_norm_stats_floats": (_size_t, [_long, _long, _int, _int]),
     "s2cnn_layer_norm_bwd_workspace": (_size_t, [_long, _long, _int]),
     "s2cnn_layer_norm_bwd": (_int, [_vp] * 10 + [_size_t, _long, _long, ctypes.c_double, ctypes.c_ulonglong, _vp, _int, _int, _vp]),
+    "s2cnn_column_sums_workspace": (_size_t, [_long, _long, _int]),
+    "s2cnn_column_sums": (_int, [_vp, _vp, _vp, _size_t, _long, _long, _int, _vp]),
     "s2cnn_dropout": (_int, [_vp, _vp, _long, ctypes.c_double, ctypes.c_ulonglong, _vp, _int, _vp]),
     "s2cnn_so3_integrate_grad": (_int, [_c_float_p, _c_float_p, _c_float_p, _int, _long, _vp]),
 }

@@ -449,11 +449,28 @@ template <class T> __global__ __launch_bounds__(THREADS) void long_weights_kerne
   }
 }
 
-// the sums of the workgroups: 32 features a workgroup, 32 groups of lanes over the parts
-template <class T> __global__ __launch_bounds__(1024) void sum_kernel(const float* partial, int parts, int features, T* gw, T* gb) {
+// Sums over the rows of a tensor (the gradient of a bias), in parts like these: torch's own sum clears a counter in memory first, and a
+// captured graph that holds such a node gives other sums when it is replayed.
+template <class T> __global__ __launch_bounds__(THREADS) void column_parts_kernel(const T* x, float* partial, long rows, int features, int parts) {
+  __shared__ float sums[4][64];
+  const int i = threadIdx.x & 63, f = blockIdx.x * 64 + i, wave = threadIdx.x >> 6;
+  const long step = 4L * parts;
+  float t[4] = {0.f, 0.f, 0.f, 0.f};
+  if (f < features)
+    for (long r = (long)blockIdx.y * 4 + wave; r < rows; r += 4 * step)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (r + j * step < rows) t[j] += (float)x[(r + j * step) * features + f];
+  sums[wave][i] = (t[0] + t[1]) + (t[2] + t[3]);
+  __syncthreads();
+  if (wave == 0 && f < features) partial[(long)blockIdx.y * features + f] = (sums[0][i] + sums[1][i]) + (sums[2][i] + sums[3][i]);
+}
+
+// the sums of the workgroups, of `tensors` tensors: 32 features a workgroup, 32 groups of lanes over the parts
+template <class T> __global__ __launch_bounds__(1024) void sum_kernel(const float* partial, int parts, int features, int tensors, T* gw, T* gb) {
   __shared__ float sums[32][33];
   const int i = threadIdx.x & 31, s = threadIdx.x >> 5;
-  const long col = (long)blockIdx.x * 32 + i, width = 2L * features;
+  const long col = (long)blockIdx.x * 32 + i, width = (long)tensors * features;
   float t = 0.f;
   if (col < width)
     for (int k = s; k < parts; k += 32) t += partial[k * width + col];
@@ -560,13 +577,24 @@ template <class T> void backward(const Backward& p, bool step, int dtype, void* 
   if (!p.partial) return;
   if (is_long(dtype, p.features))
     hipLaunchKernelGGL(long_weights_kernel<T>, dim3((unsigned)((p.features + 63) / 64), (unsigned)parts), dim3(THREADS), 0, s, p, parts, step);
-  hipLaunchKernelGGL(sum_kernel<T>, dim3((unsigned)((2L * p.features + 31) / 32)), dim3(1024), 0, s, p.partial, parts, p.features, static_cast<T*>(gw),
+  hipLaunchKernelGGL(sum_kernel<T>, dim3((unsigned)((2L * p.features + 31) / 32)), dim3(1024), 0, s, p.partial, parts, p.features, 2, static_cast<T*>(gw),
                      static_cast<T*>(gb));
 }
 template <class T> void dropout(const void* x, void* y, long n, const Dropout& d, hipStream_t s) {
   const long need = (n + 8 * THREADS - 1) / (8 * THREADS), most = CUS * 16;
   hipLaunchKernelGGL(dropout_kernel<T>, dim3((unsigned)(need < most ? need : most)), dim3(THREADS), 0, s, static_cast<const T*>(x), static_cast<T*>(y), n, d,
                      (size_t)n * sizeof(T) >= STREAM_BYTES);
+}
+
+// At least 64 rows a part, and up to 1024 workgroups.
+int column_parts(long rows, long features) {
+  const long most = 1024 / ((features + 63) / 64), need = (rows + 63) / 64, parts = need < most ? need : most;
+  return parts < 1 ? 1 : (int)parts;
+}
+template <class T> void column_sums(const void* x, float* out, float* partial, long rows, int features, hipStream_t s) {
+  const int parts = column_parts(rows, features);
+  hipLaunchKernelGGL(column_parts_kernel<T>, dim3((unsigned)((features + 63) / 64), (unsigned)parts), dim3(THREADS), 0, s, static_cast<const T*>(x), partial, rows, features, parts);
+  hipLaunchKernelGGL(sum_kernel<float>, dim3((unsigned)((features + 31) / 32)), dim3(1024), 0, s, partial, parts, features, 1, out, nullptr);
 }
 
 bool sizes_ok(long rows, long features, int dtype) {
@@ -621,6 +649,23 @@ extern "C" int s2cnn_layer_norm_bwd(const void* h, const void* g, const void* g_
   if (dtype == S2CNN_F32) norm::backward<float>(b, step != 0, dtype, gweight, gbias, s);
   else if (dtype == S2CNN_BF16) norm::backward<__bf16>(b, step != 0, dtype, gweight, gbias, s);
   else norm::backward<half_t>(b, step != 0, dtype, gweight, gbias, s);
+  return launch_status();
+}
+
+extern "C" size_t s2cnn_column_sums_workspace(long rows, long features, int dtype) {
+  return sizes_ok(rows, features, dtype) ? (size_t)column_parts(rows, features) * features * sizeof(float) : 0;
+}
+
+extern "C" int s2cnn_column_sums(const void* x, float* out, void* workspace, size_t workspace_bytes, long rows, long features, int dtype, void* stream) {
+  clear_stale_error();
+  if (!sizes_ok(rows, features, dtype) || !x || !out) return S2CNN_EINVAL;
+  if (!aligned(dtype, x) || !aligned(S2CNN_F32, out)) return S2CNN_EALIGN;
+  if (!workspace || workspace_bytes < s2cnn_column_sums_workspace(rows, features, dtype) || !aligned16(workspace)) return S2CNN_EWORKSPACE;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  float* const partial = static_cast<float*>(workspace);
+  if (dtype == S2CNN_F32) norm::column_sums<float>(x, out, partial, rows, (int)features, s);
+  else if (dtype == S2CNN_BF16) norm::column_sums<__bf16>(x, out, partial, rows, (int)features, s);
+  else norm::column_sums<half_t>(x, out, partial, rows, (int)features, s);
   return launch_status();
 }
 

@@ -23,6 +23,7 @@ import torch.nn.functional as F
 from torch import nn
 
 from .soft.bn_relu import evaluate_sequence, run_sequence
+from .soft.s2_transformer import Linear
 from . import (S2Convolution, S2Transformer, SO3Convolution, s2_equatorial_grid, s2_near_identity_grid, so3_equatorial_grid, so3_integrate,
                so3_near_identity_grid)
 
@@ -120,7 +121,7 @@ class SphereTransformer(nn.Module):
         grid = s2_near_identity_grid(n_alpha=8, max_beta=0.2, n_beta=2)
         self.conv = S2Convolution(nfeature_in=6, nfeature_out=features, b_in=b_in, b_out=b, grid=grid, activation="relu")
         self.transformer = S2Transformer(features, heads=6, b=b, layers=2, dropout=dropout, seed=seed)
-        self.out_layer = nn.Linear(features, nclasses)
+        self.out_layer = Linear(features, nclasses)
 
     def forward(self, x):  # pylint: disable=W0221
         x = self.conv(x).mean(-1)                                           # [batch, feature, beta, alpha]

@@ -134,6 +134,26 @@ class _LayerNorm(torch.autograd.Function):
         return gx, gresidual, gw, gb, None, None, None, None, None
 
 
+@lru_cache(maxsize=1024)
+def _column_sums_bytes(rows, features, dtype):
+    return _hip.lib().s2cnn_column_sums_workspace(rows, features, dtype)
+
+
+def column_sums(x):
+    """Sums of x [..., features] (float32, bfloat16 or float16) over all other axes, float32.  Not differentiable: the gradient of a bias."""
+    dtype = _hip.require_gpu_float(x)
+    features = x.size(-1)
+    rows = x.numel() // features
+    if not rows:
+        return x.new_zeros(features, dtype=torch.float32)
+    x = x.contiguous()
+    out = x.new_empty(features, dtype=torch.float32)
+    nbytes = _column_sums_bytes(rows, features, dtype)
+    ws = _hip.workspace(nbytes, x.device)
+    _hip.call("s2cnn_column_sums", x.data_ptr(), out.data_ptr(), ws.data_ptr(), nbytes, rows, features, dtype, _hip.stream_ptr())
+    return out
+
+
 def _check_affine(x, weight, bias):
     assert x.dim() >= 1 and x.size(-1) >= 1
     assert weight is None or weight.shape == x.shape[-1:]

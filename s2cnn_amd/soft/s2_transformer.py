@@ -12,9 +12,53 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
+from .. import _hip
 from ..attention import attention, s2_angle_buckets, s2_log_weights
-from ..layer_norm import dropout_add_layer_norm, layer_norm
+from ..layer_norm import column_sums, dropout_add_layer_norm, layer_norm
 from ..s2_grid import s2_soft_grid
+
+
+class _BiasGradient(torch.autograd.Function):
+    """y, which has had the bias added to its last axis (without a gradient), and the gradient of the bias."""
+
+    @staticmethod
+    def forward(ctx, y, bias):  # pylint: disable=W
+        ctx.dtype = bias.dtype
+        return y.view_as(y)
+
+    @staticmethod
+    @_hip.once_differentiable
+    def backward(ctx, g):  # pylint: disable=W
+        return g, column_sums(g).to(ctx.dtype)
+
+
+class _Expand(torch.autograd.Function):
+    """x [...] for each of n signals: [n, ...], one storage."""
+
+    @staticmethod
+    def forward(ctx, x, n):  # pylint: disable=W
+        return x.expand(n, *x.shape)
+
+    @staticmethod
+    @_hip.once_differentiable
+    def backward(ctx, g):  # pylint: disable=W
+        return column_sums(g.reshape(g.size(0), -1)).to(g.dtype).view(g.shape[1:]), None
+
+
+def _sums_of_its_own(x, parameter):
+    """Whether the gradient of a parameter that all rows of x share is summed by the library: while a graph is captured.  torch's sum over many
+    rows clears a counter with a memset, and replays of a graph with such a node have other gradients from the second on.  Not otherwise:
+    nodes of autograd in Python cost an eager step of two blocks 0.12 ms of 2.6."""
+    return x.is_cuda and x.dtype in _hip.FLOATS and torch.cuda.is_current_stream_capturing() and parameter.requires_grad and torch.is_grad_enabled()
+
+
+class Linear(nn.Linear):
+    """nn.Linear that can be captured into a graph with its gradients."""
+
+    def forward(self, x):  # pylint: disable=W
+        if self.bias is None or not _sums_of_its_own(x, self.bias):
+            return super().forward(x)
+        return _BiasGradient.apply(F.linear(x, self.weight, self.bias.detach()), self.bias)
 
 
 class _Norm(nn.Module):
@@ -52,8 +96,8 @@ class S2TransformerBlock(nn.Module):
         self.features, self.heads, self.b, self.dropout = features, heads, b, dropout
         hidden = 2 * features if hidden is None else hidden
         self.norm1, self.norm2 = _Norm(features), _Norm(features)
-        self.qkv, self.out = nn.Linear(features, 3 * features), nn.Linear(features, features)
-        self.expand, self.contract = nn.Linear(features, hidden), nn.Linear(hidden, features)
+        self.qkv, self.out = Linear(features, 3 * features), Linear(features, features)
+        self.expand, self.contract = Linear(features, hidden), Linear(hidden, features)
         self.bias_table = nn.Parameter(torch.zeros(heads, n_buckets))
         self.register_buffer("buckets", s2_angle_buckets(s2_soft_grid(b), n_buckets=n_buckets, max_angle=max_angle), persistent=False)
         self.log_weights = _PointWeights(b)
@@ -87,13 +131,14 @@ class S2AttentionPool(nn.Module):
         assert features % heads == 0
         self.heads = heads
         self.query = nn.Parameter(torch.zeros(heads, 1, features // heads))
-        self.kv = nn.Linear(features, 2 * features)
+        self.kv = Linear(features, 2 * features)
         self.log_weights = _PointWeights(b)
 
     def forward(self, y):  # pylint: disable=W
         batch, points, features = y.shape
         k, v = self.kv(y).view(batch, points, 2, self.heads, features // self.heads).permute(2, 0, 3, 1, 4)
-        q = self.query.to(k.dtype).expand(batch, -1, -1, -1)
+        q = self.query.to(k.dtype)
+        q = _Expand.apply(q, batch) if _sums_of_its_own(k, q) else q.expand(batch, -1, -1, -1)
         return attention(q, k, v, key_bias=self.log_weights()).reshape(batch, features)
 
 

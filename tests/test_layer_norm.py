@@ -364,6 +364,52 @@ def test_some_gradients_only_and_empty_sizes(hip):
     assert s2cnn_amd.dropout_add_layer_norm(e, e, 0.5, 1)[0].shape == e.shape
 
 
+@pytest.mark.gpu
+@TYPES
+@pytest.mark.parametrize("shape", [(1, 1), (3, 2), (64, 63), (65, 64), (1000, 65), (1600, 192), (4097, 7), (100003, 20), (17, 3001), (2, 70001)], ids=lambda s: "%dx%d" % s)
+def test_column_sums(hip, shape, dtype):
+    """Sums over the rows, strided and contiguous; float32 whatever the type."""
+    from s2cnn_amd.layer_norm import column_sums
+    x = torch.randn(*shape, generator=torch.Generator().manual_seed(sum(shape))).to(dtype).cuda()
+    want, mag = x.cpu().double().sum(0), x.cpu().double().abs().sum(0)
+    for t in (x, x.t().contiguous().t(), x.view(1, *shape)):
+        got = column_sums(t)
+        _close(got, want, F32, "sums", mag)
+        assert torch.equal(got, column_sums(x))
+    assert (column_sums(x[:0]) == 0).all() and column_sums(x[:0]).shape == shape[1:]
+
+
+@pytest.mark.gpu
+def test_column_sums_replayed_from_a_graph(hip):
+    from s2cnn_amd.layer_norm import column_sums
+    x = torch.randn(1600, 192, device="cuda")
+    column_sums(x)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        static = column_sums(x)
+    for k in range(4):
+        x.mul_(1.0 + 0.1 * k)
+        want = column_sums(x)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(static, want)
+
+
+def test_column_sums_refused_without_a_gpu():
+    from s2cnn_amd import _hip
+    from s2cnn_amd.layer_norm import column_sums
+    lib, f = _hip.lib(), 0x1000
+    n = lib.s2cnn_column_sums_workspace(1600, 192, 0)
+    assert n > 0 and lib.s2cnn_column_sums_workspace(0, 192, 0) == 0 and lib.s2cnn_column_sums_workspace(4, 0, 0) == 0
+    call = lambda x=f, out=f, ws=f, size=n, rows=1600, features=192, dtype=0: lib.s2cnn_column_sums(x, out, ws, size, rows, features, dtype, None)
+    assert call(x=None) == -1 and call(out=None) == -1 and call(rows=0) == -1 and call(features=0) == -1 and call(dtype=3) == -1
+    assert call(x=f + 2) == -3 and call(out=f + 2) == -3 and call(size=n - 1) == -2 and call(ws=None) == -2 and call(ws=f + 8) == -2
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        column_sums(torch.zeros(2, 3))
+
+
 def test_refusals():
     z = torch.zeros
     for f in (lambda: s2cnn_amd.layer_norm(z(2, 0)), lambda: s2cnn_amd.layer_norm(z(())), lambda: s2cnn_amd.layer_norm(z(2, 3), z(4)),

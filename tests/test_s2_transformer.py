@@ -216,6 +216,98 @@ def test_step_replayed_from_a_graph(hip):
     assert max(abs(a - b) for a, b in zip(eager[3:], replayed)) < 1e-4 * abs(eager[0])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("cast", [False, True], ids=["", "autocast"])
+def test_linear_captured_with_its_gradients(hip, cast, dtype):
+    """nn.Linear outside of a capture; captured, the outputs and the gradients of the input and the weight are its own bit by bit, in every replay,
+    and the bias's is the sum of the gradient's rows: float32 sums, rounded to the type."""
+    from s2cnn_amd.soft.s2_transformer import Linear
+    gen = torch.Generator().manual_seed(8)
+    a, b = Linear(96, 192).to(dtype).cuda(), torch.nn.Linear(96, 192).to(dtype).cuda()
+    b.load_state_dict(a.state_dict())
+    x, g = (torch.randn(4, 400, n, generator=gen).to(dtype).cuda() for n in (96, 192))
+    x.requires_grad_()
+
+    def run(m):
+        with torch.autocast("cuda", dtype=torch.bfloat16, enabled=cast, cache_enabled=False):
+            y = m(x)
+        return (y, *torch.autograd.grad(y, [x, m.weight, m.bias], g.to(y.dtype)))
+
+    for m in (a, b):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            run(m)
+        torch.cuda.current_stream().wait_stream(side)
+    for u, v in zip(run(a), run(b)):
+        assert torch.equal(u, v)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        static = run(a)
+    unit = 2.0 ** -8 if cast or dtype == torch.bfloat16 else 2.0 ** -20
+    for k in range(4):
+        with torch.no_grad():
+            g.mul_(1.0 + 0.25 * k)
+        want = run(b)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for u, v in zip(static[:3], want):
+            assert torch.equal(u, v), k
+        assert static[3].dtype == want[3].dtype
+        assert _relative(static[3], g.to(static[0].dtype).double().sum((0, 1)).cpu()) <= unit, k
+
+
+@pytest.mark.gpu
+def test_replays_between_eager_steps(hip, monkeypatch):
+    """The captured training step, and a twin that makes the same steps eagerly between its replays (with synchronisations, and other work that
+    allocates and clears memory): losses, gradients and weights of each are the other's.  The twin sums its biases' gradients as captured work
+    does, so that all kernels are the same, sums in the same order."""
+    from s2cnn_amd.soft import s2_transformer
+    monkeypatch.setattr(s2_transformer, "_sums_of_its_own", lambda x, parameter: True)
+    x, y = harness.synthetic_batch("sphere_transformer", 4, "cuda:0")
+    loss_fn = harness.NETWORKS["sphere_transformer"][3]
+
+    def make():
+        torch.manual_seed(0)
+        model = harness.NETWORKS["sphere_transformer"][0]().cuda().train()
+        opt = torch.optim.SGD(model.parameters(), lr=0.02, momentum=0.9)
+
+        def step():
+            opt.zero_grad(set_to_none=True)
+            loss = loss_fn(model(x), y)
+            loss.backward()
+            opt.step()
+            return loss
+        return model, opt, step
+
+    (model, opt, step), (twin, _, twin_step) = make(), make()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            step(), twin_step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    opt.zero_grad(set_to_none=True)
+    with torch.cuda.graph(graph):
+        static = step()
+    for k in range(5):
+        want = twin_step()
+        torch.cuda.synchronize()
+        junk = [torch.randn(1 << 20, device="cuda").sum() for _ in range(4)] + [torch.zeros(777, device="cuda")]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.isfinite(j).all() for j in junk)
+        assert abs(float(static) - float(want)) <= 1e-6 * abs(float(want)), k
+        for (name, a), b in zip(model.named_parameters(), twin.parameters()):
+            assert _relative(a.grad, b.grad.double().cpu()) < 1e-5, (k, name)
+            assert _relative(a, b.double().cpu()) < 1e-5, (k, name)
+
+
 def test_refusals():
     with pytest.raises(AssertionError):
         s2cnn_amd.S2TransformerBlock(25, 3, 3)
