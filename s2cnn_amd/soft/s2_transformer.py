@@ -160,12 +160,13 @@ class S2Transformer(nn.Module):
         self.pool = S2AttentionPool(features, heads, b)
         self.register_buffer("drops", torch.zeros(1, dtype=torch.int64))
         high = (seed & 0xFFFFFFFF) << 32                                    # the count takes the low 32 bits
-        self.register_buffer("calls", torch.arange(2 * layers) + (high - (1 << 64) if high >> 63 else high), persistent=False)
+        self.base = high - (1 << 64) if high >> 63 else high                # no buffer: data-parallel jobs hand those of one rank to all
+        self.register_buffer("calls", torch.arange(2 * layers), persistent=False)
 
     def next_seeds(self):
         """The seeds of the dropouts of one pass in training, [2 layers]: others at each call."""
         self.drops.add_(1)
-        return self.drops * (2 * len(self.blocks)) + self.calls
+        return torch.add(self.calls, self.drops, alpha=2 * len(self.blocks)).add_(self.base)
 
     def forward(self, x, seeds=None):  # pylint: disable=W
         """seeds: from next_seeds, or None to count one pass on"""

@@ -180,6 +180,18 @@ def test_seeds_of_stacks():
     assert first(7) == first(7) and first(7) == first(7 + 2 ** 40)
 
 
+def test_seeds_of_ranks_whose_buffers_are_those_of_one():
+    """What a data-parallel job does before each pass: the buffers of rank 0 go to all ranks, which still drop other elements."""
+    ranks = [s2cnn_amd.S2Transformer(8, 2, 2, 2, dropout=0.1, seed=3 + rank) for rank in range(3)]
+    seen = []
+    for _ in range(4):
+        for model in ranks[1:]:
+            for a, b in zip(ranks[0].buffers(), model.buffers()):
+                b.copy_(a)
+        seen += [n for model in ranks for n in model.next_seeds().tolist()]
+    assert len(set(seen)) == len(seen) == 4 * 3 * 4
+
+
 @pytest.mark.gpu
 def test_stacks_of_one_network_drop_other_elements(hip):
     x = torch.randn(2, 24, 6, 6, generator=torch.Generator().manual_seed(2)).cuda()
