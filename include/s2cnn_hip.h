@@ -416,7 +416,7 @@ int s2cnn_so3_integrate_grad(const float *g, const float *w, float *gx, int b, l
  * h' = h / (heads / kv_heads), n = buckets[b,i,j].  A key takes no part where j >= lengths[b] or key_bias[b,j] = -inf (its k and
  * v are not used at all then), a pair where n is outside 0 .. n_buckets - 1.  A row without any key: out = 0, no gradients.
  * Types of q, k, v, table, out and all gradients: dtype; sums, the softmax and its gradient are float32, float32 products
- * have float32 errors.  Entries of q, k, v and gout that take part are finite (of an infinite one come NaN or infinities).  A tensor's vectors are contiguous, strides are those of (batch, head, vector) in entries.
+ * have float32 errors.  Entries of q, k, v and gout that take part are finite, float32 below 3.38e38 (of others come NaN or infinities).  A tensor's vectors are contiguous, strides are those of (batch, head, vector) in entries.
  * Optional pointers may be NULL: table and buckets (together; n_buckets 0), key_bias, lengths, stats and out_f32 (if no
  * backward pass follows); where n_k is 0 also k, v and buckets.  fwd reads q .. lengths and writes out, stats and out_f32; bwd reads those and gout and writes gq, and where not NULL gtable,
  * gk and gv (both or none).  Results do not depend on the order of execution.
@@ -451,8 +451,8 @@ int s2cnn_attention_fwd(const s2cnn_attention_t *a, void *workspace, size_t work
 int s2cnn_attention_bwd(const s2cnn_attention_t *a, void *workspace, size_t workspace_bytes, void *stream);
 
 /* ---- layer normalisation, dropout, and both with a residual ---------------------------------
- * Rows of `features` entries, dense; types by dtype (S2CNN_F32, ...), sums in float32; weight and bias of the same type, or NULL.
- * dropout : y[i] = 0 where u(i) < T, else x[i] 65536 / (65536 - T), T = round(65536 p), 0 <= p < 1; u(i) = 16 bits of
+ * Rows of `features` < 2^24 entries, fewer than 2^31 of them (dropout: fewer than 2^40 elements), dense; types by dtype (S2CNN_F32, ...), sums in float32; weight and bias of the same type, or NULL.
+ * dropout : y[i] = 0 where u(i) < T, else x[i] 65536 / (65536 - T), T = min(65535, round(65536 p)), 0 <= p < 1; u(i) = 16 bits of
  *           Philox4x32-10 of counter i / 8 and key seed: half i % 2 of word (i % 8) / 2, i the index in the dense tensor.  The gradient is
  *           the same map.  seed_at: device memory that holds the seed instead, or NULL.
  * fwd     : y = (h - mean) rstd weight + bias per row, rstd = 1 / sqrt(variance + eps), variance = mean of (h - mean)^2;

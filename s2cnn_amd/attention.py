@@ -116,7 +116,7 @@ def attention(q, k, v, table=None, buckets=None, key_bias=None, lengths=None, sc
     :param k, v: [batch, kv_heads, n_k, d], kv_heads dividing heads: head h reads the keys of h // (heads // kv_heads)
     :param table: [heads, n_buckets], n_buckets <= 64, the type of q: the learned bias; with buckets, and at most 128 heads a key head
     :param buckets: [n_q, n_k] or [batch, n_q, n_k] int8: the bucket of every pair.  A number outside 0 .. n_buckets - 1
-        excludes the pair; what k and v hold there has still to be finite, as 0 * inf is not 0
+        excludes the pair; what k and v hold there has still to be finite (see below), as 0 * inf is not 0
     :param key_bias: [n_k] or [batch, n_k] float32, not differentiated: logarithms of quadrature weights, or -inf for a key
         that takes no part (its k and v are not used at all)
     :param lengths: [batch] int32: keys from lengths[b] on take no part
@@ -127,7 +127,7 @@ def attention(q, k, v, table=None, buckets=None, key_bias=None, lengths=None, sc
     are rounded, and before them nothing to less than 16 bits (float16: 22): probabilities and their gradients, as two parts.  The backward pass
     recomputes the probabilities.  Results do not depend on the order of execution.
 
-    What takes part has to be finite.  Of an infinite entry of v or q, and of k in float32, come NaN (or an infinity) in all that depends on it,
+    What takes part has to be finite, in float32 below 3.38e38.  Of an infinite entry of v or q, and of k in float32, come NaN (or an infinity) in all that depends on it,
     where the formula may have an infinity, or no weight for that key: products are of parts of the operands, and an infinity has none.  A table's
     entry or a key bias may be -inf; those of the type's lowest value leave no weight beside others, and even weights among themselves.
     """

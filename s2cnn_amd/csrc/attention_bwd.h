@@ -8,11 +8,11 @@
 // runs over the queries of all heads that share them (dk, dv).  The price is that both form x and dp: seven products instead
 // of five; storing ds would cost 2 n_q n_k floats of traffic per head, more time than two products.
 //
-// What bounds them, and what they measured.  float32, 4 signals, 8 heads, 4096 points, D = 64: dq 1.24 ms (166 TFLOP/s of float32 products),
-// dk and dv 1.47 ms (187): matrix and vector instructions together take nine tenths of a SIMD's time, and a third of a tile's step goes into
-// staging its rows.  bfloat16, 16 signals, 8 heads on 2, 1024 points, those within a radian: 134 and 142 us, vector instructions 0.40 and 0.35 of
-// the time, matrix ones 0.12 and 0.15, the rest the latency of a tile's steps with two or three waves a SIMD.  float32, 32 signals, 5 heads,
-// 400 points of 20 entries: 65 and 73 us.
+// What bounds them, and what they measured.  float32, 4 signals, 8 heads, 4096 points, D = 64: dq 1.17 ms (176 TFLOP/s of float32 products),
+// dk and dv 1.42 ms (193): matrix and vector instructions together take nine tenths of a SIMD's time, and a third of a tile's step goes into
+// staging its rows.  bfloat16, 16 signals, 8 heads on 2, 1024 points, those within a radian: 125 and 132 us, vector instructions 0.40 and 0.38 of
+// the time, matrix ones 0.11 and 0.16, the rest the latency of a tile's steps with two or three waves a SIMD.  float32, 32 signals, 5 heads,
+// 400 points of 20 entries: 62 and 72 us.
 #pragma once
 #include "attention.h"
 
@@ -284,8 +284,8 @@ template <class T> __global__ __launch_bounds__(256) void sum_table_kernel(Args 
 // ---- dk, dv ---------------------------------------------------------------------------------------------------------
 // Columns: keys of one key head.  Rows: the queries of its heads, tile by tile, head by head.
 constexpr int BUCKET_LD = 9;
-// One tile in LDS, not two, for float32 at D = 32: so three workgroups fit a CU (79 us against 92 with two, at the size above), although 24
-// registers are spilled for it.  For the 16-bit types at 64 the third costs 38, and 189 us against 156; at 128 the second costs 29, and is
+// One tile in LDS, not two, for float32 at D = 32: so three workgroups fit a CU (79 us against 92 with two, at the size above), although 22
+// registers are spilled for it.  For the 16-bit types at 64 the third costs 38, and 189 us against 156; at 128 the second costs 36, and is
 // worth it (322 us against 409, 4 signals, 8 heads, 2048 points of 100).
 template <class T> constexpr int row_arrays = T::PARTS == 3 ? 3 : 4;      // numbers of a row in LDS
 template <class T, int D, int W> constexpr int kv_buffers() { return T::PARTS * D == 96 ? 1 : buffers<T, D, W>(4); }

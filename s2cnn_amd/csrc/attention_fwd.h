@@ -5,11 +5,11 @@
 // values.  The columns run over all queries of the heads that share a key head, so that a single query of 8 heads reads its
 // keys once; few columns and many keys: the keys are split over workgroups, and a second kernel joins their results.
 //
-// What bounds it, and what it measured.  float32, 4 signals, 8 heads, 4096 points, D = 64: 0.84 ms, 164 TFLOP/s of float32 products (980 of
-// bf16 ones; a library product of 8192^3 reaches 1238): matrix and vector instructions take 0.45 and 0.51 of a SIMD's time, and of the vector
-// ones a third cut the staged rows into parts.  bfloat16, 16 signals, 8 heads on 2, 1024 points, those within a radian, D = 64: 82 us,
+// What bounds it, and what it measured.  float32, 4 signals, 8 heads, 4096 points, D = 64: 0.79 ms, 174 TFLOP/s of float32 products (1046 of
+// bf16 ones; a library product of 8192^3 reaches 1238): matrix and vector instructions take 0.44 and 0.50 of a SIMD's time, and of the vector
+// ones a third cut the staged rows into parts.  bfloat16, 16 signals, 8 heads on 2, 1024 points, those within a radian, D = 64: 77 us,
 // bound by vector instructions (half of the SIMDs' time; matrix instructions 0.14) and the latency of a tile's steps.  One query a
-// head, float32, 8 signals, 8 heads on 2, 32768 keys of 50: 55 us and 6 for the join, 3.8 TB/s of keys and values.  A kernel of one tile
+// head, float32, 8 signals, 8 heads on 2, 32768 keys of 50: 60 us and 6 for the join, 3.5 TB/s of keys and values.  A kernel of one tile
 // takes 8.5 us: the launch and one trip to memory after another.
 #pragma once
 #include "attention.h"
@@ -17,8 +17,8 @@
 namespace s2cnn {
 namespace attn {
 
-// Workgroups of four waves a CU: four for the 16-bit types up to D = 64 (127 registers, none spilled), three for float32 at 64 (4 spilled; 868 us
-// against 906 with two, 4 signals, 8 heads, 4096 points, on one card), two for the others; float32 at 32 takes 136 and gets three.  Three for the
+// Workgroups of four waves a CU: four for the 16-bit types up to D = 64 (128 registers, none spilled), three for float32 at 64 (4 spilled; 868 us
+// against 906 with two, 4 signals, 8 heads, 4096 points, on one card), two for the others; float32 at 32 takes 128 and gets four.  Three for the
 // 16-bit types at 128 cost 14 registers, and 135 us against 101 (7 sets of 1009 queries and up to 2501 keys, 6 heads of 100); one for
 // float32 at 128 leaves more registers, and takes 537 us against 397 (4 signals, 8 heads, 2048 points of 100).
 template <class T, int D, int W> __global__ __launch_bounds__(64 * W, T::PARTS * D == 192 && W > 1 ? 3 : W == 1 || T::PARTS * D > 64 ? 2 : 4) void forward_kernel(Args p) {

@@ -71,7 +71,7 @@ def dropout(x, p, seed):
     in training), differentiable.
 
     :param x: float32, bfloat16 or float16, any shape
-    :param p: in [0, 1), taken to the nearest multiple of 2^-16
+    :param p: in [0, 1), taken to the nearest multiple of 2^-16 below one
     :param seed: an int, or an int64 tensor of one element on the GPU that is read when the kernel runs (so that a captured
         graph drops others at each replay).  Equal seeds and sizes drop equal elements: give each call of a step its own
     :return y: contiguous; element i of it depends on seed and i alone (include/s2cnn_hip.h has the generator)
