@@ -451,7 +451,8 @@ int s2cnn_attention_fwd(const s2cnn_attention_t *a, void *workspace, size_t work
 int s2cnn_attention_bwd(const s2cnn_attention_t *a, void *workspace, size_t workspace_bytes, void *stream);
 
 /* ---- layer normalisation, dropout, and both with a residual ---------------------------------
- * Rows of `features` < 2^24 entries, fewer than 2^31 of them (dropout: fewer than 2^40 elements), dense; types by dtype (S2CNN_F32, ...), sums in float32; weight and bias of the same type, or NULL.
+ * Rows of `features` < 2^24 entries, fewer than 2^31 of them (dropout: fewer than 2^40 elements), dense; types by dtype (S2CNN_F32, ...), sums
+ * in float32; weight and bias of the same type, or NULL.
  * dropout : y[i] = 0 where u(i) < T, else x[i] 65536 / (65536 - T), T = min(65535, round(65536 p)), 0 <= p < 1; u(i) = 16 bits of
  *           Philox4x32-10 of counter i / 8 and key seed: half i % 2 of word (i % 8) / 2, i the index in the dense tensor.  The gradient is
  *           the same map.  seed_at: device memory that holds the seed instead, or NULL.

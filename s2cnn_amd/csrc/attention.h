@@ -211,8 +211,8 @@ __device__ __forceinline__ unsigned load_word_at(const signed char* uniform, uns
 template <class T> __device__ __forceinline__ Quad load_quad(const typename T::type* p, int q, int d) {
   Quad v = load_four<T>(p + quad_at(q, d));
   // So many of its first entries count as zero.  A column's quads each have their own number and four conditions on it, which the
-  // compiler must not share between the vectors of a column (hundreds of scalar registers, and spills of them that went with wrong results; the build refuses those):
-  // the empty statement hides that the numbers are equal.
+  // compiler must not share between the vectors of a column (hundreds of scalar registers, and spills of them that went with wrong
+  // results; the build refuses those): the empty statement hides that the numbers are equal.
   int twice = 4 * q < d ? 4 * q - quad_at(q, d) : 4;
   asm volatile("" : "+v"(twice));
   if constexpr (T::PARTS == 3) {
@@ -494,8 +494,9 @@ template <class T, int D, int THREADS, int LA, int LB, bool SCALE = false> struc
 //
 // The product starts from the biases instead of zero: x = c (q.k + bias / c), c = log2(e) |scale|; float32 takes c into the queries as
 // they are loaded, and needs no factor; the other types take the sign.  All kernels form a score from the same numbers in the same order: the
-// references are of scores as the forward pass had them, and a score of a thousand that is rounded otherwise makes another probability.  Biases of keys and entries of the table are held within +-1.5e38 of a score, so that
-// the type's lowest value stays finite, and the sum of two: keys that all have it share a row evenly.
+// references are of scores as the forward pass had them, and a score of 10^4 that is rounded otherwise makes another probability.  Biases of
+// keys and entries of the table are held within +-1.5e38 of a score, so that the type's lowest value stays finite, and the sum of two: keys
+// that all have it share a row evenly.
 // In two steps, the load and what is made of it: the tiles' loads are under way in between, and a wait for this one, issued before them,
 // is no wait for them.
 __device__ __forceinline__ float load_key_bias(const float* key_bias, int key, int end) { return key_bias ? key_bias[max(min(key, end - 1), 0)] : 0.f; }
