@@ -13,7 +13,8 @@
 // The two sums over the rows are kept in registers by the groups, which run over many rows each, joined per workgroup in LDS,
 // and a second kernel adds the workgroups' sums in a fixed order.  The backward pass reads h, which is rounded to the tensors' type; in the
 // step with a residual what the rounding left goes along in 8 bits an entry (16-bit types).  Without it the weights' gradient had that rounding
-// beside its own, 1.41 times the error; x and the residual once more instead of h would be twice the traffic.
+// beside its own, 1.41 times the error; x and the residual once more instead of h would be twice the traffic.  The error of a normalised entry in
+// the backward pass is then 2^-16 (float16: 2^-19) of |h| over the row's deviation: below the rounding of the results up to offsets of 100 deviations.
 //
 // Measured, with a copy of 1 GiB at 5.1 TB/s: 65536 rows of 1024 in bfloat16: forward 58 us, 4.6 TB/s, backward 82 us, 4.9 TB/s; the step
 // with a residual and dropout, 16384 rows of 512: 20 us, 3.8 TB/s, and 25 us, 3.7 TB/s (tensors of 17 MB: a third of the time is launch and
