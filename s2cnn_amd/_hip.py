@@ -34,6 +34,20 @@ class Attention(ctypes.Structure):
 
 _ATTENTION_P = ctypes.POINTER(Attention)
 
+
+class RotarySide(ctypes.Structure):
+    """s2cnn_rotary_side_t"""
+    _fields_ = [(n, _vp) for n in ("x", "weight", "g", "y", "gweight")] + [(n, _long * 3) for n in ("x_stride", "g_stride", "y_stride")] + [("heads", _int)]
+
+
+class Rotary(ctypes.Structure):
+    """s2cnn_rotary_t"""
+    _fields_ = ([("side", RotarySide * 2), ("table", _vp), ("index", _vp), ("table_stride", _long), ("index_stride", _long)]
+                + [(n, _int) for n in ("batch", "n", "d", "pairs", "rows", "norm", "interleaved", "dtype")] + [("eps", _float)])
+
+
+_ROTARY_P = ctypes.POINTER(Rotary)
+
 SIGNATURES = {
     "s2cnn_abi_version": (_int, []),
     "s2cnn_strerror": (ctypes.c_char_p, [_int]),
@@ -107,6 +121,10 @@ SIGNATURES = {
     "s2cnn_column_sums_workspace": (_size_t, [_long, _long, _int]),
     "s2cnn_column_sums": (_int, [_vp, _vp, _vp, _size_t, _long, _long, _int, _vp]),
     "s2cnn_dropout": (_int, [_vp, _vp, _long, ctypes.c_double, ctypes.c_ulonglong, _vp, _int, _vp]),
+    "s2cnn_rotary_fwd": (_int, [_ROTARY_P, _vp]),
+    "s2cnn_rotary_workspace": (_size_t, [_ROTARY_P]),
+    "s2cnn_rotary_bwd": (_int, [_ROTARY_P, _vp, _size_t, _vp]),
+    "s2cnn_rotary_table": (_int, [_vp, _int, _vp, _vp, _long, _int, _int, _float, _vp]),
     "s2cnn_so3_integrate_grad": (_int, [_c_float_p, _c_float_p, _c_float_p, _int, _long, _vp]),
 }
 

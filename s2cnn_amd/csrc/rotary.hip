@@ -1,0 +1,472 @@
+// Rotation of queries and keys by position, alone or after a normalisation of every head's vectors, forward and backward, and the table of
+// the rotations.
+//
+//   forward    y = R (w x r),  r = 1 / sqrt(mean(x^2) + eps)     (without the normalisation: y = R x)
+//   backward   g = R^T gy, u = g w, gx = r (u - xh mean(u xh)) with xh = x r, gw = sum of g xh over all vectors
+//
+// R turns pair j of a vector's entries by the angle of row n of the table: (a, b) -> (a cos - b sin, a sin + b cos).  Pairs are neighbours (2j,
+// 2j + 1), or halves apart (j, pairs + j); entries from 2 pairs on stay.  R^T is the same with -sin.
+//
+// All of it is bound by memory: x (and gy) read once, y (or gx) written once, the rest in registers; r is formed again in the backward pass from x, which
+// it reads anyway.  A vector belongs to a group of L lanes (a power of two).  A lane holds two chunks of 16 bytes, so that both entries of a pair
+// are its own: no exchange between lanes but the sums over a vector.  Where a chunk would run past the end of its part, it begins earlier and
+// overlaps the one before (both lanes form the same numbers; sums count them once), so that all accesses are 16 bytes wide, at any alignment; only
+// parts shorter than a chunk are loaded entry by entry.
+#include "chunk.h"
+
+namespace s2cnn {
+namespace rotary {
+
+constexpr int THREADS = 256;
+constexpr int MAX_D = 256;
+
+// x / divisor for 0 <= x < 2^31 by a product: (mulhi(x, magic) + x) >> shift
+struct Divider {
+  unsigned magic, shift, divisor;
+};
+inline Divider divider(long n) {
+  unsigned s = 0;
+  while ((1L << s) < n) ++s;
+  return {(unsigned)((((1UL << s) - (unsigned long)n) << 32) / (unsigned long)n + 1), s, (unsigned)n};
+}
+__device__ __forceinline__ unsigned divide(unsigned x, const Divider& d, unsigned& rest) {
+  const unsigned q = (__umulhi(x, d.magic) + x) >> d.shift;
+  rest = x - q * d.divisor;
+  return q;
+}
+
+struct Tensor {                  // vectors of a tensor: entries between those of consecutive inner, middle and outer numbers
+  const void* at;
+  long inner, middle, outer;
+};
+struct Side {                    // queries, or keys
+  Tensor x, g;
+  void* y;
+  long y_inner, y_middle, y_outer;
+  const void* weight;
+  float* partial;                // [workgroups, d]
+  Divider inner, middle;
+  unsigned vectors;
+  int heads_inside;              // the inner number is the head (else the place)
+};
+struct Args {
+  Side side[2];
+  unsigned blocks0;              // workgroups of side 0
+  const float2* table;
+  const int* index;
+  long table_stride, index_stride;      // of the batch
+  int rows, d, pairs, units, lanes;
+  float eps, sign;
+};
+
+// The part of a vector that a lane holds.
+struct Part {
+  int a, b, na, nb;              // first entries and numbers of entries of its two chunks
+  int skip_a, skip_b;            // leading entries that belong to another lane as well
+  int pair;                      // the pair of the first entry
+};
+template <int V, bool NEIGHBOURS> __device__ __forceinline__ Part part_of(int u, int units, int d, int pairs) {
+  Part p = {0, 0, 0, 0, 0, 0, pairs};
+  if (u >= units) return p;
+  int first, length;                                               // a run of entries that is cut into two chunks a lane
+  if (!NEIGHBOURS && u < (pairs + V - 1) / V) {
+    p.pair = pairs >= V ? min(u * V, pairs - V) : 0;
+    p.a = p.pair, p.b = pairs + p.pair;
+    p.na = p.nb = min(pairs, V);
+    p.skip_a = p.skip_b = u * V - p.pair;
+    return p;
+  }
+  if (NEIGHBOURS) {
+    first = 0, length = d & ~1;
+    if (u >= (length + 2 * V - 1) / (2 * V)) first = length, length = 1, u = 0;
+  } else {
+    first = 2 * pairs, length = d - first, u -= (pairs + V - 1) / V;
+  }
+  const int at = length >= 2 * V ? min(u * 2 * V, length - 2 * V) : 0, skip = u * 2 * V - at;
+  p.a = first + at, p.b = p.a + V;
+  p.na = min(length, V), p.nb = min(length - p.na, V);
+  p.skip_a = min(skip, V), p.skip_b = skip - p.skip_a;
+  if (NEIGHBOURS) p.pair = p.a / 2;
+  return p;
+}
+// A copy that the compiler takes for new: what is compared with it in a loop is compared there, and not kept as dozens of lane masks across it,
+// for which there are not enough scalar registers.
+__device__ __forceinline__ int fresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+inline int units_of(int V, int d, int pairs, bool neighbours) {
+  if (neighbours) return ((d & ~1) + 2 * V - 1) / (2 * V) + (d & 1);
+  return (pairs + V - 1) / V + (d - 2 * pairs + 2 * V - 1) / (2 * V);
+}
+
+// The first n entries at p, the others zero: 16 bytes, or entry by entry.
+template <class T> __device__ __forceinline__ void load(const T* p, int n, float (&v)[Chunk<T>::N]) {
+  constexpr int N = Chunk<T>::N;
+  if (n == N) {
+    Chunk<T>::get(load_chunk<T>(p, N), v);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = i < n ? (float)p[i] : 0.f;
+}
+
+// cos and sin of V pairs from `pair` on of a row; of pairs that do not turn 1 and 0, of a row that is not there NaN
+template <int V> __device__ __forceinline__ void load_turns(const Args& p, const float2* row, bool there, int pair, float (&c)[V], float (&s)[V]) {
+  if (there && pair + V <= p.pairs) {
+    typedef float loose __attribute__((ext_vector_type(4), aligned(8)));
+    const loose* const at = reinterpret_cast<const loose*>(row + pair);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      const loose t = at[i];
+      c[2 * i] = t[0], s[2 * i] = t[1] * p.sign, c[2 * i + 1] = t[2], s[2 * i + 1] = t[3] * p.sign;
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    float2 t = make_float2(1.f, 0.f);
+    if (pair + i < p.pairs) t = there ? row[pair + i] : make_float2(__builtin_nanf(""), __builtin_nanf(""));
+    c[i] = t.x, s[i] = t.y * p.sign;
+  }
+}
+
+template <int V, bool NEIGHBOURS> __device__ __forceinline__ void turn(const float (&c)[V], const float (&s)[V], float (&a)[V], float (&b)[V]) {
+  if constexpr (NEIGHBOURS) {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      const float x = a[2 * i], y = a[2 * i + 1], z = b[2 * i], w = b[2 * i + 1];
+      a[2 * i] = x * c[i] - y * s[i], a[2 * i + 1] = x * s[i] + y * c[i];
+      b[2 * i] = z * c[V / 2 + i] - w * s[V / 2 + i], b[2 * i + 1] = z * s[V / 2 + i] + w * c[V / 2 + i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float x = a[i], y = b[i];
+      a[i] = x * c[i] - y * s[i], b[i] = x * s[i] + y * c[i];
+    }
+  }
+}
+
+__device__ __forceinline__ float sum_of(float v, int lanes) {           // over a group, `lanes` the same in all of the launch
+  if (lanes > 1) v = add_dpp<0xB1>(v);
+  if (lanes > 2) v = add_dpp<0x4E>(v);
+  if (lanes > 4) v = add_dpp<0x141>(v);
+  if (lanes > 8) v = add_dpp<0x140>(v);
+  if (lanes > 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  if (lanes > 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  return v;
+}
+
+// sum over the entries of a lane that are its own of x y
+template <int V> __device__ __forceinline__ float dot(const Part& p, const float (&xa)[V], const float (&xb)[V], const float (&ya)[V], const float (&yb)[V]) {
+  float t = 0.f;
+  if (p.skip_a == 0 && p.skip_b == 0) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) t = fmaf(xa[i], ya[i], fmaf(xb[i], yb[i], t));
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if (i >= p.skip_a) t = fmaf(xa[i], ya[i], t);
+      if (i >= p.skip_b) t = fmaf(xb[i], yb[i], t);
+    }
+  }
+  return t;
+}
+
+enum Pass { TURN, NORM, NORM_BACK };           // TURN: both directions of the rotation alone
+
+template <class T, Pass PASS, bool NEIGHBOURS> __global__ __launch_bounds__(THREADS) void rotary_kernel(Args p) {
+  constexpr int V = Chunk<T>::N;
+  const bool second = blockIdx.x >= p.blocks0;
+  const Side& s = p.side[second];
+  const unsigned block = second ? blockIdx.x - p.blocks0 : blockIdx.x, blocks = second ? gridDim.x - p.blocks0 : p.blocks0;
+  const int lane = threadIdx.x & (p.lanes - 1);
+  const unsigned groups = (unsigned)(THREADS / p.lanes);
+  const Part kept = part_of<V, NEIGHBOURS>(lane, p.units, p.d, p.pairs);
+  const float inv_d = 1.f / (float)p.d;
+  float wa[V], wb[V], ga[V] = {}, gb[V] = {};                     // weights; sums of their gradients
+  if (PASS != TURN) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) wa[i] = wb[i] = 1.f;
+    if (s.weight) {
+      load<T>(static_cast<const T*>(s.weight) + kept.a, kept.na, wa);
+      load<T>(static_cast<const T*>(s.weight) + kept.b, kept.nb, wb);
+    }
+  }
+  // every group of the launch takes as many turns, so that no lane is missing from a sum
+  for (unsigned first = block * groups; first < s.vectors; first += blocks * groups) {
+    const unsigned mine = first + threadIdx.x / p.lanes, item = min(mine, s.vectors - 1);
+    const Part part = {kept.a, kept.b, fresh(kept.na), fresh(kept.nb), fresh(kept.skip_a), fresh(kept.skip_b), fresh(kept.pair)};
+    unsigned inner, middle;
+    const unsigned outer = divide(divide(item, s.inner, inner), s.middle, middle);
+    const unsigned place = s.heads_inside ? middle : inner;
+    int row = (int)place;
+    if (p.index) row = p.index[outer * p.index_stride + place];
+    const bool there = row < p.rows;
+    float c[V], sn[V];
+    // a row below zero: the vector is not turned
+    load_turns<V>(p, p.table + outer * p.table_stride + (long)row * p.pairs, there, p.pairs == 0 || row < 0 ? p.pairs : part.pair, c, sn);
+    const auto at = [&](const Tensor& t) { return static_cast<const T*>(t.at) + ((long)outer * t.outer + (long)middle * t.middle + (long)inner * t.inner); };
+    float a[V], b[V];
+    if constexpr (PASS != NORM_BACK) {
+      const T* const x = at(s.x);
+      load<T>(x + part.a, part.na, a);
+      load<T>(x + part.b, part.nb, b);
+      if constexpr (PASS == NORM) {
+        const float r = rsqrtf(fmaf(sum_of(dot<V>(part, a, b, a, b), p.lanes), inv_d, p.eps));
+#pragma unroll
+        for (int i = 0; i < V; ++i) a[i] = a[i] * r * wa[i], b[i] = b[i] * r * wb[i];
+      }
+      turn<V, NEIGHBOURS>(c, sn, a, b);
+    } else {
+      const T* const x = at(s.x);
+      const T* const g = at(s.g);
+      float xa[V], xb[V];
+      load<T>(x + part.a, part.na, xa);
+      load<T>(x + part.b, part.nb, xb);
+      load<T>(g + part.a, part.na, a);
+      load<T>(g + part.b, part.nb, b);
+      turn<V, NEIGHBOURS>(c, sn, a, b);
+      const float r = rsqrtf(fmaf(sum_of(dot<V>(part, xa, xb, xa, xb), p.lanes), inv_d, p.eps));
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        xa[i] *= r, xb[i] *= r;
+        if (mine < s.vectors) ga[i] = fmaf(a[i], xa[i], ga[i]), gb[i] = fmaf(b[i], xb[i], gb[i]);
+        a[i] *= wa[i], b[i] *= wb[i];
+      }
+      const float m = sum_of(dot<V>(part, a, b, xa, xb), p.lanes) * inv_d;
+#pragma unroll
+      for (int i = 0; i < V; ++i) a[i] = r * fmaf(-xa[i], m, a[i]), b[i] = r * fmaf(-xb[i], m, b[i]);
+    }
+    if (mine < s.vectors) {
+      T* const y = static_cast<T*>(s.y) + ((long)outer * s.y_outer + (long)middle * s.y_middle + (long)inner * s.y_inner);
+      store_chunk<T>(y + part.a, part.na, a);
+      store_chunk<T>(y + part.b, part.nb, b);
+    }
+  }
+  if constexpr (PASS == NORM_BACK) {
+    if (!s.partial) return;
+    __shared__ float joined[THREADS / 64][64][2 * V + 1];
+    for (int m = p.lanes; m < 64; m <<= 1)                         // groups of a wave
+#pragma unroll
+      for (int i = 0; i < V; ++i) ga[i] += __shfl_xor(ga[i], m), gb[i] += __shfl_xor(gb[i], m);
+    if ((threadIdx.x & 63) < (unsigned)p.lanes)
+#pragma unroll
+      for (int i = 0; i < V; ++i) joined[threadIdx.x >> 6][lane][i] = ga[i], joined[threadIdx.x >> 6][lane][V + i] = gb[i];
+    __syncthreads();
+    if (threadIdx.x < (unsigned)p.lanes) {
+      float* const out = s.partial + (long)block * p.d;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const auto sum = [&](int k) { return (joined[0][lane][k] + joined[1][lane][k]) + (joined[2][lane][k] + joined[3][lane][k]); };
+        if (i >= kept.skip_a && i < kept.na) out[kept.a + i] = sum(i);
+        if (i >= kept.skip_b && i < kept.nb) out[kept.b + i] = sum(V + i);
+      }
+    }
+  }
+}
+
+// The workgroups' sums of the weights' gradients, in a fixed order: 32 entries a workgroup, 32 groups of lanes over the workgroups.
+template <class T> __global__ __launch_bounds__(1024) void weights_kernel(const float* partial0, const float* partial1, unsigned blocks0, unsigned blocks1, int d, T* out0,
+                                                                       T* out1) {
+  __shared__ float sums[32][33];
+  const float* const partial = blockIdx.y ? partial1 : partial0;
+  T* const out = blockIdx.y ? out1 : out0;
+  const unsigned blocks = blockIdx.y ? blocks1 : blocks0;
+  if (!out) return;
+  const int i = threadIdx.x & 31, s = threadIdx.x >> 5, col = blockIdx.x * 32 + i;
+  float t = 0.f;
+  if (col < d)
+    for (unsigned k = s; k < blocks; k += 32) t += partial[(long)k * d + col];
+  sums[s][i] = t;
+  __syncthreads();
+  t = sum_lanes<32>(sums[i][s]);
+  if (i == 0 && (int)blockIdx.x * 32 + s < d) out[blockIdx.x * 32 + s] = (T)t;
+}
+
+// ---- the table ------------------------------------------------------------------------------------------------------
+// An angle is formed in turns and in 64 bits, and what is left of it after the next quarter of a turn in 32: positions of a million lose nothing.
+// A thread keeps its pair and takes one row after the other, THREADS / pairs of them side by side.
+template <class P> __global__ __launch_bounds__(THREADS) void table_kernel(const P* positions, const double* frequencies, float2* table, long n, int axes, int pairs,
+                                                                       float scale) {
+  const int side = THREADS / pairs, r = threadIdx.x / pairs, j = threadIdx.x - r * pairs;
+  if (r >= side) return;
+  const double f0 = frequencies[j] * 0.15915494309189533577;
+  for (long row = (long)blockIdx.x * side + r; row < n; row += (long)gridDim.x * side) {
+    double turns = (double)positions[row * axes] * f0;
+    for (int a = 1; a < axes; ++a) turns = fma((double)positions[row * axes + a] * 0.15915494309189533577, frequencies[a * pairs + j], turns);
+    const double quarters = rint(4.0 * turns);
+    const float rest = (float)(4.0 * turns - quarters);                    // of a quarter, -1/2 .. 1/2
+    float s, c;
+    sincospif(0.5f * rest, &s, &c);
+    const int q = (int)(quarters - 4.0 * floor(0.25 * quarters));
+    const float cos = q & 1 ? s : c, sin = q & 1 ? c : s;
+    table[row * pairs + j] = make_float2((q == 1 || q == 2 ? -cos : cos) * scale, (q >= 2 ? -sin : sin) * scale);
+  }
+}
+
+// ---- launches -------------------------------------------------------------------------------------------------------
+constexpr int CUS = 256;
+
+struct Plan {
+  int units, lanes;
+  unsigned vectors[2], blocks[2];
+};
+
+bool sizes_ok(const s2cnn_rotary_t* a) {
+  if (!a || (a->dtype != S2CNN_F32 && a->dtype != S2CNN_BF16 && a->dtype != S2CNN_F16)) return false;
+  if (a->batch < 1 || a->n < 1 || a->d < 1 || a->d > MAX_D || a->pairs < 0 || 2 * a->pairs > a->d) return false;
+  if (a->pairs && (!a->table || a->rows < 1 || (!a->index && a->rows < a->n))) return false;
+  if (!a->pairs && (a->table || a->index)) return false;
+  if (a->side[0].heads < 1 || a->side[1].heads < 0 || (a->norm && !(a->eps > 0.f))) return false;
+  const long limit = 1L << 31;
+  for (const s2cnn_rotary_side_t& s : a->side)
+    if ((long)a->batch * a->n >= limit || (s.heads && (long)a->batch * a->n >= limit / s.heads)) return false;
+  return true;
+}
+
+// Workgroups: eight a CU for the loads and stores that are to be under way; four where their sums of the weights' gradients are read again.
+Plan plan_of(const s2cnn_rotary_t& a, bool sums) {
+  Plan p;
+  p.units = units_of(a.dtype == S2CNN_F32 ? 4 : 8, a.d, a.pairs, a.interleaved != 0);
+  for (p.lanes = 1; p.lanes < p.units;) p.lanes *= 2;
+  const long groups = THREADS / p.lanes, most = CUS * (sums ? 4 : 8);
+  long total = 0;
+  for (int i = 0; i < 2; ++i) total += (long)a.batch * a.n * a.side[i].heads;
+  for (int i = 0; i < 2; ++i) {
+    const long vectors = (long)a.batch * a.n * a.side[i].heads, need = (vectors + groups - 1) / groups;
+    const long share = (long)((double)most * vectors / total);
+    p.vectors[i] = (unsigned)vectors;
+    p.blocks[i] = (unsigned)(need < most ? need : share < 1 ? 1 : share);
+    if (!vectors) p.blocks[i] = 0;
+  }
+  return p;
+}
+
+Args args_of(const s2cnn_rotary_t& a, const Plan& p, bool backward, float* partial) {
+  Args k = {};
+  for (int i = 0; i < 2; ++i) {
+    const s2cnn_rotary_side_t& from = a.side[i];
+    Side& s = k.side[i];
+    s.vectors = p.vectors[i];
+    if (!from.heads) continue;
+    // neighbouring groups take vectors that lie next to each other
+    s.heads_inside = a.n == 1 || (from.heads > 1 && (backward && !a.norm ? from.g_stride : from.x_stride)[1] <= (backward && !a.norm ? from.g_stride : from.x_stride)[2]);
+    s.inner = divider(s.heads_inside ? from.heads : a.n);
+    s.middle = divider(s.heads_inside ? a.n : from.heads);
+    const int in = s.heads_inside ? 1 : 2, mid = s.heads_inside ? 2 : 1;
+    const auto tensor = [&](const void* at, const long* stride) { return Tensor{at, stride[in], stride[mid], stride[0]}; };
+    s.x = tensor(from.x, from.x_stride);
+    s.g = tensor(from.g, from.g_stride);
+    if (backward && !a.norm) s.x = s.g;
+    s.y = from.y;
+    s.y_inner = from.y_stride[in], s.y_middle = from.y_stride[mid], s.y_outer = from.y_stride[0];
+    s.weight = a.norm ? from.weight : nullptr;
+    if (backward && from.gweight) s.partial = partial + (i ? (long)p.blocks[0] * a.d : 0);
+  }
+  k.blocks0 = p.blocks[0];
+  k.table = reinterpret_cast<const float2*>(a.table);
+  k.index = a.index;
+  k.table_stride = a.table_stride / 2;
+  k.index_stride = a.index_stride;
+  k.rows = a.rows, k.d = a.d, k.pairs = a.pairs, k.units = p.units, k.lanes = p.lanes;
+  k.eps = a.eps;
+  k.sign = backward ? -1.f : 1.f;
+  return k;
+}
+
+template <class T, bool NEIGHBOURS> void launch(const Args& k, const Plan& p, bool norm, bool backward, hipStream_t s) {
+  const dim3 grid(p.blocks[0] + p.blocks[1]);
+  if (!norm) hipLaunchKernelGGL((rotary_kernel<T, TURN, NEIGHBOURS>), grid, dim3(THREADS), 0, s, k);
+  else if (!backward) hipLaunchKernelGGL((rotary_kernel<T, NORM, NEIGHBOURS>), grid, dim3(THREADS), 0, s, k);
+  else hipLaunchKernelGGL((rotary_kernel<T, NORM_BACK, NEIGHBOURS>), grid, dim3(THREADS), 0, s, k);
+}
+template <class T> void run(const s2cnn_rotary_t& a, bool backward, float* partial, hipStream_t s) {
+  const Plan p = plan_of(a, partial != nullptr);
+  const Args k = args_of(a, p, backward, partial);
+  if (a.interleaved) launch<T, true>(k, p, a.norm != 0, backward, s);
+  else launch<T, false>(k, p, a.norm != 0, backward, s);
+  if (partial)
+    hipLaunchKernelGGL(weights_kernel<T>, dim3((unsigned)((a.d + 31) / 32), 2), dim3(1024), 0, s, k.side[0].partial, k.side[1].partial, p.blocks[0], p.blocks[1], a.d,
+                       static_cast<T*>(a.side[0].gweight), static_cast<T*>(a.side[1].gweight));
+}
+void run(const s2cnn_rotary_t& a, bool backward, float* partial, hipStream_t s) {
+  if (a.dtype == S2CNN_F32) run<float>(a, backward, partial, s);
+  else if (a.dtype == S2CNN_BF16) run<__bf16>(a, backward, partial, s);
+  else run<half_t>(a, backward, partial, s);
+}
+
+// S2CNN_OK, or why a call is refused
+int check(const s2cnn_rotary_t* a, bool backward) {
+  if (!sizes_ok(a)) return S2CNN_EINVAL;
+  const uintptr_t mask = a->dtype == S2CNN_F32 ? 3 : 1;
+  for (const s2cnn_rotary_side_t& s : a->side) {
+    if (!s.heads) continue;
+    const bool needs_x = !backward || a->norm;
+    if ((needs_x && !s.x) || (backward && !s.g) || !s.y || (s.weight && !a->norm)) return S2CNN_EINVAL;
+    if (s.gweight && !(backward && a->norm)) return S2CNN_EINVAL;
+    uintptr_t all = reinterpret_cast<uintptr_t>(s.y) | reinterpret_cast<uintptr_t>(s.weight) | reinterpret_cast<uintptr_t>(s.gweight);
+    if (needs_x) all |= reinterpret_cast<uintptr_t>(s.x);
+    if (backward) all |= reinterpret_cast<uintptr_t>(s.g);
+    if (all & mask) return S2CNN_EALIGN;
+  }
+  if (!aligned8(a->table) || (a->table_stride & 1) || (reinterpret_cast<uintptr_t>(a->index) & 3)) return S2CNN_EALIGN;
+  return S2CNN_OK;
+}
+bool wants_sums(const s2cnn_rotary_t& a) { return a.norm && ((a.side[0].heads && a.side[0].gweight) || (a.side[1].heads && a.side[1].gweight)); }
+
+}  // namespace rotary
+}  // namespace s2cnn
+
+using namespace s2cnn;
+
+extern "C" int s2cnn_rotary_fwd(const s2cnn_rotary_t* a, void* stream) {
+  clear_stale_error();
+  const int rc = rotary::check(a, false);
+  if (rc) return rc;
+  rotary::run(*a, false, nullptr, static_cast<hipStream_t>(stream));
+  return launch_status();
+}
+
+extern "C" size_t s2cnn_rotary_workspace(const s2cnn_rotary_t* a) {
+  if (!rotary::sizes_ok(a) || !a->norm) return 0;
+  const rotary::Plan p = rotary::plan_of(*a, true);
+  return ((size_t)p.blocks[0] + p.blocks[1]) * a->d * sizeof(float);
+}
+
+extern "C" int s2cnn_rotary_bwd(const s2cnn_rotary_t* a, void* workspace, size_t workspace_bytes, void* stream) {
+  clear_stale_error();
+  const int rc = rotary::check(a, true);
+  if (rc) return rc;
+  const bool sums = rotary::wants_sums(*a);
+  if (sums && (!workspace || workspace_bytes < s2cnn_rotary_workspace(a) || !aligned16(workspace))) return S2CNN_EWORKSPACE;
+  rotary::run(*a, true, sums ? static_cast<float*>(workspace) : nullptr, static_cast<hipStream_t>(stream));
+  return launch_status();
+}
+
+extern "C" int s2cnn_rotary_table(const void* positions, int positions_type, const double* frequencies, float* table, long n, int axes, int pairs, float scale, void* stream) {
+  clear_stale_error();
+  if (!positions || !frequencies || !table || n < 1 || axes < 1 || axes > 1024 || pairs < 1 || pairs > rotary::MAX_D / 2 || n >= (1L << 40)) return S2CNN_EINVAL;
+  if (positions_type < S2CNN_POSITIONS_F32 || positions_type > S2CNN_POSITIONS_I64) return S2CNN_EINVAL;
+  const bool wide = positions_type == S2CNN_POSITIONS_F64 || positions_type == S2CNN_POSITIONS_I64;
+  if ((reinterpret_cast<uintptr_t>(positions) & (wide ? 7 : 3)) || !aligned8(frequencies) || !aligned8(table)) return S2CNN_EALIGN;
+  const long side = rotary::THREADS / pairs, need = (n + side - 1) / side, most = rotary::CUS * 16;
+  const dim3 grid((unsigned)(need < most ? need : most)), block(rotary::THREADS);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  float2* const out = reinterpret_cast<float2*>(table);
+  const auto run = [&](auto* at) { hipLaunchKernelGGL(rotary::table_kernel, grid, block, 0, s, at, frequencies, out, n, axes, pairs, scale); };
+  switch (positions_type) {
+    case S2CNN_POSITIONS_F32: run(static_cast<const float*>(positions)); break;
+    case S2CNN_POSITIONS_F64: run(static_cast<const double*>(positions)); break;
+    case S2CNN_POSITIONS_I32: run(static_cast<const int*>(positions)); break;
+    default: run(static_cast<const long long*>(positions));
+  }
+  return launch_status();
+}
