@@ -514,6 +514,41 @@ int s2cnn_rotary_bwd(const s2cnn_rotary_t *a, void *workspace, size_t workspace_
 int s2cnn_rotary_table(const void *positions, int positions_type, const double *frequencies, float *table, long n, int axes, int pairs,
                        float scale, void *stream);
 
+/* ---- the step of an optimizer over a list of tensors --------------------------------------------
+ * adamw_step: for every tensor i of n[i] entries, dense: g' = g min(1, max_norm / *norm) (norm NULL: g), m = beta1 m + (1 - beta1) g',
+ *   v = beta2 v + (1 - beta2) g'^2, p = p - lr weight_decay p - lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps), arithmetic in float32.
+ *   p, g: of dtype.  masters: float32 copies of 16-bit parameters, or NULL: the step is made there and p is its rounding; where p was not the
+ *   master's rounding, p is taken.  t = step >= 1, or *step_at; lr, or *lr_at: device memory that is read when the kernel runs, or NULL.
+ *   Where *norm is infinite or no number, nothing is written.  Tensors do not overlap.
+ *   bits 32: first and second are float32, scales NULL.  bits 8: first is of one byte an entry (float8 of 4 exponent and 3 mantissa bits), second of one
+ *   (f(c) = c for c < 8, (8 + c % 8) 2^(c / 8 - 1) beyond), scales [ceil(n / 256)][2] float32, 8-byte aligned: the factors of m (in units of 2^-9) and v of
+ *   every 256 entries.  Rounded at random: halves of word e % 4 of Philox4x32-10 of counter (e / 4, t) and key seed, e the entry's number in the list,
+ *   every tensor from a multiple of 256 on.  A factor is the largest entry over f(126) or f(255), 0 (and the block's entries) where below 2^-126;
+ *   of a block with an infinite entry, or one that is no number, all entries become such.
+ * adamw_states: the moments of 8 bits in float32, n[i] entries each.
+ * grad_norm: *out = sqrt of the sum of squares of all entries of a list of tensors of any types, summed in 64 bits.
+ * Lists are host memory, read during the call; tensors without entries are left out (their pointers may be NULL).
+ */
+typedef struct s2cnn_adamw_t {
+  void *const *p;
+  const void *const *g;
+  void *const *first, *const *second, *const *scales, *const *masters;
+  const long *n;
+  const float *lr_at, *norm;
+  const long long *step_at;
+  long long step;
+  unsigned long long seed;
+  double lr, beta1, beta2, eps, weight_decay, max_norm;      /* 1e-30 <= eps; max_norm > 0 (with norm) */
+  int count, dtype, bits;
+} s2cnn_adamw_t;
+
+int s2cnn_adamw_step(const s2cnn_adamw_t *a, void *stream);
+int s2cnn_adamw_states(const void *const *first, const void *const *second, const void *const *scales, void *const *first_out,
+                       void *const *second_out, const long *n, int count, void *stream);
+size_t s2cnn_grad_norm_workspace(const long *n, const int *dtypes, int count);     /* 0 also for lists that are refused */
+int s2cnn_grad_norm(const void *const *g, const long *n, const int *dtypes, int count, float *out, void *workspace, size_t workspace_bytes,
+                    void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -11,6 +11,7 @@ from .so3_real import so3_mm_real, so3_rft_real, so3_spectrum_to_complex, so3_sp
 from .s2_real import s2_mm_real, s2_rft_real, s2_spectrum_to_real
 from .attention import attention, s2_angle_buckets, s2_log_weights
 from .layer_norm import dropout, dropout_add_layer_norm, layer_norm
+from .optim import AdamW, adamw_states, adamw_step, grad_norm
 from .rotary import norm_rotary, rotary, rotary_frequencies, rotary_table, s2_rotary_frequencies, s2_rotary_table
 from .soft.s2_transformer import S2AttentionPool, S2Transformer, S2TransformerBlock
 

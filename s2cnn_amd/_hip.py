@@ -48,6 +48,13 @@ class Rotary(ctypes.Structure):
 
 _ROTARY_P = ctypes.POINTER(Rotary)
 
+
+class AdamW(ctypes.Structure):
+    """s2cnn_adamw_t"""
+    _fields_ = ([(n, _vp) for n in ("p", "g", "first", "second", "scales", "masters", "n", "lr_at", "norm", "step_at")]
+                + [("step", ctypes.c_longlong), ("seed", ctypes.c_ulonglong)]
+                + [(n, ctypes.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay", "max_norm")] + [(n, _int) for n in ("count", "dtype", "bits")])
+
 SIGNATURES = {
     "s2cnn_abi_version": (_int, []),
     "s2cnn_strerror": (ctypes.c_char_p, [_int]),
@@ -125,6 +132,10 @@ SIGNATURES = {
     "s2cnn_rotary_workspace": (_size_t, [_ROTARY_P]),
     "s2cnn_rotary_bwd": (_int, [_ROTARY_P, _vp, _size_t, _vp]),
     "s2cnn_rotary_table": (_int, [_vp, _int, _vp, _vp, _long, _int, _int, _float, _vp]),
+    "s2cnn_adamw_step": (_int, [ctypes.POINTER(AdamW), _vp]),
+    "s2cnn_adamw_states": (_int, [_vp] * 6 + [_int, _vp]),
+    "s2cnn_grad_norm_workspace": (_size_t, [_vp, _vp, _int]),
+    "s2cnn_grad_norm": (_int, [_vp, _vp, _vp, _int, _vp, _vp, _size_t, _vp]),
     "s2cnn_so3_integrate_grad": (_int, [_c_float_p, _c_float_p, _c_float_p, _int, _long, _vp]),
 }
 

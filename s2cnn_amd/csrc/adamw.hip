@@ -1,0 +1,456 @@
+// The step of an optimizer over a list of tensors (AdamW), with moments in 32 or in 8 bits, and the norm of a list of gradients.
+//
+//   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,  p = p - lr decay p - lr (m / (1 - b1^t)) / (sqrt(v / (1 - b2^t)) + eps)
+//
+// with g multiplied by min(1, max_norm / norm) first where a norm is given.  Bound by memory: every tensor is read once and written once, in one
+// launch for some fifty tensors, whose addresses travel in the kernel's arguments: nothing is copied to the device, and a captured graph keeps them.
+// A workgroup takes 4096 entries of one tensor, a wave 256 at a time, four a lane.
+//
+// Moments in 8 bits.  A block of 256 entries (a wave's) has a factor s of each moment; an entry is s f(c), f(c) = c for c < 8, (8 + c % 8) 2^(c / 8 - 1)
+// beyond: three bits after the leading one, so that a step is 1/8 to 1/16 of the value.  First moments: a sign and c <= 126, in units of 2^-9
+// the type float8_e4m3fn.  Second moments: c <= 255, 2^34 from the smallest to the largest, because their roots go through the same range as
+// first moments do, and never 0 where the moment is not: the quotient stays bounded.  A step changes a second moment by a thousandth
+// (b2 = 0.999), far below the spacing, and would be rounded away; so both are rounded up or down at random, with the probability that leaves the
+// mean right.  The random bits are a function of the seed, the step and the entry's number: 16 for each moment.
+// m, v, s and the codes are formed by single float32 operations in the order written, without fused ones: a program that does the same gets the same codes.
+#include "chunk.h"
+#include "counter_random.h"
+
+namespace s2cnn {
+namespace adamw {
+
+constexpr int THREADS = 256;
+constexpr int BLOCK = 256;                     // entries of a factor
+constexpr int PART = 4096;                     // entries of a workgroup
+constexpr int MOST = 56;                       // tensors of a launch: 4 KB of arguments
+constexpr int MOST_SUMS = 184;
+constexpr float TOP_FIRST = 229376.f, TOP_SECOND = 15.f * 1073741824.f;      // f(126), f(255)
+
+struct Tensors {
+  void* p[MOST];
+  const void* g[MOST];
+  void* first[MOST];
+  void* second[MOST];
+  float2* scales[MOST];
+  float* master[MOST];
+  long n[MOST];
+  unsigned long long counter[MOST];            // random numbers before this tensor's, in fours
+  unsigned part[MOST + 1];                     // workgroups before this tensor's
+  int count;
+};
+struct Step {
+  const float *lr_at, *norm;
+  const long long* step_at;
+  long long step;
+  unsigned long long seed;
+  double log_b1, log_b2;
+  float lr, b1, rest1, b2, rest2, eps, decay, max_norm;
+};
+static_assert(sizeof(Tensors) + sizeof(Step) <= 4096, "kernel arguments");
+
+// The tensor of workgroup `part`: the last whose first workgroup is not behind it.
+template <int N> __device__ __forceinline__ int tensor_of(const unsigned (&first)[N], int count, unsigned part) {
+  int low = 0, high = count;
+  while (high - low > 1) {
+    const int mid = (low + high) / 2;
+    if (first[mid] <= part) low = mid;
+    else high = mid;
+  }
+  return low;
+}
+
+// Four entries at any address of the type, the first n of them
+template <class T> __device__ __forceinline__ void load4(const T* p, long n, float (&v)[4]) {
+  if (n >= 4) {
+    if constexpr (sizeof(T) == 4) {
+      typedef float loose __attribute__((ext_vector_type(4), aligned(4)));
+      const loose x = *reinterpret_cast<const loose*>(p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = x[i];
+    } else {
+      typedef T loose __attribute__((ext_vector_type(4), aligned(2)));
+      const loose x = *reinterpret_cast<const loose*>(p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = (float)x[i];
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = i < n ? (float)p[i] : 0.f;
+}
+template <class T> __device__ __forceinline__ void store4(T* p, long n, const float (&v)[4]) {
+  if (n >= 4) {
+    typedef T loose __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    *reinterpret_cast<loose*>(p) = loose{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < n) p[i] = (T)v[i];
+}
+typedef unsigned loose_bytes __attribute__((aligned(1)));
+__device__ __forceinline__ unsigned load4(const unsigned char* p, long n) {
+  if (n >= 4) return *reinterpret_cast<const loose_bytes*>(p);
+  unsigned c = 0;
+#pragma unroll
+  for (int i = 0; i < 3; ++i)
+    if (i < n) c |= (unsigned)p[i] << (8 * i);
+  return c;
+}
+__device__ __forceinline__ void store4(unsigned char* p, long n, unsigned c) {
+  if (n >= 4) {
+    *reinterpret_cast<loose_bytes*>(p) = c;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 3; ++i)
+    if (i < n) p[i] = (unsigned char)(c >> (8 * i));
+}
+
+// ---- codes ----------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void first_of(unsigned c, float s, float (&m)[4]) {
+  const f2 low = __builtin_amdgcn_cvt_pk_f32_fp8(c, false), high = __builtin_amdgcn_cvt_pk_f32_fp8(c, true);
+  m[0] = low[0] * 512.f * s, m[1] = low[1] * 512.f * s, m[2] = high[0] * 512.f * s, m[3] = high[1] * 512.f * s;
+}
+__device__ __forceinline__ void second_of(unsigned codes, float s, float (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const unsigned c = (codes >> (8 * i)) & 255u;
+    v[i] = (c < 8 ? (float)c : __uint_as_float((c << 20) + (129u << 23))) * s;
+  }
+}
+// The code of y >= 0, rounded by 16 random bits: where y >= 8, the bits of the float32 with those added behind the three that stay.
+__device__ __forceinline__ unsigned code_of(float y, unsigned random, unsigned most) {
+  const unsigned high = ((__float_as_uint(y) + (random << 4)) >> 20) - (129u << 3), low = (unsigned)floorf(y + (float)random * 0x1p-16f);
+  return min(y >= 8.f ? high : low, most);
+}
+__device__ __forceinline__ unsigned max_wave(unsigned v) {           // in all 64 lanes
+  const auto with = [&](unsigned o) { v = max(v, o); };
+  with(__builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, true));
+  with(__builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, true));
+  with(__builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true));
+  with(__builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, true));
+  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return max(b[0], b[1]);
+}
+// A block's factor from its largest entry (the bits of a float32 without sign, so that what is no number is the largest); below 2^-126 none.
+__device__ __forceinline__ float factor_of(unsigned largest, float inverse_top) {
+#pragma clang fp contract(off)
+  const float s = __uint_as_float(largest) * inverse_top;
+  return s < 0x1p-126f ? 0.f : s;
+}
+
+template <class T, int BITS, bool MASTER> __global__ __launch_bounds__(THREADS) void step_kernel(Tensors t, Step h) {
+  const int k = tensor_of(t.part, t.count, blockIdx.x);
+  float clip = 1.f;
+  if (h.norm) {
+    const float norm = *h.norm;
+    if (!(norm < __builtin_inff())) return;                         // infinite, or no number: the step is left out
+    clip = fminf(h.max_norm / norm, 1.f);
+  }
+  const long long step = h.step_at ? *h.step_at : h.step;
+  const float lr = h.lr_at ? *h.lr_at : h.lr;
+  const float size = lr / -expm1f((float)((double)step * h.log_b1)), inverse2 = 1.f / -expm1f((float)((double)step * h.log_b2)), decay = lr * h.decay;
+  const long n = t.n[k];
+  const int lane = threadIdx.x & 63;
+  const long start = (long)(blockIdx.x - t.part[k]) * PART + (threadIdx.x >> 6) * BLOCK;
+
+#pragma unroll 2
+  for (int turn = 0; turn < PART / (4 * BLOCK); ++turn) {
+    const long block = start + (long)turn * 4 * BLOCK, at = block + lane * 4, left = n - at;
+    if (block >= n) break;
+    float g[4], p[4], m[4], v[4], master[4];
+    load4<T>(static_cast<const T*>(t.g[k]) + at, left, g);
+    load4<T>(static_cast<T*>(t.p[k]) + at, left, p);
+    if constexpr (MASTER) load4<float>(t.master[k] + at, left, master);
+    if constexpr (BITS == 32) {
+      load4<float>(static_cast<float*>(t.first[k]) + at, left, m);
+      load4<float>(static_cast<float*>(t.second[k]) + at, left, v);
+    } else {
+      const float2 s = t.scales[k][block / BLOCK];
+      first_of(load4(static_cast<unsigned char*>(t.first[k]) + at, left), s.x, m);
+      second_of(load4(static_cast<unsigned char*>(t.second[k]) + at, left), s.y, v);
+    }
+    {
+#pragma clang fp contract(off)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        g[i] *= clip;
+        m[i] = m[i] * h.b1 + g[i] * h.rest1;
+        v[i] = v[i] * h.b2 + (g[i] * g[i]) * h.rest2;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      // where the parameter is not its master's rounding, the program has set it since
+      const float x = MASTER && (float)(T)master[i] == p[i] ? master[i] : p[i];
+      const float denominator = __builtin_amdgcn_sqrtf(v[i] * inverse2) + h.eps;
+      p[i] = fmaf(-size, m[i] * __builtin_amdgcn_rcpf(denominator), fmaf(-decay, x, x));
+    }
+    store4<T>(static_cast<T*>(t.p[k]) + at, left, p);
+    if constexpr (MASTER) store4<float>(t.master[k] + at, left, p);
+    if constexpr (BITS == 32) {
+      store4<float>(static_cast<float*>(t.first[k]) + at, left, m);
+      store4<float>(static_cast<float*>(t.second[k]) + at, left, v);
+    } else {
+#pragma clang fp contract(off)
+      unsigned top1 = 0, top2 = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top1 = max(top1, __float_as_uint(fabsf(m[i]))), top2 = max(top2, __float_as_uint(fabsf(v[i])));
+      const float s1 = factor_of(max_wave(top1), (float)(1.0 / TOP_FIRST)), s2 = factor_of(max_wave(top2), (float)(1.0 / TOP_SECOND));
+      const float i1 = s1 == 0.f ? 0.f : 1.f / s1, i2 = s2 == 0.f ? 0.f : 1.f / s2;
+      const uint4 r = philox(t.counter[k] + (unsigned long long)(at >> 2), h.seed, (unsigned long long)step);
+      const unsigned random[4] = {r.x, r.y, r.z, r.w};
+      unsigned c1 = 0, c2 = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        c1 |= (code_of(fabsf(m[i]) * i1, random[i] & 0xffffu, 126u) | (m[i] < 0.f ? 128u : 0u)) << (8 * i);
+        c2 |= max(code_of(v[i] * i2, random[i] >> 16, 255u), v[i] > 0.f && i2 > 0.f ? 1u : 0u) << (8 * i);
+      }
+      store4(static_cast<unsigned char*>(t.first[k]) + at, left, c1);
+      store4(static_cast<unsigned char*>(t.second[k]) + at, left, c2);
+      if (lane == 0) t.scales[k][block / BLOCK] = make_float2(s1, s2);
+    }
+  }
+}
+
+// The moments that 8-bit codes stand for: p and master hold where they are written.
+__global__ __launch_bounds__(THREADS) void states_kernel(Tensors t) {
+  const int k = tensor_of(t.part, t.count, blockIdx.x);
+  const long n = t.n[k];
+  const long start = (long)(blockIdx.x - t.part[k]) * PART + threadIdx.x * 4;
+#pragma unroll
+  for (int turn = 0; turn < PART / (4 * THREADS); ++turn) {
+    const long at = start + turn * 4 * THREADS, left = n - at;
+    if (left <= 0) break;
+    const float2 s = t.scales[k][at / BLOCK];
+    float m[4], v[4];
+    first_of(load4(static_cast<unsigned char*>(t.first[k]) + at, left), s.x, m);
+    second_of(load4(static_cast<unsigned char*>(t.second[k]) + at, left), s.y, v);
+    store4<float>(static_cast<float*>(t.p[k]) + at, left, m);
+    store4<float>(t.master[k] + at, left, v);
+  }
+}
+
+// ---- the norm of a list ---------------------------------------------------------------------------------------------
+// Squares are summed in 64 bits: the factor that gradients are clipped by does not depend on the order, but for ties of its one rounding, and no square
+// overflows or vanishes.  A workgroup sums 32 KB of a tensor, eight loads of 16 bytes a lane under way, and a single one joins their sums.
+struct Lists {
+  const void* g[MOST_SUMS];
+  long n[MOST_SUMS];
+  unsigned part[MOST_SUMS + 1];
+  unsigned char dtype[MOST_SUMS];
+  int count;
+};
+static_assert(sizeof(Lists) + 16 <= 4096, "kernel arguments");
+constexpr int LOADS = 8;
+inline long sums_part(int dtype) { return (long)LOADS * THREADS * (dtype == S2CNN_F32 ? 4 : 8); }
+
+template <class T> __device__ __forceinline__ double squares(const T* g, long n) {
+  typedef Chunk<T> C;
+  uint4 raw[LOADS];
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    const long at = ((long)i * THREADS + threadIdx.x) * C::N;
+    raw[i] = at < n ? load_chunk<T>(g + at, (int)min(n - at, (long)C::N)) : make_uint4(0, 0, 0, 0);
+  }
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    float v[C::N];
+    C::get(raw[i], v);
+#pragma unroll
+    for (int j = 0; j < C::N; ++j) sum = fma((double)v[j], (double)v[j], sum);
+  }
+  return sum;
+}
+// over a workgroup, in thread 0
+template <int WAVES> __device__ __forceinline__ double sum_workgroup(double v) {
+  __shared__ double waves[WAVES];
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
+  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0.0;
+  for (int i = 0; i < WAVES; ++i) v += waves[i];
+  return v;
+}
+__global__ __launch_bounds__(THREADS) void squares_kernel(Lists t, double* partial) {
+  const int k = tensor_of(t.part, t.count, blockIdx.x), dtype = t.dtype[k];
+  const long per = (long)LOADS * THREADS * (dtype == S2CNN_F32 ? 4 : 8), at = (long)(blockIdx.x - t.part[k]) * per, n = t.n[k] - at;
+  double sum;
+  if (dtype == S2CNN_F32) sum = squares(static_cast<const float*>(t.g[k]) + at, n);
+  else if (dtype == S2CNN_BF16) sum = squares(static_cast<const __bf16*>(t.g[k]) + at, n);
+  else sum = squares(static_cast<const half_t*>(t.g[k]) + at, n);
+  sum = sum_workgroup<THREADS / 64>(sum);
+  if (threadIdx.x == 0) partial[blockIdx.x] = sum;
+}
+__global__ __launch_bounds__(1024) void norm_kernel(const double* partial, long parts, float* out) {
+  double sum[4] = {0.0, 0.0, 0.0, 0.0};
+  for (long i = threadIdx.x; i < parts; i += 4 * 1024)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i + j * 1024 < parts) sum[j] += partial[i + j * 1024];
+  const double all = sum_workgroup<16>((sum[0] + sum[1]) + (sum[2] + sum[3]));
+  if (threadIdx.x == 0) *out = (float)sqrt(all);
+}
+
+// ---- launches -------------------------------------------------------------------------------------------------------
+constexpr long MOST_ENTRIES = 1L << 42;
+
+template <class T, int BITS> void launch(const Tensors& t, const Step& h, bool master, hipStream_t s) {
+  const dim3 grid(t.part[t.count]), block(THREADS);
+  if constexpr (sizeof(T) == 2)
+    if (master) {
+      hipLaunchKernelGGL((step_kernel<T, BITS, true>), grid, block, 0, s, t, h);
+      return;
+    }
+  hipLaunchKernelGGL((step_kernel<T, BITS, false>), grid, block, 0, s, t, h);
+}
+void launch(const Tensors& t, const Step& h, int dtype, int bits, bool master, hipStream_t s) {
+  if (dtype == S2CNN_F32) bits == 8 ? launch<float, 8>(t, h, false, s) : launch<float, 32>(t, h, false, s);
+  else if (dtype == S2CNN_BF16) bits == 8 ? launch<__bf16, 8>(t, h, master, s) : launch<__bf16, 32>(t, h, master, s);
+  else bits == 8 ? launch<half_t, 8>(t, h, master, s) : launch<half_t, 32>(t, h, master, s);
+}
+
+bool misaligned(const void* p, unsigned size) { return (reinterpret_cast<uintptr_t>(p) & (size - 1)) != 0; }
+bool known(int dtype) { return dtype == S2CNN_F32 || dtype == S2CNN_BF16 || dtype == S2CNN_F16; }
+
+// Lists of tensors, MOST of them and fewer than 2^31 workgroups at a time, to `run`; those without entries are left out.
+template <class F> void for_parts(int count, const long* n, const F& add, void (*launch_part)(const Tensors&, const void*), const void* with) {
+  Tensors t = {};
+  unsigned long long counter = 0;
+  for (int i = 0; i < count; ++i) {
+    if (!n[i]) continue;
+    const unsigned long need = (unsigned long)(n[i] + PART - 1) / PART;
+    if (t.count == MOST || (t.count && t.part[t.count] + need > 0x7fffffffUL)) {
+      launch_part(t, with);
+      t.count = 0;
+    }
+    const int k = t.count++;
+    add(t, k, i);
+    t.n[k] = n[i];
+    t.counter[k] = counter;
+    t.part[k + 1] = (k ? t.part[k] : 0) + (unsigned)need;
+    t.part[0] = 0;
+    counter += (unsigned long long)((n[i] + BLOCK - 1) / BLOCK) * (BLOCK / 4);
+  }
+  if (t.count) launch_part(t, with);
+}
+
+}  // namespace adamw
+}  // namespace s2cnn
+
+using namespace s2cnn;
+using namespace s2cnn::adamw;
+
+extern "C" int s2cnn_adamw_step(const s2cnn_adamw_t* a, void* stream) {
+  clear_stale_error();
+  if (!a || a->count < 0 || !known(a->dtype) || (a->bits != 8 && a->bits != 32) || (a->masters && a->dtype == S2CNN_F32)) return S2CNN_EINVAL;
+  if (a->count && (!a->p || !a->g || !a->first || !a->second || !a->n || (a->bits == 8) != (a->scales != nullptr))) return S2CNN_EINVAL;
+  if (!(a->beta1 >= 0.0 && a->beta1 < 1.0 && a->beta2 >= 0.0 && a->beta2 < 1.0 && a->eps >= 1e-30 && a->eps < 1e30)) return S2CNN_EINVAL;
+  if (!(a->lr >= 0.0 && a->lr < 1e30 && a->weight_decay >= 0.0 && a->weight_decay < 1e30) || (!a->step_at && a->step < 1)) return S2CNN_EINVAL;
+  if (a->norm && !(a->max_norm > 0.0 && a->max_norm < 1e38)) return S2CNN_EINVAL;
+  if (misaligned(a->lr_at, 4) || misaligned(a->norm, 4) || misaligned(a->step_at, 8)) return S2CNN_EALIGN;
+  if (!a->count) return S2CNN_OK;
+  const unsigned size = a->dtype == S2CNN_F32 ? 4 : 2, state = a->bits == 8 ? 1 : 4;
+  for (int i = 0; i < a->count; ++i) {
+    if (a->n[i] < 0 || a->n[i] >= MOST_ENTRIES) return S2CNN_EINVAL;
+    if (!a->n[i]) continue;
+    if (!a->p[i] || !a->g[i] || !a->first[i] || !a->second[i] || (a->scales && !a->scales[i]) || (a->masters && !a->masters[i])) return S2CNN_EINVAL;
+    if (misaligned(a->p[i], size) || misaligned(a->g[i], size) || misaligned(a->first[i], state) || misaligned(a->second[i], state)) return S2CNN_EALIGN;
+    if ((a->scales && misaligned(a->scales[i], 8)) || (a->masters && misaligned(a->masters[i], 4))) return S2CNN_EALIGN;
+  }
+  struct With {
+    const s2cnn_adamw_t* a;
+    Step h;
+    hipStream_t s;
+  } with = {a,
+            {a->lr_at, a->norm, a->step_at, a->step, a->seed, __builtin_log(a->beta1), __builtin_log(a->beta2), (float)a->lr, (float)a->beta1, (float)(1.0 - a->beta1),
+             (float)a->beta2, (float)(1.0 - a->beta2), (float)a->eps, (float)a->weight_decay, (float)a->max_norm},
+            static_cast<hipStream_t>(stream)};
+  for_parts(
+      a->count, a->n,
+      [&](Tensors& t, int k, int i) {
+        t.p[k] = a->p[i], t.g[k] = a->g[i], t.first[k] = a->first[i], t.second[k] = a->second[i];
+        t.scales[k] = a->scales ? static_cast<float2*>(a->scales[i]) : nullptr;
+        t.master[k] = a->masters ? static_cast<float*>(a->masters[i]) : nullptr;
+      },
+      [](const Tensors& t, const void* w) {
+        const With& of = *static_cast<const With*>(w);
+        launch(t, of.h, of.a->dtype, of.a->bits, of.a->masters != nullptr, of.s);
+      },
+      &with);
+  return launch_status();
+}
+
+extern "C" int s2cnn_adamw_states(const void* const* first, const void* const* second, const void* const* scales, void* const* first_out, void* const* second_out,
+                                  const long* n, int count, void* stream) {
+  clear_stale_error();
+  if (count < 0 || (count && (!first || !second || !scales || !first_out || !second_out || !n))) return S2CNN_EINVAL;
+  if (!count) return S2CNN_OK;
+  for (int i = 0; i < count; ++i) {
+    if (n[i] < 0 || n[i] >= MOST_ENTRIES) return S2CNN_EINVAL;
+    if (!n[i]) continue;
+    if (!first[i] || !second[i] || !scales[i] || !first_out[i] || !second_out[i]) return S2CNN_EINVAL;
+    if (misaligned(scales[i], 8) || misaligned(first_out[i], 4) || misaligned(second_out[i], 4)) return S2CNN_EALIGN;
+  }
+  for_parts(
+      count, n,
+      [&](Tensors& t, int k, int i) {
+        t.first[k] = const_cast<void*>(first[i]), t.second[k] = const_cast<void*>(second[i]);
+        t.scales[k] = static_cast<float2*>(const_cast<void*>(scales[i]));
+        t.p[k] = first_out[i], t.master[k] = static_cast<float*>(second_out[i]);
+      },
+      [](const Tensors& t, const void* s) { hipLaunchKernelGGL(states_kernel, dim3(t.part[t.count]), dim3(THREADS), 0, static_cast<hipStream_t>(const_cast<void*>(s)), t); }, stream);
+  return launch_status();
+}
+
+// Sums of the workgroups of the whole list, 0 for a list that is refused
+static long parts_of(const long* n, const int* dtypes, int count) {
+  long parts = 0;
+  for (int i = 0; i < count; ++i) {
+    if (n[i] < 0 || n[i] >= MOST_ENTRIES || !known(dtypes[i])) return -1;
+    parts += (n[i] + sums_part(dtypes[i]) - 1) / sums_part(dtypes[i]);
+  }
+  return parts;
+}
+
+extern "C" size_t s2cnn_grad_norm_workspace(const long* n, const int* dtypes, int count) {
+  const long parts = count < 0 || (count && (!n || !dtypes)) ? -1 : parts_of(n, dtypes, count);
+  return parts < 0 ? 0 : (size_t)parts * sizeof(double);
+}
+
+extern "C" int s2cnn_grad_norm(const void* const* g, const long* n, const int* dtypes, int count, float* out, void* workspace, size_t workspace_bytes, void* stream) {
+  clear_stale_error();
+  if (count < 0 || !out || (count && (!g || !n || !dtypes))) return S2CNN_EINVAL;
+  const long parts = parts_of(n, dtypes, count);
+  if (parts < 0) return S2CNN_EINVAL;
+  if (misaligned(out, 4)) return S2CNN_EALIGN;
+  for (int i = 0; i < count; ++i) {
+    if (n[i] && !g[i]) return S2CNN_EINVAL;
+    if (n[i] && misaligned(g[i], dtypes[i] == S2CNN_F32 ? 4 : 2)) return S2CNN_EALIGN;
+  }
+  if (parts && (!workspace || workspace_bytes < (size_t)parts * sizeof(double) || !aligned16(workspace))) return S2CNN_EWORKSPACE;
+  double* partial = static_cast<double*>(workspace);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  Lists t = {};
+  const auto run = [&] {
+    if (t.count) hipLaunchKernelGGL(squares_kernel, dim3(t.part[t.count]), dim3(THREADS), 0, s, t, partial);
+    partial += t.part[t.count];
+    t.count = 0;
+  };
+  for (int i = 0; i < count; ++i) {
+    if (!n[i]) continue;
+    const unsigned long need = (unsigned long)((n[i] + sums_part(dtypes[i]) - 1) / sums_part(dtypes[i]));
+    if (t.count == MOST_SUMS || (t.count && t.part[t.count] + need > 0x7fffffffUL)) run();
+    const int k = t.count++;
+    t.g[k] = g[i], t.n[k] = n[i], t.dtype[k] = (unsigned char)dtypes[i];
+    t.part[k + 1] = t.part[k] + (unsigned)need;
+  }
+  run();
+  hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(1024), 0, s, static_cast<const double*>(workspace), parts, out);
+  return launch_status();
+}

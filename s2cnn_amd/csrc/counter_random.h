@@ -32,8 +32,8 @@ inline Dropout make_dropout(double p, unsigned long long seed, const long long* 
 
 __device__ __forceinline__ unsigned long long dropout_seed(const Dropout& d) { return d.seed_at ? (unsigned long long)*d.seed_at : d.seed; }
 
-__device__ __forceinline__ uint4 philox(unsigned long long counter, unsigned long long key) {
-  unsigned c0 = (unsigned)counter, c1 = (unsigned)(counter >> 32), c2 = 0, c3 = 0, k0 = (unsigned)key, k1 = (unsigned)(key >> 32);
+__device__ __forceinline__ uint4 philox(unsigned long long counter, unsigned long long key, unsigned long long upper = 0) {      // upper half of the counter
+  unsigned c0 = (unsigned)counter, c1 = (unsigned)(counter >> 32), c2 = (unsigned)upper, c3 = (unsigned)(upper >> 32), k0 = (unsigned)key, k1 = (unsigned)(key >> 32);
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
     const unsigned long long a = (unsigned long long)c0 * 0xD2511F53u, b = (unsigned long long)c2 * 0xCD9E8D57u;

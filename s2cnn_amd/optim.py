@@ -1,0 +1,291 @@
+"""The step that trains a network: AdamW over all its tensors at once, with moments in 32 or 8 bits, and the norm of their gradients.
+
+The reference trains with torch's own optimizers (examples/mnist/run.py:150-153, examples/shrec17/train.py:66), a handful of launches for
+every tensor or every dozen of them; its networks have some tens of tensors of which most are small.  Here all tensors of a list are one launch
+(some fifty a launch), the clipping of gradients is part of it, and the moments may take a quarter of the memory.
+"""
+import ctypes
+import math
+from array import array
+from operator import attrgetter
+
+import torch
+
+from . import _hip
+
+BLOCK = 256                                              # entries that share a factor where moments are held in 8 bits
+
+_dtype, _shape = attrgetter("dtype"), attrgetter("shape")
+_contiguous, _device, _numel, _address = torch.Tensor.is_contiguous, torch.Tensor.get_device, torch.Tensor.numel, torch.Tensor.data_ptr
+
+
+def _check_list(tensors, dtype, device, what):
+    """Dense tensors of one type on one device."""
+    if set(map(_dtype, tensors)) != {dtype}:
+        raise RuntimeError("%s of one type only, %s (got %s)" % (what, dtype, ", ".join(sorted(map(str, set(map(_dtype, tensors)))))))
+    if set(map(_device, tensors)) != {device}:
+        raise RuntimeError("%s on the current GPU only, cuda:%d; there is no CPU path" % (what, torch.cuda.current_device() if torch.cuda.is_available() else 0))
+    if not all(map(_contiguous, tensors)):
+        raise RuntimeError("%s have to be contiguous" % what)
+
+
+def _addresses(tensors):
+    return array("Q", map(_address, tensors))
+
+
+def _at(a):
+    return a.buffer_info()[0] if a is not None else None
+
+
+def _current_device(tensors):
+    t = tensors[0]
+    if not t.is_cuda:
+        raise RuntimeError("tensors on the GPU only (got one on %s); there is no CPU path" % t.device)
+    return torch._C._cuda_getDevice()
+
+
+def grad_norm(tensors):
+    """
+    The root of the sum of squares of all entries of a list of tensors: the norm that gradients are clipped by.
+
+    :param tensors: float32, bfloat16 or float16 (also mixed), on the current GPU; copied where they are not contiguous
+    :return: float32, no axes, on the GPU: nothing waits for it.  Squares are summed in 64 bits and in an order of their own, so that the result is the
+        same every time
+    """
+    tensors = list(tensors)
+    if not tensors:
+        return torch.zeros((), device="cuda")
+    device = _current_device(tensors)
+    if not all(map(_contiguous, tensors)):
+        tensors = [t.contiguous() for t in tensors]
+    dtypes = set(map(_dtype, tensors))
+    if not dtypes <= _hip.FLOATS.keys():
+        raise RuntimeError("tensors of float32, bfloat16 or float16 only (got %s)" % ", ".join(sorted(map(str, dtypes))))
+    if set(map(_device, tensors)) != {device}:
+        raise RuntimeError("tensors on the current GPU only, cuda:%d" % device)
+    n, count = array("q", map(_numel, tensors)), len(tensors)
+    kinds = array("i", [_hip.FLOATS[d] for d in map(_dtype, tensors)]) if len(dtypes) > 1 else array("i", [_hip.FLOATS[tensors[0].dtype]]) * count
+    out = torch.empty((), dtype=torch.float32, device=tensors[0].device)
+    nbytes = _hip.lib().s2cnn_grad_norm_workspace(_at(n), _at(kinds), count)
+    ws = _hip.workspace(nbytes, out.device)
+    addresses = _addresses(tensors)
+    _hip.call("s2cnn_grad_norm", _at(addresses), _at(n), _at(kinds), count, out.data_ptr(), ws.data_ptr(), nbytes, _hip.stream_ptr())
+    return out
+
+
+def _check_states(first, second, scales, shapes, device):
+    """Moments in 32 bits (no scales) or 8 beside tensors of these shapes."""
+    assert len(first) == len(second) == len(shapes) and (scales is None or len(scales) == len(shapes))
+    _check_list(first, torch.float32 if scales is None else torch.float8_e4m3fn, device, "first moments")
+    _check_list(second, torch.float32 if scales is None else torch.uint8, device, "second moments")
+    assert list(map(_shape, first)) == shapes and list(map(_shape, second)) == shapes
+    if scales is not None:
+        _check_list(scales, torch.float32, device, "scales")
+        assert [tuple(t.shape) for t in scales] == [(-(-t.numel() // BLOCK), 2) for t in first]
+
+
+@torch.no_grad()
+def adamw_step(params, grads, first, second, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, masters=None, scales=None, norm=None,
+               max_norm=None, seed=0):
+    """
+    One step of AdamW on a list of tensors, in place:
+    m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2, p = p - lr weight_decay p - lr (m / (1 - b1^step)) / (sqrt(v / (1 - b2^step)) + eps).
+
+    :param params, grads: tensors of one type (float32, bfloat16 or float16) on the current GPU; parameters contiguous, none twice
+    :param first, second: the moments m and v, of the parameters' shapes: float32, or with scales float8_e4m3fn and uint8
+    :param step: which step it is, from 1 on: an int, or an int64 tensor of one element on the GPU that is read when the kernels run
+    :param lr: a number, or a float32 tensor of one element on the GPU
+    :param eps: >= 1e-30
+    :param masters: float32 copies of 16-bit parameters, or None: the step is made there, and the parameters are their roundings.  Where a parameter
+        is not (the program has set it since), the parameter counts
+    :param scales: [ceil(n / 256), 2] float32 for each tensor of n entries: the moments are held in 8 bits, with a factor of each for every
+        256 entries, and rounded at random so that their means are right (include/s2cnn_hip.h has the codes; `adamw_states` gives their values).  Zeros
+        in all three are moments of zero.  An infinite gradient, or one that is no number, makes all of its 256 entries' moments such
+    :param norm, max_norm: gradients are multiplied by min(1, max_norm / norm), norm as `grad_norm` gives it; both or none.  Where it is infinite or no
+        number nothing is written
+    :param seed: of the random rounding, an int; equal seeds and steps round equal lists alike
+    """
+    params, grads, first, second = list(params), list(grads), list(first), list(second)
+    masters, scales = (list(t) if t is not None else None for t in (masters, scales))
+    assert len(params) == len(grads)
+    assert 0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0 and 1e-30 <= eps < 1e30 and 0.0 <= weight_decay < 1e30
+    assert torch.is_tensor(lr) or 0.0 <= lr < 1e30
+    assert isinstance(seed, int)
+    assert step.numel() == 1 if torch.is_tensor(step) else isinstance(step, int) and step >= 1
+    assert not torch.is_tensor(lr) or lr.numel() == 1
+    assert (norm is None) == (max_norm is None)
+    if norm is not None:
+        assert norm.numel() == 1 and 0.0 < max_norm < 1e38
+    if not params:
+        assert not first and not second and not masters and not scales
+        return
+    dtype, device = params[0].dtype, _current_device(params)
+    if dtype not in _hip.FLOATS:
+        raise RuntimeError("float32, bfloat16 or float16 parameters only (got %s)" % dtype)
+    shapes = list(map(_shape, params))
+    _check_list(params, dtype, device, "parameters")
+    if not all(map(_contiguous, grads)):
+        grads = [g.contiguous() for g in grads]
+    _check_list(grads, dtype, device, "gradients")
+    assert list(map(_shape, grads)) == shapes
+    _check_states(first, second, scales, shapes, device)
+    if masters is not None:
+        assert dtype != torch.float32, "float32 parameters have no masters"
+        _check_list(masters, torch.float32, device, "masters")
+        assert list(map(_shape, masters)) == shapes
+    if torch.is_tensor(step):
+        _hip.require_gpu_of(torch.int64, step)
+    if torch.is_tensor(lr):
+        _hip.require_gpu_of(torch.float32, lr)
+    _hip.require_gpu_of(torch.float32, norm)
+
+    n = array("q", map(_numel, params))
+    lists = [_addresses(t) if t is not None else None for t in (params, grads, first, second, scales, masters)]
+    present = len(n) - n.count(0)
+    assert len(set(lists[0]) - {0}) == present, "a parameter twice in the list"
+    a = _hip.AdamW()
+    a.p, a.g, a.first, a.second, a.scales, a.masters = map(_at, lists)
+    a.n, a.count, a.dtype, a.bits = _at(n), len(n), _hip.FLOATS[dtype], 32 if scales is None else 8
+    if torch.is_tensor(step):
+        a.step_at = step.data_ptr()
+    else:
+        a.step = step
+    if torch.is_tensor(lr):
+        a.lr_at = lr.data_ptr()
+    else:
+        a.lr = lr
+    (a.beta1, a.beta2), a.eps, a.weight_decay, a.seed = betas, eps, weight_decay, seed & 0xFFFFFFFFFFFFFFFF
+    if norm is not None:
+        a.norm, a.max_norm = norm.data_ptr(), max_norm
+    _hip.call("s2cnn_adamw_step", ctypes.byref(a), _hip.stream_ptr())
+
+
+def adamw_states(first, second, scales):
+    """
+    The moments that are held in 8 bits, in float32: (list of first moments, list of second moments), of the shapes of the arguments.
+
+    :param first, second, scales: as for `adamw_step`
+    """
+    first, second, scales = list(first), list(second), list(scales)
+    if not first:
+        assert not second and not scales
+        return [], []
+    device = _current_device(first)
+    _check_states(first, second, scales, list(map(_shape, first)), device)
+    out = [[torch.empty(t.shape, dtype=torch.float32, device=t.device) for t in first] for _ in range(2)]
+    n = array("q", map(_numel, first))
+    lists = [_addresses(t) for t in (first, second, scales, *out)]
+    _hip.call("s2cnn_adamw_states", *map(_at, lists), _at(n), len(n), _hip.stream_ptr())
+    return tuple(out)
+
+
+class AdamW(torch.optim.Optimizer):
+    """
+    torch.optim.AdamW's steps by `adamw_step`: one launch for some fifty tensors, which a HIP graph may hold.
+
+    :param params: parameters or groups of them, float32, bfloat16 or float16, contiguous, on one GPU.  A group may have its own lr, betas, eps,
+        weight_decay, state_bits and masters
+    :param lr: a number, or a float32 tensor of one element on the GPU, which a captured step reads at every replay
+    :param state_bits: 32, or 8: two bytes a parameter for the moments instead of eight, and a thirty-second of one for their factors
+    :param masters: float32 copies of 16-bit parameters, in which small steps add up.  The program may set the parameters at any time (load a
+        state dict): where they are not their masters' roundings, they count
+    :param max_norm: gradients are clipped to this norm, of all groups together (`self.norm` is the norm of the last step, before it); a step whose norm is
+        infinite or no number is left out and not counted.  None: neither
+    :param seed: of the random rounding of moments in 8 bits; ranks of a job that hold the same parameters need the same
+
+    Steps are counted on the device, for every parameter those that it had a gradient in.  State dicts hold the moments as they are.
+    """
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, masters=True, max_norm=None, seed=0):
+        assert max_norm is None or 0.0 < max_norm < 1e38
+        assert isinstance(seed, int)
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, masters=masters))
+        self.max_norm, self.seed, self.norm = max_norm, seed, None
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        assert group["state_bits"] in (8, 32)
+        assert 0.0 <= group["betas"][0] < 1.0 and 0.0 <= group["betas"][1] < 1.0 and 1e-30 <= group["eps"] < 1e30 and 0.0 <= group["weight_decay"] < 1e30
+        assert torch.is_tensor(group["lr"]) and group["lr"].numel() == 1 or 0.0 <= group["lr"] < 1e30
+        for p in group["params"]:
+            if p.dtype not in _hip.FLOATS:
+                raise RuntimeError("float32, bfloat16 or float16 parameters only (got %s)" % p.dtype)
+
+    def _new_state(self, p, group, count):
+        state = {"step": count}
+        if group["state_bits"] == 8:
+            state["first"] = torch.zeros(p.shape, dtype=torch.uint8, device=p.device).view(torch.float8_e4m3fn)
+            state["second"] = torch.zeros(p.shape, dtype=torch.uint8, device=p.device)
+            state["scales"] = torch.zeros(-(-p.numel() // BLOCK), 2, device=p.device)
+        else:
+            state["first"], state["second"] = (torch.zeros(p.shape, device=p.device) for _ in range(2))
+        if group["masters"] and p.dtype != torch.float32:
+            state["master"] = p.detach().float().contiguous()
+        return state
+
+    def _lists(self, group):
+        """[(count of steps, parameters)] of a group's parameters that have a gradient, those of equal counts together, by type.  Parameters that were
+        stepped together so far share one count."""
+        members, stepped, fresh = {}, {}, {}
+        for p in group["params"]:
+            state = self.state[p] if p in self.state else None
+            if state:
+                members[id(state["step"])] = members.get(id(state["step"]), 0) + 1
+            if p.grad is None:
+                continue
+            if p.grad.is_sparse:
+                raise RuntimeError("AdamW takes no sparse gradients")
+            if not state:
+                key = p.device
+                if key not in fresh:
+                    fresh[key] = torch.zeros(1, dtype=torch.int64, device=p.device)
+                state = self.state[p] = self._new_state(p, group, fresh[key])
+                members[id(state["step"])] = members.get(id(state["step"]), 0) + 1
+            stepped.setdefault(id(state["step"]), []).append(p)
+        lists = []
+        for key, params in stepped.items():
+            count = self.state[params[0]]["step"]
+            if len(params) < members[key]:                               # some of them are left out of this step: from here on they count apart
+                count = count.clone()
+                for p in params:
+                    self.state[p]["step"] = count
+            lists.append((count, params))
+        return lists
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        """One step on all parameters that have a gradient; the loss of `closure`, if there is one."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        finite = None
+        if self.max_norm is not None:
+            self.norm = grad_norm([p.grad for group in self.param_groups for p in group["params"] if p.grad is not None])
+            finite = torch.isfinite(self.norm)
+        for group in self.param_groups:
+            for count, params in self._lists(group):
+                count.add_(1 if finite is None else finite)
+                for dtype in dict.fromkeys(map(_dtype, params)):
+                    some = [p for p in params if p.dtype == dtype]
+                    states = [self.state[p] for p in some]
+                    adamw_step(some, [p.grad for p in some], [s["first"] for s in states], [s["second"] for s in states], count, group["lr"], group["betas"],
+                               group["eps"], group["weight_decay"], [s["master"] for s in states] if "master" in states[0] else None,
+                               [s["scales"] for s in states] if "scales" in states[0] else None, self.norm if finite is not None else None,
+                               self.max_norm, self.seed)
+        return loss
+
+    def load_state_dict(self, state_dict):
+        """States keep their types (torch's own method takes them to the parameters')."""
+        super().load_state_dict(state_dict)
+        saved = [i for group in state_dict["param_groups"] for i in group["params"]]
+        params = [p for group in self.param_groups for p in group["params"]]
+        counts = {}
+        for i, p in zip(saved, params):
+            if i not in state_dict["state"]:
+                continue
+            state = {k: t.detach().to(p.device, copy=True) for k, t in state_dict["state"][i].items()}
+            count = (int(state["step"]), p.device)
+            state["step"] = counts.setdefault(count, state["step"])
+            self.state[p] = state
