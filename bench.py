@@ -472,24 +472,25 @@ def measure_fft_floor(torch, dev, nvol=256, reps=10):
             "frac_of_hbm_peak_shipped": round(2 * bytes_dir / ((full["s2cnn_so3_analysis"] + full["s2cnn_so3_synthesis"]) * 1e-6) / 1e9 / PEAK_HBM_GBS, 4)}
 
 
-def measure_example_network(torch, name, steps, warmup, batch=32):
+def measure_example_network(torch, name, steps, warmup, batch=32, optimizer="sgd"):
     """One of the reference's example networks (examples/mnist/run.py:55-98, examples/shrec17/model.py, model_original.py) in
-    its training step (forward, loss, backward, SGD with momentum) on a fixed synthetic batch; time inside library calls
-    listed beside the step time."""
+    its training step (forward, loss, backward, SGD with momentum or another optimizer of the harness) on a fixed synthetic batch; time
+    inside library calls listed beside the step time."""
     from s2cnn_amd import _hip, harness
     if name == "shrec17_original":
         batch = 16
-    model, losses, ms = harness.train_steps(name, batch=batch, steps=steps, warmup=warmup, lr=0.01)
+    lr = 0.01 if optimizer == "sgd" else 0.001
+    model, losses, ms = harness.train_steps(name, batch=batch, steps=steps, warmup=warmup, lr=lr, optimizer=optimizer)
     with _hip.KernelTimer() as kt:
-        harness.train_steps(name, batch=batch, steps=1, warmup=0, lr=0.01, model=model)
+        harness.train_steps(name, batch=batch, steps=1, warmup=0, lr=lr, optimizer=optimizer, model=model)
         torch.cuda.synchronize()
     calls = {k: round(sum(v), 3) for k, v in sorted(kt.summary().items(), key=lambda kv: -sum(kv[1]))}
-    out = {"workload": "%s training step (s2cnn_amd/harness.py), batch %d, synthetic data" % (name, batch),
+    out = {"workload": "%s training step (s2cnn_amd/harness.py), batch %d, synthetic data" % (name, batch), "optimizer": optimizer,
            "ms_per_step": round(ms, 3), "samples_per_s": round(batch / (ms * 1e-3), 1), "first_loss": round(losses[0], 4),
            "last_loss": round(losses[-1], 4), "library_ms": round(sum(calls.values()), 3), "library_calls_ms": calls}
-    if name in ("mnist", "sphere_transformer"):
+    if name in ("mnist", "sphere_transformer", "sphere_transformer_rotary"):
         # the same step captured into one HIP graph and replayed (the eager step is bound by its launches)
-        _, rlosses, rms = harness.train_steps_replayed(name, batch=batch, steps=max(steps, 20), warmup=3, lr=0.01)
+        _, rlosses, rms = harness.train_steps_replayed(name, batch=batch, steps=max(steps, 20), warmup=3, lr=lr, optimizer=optimizer)
         out["graph_replay"] = {"ms_per_step": round(rms, 3), "samples_per_s": round(batch / (rms * 1e-3), 1),
                                "first_loss": round(rlosses[0], 4), "last_loss": round(rlosses[-1], 4)}
     if name.startswith("shrec17"):
@@ -499,9 +500,9 @@ def measure_example_network(torch, name, steps, warmup, batch=32):
         torch.manual_seed(0)
         fused = harness.NETWORKS[name][0]()
         fused.fused_norm = True
-        model, flosses, fms = harness.train_steps(name, batch=batch, steps=steps, warmup=warmup, lr=0.01, model=fused)
+        model, flosses, fms = harness.train_steps(name, batch=batch, steps=steps, warmup=warmup, lr=lr, optimizer=optimizer, model=fused)
         with _hip.KernelTimer() as kt:
-            harness.train_steps(name, batch=batch, steps=1, warmup=0, lr=0.01, model=model)
+            harness.train_steps(name, batch=batch, steps=1, warmup=0, lr=lr, optimizer=optimizer, model=model)
             torch.cuda.synchronize()
         fcalls = {k: round(sum(v), 3) for k, v in sorted(kt.summary().items(), key=lambda kv: -sum(kv[1]))}
         out["fused_norm"] = {"ms_per_step": round(fms, 3), "samples_per_s": round(batch / (fms * 1e-3), 1),
@@ -513,7 +514,7 @@ def measure_example_network(torch, name, steps, warmup, batch=32):
         torch.manual_seed(0)
         fused = harness.NETWORKS[name][0]()
         fused.fused_norm = True
-        _, rlosses, rms = harness.train_steps_replayed(name, batch=batch, steps=steps, warmup=3, lr=0.01, model=fused)
+        _, rlosses, rms = harness.train_steps_replayed(name, batch=batch, steps=steps, warmup=3, lr=lr, optimizer=optimizer, model=fused)
         out["fused_norm"]["graph_replay"] = {"ms_per_step": round(rms, 3), "samples_per_s": round(batch / (rms * 1e-3), 1),
                                              "last_loss": round(rlosses[-1], 4)}
     return out
@@ -535,10 +536,12 @@ def main():
                     help="also time the per-volume 64^3 kernels with their Wigner contraction compiled out (adds a `fft_floor` object)")
     ap.add_argument("--overlap", action="store_true",
                     help="also time a transform and a product of half the layer's batch on one stream and on two (adds an `overlap` object)")
-    ap.add_argument("--network", nargs="?", const="config5", default=None, choices=["config5", "mnist", "shrec17", "shrec17_original", "sphere_transformer"],
+    ap.add_argument("--network", nargs="?", const="config5", default=None,
+                    choices=["config5", "mnist", "shrec17", "shrec17_original", "sphere_transformer", "sphere_transformer_rotary"],
                     help="also time a whole network, forward + backward (adds a `network` object): config5 = the SHREC17-shaped "
                          "network of benchmark config 5 (default); mnist, shrec17, shrec17_original = the reference's example "
                          "networks (s2cnn_amd/harness.py) in a training step with SGD on a synthetic batch of 32")
+    ap.add_argument("--optimizer", default="sgd", choices=["sgd", "adamw", "adamw_8bit"], help="of --network's training step (not of config5)")
     ap.add_argument("--batch", type=int, default=16)
     ap.add_argument("--b", type=int, default=32)
     ap.add_argument("--features", type=int, default=64)
@@ -673,7 +676,7 @@ def main():
     if args.network == "config5":
         result["network"] = measure_network(torch, dev, args.steps, args.warmup)
     elif args.network:
-        result["network"] = measure_example_network(torch, args.network, args.steps, args.warmup)
+        result["network"] = measure_example_network(torch, args.network, args.steps, args.warmup, optimizer=args.optimizer)
 
     # ---- CPU baseline: the oracle (a restatement of the reference's CPU branches) on a bounded sample
     if not args.no_cpu:

@@ -12,7 +12,8 @@ other (examples/shrec17/train.py:123 saves `model.state_dict()`, examples/shrec1
                                                             grid instead of the integral, BatchNorm1d in the output layer
 
   SphereTransformer    (not of the reference)               S2Conv 6->96 (b 64->10), ReLU, mean over gamma, two transformer blocks
-                                                            over the 400 points, attention pooling, Linear, log_softmax
+                                                            over the 400 points, attention pooling, Linear, log_softmax; "rotary":
+                                                            queries and keys normalised and turned by the points' places
 
 Data sets, loaders and logging of the reference's scripts are not reproduced: `train_steps` feeds a fixed synthetic batch.
 """
@@ -24,7 +25,7 @@ from torch import nn
 
 from .soft.bn_relu import evaluate_sequence, run_sequence
 from .soft.s2_transformer import Linear
-from . import (S2Convolution, S2Transformer, SO3Convolution, s2_equatorial_grid, s2_near_identity_grid, so3_equatorial_grid, so3_integrate,
+from . import (AdamW, S2Convolution, S2Transformer, SO3Convolution, s2_equatorial_grid, s2_near_identity_grid, so3_equatorial_grid, so3_integrate,
                so3_near_identity_grid)
 
 
@@ -113,14 +114,15 @@ class Shrec17ModelOriginal(nn.Module):
 class SphereTransformer(nn.Module):
     """Not of the reference: its first spectral layer, local features by correlation, then a transformer over the points of the
     sphere in place of further layers and of the integral.  S2Conv 6->96 (b 64->10, kernel about the identity), ReLU, the
-    mean over gamma (a signal on the sphere), two blocks of 6 heads with a bias by 32 buckets of the angle, pooling, Linear."""
+    mean over gamma (a signal on the sphere), two blocks of 6 heads with a bias by 32 buckets of the angle, pooling, Linear.
+    placed: queries and keys are normalised and turned by the places of the points."""
 
-    def __init__(self, nclasses, dropout=0.1, seed=0):
+    def __init__(self, nclasses, dropout=0.1, seed=0, placed=False):
         super().__init__()
         features, b_in, b = 96, 64, 10
         grid = s2_near_identity_grid(n_alpha=8, max_beta=0.2, n_beta=2)
         self.conv = S2Convolution(nfeature_in=6, nfeature_out=features, b_in=b_in, b_out=b, grid=grid, activation="relu")
-        self.transformer = S2Transformer(features, heads=6, b=b, layers=2, dropout=dropout, seed=seed)
+        self.transformer = S2Transformer(features, heads=6, b=b, layers=2, dropout=dropout, seed=seed, qk_norm=placed, rotary=placed)
         self.out_layer = Linear(features, nclasses)
 
     def forward(self, x):  # pylint: disable=W0221
@@ -134,6 +136,14 @@ NETWORKS = {
     "shrec17": (lambda: Shrec17Model(55), (6, 128, 128), 55, F.nll_loss),                  # examples/shrec17/train.py:70-82
     "shrec17_original": (lambda: Shrec17ModelOriginal(55), (6, 256, 256), 55, F.nll_loss),
     "sphere_transformer": (lambda: SphereTransformer(55), (6, 128, 128), 55, F.nll_loss),
+    "sphere_transformer_rotary": (lambda: SphereTransformer(55, placed=True), (6, 128, 128), 55, F.nll_loss),
+}
+
+OPTIMIZERS = {
+    # name: parameters and learning rate -> optimizer
+    "sgd": lambda params, lr: torch.optim.SGD(params, lr=lr, momentum=0.9),                # examples/shrec17/train.py:66
+    "adamw": lambda params, lr: AdamW(params, lr=lr, max_norm=1.0),
+    "adamw_8bit": lambda params, lr: AdamW(params, lr=lr, max_norm=1.0, state_bits=8),
 }
 
 
@@ -165,8 +175,8 @@ def smooth_spherical_batch(batch, channels, b, device, seed=0, lmax=16, noise=0.
     return flat.clamp_(0.0, 1.0 - 1e-7).view(batch, channels, 2 * b, 2 * b)
 
 
-def train_steps(name, batch=32, steps=10, warmup=2, lr=0.05, device="cuda:0", seed=0, model=None):
-    """`warmup + steps` SGD steps (momentum 0.9, as examples/shrec17/train.py:66) on one synthetic batch.
+def train_steps(name, batch=32, steps=10, warmup=2, lr=0.05, device="cuda:0", seed=0, model=None, optimizer="sgd"):
+    """`warmup + steps` steps on one synthetic batch, of SGD (momentum 0.9, as examples/shrec17/train.py:66) or another of OPTIMIZERS.
     Returns (model, losses of all steps, milliseconds per timed step)."""
     ctor, _, _, loss_fn = NETWORKS[name]
     torch.manual_seed(seed)
@@ -175,7 +185,7 @@ def train_steps(name, batch=32, steps=10, warmup=2, lr=0.05, device="cuda:0", se
     model = model.to(device)
     model.train()
     x, y = synthetic_batch(name, batch, device, seed)
-    opt = torch.optim.SGD(model.parameters(), lr=lr, momentum=0.9)
+    opt = OPTIMIZERS[optimizer](model.parameters(), lr)
     losses = []
 
     def step():
@@ -196,9 +206,9 @@ def train_steps(name, batch=32, steps=10, warmup=2, lr=0.05, device="cuda:0", se
     return model, [float(l) for l in losses], ms
 
 
-def train_steps_replayed(name, batch=32, steps=10, warmup=3, lr=0.05, device="cuda:0", seed=0, model=None):
+def train_steps_replayed(name, batch=32, steps=10, warmup=3, lr=0.05, device="cuda:0", seed=0, model=None, optimizer="sgd"):
     """The step of `train_steps` captured once into a HIP graph (torch.cuda.graph) and replayed `steps` times: nothing on
-    the path allocates through HIP, synchronises or records a memset, so the whole step (forward, loss, backward, SGD
+    the path allocates through HIP, synchronises or records a memset, so the whole step (forward, loss, backward,
     update) is one graph launch; for the small networks, whose step is bound by launches, that is most of the time.
     Returns (model, losses of the replayed steps, milliseconds per replayed step)."""
     ctor, _, _, loss_fn = NETWORKS[name]
@@ -208,7 +218,7 @@ def train_steps_replayed(name, batch=32, steps=10, warmup=3, lr=0.05, device="cu
     model = model.to(device)
     model.train()
     x, y = synthetic_batch(name, batch, device, seed)
-    opt = torch.optim.SGD(model.parameters(), lr=lr, momentum=0.9)
+    opt = OPTIMIZERS[optimizer](model.parameters(), lr)
 
     def step():
         opt.zero_grad(set_to_none=True)
@@ -220,7 +230,7 @@ def train_steps_replayed(name, batch=32, steps=10, warmup=3, lr=0.05, device="cu
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
-        for _ in range(max(warmup, 3)):     # tables, workspaces, momentum buffers and allocator pools exist before the capture
+        for _ in range(max(warmup, 3)):     # tables, workspaces, the optimizer's states and allocator pools exist before the capture
             step()
     torch.cuda.current_stream().wait_stream(side)
     torch.cuda.synchronize()

@@ -15,6 +15,7 @@ from torch import nn
 from .. import _hip
 from ..attention import attention, s2_angle_buckets, s2_log_weights
 from ..layer_norm import column_sums, dropout_add_layer_norm, layer_norm
+from ..rotary import norm_rotary, rotary as turned, s2_rotary_table
 from ..s2_grid import s2_soft_grid
 
 
@@ -82,17 +83,30 @@ class _PointWeights(nn.Module):
         return self.bits.view(torch.float32)
 
 
+class _PointTurns(_PointWeights):
+    """Cosines and sines of the points' rotations, float32 in the same way."""
+
+    def __init__(self, b, pairs):
+        nn.Module.__init__(self)
+        self.register_buffer("bits", s2_rotary_table(b, pairs).view(torch.int32), persistent=False)
+
+
 class S2TransformerBlock(nn.Module):
     """Attention over the 4 b^2 points of the 2b x 2b grid and a pointwise network, each with a residual and a normalisation
     before it.  Between the sublayers the residual, the dropout and the next normalisation are one pass over the features.
 
     The block takes and gives the pair (h, y): the residual stream, and its normalisation by the block's first norm.  `norm`
     makes the first pair of a stack; the last normalisation of a block is that of the block after it (`next_norm`).
+
+    qk_norm: the queries and keys of each head are normalised, with a learned weight, before their products.  rotary: they are turned by the places of
+    the points (`s2_rotary_table`), so that scores depend on the direction from one point to another too, along the circles of latitude and
+    across them; rotations about the polar axis still permute the points of a ring, others no longer commute with the block.
     """
 
-    def __init__(self, features, heads, b, n_buckets=32, max_angle=math.pi, hidden=None, dropout=0.0):
+    def __init__(self, features, heads, b, n_buckets=32, max_angle=math.pi, hidden=None, dropout=0.0, qk_norm=False, rotary=False):
         super().__init__()
         assert features % heads == 0
+        assert not rotary or features // heads >= 2
         self.features, self.heads, self.b, self.dropout = features, heads, b, dropout
         hidden = 2 * features if hidden is None else hidden
         self.norm1, self.norm2 = _Norm(features), _Norm(features)
@@ -101,6 +115,17 @@ class S2TransformerBlock(nn.Module):
         self.bias_table = nn.Parameter(torch.zeros(heads, n_buckets))
         self.register_buffer("buckets", s2_angle_buckets(s2_soft_grid(b), n_buckets=n_buckets, max_angle=max_angle), persistent=False)
         self.log_weights = _PointWeights(b)
+        self.qk_norm = qk_norm
+        if qk_norm:
+            self.q_weight, self.k_weight = (nn.Parameter(torch.ones(features // heads)) for _ in range(2))
+        self.turns = _PointTurns(b, features // heads // 2) if rotary else None
+
+    def _placed(self, q, k):
+        """Queries and keys as the attention takes them."""
+        table = self.turns() if self.turns is not None else None
+        if self.qk_norm:
+            return norm_rotary(q, k, self.q_weight.to(q.dtype), self.k_weight.to(q.dtype), table)
+        return (q, k) if table is None else turned(q, k, table)
 
     def norm(self, h):
         """(h, y) of the residual stream h [batch, points, features]"""
@@ -115,6 +140,7 @@ class S2TransformerBlock(nn.Module):
         batch, points, features = h.shape
         assert points == 4 * self.b ** 2
         q, k, v = self.qkv(y).view(batch, points, 3, self.heads, features // self.heads).permute(2, 0, 3, 1, 4)
+        q, k = self._placed(q, k)
         x = attention(q, k, v, table=self.bias_table.to(q.dtype), buckets=self.buckets, key_bias=self.log_weights())
         x = self.out(x.transpose(1, 2).reshape(batch, points, features))
         h, y = self._step(x, h, seeds[0], self.norm2)
@@ -151,11 +177,14 @@ class S2Transformer(nn.Module):
 
     What is dropped is a function of `seed` and of the count alone, not of torch's generator: stacks of one network, the ranks of a
     data-parallel job and runs that are to differ need a `seed` each (`torch.initial_seed() + rank`, say).  Its low 32 bits count, and stacks
-    in which they differ never use the same number.  It is the program's to keep, as the learning rate is: no part of the state dict."""
+    in which they differ never use the same number.  It is the program's to keep, as the learning rate is: no part of the state dict.
 
-    def __init__(self, features, heads, b, layers, n_buckets=32, max_angle=math.pi, dropout=0.0, seed=0):
+    qk_norm, rotary: of the blocks."""
+
+    def __init__(self, features, heads, b, layers, n_buckets=32, max_angle=math.pi, dropout=0.0, seed=0, qk_norm=False, rotary=False):
         super().__init__()
-        self.blocks = nn.ModuleList(S2TransformerBlock(features, heads, b, n_buckets, max_angle, dropout=dropout) for _ in range(layers))
+        self.blocks = nn.ModuleList(S2TransformerBlock(features, heads, b, n_buckets, max_angle, dropout=dropout, qk_norm=qk_norm, rotary=rotary)
+                                    for _ in range(layers))
         self.last_norm = _Norm(features)
         self.pool = S2AttentionPool(features, heads, b)
         self.register_buffer("drops", torch.zeros(1, dtype=torch.int64))
