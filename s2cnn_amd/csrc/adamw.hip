@@ -4,9 +4,9 @@
 //
 // with g multiplied by min(1, max_norm / norm) first where a norm is given.  Bound by memory: every tensor is read once and written once, in one
 // launch for some fifty tensors, whose addresses travel in the kernel's arguments: nothing is copied to the device, and a captured graph keeps them.
-// A workgroup takes 4096 entries of one tensor, a wave 256 at a time, four a lane.
+// A workgroup takes 2048 entries of one tensor, four or eight a lane at a time.
 //
-// Moments in 8 bits.  A block of 256 entries (a wave's) has a factor s of each moment; an entry is s f(c), f(c) = c for c < 8, (8 + c % 8) 2^(c / 8 - 1)
+// Moments in 8 bits.  A block of 256 entries (32 lanes') has a factor s of each moment; an entry is s f(c), f(c) = c for c < 8, (8 + c % 8) 2^(c / 8 - 1)
 // beyond: three bits after the leading one, so that a step is 1/8 to 1/16 of the value.  First moments: a sign and c <= 126, in units of 2^-9
 // the type float8_e4m3fn.  Second moments: c <= 255, 2^34 from the smallest to the largest, because their roots go through the same range as
 // first moments do, and never 0 where the moment is not: the quotient stays bounded.  A step changes a second moment by a thousandth
@@ -21,7 +21,7 @@ namespace adamw {
 
 constexpr int THREADS = 256;
 constexpr int BLOCK = 256;                     // entries of a factor
-constexpr int PART = 4096;                     // entries of a workgroup
+constexpr int PART = 2048;                     // entries of a workgroup
 constexpr int MOST = 56;                       // tensors of a launch: 4 KB of arguments
 constexpr int MOST_SUMS = 184;
 constexpr float TOP_FIRST = 229376.f, TOP_SECOND = 15.f * 1073741824.f;      // f(126), f(255)
@@ -43,8 +43,7 @@ struct Step {
   const long long* step_at;
   long long step;
   unsigned long long seed;
-  double log_b1, log_b2;
-  float lr, b1, rest1, b2, rest2, eps, decay, max_norm;
+  float log_b1, log_b2, lr, b1, rest1, b2, rest2, eps, decay, max_norm;
 };
 static_assert(sizeof(Tensors) + sizeof(Step) <= 4096, "kernel arguments");
 
@@ -59,81 +58,75 @@ template <int N> __device__ __forceinline__ int tensor_of(const unsigned (&first
   return low;
 }
 
-// Four entries at any address of the type, the first n of them
-template <class T> __device__ __forceinline__ void load4(const T* p, long n, float (&v)[4]) {
-  if (n >= 4) {
-    if constexpr (sizeof(T) == 4) {
-      typedef float loose __attribute__((ext_vector_type(4), aligned(4)));
-      const loose x = *reinterpret_cast<const loose*>(p);
+// N entries at any address of the type; not FULL: the first n of them, the others zero
+template <bool FULL, class T, int N> __device__ __forceinline__ void load(const T* p, long n, float (&v)[N]) {
+  if (FULL || n >= N) {
+    typedef T loose __attribute__((ext_vector_type(sizeof(T) == 4 ? 4 : N), aligned(sizeof(T))));
+    constexpr int M = sizeof(T) == 4 ? 4 : N;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = x[i];
-    } else {
-      typedef T loose __attribute__((ext_vector_type(4), aligned(2)));
-      const loose x = *reinterpret_cast<const loose*>(p);
+    for (int k = 0; k < N / M; ++k) {
+      const loose x = *reinterpret_cast<const loose*>(p + k * M);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = (float)x[i];
+      for (int i = 0; i < M; ++i) v[k * M + i] = (float)x[i];
     }
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = i < n ? (float)p[i] : 0.f;
+  for (int i = 0; i < N; ++i) v[i] = i < n ? (float)p[i] : 0.f;
 }
-template <class T> __device__ __forceinline__ void store4(T* p, long n, const float (&v)[4]) {
-  if (n >= 4) {
-    typedef T loose __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-    *reinterpret_cast<loose*>(p) = loose{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+template <bool FULL, class T, int N> __device__ __forceinline__ void store(T* p, long n, const float (&v)[N]) {
+  if (FULL || n >= N) {
+    constexpr int M = sizeof(T) == 4 ? 4 : N;
+    typedef T loose __attribute__((ext_vector_type(M), aligned(sizeof(T))));
+#pragma unroll
+    for (int k = 0; k < N / M; ++k) {
+      loose x;
+#pragma unroll
+      for (int i = 0; i < M; ++i) x[i] = (T)v[k * M + i];
+      *reinterpret_cast<loose*>(p + k * M) = x;
+    }
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < N; ++i)
     if (i < n) p[i] = (T)v[i];
 }
-typedef unsigned loose_bytes __attribute__((aligned(1)));
-__device__ __forceinline__ unsigned load4(const unsigned char* p, long n) {
-  if (n >= 4) return *reinterpret_cast<const loose_bytes*>(p);
-  unsigned c = 0;
+// eight bytes in the same way
+typedef unsigned loose2 __attribute__((ext_vector_type(2), aligned(1)));
+template <bool FULL> __device__ __forceinline__ uint2 load8(const unsigned char* p, long n) {
+  if (FULL || n >= 8) {
+    const loose2 x = *reinterpret_cast<const loose2*>(p);
+    return make_uint2(x[0], x[1]);
+  }
+  unsigned c[2] = {0, 0};
 #pragma unroll
-  for (int i = 0; i < 3; ++i)
-    if (i < n) c |= (unsigned)p[i] << (8 * i);
-  return c;
+  for (int i = 0; i < 7; ++i)
+    if (i < n) c[i / 4] |= (unsigned)p[i] << (8 * (i % 4));
+  return make_uint2(c[0], c[1]);
 }
-__device__ __forceinline__ void store4(unsigned char* p, long n, unsigned c) {
-  if (n >= 4) {
-    *reinterpret_cast<loose_bytes*>(p) = c;
+template <bool FULL> __device__ __forceinline__ void store8(unsigned char* p, long n, uint2 c) {
+  if (FULL || n >= 8) {
+    *reinterpret_cast<loose2*>(p) = loose2{c.x, c.y};
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 3; ++i)
-    if (i < n) p[i] = (unsigned char)(c >> (8 * i));
+  for (int i = 0; i < 7; ++i)
+    if (i < n) p[i] = (unsigned char)((i < 4 ? c.x : c.y) >> (8 * (i % 4)));
 }
 
 // ---- codes ----------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ void first_of(unsigned c, float s, float (&m)[4]) {
-  const f2 low = __builtin_amdgcn_cvt_pk_f32_fp8(c, false), high = __builtin_amdgcn_cvt_pk_f32_fp8(c, true);
-  m[0] = low[0] * 512.f * s, m[1] = low[1] * 512.f * s, m[2] = high[0] * 512.f * s, m[3] = high[1] * 512.f * s;
-}
-__device__ __forceinline__ void second_of(unsigned codes, float s, float (&v)[4]) {
+__device__ __forceinline__ void first_of(uint2 codes, float s, float (&m)[8]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const unsigned c = (codes >> (8 * i)) & 255u;
-    v[i] = (c < 8 ? (float)c : __uint_as_float((c << 20) + (129u << 23))) * s;
+  for (int k = 0; k < 2; ++k) {
+    const unsigned c = k ? codes.y : codes.x;
+    const f2 low = __builtin_amdgcn_cvt_pk_f32_fp8(c, false), high = __builtin_amdgcn_cvt_pk_f32_fp8(c, true);
+    m[4 * k] = low[0] * 512.f * s, m[4 * k + 1] = low[1] * 512.f * s, m[4 * k + 2] = high[0] * 512.f * s, m[4 * k + 3] = high[1] * 512.f * s;
   }
 }
-// The code of y >= 0, rounded by 16 random bits: where y >= 8, the bits of the float32 with those added behind the three that stay.
-__device__ __forceinline__ unsigned code_of(float y, unsigned random, unsigned most) {
-  const unsigned high = ((__float_as_uint(y) + (random << 4)) >> 20) - (129u << 3), low = (unsigned)floorf(y + (float)random * 0x1p-16f);
-  return min(y >= 8.f ? high : low, most);
-}
-__device__ __forceinline__ unsigned max_wave(unsigned v) {           // in all 64 lanes
-  const auto with = [&](unsigned o) { v = max(v, o); };
-  with(__builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, true));
-  with(__builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, true));
-  with(__builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true));
-  with(__builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, true));
-  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-  v = max(a[0], a[1]);
-  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-  return max(b[0], b[1]);
+// f(c) 2^-129 is the float32 of bits c 2^20: the codes below eight are its subnormal numbers, and the product with 2^127 is exact.
+__device__ __forceinline__ void second_of(uint2 codes, float s, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float((((i < 4 ? codes.x : codes.y) >> (8 * (i % 4))) & 255u) << 20) * 0x1p127f * (4.f * s);
 }
 // A block's factor from its largest entry (the bits of a float32 without sign, so that what is no number is the largest); below 2^-126 none.
 __device__ __forceinline__ float factor_of(unsigned largest, float inverse_top) {
@@ -141,78 +134,137 @@ __device__ __forceinline__ float factor_of(unsigned largest, float inverse_top) 
   const float s = __uint_as_float(largest) * inverse_top;
   return s < 0x1p-126f ? 0.f : s;
 }
+__device__ __forceinline__ unsigned max_block(unsigned v) {           // over 32 lanes, in all of them
+  const auto with = [&](unsigned o) { v = max(v, o); };
+  with(__builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, true));
+  with(__builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, true));
+  with(__builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true));
+  with(__builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, true));
+  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  return max(a[0], a[1]);
+}
+// The code of y >= 0, rounded by 16 random bits, in the upper byte.  From 8 on it is in the bits of the float32 with those added behind the three that
+// stay.  No code is above that of the largest entry, which is off by less than 2^-21 of itself from its code's value: 2^-17 of a spacing, less than what
+// the largest random number leaves.
+__device__ __forceinline__ unsigned upper_code(float y, unsigned random) { return (__float_as_uint(y) + ((random << 4) - (129u << 23))) << 4; }
+__device__ __forceinline__ unsigned any_code(float y, unsigned random) {
+  return y >= 8.f ? upper_code(y, random) >> 24 : (unsigned)(y + (float)random * 0x1p-16f);
+}
+// the upper bytes of four words
+__device__ __forceinline__ unsigned upper_bytes(const unsigned (&x)[4]) {
+  const unsigned low = __builtin_amdgcn_perm(x[1], x[0], 0x0c0c0703u), high = __builtin_amdgcn_perm(x[3], x[2], 0x07030c0cu);
+  return low | high;
+}
+
+// Eight entries of a block of 256, whose factors' inverses are i1 and i2: codes of m and v.
+__device__ __forceinline__ void codes_of(const float (&m)[8], const float (&v)[8], float i1, float i2, const uint4 (&random)[2], uint2& c1, uint2& c2) {
+#pragma clang fp contract(off)
+  float a[8], b[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) a[i] = fabsf(m[i]) * i1, b[i] = v[i] * i2;
+  const unsigned r[8] = {random[0].x, random[0].y, random[0].z, random[0].w, random[1].x, random[1].y, random[1].z, random[1].w};
+  unsigned x[2][4], y[2][4];
+  bool high = true;                                                // all from 8 on; what is no number is not
+#pragma unroll
+  for (int i = 0; i < 8; ++i) high &= a[i] >= 8.f && b[i] >= 8.f;
+  if (__all(high)) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[i / 4][i % 4] = (upper_code(a[i], r[i] & 0xffffu) & 0x7fffffffu) | (__float_as_uint(m[i]) & 0x80000000u);
+      y[i / 4][i % 4] = upper_code(b[i], r[i] >> 16);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[i / 4][i % 4] = (any_code(a[i], r[i] & 0xffffu) | (m[i] < 0.f ? 128u : 0u)) << 24;
+      y[i / 4][i % 4] = max(any_code(b[i], r[i] >> 16), v[i] > 0.f && i2 > 0.f ? 1u : 0u) << 24;
+    }
+  }
+  c1 = make_uint2(upper_bytes(x[0]), upper_bytes(x[1]));
+  c2 = make_uint2(upper_bytes(y[0]), upper_bytes(y[1]));
+}
+
+struct Factors {
+  long long step;
+  float clip, size, inverse2, decay;
+};
+
+// The entries of a lane from `at` on, N of them; not FULL: the first `left`.
+template <class T, int BITS, bool MASTER, bool FULL> __device__ __forceinline__ void step_entries(const Tensors& t, int k, const Step& h, const Factors& f, long at, long left) {
+  constexpr int N = BITS == 8 ? 8 : 4;
+  float g[N], p[N], m[N], v[N], master[N];
+  load<FULL, T>(static_cast<const T*>(t.g[k]) + at, left, g);
+  load<FULL, T>(static_cast<T*>(t.p[k]) + at, left, p);
+  if constexpr (MASTER) load<FULL, float>(t.master[k] + at, left, master);
+  const long block = at / BLOCK;                                    // 8 bits: of 32 lanes
+  if constexpr (BITS == 32) {
+    load<FULL, float>(static_cast<float*>(t.first[k]) + at, left, m);
+    load<FULL, float>(static_cast<float*>(t.second[k]) + at, left, v);
+  } else {
+    const float2 s = FULL || left > 0 ? t.scales[k][block] : make_float2(0.f, 0.f);
+    const uint2 c1 = load8<FULL>(static_cast<unsigned char*>(t.first[k]) + at, left), c2 = load8<FULL>(static_cast<unsigned char*>(t.second[k]) + at, left);
+    first_of(c1, s.x, m);
+    second_of(c2, s.y, v);
+  }
+  {
+#pragma clang fp contract(off)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      g[i] *= f.clip;
+      m[i] = m[i] * h.b1 + g[i] * h.rest1;
+      v[i] = v[i] * h.b2 + (g[i] * g[i]) * h.rest2;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if constexpr (MASTER) p[i] = (float)(T)master[i] == p[i] ? master[i] : p[i];     // where it is not its master's rounding, the program has set it since
+    const float denominator = __builtin_amdgcn_sqrtf(v[i] * f.inverse2) + h.eps;
+    p[i] = fmaf(-f.size, m[i] * __builtin_amdgcn_rcpf(denominator), fmaf(-f.decay, p[i], p[i]));
+    // The parameter is the rounding of the float32 that is stored: without this the compiler makes one operation of the last product, sum and conversion
+    // to float16, which rounds once and may differ.
+    if constexpr (MASTER) asm volatile("" : "+v"(p[i]));
+  }
+  store<FULL, T>(static_cast<T*>(t.p[k]) + at, left, p);
+  if constexpr (MASTER) store<FULL, float>(t.master[k] + at, left, p);
+  if constexpr (BITS == 32) {
+    store<FULL, float>(static_cast<float*>(t.first[k]) + at, left, m);
+    store<FULL, float>(static_cast<float*>(t.second[k]) + at, left, v);
+  } else {
+    unsigned top1 = 0, top2 = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) top1 = max(top1, __float_as_uint(m[i]) & 0x7fffffffu), top2 = max(top2, __float_as_uint(v[i]) & 0x7fffffffu);
+    const float s1 = factor_of(max_block(top1), (float)(1.0 / TOP_FIRST)), s2 = factor_of(max_block(top2), (float)(1.0 / TOP_SECOND));
+    const float i1 = s1 == 0.f ? 0.f : 1.f / s1, i2 = s2 == 0.f ? 0.f : 1.f / s2;
+    const unsigned long long counter = t.counter[k] + (unsigned long long)(at >> 2);
+    const uint4 random[2] = {philox(counter, h.seed, (unsigned long long)f.step), philox(counter + 1, h.seed, (unsigned long long)f.step)};
+    uint2 c1, c2;
+    codes_of(m, v, i1, i2, random, c1, c2);
+    store8<FULL>(static_cast<unsigned char*>(t.first[k]) + at, left, c1);
+    store8<FULL>(static_cast<unsigned char*>(t.second[k]) + at, left, c2);
+    if ((threadIdx.x & 31) == 0 && (FULL || left > 0)) t.scales[k][block] = make_float2(s1, s2);
+  }
+}
 
 template <class T, int BITS, bool MASTER> __global__ __launch_bounds__(THREADS) void step_kernel(Tensors t, Step h) {
+  constexpr int N = BITS == 8 ? 8 : 4, WAVE = 64 * N;
   const int k = tensor_of(t.part, t.count, blockIdx.x);
-  float clip = 1.f;
+  Factors f;
+  f.clip = 1.f;
   if (h.norm) {
     const float norm = *h.norm;
     if (!(norm < __builtin_inff())) return;                         // infinite, or no number: the step is left out
-    clip = fminf(h.max_norm / norm, 1.f);
+    f.clip = fminf(h.max_norm / norm, 1.f);
   }
-  const long long step = h.step_at ? *h.step_at : h.step;
+  f.step = h.step_at ? *h.step_at : h.step;
   const float lr = h.lr_at ? *h.lr_at : h.lr;
-  const float size = lr / -expm1f((float)((double)step * h.log_b1)), inverse2 = 1.f / -expm1f((float)((double)step * h.log_b2)), decay = lr * h.decay;
+  // 1 - b^t = -expm1(t log b): the product's rounding is one of t log b e^(t log b) relative to 1 - b^t, at most its own
+  f.size = lr / -expm1f((float)f.step * h.log_b1), f.inverse2 = 1.f / -expm1f((float)f.step * h.log_b2), f.decay = lr * h.decay;
   const long n = t.n[k];
-  const int lane = threadIdx.x & 63;
-  const long start = (long)(blockIdx.x - t.part[k]) * PART + (threadIdx.x >> 6) * BLOCK;
-
-#pragma unroll 2
-  for (int turn = 0; turn < PART / (4 * BLOCK); ++turn) {
-    const long block = start + (long)turn * 4 * BLOCK, at = block + lane * 4, left = n - at;
-    if (block >= n) break;
-    float g[4], p[4], m[4], v[4], master[4];
-    load4<T>(static_cast<const T*>(t.g[k]) + at, left, g);
-    load4<T>(static_cast<T*>(t.p[k]) + at, left, p);
-    if constexpr (MASTER) load4<float>(t.master[k] + at, left, master);
-    if constexpr (BITS == 32) {
-      load4<float>(static_cast<float*>(t.first[k]) + at, left, m);
-      load4<float>(static_cast<float*>(t.second[k]) + at, left, v);
-    } else {
-      const float2 s = t.scales[k][block / BLOCK];
-      first_of(load4(static_cast<unsigned char*>(t.first[k]) + at, left), s.x, m);
-      second_of(load4(static_cast<unsigned char*>(t.second[k]) + at, left), s.y, v);
-    }
-    {
-#pragma clang fp contract(off)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        g[i] *= clip;
-        m[i] = m[i] * h.b1 + g[i] * h.rest1;
-        v[i] = v[i] * h.b2 + (g[i] * g[i]) * h.rest2;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      // where the parameter is not its master's rounding, the program has set it since
-      const float x = MASTER && (float)(T)master[i] == p[i] ? master[i] : p[i];
-      const float denominator = __builtin_amdgcn_sqrtf(v[i] * inverse2) + h.eps;
-      p[i] = fmaf(-size, m[i] * __builtin_amdgcn_rcpf(denominator), fmaf(-decay, x, x));
-    }
-    store4<T>(static_cast<T*>(t.p[k]) + at, left, p);
-    if constexpr (MASTER) store4<float>(t.master[k] + at, left, p);
-    if constexpr (BITS == 32) {
-      store4<float>(static_cast<float*>(t.first[k]) + at, left, m);
-      store4<float>(static_cast<float*>(t.second[k]) + at, left, v);
-    } else {
-#pragma clang fp contract(off)
-      unsigned top1 = 0, top2 = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) top1 = max(top1, __float_as_uint(fabsf(m[i]))), top2 = max(top2, __float_as_uint(fabsf(v[i])));
-      const float s1 = factor_of(max_wave(top1), (float)(1.0 / TOP_FIRST)), s2 = factor_of(max_wave(top2), (float)(1.0 / TOP_SECOND));
-      const float i1 = s1 == 0.f ? 0.f : 1.f / s1, i2 = s2 == 0.f ? 0.f : 1.f / s2;
-      const uint4 r = philox(t.counter[k] + (unsigned long long)(at >> 2), h.seed, (unsigned long long)step);
-      const unsigned random[4] = {r.x, r.y, r.z, r.w};
-      unsigned c1 = 0, c2 = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        c1 |= (code_of(fabsf(m[i]) * i1, random[i] & 0xffffu, 126u) | (m[i] < 0.f ? 128u : 0u)) << (8 * i);
-        c2 |= max(code_of(v[i] * i2, random[i] >> 16, 255u), v[i] > 0.f && i2 > 0.f ? 1u : 0u) << (8 * i);
-      }
-      store4(static_cast<unsigned char*>(t.first[k]) + at, left, c1);
-      store4(static_cast<unsigned char*>(t.second[k]) + at, left, c2);
-      if (lane == 0) t.scales[k][block / BLOCK] = make_float2(s1, s2);
-    }
+  const long start = (long)(blockIdx.x - t.part[k]) * PART + (threadIdx.x >> 6) * WAVE;
+  for (int turn = 0; turn < PART / (THREADS * N); ++turn) {
+    const long first = start + (long)turn * THREADS * N, at = first + (threadIdx.x & 63) * N;
+    if (first + WAVE <= n) step_entries<T, BITS, MASTER, true>(t, k, h, f, at, N);          // all loads under way together
+    else if (first < n) step_entries<T, BITS, MASTER, false>(t, k, h, f, at, n - at);
   }
 }
 
@@ -220,17 +272,17 @@ template <class T, int BITS, bool MASTER> __global__ __launch_bounds__(THREADS) 
 __global__ __launch_bounds__(THREADS) void states_kernel(Tensors t) {
   const int k = tensor_of(t.part, t.count, blockIdx.x);
   const long n = t.n[k];
-  const long start = (long)(blockIdx.x - t.part[k]) * PART + threadIdx.x * 4;
+  const long start = (long)(blockIdx.x - t.part[k]) * PART + threadIdx.x * 8;
 #pragma unroll
-  for (int turn = 0; turn < PART / (4 * THREADS); ++turn) {
-    const long at = start + turn * 4 * THREADS, left = n - at;
+  for (int turn = 0; turn < PART / (8 * THREADS); ++turn) {
+    const long at = start + turn * 8 * THREADS, left = n - at;
     if (left <= 0) break;
     const float2 s = t.scales[k][at / BLOCK];
-    float m[4], v[4];
-    first_of(load4(static_cast<unsigned char*>(t.first[k]) + at, left), s.x, m);
-    second_of(load4(static_cast<unsigned char*>(t.second[k]) + at, left), s.y, v);
-    store4<float>(static_cast<float*>(t.p[k]) + at, left, m);
-    store4<float>(t.master[k] + at, left, v);
+    float m[8], v[8];
+    first_of(load8<false>(static_cast<unsigned char*>(t.first[k]) + at, left), s.x, m);
+    second_of(load8<false>(static_cast<unsigned char*>(t.second[k]) + at, left), s.y, v);
+    store<false, float>(static_cast<float*>(t.p[k]) + at, left, m);
+    store<false, float>(t.master[k] + at, left, v);
   }
 }
 
@@ -368,7 +420,7 @@ extern "C" int s2cnn_adamw_step(const s2cnn_adamw_t* a, void* stream) {
     Step h;
     hipStream_t s;
   } with = {a,
-            {a->lr_at, a->norm, a->step_at, a->step, a->seed, __builtin_log(a->beta1), __builtin_log(a->beta2), (float)a->lr, (float)a->beta1, (float)(1.0 - a->beta1),
+            {a->lr_at, a->norm, a->step_at, a->step, a->seed, (float)__builtin_log(a->beta1), (float)__builtin_log(a->beta2), (float)a->lr, (float)a->beta1, (float)(1.0 - a->beta1),
              (float)a->beta2, (float)(1.0 - a->beta2), (float)a->eps, (float)a->weight_decay, (float)a->max_norm},
             static_cast<hipStream_t>(stream)};
   for_parts(

@@ -35,19 +35,18 @@ __device__ __forceinline__ unsigned divide(unsigned x, const Divider& d, unsigne
   return q;
 }
 
-struct Tensor {                  // vectors of a tensor: entries between those of consecutive inner, middle and outer numbers
+struct Tensor {                  // vectors of a tensor: entries from head to head, place to place, signal to signal
   const void* at;
-  long inner, middle, outer;
+  long head, place, batch;
 };
 struct Side {                    // queries, or keys
-  Tensor x, g;
-  void* y;
-  long y_inner, y_middle, y_outer;
+  Tensor x, g, y;
   const void* weight;
   float* partial;                // [workgroups, d]
-  Divider inner, middle;
-  unsigned vectors;
-  int heads_inside;              // the inner number is the head (else the place)
+  Divider inner, middle;         // of an item's number: runs of heads and places, or the other way round
+  unsigned items;                // runs of `run` heads at a place
+  int heads, run;
+  int heads_inside;
 };
 struct Args {
   Side side[2];
@@ -64,10 +63,11 @@ struct Part {
   int a, b, na, nb;              // first entries and numbers of entries of its two chunks
   int skip_a, skip_b;            // leading entries that belong to another lane as well
   int pair;                      // the pair of the first entry
+  bool own;                      // not: another lane's part once more, so that all lanes do the same
 };
 template <int V, bool NEIGHBOURS> __device__ __forceinline__ Part part_of(int u, int units, int d, int pairs) {
-  Part p = {0, 0, 0, 0, 0, 0, pairs};
-  if (u >= units) return p;
+  Part p = {0, 0, 0, 0, 0, 0, pairs, u < units};
+  u = min(u, units - 1);
   int first, length;                                               // a run of entries that is cut into two chunks a lane
   if (!NEIGHBOURS && u < (pairs + V - 1) / V) {
     p.pair = pairs >= V ? min(u * V, pairs - V) : 0;
@@ -100,15 +100,23 @@ inline int units_of(int V, int d, int pairs, bool neighbours) {
   return (pairs + V - 1) / V + (d - 2 * pairs + 2 * V - 1) / (2 * V);
 }
 
-// The first n entries at p, the others zero: 16 bytes, or entry by entry.
-template <class T> __device__ __forceinline__ void load(const T* p, int n, float (&v)[Chunk<T>::N]) {
+// The first n entries at p, the others zero, in 16 bytes: one load, or entry by entry.
+template <class T> __device__ __forceinline__ uint4 load(const T* p, int n) {
   constexpr int N = Chunk<T>::N;
-  if (n == N) {
-    Chunk<T>::get(load_chunk<T>(p, N), v);
-    return;
-  }
+  if (n == N) return load_chunk<T>(p, N);
+  n = fresh(n);
+  float v[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = i < n ? (float)p[i] : 0.f;
+  return Chunk<T>::put(v);
+}
+template <class T> __device__ __forceinline__ void store(T* p, int n, const float (&v)[Chunk<T>::N]) {
+  constexpr int N = Chunk<T>::N;
+  if (n == N) return store_chunk<T>(p, N, v);
+  n = fresh(n);
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i < n) p[i] = (T)v[i];
 }
 
 // cos and sin of V pairs from `pair` on of a row; of pairs that do not turn 1 and 0, of a row that is not there NaN
@@ -123,6 +131,7 @@ template <int V> __device__ __forceinline__ void load_turns(const Args& p, const
     }
     return;
   }
+  pair = fresh(pair);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     float2 t = make_float2(1.f, 0.f);
@@ -164,91 +173,107 @@ __device__ __forceinline__ float sum_of(float v, int lanes) {           // over 
   return v;
 }
 
-// sum over the entries of a lane that are its own of x y
+// Sum over the entries of a lane that are its own of x y
 template <int V> __device__ __forceinline__ float dot(const Part& p, const float (&xa)[V], const float (&xb)[V], const float (&ya)[V], const float (&yb)[V]) {
   float t = 0.f;
   if (p.skip_a == 0 && p.skip_b == 0) {
 #pragma unroll
     for (int i = 0; i < V; ++i) t = fmaf(xa[i], ya[i], fmaf(xb[i], yb[i], t));
   } else {
+    const int skip_a = fresh(p.skip_a), skip_b = fresh(p.skip_b);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      if (i >= p.skip_a) t = fmaf(xa[i], ya[i], t);
-      if (i >= p.skip_b) t = fmaf(xb[i], yb[i], t);
+      if (i >= skip_a) t = fmaf(xa[i], ya[i], t);
+      if (i >= skip_b) t = fmaf(xb[i], yb[i], t);
     }
   }
-  return t;
+  return p.own ? t : 0.f;
 }
 
 enum Pass { TURN, NORM, NORM_BACK };           // TURN: both directions of the rotation alone
 
-template <class T, Pass PASS, bool NEIGHBOURS> __global__ __launch_bounds__(THREADS) void rotary_kernel(Args p) {
+// HEADS: the most heads of a run, whose loads are under way together and which share the cosines and sines of their place.
+template <class T, Pass PASS, bool NEIGHBOURS, int HEADS> __global__ __launch_bounds__(THREADS, PASS == NORM_BACK ? 3 : 4) void rotary_kernel(Args p) {
   constexpr int V = Chunk<T>::N;
   const bool second = blockIdx.x >= p.blocks0;
   const Side& s = p.side[second];
   const unsigned block = second ? blockIdx.x - p.blocks0 : blockIdx.x, blocks = second ? gridDim.x - p.blocks0 : p.blocks0;
   const int lane = threadIdx.x & (p.lanes - 1);
   const unsigned groups = (unsigned)(THREADS / p.lanes);
-  const Part kept = part_of<V, NEIGHBOURS>(lane, p.units, p.d, p.pairs);
+  const Part part = part_of<V, NEIGHBOURS>(lane, p.units, p.d, p.pairs);
   const float inv_d = 1.f / (float)p.d;
-  float wa[V], wb[V], ga[V] = {}, gb[V] = {};                     // weights; sums of their gradients
-  if (PASS != TURN) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) wa[i] = wb[i] = 1.f;
-    if (s.weight) {
-      load<T>(static_cast<const T*>(s.weight) + kept.a, kept.na, wa);
-      load<T>(static_cast<const T*>(s.weight) + kept.b, kept.nb, wb);
-    }
+  uint4 wraw_a, wraw_b;                                            // weights
+  float ga[V] = {}, gb[V] = {};                                    // sums of their gradients
+  if (PASS != TURN && s.weight) {
+    wraw_a = load<T>(static_cast<const T*>(s.weight) + part.a, part.na);
+    wraw_b = load<T>(static_cast<const T*>(s.weight) + part.b, part.nb);
   }
+  const auto weigh = [&](float (&a)[V], float (&b)[V]) {
+    if (!s.weight) return;
+    float w[V];
+    Chunk<T>::get(wraw_a, w);
+#pragma unroll
+    for (int i = 0; i < V; ++i) a[i] *= w[i];
+    Chunk<T>::get(wraw_b, w);
+#pragma unroll
+    for (int i = 0; i < V; ++i) b[i] *= w[i];
+  };
   // every group of the launch takes as many turns, so that no lane is missing from a sum
-  for (unsigned first = block * groups; first < s.vectors; first += blocks * groups) {
-    const unsigned mine = first + threadIdx.x / p.lanes, item = min(mine, s.vectors - 1);
-    const Part part = {kept.a, kept.b, fresh(kept.na), fresh(kept.nb), fresh(kept.skip_a), fresh(kept.skip_b), fresh(kept.pair)};
+  for (unsigned first = block * groups; first < s.items; first += blocks * groups) {
+    const unsigned mine = first + threadIdx.x / p.lanes, item = min(mine, s.items - 1);
     unsigned inner, middle;
     const unsigned outer = divide(divide(item, s.inner, inner), s.middle, middle);
     const unsigned place = s.heads_inside ? middle : inner;
+    const int head = (int)(s.heads_inside ? inner : middle) * s.run, heads = mine < s.items ? min(s.run, s.heads - head) : 0;
+    const auto at = [&](const Tensor& t) { return (T*)t.at + ((long)outer * t.batch + (long)place * t.place + (long)head * t.head); };
+    uint4 raw[HEADS][2] = {}, graw[HEADS][2] = {};
+    const T* const x = at(s.x);
+    const T* const g = PASS == NORM_BACK ? at(s.g) : nullptr;
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h)
+      if (h < heads) {
+        raw[h][0] = load<T>(x + h * s.x.head + part.a, part.na), raw[h][1] = load<T>(x + h * s.x.head + part.b, part.nb);
+        if (PASS == NORM_BACK) graw[h][0] = load<T>(g + h * s.g.head + part.a, part.na), graw[h][1] = load<T>(g + h * s.g.head + part.b, part.nb);
+      }
     int row = (int)place;
     if (p.index) row = p.index[outer * p.index_stride + place];
-    const bool there = row < p.rows;
     float c[V], sn[V];
     // a row below zero: the vector is not turned
-    load_turns<V>(p, p.table + outer * p.table_stride + (long)row * p.pairs, there, p.pairs == 0 || row < 0 ? p.pairs : part.pair, c, sn);
-    const auto at = [&](const Tensor& t) { return static_cast<const T*>(t.at) + ((long)outer * t.outer + (long)middle * t.middle + (long)inner * t.inner); };
-    float a[V], b[V];
-    if constexpr (PASS != NORM_BACK) {
-      const T* const x = at(s.x);
-      load<T>(x + part.a, part.na, a);
-      load<T>(x + part.b, part.nb, b);
-      if constexpr (PASS == NORM) {
+    load_turns<V>(p, p.table + outer * p.table_stride + (long)row * p.pairs, row < p.rows, p.pairs == 0 || row < 0 ? p.pairs : part.pair, c, sn);
+    T* const y = at(s.y);
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h) {
+      if (h >= s.run) break;
+      float a[V], b[V];
+      Chunk<T>::get(raw[h][0], a);
+      Chunk<T>::get(raw[h][1], b);
+      if constexpr (PASS == TURN) {
+        turn<V, NEIGHBOURS>(c, sn, a, b);
+      } else {
         const float r = rsqrtf(fmaf(sum_of(dot<V>(part, a, b, a, b), p.lanes), inv_d, p.eps));
 #pragma unroll
-        for (int i = 0; i < V; ++i) a[i] = a[i] * r * wa[i], b[i] = b[i] * r * wb[i];
-      }
-      turn<V, NEIGHBOURS>(c, sn, a, b);
-    } else {
-      const T* const x = at(s.x);
-      const T* const g = at(s.g);
-      float xa[V], xb[V];
-      load<T>(x + part.a, part.na, xa);
-      load<T>(x + part.b, part.nb, xb);
-      load<T>(g + part.a, part.na, a);
-      load<T>(g + part.b, part.nb, b);
-      turn<V, NEIGHBOURS>(c, sn, a, b);
-      const float r = rsqrtf(fmaf(sum_of(dot<V>(part, xa, xb, xa, xb), p.lanes), inv_d, p.eps));
+        for (int i = 0; i < V; ++i) a[i] *= r, b[i] *= r;
+        if constexpr (PASS == NORM) {
+          weigh(a, b);
+          turn<V, NEIGHBOURS>(c, sn, a, b);
+        } else {
+          float u[V], v[V];
+          Chunk<T>::get(graw[h][0], u);
+          Chunk<T>::get(graw[h][1], v);
+          turn<V, NEIGHBOURS>(c, sn, u, v);
+          if (h < heads)
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        xa[i] *= r, xb[i] *= r;
-        if (mine < s.vectors) ga[i] = fmaf(a[i], xa[i], ga[i]), gb[i] = fmaf(b[i], xb[i], gb[i]);
-        a[i] *= wa[i], b[i] *= wb[i];
-      }
-      const float m = sum_of(dot<V>(part, a, b, xa, xb), p.lanes) * inv_d;
+            for (int i = 0; i < V; ++i) ga[i] = fmaf(u[i], a[i], ga[i]), gb[i] = fmaf(v[i], b[i], gb[i]);
+          weigh(u, v);
+          const float m = sum_of(dot<V>(part, u, v, a, b), p.lanes) * inv_d;
 #pragma unroll
-      for (int i = 0; i < V; ++i) a[i] = r * fmaf(-xa[i], m, a[i]), b[i] = r * fmaf(-xb[i], m, b[i]);
-    }
-    if (mine < s.vectors) {
-      T* const y = static_cast<T*>(s.y) + ((long)outer * s.y_outer + (long)middle * s.y_middle + (long)inner * s.y_inner);
-      store_chunk<T>(y + part.a, part.na, a);
-      store_chunk<T>(y + part.b, part.nb, b);
+          for (int i = 0; i < V; ++i) a[i] = r * fmaf(-a[i], m, u[i]), b[i] = r * fmaf(-b[i], m, v[i]);
+        }
+      }
+      if (h < heads && part.own) {
+        store<T>(y + h * s.y.head + part.a, part.na, a);
+        store<T>(y + h * s.y.head + part.b, part.nb, b);
+      }
     }
   }
   if constexpr (PASS == NORM_BACK) {
@@ -266,8 +291,8 @@ template <class T, Pass PASS, bool NEIGHBOURS> __global__ __launch_bounds__(THRE
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const auto sum = [&](int k) { return (joined[0][lane][k] + joined[1][lane][k]) + (joined[2][lane][k] + joined[3][lane][k]); };
-        if (i >= kept.skip_a && i < kept.na) out[kept.a + i] = sum(i);
-        if (i >= kept.skip_b && i < kept.nb) out[kept.b + i] = sum(V + i);
+        if (i >= part.skip_a && i < part.na) out[part.a + i] = sum(i);
+        if (i >= part.skip_b && i < part.nb) out[part.b + i] = sum(V + i);
       }
     }
   }
@@ -283,8 +308,10 @@ template <class T> __global__ __launch_bounds__(1024) void weights_kernel(const 
   if (!out) return;
   const int i = threadIdx.x & 31, s = threadIdx.x >> 5, col = blockIdx.x * 32 + i;
   float t = 0.f;
-  if (col < d)
+  if (col < d) {
+#pragma unroll 8
     for (unsigned k = s; k < blocks; k += 32) t += partial[(long)k * d + col];
+  }
   sums[s][i] = t;
   __syncthreads();
   t = sum_lanes<32>(sums[i][s]);
@@ -299,6 +326,7 @@ template <class P> __global__ __launch_bounds__(THREADS) void table_kernel(const
   const int side = THREADS / pairs, r = threadIdx.x / pairs, j = threadIdx.x - r * pairs;
   if (r >= side) return;
   const double f0 = frequencies[j] * 0.15915494309189533577;
+#pragma unroll 4
   for (long row = (long)blockIdx.x * side + r; row < n; row += (long)gridDim.x * side) {
     double turns = (double)positions[row * axes] * f0;
     for (int a = 1; a < axes; ++a) turns = fma((double)positions[row * axes + a] * 0.15915494309189533577, frequencies[a * pairs + j], turns);
@@ -316,8 +344,9 @@ template <class P> __global__ __launch_bounds__(THREADS) void table_kernel(const
 constexpr int CUS = 256;
 
 struct Plan {
-  int units, lanes;
-  unsigned vectors[2], blocks[2];
+  int units, lanes, most;        // most: heads of a run that the kernel is made for
+  int run[2];
+  unsigned items[2], blocks[2];
 };
 
 bool sizes_ok(const s2cnn_rotary_t* a) {
@@ -332,20 +361,27 @@ bool sizes_ok(const s2cnn_rotary_t* a) {
   return true;
 }
 
-// Workgroups: eight a CU for the loads and stores that are to be under way; four where their sums of the weights' gradients are read again.
-Plan plan_of(const s2cnn_rotary_t& a, bool sums) {
+// Runs of four heads (two where x and g are read), unless there are so few vectors that each has a group of its own.  Four workgroups a CU (three), which
+// is what their registers allow: all of them run at once.
+Plan plan_of(const s2cnn_rotary_t& a, bool two) {
   Plan p;
   p.units = units_of(a.dtype == S2CNN_F32 ? 4 : 8, a.d, a.pairs, a.interleaved != 0);
   for (p.lanes = 1; p.lanes < p.units;) p.lanes *= 2;
-  const long groups = THREADS / p.lanes, most = CUS * (sums ? 4 : 8);
-  long total = 0;
-  for (int i = 0; i < 2; ++i) total += (long)a.batch * a.n * a.side[i].heads;
+  const long groups = THREADS / p.lanes, most = CUS * (two ? 3 : 4), places = (long)a.batch * a.n;
+  const long vectors = places * ((long)a.side[0].heads + a.side[1].heads);
+  p.most = two ? 2 : 4;
+  if (vectors < most * groups * p.most) p.most = 1;
+  long runs[2], total = 0;
   for (int i = 0; i < 2; ++i) {
-    const long vectors = (long)a.batch * a.n * a.side[i].heads, need = (vectors + groups - 1) / groups;
-    const long share = (long)((double)most * vectors / total);
-    p.vectors[i] = (unsigned)vectors;
-    p.blocks[i] = (unsigned)(need < most ? need : share < 1 ? 1 : share);
-    if (!vectors) p.blocks[i] = 0;
+    runs[i] = (a.side[i].heads + p.most - 1) / p.most;
+    p.run[i] = runs[i] ? (int)((a.side[i].heads + runs[i] - 1) / runs[i]) : 1;
+    runs[i] = (a.side[i].heads + p.run[i] - 1) / p.run[i];
+    p.items[i] = (unsigned)(places * runs[i]);
+    total += p.items[i];
+  }
+  for (int i = 0; i < 2; ++i) {
+    const long need = (p.items[i] + groups - 1) / groups, share = (long)((double)most * p.items[i] / total);
+    p.blocks[i] = (unsigned)(total <= most * groups || need <= share ? need : share < 1 ? 1 : share);
   }
   return p;
 }
@@ -355,19 +391,19 @@ Args args_of(const s2cnn_rotary_t& a, const Plan& p, bool backward, float* parti
   for (int i = 0; i < 2; ++i) {
     const s2cnn_rotary_side_t& from = a.side[i];
     Side& s = k.side[i];
-    s.vectors = p.vectors[i];
+    s.items = p.items[i];
     if (!from.heads) continue;
-    // neighbouring groups take vectors that lie next to each other
-    s.heads_inside = a.n == 1 || (from.heads > 1 && (backward && !a.norm ? from.g_stride : from.x_stride)[1] <= (backward && !a.norm ? from.g_stride : from.x_stride)[2]);
-    s.inner = divider(s.heads_inside ? from.heads : a.n);
-    s.middle = divider(s.heads_inside ? a.n : from.heads);
-    const int in = s.heads_inside ? 1 : 2, mid = s.heads_inside ? 2 : 1;
-    const auto tensor = [&](const void* at, const long* stride) { return Tensor{at, stride[in], stride[mid], stride[0]}; };
-    s.x = tensor(from.x, from.x_stride);
+    const bool only_g = backward && !a.norm;
+    const long* const read = only_g ? from.g_stride : from.x_stride;
+    s.heads = from.heads, s.run = p.run[i];
+    const int runs = (from.heads + s.run - 1) / s.run;
+    s.heads_inside = a.n == 1 || (from.heads > 1 && read[1] <= read[2]);      // neighbouring groups take vectors that lie next to each other
+    s.inner = divider(s.heads_inside ? runs : a.n);
+    s.middle = divider(s.heads_inside ? a.n : runs);
+    const auto tensor = [](const void* at, const long* stride) { return Tensor{at, stride[1], stride[2], stride[0]}; };
+    s.x = only_g ? tensor(from.g, from.g_stride) : tensor(from.x, from.x_stride);
     s.g = tensor(from.g, from.g_stride);
-    if (backward && !a.norm) s.x = s.g;
-    s.y = from.y;
-    s.y_inner = from.y_stride[in], s.y_middle = from.y_stride[mid], s.y_outer = from.y_stride[0];
+    s.y = tensor(from.y, from.y_stride);
     s.weight = a.norm ? from.weight : nullptr;
     if (backward && from.gweight) s.partial = partial + (i ? (long)p.blocks[0] * a.d : 0);
   }
@@ -382,14 +418,18 @@ Args args_of(const s2cnn_rotary_t& a, const Plan& p, bool backward, float* parti
   return k;
 }
 
-template <class T, bool NEIGHBOURS> void launch(const Args& k, const Plan& p, bool norm, bool backward, hipStream_t s) {
+template <class T, bool NEIGHBOURS, int HEADS> void launch(const Args& k, const Plan& p, bool norm, bool backward, hipStream_t s) {
   const dim3 grid(p.blocks[0] + p.blocks[1]);
-  if (!norm) hipLaunchKernelGGL((rotary_kernel<T, TURN, NEIGHBOURS>), grid, dim3(THREADS), 0, s, k);
-  else if (!backward) hipLaunchKernelGGL((rotary_kernel<T, NORM, NEIGHBOURS>), grid, dim3(THREADS), 0, s, k);
-  else hipLaunchKernelGGL((rotary_kernel<T, NORM_BACK, NEIGHBOURS>), grid, dim3(THREADS), 0, s, k);
+  if (!norm) hipLaunchKernelGGL((rotary_kernel<T, TURN, NEIGHBOURS, HEADS>), grid, dim3(THREADS), 0, s, k);
+  else if (!backward) hipLaunchKernelGGL((rotary_kernel<T, NORM, NEIGHBOURS, HEADS>), grid, dim3(THREADS), 0, s, k);
+  else hipLaunchKernelGGL((rotary_kernel<T, NORM_BACK, NEIGHBOURS, (HEADS < 2 ? HEADS : 2)>), grid, dim3(THREADS), 0, s, k);
+}
+template <class T, bool NEIGHBOURS> void launch(const Args& k, const Plan& p, bool norm, bool backward, hipStream_t s) {
+  if (p.most == 1) launch<T, NEIGHBOURS, 1>(k, p, norm, backward, s);
+  else launch<T, NEIGHBOURS, 4>(k, p, norm, backward, s);
 }
 template <class T> void run(const s2cnn_rotary_t& a, bool backward, float* partial, hipStream_t s) {
-  const Plan p = plan_of(a, partial != nullptr);
+  const Plan p = plan_of(a, backward && a.norm);
   const Args k = args_of(a, p, backward, partial);
   if (a.interleaved) launch<T, true>(k, p, a.norm != 0, backward, s);
   else launch<T, false>(k, p, a.norm != 0, backward, s);

@@ -62,7 +62,7 @@ def grad_norm(tensors):
     if not dtypes <= _hip.FLOATS.keys():
         raise RuntimeError("tensors of float32, bfloat16 or float16 only (got %s)" % ", ".join(sorted(map(str, dtypes))))
     if set(map(_device, tensors)) != {device}:
-        raise RuntimeError("tensors on the current GPU only, cuda:%d" % device)
+        raise RuntimeError("tensors on the current GPU only, cuda:%d; there is no CPU path" % device)
     n, count = array("q", map(_numel, tensors)), len(tensors)
     kinds = array("i", [_hip.FLOATS[d] for d in map(_dtype, tensors)]) if len(dtypes) > 1 else array("i", [_hip.FLOATS[tensors[0].dtype]]) * count
     out = torch.empty((), dtype=torch.float32, device=tensors[0].device)
@@ -73,15 +73,15 @@ def grad_norm(tensors):
     return out
 
 
-def _check_states(first, second, scales, shapes, device):
-    """Moments in 32 bits (no scales) or 8 beside tensors of these shapes."""
-    assert len(first) == len(second) == len(shapes) and (scales is None or len(scales) == len(shapes))
+def _check_states(first, second, scales, n, device):
+    """Moments in 32 bits (no scales) or 8 of tensors of n entries each."""
+    assert len(first) == len(second) == len(n) and (scales is None or len(scales) == len(n))
     _check_list(first, torch.float32 if scales is None else torch.float8_e4m3fn, device, "first moments")
     _check_list(second, torch.float32 if scales is None else torch.uint8, device, "second moments")
-    assert list(map(_shape, first)) == shapes and list(map(_shape, second)) == shapes
+    assert list(map(_numel, first)) == n and list(map(_numel, second)) == n
     if scales is not None:
         _check_list(scales, torch.float32, device, "scales")
-        assert [tuple(t.shape) for t in scales] == [(-(-t.numel() // BLOCK), 2) for t in first]
+        assert list(map(_numel, scales)) == [2 * ((x + BLOCK - 1) // BLOCK) for x in n]
 
 
 @torch.no_grad()
@@ -92,7 +92,7 @@ def adamw_step(params, grads, first, second, step, lr=1e-3, betas=(0.9, 0.999), 
     m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2, p = p - lr weight_decay p - lr (m / (1 - b1^step)) / (sqrt(v / (1 - b2^step)) + eps).
 
     :param params, grads: tensors of one type (float32, bfloat16 or float16) on the current GPU; parameters contiguous, none twice
-    :param first, second: the moments m and v, of the parameters' shapes: float32, or with scales float8_e4m3fn and uint8
+    :param first, second: the moments m and v, as many entries as the parameters: float32, or with scales float8_e4m3fn and uint8
     :param step: which step it is, from 1 on: an int, or an int64 tensor of one element on the GPU that is read when the kernels run
     :param lr: a number, or a float32 tensor of one element on the GPU
     :param eps: >= 1e-30
@@ -122,27 +122,26 @@ def adamw_step(params, grads, first, second, step, lr=1e-3, betas=(0.9, 0.999), 
     dtype, device = params[0].dtype, _current_device(params)
     if dtype not in _hip.FLOATS:
         raise RuntimeError("float32, bfloat16 or float16 parameters only (got %s)" % dtype)
-    shapes = list(map(_shape, params))
+    sizes = list(map(_numel, params))
     _check_list(params, dtype, device, "parameters")
     if not all(map(_contiguous, grads)):
         grads = [g.contiguous() for g in grads]
     _check_list(grads, dtype, device, "gradients")
-    assert list(map(_shape, grads)) == shapes
-    _check_states(first, second, scales, shapes, device)
+    assert list(map(_shape, grads)) == list(map(_shape, params))
+    _check_states(first, second, scales, sizes, device)
     if masters is not None:
         assert dtype != torch.float32, "float32 parameters have no masters"
         _check_list(masters, torch.float32, device, "masters")
-        assert list(map(_shape, masters)) == shapes
+        assert list(map(_numel, masters)) == sizes
     if torch.is_tensor(step):
         _hip.require_gpu_of(torch.int64, step)
     if torch.is_tensor(lr):
         _hip.require_gpu_of(torch.float32, lr)
     _hip.require_gpu_of(torch.float32, norm)
 
-    n = array("q", map(_numel, params))
+    n = array("q", sizes)
     lists = [_addresses(t) if t is not None else None for t in (params, grads, first, second, scales, masters)]
-    present = len(n) - n.count(0)
-    assert len(set(lists[0]) - {0}) == present, "a parameter twice in the list"
+    assert len(set(lists[0]) - {0}) == len(n) - n.count(0), "a parameter twice in the list"
     a = _hip.AdamW()
     a.p, a.g, a.first, a.second, a.scales, a.masters = map(_at, lists)
     a.n, a.count, a.dtype, a.bits = _at(n), len(n), _hip.FLOATS[dtype], 32 if scales is None else 8
@@ -171,9 +170,10 @@ def adamw_states(first, second, scales):
         assert not second and not scales
         return [], []
     device = _current_device(first)
-    _check_states(first, second, scales, list(map(_shape, first)), device)
+    sizes = list(map(_numel, first))
+    _check_states(first, second, scales, sizes, device)
     out = [[torch.empty(t.shape, dtype=torch.float32, device=t.device) for t in first] for _ in range(2)]
-    n = array("q", map(_numel, first))
+    n = array("q", sizes)
     lists = [_addresses(t) for t in (first, second, scales, *out)]
     _hip.call("s2cnn_adamw_states", *map(_at, lists), _at(n), len(n), _hip.stream_ptr())
     return tuple(out)

@@ -608,7 +608,7 @@ def test_refusals_of_tensors(hip):
         lists[i][0] = wrong
         with pytest.raises(RuntimeError):
             step(*lists, 1)
-    for i, wrong in ((0, z(3, 4)), (1, z(12)), (2, z(4, 2)), (3, z(3, 4))):
+    for i, wrong in ((0, z(3, 4)), (1, z(12)), (2, z(4, 2)), (3, z(13))):
         lists = good()
         lists[i][0] = wrong
         with pytest.raises(AssertionError):
