@@ -54,8 +54,8 @@ struct Args {
   const float2* table;
   const int* index;
   long table_stride, index_stride;      // of the batch
-  int rows, d, pairs, units, lanes;
-  float eps, sign;
+  int rows, d, pairs, units, lanes, log_lanes;
+  float inv_d, eps, sign;
 };
 
 // The part of a vector that a lane holds.
@@ -101,18 +101,18 @@ inline int units_of(int V, int d, int pairs, bool neighbours) {
 }
 
 // The first n entries at p, the others zero, in 16 bytes: one load, or entry by entry.
-template <class T> __device__ __forceinline__ uint4 load(const T* p, int n) {
+template <class T, bool FULL> __device__ __forceinline__ uint4 load(const T* p, int n) {
   constexpr int N = Chunk<T>::N;
-  if (n == N) return load_chunk<T>(p, N);
+  if (FULL || n == N) return load_chunk<T>(p, N);
   n = fresh(n);
   float v[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = i < n ? (float)p[i] : 0.f;
   return Chunk<T>::put(v);
 }
-template <class T> __device__ __forceinline__ void store(T* p, int n, const float (&v)[Chunk<T>::N]) {
+template <class T, bool FULL> __device__ __forceinline__ void store(T* p, int n, const float (&v)[Chunk<T>::N]) {
   constexpr int N = Chunk<T>::N;
-  if (n == N) return store_chunk<T>(p, N, v);
+  if (FULL || n == N) return store_chunk<T>(p, N, v);
   n = fresh(n);
 #pragma unroll
   for (int i = 0; i < N; ++i)
@@ -132,6 +132,11 @@ template <int V> __device__ __forceinline__ void load_turns(const Args& p, const
     return;
   }
   pair = fresh(pair);
+  if (pair >= p.pairs) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) c[i] = 1.f, s[i] = 0.f;
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     float2 t = make_float2(1.f, 0.f);
@@ -192,21 +197,20 @@ template <int V> __device__ __forceinline__ float dot(const Part& p, const float
 
 enum Pass { TURN, NORM, NORM_BACK };           // TURN: both directions of the rotation alone
 
-// HEADS: the most heads of a run, whose loads are under way together and which share the cosines and sines of their place.
-template <class T, Pass PASS, bool NEIGHBOURS, int HEADS> __global__ __launch_bounds__(THREADS, PASS == NORM_BACK ? 3 : 4) void rotary_kernel(Args p) {
+// FULL: no lane's chunks are shorter than 16 bytes.  HEADS: the most heads of a run, whose loads are under way together and which share the cosines and sines of their place.
+template <class T, Pass PASS, bool NEIGHBOURS, int HEADS, bool FULL> __global__ __launch_bounds__(THREADS, PASS == NORM_BACK ? 3 : 4) void rotary_kernel(Args p) {
   constexpr int V = Chunk<T>::N;
   const bool second = blockIdx.x >= p.blocks0;
-  const Side& s = p.side[second];
+  const Side& s = p.side[__builtin_amdgcn_readfirstlane((int)second)];        // a number, so that the fields are loaded together
   const unsigned block = second ? blockIdx.x - p.blocks0 : blockIdx.x, blocks = second ? gridDim.x - p.blocks0 : p.blocks0;
   const int lane = threadIdx.x & (p.lanes - 1);
-  const unsigned groups = (unsigned)(THREADS / p.lanes);
+  const unsigned groups = (unsigned)(THREADS >> p.log_lanes);
   const Part part = part_of<V, NEIGHBOURS>(lane, p.units, p.d, p.pairs);
-  const float inv_d = 1.f / (float)p.d;
   uint4 wraw_a, wraw_b;                                            // weights
   float ga[V] = {}, gb[V] = {};                                    // sums of their gradients
   if (PASS != TURN && s.weight) {
-    wraw_a = load<T>(static_cast<const T*>(s.weight) + part.a, part.na);
-    wraw_b = load<T>(static_cast<const T*>(s.weight) + part.b, part.nb);
+    wraw_a = load<T, FULL>(static_cast<const T*>(s.weight) + part.a, part.na);
+    wraw_b = load<T, FULL>(static_cast<const T*>(s.weight) + part.b, part.nb);
   }
   const auto weigh = [&](float (&a)[V], float (&b)[V]) {
     if (!s.weight) return;
@@ -220,7 +224,7 @@ template <class T, Pass PASS, bool NEIGHBOURS, int HEADS> __global__ __launch_bo
   };
   // every group of the launch takes as many turns, so that no lane is missing from a sum
   for (unsigned first = block * groups; first < s.items; first += blocks * groups) {
-    const unsigned mine = first + threadIdx.x / p.lanes, item = min(mine, s.items - 1);
+    const unsigned mine = first + (threadIdx.x >> p.log_lanes), item = min(mine, s.items - 1);
     unsigned inner, middle;
     const unsigned outer = divide(divide(item, s.inner, inner), s.middle, middle);
     const unsigned place = s.heads_inside ? middle : inner;
@@ -232,8 +236,8 @@ template <class T, Pass PASS, bool NEIGHBOURS, int HEADS> __global__ __launch_bo
 #pragma unroll
     for (int h = 0; h < HEADS; ++h)
       if (h < heads) {
-        raw[h][0] = load<T>(x + h * s.x.head + part.a, part.na), raw[h][1] = load<T>(x + h * s.x.head + part.b, part.nb);
-        if (PASS == NORM_BACK) graw[h][0] = load<T>(g + h * s.g.head + part.a, part.na), graw[h][1] = load<T>(g + h * s.g.head + part.b, part.nb);
+        raw[h][0] = load<T, FULL>(x + h * s.x.head + part.a, part.na), raw[h][1] = load<T, FULL>(x + h * s.x.head + part.b, part.nb);
+        if (PASS == NORM_BACK) graw[h][0] = load<T, FULL>(g + h * s.g.head + part.a, part.na), graw[h][1] = load<T, FULL>(g + h * s.g.head + part.b, part.nb);
       }
     int row = (int)place;
     if (p.index) row = p.index[outer * p.index_stride + place];
@@ -250,7 +254,7 @@ template <class T, Pass PASS, bool NEIGHBOURS, int HEADS> __global__ __launch_bo
       if constexpr (PASS == TURN) {
         turn<V, NEIGHBOURS>(c, sn, a, b);
       } else {
-        const float r = rsqrtf(fmaf(sum_of(dot<V>(part, a, b, a, b), p.lanes), inv_d, p.eps));
+        const float r = rsqrtf(fmaf(sum_of(dot<V>(part, a, b, a, b), p.lanes), p.inv_d, p.eps));
 #pragma unroll
         for (int i = 0; i < V; ++i) a[i] *= r, b[i] *= r;
         if constexpr (PASS == NORM) {
@@ -265,14 +269,14 @@ template <class T, Pass PASS, bool NEIGHBOURS, int HEADS> __global__ __launch_bo
 #pragma unroll
             for (int i = 0; i < V; ++i) ga[i] = fmaf(u[i], a[i], ga[i]), gb[i] = fmaf(v[i], b[i], gb[i]);
           weigh(u, v);
-          const float m = sum_of(dot<V>(part, u, v, a, b), p.lanes) * inv_d;
+          const float m = sum_of(dot<V>(part, u, v, a, b), p.lanes) * p.inv_d;
 #pragma unroll
           for (int i = 0; i < V; ++i) a[i] = r * fmaf(-a[i], m, u[i]), b[i] = r * fmaf(-b[i], m, v[i]);
         }
       }
       if (h < heads && part.own) {
-        store<T>(y + h * s.y.head + part.a, part.na, a);
-        store<T>(y + h * s.y.head + part.b, part.nb, b);
+        store<T, FULL>(y + h * s.y.head + part.a, part.na, a);
+        store<T, FULL>(y + h * s.y.head + part.b, part.nb, b);
       }
     }
   }
@@ -319,24 +323,51 @@ template <class T> __global__ __launch_bounds__(1024) void weights_kernel(const 
 }
 
 // ---- the table ------------------------------------------------------------------------------------------------------
-// An angle is formed in turns and in 64 bits, and what is left of it after the next quarter of a turn in 32: positions of a million lose nothing.
-// A thread keeps its pair and takes one row after the other, THREADS / pairs of them side by side.
-template <class P> __global__ __launch_bounds__(THREADS) void table_kernel(const P* positions, const double* frequencies, float2* table, long n, int axes, int pairs,
-                                                                       float scale) {
-  const int side = THREADS / pairs, r = threadIdx.x / pairs, j = threadIdx.x - r * pairs;
+// An angle is formed in quarters of a turn and in 64 bits; adding 1.5 2^52 leaves the nearest whole number, whose lowest bits say which sine or cosine to
+// take of what is left, -1/2 .. 1/2, in 32 bits: positions of a million lose nothing.  Sine and cosine of that are polynomials of its square that interpolate
+// them at Chebyshev's points, off by 1.5 2^-24 and 2^-24.  A thread keeps its PER neighbouring pairs and takes one row after the other, so that a position is
+// converted once for 16 bytes of the table.  262144 rows of 64 pairs, 134 MB: see the launch.
+__device__ __forceinline__ float2 turn_of(double quarters, float scale) {
+  double whole = (quarters + 0x1.8p52) - 0x1.8p52;
+  unsigned q = (unsigned)__double_as_longlong(quarters + 0x1.8p52);
+  if (!(fabs(quarters) < 0x1p50)) {                                       // beyond: what 64 bits have of it
+    whole = rint(quarters);
+    q = (unsigned)(int)(whole - 4.0 * floor(0.25 * whole));
+  }
+  const float x = (float)(quarters - whole), z = x * x;
+  const float sin = x * fmaf(z, fmaf(z, fmaf(z, -0x1.2d9b40p-8f, 0x1.465ec4p-4f), -0x1.4abbbap-1f), 0x1.921fb6p+0f);
+  const float cos = fmaf(z, fmaf(z, fmaf(z, fmaf(z, 0x1.d9c2e8p-11f, -0x1.55c57ap-6f), 0x1.03c1dcp-2f), -0x1.3bd3ccp+0f), 1.f);
+  const float c = q & 1 ? sin : cos, s = q & 1 ? cos : sin;
+  return make_float2(__uint_as_float(__float_as_uint(c) ^ (((q + 1) & 2) << 30)) * scale, __uint_as_float(__float_as_uint(s) ^ ((q & 2) << 30)) * scale);
+}
+
+template <int PER, class P> __global__ __launch_bounds__(THREADS) void table_kernel(const P* positions, const double* frequencies, float2* table, long n, int axes, int pairs,
+                                                                                float scale) {
+  constexpr double QUARTERS = 0.63661977236758134308;                    // of a turn in a radian
+  const int threads = pairs / PER, side = THREADS / threads, r = threadIdx.x / threads, j = (threadIdx.x - r * threads) * PER;
   if (r >= side) return;
-  const double f0 = frequencies[j] * 0.15915494309189533577;
+  double f[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) f[i] = frequencies[j + i] * QUARTERS;
 #pragma unroll 4
   for (long row = (long)blockIdx.x * side + r; row < n; row += (long)gridDim.x * side) {
-    double turns = (double)positions[row * axes] * f0;
-    for (int a = 1; a < axes; ++a) turns = fma((double)positions[row * axes + a] * 0.15915494309189533577, frequencies[a * pairs + j], turns);
-    const double quarters = rint(4.0 * turns);
-    const float rest = (float)(4.0 * turns - quarters);                    // of a quarter, -1/2 .. 1/2
-    float s, c;
-    sincospif(0.5f * rest, &s, &c);
-    const int q = (int)(quarters - 4.0 * floor(0.25 * quarters));
-    const float cos = q & 1 ? s : c, sin = q & 1 ? c : s;
-    table[row * pairs + j] = make_float2((q == 1 || q == 2 ? -cos : cos) * scale, (q >= 2 ? -sin : sin) * scale);
+    const double p = (double)positions[row * axes];
+    double quarters[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) quarters[i] = p * f[i];
+    for (int a = 1; a < axes; ++a) {
+      const double q = (double)positions[row * axes + a] * QUARTERS;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) quarters[i] = fma(q, frequencies[a * pairs + j + i], quarters[i]);
+    }
+    float2* const out = table + row * pairs + j;
+    if constexpr (PER == 2) {
+      typedef float loose __attribute__((ext_vector_type(4), aligned(8)));
+      const float2 u = turn_of(quarters[0], scale), v = turn_of(quarters[1], scale);
+      *reinterpret_cast<loose*>(out) = loose{u.x, u.y, v.x, v.y};
+    } else {
+      *out = turn_of(quarters[0], scale);
+    }
   }
 }
 
@@ -344,7 +375,8 @@ template <class P> __global__ __launch_bounds__(THREADS) void table_kernel(const
 constexpr int CUS = 256;
 
 struct Plan {
-  int units, lanes, most;        // most: heads of a run that the kernel is made for
+  int units, lanes, log_lanes, most;      // most: heads of a run that the kernel is made for
+  bool full;
   int run[2];
   unsigned items[2], blocks[2];
 };
@@ -361,16 +393,18 @@ bool sizes_ok(const s2cnn_rotary_t* a) {
   return true;
 }
 
-// Runs of four heads (two where x and g are read), unless there are so few vectors that each has a group of its own.  Four workgroups a CU (three), which
-// is what their registers allow: all of them run at once.
+// Runs of four heads (two where x and g are read) where that leaves every group two runs or more, else of one.  As many workgroups as run at once, four a CU
+// (three; runs of one head: eight, four), or fewer that take as many turns.
 Plan plan_of(const s2cnn_rotary_t& a, bool two) {
   Plan p;
   p.units = units_of(a.dtype == S2CNN_F32 ? 4 : 8, a.d, a.pairs, a.interleaved != 0);
-  for (p.lanes = 1; p.lanes < p.units;) p.lanes *= 2;
-  const long groups = THREADS / p.lanes, most = CUS * (two ? 3 : 4), places = (long)a.batch * a.n;
-  const long vectors = places * ((long)a.side[0].heads + a.side[1].heads);
+  for (p.lanes = 1, p.log_lanes = 0; p.lanes < p.units; ++p.log_lanes) p.lanes *= 2;
+  const int V = a.dtype == S2CNN_F32 ? 4 : 8, rest = a.d - 2 * a.pairs;
+  p.full = a.interleaved ? a.d % 2 == 0 && a.d >= 2 * V : (a.pairs == 0 || a.pairs >= V) && (rest == 0 || rest >= 2 * V);
+  const long groups = THREADS / p.lanes, places = (long)a.batch * a.n, vectors = places * ((long)a.side[0].heads + a.side[1].heads);
   p.most = two ? 2 : 4;
-  if (vectors < most * groups * p.most) p.most = 1;
+  long most = CUS * (two ? 3 : 4);
+  if (vectors < 2 * most * groups * p.most) p.most = 1, most = CUS * (two ? 4 : 8);
   long runs[2], total = 0;
   for (int i = 0; i < 2; ++i) {
     runs[i] = (a.side[i].heads + p.most - 1) / p.most;
@@ -380,8 +414,11 @@ Plan plan_of(const s2cnn_rotary_t& a, bool two) {
     total += p.items[i];
   }
   for (int i = 0; i < 2; ++i) {
-    const long need = (p.items[i] + groups - 1) / groups, share = (long)((double)most * p.items[i] / total);
-    p.blocks[i] = (unsigned)(total <= most * groups || need <= share ? need : share < 1 ? 1 : share);
+    const long need = (p.items[i] + groups - 1) / groups;
+    long share = (long)((double)most * p.items[i] / total);
+    if (share < 1) share = 1;
+    const long turns = (need + share - 1) / share;
+    p.blocks[i] = (unsigned)(total <= most * groups ? need : need ? (need + turns - 1) / turns : 0);
   }
   return p;
 }
@@ -412,21 +449,22 @@ Args args_of(const s2cnn_rotary_t& a, const Plan& p, bool backward, float* parti
   k.index = a.index;
   k.table_stride = a.table_stride / 2;
   k.index_stride = a.index_stride;
-  k.rows = a.rows, k.d = a.d, k.pairs = a.pairs, k.units = p.units, k.lanes = p.lanes;
+  k.rows = a.rows, k.d = a.d, k.pairs = a.pairs, k.units = p.units, k.lanes = p.lanes, k.log_lanes = p.log_lanes;
+  k.inv_d = 1.f / (float)a.d;
   k.eps = a.eps;
   k.sign = backward ? -1.f : 1.f;
   return k;
 }
 
-template <class T, bool NEIGHBOURS, int HEADS> void launch(const Args& k, const Plan& p, bool norm, bool backward, hipStream_t s) {
+template <class T, bool NEIGHBOURS, int HEADS, bool FULL> void launch(const Args& k, const Plan& p, bool norm, bool backward, hipStream_t s) {
   const dim3 grid(p.blocks[0] + p.blocks[1]);
-  if (!norm) hipLaunchKernelGGL((rotary_kernel<T, TURN, NEIGHBOURS, HEADS>), grid, dim3(THREADS), 0, s, k);
-  else if (!backward) hipLaunchKernelGGL((rotary_kernel<T, NORM, NEIGHBOURS, HEADS>), grid, dim3(THREADS), 0, s, k);
-  else hipLaunchKernelGGL((rotary_kernel<T, NORM_BACK, NEIGHBOURS, (HEADS < 2 ? HEADS : 2)>), grid, dim3(THREADS), 0, s, k);
+  if (!norm) hipLaunchKernelGGL((rotary_kernel<T, TURN, NEIGHBOURS, HEADS, FULL>), grid, dim3(THREADS), 0, s, k);
+  else if (!backward) hipLaunchKernelGGL((rotary_kernel<T, NORM, NEIGHBOURS, HEADS, FULL>), grid, dim3(THREADS), 0, s, k);
+  else hipLaunchKernelGGL((rotary_kernel<T, NORM_BACK, NEIGHBOURS, (HEADS < 2 ? HEADS : 2), FULL>), grid, dim3(THREADS), 0, s, k);
 }
 template <class T, bool NEIGHBOURS> void launch(const Args& k, const Plan& p, bool norm, bool backward, hipStream_t s) {
-  if (p.most == 1) launch<T, NEIGHBOURS, 1>(k, p, norm, backward, s);
-  else launch<T, NEIGHBOURS, 4>(k, p, norm, backward, s);
+  if (p.most == 1) p.full ? launch<T, NEIGHBOURS, 1, true>(k, p, norm, backward, s) : launch<T, NEIGHBOURS, 1, false>(k, p, norm, backward, s);
+  else p.full ? launch<T, NEIGHBOURS, 4, true>(k, p, norm, backward, s) : launch<T, NEIGHBOURS, 4, false>(k, p, norm, backward, s);
 }
 template <class T> void run(const s2cnn_rotary_t& a, bool backward, float* partial, hipStream_t s) {
   const Plan p = plan_of(a, backward && a.norm);
@@ -497,11 +535,15 @@ extern "C" int s2cnn_rotary_table(const void* positions, int positions_type, con
   if (positions_type < S2CNN_POSITIONS_F32 || positions_type > S2CNN_POSITIONS_I64) return S2CNN_EINVAL;
   const bool wide = positions_type == S2CNN_POSITIONS_F64 || positions_type == S2CNN_POSITIONS_I64;
   if ((reinterpret_cast<uintptr_t>(positions) & (wide ? 7 : 3)) || !aligned8(frequencies) || !aligned8(table)) return S2CNN_EALIGN;
-  const long side = rotary::THREADS / pairs, need = (n + side - 1) / side, most = rotary::CUS * 16;
+  const bool two = pairs % 2 == 0;
+  const long side = rotary::THREADS / (two ? pairs / 2 : pairs), need = (n + side - 1) / side, most = rotary::CUS * 16;
   const dim3 grid((unsigned)(need < most ? need : most)), block(rotary::THREADS);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   float2* const out = reinterpret_cast<float2*>(table);
-  const auto run = [&](auto* at) { hipLaunchKernelGGL(rotary::table_kernel, grid, block, 0, s, at, frequencies, out, n, axes, pairs, scale); };
+  const auto run = [&](auto* at) {
+    if (two) hipLaunchKernelGGL(rotary::table_kernel<2>, grid, block, 0, s, at, frequencies, out, n, axes, pairs, scale);
+    else hipLaunchKernelGGL(rotary::table_kernel<1>, grid, block, 0, s, at, frequencies, out, n, axes, pairs, scale);
+  };
   switch (positions_type) {
     case S2CNN_POSITIONS_F32: run(static_cast<const float*>(positions)); break;
     case S2CNN_POSITIONS_F64: run(static_cast<const double*>(positions)); break;
