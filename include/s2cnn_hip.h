@@ -478,8 +478,8 @@ int s2cnn_dropout(const void *x, void *y, long n, double p, unsigned long long s
 /* ---- rotations of queries and keys by position, normalisation of every head's vectors -------------
  * Vectors x[b,h,n] of d <= 256 entries, 2 pairs <= d of which are turned: y = R(table row) x, and with norm != 0 y = R(row) (weight x r),
  * r = 1 / sqrt(mean of x^2 + eps) over all d entries.  R turns the pair (x[j], x[pairs + j]), or with interleaved != 0 (x[2j], x[2j + 1]), to
- * (a cos - b sin, a sin + b cos), cos and sin being entry j of the row; entries from 2 pairs on are not turned.  Two tensors, side[0] and side[1]
- * (queries and keys; heads 0: none), share the table.
+ * (a cos - b sin, a sin + b cos), cos and sin being entry j of the row; entries from 2 pairs on are not turned.  Two tensors, queries [0] and
+ * keys [1] (heads 0: none; not the first), share the table.
  * table  : [batch, rows, pairs, 2] float32, rows contiguous, table_stride floats from batch to batch (0: one for all; even), 8-byte aligned; NULL
  *          where pairs is 0.  Row of vector n: n, or index[b,n] (index_stride entries from batch to batch, 0: one for all; NULL: n).  A row below zero:
  *          the vector is not turned; from rows on: what would be turned becomes NaN.
@@ -487,18 +487,14 @@ int s2cnn_dropout(const void *x, void *y, long n, double p, unsigned long long s
  * Types: dtype; arithmetic float32, results rounded once.  A tensor's vectors are contiguous, strides are those of (batch, head, n) in entries.
  * batch n heads < 2^31 for each side.  Results do not depend on the order of execution.
  */
-typedef struct s2cnn_rotary_side_t {
-  const void *x, *weight, *g;  /* weight: [d], or NULL (ones)                               */
-  void *y, *gweight;
-  long x_stride[3], g_stride[3], y_stride[3];
-  int heads;
-} s2cnn_rotary_side_t;
-
 typedef struct s2cnn_rotary_t {
-  s2cnn_rotary_side_t side[2];
+  const void *x[2], *weight[2], *g[2];      /* weight: [d], or NULL (ones)                  */
+  void *y[2], *gweight[2];
   const float *table;
   const int *index;
+  long x_stride[2][3], g_stride[2][3], y_stride[2][3];
   long table_stride, index_stride;
+  int heads[2];
   int batch, n, d, pairs, rows, norm, interleaved, dtype;
   float eps;
 } s2cnn_rotary_t;

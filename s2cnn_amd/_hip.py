@@ -35,14 +35,10 @@ class Attention(ctypes.Structure):
 _ATTENTION_P = ctypes.POINTER(Attention)
 
 
-class RotarySide(ctypes.Structure):
-    """s2cnn_rotary_side_t"""
-    _fields_ = [(n, _vp) for n in ("x", "weight", "g", "y", "gweight")] + [(n, _long * 3) for n in ("x_stride", "g_stride", "y_stride")] + [("heads", _int)]
-
-
 class Rotary(ctypes.Structure):
     """s2cnn_rotary_t"""
-    _fields_ = ([("side", RotarySide * 2), ("table", _vp), ("index", _vp), ("table_stride", _long), ("index_stride", _long)]
+    _fields_ = ([(n, _vp * 2) for n in ("x", "weight", "g", "y", "gweight")] + [("table", _vp), ("index", _vp)]
+                + [(n, (_long * 3) * 2) for n in ("x_stride", "g_stride", "y_stride")] + [("table_stride", _long), ("index_stride", _long), ("heads", _int * 2)]
                 + [(n, _int) for n in ("batch", "n", "d", "pairs", "rows", "norm", "interleaved", "dtype")] + [("eps", _float)])
 
 

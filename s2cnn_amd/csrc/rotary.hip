@@ -386,10 +386,10 @@ bool sizes_ok(const s2cnn_rotary_t* a) {
   if (a->batch < 1 || a->n < 1 || a->d < 1 || a->d > MAX_D || a->pairs < 0 || 2 * a->pairs > a->d) return false;
   if (a->pairs && (!a->table || a->rows < 1 || (!a->index && a->rows < a->n))) return false;
   if (!a->pairs && (a->table || a->index)) return false;
-  if (a->side[0].heads < 1 || a->side[1].heads < 0 || (a->norm && !(a->eps > 0.f))) return false;
+  if (a->heads[0] < 1 || a->heads[1] < 0 || (a->norm && !(a->eps > 0.f))) return false;
   const long limit = 1L << 31;
-  for (const s2cnn_rotary_side_t& s : a->side)
-    if ((long)a->batch * a->n >= limit || (s.heads && (long)a->batch * a->n >= limit / s.heads)) return false;
+  for (int heads : a->heads)
+    if ((long)a->batch * a->n >= limit || (heads && (long)a->batch * a->n >= limit / heads)) return false;
   return true;
 }
 
@@ -401,15 +401,15 @@ Plan plan_of(const s2cnn_rotary_t& a, bool two) {
   for (p.lanes = 1, p.log_lanes = 0; p.lanes < p.units; ++p.log_lanes) p.lanes *= 2;
   const int V = a.dtype == S2CNN_F32 ? 4 : 8, rest = a.d - 2 * a.pairs;
   p.full = a.interleaved ? a.d % 2 == 0 && a.d >= 2 * V : (a.pairs == 0 || a.pairs >= V) && (rest == 0 || rest >= 2 * V);
-  const long groups = THREADS / p.lanes, places = (long)a.batch * a.n, vectors = places * ((long)a.side[0].heads + a.side[1].heads);
+  const long groups = THREADS / p.lanes, places = (long)a.batch * a.n, vectors = places * ((long)a.heads[0] + a.heads[1]);
   p.most = two ? 2 : 4;
   long most = CUS * (two ? 3 : 4);
   if (vectors < 2 * most * groups * p.most) p.most = 1, most = CUS * (two ? 4 : 8);
   long runs[2], total = 0;
   for (int i = 0; i < 2; ++i) {
-    runs[i] = (a.side[i].heads + p.most - 1) / p.most;
-    p.run[i] = runs[i] ? (int)((a.side[i].heads + runs[i] - 1) / runs[i]) : 1;
-    runs[i] = (a.side[i].heads + p.run[i] - 1) / p.run[i];
+    runs[i] = (a.heads[i] + p.most - 1) / p.most;
+    p.run[i] = runs[i] ? (int)((a.heads[i] + runs[i] - 1) / runs[i]) : 1;
+    runs[i] = (a.heads[i] + p.run[i] - 1) / p.run[i];
     p.items[i] = (unsigned)(places * runs[i]);
     total += p.items[i];
   }
@@ -426,23 +426,22 @@ Plan plan_of(const s2cnn_rotary_t& a, bool two) {
 Args args_of(const s2cnn_rotary_t& a, const Plan& p, bool backward, float* partial) {
   Args k = {};
   for (int i = 0; i < 2; ++i) {
-    const s2cnn_rotary_side_t& from = a.side[i];
     Side& s = k.side[i];
     s.items = p.items[i];
-    if (!from.heads) continue;
+    if (!a.heads[i]) continue;
     const bool only_g = backward && !a.norm;
-    const long* const read = only_g ? from.g_stride : from.x_stride;
-    s.heads = from.heads, s.run = p.run[i];
-    const int runs = (from.heads + s.run - 1) / s.run;
-    s.heads_inside = a.n == 1 || (from.heads > 1 && read[1] <= read[2]);      // neighbouring groups take vectors that lie next to each other
+    const long* const read = only_g ? a.g_stride[i] : a.x_stride[i];
+    s.heads = a.heads[i], s.run = p.run[i];
+    const int runs = (s.heads + s.run - 1) / s.run;
+    s.heads_inside = a.n == 1 || (s.heads > 1 && read[1] <= read[2]);      // neighbouring groups take vectors that lie next to each other
     s.inner = divider(s.heads_inside ? runs : a.n);
     s.middle = divider(s.heads_inside ? a.n : runs);
     const auto tensor = [](const void* at, const long* stride) { return Tensor{at, stride[1], stride[2], stride[0]}; };
-    s.x = only_g ? tensor(from.g, from.g_stride) : tensor(from.x, from.x_stride);
-    s.g = tensor(from.g, from.g_stride);
-    s.y = tensor(from.y, from.y_stride);
-    s.weight = a.norm ? from.weight : nullptr;
-    if (backward && from.gweight) s.partial = partial + (i ? (long)p.blocks[0] * a.d : 0);
+    s.x = only_g ? tensor(a.g[i], a.g_stride[i]) : tensor(a.x[i], a.x_stride[i]);
+    s.g = tensor(a.g[i], a.g_stride[i]);
+    s.y = tensor(a.y[i], a.y_stride[i]);
+    s.weight = a.norm ? a.weight[i] : nullptr;
+    if (backward && a.gweight[i]) s.partial = partial + (i ? (long)p.blocks[0] * a.d : 0);
   }
   k.blocks0 = p.blocks[0];
   k.table = reinterpret_cast<const float2*>(a.table);
@@ -473,7 +472,7 @@ template <class T> void run(const s2cnn_rotary_t& a, bool backward, float* parti
   else launch<T, false>(k, p, a.norm != 0, backward, s);
   if (partial)
     hipLaunchKernelGGL(weights_kernel<T>, dim3((unsigned)((a.d + 31) / 32), 2), dim3(1024), 0, s, k.side[0].partial, k.side[1].partial, p.blocks[0], p.blocks[1], a.d,
-                       static_cast<T*>(a.side[0].gweight), static_cast<T*>(a.side[1].gweight));
+                       static_cast<T*>(a.heads[0] ? a.gweight[0] : nullptr), static_cast<T*>(a.heads[1] ? a.gweight[1] : nullptr));
 }
 void run(const s2cnn_rotary_t& a, bool backward, float* partial, hipStream_t s) {
   if (a.dtype == S2CNN_F32) run<float>(a, backward, partial, s);
@@ -485,20 +484,20 @@ void run(const s2cnn_rotary_t& a, bool backward, float* partial, hipStream_t s) 
 int check(const s2cnn_rotary_t* a, bool backward) {
   if (!sizes_ok(a)) return S2CNN_EINVAL;
   const uintptr_t mask = a->dtype == S2CNN_F32 ? 3 : 1;
-  for (const s2cnn_rotary_side_t& s : a->side) {
-    if (!s.heads) continue;
+  for (int i = 0; i < 2; ++i) {
+    if (!a->heads[i]) continue;
     const bool needs_x = !backward || a->norm;
-    if ((needs_x && !s.x) || (backward && !s.g) || !s.y || (s.weight && !a->norm)) return S2CNN_EINVAL;
-    if (s.gweight && !(backward && a->norm)) return S2CNN_EINVAL;
-    uintptr_t all = reinterpret_cast<uintptr_t>(s.y) | reinterpret_cast<uintptr_t>(s.weight) | reinterpret_cast<uintptr_t>(s.gweight);
-    if (needs_x) all |= reinterpret_cast<uintptr_t>(s.x);
-    if (backward) all |= reinterpret_cast<uintptr_t>(s.g);
+    if ((needs_x && !a->x[i]) || (backward && !a->g[i]) || !a->y[i] || (a->weight[i] && !a->norm)) return S2CNN_EINVAL;
+    if (a->gweight[i] && !(backward && a->norm)) return S2CNN_EINVAL;
+    uintptr_t all = reinterpret_cast<uintptr_t>(a->y[i]) | reinterpret_cast<uintptr_t>(a->weight[i]) | reinterpret_cast<uintptr_t>(a->gweight[i]);
+    if (needs_x) all |= reinterpret_cast<uintptr_t>(a->x[i]);
+    if (backward) all |= reinterpret_cast<uintptr_t>(a->g[i]);
     if (all & mask) return S2CNN_EALIGN;
   }
   if (!aligned8(a->table) || (a->table_stride & 1) || (reinterpret_cast<uintptr_t>(a->index) & 3)) return S2CNN_EALIGN;
   return S2CNN_OK;
 }
-bool wants_sums(const s2cnn_rotary_t& a) { return a.norm && ((a.side[0].heads && a.side[0].gweight) || (a.side[1].heads && a.side[1].gweight)); }
+bool wants_sums(const s2cnn_rotary_t& a) { return a.norm && ((a.heads[0] && a.gweight[0]) || (a.heads[1] && a.gweight[1])); }
 
 }  // namespace rotary
 }  // namespace s2cnn

@@ -19,13 +19,13 @@ _dtype, _shape = attrgetter("dtype"), attrgetter("shape")
 _contiguous, _device, _numel, _address = torch.Tensor.is_contiguous, torch.Tensor.get_device, torch.Tensor.numel, torch.Tensor.data_ptr
 
 
-def _check_list(tensors, dtype, device, what):
-    """Dense tensors of one type on one device."""
+def _check_list(tensors, dtype, device, what, dense=False):
+    """Dense tensors (dense: that is known) of one type on one device."""
     if set(map(_dtype, tensors)) != {dtype}:
         raise RuntimeError("%s of one type only, %s (got %s)" % (what, dtype, ", ".join(sorted(map(str, set(map(_dtype, tensors)))))))
     if set(map(_device, tensors)) != {device}:
         raise RuntimeError("%s on the current GPU only, cuda:%d; there is no CPU path" % (what, torch.cuda.current_device() if torch.cuda.is_available() else 0))
-    if not all(map(_contiguous, tensors)):
+    if not dense and not all(map(_contiguous, tensors)):
         raise RuntimeError("%s have to be contiguous" % what)
 
 
@@ -126,7 +126,7 @@ def adamw_step(params, grads, first, second, step, lr=1e-3, betas=(0.9, 0.999), 
     _check_list(params, dtype, device, "parameters")
     if not all(map(_contiguous, grads)):
         grads = [g.contiguous() for g in grads]
-    _check_list(grads, dtype, device, "gradients")
+    _check_list(grads, dtype, device, "gradients", dense=True)
     assert list(map(_shape, grads)) == list(map(_shape, params))
     _check_states(first, second, scales, sizes, device)
     if masters is not None:

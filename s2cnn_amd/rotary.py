@@ -21,7 +21,7 @@ MAX_HEAD = 256
 MAX_VECTORS = 1 << 31
 POSITIONS = {torch.float32: 0, torch.float64: 1, torch.int32: 2, torch.int64: 3}
 
-_SIDE, _SHARED = struct.Struct("5P"), struct.Struct("2P")             # the pointers of s2cnn_rotary_side_t, and of s2cnn_rotary_t behind its two sides
+_POINTERS = struct.Struct("12P")                         # the first fields of s2cnn_rotary_t
 
 
 def _vectors(t):
@@ -30,84 +30,87 @@ def _vectors(t):
 
 
 @lru_cache(maxsize=1024)
-def _plan(shapes, strides, table, index_stride, norm, interleaved, eps, dtype):
+def _plan(shape, other, strides, table, index_stride, norm, interleaved, eps, dtype):
     """(the library's struct without its pointers, bytes of the workspace of the weights' gradients) of a call of these sizes.
-    strides: per tensor of x, g and y, as torch gives them; table: its batch stride, rows and pairs."""
+    shape, other: of the first tensor and of the second, or None; strides: of x, g and y of the first, then of the second, as torch gives them, or None;
+    table: its batch stride, rows and pairs."""
     a = _hip.Rotary()
-    present = [(shape, of) for shape, of in zip(shapes, strides) if shape is not None]      # one tensor alone is the first
-    a.batch, _, a.n, a.d = present[0][0]
-    for side, (shape, of) in zip(a.side, present):
-        side.heads = shape[1]
-        for name, stride in zip(("x_stride", "g_stride", "y_stride"), of):
-            getattr(side, name)[:] = stride[:3] if stride is not None else (0, 0, 0)
+    a.batch, a.heads[0], a.n, a.d = shape
+    a.heads[1] = 0 if other is None else other[1]
+    for i in range(len(strides) // 3):
+        for to, stride in zip((a.x_stride, a.g_stride, a.y_stride), strides[3 * i:]):
+            to[i][:] = stride[:3] if stride is not None else (0, 0, 0)
     a.table_stride, a.rows, a.pairs = table
     a.index_stride, a.norm, a.interleaved, a.eps, a.dtype = index_stride, norm, interleaved, eps, dtype
-    a.table = 16 if a.pairs else None                       # some address: the sizes are refused without
+    a.table = 16 if a.pairs else None                    # some address: the sizes are refused without
     nbytes = _hip.lib().s2cnn_rotary_workspace(ctypes.byref(a))
     a.table = None
     return bytes(a), nbytes
 
 
-def _run(backward, plan, tensors, table, index, sums):
-    """tensors: (x, weight, g, y, gweight) of each side"""
+def _at(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _run(plan, table, index, backward, x, w, g, y, gw=None, x2=None, w2=None, g2=None, y2=None, gw2=None):
     a = _hip.Rotary.from_buffer_copy(plan[0])
-    tensors = [t for t in tensors if t is not None]
-    for i, t in enumerate(tensors):
-        _SIDE.pack_into(a, i * ctypes.sizeof(_hip.RotarySide), *[0 if x is None else x.data_ptr() for x in t])
-    _SHARED.pack_into(a, 2 * ctypes.sizeof(_hip.RotarySide), 0 if table is None else table.data_ptr(), 0 if index is None else index.data_ptr())
+    _POINTERS.pack_into(a, 0, _at(x), _at(x2), _at(w), _at(w2), _at(g), _at(g2), y.data_ptr(), _at(y2), _at(gw), _at(gw2), _at(table), _at(index))
     if not backward:
         _hip.call("s2cnn_rotary_fwd", ctypes.byref(a), _hip.stream_ptr())
-        return
-    ws = _hip.workspace(plan[1], tensors[0][2].device) if sums else None
-    _hip.call("s2cnn_rotary_bwd", ctypes.byref(a), _hip.ptr_or_none(ws), plan[1] if sums else 0, _hip.stream_ptr())
+    elif gw is None and gw2 is None:
+        _hip.call("s2cnn_rotary_bwd", ctypes.byref(a), None, 0, _hip.stream_ptr())
+    else:
+        ws = _hip.workspace(plan[1], y.device)
+        _hip.call("s2cnn_rotary_bwd", ctypes.byref(a), ws.data_ptr(), plan[1], _hip.stream_ptr())
 
 
-def _sizes(table, index):
-    return ((table.stride(0) if table is not None and table.dim() == 4 and table.size(0) > 1 else 0, *(table.shape[-3:-1] if table is not None else (0, 0))),
-            index.stride(0) if index is not None and index.dim() == 2 and index.size(0) > 1 else 0)
-
-
-def _forward(q, k, q_weight, k_weight, table, index, options):
-    out = [None if x is None else _like(x) for x in (q, k)]
-    if q.size(0) * q.size(2) == 0 or q.size(1) == 0 and (k is None or k.size(1) == 0):
-        return out
-    xs = [None if x is None or not x.numel() else x for x in (q, k)]
-    plan = _plan(tuple(None if x is None else x.shape for x in xs), tuple(None if x is None else (x.stride(), None, y.stride()) for x, y in zip(xs, out)),
-                 *_sizes(table, index), *options)
-    _run(False, plan, [None if x is None else (x, w, None, y, None) for x, w, y in zip(xs, (q_weight, k_weight), out)], table, index, False)
-    return out
+def _forward(q, k, q_weight, k_weight, table, index, sizes):
+    """sizes: of the table and the index, and the options, as _plan takes them"""
+    y = _like(q)
+    z = None if k is None else _like(k)
+    one, two = y.numel() > 0, z is not None and z.numel() > 0
+    if one and two:
+        plan = _plan(q.shape, k.shape, (q.stride(), None, y.stride(), k.stride(), None, z.stride()), *sizes)
+        _run(plan, table, index, False, q, q_weight, None, y, None, k, k_weight, None, z)
+    elif one:
+        _run(_plan(q.shape, None, (q.stride(), None, y.stride()), *sizes), table, index, False, q, q_weight, None, y)
+    elif two:
+        _run(_plan(k.shape, None, (k.stride(), None, z.stride()), *sizes), table, index, False, k, k_weight, None, z)
+    return y, z
 
 
 class _Rotary(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, table, index, options):  # pylint: disable=W
+    def forward(ctx, q, k, q_weight, k_weight, table, index, sizes):  # pylint: disable=W
         ctx.set_materialize_grads(False)
-        norm = options[0]
-        ctx.save_for_backward(q if norm else None, k if norm else None, q_weight, k_weight, table, index)
-        ctx.options = options
-        return tuple(_forward(q, k, q_weight, k_weight, table, index, options))
+        if sizes[2]:
+            ctx.save_for_backward(q, k, q_weight, k_weight, table, index)
+        else:
+            ctx.save_for_backward(None, None, None, None, table, index)
+        ctx.sizes = sizes
+        return _forward(q, k, q_weight, k_weight, table, index, sizes)
 
     @staticmethod
     @_hip.once_differentiable
-    def backward(ctx, *grads):  # pylint: disable=W
-        *xs, q_weight, k_weight, table, index = ctx.saved_tensors
-        weights = (q_weight, k_weight)
-        gx, gw, tensors, shapes, strides = [None, None], [None, None], [None, None], [None, None], [None, None]
-        for i, (x, w, g) in enumerate(zip(xs, weights, grads)):
-            wants = ctx.needs_input_grad[2 + i] and w is not None
-            if g is None or not (ctx.needs_input_grad[i] or wants):
+    def backward(ctx, g, g2):  # pylint: disable=W
+        q, k, q_weight, k_weight, table, index = ctx.saved_tensors
+        wants_q, wants_k, wants_qw, wants_kw = ctx.needs_input_grad[:4]
+        sides, out = [], [None] * 7
+        for i, x, w, g, wants_x, wants_w in ((0, q, q_weight, g, wants_q, wants_qw), (1, k, k_weight, g2, wants_k, wants_kw)):
+            if g is None or not (wants_x or wants_w):
                 continue
             g = _vectors(g)
-            gx[i] = _like(g if x is None else x)
-            if wants:
-                gw[i] = torch.empty_like(w) if g.numel() else torch.zeros_like(w)
-            if g.numel():
-                tensors[i] = (x, w, g, gx[i], gw[i])
-                shapes[i], strides[i] = g.shape, (None if x is None else x.stride(), g.stride(), gx[i].stride())
-        if any(t is not None for t in tensors):
-            plan = _plan(tuple(shapes), tuple(strides), *_sizes(table, index), *ctx.options)
-            _run(True, plan, tensors, table, index, any(t is not None and t[4] is not None for t in tensors))
-        return (*(g if ctx.needs_input_grad[i] else None for i, g in enumerate(gx)), *gw, None, None, None)
+            y = _like(g if x is None else x)
+            some = g.numel() > 0
+            gw = None if not wants_w else torch.empty_like(w) if some else torch.zeros_like(w)
+            out[i], out[2 + i] = y if wants_x else None, gw
+            if some:
+                sides.append((x, w, g, y, gw))
+        if sides:
+            strides = tuple(None if t is None else t.stride() for side in sides for t in (side[0], side[2], side[3]))
+            plan = _plan(sides[0][2].shape, sides[1][2].shape if len(sides) > 1 else None, strides, *ctx.sizes)
+            _run(plan, table, index, True, *sides[0], *(sides[1] if len(sides) > 1 else ()))
+        return tuple(out)
 
 
 def _call(q, k, q_weight, k_weight, table, index, norm, eps, interleaved):
@@ -132,10 +135,11 @@ def _call(q, k, q_weight, k_weight, table, index, norm, eps, interleaved):
     q, k = _vectors(q), None if k is None else _vectors(k)
     table = table.contiguous() if table is not None else None
     index = index.contiguous() if index is not None else None
-    options = (int(norm), int(interleaved), eps, dtype)
+    sizes = ((0, 0, 0) if table is None else (table.stride(0) if table.dim() == 4 and batch > 1 else 0, *table.shape[-3:-1]),
+             0 if index is None or index.dim() == 1 or batch == 1 else n, int(norm), int(interleaved), eps, dtype)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
-        return _Rotary.apply(q, k, q_weight, k_weight, table, index, options)
-    return tuple(_forward(q, k, q_weight, k_weight, table, index, options))
+        return _Rotary.apply(q, k, q_weight, k_weight, table, index, sizes)
+    return _forward(q, k, q_weight, k_weight, table, index, sizes)
 
 
 def rotary(q, k, table, index=None, interleaved=False):

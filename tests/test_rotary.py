@@ -439,10 +439,10 @@ def test_entry_points_refuse_sizes():
     def make(**kw):
         a = _hip.Rotary()
         a.batch, a.n, a.d, a.pairs, a.rows, a.eps, a.table = 2, 3, 16, 8, 3, 1e-6, fake
-        a.side[0].heads, a.side[0].x, a.side[0].g, a.side[0].y = 4, fake, fake, fake
+        a.heads[0], a.x[0], a.g[0], a.y[0] = 4, fake, fake, fake
         for name, v in kw.items():
             if name.startswith("side_"):
-                setattr(a.side[0], name[5:], v)
+                getattr(a, name[5:])[0] = v
             else:
                 setattr(a, name, v)
         return ctypes.byref(a)
