@@ -544,6 +544,13 @@ int s2cnn_adamw_states(const void *const *first, const void *const *second, cons
 size_t s2cnn_grad_norm_workspace(const long *n, const int *dtypes, int count);     /* 0 also for lists that are refused */
 int s2cnn_grad_norm(const void *const *g, const long *n, const int *dtypes, int count, float *out, void *workspace, size_t workspace_bytes,
                     void *stream);
+/* What a program holds in a list of `count` tensors, for the entries above; host memory only.  objects: addresses of the tensors as objects of
+ * the library that they are of, describe: its function of the DLPack exchange interface that fills a DLTensor in (it may need the interpreter's lock,
+ * and the objects have to be such tensors).  addresses [count] and n [count] are written: of the first entries (0 where there are none), numbers of entries;
+ * with known != 0 n is compared with instead.  0 where all tensors are dense, of the type (code, bits) and on the device given, in DLPack's numbers; else the
+ * number, from 1 on, of the first that is not, or that could not be described. */
+int s2cnn_tensor_list(int (*describe)(void *object, void *tensor), const unsigned long long *objects, int count, int code, int bits,
+                      int device_type, int device, unsigned long long *addresses, long long *n, int known);
 
 #ifdef __cplusplus
 }

@@ -132,6 +132,7 @@ SIGNATURES = {
     "s2cnn_adamw_states": (_int, [_vp] * 6 + [_int, _vp]),
     "s2cnn_grad_norm_workspace": (_size_t, [_vp, _vp, _int]),
     "s2cnn_grad_norm": (_int, [_vp, _vp, _vp, _int, _vp, _vp, _size_t, _vp]),
+    "s2cnn_tensor_list": (_int, [_vp, _vp, _int, _int, _int, _int, _int, _vp, _vp, _int]),
     "s2cnn_so3_integrate_grad": (_int, [_c_float_p, _c_float_p, _c_float_p, _int, _long, _vp]),
 }
 
@@ -148,6 +149,25 @@ def lib():
         fn.restype = res
         fn.argtypes = args
     return handle
+
+
+@lru_cache(maxsize=1)
+def tensor_list():
+    """(s2cnn_tensor_list, called with the interpreter's lock held, and torch's function for it): None if this torch has no DLPack exchange interface
+    of version 1, whose first functions are an allocator, two for managed tensors and the one that describes a tensor."""
+    capsule = getattr(torch.Tensor, "__dlpack_c_exchange_api__", None)
+    if capsule is None:
+        return None
+    address = ctypes.pythonapi.PyCapsule_GetPointer
+    address.restype, address.argtypes = _vp, [ctypes.py_object, ctypes.c_char_p]
+    at = address(capsule, b"dlpack_exchange_api")
+    if ctypes.c_uint32.from_address(at).value != 1:
+        return None
+    describe = _vp.from_address(at + 16 + 3 * ctypes.sizeof(_vp)).value          # behind the version and the address of an older interface
+    lib()
+    fn = ctypes.PyDLL(LIB_PATH).s2cnn_tensor_list
+    fn.restype, fn.argtypes = SIGNATURES["s2cnn_tensor_list"]
+    return fn, describe
 
 
 PROBE_LIB_PATH = os.path.join(_HERE, "csrc", "libs2cnn_probe.so")

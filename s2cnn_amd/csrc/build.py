@@ -19,7 +19,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(os.path.dirname(HERE))
 SOURCES = ["so3_mm.hip", "so3_mm_real.hip", "so3_real_basis.hip", "so3_rft.hip", "so3_fft.hip", "s2_fft.hip", "s2_mm.hip",
            "s2_mm_real.hip", "so3_integrate.hip", "attention.hip", "attention_f32.hip", "attention_bf16.hip", "attention_f16.hip",
-           "layer_norm.hip", "rotary.hip", "adamw.hip"]
+           "layer_norm.hip", "rotary.hip", "adamw.hip", "tensor_list.hip"]
 PROBE_SOURCES = ["probe/so3_fft64_probe.hip"]
 LIB = os.path.join(HERE, "libs2cnn_hip.so")
 PROBE_LIB = os.path.join(HERE, "libs2cnn_probe.so")

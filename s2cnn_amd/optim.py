@@ -17,20 +17,38 @@ BLOCK = 256                                              # entries that share a 
 
 _dtype, _shape = attrgetter("dtype"), attrgetter("shape")
 _contiguous, _device, _numel, _address = torch.Tensor.is_contiguous, torch.Tensor.get_device, torch.Tensor.numel, torch.Tensor.data_ptr
+_TENSORS = {torch.Tensor, torch.nn.Parameter}
+_CODES = {torch.float32: (2, 32), torch.float16: (2, 16), torch.bfloat16: (4, 16), torch.float8_e4m3fn: (10, 8), torch.uint8: (1, 8)}      # DLPack's
+_ROCM = 10
 
 
-def _check_list(tensors, dtype, device, what, dense=False):
-    """Dense tensors (dense: that is known) of one type on one device."""
+def _check_list(tensors, dtype, device, what):
+    """Dense tensors of one type on one device."""
     if set(map(_dtype, tensors)) != {dtype}:
         raise RuntimeError("%s of one type only, %s (got %s)" % (what, dtype, ", ".join(sorted(map(str, set(map(_dtype, tensors)))))))
     if set(map(_device, tensors)) != {device}:
         raise RuntimeError("%s on the current GPU only, cuda:%d; there is no CPU path" % (what, torch.cuda.current_device() if torch.cuda.is_available() else 0))
-    if not dense and not all(map(_contiguous, tensors)):
+    if not all(map(_contiguous, tensors)):
         raise RuntimeError("%s have to be contiguous" % what)
 
 
-def _addresses(tensors):
-    return array("Q", map(_address, tensors))
+def _list(tensors, dtype, device, what, n=None, copy=False):
+    """(addresses, numbers of entries, tensors) of dense tensors of one type on one device; n: the numbers that they have to have; copy: others are copied."""
+    lister = _hip.tensor_list()
+    if lister is not None and _TENSORS.issuperset(map(type, tensors)):
+        count = len(tensors)
+        out = array("Q", bytes(8 * count))
+        found = array("q", bytes(8 * count)) if n is None else n
+        objects = array("Q", map(id, tensors))
+        code, bits = _CODES[dtype]
+        if not lister[0](lister[1], objects.buffer_info()[0], count, code, bits, _ROCM, device, out.buffer_info()[0], found.buffer_info()[0], int(n is not None)):
+            return out, found, tensors
+    if copy and not all(map(_contiguous, tensors)):
+        tensors = [t.contiguous() for t in tensors]
+    _check_list(tensors, dtype, device, what)                        # says what is wrong, if anything is
+    found = array("q", map(_numel, tensors))
+    assert n is None or found == n, "%s of other sizes" % what
+    return array("Q", map(_address, tensors)), found, tensors
 
 
 def _at(a):
@@ -55,33 +73,35 @@ def grad_norm(tensors):
     tensors = list(tensors)
     if not tensors:
         return torch.zeros((), device="cuda")
-    device = _current_device(tensors)
-    if not all(map(_contiguous, tensors)):
-        tensors = [t.contiguous() for t in tensors]
+    device, count = _current_device(tensors), len(tensors)
     dtypes = set(map(_dtype, tensors))
     if not dtypes <= _hip.FLOATS.keys():
         raise RuntimeError("tensors of float32, bfloat16 or float16 only (got %s)" % ", ".join(sorted(map(str, dtypes))))
-    if set(map(_device, tensors)) != {device}:
-        raise RuntimeError("tensors on the current GPU only, cuda:%d; there is no CPU path" % device)
-    n, count = array("q", map(_numel, tensors)), len(tensors)
-    kinds = array("i", [_hip.FLOATS[d] for d in map(_dtype, tensors)]) if len(dtypes) > 1 else array("i", [_hip.FLOATS[tensors[0].dtype]]) * count
+    if len(dtypes) == 1:
+        dtype, = dtypes
+        addresses, n, tensors = _list(tensors, dtype, device, "tensors", copy=True)
+        kinds = array("i", [_hip.FLOATS[dtype]]) * count
+    else:
+        if set(map(_device, tensors)) != {device}:
+            raise RuntimeError("tensors on the current GPU only, cuda:%d; there is no CPU path" % device)
+        tensors = [t.contiguous() for t in tensors]
+        addresses, n = array("Q", map(_address, tensors)), array("q", map(_numel, tensors))
+        kinds = array("i", [_hip.FLOATS[d] for d in map(_dtype, tensors)])
     out = torch.empty((), dtype=torch.float32, device=tensors[0].device)
     nbytes = _hip.lib().s2cnn_grad_norm_workspace(_at(n), _at(kinds), count)
     ws = _hip.workspace(nbytes, out.device)
-    addresses = _addresses(tensors)
     _hip.call("s2cnn_grad_norm", _at(addresses), _at(n), _at(kinds), count, out.data_ptr(), ws.data_ptr(), nbytes, _hip.stream_ptr())
     return out
 
 
-def _check_states(first, second, scales, n, device):
-    """Moments in 32 bits (no scales) or 8 of tensors of n entries each."""
+def _states(first, second, scales, n, device):
+    """Addresses of the moments, in 32 bits (no scales) or 8, of tensors of n entries each."""
     assert len(first) == len(second) == len(n) and (scales is None or len(scales) == len(n))
-    _check_list(first, torch.float32 if scales is None else torch.float8_e4m3fn, device, "first moments")
-    _check_list(second, torch.float32 if scales is None else torch.uint8, device, "second moments")
-    assert list(map(_numel, first)) == n and list(map(_numel, second)) == n
-    if scales is not None:
-        _check_list(scales, torch.float32, device, "scales")
-        assert list(map(_numel, scales)) == [2 * ((x + BLOCK - 1) // BLOCK) for x in n]
+    one = _list(first, torch.float32 if scales is None else torch.float8_e4m3fn, device, "first moments", n)[0]
+    two = _list(second, torch.float32 if scales is None else torch.uint8, device, "second moments", n)[0]
+    if scales is None:
+        return one, two, None
+    return one, two, _list(scales, torch.float32, device, "scales", array("q", [2 * ((x + BLOCK - 1) // BLOCK) for x in n]))[0]
 
 
 @torch.no_grad()
@@ -91,7 +111,7 @@ def adamw_step(params, grads, first, second, step, lr=1e-3, betas=(0.9, 0.999), 
     One step of AdamW on a list of tensors, in place:
     m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2, p = p - lr weight_decay p - lr (m / (1 - b1^step)) / (sqrt(v / (1 - b2^step)) + eps).
 
-    :param params, grads: tensors of one type (float32, bfloat16 or float16) on the current GPU; parameters contiguous, none twice
+    :param params, grads: tensors of one type (float32, bfloat16 or float16) on the current GPU, as many entries each; parameters contiguous, none twice
     :param first, second: the moments m and v, as many entries as the parameters: float32, or with scales float8_e4m3fn and uint8
     :param step: which step it is, from 1 on: an int, or an int64 tensor of one element on the GPU that is read when the kernels run
     :param lr: a number, or a float32 tensor of one element on the GPU
@@ -122,28 +142,23 @@ def adamw_step(params, grads, first, second, step, lr=1e-3, betas=(0.9, 0.999), 
     dtype, device = params[0].dtype, _current_device(params)
     if dtype not in _hip.FLOATS:
         raise RuntimeError("float32, bfloat16 or float16 parameters only (got %s)" % dtype)
-    sizes = list(map(_numel, params))
-    _check_list(params, dtype, device, "parameters")
-    if not all(map(_contiguous, grads)):
-        grads = [g.contiguous() for g in grads]
-    _check_list(grads, dtype, device, "gradients", dense=True)
-    assert list(map(_shape, grads)) == list(map(_shape, params))
-    _check_states(first, second, scales, sizes, device)
+    p, n, _ = _list(params, dtype, device, "parameters")
+    assert len(set(p) - {0}) == len(n) - n.count(0), "a parameter twice in the list"
+    g, _, grads = _list(grads, dtype, device, "gradients", n, copy=True)
+    one, two, factors = _states(first, second, scales, n, device)
+    copies = None
     if masters is not None:
         assert dtype != torch.float32, "float32 parameters have no masters"
-        _check_list(masters, torch.float32, device, "masters")
-        assert list(map(_numel, masters)) == sizes
+        assert len(masters) == len(n)
+        copies = _list(masters, torch.float32, device, "masters", n)[0]
     if torch.is_tensor(step):
         _hip.require_gpu_of(torch.int64, step)
     if torch.is_tensor(lr):
         _hip.require_gpu_of(torch.float32, lr)
     _hip.require_gpu_of(torch.float32, norm)
 
-    n = array("q", sizes)
-    lists = [_addresses(t) if t is not None else None for t in (params, grads, first, second, scales, masters)]
-    assert len(set(lists[0]) - {0}) == len(n) - n.count(0), "a parameter twice in the list"
     a = _hip.AdamW()
-    a.p, a.g, a.first, a.second, a.scales, a.masters = map(_at, lists)
+    a.p, a.g, a.first, a.second, a.scales, a.masters = map(_at, (p, g, one, two, factors, copies))
     a.n, a.count, a.dtype, a.bits = _at(n), len(n), _hip.FLOATS[dtype], 32 if scales is None else 8
     if torch.is_tensor(step):
         a.step_at = step.data_ptr()
@@ -170,11 +185,10 @@ def adamw_states(first, second, scales):
         assert not second and not scales
         return [], []
     device = _current_device(first)
-    sizes = list(map(_numel, first))
-    _check_states(first, second, scales, sizes, device)
+    n = array("q", map(_numel, first))
+    lists = _states(first, second, scales, n, device)
     out = [[torch.empty(t.shape, dtype=torch.float32, device=t.device) for t in first] for _ in range(2)]
-    n = array("q", sizes)
-    lists = [_addresses(t) for t in (first, second, scales, *out)]
+    lists += tuple(array("Q", map(_address, t)) for t in out)
     _hip.call("s2cnn_adamw_states", *map(_at, lists), _at(n), len(n), _hip.stream_ptr())
     return tuple(out)
 

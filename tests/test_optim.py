@@ -608,7 +608,7 @@ def test_refusals_of_tensors(hip):
         lists[i][0] = wrong
         with pytest.raises(RuntimeError):
             step(*lists, 1)
-    for i, wrong in ((0, z(3, 4)), (1, z(12)), (2, z(4, 2)), (3, z(13))):
+    for i, wrong in ((0, z(3, 5)), (1, z(13)), (2, z(4, 2)), (3, z(13))):
         lists = good()
         lists[i][0] = wrong
         with pytest.raises(AssertionError):
@@ -635,6 +635,55 @@ def test_refusals_of_tensors(hip):
         s2cnn_amd.grad_norm([z(3), z(3).double()])
     with pytest.raises(RuntimeError):
         s2cnn_amd.grad_norm([z(3), torch.zeros(3)])
+
+
+def test_lists_of_tensors():
+    """What s2cnn_tensor_list says of tensors in host memory (device type 1 of DLPack), against torch's own words."""
+    from array import array
+    from s2cnn_amd import _hip
+    fn, describe = _hip.tensor_list()
+    at = lambda a: a.buffer_info()[0]
+
+    def run(tensors, code=2, bits=32, known=None):
+        objects, out = array("Q", map(id, tensors)), array("Q", bytes(8 * len(tensors)))
+        n = array("q", bytes(8 * len(tensors))) if known is None else array("q", known)
+        return fn(describe, at(objects), len(tensors), code, bits, 1, 0, at(out), at(n), int(known is not None)), list(out), list(n)
+
+    base = torch.zeros(4, 6)
+    good = [base, torch.nn.Parameter(torch.zeros(3)), torch.zeros(()), base.view(-1)[5:], torch.zeros(2, 0, 3), base[2:3, :], base[:1].T, torch.zeros(5, 1, 2)[:, 0]]
+    rc, addresses, n = run(good)
+    assert rc == 0 and n == [t.numel() for t in good] and addresses == [t.data_ptr() for t in good]
+    assert run(good, known=n)[0] == 0 and run(good, known=n[:3] + [1] + n[4:])[0] == 4
+    for wrong in (base.T, base[:, 1:], base.expand(2, 4, 6), torch.zeros(3, dtype=torch.float64), torch.zeros(3, dtype=torch.int32), torch.zeros(3, dtype=torch.complex64)):
+        assert run([base, wrong, base])[0] == 2
+    assert run([base.half()], 2, 16)[0] == run([base.bfloat16()], 4, 16)[0] == run([base.to(torch.float8_e4m3fn)], 10, 8)[0] == run([base.byte()], 1, 8)[0] == 0
+    assert run([base.bfloat16()], 2, 16)[0] == run([base.to(torch.float8_e5m2)], 10, 8)[0] == run([base.char()], 1, 8)[0] == 1
+    with pytest.raises(Exception):
+        run([torch.zeros(2, device="meta")])
+    assert fn(None, None, 0, 2, 32, 1, 0, None, None, 0) == -1 and fn(describe, None, 1, 2, 32, 1, 0, None, None, 0) == -1 and fn(describe, None, -1, 2, 32, 1, 0, None, None, 0) == -1
+
+
+@pytest.mark.gpu
+def test_lists_without_the_exchange_interface(hip, monkeypatch):
+    """Tensor by tensor, as for subclasses of tensors: the same results and refusals."""
+    from s2cnn_amd import _hip
+    shapes = [(300,), (7, 3), (0,)]
+    sides = []
+    for direct in (True, False):
+        if not direct:
+            monkeypatch.setattr(_hip, "tensor_list", lambda: None)
+        params, grads, (first, second, scales) = _random(shapes, BF16, 1), _random(shapes, BF16, 2), _zeros(shapes, 8)
+        grads[1] = grads[1].T.contiguous().T
+        masters = [p.float() for p in params]
+        s2cnn_amd.adamw_step(params, grads, first, second, 1, masters=masters, scales=scales, norm=s2cnn_amd.grad_norm(grads), max_norm=1.0)
+        m, v = s2cnn_amd.adamw_states(first, second, scales)
+        sides.append(params + masters + m + v)
+        for bad in ((grads[0].float(), 1), (params[1].T, 0), (first[0].view(torch.uint8), 2)):
+            lists = [list(x) for x in (params, grads, first, second)]
+            lists[bad[1]][0] = bad[0]
+            with pytest.raises(RuntimeError):
+                s2cnn_amd.adamw_step(*lists, 1, masters=masters, scales=scales)
+    assert all(torch.equal(a, b) for a, b in zip(*sides))
 
 
 def test_entry_points_refuse_lists():
