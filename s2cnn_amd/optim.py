@@ -207,7 +207,8 @@ class AdamW(torch.optim.Optimizer):
         infinite or no number is left out and not counted.  None: neither
     :param seed: of the random rounding of moments in 8 bits; ranks of a job that hold the same parameters need the same
 
-    Steps are counted on the device, for every parameter those that it had a gradient in.  State dicts hold the moments as they are.
+    Steps are counted on the device, for every parameter those that it had a gradient in.  State dicts hold the moments as they are; max_norm and seed are the
+    program's to keep.  A step that a graph captures needs the moments to exist, and the same parameters to have gradients as before: make one before.
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, masters=True, max_norm=None, seed=0):
@@ -215,6 +216,9 @@ class AdamW(torch.optim.Optimizer):
         assert isinstance(seed, int)
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, masters=masters))
         self.max_norm, self.seed, self.norm = max_norm, seed, None
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "max_norm": self.max_norm, "seed": self.seed, "norm": self.norm}
 
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
@@ -225,6 +229,11 @@ class AdamW(torch.optim.Optimizer):
         for p in group["params"]:
             if p.dtype not in _hip.FLOATS:
                 raise RuntimeError("float32, bfloat16 or float16 parameters only (got %s)" % p.dtype)
+
+    @staticmethod
+    def _no_capture(what):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW %s in a captured step, which every replay would do again: make a step before the capture" % what)
 
     def _new_state(self, p, group, count):
         state = {"step": count}
@@ -251,6 +260,7 @@ class AdamW(torch.optim.Optimizer):
             if p.grad.is_sparse:
                 raise RuntimeError("AdamW takes no sparse gradients")
             if not state:
+                self._no_capture("begins with a parameter")
                 key = p.device
                 if key not in fresh:
                     fresh[key] = torch.zeros(1, dtype=torch.int64, device=p.device)
@@ -261,6 +271,7 @@ class AdamW(torch.optim.Optimizer):
         for key, params in stepped.items():
             count = self.state[params[0]]["step"]
             if len(params) < members[key]:                               # some of them are left out of this step: from here on they count apart
+                self._no_capture("leaves a parameter out for the first time")
                 count = count.clone()
                 for p in params:
                     self.state[p]["step"] = count

@@ -568,6 +568,46 @@ def test_captured_training_steps(hip):
     assert {s["step"].item() for o in opts for s in o.state.values()} == {6}
 
 
+@pytest.mark.gpu
+def test_captured_steps_need_a_step_before(hip):
+    """A capture that would make moments, or begin a count of steps, is refused; the program goes on with eager steps."""
+    net = _network()
+    params = list(net.parameters())
+    opt = s2cnn_amd.AdamW(params, lr=0.01)
+    for p in params:
+        p.grad = torch.ones_like(p)
+
+    def refused(match):
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match=match):
+            with torch.cuda.graph(graph):
+                opt.step()
+
+    refused("begins with a parameter")
+    assert not any(opt.state[p] for p in params if p in opt.state)
+    opt.step()
+    params[1].grad = None
+    refused("leaves a parameter out")
+    before = [p.detach().clone() for p in params]
+    opt.step()
+    assert [opt.state[p]["step"].item() for p in params] == [2, 1, 2, 2] and torch.equal(before[1], params[1]) and not torch.equal(before[0], params[0])
+
+
+@pytest.mark.gpu
+def test_copies_of_an_optimizer(hip):
+    """copy.deepcopy and pickles keep the clipping and the seed."""
+    p = torch.nn.Parameter(torch.ones(300, device="cuda"))
+    p.grad = torch.ones_like(p)
+    opt = s2cnn_amd.AdamW([p], lr=0.1, state_bits=8, max_norm=0.5, seed=7)
+    opt.step()
+    twin = copy.deepcopy(opt)
+    q = twin.param_groups[0]["params"][0]
+    q.grad = p.grad.clone()
+    for o in (opt, twin):
+        o.step()
+    assert twin.max_norm == 0.5 and twin.seed == 7 and torch.equal(p, q) and torch.equal(opt.state[p]["second"], twin.state[q]["second"])
+
+
 # ---- refusals -------------------------------------------------------------------------------------------------------
 def test_refusals_before_the_gpu():
     t = [torch.zeros(3)]
