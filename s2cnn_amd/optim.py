@@ -5,7 +5,7 @@ every tensor or every dozen of them; its networks have some tens of tensors of w
 (some fifty a launch), the clipping of gradients is part of it, and the moments may take a quarter of the memory.
 """
 import ctypes
-import math
+import struct
 from array import array
 from operator import attrgetter
 
@@ -20,6 +20,7 @@ _contiguous, _device, _numel, _address = torch.Tensor.is_contiguous, torch.Tenso
 _TENSORS = {torch.Tensor, torch.nn.Parameter}
 _CODES = {torch.float32: (2, 32), torch.float16: (2, 16), torch.bfloat16: (4, 16), torch.float8_e4m3fn: (10, 8), torch.uint8: (1, 8)}      # DLPack's
 _ROCM = 10
+_STEP = struct.Struct("10PqQ6d3i4x")                     # s2cnn_adamw_t
 
 
 def _check_list(tensors, dtype, device, what):
@@ -44,7 +45,8 @@ def _list(tensors, dtype, device, what, n=None, copy=False):
         if not lister[0](lister[1], objects.buffer_info()[0], count, code, bits, _ROCM, device, out.buffer_info()[0], found.buffer_info()[0], int(n is not None)):
             return out, found, tensors
     if copy and not all(map(_contiguous, tensors)):
-        tensors = [t.contiguous() for t in tensors]
+        with torch.no_grad():
+            tensors = [t.contiguous() for t in tensors]
     _check_list(tensors, dtype, device, what)                        # says what is wrong, if anything is
     found = array("q", map(_numel, tensors))
     assert n is None or found == n, "%s of other sizes" % what
@@ -52,7 +54,7 @@ def _list(tensors, dtype, device, what, n=None, copy=False):
 
 
 def _at(a):
-    return a.buffer_info()[0] if a is not None else None
+    return a.buffer_info()[0] if a is not None else 0
 
 
 def _current_device(tensors):
@@ -84,7 +86,8 @@ def grad_norm(tensors):
     else:
         if set(map(_device, tensors)) != {device}:
             raise RuntimeError("tensors on the current GPU only, cuda:%d; there is no CPU path" % device)
-        tensors = [t.contiguous() for t in tensors]
+        with torch.no_grad():
+            tensors = [t.contiguous() for t in tensors]
         addresses, n = array("Q", map(_address, tensors)), array("q", map(_numel, tensors))
         kinds = array("i", [_hip.FLOATS[d] for d in map(_dtype, tensors)])
     out = torch.empty((), dtype=torch.float32, device=tensors[0].device)
@@ -104,7 +107,6 @@ def _states(first, second, scales, n, device):
     return one, two, _list(scales, torch.float32, device, "scales", array("q", [2 * ((x + BLOCK - 1) // BLOCK) for x in n]))[0]
 
 
-@torch.no_grad()
 def adamw_step(params, grads, first, second, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, masters=None, scales=None, norm=None,
                max_norm=None, seed=0):
     """
@@ -157,21 +159,13 @@ def adamw_step(params, grads, first, second, step, lr=1e-3, betas=(0.9, 0.999), 
         _hip.require_gpu_of(torch.float32, lr)
     _hip.require_gpu_of(torch.float32, norm)
 
-    a = _hip.AdamW()
-    a.p, a.g, a.first, a.second, a.scales, a.masters = map(_at, (p, g, one, two, factors, copies))
-    a.n, a.count, a.dtype, a.bits = _at(n), len(n), _hip.FLOATS[dtype], 32 if scales is None else 8
-    if torch.is_tensor(step):
-        a.step_at = step.data_ptr()
-    else:
-        a.step = step
-    if torch.is_tensor(lr):
-        a.lr_at = lr.data_ptr()
-    else:
-        a.lr = lr
-    (a.beta1, a.beta2), a.eps, a.weight_decay, a.seed = betas, eps, weight_decay, seed & 0xFFFFFFFFFFFFFFFF
-    if norm is not None:
-        a.norm, a.max_norm = norm.data_ptr(), max_norm
+    step_at, step = (step.data_ptr(), 0) if torch.is_tensor(step) else (0, step)
+    lr_at, lr = (lr.data_ptr(), 0.0) if torch.is_tensor(lr) else (0, lr)
+    a = _hip.AdamW.from_buffer_copy(_STEP.pack(
+        _at(p), _at(g), _at(one), _at(two), _at(factors), _at(copies), _at(n), lr_at, 0 if norm is None else norm.data_ptr(), step_at, step,
+        seed & 0xFFFFFFFFFFFFFFFF, lr, *betas, eps, weight_decay, max_norm or 0.0, len(n), _hip.FLOATS[dtype], 32 if scales is None else 8))
     _hip.call("s2cnn_adamw_step", ctypes.byref(a), _hip.stream_ptr())
+    torch.autograd.graph.increment_version(params)                   # as other operations in place do
 
 
 def adamw_states(first, second, scales):

@@ -133,7 +133,10 @@ def _call(q, k, q_weight, k_weight, table, index, norm, eps, interleaved):
     _hip.require_gpu_of(torch.float32, table)
     _hip.require_gpu_of(torch.int32, index)
     q, k = _vectors(q), None if k is None else _vectors(k)
-    table = table.contiguous() if table is not None else None
+    if table is not None:
+        table = table.contiguous()
+        if table.data_ptr() & 7:                         # a view at an odd float
+            table = table.clone()
     index = index.contiguous() if index is not None else None
     sizes = ((0, 0, 0) if table is None else (table.stride(0) if table.dim() == 4 and batch > 1 else 0, *table.shape[-3:-1]),
              0 if index is None or index.dim() == 1 or batch == 1 else n, int(norm), int(interleaved), eps, dtype)

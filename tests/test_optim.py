@@ -404,6 +404,53 @@ def test_numbers_on_the_device_and_captured_steps(hip, bits):
             assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)) and torch.equal(a.view(torch.uint8), c.view(torch.uint8))
 
 
+@pytest.mark.gpu
+def test_graphs_that_saved_a_parameter_notice_the_step(hip):
+    """As after any operation in place: a backward pass through the old value is refused, not made with the new one."""
+    p = torch.nn.Parameter(torch.ones(5, device="cuda"))
+    loss = (p * p).sum()
+    s2cnn_amd.adamw_step([p], [torch.ones(5, device="cuda")], [torch.zeros(5, device="cuda")], [torch.zeros(5, device="cuda")], 1)
+    with pytest.raises(RuntimeError, match="inplace"):
+        loss.backward()
+
+
+@pytest.mark.gpu
+def test_two_graphs_and_streams_between_each_other(hip):
+    """Captured steps of two lists, replayed in turns on two streams with eager norms between them: each as by itself."""
+    shapes = [(3000,), (77, 5)]
+    lists = [(_random(shapes, F32, i), _random(shapes, F32, 10 + i, 0.1), *_zeros(shapes, 8)) for i in range(2)]
+    alone = [[[t.clone() for t in x] for x in side] for side in lists]
+    counts = [torch.zeros(1, dtype=torch.int64, device="cuda") for _ in range(2)]
+    graphs, norms = [torch.cuda.CUDAGraph() for _ in range(2)], [None, None]
+
+    def step(side, count, seed):
+        params, grads, first, second, scales = side
+        norm = s2cnn_amd.grad_norm(grads)
+        s2cnn_amd.adamw_step(params, grads, first, second, count, scales=scales, norm=norm, max_norm=0.3, seed=seed)
+        return norm
+
+    s2cnn_amd.grad_norm(lists[0][1])
+    torch.cuda.synchronize()
+    for i, graph in enumerate(graphs):
+        with torch.cuda.graph(graph):
+            counts[i].add_(1)
+            norms[i] = step(lists[i], counts[i], i)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for turn in range(4):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        other = s2cnn_amd.grad_norm(lists[1][1])
+        torch.cuda.synchronize()
+        assert torch.equal(other, norms[1])
+    for i in range(2):
+        for turn in range(4):
+            step(alone[i], turn + 1, i)
+        for a, b in zip(lists[i], alone[i]):
+            assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(a, b))
+
+
 # ---- the norm -------------------------------------------------------------------------------------------------------
 @pytest.mark.gpu
 def test_grad_norm(hip):

@@ -273,6 +273,18 @@ def test_many_vectors_and_far_offsets(hip):
 
 
 @pytest.mark.gpu
+def test_tables_at_any_address_and_stride(hip):
+    n, d, pairs = 20, 24, 9
+    table = _table(n, pairs).cuda()
+    x = torch.randn(2, 3, n, d, generator=torch.Generator().manual_seed(2)).cuda()
+    want = s2cnn_amd.rotary(x, None, table)[0]
+    flat = torch.empty(1 + table.numel(), device="cuda")
+    for t in (flat[1:].view(table.shape).copy_(table), table.permute(2, 0, 1).contiguous().permute(1, 2, 0), table.expand(2, n, pairs, 2),
+              torch.cat([table, table], -1)[..., :2]):
+        assert torch.equal(t.expand_as(table) if t.dim() == 3 else t[0], table) and torch.equal(s2cnn_amd.rotary(x, None, t)[0], want)
+
+
+@pytest.mark.gpu
 def test_empty_tensors(hip):
     table = _table(4, 3).cuda()
     w = torch.ones(6, device="cuda", requires_grad=True)
