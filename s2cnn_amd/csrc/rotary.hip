@@ -11,7 +11,12 @@
 // it reads anyway.  A vector belongs to a group of L lanes (a power of two).  A lane holds two chunks of 16 bytes, so that both entries of a pair
 // are its own: no exchange between lanes but the sums over a vector.  Where a chunk would run past the end of its part, it begins earlier and
 // overlaps the one before (both lanes form the same numbers; sums count them once), so that all accesses are 16 bytes wide, at any alignment; only
-// parts shorter than a chunk are loaded entry by entry.
+// parts shorter than a chunk are loaded entry by entry, in kernels of their own (FULL; rotations of 4 x 16 heads x 4096 places x 64 in float32, both ways:
+// 51 us, with the tests for tails 65).
+//
+// Measured, with a copy of 1 GiB at 5.1 TB/s: 4 x (32 + 8) heads x 8192 places x 128 in bfloat16: forward 122 us, 5.5 TB/s, backward 185 to 195 us, 5.2 to
+// 5.4 TB/s, and 4 us for the sums of its weights' gradients; tensors of 256 MB or more go past the caches (in them: 127 and 205 to 215 us).  A
+// batch of 32 x 10 heads x 400 places of 20 in float32: 9 and 12 us, a launch, two trips to memory and their instructions; single places 3 to 5 us.
 #include "chunk.h"
 
 namespace s2cnn {
@@ -56,6 +61,7 @@ struct Args {
   long table_stride, index_stride;      // of the batch
   int rows, d, pairs, units, lanes, log_lanes;
   float inv_d, eps, sign;
+  bool stream;
 };
 
 // The part of a vector that a lane holds.
@@ -101,18 +107,18 @@ inline int units_of(int V, int d, int pairs, bool neighbours) {
 }
 
 // The first n entries at p, the others zero, in 16 bytes: one load, or entry by entry.
-template <class T, bool FULL> __device__ __forceinline__ uint4 load(const T* p, int n) {
+template <class T, bool FULL> __device__ __forceinline__ uint4 load(const T* p, int n, bool stream = false) {
   constexpr int N = Chunk<T>::N;
-  if (FULL || n == N) return load_chunk<T>(p, N);
+  if (FULL || n == N) return load_chunk<T>(p, N, FULL && stream);
   n = fresh(n);
   float v[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = i < n ? (float)p[i] : 0.f;
   return Chunk<T>::put(v);
 }
-template <class T, bool FULL> __device__ __forceinline__ void store(T* p, int n, const float (&v)[Chunk<T>::N]) {
+template <class T, bool FULL> __device__ __forceinline__ void store(T* p, int n, const float (&v)[Chunk<T>::N], bool stream) {
   constexpr int N = Chunk<T>::N;
-  if (FULL || n == N) return store_chunk<T>(p, N, v);
+  if (FULL || n == N) return store_chunk<T>(p, N, v, FULL && stream);
   n = fresh(n);
 #pragma unroll
   for (int i = 0; i < N; ++i)
@@ -236,8 +242,8 @@ template <class T, Pass PASS, bool NEIGHBOURS, int HEADS, bool FULL> __global__ 
 #pragma unroll
     for (int h = 0; h < HEADS; ++h)
       if (h < heads) {
-        raw[h][0] = load<T, FULL>(x + h * s.x.head + part.a, part.na), raw[h][1] = load<T, FULL>(x + h * s.x.head + part.b, part.nb);
-        if (PASS == NORM_BACK) graw[h][0] = load<T, FULL>(g + h * s.g.head + part.a, part.na), graw[h][1] = load<T, FULL>(g + h * s.g.head + part.b, part.nb);
+        raw[h][0] = load<T, FULL>(x + h * s.x.head + part.a, part.na, p.stream), raw[h][1] = load<T, FULL>(x + h * s.x.head + part.b, part.nb, p.stream);
+        if (PASS == NORM_BACK) graw[h][0] = load<T, FULL>(g + h * s.g.head + part.a, part.na, p.stream), graw[h][1] = load<T, FULL>(g + h * s.g.head + part.b, part.nb, p.stream);
       }
     int row = (int)place;
     if (p.index) row = p.index[outer * p.index_stride + place];
@@ -275,8 +281,8 @@ template <class T, Pass PASS, bool NEIGHBOURS, int HEADS, bool FULL> __global__ 
         }
       }
       if (h < heads && part.own) {
-        store<T, FULL>(y + h * s.y.head + part.a, part.na, a);
-        store<T, FULL>(y + h * s.y.head + part.b, part.nb, b);
+        store<T, FULL>(y + h * s.y.head + part.a, part.na, a, p.stream);
+        store<T, FULL>(y + h * s.y.head + part.b, part.nb, b, p.stream);
       }
     }
   }
@@ -326,7 +332,7 @@ template <class T> __global__ __launch_bounds__(1024) void weights_kernel(const 
 // An angle is formed in quarters of a turn and in 64 bits; adding 1.5 2^52 leaves the nearest whole number, whose lowest bits say which sine or cosine to
 // take of what is left, -1/2 .. 1/2, in 32 bits: positions of a million lose nothing.  Sine and cosine of that are polynomials of its square that interpolate
 // them at Chebyshev's points, off by 1.5 2^-24 and 2^-24.  A thread keeps its PER neighbouring pairs and takes one row after the other, so that a position is
-// converted once for 16 bytes of the table.  262144 rows of 64 pairs, 134 MB: see the launch.
+// converted once for 16 bytes of the table.  262144 rows of 64 pairs, 134 MB: 26 to 28 us, 4.8 to 5.1 TB/s (one pair a thread and the library's sincospi: 43).
 __device__ __forceinline__ float2 turn_of(double quarters, float scale) {
   double whole = (quarters + 0x1.8p52) - 0x1.8p52;
   unsigned q = (unsigned)__double_as_longlong(quarters + 0x1.8p52);
@@ -393,8 +399,9 @@ bool sizes_ok(const s2cnn_rotary_t* a) {
   return true;
 }
 
-// Runs of four heads (two where x and g are read) where that leaves every group two runs or more, else of one.  As many workgroups as run at once, four a CU
-// (three; runs of one head: eight, four), or fewer that take as many turns.
+// Runs of four heads (two where x and g are read) where that leaves every group two runs or more, else of one: 4 x 40 heads x 8192 places of 128 in bfloat16,
+// forward and backward, 128 and 205 us, of one head each 160 and 224; 32 x 10 heads x 400 places of 20 in float32 the other way round, 10.7 and 14.5 us, of one 9.4
+// and 12.5.  As many workgroups as run at once, four a CU (three; runs of one head: eight, four), or fewer that take as many turns.
 Plan plan_of(const s2cnn_rotary_t& a, bool two) {
   Plan p;
   p.units = units_of(a.dtype == S2CNN_F32 ? 4 : 8, a.d, a.pairs, a.interleaved != 0);
@@ -451,6 +458,7 @@ Args args_of(const s2cnn_rotary_t& a, const Plan& p, bool backward, float* parti
   k.rows = a.rows, k.d = a.d, k.pairs = a.pairs, k.units = p.units, k.lanes = p.lanes, k.log_lanes = p.log_lanes;
   k.inv_d = 1.f / (float)a.d;
   k.eps = a.eps;
+  k.stream = (size_t)(p.items[0] + p.items[1]) * p.most * a.d * (a.dtype == S2CNN_F32 ? 4 : 2) >= STREAM_BYTES;
   k.sign = backward ? -1.f : 1.f;
   return k;
 }

@@ -476,6 +476,17 @@ def test_grad_norm(hip):
 
 
 @pytest.mark.gpu
+def test_grad_norm_of_lists_larger_than_the_caches(hip):
+    """From 256 MB on they are read past the caches."""
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    for dtype, n in ((F32, 70000001), (BF16, 140000003)):
+        t = torch.randn(n, device="cuda", generator=gen).to(dtype)
+        want = math.sqrt(sum(p.double().square().sum().item() for p in t.split(1 << 24)))
+        assert abs(s2cnn_amd.grad_norm([t]).item() - want) <= 2 * W * want
+        assert torch.equal(s2cnn_amd.grad_norm([t[:1 << 20]]), s2cnn_amd.grad_norm([t[:1 << 20].clone()]))
+
+
+@pytest.mark.gpu
 def test_grad_norm_of_extreme_values(hip):
     for value in (1e30, 1e-30, 3e38, 1e-44):
         t = torch.full((1000,), value, device="cuda")

@@ -273,6 +273,27 @@ def test_many_vectors_and_far_offsets(hip):
 
 
 @pytest.mark.gpu
+@LAYOUTS
+def test_tensors_larger_than_the_caches(hip, interleaved):
+    """From 256 MB on accesses go past the caches: the same bits as in pieces, forward and backward."""
+    n, d, pairs = 300001, 64, 32
+    table = _table(n, pairs).cuda()
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x, g = (torch.randn(1, n, 8, d, device="cuda", generator=gen).bfloat16().transpose(1, 2) for _ in range(2))
+    w = (torch.rand(d, device="cuda", generator=gen) + 0.5).bfloat16()
+
+    def both(x, g, table):
+        x = x.detach().requires_grad_()
+        y = s2cnn_amd.norm_rotary(x, None, w, table=table, interleaved=interleaved)[0]
+        return y.detach(), torch.autograd.grad(y, x, g)[0], s2cnn_amd.rotary(x.detach(), None, table, interleaved=interleaved)[0]
+
+    whole = both(x, g, table)
+    for at in (0, 123457, n - 1000):
+        part = both(*(t[:, :, at:at + 1000] for t in (x, g)), table[at:at + 1000])
+        assert all(torch.equal(a[:, :, at:at + 1000], b) for a, b in zip(whole, part))
+
+
+@pytest.mark.gpu
 def test_tables_at_any_address_and_stride(hip):
     n, d, pairs = 20, 24, 9
     table = _table(n, pairs).cuda()
