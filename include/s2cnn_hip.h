@@ -485,7 +485,7 @@ int s2cnn_dropout(const void *x, void *y, long n, double p, unsigned long long s
  *          the vector is not turned; from rows on: what would be turned becomes NaN.
  * fwd    : y from x.   bwd: y (the gradient of x) from g (that of fwd's y), with norm from x too and, where not NULL, gweight [d].
  * Types: dtype; arithmetic float32, results rounded once.  A tensor's vectors are contiguous, strides are those of (batch, head, n) in entries.
- * batch n heads < 2^31 for each side.  Results do not depend on the order of execution.
+ * batch n heads < 2^31 for each side.  Results do not depend on the order of execution, a vector's not on what else is in the call.
  */
 typedef struct s2cnn_rotary_t {
   const void *x[2], *weight[2], *g[2];      /* weight: [d], or NULL (ones)                  */

@@ -151,19 +151,21 @@ template <int V> __device__ __forceinline__ void load_turns(const Args& p, const
   }
 }
 
+// Sums of products are written as fused operations, here and below, and the compiler makes no others: a vector's result is the same bits in every kernel.
 template <int V, bool NEIGHBOURS> __device__ __forceinline__ void turn(const float (&c)[V], const float (&s)[V], float (&a)[V], float (&b)[V]) {
+#pragma clang fp contract(off)
   if constexpr (NEIGHBOURS) {
 #pragma unroll
     for (int i = 0; i < V / 2; ++i) {
       const float x = a[2 * i], y = a[2 * i + 1], z = b[2 * i], w = b[2 * i + 1];
-      a[2 * i] = x * c[i] - y * s[i], a[2 * i + 1] = x * s[i] + y * c[i];
-      b[2 * i] = z * c[V / 2 + i] - w * s[V / 2 + i], b[2 * i + 1] = z * s[V / 2 + i] + w * c[V / 2 + i];
+      a[2 * i] = fmaf(x, c[i], -(y * s[i])), a[2 * i + 1] = fmaf(x, s[i], y * c[i]);
+      b[2 * i] = fmaf(z, c[V / 2 + i], -(w * s[V / 2 + i])), b[2 * i + 1] = fmaf(z, s[V / 2 + i], w * c[V / 2 + i]);
     }
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const float x = a[i], y = b[i];
-      a[i] = x * c[i] - y * s[i], b[i] = x * s[i] + y * c[i];
+      a[i] = fmaf(x, c[i], -(y * s[i])), b[i] = fmaf(x, s[i], y * c[i]);
     }
   }
 }
@@ -205,6 +207,7 @@ enum Pass { TURN, NORM, NORM_BACK };           // TURN: both directions of the r
 
 // FULL: no lane's chunks are shorter than 16 bytes.  HEADS: the most heads of a run, whose loads are under way together and which share the cosines and sines of their place.
 template <class T, Pass PASS, bool NEIGHBOURS, int HEADS, bool FULL> __global__ __launch_bounds__(THREADS, PASS == NORM_BACK ? 3 : 4) void rotary_kernel(Args p) {
+#pragma clang fp contract(off)
   constexpr int V = Chunk<T>::N;
   const bool second = blockIdx.x >= p.blocks0;
   const Side& s = p.side[__builtin_amdgcn_readfirstlane((int)second)];        // a number, so that the fields are loaded together
