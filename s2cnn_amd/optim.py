@@ -298,13 +298,10 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         """States keep their types (torch's own method takes them to the parameters')."""
         super().load_state_dict(state_dict)
-        saved = [i for group in state_dict["param_groups"] for i in group["params"]]
-        params = [p for group in self.param_groups for p in group["params"]]
-        counts = {}
-        for i, p in zip(saved, params):
-            if i not in state_dict["state"]:
-                continue
-            state = {k: t.detach().to(p.device, copy=True) for k, t in state_dict["state"][i].items()}
-            count = (int(state["step"]), p.device)
-            state["step"] = counts.setdefault(count, state["step"])
-            self.state[p] = state
+        for group, from_group in zip(self.param_groups, state_dict["param_groups"]):
+            counts = {}                                              # parameters of a group that had as many steps go on together
+            for i, p in zip(from_group["params"], group["params"]):
+                if i in state_dict["state"]:
+                    state = {k: t.detach().to(p.device, copy=True) for k, t in state_dict["state"][i].items()}
+                    state["step"] = counts.setdefault((int(state["step"]), p.device), state["step"])
+                    self.state[p] = state

@@ -574,6 +574,22 @@ def test_state_dicts(hip, bits, dtype):
 
 
 @pytest.mark.gpu
+def test_loaded_groups_count_their_own_steps(hip):
+    """Two groups of as many steps, saved and loaded: one step counts one in each."""
+    params = [torch.nn.Parameter(torch.ones(30, device="cuda")) for _ in range(4)]
+    make = lambda: s2cnn_amd.AdamW([{"params": params[:2]}, {"params": params[2:], "lr": 0.5}], lr=0.1)
+    for p in params:
+        p.grad = torch.ones_like(p)
+    opt = make()
+    opt.step()
+    again = make()
+    again.load_state_dict(opt.state_dict())
+    again.step()
+    assert [again.state[p]["step"].item() for p in params] == [2] * 4 and len({id(again.state[p]["step"]) for p in params}) == 2
+    assert [opt.state[p]["step"].item() for p in params] == [1] * 4
+
+
+@pytest.mark.gpu
 def test_groups_types_and_steps_left_out(hip):
     """Parameters of two types and a group in 8 bits; a step without a finite norm is neither made nor counted."""
     a, b, c = (torch.nn.Parameter(torch.ones(300, device="cuda", dtype=d)) for d in (F32, BF16, F32))
