@@ -33,17 +33,26 @@ def _check_list(tensors, dtype, device, what):
         raise RuntimeError("%s have to be contiguous" % what)
 
 
+def _described(tensors, dtype, device, n=None):
+    """(addresses, numbers of entries) of dense tensors of one type on one device, n the numbers that they have to have; None if they are not, or if
+    the library cannot ask."""
+    lister = _hip.tensor_list()
+    if lister is None or not _TENSORS.issuperset(map(type, tensors)):
+        return None
+    count = len(tensors)
+    out = array("Q", bytes(8 * count))
+    found = array("q", bytes(8 * count)) if n is None else n
+    objects = array("Q", map(id, tensors))
+    code, bits = _CODES[dtype]
+    rc = lister[0](lister[1], objects.buffer_info()[0], count, code, bits, _ROCM, device, out.buffer_info()[0], found.buffer_info()[0], int(n is not None))
+    return (out, found) if rc == 0 else None
+
+
 def _list(tensors, dtype, device, what, n=None, copy=False):
     """(addresses, numbers of entries, tensors) of dense tensors of one type on one device; n: the numbers that they have to have; copy: others are copied."""
-    lister = _hip.tensor_list()
-    if lister is not None and _TENSORS.issuperset(map(type, tensors)):
-        count = len(tensors)
-        out = array("Q", bytes(8 * count))
-        found = array("q", bytes(8 * count)) if n is None else n
-        objects = array("Q", map(id, tensors))
-        code, bits = _CODES[dtype]
-        if not lister[0](lister[1], objects.buffer_info()[0], count, code, bits, _ROCM, device, out.buffer_info()[0], found.buffer_info()[0], int(n is not None)):
-            return out, found, tensors
+    known = _described(tensors, dtype, device, n)
+    if known is not None:
+        return (*known, tensors)
     if copy and not all(map(_contiguous, tensors)):
         with torch.no_grad():
             tensors = [t.contiguous() for t in tensors]
@@ -75,15 +84,15 @@ def grad_norm(tensors):
     tensors = list(tensors)
     if not tensors:
         return torch.zeros((), device="cuda")
-    device, count = _current_device(tensors), len(tensors)
-    dtypes = set(map(_dtype, tensors))
-    if not dtypes <= _hip.FLOATS.keys():
-        raise RuntimeError("tensors of float32, bfloat16 or float16 only (got %s)" % ", ".join(sorted(map(str, dtypes))))
-    if len(dtypes) == 1:
-        dtype, = dtypes
-        addresses, n, tensors = _list(tensors, dtype, device, "tensors", copy=True)
+    device, count, dtype = _current_device(tensors), len(tensors), tensors[0].dtype
+    known = _described(tensors, dtype, device) if dtype in _hip.FLOATS else None
+    if known is not None:
+        addresses, n = known
         kinds = array("i", [_hip.FLOATS[dtype]]) * count
-    else:
+    else:                                                # of several types, or not all dense
+        dtypes = set(map(_dtype, tensors))
+        if not dtypes <= _hip.FLOATS.keys():
+            raise RuntimeError("tensors of float32, bfloat16 or float16 only (got %s)" % ", ".join(sorted(map(str, dtypes))))
         if set(map(_device, tensors)) != {device}:
             raise RuntimeError("tensors on the current GPU only, cuda:%d; there is no CPU path" % device)
         with torch.no_grad():
