@@ -223,7 +223,9 @@ template <class T, int BITS, bool MASTER, bool FULL> __device__ __forceinline__ 
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     if constexpr (MASTER) p[i] = (float)(T)master[i] == p[i] ? master[i] : p[i];     // where it is not its master's rounding, the program has set it since
-    const float denominator = __builtin_amdgcn_sqrtf(v[i] * f.inverse2) + h.eps;
+    // the instruction takes a subnormal number's root for zero: small ones are taken times 2^32
+    const bool small = v[i] < 0x1p-96f;
+    const float denominator = fmaf(__builtin_amdgcn_sqrtf(v[i] * (small ? f.inverse2 * 0x1p32f : f.inverse2)), small ? 0x1p-16f : 1.f, h.eps);
     p[i] = fmaf(-f.size, m[i] * __builtin_amdgcn_rcpf(denominator), fmaf(-f.decay, p[i], p[i]));
     // The parameter is the rounding of the float32 that is stored: without this the compiler makes one operation of the last product, sum and conversion
     // to float16, which rounds once and may differ.

@@ -240,6 +240,16 @@ def test_random_rounding_has_the_right_mean(hip):
 
 
 @pytest.mark.gpu
+def test_gradients_whose_squares_are_subnormal(hip):
+    """An eps far below them: the quotient of the moments is one, as exactly as the square is (2^-13 of 2^-136, half of it in the root)."""
+    for size in (2.0 ** -68, 2.0 ** -64, 2.0 ** -40, 2.0 ** 60):
+        p, g = torch.zeros(600, device="cuda"), torch.full((600,), size, device="cuda")
+        m, v = torch.zeros(600, device="cuda"), torch.zeros(600, device="cuda")
+        s2cnn_amd.adamw_step([p], [g], [m], [v], 1, lr=1.0, betas=(0.0, 0.0), eps=1e-30, weight_decay=0.0)
+        assert (p + 1).abs().max() <= 2.0 ** -13, size
+
+
+@pytest.mark.gpu
 def test_small_second_moments_never_vanish(hip):
     g = torch.full((300,), 1e-12, device="cuda")
     g[0], g[7], g[299] = 1.0, 0.0, 0.0
