@@ -395,7 +395,7 @@ bool sizes_ok(const s2cnn_rotary_t* a) {
   if (a->batch < 1 || a->n < 1 || a->d < 1 || a->d > MAX_D || a->pairs < 0 || 2 * a->pairs > a->d) return false;
   if (a->pairs && (!a->table || a->rows < 1 || (!a->index && a->rows < a->n))) return false;
   if (!a->pairs && (a->table || a->index)) return false;
-  if (a->heads[0] < 1 || a->heads[1] < 0 || (a->norm && !(a->eps > 0.f))) return false;
+  if (a->heads[0] < 1 || a->heads[1] < 0 || (a->norm && !(a->eps >= 0x1p-126f))) return false;
   const long limit = 1L << 31;
   for (int heads : a->heads)
     if ((long)a->batch * a->n >= limit || (heads && (long)a->batch * a->n >= limit / heads)) return false;

@@ -170,11 +170,11 @@ def norm_rotary(q, k, q_weight=None, k_weight=None, table=None, index=None, eps=
 
     :param q, k, table, index, interleaved: as for `rotary`
     :param q_weight, k_weight: [d], the type of q, shared by the heads, or None
-    :param eps: > 0
+    :param eps: >= 2^-126
     :return (q, k): as for `rotary`.  Squares are summed in float32: entries are below 2^63 in size
     """
     eps = ctypes.c_float(eps).value
-    assert 0.0 < eps < math.inf
+    assert 2.0 ** -126 <= eps < math.inf
     assert q_weight is None or q_weight.shape == q.shape[-1:]
     assert k_weight is None or (k is not None and k_weight.shape == k.shape[-1:])
     q_weight = q_weight.contiguous() if q_weight is not None else None

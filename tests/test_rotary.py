@@ -238,6 +238,8 @@ def test_large_small_and_infinite_entries(hip):
     y = s2cnn_amd.norm_rotary(x, None, table=table)[0][0, 0]
     assert (y[0] == 0).all() and torch.isfinite(y[1:3]).all() and torch.isfinite(y[5]).all() and y[3:5].isnan().any(-1).all()
     assert abs(y[1].norm().item() - 4) < 1e-5 and y[2].abs().max() < 1e-26
+    least = s2cnn_amd.norm_rotary(x, None, table=table, eps=2.0 ** -126)[0][0, 0]
+    assert (least[0] == 0).all() and torch.isfinite(least[2]).all() and abs(least[5].norm().item() - 4) < 1e-5
     turned = s2cnn_amd.rotary(x, None, table)[0][0, 0]
     assert torch.isfinite(turned[[0, 1, 2, 5]]).all() and torch.isfinite(turned[3, 1:8]).all() and torch.isfinite(turned[3, 9:]).all()
 
@@ -435,7 +437,7 @@ def test_refusals_before_the_gpu():
                 lambda: s2cnn_amd.rotary(q, k, table, index=torch.zeros(4, dtype=torch.int32)), lambda: s2cnn_amd.rotary(q, k, table.requires_grad_()),
                 lambda: s2cnn_amd.norm_rotary(q, k, index=torch.zeros(5, dtype=torch.int32)), lambda: s2cnn_amd.norm_rotary(q, k, torch.ones(7)),
                 lambda: s2cnn_amd.norm_rotary(q, k, None, torch.ones(2, 8)), lambda: s2cnn_amd.norm_rotary(q, None, None, torch.ones(8)),
-                lambda: s2cnn_amd.norm_rotary(q, k, eps=0.0), lambda: s2cnn_amd.norm_rotary(q, k, eps=1e-60), lambda: s2cnn_amd.norm_rotary(q, k, eps=float("nan")),
+                lambda: s2cnn_amd.norm_rotary(q, k, eps=0.0), lambda: s2cnn_amd.norm_rotary(q, k, eps=1e-60), lambda: s2cnn_amd.norm_rotary(q, k, eps=1e-39), lambda: s2cnn_amd.norm_rotary(q, k, eps=float("nan")),
                 lambda: s2cnn_amd.rotary(torch.zeros(1, 1, 1, 258), None, torch.zeros(1, 128, 2)),
                 lambda: s2cnn_amd.rotary_table(torch.zeros(4, 2), torch.zeros(1, 3, dtype=torch.float64)),
                 lambda: s2cnn_amd.rotary_table(torch.zeros(4, 1), torch.zeros(1, 129, dtype=torch.float64)),
