@@ -125,52 +125,45 @@ template <class T, bool FULL> __device__ __forceinline__ void store(T* p, int n,
     if (i < n) p[i] = (T)v[i];
 }
 
-// cos and sin of V pairs from `pair` on of a row; of pairs that do not turn 1 and 0, of a row that is not there NaN
-template <int V> __device__ __forceinline__ void load_turns(const Args& p, const float2* row, bool there, int pair, float (&c)[V], float (&s)[V]) {
-  if (there && pair + V <= p.pairs) {
+// cos and sin of the first `turned` of V pairs from `pair` on of a row; of a row that is not there NaN.  FULL: all or none of them.
+template <int V, bool FULL> __device__ __forceinline__ void load_turns(const float2* row, bool there, int pair, int turned, float sign, float (&c)[V], float (&s)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) c[i] = s[i] = __builtin_nanf("");
+  if (there && turned == V) {
     typedef float loose __attribute__((ext_vector_type(4), aligned(8)));
     const loose* const at = reinterpret_cast<const loose*>(row + pair);
 #pragma unroll
     for (int i = 0; i < V / 2; ++i) {
       const loose t = at[i];
-      c[2 * i] = t[0], s[2 * i] = t[1] * p.sign, c[2 * i + 1] = t[2], s[2 * i + 1] = t[3] * p.sign;
+      c[2 * i] = t[0], s[2 * i] = t[1] * sign, c[2 * i + 1] = t[2], s[2 * i + 1] = t[3] * sign;
     }
-    return;
-  }
-  pair = fresh(pair);
-  if (pair >= p.pairs) {
+  } else if (!FULL && there) {
+    turned = fresh(turned);
 #pragma unroll
-    for (int i = 0; i < V; ++i) c[i] = 1.f, s[i] = 0.f;
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    float2 t = make_float2(1.f, 0.f);
-    if (pair + i < p.pairs) t = there ? row[pair + i] : make_float2(__builtin_nanf(""), __builtin_nanf(""));
-    c[i] = t.x, s[i] = t.y * p.sign;
+    for (int i = 0; i < V; ++i)
+      if (i < turned) c[i] = row[pair + i].x, s[i] = row[pair + i].y * sign;
   }
 }
 
+// The first `turned` pairs of a lane.  Others are left alone rather than turned by nothing: 0 times an infinity is none.
 // Sums of products are written as fused operations, here and below, and the compiler makes no others: a vector's result is the same bits in every kernel.
-template <int V, bool NEIGHBOURS> __device__ __forceinline__ void turn(const float (&c)[V], const float (&s)[V], float (&a)[V], float (&b)[V]) {
+template <int V, bool NEIGHBOURS, bool FULL> __device__ __forceinline__ void turn(int turned, const float (&c)[V], const float (&s)[V], float (&a)[V], float (&b)[V]) {
 #pragma clang fp contract(off)
-  if constexpr (NEIGHBOURS) {
+  if (!FULL) turned = fresh(turned);
+  const bool whole = turned == V;
 #pragma unroll
-    for (int i = 0; i < V / 2; ++i) {
-      const float x = a[2 * i], y = a[2 * i + 1], z = b[2 * i], w = b[2 * i + 1];
-      a[2 * i] = fmaf(x, c[i], -(y * s[i])), a[2 * i + 1] = fmaf(x, s[i], y * c[i]);
-      b[2 * i] = fmaf(z, c[V / 2 + i], -(w * s[V / 2 + i])), b[2 * i + 1] = fmaf(z, s[V / 2 + i], w * c[V / 2 + i]);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float x = a[i], y = b[i];
-      a[i] = fmaf(x, c[i], -(y * s[i])), b[i] = fmaf(x, s[i], y * c[i]);
-    }
+  for (int i = 0; i < V; ++i) {
+    float& u = NEIGHBOURS ? (i < V / 2 ? a[(2 * i) % V] : b[(2 * i) % V]) : a[i];
+    float& v = NEIGHBOURS ? (i < V / 2 ? a[(2 * i + 1) % V] : b[(2 * i + 1) % V]) : b[i];
+    const float x = u, y = v;
+    const bool mine = FULL ? whole : i < turned;
+    u = mine ? fmaf(x, c[i], -(y * s[i])) : x;
+    v = mine ? fmaf(x, s[i], y * c[i]) : y;
   }
 }
 
 __device__ __forceinline__ float sum_of(float v, int lanes) {           // over a group, `lanes` the same in all of the launch
+  asm volatile("" : "+s"(lanes));                                       // compared here each time, as above
   if (lanes > 1) v = add_dpp<0xB1>(v);
   if (lanes > 2) v = add_dpp<0x4E>(v);
   if (lanes > 4) v = add_dpp<0x141>(v);
@@ -205,7 +198,7 @@ template <int V> __device__ __forceinline__ float dot(const Part& p, const float
 
 enum Pass { TURN, NORM, NORM_BACK };           // TURN: both directions of the rotation alone
 
-// FULL: no lane's chunks are shorter than 16 bytes.  HEADS: the most heads of a run, whose loads are under way together and which share the cosines and sines of their place.
+// FULL: no lane's chunks are shorter than 16 bytes, and each is turned whole or not at all.  HEADS: the most heads of a run, whose loads are under way together and which share the cosines and sines of their place.
 template <class T, Pass PASS, bool NEIGHBOURS, int HEADS, bool FULL> __global__ __launch_bounds__(THREADS, PASS == NORM_BACK ? 3 : 4) void rotary_kernel(Args p) {
 #pragma clang fp contract(off)
   constexpr int V = Chunk<T>::N;
@@ -251,8 +244,8 @@ template <class T, Pass PASS, bool NEIGHBOURS, int HEADS, bool FULL> __global__ 
     int row = (int)place;
     if (p.index) row = p.index[outer * p.index_stride + place];
     float c[V], sn[V];
-    // a row below zero: the vector is not turned
-    load_turns<V>(p, p.table + outer * p.table_stride + (long)row * p.pairs, row < p.rows, p.pairs == 0 || row < 0 ? p.pairs : part.pair, c, sn);
+    const int turned = row < 0 ? 0 : max(min(p.pairs - part.pair, V), 0);     // a row below zero: the vector is not turned
+    load_turns<V, FULL>(p.table + outer * p.table_stride + (long)row * p.pairs, row < p.rows, part.pair, turned, p.sign, c, sn);
     T* const y = at(s.y);
 #pragma unroll
     for (int h = 0; h < HEADS; ++h) {
@@ -261,19 +254,19 @@ template <class T, Pass PASS, bool NEIGHBOURS, int HEADS, bool FULL> __global__ 
       Chunk<T>::get(raw[h][0], a);
       Chunk<T>::get(raw[h][1], b);
       if constexpr (PASS == TURN) {
-        turn<V, NEIGHBOURS>(c, sn, a, b);
+        turn<V, NEIGHBOURS, FULL>(turned, c, sn, a, b);
       } else {
         const float r = rsqrtf(fmaf(sum_of(dot<V>(part, a, b, a, b), p.lanes), p.inv_d, p.eps));
 #pragma unroll
         for (int i = 0; i < V; ++i) a[i] *= r, b[i] *= r;
         if constexpr (PASS == NORM) {
           weigh(a, b);
-          turn<V, NEIGHBOURS>(c, sn, a, b);
+          turn<V, NEIGHBOURS, FULL>(turned, c, sn, a, b);
         } else {
           float u[V], v[V];
           Chunk<T>::get(graw[h][0], u);
           Chunk<T>::get(graw[h][1], v);
-          turn<V, NEIGHBOURS>(c, sn, u, v);
+          turn<V, NEIGHBOURS, FULL>(turned, c, sn, u, v);
           if (h < heads)
 #pragma unroll
             for (int i = 0; i < V; ++i) ga[i] = fmaf(u[i], a[i], ga[i]), gb[i] = fmaf(v[i], b[i], gb[i]);
@@ -410,11 +403,12 @@ Plan plan_of(const s2cnn_rotary_t& a, bool two) {
   p.units = units_of(a.dtype == S2CNN_F32 ? 4 : 8, a.d, a.pairs, a.interleaved != 0);
   for (p.lanes = 1, p.log_lanes = 0; p.lanes < p.units; ++p.log_lanes) p.lanes *= 2;
   const int V = a.dtype == S2CNN_F32 ? 4 : 8, rest = a.d - 2 * a.pairs;
-  p.full = a.interleaved ? a.d % 2 == 0 && a.d >= 2 * V : (a.pairs == 0 || a.pairs >= V) && (rest == 0 || rest >= 2 * V);
+  p.full = a.interleaved ? a.d % 2 == 0 && a.d >= 2 * V && (rest == 0 || a.pairs == 0 || (a.d % (2 * V) == 0 && a.pairs % V == 0))
+                         : (a.pairs == 0 || a.pairs >= V) && (rest == 0 || rest >= 2 * V);
   const long groups = THREADS / p.lanes, places = (long)a.batch * a.n, vectors = places * ((long)a.heads[0] + a.heads[1]);
   p.most = two ? 2 : 4;
   long most = CUS * (two ? 3 : 4);
-  if (vectors < 2 * most * groups * p.most) p.most = 1, most = CUS * (two ? 4 : 8);
+  if (!p.full || vectors < 2 * most * groups * p.most) p.most = 1, most = CUS * (two ? 4 : 8);
   long runs[2], total = 0;
   for (int i = 0; i < 2; ++i) {
     runs[i] = (a.heads[i] + p.most - 1) / p.most;
@@ -473,8 +467,9 @@ template <class T, bool NEIGHBOURS, int HEADS, bool FULL> void launch(const Args
   else hipLaunchKernelGGL((rotary_kernel<T, NORM_BACK, NEIGHBOURS, (HEADS < 2 ? HEADS : 2), FULL>), grid, dim3(THREADS), 0, s, k);
 }
 template <class T, bool NEIGHBOURS> void launch(const Args& k, const Plan& p, bool norm, bool backward, hipStream_t s) {
-  if (p.most == 1) p.full ? launch<T, NEIGHBOURS, 1, true>(k, p, norm, backward, s) : launch<T, NEIGHBOURS, 1, false>(k, p, norm, backward, s);
-  else p.full ? launch<T, NEIGHBOURS, 4, true>(k, p, norm, backward, s) : launch<T, NEIGHBOURS, 4, false>(k, p, norm, backward, s);
+  if (!p.full) launch<T, NEIGHBOURS, 1, false>(k, p, norm, backward, s);
+  else if (p.most == 1) launch<T, NEIGHBOURS, 1, true>(k, p, norm, backward, s);
+  else launch<T, NEIGHBOURS, 4, true>(k, p, norm, backward, s);
 }
 template <class T> void run(const s2cnn_rotary_t& a, bool backward, float* partial, hipStream_t s) {
   const Plan p = plan_of(a, backward && a.norm);

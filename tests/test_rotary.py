@@ -246,6 +246,37 @@ def test_large_small_and_infinite_entries(hip):
 
 @pytest.mark.gpu
 @TYPES
+@LAYOUTS
+@pytest.mark.parametrize("d,pairs", [(64, 24), (64, 8), (40, 3), (23, 9), (7, 3), (128, 13)])
+def test_what_is_not_turned_stays_bit_by_bit(hip, d, pairs, interleaved, dtype):
+    """Entries behind the pairs, and vectors whose row is below zero, beside infinities, what is no number and zeros with a sign; gradients likewise."""
+    n = 9
+    gen = torch.Generator().manual_seed(d)
+    x, g = (torch.randn(2, 2, n, d, generator=gen) for _ in range(2))
+    for t in (x, g):
+        t[torch.rand(t.shape, generator=gen) < 0.2] = -0.0
+        t[torch.rand(t.shape, generator=gen) < 0.1] = math.inf
+        t[torch.rand(t.shape, generator=gen) < 0.1] = math.nan
+        t[..., 2 * pairs] = -math.inf
+    x, g = (t.to(dtype).cuda() for t in (x, g))
+    table = _table(n, pairs).cuda()
+    index = torch.arange(n, dtype=torch.int32)
+    index[::3] = -1
+    leaf = x.detach().requires_grad_()
+    y = s2cnn_amd.rotary(leaf, None, table, index=index.cuda(), interleaved=interleaved)[0]
+    gx, = torch.autograd.grad(y, leaf, g)
+    bits = torch.int32 if dtype == F32 else torch.int16
+    for got, of in ((y.detach(), x), (gx, g)):
+        assert torch.equal(got[..., 2 * pairs:].contiguous().view(bits), of[..., 2 * pairs:].contiguous().view(bits))
+        assert torch.equal(got[:, :, ::3].contiguous().view(bits), of[:, :, ::3].contiguous().view(bits))
+        # a pair with only finite entries has a finite result
+        halves = (lambda t: (t[..., :2 * pairs:2], t[..., 1:2 * pairs:2])) if interleaved else (lambda t: (t[..., :pairs], t[..., pairs:2 * pairs]))
+        one, two = (torch.isfinite(h)[:, :, 1::3] for h in halves(of))
+        assert all(torch.equal(torch.isfinite(h)[:, :, 1::3], one & two) for h in halves(got))
+
+
+@pytest.mark.gpu
+@TYPES
 def test_nothing_beside_the_vectors_is_written_or_read(hip, dtype):
     """Vectors with gaps between them that hold NaN, results in a tensor of the same form."""
     b, h, n, d, pairs = 2, 2, 5, 21, 9
