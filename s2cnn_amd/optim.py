@@ -304,6 +304,16 @@ class AdamW(torch.optim.Optimizer):
                                self.max_norm, self.seed)
         return loss
 
+    def moments(self, p):
+        """(first, second) moments of a parameter in float32, whatever they are held in; None before its first step."""
+        state = self.state[p] if p in self.state else None
+        if not state:
+            return None
+        if "scales" not in state:
+            return state["first"], state["second"]
+        (first,), (second,) = adamw_states([state["first"]], [state["second"]], [state["scales"]])
+        return first, second
+
     def load_state_dict(self, state_dict):
         """States keep their types (torch's own method takes them to the parameters')."""
         super().load_state_dict(state_dict)

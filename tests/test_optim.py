@@ -678,6 +678,24 @@ def test_captured_steps_need_a_step_before(hip):
 
 
 @pytest.mark.gpu
+def test_moments_of_a_parameter(hip):
+    """Of 8 bits within a spacing (1/8) of those of 32, after one step; None before it."""
+    g = torch.randn(40, 30, generator=torch.Generator().manual_seed(1)).cuda()
+    got = []
+    for bits in (32, 8):
+        p = torch.nn.Parameter(torch.ones(40, 30, device="cuda"))
+        opt = s2cnn_amd.AdamW([p], state_bits=bits)
+        assert opt.moments(p) is None
+        p.grad = g.clone()
+        opt.step()
+        got.append(opt.moments(p))
+    for a, b, of in zip(*got, (0.1 * g, 0.001 * g * g)):
+        assert a.dtype == b.dtype == F32 and a.shape == b.shape == p.shape
+        assert (a - of).abs().max() <= 8 * W * of.abs().max()
+        assert ((a - b).abs() <= a.abs() / 8 + 1e-4 * a.abs().max()).all()
+
+
+@pytest.mark.gpu
 def test_copies_of_an_optimizer(hip):
     """copy.deepcopy and pickles keep the clipping and the seed."""
     p = torch.nn.Parameter(torch.ones(300, device="cuda"))
