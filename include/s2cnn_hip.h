@@ -523,7 +523,7 @@ int s2cnn_rotary_table(const void *positions, int positions_type, const double *
  *   of a block with an infinite entry, or one that is no number, all entries become such.
  * adamw_states: the moments of 8 bits in float32, n[i] entries each.
  * grad_norm: *out = sqrt of the sum of squares of all entries of a list of tensors of any types, summed in 64 bits.
- * Lists are host memory, read during the call; tensors without entries are left out (their pointers may be NULL).
+ * Lists are host memory, read during the call; tensors without entries are left out (their pointers may be NULL).  n[i] <= 2^35 - 2048.
  */
 typedef struct s2cnn_adamw_t {
   void *const *p;

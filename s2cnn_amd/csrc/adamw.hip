@@ -359,7 +359,8 @@ __global__ __launch_bounds__(1024) void norm_kernel(const double* partial, long 
 }
 
 // ---- launches -------------------------------------------------------------------------------------------------------
-constexpr long MOST_ENTRIES = 1L << 42;
+constexpr unsigned long MOST_PARTS = (1UL << 24) - 1;      // workgroups of a launch: fewer than 2^32 threads
+constexpr long MOST_ENTRIES = (long)MOST_PARTS * PART;     // of a tensor, which no launch cuts
 
 template <class T, int BITS> void launch(const Tensors& t, const Step& h, bool master, hipStream_t s) {
   const dim3 grid(t.part[t.count]), block(THREADS);
@@ -379,14 +380,14 @@ void launch(const Tensors& t, const Step& h, int dtype, int bits, bool master, h
 bool misaligned(const void* p, unsigned size) { return (reinterpret_cast<uintptr_t>(p) & (size - 1)) != 0; }
 bool known(int dtype) { return dtype == S2CNN_F32 || dtype == S2CNN_BF16 || dtype == S2CNN_F16; }
 
-// Lists of tensors, MOST of them and fewer than 2^31 workgroups at a time, to `run`; those without entries are left out.
+// Lists of tensors, MOST of them and MOST_PARTS workgroups at a time, to `run`; those without entries are left out.
 template <class F> void for_parts(int count, const long* n, const F& add, void (*launch_part)(const Tensors&, const void*), const void* with) {
   Tensors t = {};
   unsigned long long counter = 0;
   for (int i = 0; i < count; ++i) {
     if (!n[i]) continue;
     const unsigned long need = (unsigned long)(n[i] + PART - 1) / PART;
-    if (t.count == MOST || (t.count && t.part[t.count] + need > 0x7fffffffUL)) {
+    if (t.count == MOST || (t.count && t.part[t.count] + need > MOST_PARTS)) {
       launch_part(t, with);
       t.count = 0;
     }
@@ -418,7 +419,7 @@ extern "C" int s2cnn_adamw_step(const s2cnn_adamw_t* a, void* stream) {
   if (!a->count) return S2CNN_OK;
   const unsigned size = a->dtype == S2CNN_F32 ? 4 : 2, state = a->bits == 8 ? 1 : 4;
   for (int i = 0; i < a->count; ++i) {
-    if (a->n[i] < 0 || a->n[i] >= MOST_ENTRIES) return S2CNN_EINVAL;
+    if (a->n[i] < 0 || a->n[i] > MOST_ENTRIES) return S2CNN_EINVAL;
     if (!a->n[i]) continue;
     if (!a->p[i] || !a->g[i] || !a->first[i] || !a->second[i] || (a->scales && !a->scales[i]) || (a->masters && !a->masters[i])) return S2CNN_EINVAL;
     if (misaligned(a->p[i], size) || misaligned(a->g[i], size) || misaligned(a->first[i], state) || misaligned(a->second[i], state)) return S2CNN_EALIGN;
@@ -453,7 +454,7 @@ extern "C" int s2cnn_adamw_states(const void* const* first, const void* const* s
   if (count < 0 || (count && (!first || !second || !scales || !first_out || !second_out || !n))) return S2CNN_EINVAL;
   if (!count) return S2CNN_OK;
   for (int i = 0; i < count; ++i) {
-    if (n[i] < 0 || n[i] >= MOST_ENTRIES) return S2CNN_EINVAL;
+    if (n[i] < 0 || n[i] > MOST_ENTRIES) return S2CNN_EINVAL;
     if (!n[i]) continue;
     if (!first[i] || !second[i] || !scales[i] || !first_out[i] || !second_out[i]) return S2CNN_EINVAL;
     if (misaligned(scales[i], 8) || misaligned(first_out[i], 4) || misaligned(second_out[i], 4)) return S2CNN_EALIGN;
@@ -473,7 +474,7 @@ extern "C" int s2cnn_adamw_states(const void* const* first, const void* const* s
 static long parts_of(const long* n, const int* dtypes, int count) {
   long parts = 0;
   for (int i = 0; i < count; ++i) {
-    if (n[i] < 0 || n[i] >= MOST_ENTRIES || !known(dtypes[i])) return -1;
+    if (n[i] < 0 || n[i] > MOST_ENTRIES || !known(dtypes[i])) return -1;
     parts += (n[i] + sums_part(dtypes[i]) - 1) / sums_part(dtypes[i]);
   }
   return parts;
@@ -509,7 +510,7 @@ extern "C" int s2cnn_grad_norm(const void* const* g, const long* n, const int* d
   for (int i = 0; i < count; ++i) {
     if (!n[i]) continue;
     const unsigned long need = (unsigned long)((n[i] + sums_part(dtypes[i]) - 1) / sums_part(dtypes[i]));
-    if (t.count == MOST_SUMS || (t.count && t.part[t.count] + need > 0x7fffffffUL)) run();
+    if (t.count == MOST_SUMS || (t.count && t.part[t.count] + need > MOST_PARTS)) run();
     const int k = t.count++;
     t.g[k] = g[i], t.n[k] = n[i], t.dtype[k] = (unsigned char)dtypes[i];
     t.part[k + 1] = t.part[k] + (unsigned)need;

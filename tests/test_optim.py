@@ -864,3 +864,28 @@ def test_entry_points_refuse_lists():
     assert lib.s2cnn_grad_norm(z, at(n), at(kinds), 1, 0x1000, 0x1000, 8, None) == -1 and lib.s2cnn_grad_norm(f, at(n), at(kinds), 1, 0x1000, 0x1000, 7, None) == -2
     assert lib.s2cnn_grad_norm(o, at(n), at(kinds), 1, 0x1000, 0x1000, 8, None) == -3 and lib.s2cnn_grad_norm(f, at(n), at(kinds), 1, 0x1002, 0x1000, 8, None) == -3
     assert lib.s2cnn_grad_norm(f, at(n), at(kinds), 1, None, 0x1000, 8, None) == -1 and lib.s2cnn_grad_norm(f, at(n), at(kinds), 1, 0x1000, None, 8, None) == -2
+
+
+def test_sizes_that_fit_a_launch():
+    """A launch has fewer than 2^32 threads: tensors of more are refused, the largest is not."""
+    from s2cnn_amd import _hip
+    lib = _hip.lib()
+    most = (1 << 35) - 2048
+    odd, fake = ((ctypes.c_void_p * 1)(x) for x in (0x1002, 0x1000))
+    kind = (ctypes.c_int * 1)(0)
+    for entries, rc in ((most, -3), (most + 1, -1)):                                        # at the address 0x1002 the largest is refused all the same
+        n = (ctypes.c_long * 1)(entries)
+        a = _hip.AdamW()
+        a.p, a.g, a.first, a.second, a.n = (ctypes.cast(x, ctypes.c_void_p).value for x in (odd, fake, fake, fake, n))
+        a.count, a.dtype, a.bits, a.step, a.lr, a.beta1, a.beta2, a.eps = 1, 0, 32, 1, 1e-3, 0.9, 0.99, 1e-8
+        assert lib.s2cnn_adamw_step(ctypes.byref(a), None) == rc
+        assert lib.s2cnn_adamw_states(fake, fake, fake, odd, fake, n, 1, None) == rc
+        assert lib.s2cnn_grad_norm(odd, n, kind, 1, 0x1000, 0x1000, 8, None) == rc
+        assert (lib.s2cnn_grad_norm_workspace(n, kind, 1) > 0) == (rc == -3)
+
+
+@pytest.mark.gpu
+def test_lists_of_more_than_a_launch(hip):
+    """One tensor 33 times, of 2^19 workgroups each: more than 2^32 threads, in two launches.  Counts of ones are exact."""
+    t = torch.ones(1 << 33, dtype=BF16, device="cuda")
+    assert s2cnn_amd.grad_norm([t] * 33).item() == np.float32(math.sqrt(33 * 2.0 ** 33))
