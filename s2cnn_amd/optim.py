@@ -319,6 +319,8 @@ class AdamW(torch.optim.Optimizer):
         """States keep their types (torch's own method takes them to the parameters')."""
         super().load_state_dict(state_dict)
         for group, from_group in zip(self.param_groups, state_dict["param_groups"]):
+            if torch.is_tensor(group["lr"]):
+                group["lr"] = group["lr"].to(group["params"][0].device)
             counts = {}                                              # parameters of a group that had as many steps go on together
             for i, p in zip(from_group["params"], group["params"]):
                 if i in state_dict["state"]:

@@ -889,3 +889,22 @@ def test_lists_of_more_than_a_launch(hip):
     """One tensor 33 times, of 2^19 workgroups each: more than 2^32 threads, in two launches.  Counts of ones are exact."""
     t = torch.ones(1 << 33, dtype=BF16, device="cuda")
     assert s2cnn_amd.grad_norm([t] * 33).item() == np.float32(math.sqrt(33 * 2.0 ** 33))
+
+
+@pytest.mark.gpu
+def test_loaded_rates_are_on_the_gpu(hip):
+    """A rate that is a tensor, from a checkpoint that was read to the host."""
+    p = torch.nn.Parameter(torch.ones(30, device="cuda"))
+    p.grad = torch.ones_like(p)
+    opt = s2cnn_amd.AdamW([p], lr=torch.full((1,), 0.25, device="cuda"))
+    opt.step()
+    file = io.BytesIO()
+    torch.save(opt.state_dict(), file)
+    file.seek(0)
+    saved = torch.load(file, weights_only=True, map_location="cpu")
+    again = s2cnn_amd.AdamW([p], lr=torch.zeros(1, device="cuda"))
+    again.load_state_dict(saved)
+    before = p.detach().clone()
+    again.step()
+    assert again.param_groups[0]["lr"].is_cuda and again.param_groups[0]["lr"].item() == 0.25 and not torch.equal(before, p)
+    assert not saved["param_groups"][0]["lr"].is_cuda
