@@ -33,7 +33,7 @@ def _vectors(t):
 def _plan(shape, other, strides, table, index_stride, norm, interleaved, eps, dtype):
     """(the library's struct without its pointers, bytes of the workspace of the weights' gradients) of a call of these sizes.
     shape, other: of the first tensor and of the second, or None; strides: of x, g and y of the first, then of the second, as torch gives them, or None;
-    table: its batch stride, rows and pairs."""
+    table: its batch stride, rows and pairs; index_stride: None without an index."""
     a = _hip.Rotary()
     a.batch, a.heads[0], a.n, a.d = shape
     a.heads[1] = 0 if other is None else other[1]
@@ -41,10 +41,11 @@ def _plan(shape, other, strides, table, index_stride, norm, interleaved, eps, dt
         for to, stride in zip((a.x_stride, a.g_stride, a.y_stride), strides[3 * i:]):
             to[i][:] = stride[:3] if stride is not None else (0, 0, 0)
     a.table_stride, a.rows, a.pairs = table
-    a.index_stride, a.norm, a.interleaved, a.eps, a.dtype = index_stride, norm, interleaved, eps, dtype
-    a.table = 16 if a.pairs else None                    # some address: the sizes are refused without
+    a.index_stride, a.norm, a.interleaved, a.eps, a.dtype = index_stride or 0, norm, interleaved, eps, dtype
+    a.table = 16 if a.pairs else None                    # some addresses: the sizes are refused without, and fewer rows than places without an index
+    a.index = None if index_stride is None else 16
     nbytes = _hip.lib().s2cnn_rotary_workspace(ctypes.byref(a))
-    a.table = None
+    a.table = a.index = None
     return bytes(a), nbytes
 
 
@@ -139,7 +140,7 @@ def _call(q, k, q_weight, k_weight, table, index, norm, eps, interleaved):
             table = table.clone()
     index = index.contiguous() if index is not None else None
     sizes = ((0, 0, 0) if table is None else (table.stride(0) if table.dim() == 4 and batch > 1 else 0, *table.shape[-3:-1]),
-             0 if index is None or index.dim() == 1 or batch == 1 else n, int(norm), int(interleaved), eps, dtype)
+             None if index is None else 0 if index.dim() == 1 or batch == 1 else n, int(norm), int(interleaved), eps, dtype)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
         return _Rotary.apply(q, k, q_weight, k_weight, table, index, sizes)
     return _forward(q, k, q_weight, k_weight, table, index, sizes)

@@ -7,6 +7,7 @@ subtracts a mean of the vector's entries: 16 * 2^-24 of the size of what is subt
 16 * 2^-24 of the 2-norm of the sums of magnitudes on top (n at most some thousand, in parts).  Entries of the table: an angle to 2^-53 of its
 turns (below 2^26), its rest in float32 (2^-25 of a quarter turn) and one or two roundings of a value up to one: 4 * 2^-24 each."""
 import ctypes
+import importlib
 import math
 
 import pytest
@@ -177,6 +178,27 @@ def test_rows_by_index(hip, normed, per_batch, interleaved):
         for a, y in zip(bad, out):
             assert a[:, :, 5:7, :2 * pairs].isnan().all() and torch.isfinite(a[:, :, 5:7, 2 * pairs:]).all()
             assert torch.equal(a[:, :, :5], y[:, :, :5]) and torch.equal(a[:, :, 7:], y[:, :, 7:])
+
+
+@pytest.mark.gpu
+@LAYOUTS
+@pytest.mark.parametrize("per_batch", [False, True])
+def test_gradients_with_fewer_rows_than_places(hip, per_batch, interleaved):
+    """Packed sequences and places that share rows: weights' gradients too, with one index for all signals or one for each."""
+    b, h, hk, n, d, pairs, rows = 3, 4, 2, 40, 24, 10, 7
+    q, k, weights, gs = _make((b, h, hk, n, d, pairs), F32, seed=4)
+    table = _table(rows, pairs)
+    index = torch.randint(0, rows, (b, n) if per_batch else (n,), generator=torch.Generator().manual_seed(8), dtype=torch.int32)
+    taken = table[index.expand(b, n).long()].unsqueeze(1)
+    leaves = [t.detach().requires_grad_() for t in (q, k, *weights)]
+    out = s2cnn_amd.norm_rotary(*leaves, table.cuda(), index=index.cuda(), eps=EPS, interleaved=interleaved)
+    grads = torch.autograd.grad(out, leaves, gs)
+    for i in range(2):
+        x, w, g = _cpu(leaves[i], weights[i], gs[i])
+        y, gx, gw, parts, magnitudes = _gradients(x, w, _turned(g, taken, interleaved, back=True))
+        _close(out[i], _turned(y, taken, interleaved), F32, "y", 16)
+        _close(grads[i], gx, F32, "gx", 16, parts)
+        _close(grads[2 + i], gw, F32, "gw", 16, magnitudes)
 
 
 @pytest.mark.gpu
@@ -494,6 +516,16 @@ def test_refusals_of_types(hip):
     y, = torch.autograd.grad(s2cnn_amd.rotary(x, None, table)[0].square().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable|differentiat"):
         torch.autograd.grad(y.sum(), x)
+
+
+@pytest.mark.parametrize("index_stride", [0, 100])
+def test_workspaces_with_fewer_rows_than_places(index_stride):
+    """With an index a table may have any number of rows: the workspace of the weights' gradients does not depend on it."""
+    plan = importlib.import_module("s2cnn_amd.rotary")._plan
+    strides = ((6400 * 4, 6400, 64, 1),) * 3
+    of = lambda rows, index: plan((2, 4, 100, 64), None, strides, (0, rows, 32), index, 1, 0, EPS, 0)[1]
+    assert of(50, index_stride) == of(100, index_stride) == of(100, None) > 0
+    assert of(50, None) == 0                                               # without an index refused
 
 
 def test_entry_points_refuse_sizes():
