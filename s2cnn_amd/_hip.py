@@ -9,6 +9,7 @@ import os
 from functools import lru_cache
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "csrc", "libs2cnn_hip.so")
@@ -284,6 +285,11 @@ def once_differentiable(backward):
     def run(ctx, *grads):
         return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
     return run
+
+
+def have_tangents(*tensors):
+    """Whether one of the tensors has a tangent of forward mode, which a call of the library would lose."""
+    return forward_ad._current_level >= 0 and any(t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def ptr_or_none(t):

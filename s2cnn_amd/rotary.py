@@ -13,6 +13,7 @@ from functools import lru_cache
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _hip
 from .attention import _like
@@ -141,7 +142,8 @@ def _call(q, k, q_weight, k_weight, table, index, norm, eps, interleaved):
     index = index.contiguous() if index is not None else None
     sizes = ((0, 0, 0) if table is None else (table.stride(0) if table.dim() == 4 and batch > 1 else 0, *table.shape[-3:-1]),
              None if index is None else 0 if index.dim() == 1 or batch == 1 else n, int(norm), int(interleaved), eps, dtype)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+    # tangents of forward mode, which is on under no_grad as well, are refused there
+    if forward_ad._current_level >= 0 or torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
         return _Rotary.apply(q, k, q_weight, k_weight, table, index, sizes)
     return _forward(q, k, q_weight, k_weight, table, index, sizes)
 
@@ -201,6 +203,7 @@ def rotary_table(positions, frequencies, scale=1.0):
     _hip.require_gpu_of(positions.dtype, positions)
     _hip.require_gpu_of(torch.float64, frequencies)
     assert not positions.requires_grad and not frequencies.requires_grad, "the table is not differentiated"
+    assert not _hip.have_tangents(positions, frequencies), "the table is not differentiated"
     positions, frequencies = positions.contiguous(), frequencies.contiguous()
     table = torch.empty(*positions.shape[:-1], pairs, 2, dtype=torch.float32, device=positions.device)
     n = positions.numel() // axes

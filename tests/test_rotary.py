@@ -12,6 +12,7 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import s2cnn_amd
 
@@ -526,6 +527,27 @@ def test_workspaces_with_fewer_rows_than_places(index_stride):
     of = lambda rows, index: plan((2, 4, 100, 64), None, strides, (0, rows, 32), index, 1, 0, EPS, 0)[1]
     assert of(50, index_stride) == of(100, index_stride) == of(100, None) > 0
     assert of(50, None) == 0                                               # without an index refused
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("with_grad", [False, True])
+def test_tangents_of_forward_mode_are_refused(hip, with_grad):
+    """None is lost without a word, with and without gradients of the other mode; inside a level without tangents all is as outside."""
+    x, w, table = torch.randn(2, 4, 5, 8).cuda(), torch.ones(8, device="cuda"), _table(5, 4).cuda()
+    places, f = torch.arange(5.0, device="cuda").view(5, 1), torch.ones(1, 4, dtype=torch.float64, device="cuda")
+    want = s2cnn_amd.norm_rotary(x, x, w, w, table) + s2cnn_amd.rotary(x, x, table) + (s2cnn_amd.rotary_table(places, f),)
+    with forward_ad.dual_level(), torch.set_grad_enabled(with_grad):
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: s2cnn_amd.rotary(dual(x), None, table), lambda: s2cnn_amd.rotary(x, dual(x), table), lambda: s2cnn_amd.rotary(x, None, dual(table)),
+                     lambda: s2cnn_amd.norm_rotary(dual(x), x, w, w, table), lambda: s2cnn_amd.norm_rotary(x, x, dual(w), w), lambda: s2cnn_amd.norm_rotary(x, x, w, dual(w), table)):
+            with pytest.raises(NotImplementedError, match="forward mode"):
+                call()
+        for call in (lambda: s2cnn_amd.rotary_table(dual(places), f), lambda: s2cnn_amd.rotary_table(places, dual(f))):
+            with pytest.raises(AssertionError, match="not differentiated"):
+                call()
+        got = s2cnn_amd.norm_rotary(x, x, w, w, table) + s2cnn_amd.rotary(x, x, table) + (s2cnn_amd.rotary_table(places, f),)
+        assert s2cnn_amd.rotary_table(torch.arange(5, device="cuda").view(5, 1), f).equal(want[-1])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 def test_entry_points_refuse_sizes():
