@@ -317,7 +317,17 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """States keep their types (torch's own method takes them to the parameters')."""
-        super().load_state_dict(state_dict)
+        loaded = {}
+        # behind the program's hooks before the loading, which may give another dict, and in front of those after it
+        hooks = [self.register_load_state_dict_pre_hook(lambda _, seen: loaded.update(seen)),
+                 self.register_load_state_dict_post_hook(lambda _: self._restore(loaded), prepend=True)]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
+    def _restore(self, state_dict):
         for group, from_group in zip(self.param_groups, state_dict["param_groups"]):
             if torch.is_tensor(group["lr"]):
                 group["lr"] = group["lr"].to(group["params"][0].device)

@@ -583,6 +583,43 @@ def test_state_dicts(hip, bits, dtype):
     assert [s["step"].item() for s in opt.state.values()] == [6, 6, 6, 5]
 
 
+@pytest.mark.parametrize("bits", [8, 32])
+def test_hooks_of_loading(bits):
+    """What a hook before the loading gives is loaded, in the states' types; what one after it writes stays.  Hooks are the program's: none is left."""
+    def make():
+        p = torch.nn.Parameter(torch.ones(300, dtype=BF16))
+        return p, s2cnn_amd.AdamW([p], state_bits=bits)
+
+    p, opt = make()
+    opt.state[p] = opt._new_state(p, opt.param_groups[0], torch.full((1,), 3))
+    opt.state[p]["first"].view(torch.uint8).fill_(7)
+    saved = opt.state_dict()
+    q, other = make()
+
+    def before(_, state_dict):
+        return {**state_dict, "state": {i: {**s, "second": s["second"] + 5, "step": s["step"] + 1} for i, s in state_dict["state"].items()}}
+
+    def after(o):
+        assert (o.state[q]["second"] == 5).all()
+        o.state[q]["master"].fill_(2.0)
+
+    kept = [other.register_load_state_dict_pre_hook(before), other.register_load_state_dict_post_hook(after)]
+    for times in range(2):
+        other.load_state_dict(saved)
+        state = other.state[q]
+        assert state["step"].item() == 4 and state["step"].dtype == torch.int64 and (state["second"] == 5).all() and (state["master"] == 2).all()
+        assert state["first"].dtype == opt.state[p]["first"].dtype and state["second"].dtype == opt.state[p]["second"].dtype and state["master"].dtype == F32
+        assert torch.equal(state["first"].view(torch.uint8), opt.state[p]["first"].view(torch.uint8)) and state["first"].data_ptr() != opt.state[p]["first"].data_ptr()
+        assert (opt.state[p]["second"] == 0).all() and opt.state[p]["step"].item() == 3
+    for hook in kept:
+        hook.remove()
+    with pytest.raises(ValueError):
+        other.load_state_dict({"state": {}, "param_groups": []})
+    other.load_state_dict(saved)
+    assert (other.state[q]["second"] == 0).all() and (other.state[q]["master"] == 1).all() and other.state[q]["step"].item() == 3
+    assert not other._optimizer_load_state_dict_pre_hooks and not other._optimizer_load_state_dict_post_hooks
+
+
 @pytest.mark.gpu
 def test_loaded_groups_count_their_own_steps(hip):
     """Two groups of as many steps, saved and loaded: one step counts one in each."""
