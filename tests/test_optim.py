@@ -14,6 +14,7 @@ import math
 import numpy as np
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import s2cnn_amd
 
@@ -507,6 +508,23 @@ def test_grad_norm_of_extreme_values(hip):
         t = torch.ones(20000, device="cuda")
         t[19999] = value
         assert not math.isfinite(s2cnn_amd.grad_norm([torch.ones(5, device="cuda"), t]).item())
+
+
+@pytest.mark.gpu
+def test_grad_norm_is_not_differentiated(hip):
+    """What would have a graph, or a tangent, is refused and not cut off without a word: a penalty on it would train nothing."""
+    x = torch.nn.Parameter(torch.randn(300, 5, device="cuda"))
+    g, = torch.autograd.grad(x.pow(3).sum(), x, create_graph=True)
+    for tensors in ([g], [x], [x.detach(), x], [x.T], [x.detach().half(), g]):
+        with pytest.raises(AssertionError, match="not differentiated"):
+            s2cnn_amd.grad_norm(tensors)
+        with torch.no_grad():
+            norm = s2cnn_amd.grad_norm(tensors)
+        assert torch.equal(norm, s2cnn_amd.grad_norm([t.detach() for t in tensors])) and not norm.requires_grad
+    with torch.no_grad(), forward_ad.dual_level():
+        with pytest.raises(AssertionError, match="not differentiated"):
+            s2cnn_amd.grad_norm([x, forward_ad.make_dual(x.detach(), torch.ones_like(x))])
+        assert torch.equal(s2cnn_amd.grad_norm([x]), s2cnn_amd.grad_norm([x.detach()]))
 
 
 # ---- the optimizer --------------------------------------------------------------------------------------------------
