@@ -141,6 +141,13 @@ def adamw_step(params, grads, first, second, step, lr=1e-3, betas=(0.9, 0.999), 
         number nothing is written
     :param seed: of the random rounding, an int; equal seeds and steps round equal lists alike
     """
+    step_of_list = _prepared(params, grads, first, second, step, lr, betas, eps, weight_decay, masters, scales, norm, max_norm, seed)
+    if step_of_list is not None:
+        _launch(step_of_list)
+
+
+def _prepared(params, grads, first, second, step, lr, betas, eps, weight_decay, masters, scales, norm, max_norm, seed):
+    """`adamw_step`'s arguments, checked: (the library's struct, the parameters, what the struct points into), or None where there is nothing to do."""
     params, grads, first, second = list(params), list(grads), list(first), list(second)
     masters, scales = (list(t) if t is not None else None for t in (masters, scales))
     assert len(params) == len(grads)
@@ -154,7 +161,7 @@ def adamw_step(params, grads, first, second, step, lr=1e-3, betas=(0.9, 0.999), 
         assert norm.numel() == 1 and 0.0 < max_norm < 1e38
     if not params:
         assert not first and not second and not masters and not scales
-        return
+        return None
     dtype, device = params[0].dtype, _current_device(params)
     if dtype not in _hip.FLOATS:
         raise RuntimeError("float32, bfloat16 or float16 parameters only (got %s)" % dtype)
@@ -178,8 +185,12 @@ def adamw_step(params, grads, first, second, step, lr=1e-3, betas=(0.9, 0.999), 
     a = _hip.AdamW.from_buffer_copy(_STEP.pack(
         _at(p), _at(g), _at(one), _at(two), _at(factors), _at(copies), _at(n), lr_at, 0 if norm is None else norm.data_ptr(), step_at, step,
         seed & 0xFFFFFFFFFFFFFFFF, lr, *betas, eps, weight_decay, max_norm or 0.0, len(n), _hip.FLOATS[dtype], 32 if scales is None else 8))
-    _hip.call("s2cnn_adamw_step", ctypes.byref(a), _hip.stream_ptr())
-    torch.autograd.graph.increment_version(params)                   # as other operations in place do
+    return a, params, (p, g, one, two, factors, copies, n, grads, first, second, masters, scales)
+
+
+def _launch(prepared):
+    _hip.call("s2cnn_adamw_step", ctypes.byref(prepared[0]), _hip.stream_ptr())
+    torch.autograd.graph.increment_version(prepared[1])              # as other operations in place do
 
 
 def adamw_states(first, second, scales):
@@ -297,16 +308,21 @@ class AdamW(torch.optim.Optimizer):
         if self.max_norm is not None:
             self.norm = grad_norm([p.grad for group in self.param_groups for p in group["params"] if p.grad is not None])
             finite = torch.isfinite(self.norm)
+        steps, counts = [], []                                           # all lists are checked before the first is stepped or counted
         for group in self.param_groups:
             for count, params in self._lists(group):
-                count.add_(1 if finite is None else finite)
+                counts.append(count)
                 for dtype in dict.fromkeys(map(_dtype, params)):
                     some = [p for p in params if p.dtype == dtype]
                     states = [self.state[p] for p in some]
-                    adamw_step(some, [p.grad for p in some], [s["first"] for s in states], [s["second"] for s in states], count, group["lr"], group["betas"],
-                               group["eps"], group["weight_decay"], [s["master"] for s in states] if "master" in states[0] else None,
-                               [s["scales"] for s in states] if "scales" in states[0] else None, self.norm if finite is not None else None,
-                               self.max_norm, self.seed)
+                    steps.append(_prepared(some, [p.grad for p in some], [s["first"] for s in states], [s["second"] for s in states], count, group["lr"],
+                                           group["betas"], group["eps"], group["weight_decay"], [s["master"] for s in states] if "master" in states[0] else None,
+                                           [s["scales"] for s in states] if "scales" in states[0] else None, self.norm if finite is not None else None,
+                                           self.max_norm, self.seed))
+        for count in counts:
+            count.add_(1 if finite is None else finite)
+        for prepared in steps:
+            _launch(prepared)
         return loss
 
     def moments(self, p):

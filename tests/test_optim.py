@@ -675,6 +675,36 @@ def test_groups_types_and_steps_left_out(hip):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("clip", [None, 1.0])
+def test_refused_steps_are_neither_made_nor_counted(hip, clip):
+    """What one list is refused for leaves the lists before it, and all counts, as they were."""
+    params = [torch.nn.Parameter(torch.ones(4, 3, device="cuda")) for _ in range(3)]
+    opt = s2cnn_amd.AdamW([{"params": params[:1]}, {"params": params[1:]}], lr=0.1, max_norm=clip)
+    for p in params:
+        p.grad = torch.ones_like(p)
+    opt.step()
+    kept = [p.detach().clone() for p in params]
+    group, data = opt.param_groups[1], params[2].data
+
+    def unchanged():
+        assert all(torch.equal(p, k) for p, k in zip(params, kept))
+        assert all(opt.state[p]["step"].item() == 1 for p in params) and all((opt.state[p]["first"] == opt.state[params[0]]["first"][0, 0]).all() for p in params)
+
+    group["lr"] = -1.0
+    with pytest.raises(AssertionError):
+        opt.step()
+    unchanged()
+    group["lr"] = 0.1
+    params[2].data = data.T
+    with pytest.raises(RuntimeError, match="contiguous"):
+        opt.step()
+    params[2].data = data
+    unchanged()
+    opt.step()
+    assert all(opt.state[p]["step"].item() == 2 for p in params) and all((p < k).all() for p, k in zip(params, kept))
+
+
+@pytest.mark.gpu
 def test_captured_training_steps(hip):
     """Backward pass, norm and step in one graph, against the same steps made eagerly."""
     nets = [_network() for _ in range(2)]
