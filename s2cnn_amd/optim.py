@@ -312,12 +312,15 @@ class AdamW(torch.optim.Optimizer):
         for group in self.param_groups:
             for count, params in self._lists(group):
                 counts.append(count)
-                for dtype in dict.fromkeys(map(_dtype, params)):
-                    some = [p for p in params if p.dtype == dtype]
+                kinds = {}                                               # what is held of a parameter was chosen when it was first stepped
+                for p in params:
+                    state = self.state[p]
+                    kinds.setdefault((p.dtype, "master" in state, "scales" in state), []).append(p)
+                for (_, masters, scales), some in kinds.items():
                     states = [self.state[p] for p in some]
                     steps.append(_prepared(some, [p.grad for p in some], [s["first"] for s in states], [s["second"] for s in states], count, group["lr"],
-                                           group["betas"], group["eps"], group["weight_decay"], [s["master"] for s in states] if "master" in states[0] else None,
-                                           [s["scales"] for s in states] if "scales" in states[0] else None, self.norm if finite is not None else None,
+                                           group["betas"], group["eps"], group["weight_decay"], [s["master"] for s in states] if masters else None,
+                                           [s["scales"] for s in states] if scales else None, self.norm if finite is not None else None,
                                            self.max_norm, self.seed))
         for count in counts:
             count.add_(1 if finite is None else finite)

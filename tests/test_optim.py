@@ -655,6 +655,33 @@ def test_loaded_groups_count_their_own_steps(hip):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("option,then", [("state_bits", 8), ("state_bits", 32), ("masters", False), ("masters", True)])
+def test_options_changed_between_first_steps(hip, option, then):
+    """Parameters keep what they were first stepped with; loaded with equal counts they go on together, each as it is held."""
+    before = {"state_bits": 40 - then} if option == "state_bits" else {"masters": not then}
+    params = [torch.nn.Parameter(torch.ones(300, device="cuda", dtype=BF16)) for _ in range(3)]
+    opt = s2cnn_amd.AdamW(params, lr=0.1, **before)
+    params[0].grad = torch.ones_like(params[0])
+    opt.step()
+    params[0].grad = None
+    opt.param_groups[0][option] = then
+    for p in params[1:]:
+        p.grad = torch.ones_like(p)
+    opt.step()
+    again = s2cnn_amd.AdamW(params, lr=0.1)
+    again.load_state_dict(opt.state_dict())
+    held = [set(again.state[p]) for p in params]
+    assert held[1] == held[2] != held[0] and len({id(again.state[p]["step"]) for p in params}) == 1
+    kept = [p.detach().clone() for p in params]
+    params[0].grad = torch.ones_like(params[0])
+    for o in (again, again):
+        o.step()
+    assert all(again.state[p]["step"].item() == 3 for p in params) and all((p < k).all() for p, k in zip(params, kept))
+    assert [set(again.state[p]) for p in params] == held and torch.equal(params[1], params[2])
+    assert all(torch.equal(p, again.state[p]["master"].to(BF16)) for p in params if "master" in again.state[p])
+
+
+@pytest.mark.gpu
 def test_groups_types_and_steps_left_out(hip):
     """Parameters of two types and a group in 8 bits; a step without a finite norm is neither made nor counted."""
     a, b, c = (torch.nn.Parameter(torch.ones(300, device="cuda", dtype=d)) for d in (F32, BF16, F32))
