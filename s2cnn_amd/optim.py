@@ -20,6 +20,7 @@ _contiguous, _device, _numel, _address = torch.Tensor.is_contiguous, torch.Tenso
 _TENSORS = {torch.Tensor, torch.nn.Parameter}
 _CODES = {torch.float32: (2, 32), torch.float16: (2, 16), torch.bfloat16: (4, 16), torch.float8_e4m3fn: (10, 8), torch.uint8: (1, 8)}      # DLPack's
 _ROCM = 10
+_LISTS = 0x9E3779B97F4A7C15                              # from the seed of one list of a step to the next's, mod 2^64: odd, so that none comes twice
 _STEP = struct.Struct("10PqQ6d3i4x")                     # s2cnn_adamw_t
 
 
@@ -224,7 +225,8 @@ class AdamW(torch.optim.Optimizer):
         state dict): where they are not their masters' roundings, they count
     :param max_norm: gradients are clipped to this norm, of all groups together (`self.norm` is the norm of the last step, before it); a step whose norm is
         infinite or no number is left out and not counted.  None: neither
-    :param seed: of the random rounding of moments in 8 bits; ranks of a job that hold the same parameters need the same
+    :param seed: of the random rounding of moments in 8 bits; ranks of a job that hold the same parameters need the same.  Lists of a step (groups, types,
+        counts) take random numbers of their own each
 
     Steps are counted on the device, for every parameter those that it had a gradient in.  State dicts hold the moments as they are; max_norm and seed are the
     program's to keep.  A step that a graph captures needs the moments to exist, and the same parameters to have gradients as before: make one before.
@@ -321,7 +323,7 @@ class AdamW(torch.optim.Optimizer):
                     steps.append(_prepared(some, [p.grad for p in some], [s["first"] for s in states], [s["second"] for s in states], count, group["lr"],
                                            group["betas"], group["eps"], group["weight_decay"], [s["master"] for s in states] if masters else None,
                                            [s["scales"] for s in states] if scales else None, self.norm if finite is not None else None,
-                                           self.max_norm, self.seed))
+                                           self.max_norm, self.seed + len(steps) * _LISTS))
         for count in counts:
             count.add_(1 if finite is None else finite)
         for prepared in steps:

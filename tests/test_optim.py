@@ -655,6 +655,28 @@ def test_loaded_groups_count_their_own_steps(hip):
 
 
 @pytest.mark.gpu
+def test_lists_of_a_step_round_apart(hip):
+    """Groups of equal gradients, moments in 8 bits: the first list's codes are those of adamw_step with the seed, the others' are rounded at random numbers of
+    their own.  A code is one of two: of n independent ones, each rounded up with the same probability on both sides, at least n / 100 differ where it
+    lies between 0.1 and 0.9 for a tenth of them (n / 10 * 2 * 0.09 = n / 55 expected; the spread is below sqrt(n))."""
+    n = 20000
+    g = torch.randn(n, generator=torch.Generator().manual_seed(2)).cuda()
+    params = [torch.nn.Parameter(torch.ones(n, device="cuda", dtype=d)) for d in (F32, F32, F32, BF16)]
+    opt = s2cnn_amd.AdamW([{"params": params[:1]}, {"params": params[1:2], "weight_decay": 0.0}, {"params": params[2:]}], state_bits=8, seed=-3)
+    for p in params:
+        p.grad = g.to(p.dtype)
+    opt.step()
+    first, second, scales = _zeros([(n,)], 8)
+    s2cnn_amd.adamw_step([torch.ones(n, device="cuda")], [g], first, second, 1, scales=scales, seed=-3)
+    codes = [[opt.state[p][k].view(torch.uint8) for k in ("first", "second")] for p in params]
+    assert torch.equal(codes[0][0], first[0].view(torch.uint8)) and torch.equal(codes[0][1], second[0])
+    for i in range(4):
+        for j in range(i):
+            for a, b in zip(codes[i], codes[j]):
+                assert (a != b).sum().item() > n / 100, (i, j)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("option,then", [("state_bits", 8), ("state_bits", 32), ("masters", False), ("masters", True)])
 def test_options_changed_between_first_steps(hip, option, then):
     """Parameters keep what they were first stepped with; loaded with equal counts they go on together, each as it is held."""
