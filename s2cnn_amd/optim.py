@@ -127,8 +127,8 @@ def adamw_step(params, grads, first, second, step, lr=1e-3, betas=(0.9, 0.999), 
     One step of AdamW on a list of tensors, in place:
     m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2, p = p - lr weight_decay p - lr (m / (1 - b1^step)) / (sqrt(v / (1 - b2^step)) + eps).
 
-    :param params, grads: tensors of one type (float32, bfloat16 or float16) on the current GPU, as many entries each; parameters contiguous, none twice and
-        no two overlapping
+    :param params, grads: tensors of one type (float32, bfloat16 or float16) on the current GPU, as many entries each; parameters contiguous.  No tensor that
+        is written (all but the gradients) stands twice in the lists, and no two overlap
     :param first, second: the moments m and v, as many entries as the parameters: float32, or with scales float8_e4m3fn and uint8
     :param step: which step it is, from 1 on: an int, or an int64 tensor of one element on the GPU that is read when the kernels run
     :param lr: a number, or a float32 tensor of one element on the GPU

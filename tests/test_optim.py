@@ -1000,6 +1000,36 @@ def test_entry_points_refuse_lists():
     assert lib.s2cnn_grad_norm(f, at(n), at(kinds), 1, None, 0x1000, 8, None) == -1 and lib.s2cnn_grad_norm(f, at(n), at(kinds), 1, 0x1000, None, 8, None) == -2
 
 
+def test_entry_points_refuse_tensors_twice():
+    """One that is written by two workgroups of a launch, in one list or in two; refused on the host.  Tensors without entries may be anything."""
+    from s2cnn_amd import _hip
+    lib = _hip.lib()
+    names = ("p", "g", "first", "second", "scales", "masters")
+
+    def run(count, same=None, empty=()):
+        arrays = {k: [0x1000000 * (j + 1) + 0x1000 * i for i in range(count)] for j, k in enumerate(names)}
+        if same:
+            (a, i), (b, j) = same
+            arrays[a][i] = arrays[b][j]
+        a, keep = _hip.AdamW(), []
+        for k, v in arrays.items():
+            keep.append((ctypes.c_void_p * count)(*v))
+            setattr(a, k, ctypes.cast(keep[-1], ctypes.c_void_p).value)
+        keep.append((ctypes.c_long * count)(*(0 if i in empty or not same else 5 for i in range(count))))
+        a.n, a.count, a.dtype, a.bits, a.step = ctypes.cast(keep[-1], ctypes.c_void_p).value, count, 1, 8, 1
+        a.lr, a.beta1, a.beta2, a.eps = 1e-3, 0.9, 0.99, 1e-8
+        return lib.s2cnn_adamw_step(ctypes.byref(a), None)
+
+    written = [k for k in names if k != "g"]
+    for count in (2, 3, 56, 57, 500):
+        for a in written:
+            assert run(count, ((a, 0), (a, count - 1))) == -1
+            for b in written:
+                if a != b:
+                    assert run(count, ((a, 0), (b, 1))) == run(count, ((a, 1), (b, 1))) == -1
+        assert run(count, (("p", 0), ("p", 1)), empty=range(count)) != -1         # nothing to do: not refused (where there is no GPU its status tells of that)
+
+
 def test_sizes_that_fit_a_launch():
     """A launch has fewer than 2^32 threads: tensors of more are refused, the largest is not."""
     from s2cnn_amd import _hip
@@ -1016,6 +1046,17 @@ def test_sizes_that_fit_a_launch():
         assert lib.s2cnn_adamw_states(fake, fake, fake, odd, fake, n, 1, None) == rc
         assert lib.s2cnn_grad_norm(odd, n, kind, 1, 0x1000, 0x1000, 8, None) == rc
         assert (lib.s2cnn_grad_norm_workspace(n, kind, 1) > 0) == (rc == -3)
+
+
+@pytest.mark.gpu
+def test_moments_given_twice_are_refused(hip):
+    z = lambda: torch.zeros(300, device="cuda")
+    params, grads, first, second = ([z() for _ in range(3)] for _ in range(4))
+    g = grads[:1] * 3                                                                       # gradients are only read
+    s2cnn_amd.adamw_step(params, g, first, second, 1)
+    for lists in ((params, g, [first[0], first[1], first[0]], second), (params, g, first, first), (params, g, first, [second[0], second[1], params[0]])):
+        with pytest.raises(RuntimeError):
+            s2cnn_amd.adamw_step(*lists, 1)
 
 
 @pytest.mark.gpu
