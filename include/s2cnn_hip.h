@@ -477,9 +477,9 @@ int s2cnn_dropout(const void *x, void *y, long n, double p, unsigned long long s
 
 /* ---- rotations of queries and keys by position, normalisation of every head's vectors -------------
  * Vectors x[b,h,n] of d <= 256 entries, 2 pairs <= d of which are turned: y = R(table row) x, and with norm != 0 y = R(row) (weight x r),
- * r = 1 / sqrt(mean of x^2 + eps) over all d entries, eps >= 2^-126.  R turns the pair (x[j], x[pairs + j]), or with interleaved != 0 (x[2j], x[2j + 1]), to
- * (a cos - b sin, a sin + b cos), cos and sin being entry j of the row; entries from 2 pairs on are not turned.  Two tensors, queries [0] and
- * keys [1] (heads 0: none; not the first), share the table.
+ * r = 1 / sqrt(mean of x^2 + eps) over all d entries, eps >= 2^-126, the sum of x^2 below 2^127 (summed in float32).  R turns the pair
+ * (x[j], x[pairs + j]), or with interleaved != 0 (x[2j], x[2j + 1]), to (a cos - b sin, a sin + b cos), cos and sin being entry j of the row; entries
+ * from 2 pairs on are not turned.  Two tensors, queries [0] and keys [1] (heads 0: none; not the first), share the table.
  * table  : [batch, rows, pairs, 2] float32, rows contiguous, table_stride floats from batch to batch (0: one for all; even), 8-byte aligned; NULL
  *          where pairs is 0.  Row of vector n: n, or index[b,n] (index_stride entries from batch to batch, 0: one for all; NULL: n).  A row below zero:
  *          the vector is not turned; from rows on: what would be turned becomes NaN.

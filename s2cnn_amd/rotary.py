@@ -174,7 +174,8 @@ def norm_rotary(q, k, q_weight=None, k_weight=None, table=None, index=None, eps=
     :param q, k, table, index, interleaved: as for `rotary`
     :param q_weight, k_weight: [d], the type of q, shared by the heads, or None
     :param eps: >= 2^-126
-    :return (q, k): as for `rotary`.  Squares are summed in float32: entries are below 2^63 in size
+    :return (q, k): as for `rotary`.  Squares are summed in float32: a vector's have to stay below 2^127 together (entries below 2^59 in size do for any d);
+        beyond, the vector becomes zero or NaN
     """
     eps = ctypes.c_float(eps).value
     assert 2.0 ** -126 <= eps < math.inf

@@ -268,6 +268,32 @@ def test_large_small_and_infinite_entries(hip):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("d", [256, 255, 4, 1])
+def test_largest_entries_of_a_normalisation(hip, d, dtype):
+    """All entries just below the documented 2^59, at the largest d too, forward and backward; one entry of a single one just below 2^63.5."""
+    gen = torch.Generator().manual_seed(d)
+    below = 1 - 2.0 ** -8
+    x = torch.where(torch.rand(1, 2, 5, d, generator=gen) < 0.5, -below, below).double()
+    x[:, 1] *= torch.rand(1, 5, d, generator=gen)
+    x *= 2.0 ** 59
+    if d == 1:
+        x.copy_(x.sign() * below * 2.0 ** 63.5)
+    x = x.to(dtype)
+    pairs = d // 2
+    table = _table(5, pairs) if pairs else None
+    g, w = torch.randn(1, 2, 5, d, generator=gen).to(dtype), (torch.rand(d, generator=gen) + 0.5).to(dtype)
+    leaf = x.cuda().requires_grad_()
+    y = s2cnn_amd.norm_rotary(leaf, None, w.cuda(), table=table.cuda() if pairs else None, eps=EPS)[0]
+    gx, = torch.autograd.grad(y, leaf, g.cuda())
+    xd, gd = x.double(), _turned(g.double(), table, False, back=True) if pairs else g.double()
+    want, want_gx, _, parts, _ = _gradients(xd, w.double(), gd)
+    _close(y, _turned(want, table, False) if pairs else want, dtype, "y", 16)
+    _close(gx * 2.0 ** 40, want_gx * 2.0 ** 40, dtype, "gx", 16, parts * 2.0 ** 40)
+    assert float(y.detach().float().norm()) > 1
+
+
+@pytest.mark.gpu
 @TYPES
 @LAYOUTS
 @pytest.mark.parametrize("d,pairs", [(64, 24), (64, 8), (40, 3), (23, 9), (7, 3), (128, 13)])
