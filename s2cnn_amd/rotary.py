@@ -193,8 +193,8 @@ def rotary_table(positions, frequencies, scale=1.0):
     :param positions: [..., axes] float32, float64, int32 or int64: places on an axis, angles on the sphere, points in space
     :param frequencies: [axes, pairs] float64 in radians (`rotary_frequencies`, `s2_rotary_frequencies`), pairs <= 128
     :param scale: a factor of both, which multiplies scores by its square where queries and keys are turned with the table
-    :return [..., pairs, 2]: float32.  Angles are formed in 64 bits: no place is too far for its angle to be accurate to 2^-24
-        below 2^26 turns
+    :return [..., pairs, 2]: float32.  Angles are formed in 64 bits, with up to three roundings of each axis's part: where that is below 2^24 turns an angle is
+        off by less than 2^-24, and an entry by less than 3 * 2^-24 of the scale; beyond, in proportion more
     """
     assert positions.dim() >= 1 and frequencies.dim() == 2
     axes, pairs = frequencies.shape

@@ -453,6 +453,22 @@ def test_rotary_table(hip, shape, axes, pairs, kind):
 
 
 @pytest.mark.gpu
+def test_rotary_table_is_rounded_little_more_than_once(hip):
+    """Entries that a sine's polynomial gives (below 0.7 in size), x in quarter turns, u = 2^-24: the result's rounding u / 2, x's 2^-26 by at most 1.45 (1.36
+    where the result is above a half: 0.34 u), the product beyond pi/2 x, of at most 0.08: two roundings of its relative size and its own, 0.22 u, and what the
+    polynomial leaves, below 0.04 u: 1.1 u in all.  Cosines' (above 0.71): the result's u / 2, x's 2^-26 by at most 1.12 (0.28 u), the square's and
+    two more of at most 0.31: 0.5 u: 1.3 u.  Far places: the angle's own three roundings of 2^24 turns, 0.6 u."""
+    places = torch.linspace(-9.0, 9.0, 1000003, dtype=torch.float64).view(-1, 1)
+    f = torch.ones(1, 1, dtype=torch.float64)
+    for base, more in ((0.0, 0.0), (2.0 ** 23 * 2 * math.pi, 0.3)):
+        p = places + base
+        got = s2cnn_amd.rotary_table(p.cuda(), f.cuda()).cpu().double().flatten()
+        want = torch.stack([p.cos(), p.sin()], -1).flatten()
+        off = (got - want).abs() * 2.0 ** 24
+        assert off[want.abs() < 0.7].max() <= 1.1 + more and off[want.abs() > 0.71].max() <= 1.3 + more
+
+
+@pytest.mark.gpu
 def test_rotary_table_of_quarter_turns_and_far_places(hip):
     f = torch.tensor([[math.pi / 2, 2 * math.pi, 1.0]], dtype=torch.float64).cuda()
     t = s2cnn_amd.rotary_table(torch.arange(-4, 9).view(-1, 1).cuda(), f).cpu()
