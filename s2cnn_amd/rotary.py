@@ -128,7 +128,7 @@ def _call(q, k, q_weight, k_weight, table, index, norm, eps, interleaved):
         if index is None:
             assert table.size(-3) == n
         else:
-            assert index.shape in ((n,), (batch, n)) and table.size(-3) >= 1
+            assert index.shape in ((n,), (batch, n)) and 1 <= table.size(-3) < MAX_VECTORS
     else:
         assert index is None
     dtype = _hip.require_gpu_float(q, k, q_weight, k_weight)
@@ -157,7 +157,7 @@ def rotary(q, k, table, index=None, interleaved=False):
     :param q: [batch, heads, n, d], d <= 256; float32, bfloat16 or float16, any strides (copied if the last axis is strided)
     :param k: [batch, kv_heads, n, d] of the same places, or None
     :param table: [rows, pairs, 2] or [batch, rows, pairs, 2] float32, cosines and sines (`rotary_table`); without an index row n is the place's, and
-        there are n of them.  Not differentiated
+        there are n of them, with one any number below 2^31.  Not differentiated
     :param index: [n] or [batch, n] int32: the row of every place.  A place whose row is below zero is not turned (padding); of one from `rows` on
         what would be turned becomes NaN
     :return (q, k): the types and orders of axes of the arguments; arithmetic is float32, rounded once.  k: None for None

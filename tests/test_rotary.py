@@ -545,6 +545,16 @@ def test_refusals_before_the_gpu():
         s2cnn_amd.rotary_table(torch.zeros(4, 1, dtype=torch.int16), torch.zeros(1, 3, dtype=torch.float64))
 
 
+def test_tables_of_too_many_rows_are_refused():
+    """Rows are numbered by int32: 2^32 + 5 of them would be taken for five, and the others for none."""
+    q, index = torch.zeros(1, 1, 3, 2), torch.zeros(3, dtype=torch.int32)
+    for rows in (1 << 31, (1 << 32) + 5):
+        with pytest.raises(AssertionError):
+            s2cnn_amd.rotary(q, None, torch.zeros(1, 1, 2).expand(rows, 1, 2), index=index)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        s2cnn_amd.rotary(q, None, torch.zeros(1, 1, 2).expand((1 << 31) - 1, 1, 2), index=index)
+
+
 @pytest.mark.gpu
 def test_refusals_of_types(hip):
     q, table = torch.zeros(2, 4, 5, 8, device="cuda"), torch.zeros(5, 4, 2, device="cuda")
