@@ -243,7 +243,14 @@ class AdamW(torch.optim.Optimizer):
 
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
-        group = self.param_groups[-1]
+        try:
+            self._check_group(self.param_groups[-1])
+        except Exception:
+            self.param_groups.pop()
+            raise
+
+    @staticmethod
+    def _check_group(group):
         assert group["state_bits"] in (8, 32)
         assert 0.0 <= group["betas"][0] < 1.0 and 0.0 <= group["betas"][1] < 1.0 and 1e-30 <= group["eps"] < 1e30 and 0.0 <= group["weight_decay"] < 1e30
         assert torch.is_tensor(group["lr"]) and group["lr"].numel() == 1 or 0.0 <= group["lr"] < 1e30

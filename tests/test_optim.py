@@ -872,6 +872,18 @@ def test_refusals_before_the_gpu():
         s2cnn_amd.AdamW([torch.nn.Parameter(torch.zeros(3, dtype=torch.float64))])
 
 
+def test_refused_groups_are_not_added():
+    p, q = (torch.nn.Parameter(torch.zeros(3)) for _ in range(2))
+    opt = s2cnn_amd.AdamW([p])
+    for group in ({"params": [q], "state_bits": 16}, {"params": [q], "eps": 0.0}, {"params": [q], "lr": -1.0},
+                  {"params": [torch.nn.Parameter(torch.zeros(3, dtype=torch.float64))]}):
+        with pytest.raises((AssertionError, RuntimeError)):
+            opt.add_param_group(group)
+        assert len(opt.param_groups) == 1
+    opt.add_param_group({"params": [q], "state_bits": 8})
+    assert [len(g["params"]) for g in opt.param_groups] == [1, 1]
+
+
 @pytest.mark.gpu
 def test_refusals_of_tensors(hip):
     z = lambda *s, d=F32: torch.zeros(*s, dtype=d, device="cuda")
