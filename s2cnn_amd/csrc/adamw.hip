@@ -18,6 +18,7 @@
 // (b2 = 0.999), far below the spacing, and would be rounded away; so both are rounded up or down at random, with the probability that leaves the
 // mean right.  The random bits are a function of the seed, the step and the entry's number: 16 for each moment.
 // m, v, s and the codes are formed by single float32 operations in the order written, without fused ones: a program that does the same gets the same codes.
+#include <float.h>
 #include <stdlib.h>
 #include "chunk.h"
 #include "counter_random.h"
@@ -227,7 +228,9 @@ template <class T, int BITS, bool MASTER, bool FULL> __device__ __forceinline__ 
     // the instruction takes a subnormal number's root for zero: small ones are taken times 2^32
     const bool small = v[i] < 0x1p-96f;
     const float denominator = fmaf(__builtin_amdgcn_sqrtf(v[i] * (small ? f.inverse2 * 0x1p32f : f.inverse2)), small ? 0x1p-16f : 1.f, h.eps);
-    p[i] = fmaf(-f.size, m[i] * __builtin_amdgcn_rcpf(denominator), fmaf(-f.decay, p[i], p[i]));
+    // what decays of an infinite parameter (a mask) is finite: it stays
+    const float kept = fmaf(-f.decay, __builtin_amdgcn_fmed3f(p[i], -FLT_MAX, FLT_MAX), p[i]);
+    p[i] = fmaf(-f.size, m[i] * __builtin_amdgcn_rcpf(denominator), kept);
     // The parameter is the rounding of the float32 that is stored: without this the compiler makes one operation of the last product, sum and conversion
     // to float16, which rounds once and may differ.
     if constexpr (MASTER) asm volatile("" : "+v"(p[i]));

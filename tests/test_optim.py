@@ -378,6 +378,27 @@ def test_masters_hold_small_steps_and_follow_the_program(hip, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("bits", [8, 32])
+@TYPES
+@pytest.mark.parametrize("weight_decay", [0.0, 0.1])
+def test_infinite_parameters_stay(hip, weight_decay, dtype, bits):
+    """Masks among the parameters, as torch's p (1 - lr weight_decay) leaves them; the type's lowest values move; what is no number stays none."""
+    lowest = torch.finfo(dtype).min
+    start = torch.tensor([-math.inf, math.inf, math.nan, lowest, -lowest, 1.0] * 50).to(dtype).cuda()
+    for size in (0.0, 1.0):
+        p, masters = [start.clone()], [start.float()] if dtype != F32 else None
+        first, second, scales = _zeros([start.shape], bits)
+        for step in (1, 2):
+            g = [torch.full_like(start, size)]
+            s2cnn_amd.adamw_step(p, g, first, second, step, lr=0.5, weight_decay=weight_decay, masters=masters, scales=scales)
+        for t in p + (masters or []):
+            assert torch.equal(t[0::6], start[0::6].to(t.dtype)) and torch.equal(t[1::6], start[1::6].to(t.dtype)) and t[2::6].isnan().all()
+            assert torch.isfinite(t.view(-1, 6)[:, 3:]).all() and (t[3::6] < 0).all() and (t[4::6] > 0).all()
+            if size == 0.0:                                                              # with gradients a master of float16 moves from -65504 by two steps of 0.5
+                assert (t[3::6] == lowest).all() == (t[5::6] == 1).all() == (weight_decay == 0.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [8, 32])
 def test_numbers_on_the_device_and_captured_steps(hip, bits):
     """The step and the learning rate as tensors give the same results as numbers; a captured step reads them at every replay."""
     shapes = [(40, 30), (77,), (5000,)]
