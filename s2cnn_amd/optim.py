@@ -167,7 +167,7 @@ def _prepared(params, grads, first, second, step, lr, betas, eps, weight_decay, 
     if dtype not in _hip.FLOATS:
         raise RuntimeError("float32, bfloat16 or float16 parameters only (got %s)" % dtype)
     p, n, _ = _list(params, dtype, device, "parameters")
-    assert len(set(p) - {0}) == len(n) - n.count(0), "a parameter twice in the list"
+    assert len(set(p)) == len(n) or len(set(p) - {0}) == len(n) - n.count(0), "a parameter twice in the list"
     g, _, grads = _list(grads, dtype, device, "gradients", n, copy=True)
     one, two, factors = _states(first, second, scales, n, device)
     copies = None
