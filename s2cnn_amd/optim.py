@@ -126,6 +126,7 @@ def adamw_step(params, grads, first, second, step, lr=1e-3, betas=(0.9, 0.999), 
     """
     One step of AdamW on a list of tensors, in place:
     m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2, p = p - lr weight_decay p - lr (m / (1 - b1^step)) / (sqrt(v / (1 - b2^step)) + eps).
+    An infinite p stays what it is.
 
     :param params, grads: tensors of one type (float32, bfloat16 or float16) on the current GPU, as many entries each; parameters contiguous.  No tensor that
         is written (all but the gradients) stands twice in the lists, and no two overlap
@@ -218,17 +219,18 @@ class AdamW(torch.optim.Optimizer):
     torch.optim.AdamW's steps by `adamw_step`: one launch for some fifty tensors, which a HIP graph may hold.
 
     :param params: parameters or groups of them, float32, bfloat16 or float16, contiguous, on one GPU.  A group may have its own lr, betas, eps,
-        weight_decay, state_bits and masters
+        weight_decay, state_bits and masters (the last two count at a parameter's first step)
     :param lr: a number, or a float32 tensor of one element on the GPU, which a captured step reads at every replay
     :param state_bits: 32, or 8: two bytes a parameter for the moments instead of eight, and a thirty-second of one for their factors
     :param masters: float32 copies of 16-bit parameters, in which small steps add up.  The program may set the parameters at any time (load a
         state dict): where they are not their masters' roundings, they count
-    :param max_norm: gradients are clipped to this norm, of all groups together (`self.norm` is the norm of the last step, before it); a step whose norm is
-        infinite or no number is left out and not counted.  None: neither
+    :param max_norm: gradients are clipped to this norm, of all groups together (`self.norm` is the norm of the last step, before it): multiplied by
+        min(1, max_norm / norm), where torch's clipping adds 1e-6 to the norm; a step whose norm is infinite or no number is left out and not
+        counted.  None: neither
     :param seed: of the random rounding of moments in 8 bits; ranks of a job that hold the same parameters need the same.  Lists of a step (groups, types,
         counts) take random numbers of their own each
 
-    Steps are counted on the device, for every parameter those that it had a gradient in.  State dicts hold the moments as they are; max_norm and seed are the
+    Steps are counted on the device, for every parameter those that it had a gradient in; a step that raises is not made for any.  State dicts hold the moments as they are; max_norm and seed are the
     program's to keep.  A step that a graph captures needs the moments to exist, and the same parameters to have gradients as before: make one before.
     """
 
@@ -276,11 +278,11 @@ class AdamW(torch.optim.Optimizer):
         return state
 
     def _lists(self, group):
-        """[(count of steps, parameters)] of a group's parameters that have a gradient, those of equal counts together, by type.  Parameters that were
-        stepped together so far share one count."""
+        """[(count of steps, parameters, their states)] of a group's parameters that have a gradient, those of equal counts together, by type.  Parameters
+        that were stepped together so far share one count."""
         members, stepped, fresh = {}, {}, {}
         for p in group["params"]:
-            state = self.state[p] if p in self.state else None
+            state = self.state.get(p)
             if state:
                 members[id(state["step"])] = members.get(id(state["step"]), 0) + 1
             if p.grad is None:
@@ -294,16 +296,18 @@ class AdamW(torch.optim.Optimizer):
                     fresh[key] = torch.zeros(1, dtype=torch.int64, device=p.device)
                 state = self.state[p] = self._new_state(p, group, fresh[key])
                 members[id(state["step"])] = members.get(id(state["step"]), 0) + 1
-            stepped.setdefault(id(state["step"]), []).append(p)
+            params, states = stepped.setdefault(id(state["step"]), ([], []))
+            params.append(p)
+            states.append(state)
         lists = []
-        for key, params in stepped.items():
-            count = self.state[params[0]]["step"]
+        for key, (params, states) in stepped.items():
+            count = states[0]["step"]
             if len(params) < members[key]:                               # some of them are left out of this step: from here on they count apart
                 self._no_capture("leaves a parameter out for the first time")
                 count = count.clone()
-                for p in params:
-                    self.state[p]["step"] = count
-            lists.append((count, params))
+                for state in states:
+                    state["step"] = count
+            lists.append((count, params, states))
         return lists
 
     @torch.no_grad()
@@ -319,17 +323,17 @@ class AdamW(torch.optim.Optimizer):
             finite = torch.isfinite(self.norm)
         steps, counts = [], []                                           # all lists are checked before the first is stepped or counted
         for group in self.param_groups:
-            for count, params in self._lists(group):
+            for count, params, states in self._lists(group):
                 counts.append(count)
                 kinds = {}                                               # what is held of a parameter was chosen when it was first stepped
-                for p in params:
-                    state = self.state[p]
-                    kinds.setdefault((p.dtype, "master" in state, "scales" in state), []).append(p)
-                for (_, masters, scales), some in kinds.items():
-                    states = [self.state[p] for p in some]
-                    steps.append(_prepared(some, [p.grad for p in some], [s["first"] for s in states], [s["second"] for s in states], count, group["lr"],
-                                           group["betas"], group["eps"], group["weight_decay"], [s["master"] for s in states] if masters else None,
-                                           [s["scales"] for s in states] if scales else None, self.norm if finite is not None else None,
+                for p, state in zip(params, states):
+                    some, held = kinds.setdefault((p.dtype, "master" in state, "scales" in state), ([], []))
+                    some.append(p)
+                    held.append(state)
+                for (_, masters, scales), (some, held) in kinds.items():
+                    steps.append(_prepared(some, [p.grad for p in some], [s["first"] for s in held], [s["second"] for s in held], count, group["lr"],
+                                           group["betas"], group["eps"], group["weight_decay"], [s["master"] for s in held] if masters else None,
+                                           [s["scales"] for s in held] if scales else None, self.norm if finite is not None else None,
                                            self.max_norm, self.seed + len(steps) * _LISTS))
         for count in counts:
             count.add_(1 if finite is None else finite)
