@@ -512,8 +512,8 @@ int s2cnn_rotary_table(const void *positions, int positions_type, const double *
 
 /* ---- the step of an optimizer over a list of tensors --------------------------------------------
  * adamw_step: for every tensor i of n[i] entries, dense: g' = g min(1, max_norm / *norm) (norm NULL: g), m = beta1 m + (1 - beta1) g',
- *   v = beta2 v + (1 - beta2) g'^2, p = p - lr weight_decay p - lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps), arithmetic in float32.
- *   p, g: of dtype.  masters: float32 copies of 16-bit parameters, or NULL: the step is made there and p is its rounding; where p was not the
+ *   v = beta2 v + (1 - beta2) g'^2, p = p - lr weight_decay p - lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps), arithmetic in float32; an infinite p
+ *   stays what it is.  p, g: of dtype.  masters: float32 copies of 16-bit parameters, or NULL: the step is made there and p is its rounding; where p was not the
  *   master's rounding, p is taken.  t = step >= 1, or *step_at; lr, or *lr_at: device memory that is read when the kernel runs, or NULL.
  *   Where *norm is infinite or no number, nothing is written.  Tensors do not overlap; one that is
  *   written and stands in the lists twice is refused.
@@ -523,7 +523,7 @@ int s2cnn_rotary_table(const void *positions, int positions_type, const double *
  *   every tensor from a multiple of 256 on.  A factor is the largest entry over f(126) or f(255), 0 (and the block's entries) where below 2^-126;
  *   of a block with an infinite entry, or one that is no number, all entries become such.
  * adamw_states: the moments of 8 bits in float32, n[i] entries each.
- * grad_norm: *out = sqrt of the sum of squares of all entries of a list of tensors of any types, summed in 64 bits.
+ * grad_norm: *out = sqrt of the sum of squares of all entries of a list of tensors of any of the three types, summed in 64 bits.
  * Lists are host memory, read during the call; tensors without entries are left out (their pointers may be NULL).  n[i] <= 2^35 - 2048.
  */
 typedef struct s2cnn_adamw_t {

@@ -11,12 +11,15 @@
 // it reads anyway.  A vector belongs to a group of L lanes (a power of two).  A lane holds two chunks of 16 bytes, so that both entries of a pair
 // are its own: no exchange between lanes but the sums over a vector.  Where a chunk would run past the end of its part, it begins earlier and
 // overlaps the one before (both lanes form the same numbers; sums count them once), so that all accesses are 16 bytes wide, at any alignment; only
-// parts shorter than a chunk are loaded entry by entry, in kernels of their own (FULL; rotations of 4 x 16 heads x 4096 places x 64 in float32, both ways:
-// 51 us, with the tests for tails 65).
+// parts shorter than a chunk are loaded entry by entry, in kernels of their own (not FULL: rotations of 4 x 16 heads x 4096 places x 64 in float32
+// take 27 us each way; with the tests for tails a quarter more).
 //
 // Measured, with a copy of 1 GiB at 5.1 TB/s: 4 x (32 + 8) heads x 8192 places x 128 in bfloat16: forward 122 us, 5.5 TB/s, backward 185 to 195 us, 5.2 to
 // 5.4 TB/s, and 4 us for the sums of its weights' gradients; tensors of 256 MB or more go past the caches (in them: 127 and 205 to 215 us).  A
 // batch of 32 x 10 heads x 400 places of 20 in float32: 9 and 12 us, a launch, two trips to memory and their instructions; single places 3 to 5 us.
+//
+// Arithmetic is float32: squares and the gradients of weights are summed in it, r is one instruction's root of a product with 1 / d.  In float32 y is off by a
+// tenth more than by a root and a quotient of their own; 16-bit results hide it.
 #include "chunk.h"
 
 namespace s2cnn {
@@ -398,8 +401,10 @@ bool sizes_ok(const s2cnn_rotary_t* a) {
 }
 
 // Runs of four heads (two where x and g are read) where that leaves every group two runs or more, else of one: 4 x 40 heads x 8192 places of 128 in bfloat16,
-// forward and backward, 128 and 205 us, of one head each 160 and 224; 32 x 10 heads x 400 places of 20 in float32 the other way round, 10.7 and 14.5 us, of one 9.4
-// and 12.5.  As many workgroups as run at once, four a CU (three; runs of one head: eight, four), or fewer that take as many turns.
+// in the caches, forward and backward, 128 and 205 us, of one head each 160 and 224; 32 x 10 heads x 400 places of 20 in float32 the other way round, 10.7 and
+// 14.5 us, of one 9.4 and 12.5.  Four workgroups a CU (three; runs of one head: eight, four), or fewer that take as many turns.  In 16 bits that is what the
+// registers let run at once, but for the normalisation of one head, which gets seven of its eight; in float32, with half the registers, up to eight
+// would fit in all of them.
 Plan plan_of(const s2cnn_rotary_t& a, bool two) {
   Plan p;
   p.units = units_of(a.dtype == S2CNN_F32 ? 4 : 8, a.d, a.pairs, a.interleaved != 0);

@@ -220,7 +220,8 @@ def rotary_frequencies(pairs, base=10000.0, factor=1.0, original=None, fast=32.0
 
     :param factor: how many times longer the axis is than the one that a model was trained on.  All frequencies are divided by it; or, where `original`
         gives the length of that axis, those that turn less than `slow` times along it, and none that turns more than `fast` times, with a linear passage
-        between them: near places stay as far apart as they were
+        between them: near places stay as far apart as they were (Peng, Quesnelle, Fan, Shippole, "YaRN: efficient context window extension of large
+        language models", 2023; its factor of the scores is the square of `rotary_table`'s scale)
     """
     assert 1 <= pairs <= MAX_HEAD // 2 and base > 0 and factor > 0 and 0 <= slow < fast
     f = base ** (-np.arange(pairs, dtype=np.float64) / pairs)
