@@ -512,11 +512,11 @@ int s2cnn_rotary_table(const void *positions, int positions_type, const double *
 
 /* ---- the step of an optimizer over a list of tensors --------------------------------------------
  * adamw_step: for every tensor i of n[i] entries, dense: g' = g min(1, max_norm / *norm) (norm NULL: g), m = beta1 m + (1 - beta1) g',
- *   v = beta2 v + (1 - beta2) g'^2, p = p - lr weight_decay p - lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps), arithmetic in float32; an infinite p
- *   stays what it is.  p, g: of dtype.  masters: float32 copies of 16-bit parameters, or NULL: the step is made there and p is its rounding; where p was not the
+ *   v = beta2 v + (1 - beta2) g'^2, p = p - lr weight_decay p - lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps), arithmetic in
+ *   float32; an infinite p stays what it is.  p, g: of dtype.  masters: float32 copies of 16-bit parameters, or NULL: the step is made there and p is its rounding; where p was not the
  *   master's rounding, p is taken.  t = step >= 1, or *step_at; lr, or *lr_at: device memory that is read when the kernel runs, or NULL.
- *   Where *norm is infinite or no number, nothing is written.  Tensors do not overlap; one that is
- *   written and stands in the lists twice is refused.
+ *   Where *norm is infinite or no number, nothing is written.  Tensors do not overlap; one that is written and stands in the
+ *   lists twice is refused.
  *   bits 32: first and second are float32, scales NULL.  bits 8: first is of one byte an entry (float8 of 4 exponent and 3 mantissa bits), second of one
  *   (f(c) = c for c < 8, (8 + c % 8) 2^(c / 8 - 1) beyond), scales [ceil(n / 256)][2] float32, 8-byte aligned: the factors of m (in units of 2^-9) and v of
  *   every 256 entries.  Rounded at random: halves of word e % 4 of Philox4x32-10 of counter (e / 4, t) and key seed, e the entry's number in the list,

@@ -230,8 +230,9 @@ class AdamW(torch.optim.Optimizer):
     :param seed: of the random rounding of moments in 8 bits; ranks of a job that hold the same parameters need the same.  Lists of a step (groups, types,
         counts) take random numbers of their own each
 
-    Steps are counted on the device, for every parameter those that it had a gradient in; a step that raises is not made for any.  State dicts hold the moments as they are; max_norm and seed are the
-    program's to keep.  A step that a graph captures needs the moments to exist, and the same parameters to have gradients as before: make one before.
+    Steps are counted on the device, for every parameter those that it had a gradient in; a step that raises is not made for any.  State dicts hold the
+    moments as they are; max_norm and seed are the program's to keep.  A step that a graph captures needs the moments to exist, and the same parameters
+    to have gradients as before: make one before.
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, masters=True, max_norm=None, seed=0):
